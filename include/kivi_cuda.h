@@ -341,7 +341,8 @@ int kivi_decode_attention_gather(const kivi_layer* layer, int64_t quant_len, int
 
 /* Reads (and synchronises with) the device fault word: bit 0 is set once a wait
  * for a bulk copy inside a kernel of this library ran out, bit 1 once a wait for
- * peer ranks in kivi_decode_attention_gather ran out.  Such a kernel returns
+ * peer ranks in kivi_decode_attention_gather ran out, bit 2 once the arrays of a
+ * kivi_paged_batch pointed outside the cache.  Such a kernel returns
  * normally (bit 0: the affected split counts as empty).  The word is sticky
  * until kivi_device_fault_clear() resets it (current device; synchronises). */
 int kivi_device_fault(int* word_out);
@@ -393,6 +394,122 @@ int kivi_decode_step_host(const kivi_layer* layer, int64_t* quant_len, int* res_
 int kivi_sample_tokens(const void* logits, int dtype, int batch, int vocab, int64_t row_stride,
                        float temperature, int top_k, int do_sample, uint64_t seed, uint64_t step,
                        int64_t* ids_out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged cache: many sequences, each with a length of its own.
+ *
+ * No counterpart in the reference, whose cache holds one batch in lock step
+ * (cache/manager.py:100-117).  The store of one layer is a pool of pages, each
+ * with page_tokens tokens of every KV head, in the blocks of kivi_layer:
+ *   k_codes  [num_pages][num_kv_heads][page_tokens/G][D*G/4]
+ *   k_scales, k_zeros [num_pages][num_kv_heads][page_tokens/G][D]
+ *   v_codes  [num_pages][num_kv_heads][page_tokens][D/4]
+ *   v_scales, v_zeros [num_pages][num_kv_heads][page_tokens][D/G]
+ *   k_res, v_res [num_slots][num_kv_heads][R][D] of res_dtype: the windows, one
+ *            slot per sequence, token t at t % R.
+ * A kivi_layer whose units are ordered (batch, kv_head) is such a pool with one page
+ * of max_tokens tokens per batch row.
+ * A sequence of t tokens has the first quant(t) in pages and the rest in its window:
+ * quant(t) = 0 for t < R, else ((t - R) / G + 1) * G, which is what kivi_cache_plan
+ * leads to however the tokens came in.
+ *
+ * A step's batch is ragged: sequence s brings rows cu_new[s] .. cu_new[s+1]-1 of the
+ * step's tensors (no rows at all is allowed) and held seq_lens[s] tokens before the
+ * step.  All four arrays are int32 in device memory and are read by the kernels, so a
+ * captured step follows them; total_new (rows the tensors hold), max_new and max_len
+ * (no sequence brings more new tokens, or is longer after the step) are given by the
+ * host and size the grids.  Rows behind cu_new[num_seqs] are neither read nor written.
+ * A sequence whose numbers contradict these limits is left out, a page outside the pool
+ * is read as page 0 (and not written): bit 2 of the device fault word tells of both.
+ * Two sequences of one call may read the same page; for kivi_paged_append no two may
+ * share a window, or a page that the call writes.
+ * ---------------------------------------------------------------------- */
+typedef struct kivi_paged_layer {
+    int32_t num_pages, page_tokens; /* page_tokens: multiple of group_size */
+    int32_t num_kv_heads, head_dim; /* head_dim: multiple of group_size, <= 256, D <= 64 or D % 64 == 0 */
+    int32_t group_size, residual_cap;
+    int32_t num_slots, res_dtype;
+    uint8_t* k_codes;
+    float* k_scales;
+    float* k_zeros;
+    uint8_t* v_codes;
+    float* v_scales;
+    float* v_zeros;
+    void* k_res;
+    void* v_res;
+} kivi_paged_layer;
+
+typedef struct kivi_paged_batch {
+    int32_t num_seqs, table_width;
+    const int32_t* page_table; /* device [num_seqs][table_width]: page of tokens i*page_tokens .. of the sequence */
+    const int32_t* slots;      /* device [num_seqs] */
+    const int32_t* seq_lens;   /* device [num_seqs]: tokens held before the step */
+    const int32_t* cu_new;     /* device [num_seqs + 1] */
+    int32_t total_new, max_new, max_len;
+    int32_t ring_shift;        /* 0; else token t of a sequence is in slot (t + ring_shift) % R, 0 <= ring_shift < R */
+} kivi_paged_batch;
+
+/* rows of a step: element d of head h of row r at data[r*row_stride + h*head_stride + d] */
+typedef struct kivi_rows {
+    void* data;
+    int64_t row_stride, head_stride;
+} kivi_rows;
+
+/* Appends a step's keys and values, all of res_dtype: whole groups leave for their pages
+ * as in kivi_cache_update (codes, scales and zeros are the same to the bit), the rest goes
+ * to the windows.
+ * rotary != NULL: keys (and the queries, q->data != NULL) are first turned to their
+ * positions, token i of a sequence by row i of rotary, device fp32
+ * [rotary_rows >= max_len][rotary_dim]: rotary_dim/2 cosines, then as many sines.  The
+ * first rotary_dim channels of a head take part, in pairs (i, i + rotary_dim/2) or, with
+ * interleaved != 0, (2i, 2i+1): a' = a cos - b sin, b' = b cos + a sin, two products and
+ * one sum in fp32, each rounded, the result rounded to res_dtype.  k_out and q_out receive
+ * the turned rows; they may be the inputs themselves. */
+int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged_batch* batch,
+                      const kivi_rows* new_k, const kivi_rows* new_v, const float* rotary, int rotary_rows,
+                      int rotary_dim, int interleaved, const kivi_rows* q, int n_rep, const kivi_rows* q_out,
+                      const kivi_rows* k_out, int rounding, void* stream);
+
+/* Attention of a step's rows after kivi_paged_append of the same batch: row i of a
+ * sequence attends to the sequence's tokens 0 .. held + i.  Tokens before the step come
+ * from pages and window, the step's own from new_k / new_v (turned, in full precision,
+ * also those that the append has already moved to pages).
+ * q, out: rows of q_dtype / out_dtype with num_kv_heads * n_rep heads.  sm_scale <= 0
+ * means head_dim^-0.5.  workspace: device scratch of kivi_paged_attention_workspace()
+ * bytes for the same arguments, contents need not be preserved. */
+size_t kivi_paged_attention_workspace(const kivi_paged_layer* layer, const kivi_paged_batch* batch, int q_dtype, int n_rep);
+int kivi_paged_attention(const kivi_paged_layer* layer, const kivi_paged_batch* batch, const kivi_rows* q,
+                         int q_dtype, const kivi_rows* new_k, const kivi_rows* new_v, const kivi_rows* out,
+                         int out_dtype, int n_rep, float sm_scale, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* Tokens starts[s] .. of every sequence as they are served, fp32: rows cu_read[s] ..
+ * cu_read[s+1]-1 of k_out and v_out, [total_read][num_kv_heads][D].  batch->seq_lens: tokens the
+ * sequences hold now; cu_new, total_new, max_new describe the rows that are read.
+ * The counterpart of kivi_cache_materialize. */
+int kivi_paged_read(const kivi_paged_layer* layer, const kivi_paged_batch* batch, const int32_t* starts,
+                    float* k_out, float* v_out, void* stream);
+
+/* Next-token choice under filters of each row's own, from given random numbers.
+ *
+ * Extends sample_token (src/kivi_sycl/generation/sampling.py:10-25) by nucleus and
+ * min-p cuts.  With x the logits of a row and m_i = exp((x_i - max x) / temperature),
+ * entry i is kept when
+ *   x_i is not below the top_k-th largest (top_k <= 0 or >= vocab: no cut; ties stay), and
+ *   the entries above x_i that the top_k cut leaves hold less than top_p of its mass
+ *     (top_p >= 1: no cut; ties stay together; the largest always stays), and
+ *   m_i >= min_p (min_p <= 0: no cut; the largest always stays),
+ * and the id is the first index at which the sum of the kept m_i exceeds uniform * (all of
+ * it).  temperature <= 0: the argmax, lowest index first.  NaN logits count as -inf, of
+ * infinite ones each has mass 1 and no other any; a row without a number above -inf gives 0.
+ * Sums are in fp64, relative error of a mass below 1e-9: a draw differs from the one in
+ * real arithmetic only within that of a boundary.
+ * logits: device [batch][row_stride >= vocab] of dtype.  uniforms: device fp32 [batch] in
+ * [0, 1).  temperature, top_p, min_p: device fp32 [batch], top_k: device int32 [batch]; NULL
+ * means 1, no cut.  ids_out: device int64 [batch]. */
+int kivi_sample_filtered(const void* logits, int dtype, int batch, int vocab, int64_t row_stride,
+                         const float* uniforms, const float* temperature, const int32_t* top_k,
+                         const float* top_p, const float* min_p, int64_t* ids_out, void* stream);
 
 /* Self-test (allocates 4 bytes, synchronises): the largest k for which the
  * tensor core, adding the products 1 and 2^-k to the addend -1 in one m16n8k16

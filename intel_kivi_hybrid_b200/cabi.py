@@ -30,6 +30,24 @@ class Layer(_c.Structure):
                 ("v_codes", _vp), ("v_scales", _vp), ("v_zeros", _vp), ("k_res", _vp), ("v_res", _vp)]
 
 
+class PagedLayer(_c.Structure):
+    """struct kivi_paged_layer of include/kivi_cuda.h."""
+    _fields_ = [(n, _c.c_int32) for n in ("num_pages", "page_tokens", "num_kv_heads", "head_dim", "group_size", "residual_cap",
+                                          "num_slots", "res_dtype")] + \
+               [(n, _vp) for n in ("k_codes", "k_scales", "k_zeros", "v_codes", "v_scales", "v_zeros", "k_res", "v_res")]
+
+
+class PagedBatch(_c.Structure):
+    """struct kivi_paged_batch of include/kivi_cuda.h."""
+    _fields_ = [("num_seqs", _c.c_int32), ("table_width", _c.c_int32), ("page_table", _vp), ("slots", _vp), ("seq_lens", _vp),
+                ("cu_new", _vp), ("total_new", _c.c_int32), ("max_new", _c.c_int32), ("max_len", _c.c_int32), ("ring_shift", _c.c_int32)]
+
+
+class Rows(_c.Structure):
+    """struct kivi_rows of include/kivi_cuda.h."""
+    _fields_ = [("data", _vp), ("row_stride", _i64), ("head_stride", _i64)]
+
+
 PEER_MAX_WORLD = 8
 
 
@@ -77,6 +95,13 @@ SIGNATURES = {
                                      _vp, _vp, _vp, _vp, _int, _int, _int, _f, _vp, _c.c_size_t, _vp, _c.c_size_t,
                                      _int, _int, _int, _int, _int, _c.POINTER(PeerGatherDesc), _i64, _vp]),
     "kivi_sample_tokens": (_int, [_vp, _int, _int, _int, _i64, _f, _int, _int, _c.c_uint64, _c.c_uint64, _vp, _vp]),
+    "kivi_sample_filtered": (_int, [_vp, _int, _int, _int, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kivi_paged_append": (_int, [_c.POINTER(PagedLayer), _c.POINTER(PagedBatch), _c.POINTER(Rows), _c.POINTER(Rows), _vp, _int, _int, _int,
+                                 _c.POINTER(Rows), _int, _c.POINTER(Rows), _c.POINTER(Rows), _int, _vp]),
+    "kivi_paged_attention_workspace": (_c.c_size_t, [_c.POINTER(PagedLayer), _c.POINTER(PagedBatch), _int, _int]),
+    "kivi_paged_attention": (_int, [_c.POINTER(PagedLayer), _c.POINTER(PagedBatch), _c.POINTER(Rows), _int, _c.POINTER(Rows), _c.POINTER(Rows),
+                                    _c.POINTER(Rows), _int, _int, _f, _vp, _c.c_size_t, _vp]),
+    "kivi_paged_read": (_int, [_c.POINTER(PagedLayer), _c.POINTER(PagedBatch), _vp, _vp, _vp, _vp]),
     "kivi_peer_alloc": (_int, [_c.c_size_t, _c.POINTER(_vp), _c.c_char_p]),
     "kivi_peer_open": (_int, [_c.c_char_p, _c.POINTER(_vp)]),
     "kivi_peer_close": (_int, [_vp]),

@@ -384,7 +384,8 @@ class KiviCache:
         if word:
             cabi.device_fault_clear()
             what = [name for bit, name in ((1, "a bulk copy inside the attention kernel did not land in time"),
-                                           (2, "a peer rank did not publish its attention outputs in time")) if word & bit]
+                                           (2, "a peer rank did not publish its attention outputs in time"),
+                                           (4, "the arrays of a paged batch pointed outside the cache")) if word & bit]
             raise RuntimeError("kivi_cuda device fault word = %d: %s; outputs since the last check may be wrong"
                                % (word, "; ".join(what)))
 

@@ -1,0 +1,375 @@
+// Attention of a step's rows over a paged cache, on the CUDA cores: every shape the cache
+// takes, fp32 accuracy.
+//
+// The rows of one sequence and KV head -- (new token, query head) pairs, n_rep heads side
+// by side -- are cut into blocks of RT; a CTA takes a block and a piece of the sequence's
+// tokens, 64 at a time: dequantized into shared memory (code * scale + zero in one
+// rounding) or copied from the window or the step's own rows, scored, folded into running
+// maxima and sums, and contracted with the values.  A thread has RPT rows and four tokens
+// of the scores, RPT rows and D/16 channels of the output; the 16 threads of a row are half
+// a warp, so weights change hands without a block barrier.
+// Row i of a sequence sees its tokens 0 .. held + i; blocks stop at their last row's.
+//
+// Bound by the FMA pipe with 64 rows, by the conversion of the codes with few.
+#include "paged_common.cuh"
+#include "paged_attention.cuh"
+
+namespace kivi {
+namespace {
+
+__device__ int g_fault = 0;
+
+constexpr int kTile = 64;                                // tokens in shared memory at a time
+
+template <typename T> __device__ __forceinline__ float4 load4(const T* p, bool vec);
+template <> __device__ __forceinline__ float4 load4<float>(const float* p, bool vec) {
+    return vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+}
+template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p, bool vec) {
+    if (!vec) return make_float4(__bfloat162float(p[0]), __bfloat162float(p[1]), __bfloat162float(p[2]), __bfloat162float(p[3]));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 load4_as(const kivi_rows& r, int dtype, int64_t row, int head, int d, bool vec) {
+    const int64_t at = row * r.row_stride + (int64_t)head * r.head_stride + d;
+    return dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(r.data) + at, vec) : load4(reinterpret_cast<const float*>(r.data) + at, vec);
+}
+
+// DT: head_dim 64 or 128, or 256 for any up to that.
+template <int RPT, int TY, int DT>
+__global__ void __launch_bounds__(TY * 16)
+paged_attention_kernel(PagedAttnArgs A) {
+    constexpr int RT = RPT * TY, kThreads = TY * 16, NC = DT / 64;       // NC: quads of channels a thread has
+    extern __shared__ __align__(16) float smem_f[];
+    __shared__ int place_s[2];
+    stream_order();
+    settle_args(A);
+    const kivi_paged_layer& L = A.L;
+    const int D = DT == 256 ? L.head_dim : DT, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + 4, Q = G / 4, W = D < 64 ? D : 64;
+    float* const q_s = smem_f;                           // [RT][S]
+    float* const k_s = q_s + RT * S;                     // [kTile][S]
+    float* const v_s = k_s + kTile * S;                  // [kTile][S]
+    float* const p_s = v_s + kTile * S;                  // [RT][kTile + 4]
+    const int h = blockIdx.y, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) report_left_out(L, A.b, &g_fault);
+    if (tid < 32) {
+        const ItemPlace p = find_item(blockIdx.x, A.b.num_seqs, [&](int i) {
+            PagedSeq q;
+            load_seq(L, A.b, i, q);
+            return (int)(((int64_t)q.n * A.n_rep + RT - 1) / RT);
+        });
+        if (tid == 0) { place_s[0] = p.s; place_s[1] = p.sub; }
+    }
+    __syncthreads();
+    const int s = place_s[0];
+    if (s >= A.b.num_seqs) return;
+    PagedSeq q;
+    load_seq(L, A.b, s, q);                              // (sequences left out have no items)
+    const int n_rep = A.n_rep, rows = q.n * n_rep, row_first = place_s[1] * RT;
+    const int n_rows = rows - row_first < RT ? rows - row_first : RT;
+    const int inside = min(quant_of(q.held + q.n, G, R), q.held);        // tokens read from pages
+    const int keys = q.held + (row_first + n_rows - 1) / n_rep + 1;      // tokens the block's last row sees
+    const int t_begin = blockIdx.z * A.chunk;
+    if (t_begin >= keys) return;
+    const int t_end = min(t_begin + A.chunk, keys);
+    const bool whole = t_end == keys && blockIdx.z == 0;                 // the only piece of this block
+    const bool vec = A.vec != 0;
+
+    for (int i = tid; i < RT * (D / 4); i += kThreads) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n_rows) {
+            const int row = row_first + r;
+            x = load4_as(A.q, A.q_dtype, (int64_t)q.row0 + row / n_rep, h * n_rep + row % n_rep, d, vec);
+        }
+        *reinterpret_cast<float4*>(q_s + r * S + d) = make_float4(x.x * A.scale_log2, x.y * A.scale_log2, x.z * A.scale_log2, x.w * A.scale_log2);
+    }
+    float m[RPT], l[RPT], o[RPT][4 * NC];
+    int last[RPT];                                       // last token that the row sees
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        m[i] = -INFINITY; l[i] = 0.0f;
+        const int r = ty * RPT + i;
+        last[i] = r < n_rows ? q.held + (row_first + r) / n_rep : -1;
+#pragma unroll
+        for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.0f;
+    }
+    const int64_t ring0 = ((int64_t)q.slot * H + h) * R;
+    for (int t0 = t_begin; t0 < t_end; t0 += kTile) {
+        __syncthreads();                                 // the tile before has been read
+        for (int i = tid; i < kTile * (D / 4); i += kThreads) {
+            const int j = i / (D / 4), d = 4 * (i % (D / 4)), t = t0 + j;
+            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+            if (t < inside) {
+                const int64_t g = ((int64_t)page_of(L, q, t, &g_fault) * H + h) * (L.page_tokens / G) + t % L.page_tokens / G;
+                const int tt = t % G, sh = 2 * (tt & 3);
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(L.k_codes + g * (D * Q) + kblock_offset(d, tt >> 2, Q, W));
+                const float4 ks = *reinterpret_cast<const float4*>(L.k_scales + g * D + d), kz = *reinterpret_cast<const float4*>(L.k_zeros + g * D + d);
+                k = make_float4(fmaf((float)((w >> sh) & 3u), ks.x, kz.x), fmaf((float)((w >> (sh + 8)) & 3u), ks.y, kz.y),
+                                fmaf((float)((w >> (sh + 16)) & 3u), ks.z, kz.z), fmaf((float)((w >> (sh + 24)) & 3u), ks.w, kz.w));
+                const uint32_t c = L.v_codes[g * (D * Q) + vcode_offset(tt, d / 4, D, G)];
+                const int64_t at = g * D + vmeta_index(tt, d / G, D, G);
+                const float vs = L.v_scales[at], vz = L.v_zeros[at];
+                v = make_float4(fmaf((float)(c & 3u), vs, vz), fmaf((float)((c >> 2) & 3u), vs, vz),
+                                fmaf((float)((c >> 4) & 3u), vs, vz), fmaf((float)(c >> 6), vs, vz));
+            } else if (t < q.held) {
+                const int64_t at = (ring0 + ring_slot(t, A.b.ring_shift, R)) * D + d;
+                if (L.res_dtype == KIVI_BF16) {
+                    k = load4(reinterpret_cast<const __nv_bfloat16*>(L.k_res) + at, true);
+                    v = load4(reinterpret_cast<const __nv_bfloat16*>(L.v_res) + at, true);
+                } else {
+                    k = load4(reinterpret_cast<const float*>(L.k_res) + at, true);
+                    v = load4(reinterpret_cast<const float*>(L.v_res) + at, true);
+                }
+            } else if (t < t_end) {
+                const int64_t row = (int64_t)q.row0 + (t - q.held);
+                k = load4_as(A.k, L.res_dtype, row, h, d, vec);
+                v = load4_as(A.v, L.res_dtype, row, h, d, vec);
+            }
+            *reinterpret_cast<float4*>(k_s + j * S + d) = k;
+            *reinterpret_cast<float4*>(v_s + j * S + d) = v;
+        }
+        __syncthreads();
+        float sc[RPT][4];
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[i][j] = 0.0f;
+#pragma unroll 4
+        for (int d = 0; d < D; d += 4) {
+            float4 a[RPT], b[4];
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ty * RPT + i) * S + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * S + d);
+#pragma unroll
+            for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    sc[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, sc[i][j]))));
+        }
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = t0 + tx + 16 * j;
+                if (t > last[i] || t >= t_end) sc[i][j] = -INFINITY;
+                mx = fmaxf(mx, sc[i][j]);
+            }
+#pragma unroll
+            for (int x = 1; x < 16; x *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            const float m_new = fmaxf(m[i], mx), base = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = exp2f(m[i] - base);      // 0 while there is no maximum
+            m[i] = m_new;
+            l[i] *= alpha;
+#pragma unroll
+            for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(sc[i][j] - base);
+                l[i] += p;
+                p_s[(ty * RPT + i) * (kTile + 4) + tx + 16 * j] = p;
+            }
+        }
+        __syncwarp();
+#pragma unroll 2
+        for (int j = 0; j < kTile; j += 4) {
+            float4 p[RPT];
+#pragma unroll
+            for (int i = 0; i < RPT; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (ty * RPT + i) * (kTile + 4) + j);
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int d = 4 * tx + 64 * c;
+                    if (DT == 256 && d >= D) break;
+                    if (DT == 64 || d < D) {
+                        const float4 v = *reinterpret_cast<const float4*>(v_s + (j + jj) * S + d);
+#pragma unroll
+                        for (int i = 0; i < RPT; ++i) {
+                            const float w = jj == 0 ? p[i].x : jj == 1 ? p[i].y : jj == 2 ? p[i].z : p[i].w;
+                            o[i][4 * c] = fmaf(w, v.x, o[i][4 * c]); o[i][4 * c + 1] = fmaf(w, v.y, o[i][4 * c + 1]);
+                            o[i][4 * c + 2] = fmaf(w, v.z, o[i][4 * c + 2]); o[i][4 * c + 3] = fmaf(w, v.w, o[i][4 * c + 3]);
+                        }
+                    }
+                }
+        }
+        __syncwarp();
+    }
+    const int64_t unit = (int64_t)blockIdx.x * H + h;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+#pragma unroll
+        for (int x = 1; x < 16; x *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+        const int r = ty * RPT + i, row = row_first + r;
+        if (r >= n_rows) continue;
+        if (whole) {
+            const float inv = 1.0f / l[i];               // (a row sees itself: l > 0)
+            const int64_t at = ((int64_t)q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (4 * tx + 64 * c < D)
+                    store_quad(A.out.data, A.out_dtype, at + 4 * tx + 64 * c, make_float4(o[i][4 * c] * inv, o[i][4 * c + 1] * inv, o[i][4 * c + 2] * inv, o[i][4 * c + 3] * inv));
+        } else {
+            const int64_t part = (unit * A.pieces + blockIdx.z) * RT + r;
+            if (tx == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m[i], l[i]);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (4 * tx + 64 * c < D)
+                    *reinterpret_cast<float4*>(A.part_o + part * D + 4 * tx + 64 * c) = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
+        }
+    }
+}
+
+// Folds the pieces of a block's rows.  grid = (blocks, KV heads), 256 threads.
+__global__ void __launch_bounds__(256)
+paged_merge_kernel(PagedAttnArgs A, int RT) {
+    __shared__ int place_s[2];
+    stream_order();
+    settle_args(A);
+    const kivi_paged_layer& L = A.L;
+    const int D = L.head_dim, H = L.num_kv_heads, h = blockIdx.y, n_rep = A.n_rep;
+    if (threadIdx.x < 32) {
+        const ItemPlace p = find_item(blockIdx.x, A.b.num_seqs, [&](int i) {
+            PagedSeq q;
+            load_seq(L, A.b, i, q);
+            return (int)(((int64_t)q.n * n_rep + RT - 1) / RT);
+        });
+        if (threadIdx.x == 0) { place_s[0] = p.s; place_s[1] = p.sub; }
+    }
+    __syncthreads();
+    const int s = place_s[0];
+    if (s >= A.b.num_seqs) return;
+    PagedSeq q;
+    load_seq(L, A.b, s, q);
+    const int rows = q.n * n_rep, row_first = place_s[1] * RT;
+    const int n_rows = rows - row_first < RT ? rows - row_first : RT;
+    const int keys = q.held + (row_first + n_rows - 1) / n_rep + 1, n_pieces = (keys + A.chunk - 1) / A.chunk;
+    if (n_pieces <= 1) return;
+    const int quads = D / 4;
+    const int64_t part0 = ((int64_t)blockIdx.x * H + h) * A.pieces;
+    for (int i = threadIdx.x; i < n_rows * quads; i += 256) {
+        const int r = i / quads, d = 4 * (i % quads);
+        float M = -INFINITY, sum = 0.0f;
+        for (int p = 0; p < n_pieces; ++p) M = fmaxf(M, A.part_ml[2 * ((part0 + p) * RT + r)]);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < n_pieces; ++p) {
+            const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * ((part0 + p) * RT + r));
+            if (ml.x == -INFINITY) continue;             // a piece behind the row's own token
+            const float w = exp2f(ml.x - M);
+            const float4 v = *reinterpret_cast<const float4*>(A.part_o + ((part0 + p) * RT + r) * D + d);
+            sum = fmaf(w, ml.y, sum);
+            a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y); a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
+        }
+        const float inv = 1.0f / sum;
+        const int row = row_first + r;
+        const int64_t at = ((int64_t)q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
+        store_quad(A.out.data, A.out_dtype, at + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+    }
+}
+
+template <int RPT, int TY, int DT>
+int run_general(const PagedAttnArgs& a, int blocks, size_t smem, cudaStream_t st) {
+    auto* const kernel = paged_attention_kernel<RPT, TY, DT>;
+    if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)blocks, (unsigned)a.L.num_kv_heads, (unsigned)a.pieces), TY * 16, smem, st, true, a));
+    return KIVI_OK;
+}
+
+}  // namespace
+
+int paged_attention_fault_word(int* out) {
+    KIVI_CUDA_OK(cudaMemcpyFromSymbol(out, g_fault, sizeof(int)));
+    return KIVI_OK;
+}
+int paged_attention_fault_clear() {
+    const int zero = 0;
+    KIVI_CUDA_OK(cudaMemcpyToSymbol(g_fault, &zero, sizeof(int)));
+    return KIVI_OK;
+}
+
+// ---- the cut of a call -----------------------------------------------------------
+// Rows per block, blocks (at most: what the host knows are bounds) and pieces of the
+// sequences' tokens.
+struct PagedPlan { int rows, blocks, pieces, chunk; };
+
+static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b, int n_rep) {
+    PagedPlan p;
+    const int64_t rows = (int64_t)b->max_new * n_rep;
+    p.rows = rows <= 8 ? 8 : 64;
+    const int64_t blocks = ((int64_t)b->total_new * n_rep) / p.rows + b->num_seqs;
+    p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
+    const int tiles = (b->max_len + kTile - 1) / kTile;
+    // as many pieces as give every SM four CTAs, no piece below two tiles
+    int64_t want = (4 * (int64_t)num_sms() + p.blocks * (int64_t)L->num_kv_heads - 1) / (p.blocks * (int64_t)L->num_kv_heads);
+    const int most = (tiles + 1) / 2;
+    if (want > most) want = most;
+    if (want > 256) want = 256;
+    if (want < 1) want = 1;
+    const int per = (int)((tiles + want - 1) / want);
+    p.chunk = per * kTile;
+    p.pieces = (tiles + per - 1) / per;
+    return p;
+}
+
+}  // namespace kivi
+
+using namespace kivi;
+
+static int check_attention(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep) {
+    if (int rc = validate_paged(L)) return rc;
+    if (int rc = validate_batch(L, b)) return rc;
+    KIVI_REQUIRE(n_rep >= 1 && n_rep <= 1024, "n_rep (%d) outside 1..1024", n_rep);
+    KIVI_REQUIRE((int64_t)b->max_new * n_rep <= (1 << 30), "max_new * n_rep must be at most 2^30");
+    KIVI_REQUIRE(q_dtype == KIVI_F32 || q_dtype == KIVI_BF16, "q dtype must be KIVI_F32 or KIVI_BF16");
+    return KIVI_OK;
+}
+
+extern "C" size_t kivi_paged_attention_workspace(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep) {
+    if (check_attention(L, b, q_dtype, n_rep) != KIVI_OK || b->max_new == 0) return 0;
+    const PagedPlan p = plan_paged(L, b, n_rep);
+    return p.pieces > 1 ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
+}
+
+extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_batch* b, const kivi_rows* q,
+                                    int q_dtype, const kivi_rows* new_k, const kivi_rows* new_v, const kivi_rows* out,
+                                    int out_dtype, int n_rep, float sm_scale, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+    if (int rc = check_attention(L, b, q_dtype, n_rep)) return rc;
+    KIVI_REQUIRE(out_dtype == KIVI_F32 || out_dtype == KIVI_BF16, "out dtype must be KIVI_F32 or KIVI_BF16");
+    for (const kivi_rows* r : {q, new_k, new_v, out}) {
+        KIVI_REQUIRE(r != nullptr && r->data != nullptr, "q, new_k, new_v or out is null");
+        KIVI_REQUIRE(r->row_stride >= 0 && r->head_stride >= 0, "q, new_k, new_v or out has a negative stride");
+    }
+    if (b->max_new == 0) { note_launches(0); return KIVI_OK; }
+    const int D = L->head_dim;
+    const PagedPlan p = plan_paged(L, b, n_rep);
+    const size_t need = kivi_paged_attention_workspace(L, b, q_dtype, n_rep);
+    KIVI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
+    KIVI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
+    if (sm_scale <= 0.0f) sm_scale = 1.0f / sqrtf((float)D);
+    auto grid4 = [](const kivi_rows& r, int dtype) {
+        return reinterpret_cast<uintptr_t>(r.data) % (4 * elem_size(dtype)) == 0 && r.row_stride % 4 == 0 && r.head_stride % 4 == 0;
+    };
+    PagedAttnArgs a{};
+    a.L = *L; a.b = *b; a.q = *q; a.k = *new_k; a.v = *new_v; a.out = *out;
+    a.q_dtype = q_dtype; a.out_dtype = out_dtype; a.n_rep = n_rep; a.scale_log2 = sm_scale * 1.4426950408889634f;
+    a.pieces = p.pieces; a.chunk = p.chunk;
+    a.part_o = reinterpret_cast<float*>(workspace);
+    a.part_ml = a.part_o + (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * D;
+    a.vec = grid4(*q, q_dtype) && grid4(*new_k, L->res_dtype) && grid4(*new_v, L->res_dtype);
+    cudaStream_t st = (cudaStream_t)stream;
+    const size_t smem = ((size_t)(p.rows + 2 * kTile) * (D + 4) + (size_t)p.rows * (kTile + 4)) * 4;
+    int rc;
+    if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
+    else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);
+    if (rc) return rc;
+    if (p.pieces > 1) {
+        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads), 256, 0, st, true, a, p.rows));
+        note_launches(2);
+    } else {
+        note_launches(1);
+    }
+    return KIVI_OK;
+}

@@ -367,6 +367,202 @@ torch::Tensor sample_tokens(const torch::Tensor& logits, double temperature, int
     return ids;
 }
 
+// ---- paged cache: sequences of many lengths --------------------------------------------
+// The store of one layer as tensors the caller owns, in the order the operators take them:
+//   k_packed [pages, H, page_tokens/G, D*G/4] u8, k_scales / k_zeros [pages, H, page_tokens/G, D] f32,
+//   v_packed [pages, H, page_tokens, D/4] u8,     v_scales / v_zeros [pages, H, page_tokens, D/G] f32,
+//   k_res / v_res [slots, H, R, D] f32 or bf16.
+// Where the entries of the int32 arrays point cannot be seen from the host: the kernels
+// check them and report through the device fault word.
+constexpr int64_t kInt32Max = 0x7fffffff;
+
+struct PagedOperands {
+    kivi_paged_layer L;
+    kivi_paged_batch b;
+    torch::Device device;
+};
+
+void check_paged_tensor(const torch::Tensor& t, const char* name, torch::ScalarType type, const torch::Device& device) {
+    TORCH_CHECK(t.device() == device, name, " is on ", t.device().str(), " but k_res is on ", device.str(), ": all tensors of one call must be on the same device");
+    TORCH_CHECK(t.scalar_type() == type, name, " must be ", torch::toString(type), " but got ", torch::toString(t.scalar_type()));
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+PagedOperands paged_operands(const torch::Tensor& k_packed, const torch::Tensor& k_scales, const torch::Tensor& k_zeros, const torch::Tensor& v_packed,
+                             const torch::Tensor& v_scales, const torch::Tensor& v_zeros, const torch::Tensor& k_res, const torch::Tensor& v_res,
+                             const torch::Tensor& page_table, const torch::Tensor& slots, const torch::Tensor& seq_lens, const torch::Tensor& cu_new,
+                             int64_t total_new, int64_t max_new, int64_t max_len, int64_t ring_shift, int64_t G) {
+    PagedOperands p{{}, {}, k_res.device()};
+    TORCH_CHECK(k_res.is_cuda(), "k_res must be on cuda but got ", k_res.device().str());
+    TORCH_CHECK(k_res.scalar_type() == torch::kFloat32 || k_res.scalar_type() == torch::kBFloat16, "k_res must be Float or BFloat16 but got ", torch::toString(k_res.scalar_type()));
+    TORCH_CHECK(k_res.dim() == 4 && v_res.sizes() == k_res.sizes(), "k_res and v_res must both be [slots, kv_heads, R, D]");
+    const auto type = k_res.scalar_type();
+    check_paged_tensor(k_res, "k_res", type, p.device);
+    check_paged_tensor(v_res, "v_res", type, p.device);
+    check_paged_tensor(k_packed, "k_packed", torch::kUInt8, p.device);
+    check_paged_tensor(v_packed, "v_packed", torch::kUInt8, p.device);
+    check_paged_tensor(k_scales, "k_scales", torch::kFloat32, p.device);
+    check_paged_tensor(k_zeros, "k_zeros", torch::kFloat32, p.device);
+    check_paged_tensor(v_scales, "v_scales", torch::kFloat32, p.device);
+    check_paged_tensor(v_zeros, "v_zeros", torch::kFloat32, p.device);
+    check_paged_tensor(page_table, "page_table", torch::kInt, p.device);
+    check_paged_tensor(slots, "slots", torch::kInt, p.device);
+    check_paged_tensor(seq_lens, "seq_lens", torch::kInt, p.device);
+    check_paged_tensor(cu_new, "cu_new", torch::kInt, p.device);
+    const int64_t n_slots = k_res.size(0), H = k_res.size(1), R = k_res.size(2), D = k_res.size(3);
+    TORCH_CHECK(G > 0 && G % 4 == 0, "group_size must be positive and divisible by 4, got ", G);
+    TORCH_CHECK(D > 0 && D % G == 0, "head_dim (", D, ") must be divisible by group_size (", G, ")");
+    TORCH_CHECK(k_scales.dim() == 4 && k_scales.size(1) == H && k_scales.size(3) == D && k_scales.numel() > 0, "k_scales must be [pages, kv_heads, page_tokens / group_size, head_dim]");
+    const int64_t pages = k_scales.size(0), gpp = k_scales.size(2), groups = pages * H * gpp;
+    TORCH_CHECK(k_zeros.numel() == groups * D, "k_zeros size must match k_scales size");
+    TORCH_CHECK(k_packed.numel() == groups * (D * G / 4), "k_packed size (", k_packed.numel(), ") must equal pages * kv_heads * page_tokens * head_dim / 4 = ", groups * (D * G / 4));
+    TORCH_CHECK(v_packed.numel() == groups * (D * G / 4), "v_packed size (", v_packed.numel(), ") must equal pages * kv_heads * page_tokens * head_dim / 4 = ", groups * (D * G / 4));
+    TORCH_CHECK(v_scales.numel() == groups * D && v_zeros.numel() == groups * D, "v_scales / v_zeros size must equal pages * kv_heads * page_tokens * head_dim / group_size = ", groups * D);
+    TORCH_CHECK(page_table.dim() == 2, "page_table must be [sequences, pages of a sequence]");
+    const int64_t n = page_table.size(0), width = page_table.size(1);
+    TORCH_CHECK(slots.numel() == n && seq_lens.numel() == n && cu_new.numel() == n + 1,
+                "slots, seq_lens and cu_new must hold ", n, ", ", n, " and ", n + 1, " entries for a page table of ", n, " sequences");
+    for (int64_t x : {n, width, pages, gpp * G, H, R, n_slots, total_new, max_new, max_len, ring_shift})
+        TORCH_CHECK(x >= 0 && x <= kInt32Max, "a size (", x, ") is outside 0 .. 2**31 - 1");
+    p.L = {(int32_t)pages, (int32_t)(gpp * G), (int32_t)H, (int32_t)D, (int32_t)G, (int32_t)R, (int32_t)n_slots, type == torch::kFloat32 ? KIVI_F32 : KIVI_BF16,
+           k_packed.data_ptr<uint8_t>(), k_scales.data_ptr<float>(), k_zeros.data_ptr<float>(), v_packed.data_ptr<uint8_t>(), v_scales.data_ptr<float>(),
+           v_zeros.data_ptr<float>(), k_res.data_ptr(), v_res.data_ptr()};
+    p.b = {(int32_t)n, (int32_t)width, page_table.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), cu_new.data_ptr<int32_t>(),
+           (int32_t)total_new, (int32_t)max_new, (int32_t)max_len, (int32_t)ring_shift};
+    return p;
+}
+
+// [rows, heads, head_dim] of one of the activation types, channels side by side
+kivi_rows rows_of(const torch::Tensor& t, const char* name, int64_t rows, int64_t heads, const PagedOperands& p) {
+    TORCH_CHECK(t.device() == p.device, name, " is on ", t.device().str(), " but k_res is on ", p.device.str(), ": all tensors of one call must be on the same device");
+    TORCH_CHECK(t.dim() == 3 && t.size(0) == rows && t.size(1) == heads && t.size(2) == p.L.head_dim, name, " must be [", rows, ", ", heads, ", ", p.L.head_dim, "]");
+    TORCH_CHECK(t.stride(2) == 1 || t.size(2) == 1 || t.numel() == 0, "the last dimension of ", name, " must be contiguous");
+    TORCH_CHECK(t.stride(0) >= 0 && t.stride(1) >= 0, name, " has a negative stride");
+    return {t.data_ptr(), t.stride(0), t.stride(1)};
+}
+// rows that are written must not share memory
+void check_written(const torch::Tensor& t, const char* name) {
+    const int64_t a = t.stride(0), b = t.stride(1), rows = t.size(0), heads = t.size(1), D = t.size(2);
+    const bool apart = rows <= 1 || heads <= 1 ? (rows <= 1 || a >= D) && (heads <= 1 || b >= D)
+                                               : (b >= D && a >= (heads - 1) * b + D) || (a >= D && b >= (rows - 1) * a + D);
+    TORCH_CHECK(apart, name, " has rows that overlap");
+}
+void check_activation(const torch::Tensor& t, const char* name, const PagedOperands& p) {
+    const auto want = p.L.res_dtype == KIVI_F32 ? torch::kFloat32 : torch::kBFloat16;
+    TORCH_CHECK(t.scalar_type() == want, name, " must be ", torch::toString(want), " like the cache's window but got ", torch::toString(t.scalar_type()));
+}
+
+void paged_append(const torch::Tensor& new_k, const torch::Tensor& new_v, const torch::Tensor& k_packed, const torch::Tensor& k_scales, const torch::Tensor& k_zeros,
+                  const torch::Tensor& v_packed, const torch::Tensor& v_scales, const torch::Tensor& v_zeros, const torch::Tensor& k_res, const torch::Tensor& v_res,
+                  const torch::Tensor& page_table, const torch::Tensor& slots, const torch::Tensor& seq_lens, const torch::Tensor& cu_new, int64_t max_new,
+                  int64_t max_len, int64_t group_size, const c10::optional<torch::Tensor>& rotary, const c10::optional<torch::Tensor>& q,
+                  const c10::optional<torch::Tensor>& q_out, const c10::optional<torch::Tensor>& k_out, bool interleaved, int rounding, int64_t ring_shift) {
+    TORCH_CHECK(new_k.dim() == 3, "new_k must be [rows, kv_heads, head_dim]");
+    const PagedOperands p = paged_operands(k_packed, k_scales, k_zeros, v_packed, v_scales, v_zeros, k_res, v_res, page_table, slots, seq_lens, cu_new,
+                                           new_k.size(0), max_new, max_len, ring_shift, group_size);
+    const int64_t rows = new_k.size(0), H = p.L.num_kv_heads;
+    check_activation(new_k, "new_k", p);
+    check_activation(new_v, "new_v", p);
+    const kivi_rows k = rows_of(new_k, "new_k", rows, H, p), v = rows_of(new_v, "new_v", rows, H, p);
+    TORCH_CHECK(rotary.has_value() == k_out.has_value(), "rotary and k_out are given together or not at all");
+    TORCH_CHECK(q.has_value() == q_out.has_value() && (!q.has_value() || rotary.has_value()), "q and q_out are given together, and only with rotary");
+    kivi_rows qr{}, qo{}, ko{};
+    int64_t n_rep = 1;
+    if (rotary.has_value()) {
+        check_paged_tensor(*rotary, "rotary", torch::kFloat32, p.device);
+        TORCH_CHECK(rotary->dim() == 2 && rotary->size(1) <= kInt32Max, "rotary must be [positions, rotary_dim]: cosines, then sines");
+        check_activation(*k_out, "k_out", p);
+        ko = rows_of(*k_out, "k_out", rows, H, p);
+        check_written(*k_out, "k_out");
+        TORCH_CHECK(ko.data != k.data || (ko.row_stride == k.row_stride && ko.head_stride == k.head_stride), "k_out starts where new_k does but is laid out differently");
+    }
+    if (q.has_value()) {
+        TORCH_CHECK(q->dim() == 3 && q->size(1) % H == 0 && q->size(1) > 0, "q must be [rows, n_rep * kv_heads, head_dim]");
+        n_rep = q->size(1) / H;
+        check_activation(*q, "q", p);
+        check_activation(*q_out, "q_out", p);
+        qr = rows_of(*q, "q", rows, q->size(1), p);
+        qo = rows_of(*q_out, "q_out", rows, q->size(1), p);
+        check_written(*q_out, "q_out");
+        TORCH_CHECK(qo.data != qr.data || (qo.row_stride == qr.row_stride && qo.head_stride == qr.head_stride), "q_out starts where q does but is laid out differently");
+    }
+    c10::cuda::CUDAGuard guard(p.device);
+    if (rows == 0) return;
+    check(kivi_paged_append(&p.L, &p.b, &k, &v, rotary.has_value() ? rotary->data_ptr<float>() : nullptr,
+                            rotary.has_value() ? (int)std::min<int64_t>(rotary->size(0), kInt32Max) : 0, rotary.has_value() ? (int)rotary->size(1) : 0,
+                            interleaved ? 1 : 0, &qr, (int)n_rep, &qo, &ko, rounding, stream_of(k_res)));
+}
+
+void paged_attention(const torch::Tensor& q, const torch::Tensor& new_k, const torch::Tensor& new_v, const torch::Tensor& k_packed, const torch::Tensor& k_scales,
+                     const torch::Tensor& k_zeros, const torch::Tensor& v_packed, const torch::Tensor& v_scales, const torch::Tensor& v_zeros, const torch::Tensor& k_res,
+                     const torch::Tensor& v_res, const torch::Tensor& page_table, const torch::Tensor& slots, const torch::Tensor& seq_lens, const torch::Tensor& cu_new,
+                     int64_t max_new, int64_t max_len, const torch::Tensor& out, int64_t group_size, double sm_scale, int64_t ring_shift) {
+    TORCH_CHECK(q.dim() == 3, "q must be [rows, n_rep * kv_heads, head_dim]");
+    const PagedOperands p = paged_operands(k_packed, k_scales, k_zeros, v_packed, v_scales, v_zeros, k_res, v_res, page_table, slots, seq_lens, cu_new,
+                                           q.size(0), max_new, max_len, ring_shift, group_size);
+    const int64_t rows = q.size(0), H = p.L.num_kv_heads;
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % H == 0, "q must be [rows, n_rep * kv_heads, head_dim]");
+    const int64_t n_rep = q.size(1) / H;
+    check_activation(new_k, "new_k", p);
+    check_activation(new_v, "new_v", p);
+    const int q_dtype = dtype_code(q, "q"), out_dtype = dtype_code(out, "out");
+    const kivi_rows qr = rows_of(q, "q", rows, q.size(1), p), k = rows_of(new_k, "new_k", rows, H, p), v = rows_of(new_v, "new_v", rows, H, p),
+                    o = rows_of(out, "out", rows, q.size(1), p);
+    check_written(out, "out");
+    c10::cuda::CUDAGuard guard(p.device);
+    if (rows == 0) return;
+    const size_t need = kivi_paged_attention_workspace(&p.L, &p.b, q_dtype, (int)n_rep);
+    const torch::Tensor ws = need ? at::empty({(int64_t)need}, q.options().dtype(torch::kUInt8)) : torch::Tensor();
+    check(kivi_paged_attention(&p.L, &p.b, &qr, q_dtype, &k, &v, &o, out_dtype, (int)n_rep, (float)sm_scale, need ? ws.data_ptr() : nullptr, need, stream_of(k_res)));
+}
+
+void paged_read(const torch::Tensor& k_packed, const torch::Tensor& k_scales, const torch::Tensor& k_zeros, const torch::Tensor& v_packed, const torch::Tensor& v_scales,
+                const torch::Tensor& v_zeros, const torch::Tensor& k_res, const torch::Tensor& v_res, const torch::Tensor& page_table, const torch::Tensor& slots,
+                const torch::Tensor& seq_lens, const torch::Tensor& starts, const torch::Tensor& cu_read, int64_t max_read, const torch::Tensor& k_out,
+                const torch::Tensor& v_out, int64_t group_size, int64_t ring_shift) {
+    TORCH_CHECK(k_out.dim() == 3, "k_out must be [rows, kv_heads, head_dim]");
+    PagedOperands p = paged_operands(k_packed, k_scales, k_zeros, v_packed, v_scales, v_zeros, k_res, v_res, page_table, slots, seq_lens, cu_read,
+                                     k_out.size(0), max_read, 0, ring_shift, group_size);
+    // the longest sequence that the page table describes
+    p.b.max_len = (int32_t)std::min<int64_t>((int64_t)p.b.table_width * p.L.page_tokens + p.L.residual_cap - 1, 1 << 30);
+    check_paged_tensor(starts, "starts", torch::kInt, p.device);
+    TORCH_CHECK(starts.numel() == p.b.num_seqs, "starts must hold an entry for every sequence");
+    check_paged_tensor(k_out, "k_out", torch::kFloat32, p.device);
+    check_paged_tensor(v_out, "v_out", torch::kFloat32, p.device);
+    TORCH_CHECK(k_out.size(1) == p.L.num_kv_heads && k_out.size(2) == p.L.head_dim && v_out.sizes() == k_out.sizes(), "k_out and v_out must both be [rows, kv_heads, head_dim]");
+    c10::cuda::CUDAGuard guard(p.device);
+    if (k_out.size(0) == 0) return;
+    check(kivi_paged_read(&p.L, &p.b, starts.data_ptr<int32_t>(), k_out.data_ptr<float>(), v_out.data_ptr<float>(), stream_of(k_res)));
+}
+
+torch::Tensor sample_filtered(const torch::Tensor& logits, const torch::Tensor& uniforms, const c10::optional<torch::Tensor>& temperature,
+                              const c10::optional<torch::Tensor>& top_k, const c10::optional<torch::Tensor>& top_p, const c10::optional<torch::Tensor>& min_p,
+                              const c10::optional<torch::Tensor>& out) {
+    TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [batch, vocab] with entries side by side");
+    TORCH_CHECK(logits.is_cuda(), "logits must be on cuda but got ", logits.device().str());
+    const int dtype = dtype_code(logits, "logits");
+    const int64_t B = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(B <= kInt32Max && V > 0 && V <= kInt32Max, "batch and vocab must be below 2**31, vocab positive");
+    TORCH_CHECK(B <= 1 || logits.stride(0) >= V, "rows of logits overlap");
+    auto per_row = [&](const torch::Tensor& t, const char* name, torch::ScalarType type) {
+        check_paged_tensor(t, name, type, logits.device());
+        TORCH_CHECK(t.numel() == B, name, " must hold an entry for each of the ", B, " rows");
+        return t.data_ptr();
+    };
+    const void* u = per_row(uniforms, "uniforms", torch::kFloat32);
+    const void* t = temperature.has_value() ? per_row(*temperature, "temperature", torch::kFloat32) : nullptr;
+    const void* k = top_k.has_value() ? per_row(*top_k, "top_k", torch::kInt) : nullptr;
+    const void* tp = top_p.has_value() ? per_row(*top_p, "top_p", torch::kFloat32) : nullptr;
+    const void* mp = min_p.has_value() ? per_row(*min_p, "min_p", torch::kFloat32) : nullptr;
+    if (out.has_value()) per_row(*out, "out", torch::kLong);
+    c10::cuda::CUDAGuard guard(logits.device());
+    const torch::Tensor ids = out.has_value() ? *out : at::empty({B}, logits.options().dtype(torch::kLong));
+    if (B == 0) return ids;
+    check(kivi_sample_filtered(logits.data_ptr(), dtype, (int)B, (int)V, std::max<int64_t>(logits.stride(0), V), (const float*)u, (const float*)t, (const int32_t*)k,
+                               (const float*)tp, (const float*)mp, ids.data_ptr<int64_t>(), stream_of(logits)));
+    return ids;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -497,4 +693,31 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("decode_attention_workspace", [](int num_units, int n_rep, int head_dim, int num_splits) {
               return (int64_t)kivi_decode_attention_workspace(num_units, n_rep, head_dim, num_splits); },
           "Bytes of scratch decode_attention needs.", py::arg("num_units"), py::arg("n_rep"), py::arg("head_dim"), py::arg("num_splits") = 0);
+
+    // ---- paged cache -----------------------------------------------------------------
+    m.def("paged_append", &paged_append, py::call_guard<py::gil_scoped_release>(),
+          "Append a step's keys and values [rows, kv_heads, head_dim] of a ragged batch to a paged cache; with rotary [positions, rotary_dim] "
+          "keys (and queries, when given) are turned to their positions on the way and written to k_out (q_out), which may be the inputs. "
+          "seq_lens: tokens held before the step. Stream-ordered.",
+          py::arg("new_k"), py::arg("new_v"), py::arg("k_packed"), py::arg("k_scales"), py::arg("k_zeros"), py::arg("v_packed"), py::arg("v_scales"),
+          py::arg("v_zeros"), py::arg("k_res"), py::arg("v_res"), py::arg("page_table"), py::arg("slots"), py::arg("seq_lens"), py::arg("cu_new"),
+          py::arg("max_new"), py::arg("max_len"), py::arg("group_size"), py::arg("rotary") = py::none(), py::arg("q") = py::none(),
+          py::arg("q_out") = py::none(), py::arg("k_out") = py::none(), py::arg("interleaved") = false, py::arg("rounding") = R0, py::arg("ring_shift") = 0);
+    m.def("paged_attention", &paged_attention, py::call_guard<py::gil_scoped_release>(),
+          "Causal attention of a step's rows over [pages || window || the step's own tokens], after paged_append of the same batch "
+          "(seq_lens as given to it). q, out: [rows, n_rep * kv_heads, head_dim]; new_k, new_v: the step's (turned) keys and values.",
+          py::arg("q"), py::arg("new_k"), py::arg("new_v"), py::arg("k_packed"), py::arg("k_scales"), py::arg("k_zeros"), py::arg("v_packed"),
+          py::arg("v_scales"), py::arg("v_zeros"), py::arg("k_res"), py::arg("v_res"), py::arg("page_table"), py::arg("slots"), py::arg("seq_lens"),
+          py::arg("cu_new"), py::arg("max_new"), py::arg("max_len"), py::arg("out"), py::arg("group_size"), py::arg("sm_scale") = 0.0, py::arg("ring_shift") = 0);
+    m.def("paged_read", &paged_read, py::call_guard<py::gil_scoped_release>(),
+          "Tokens starts[s] .. of every sequence as they are served, fp32: rows cu_read[s] .. cu_read[s+1]-1 of k_out and v_out "
+          "[rows, kv_heads, head_dim]. seq_lens: tokens held now.",
+          py::arg("k_packed"), py::arg("k_scales"), py::arg("k_zeros"), py::arg("v_packed"), py::arg("v_scales"), py::arg("v_zeros"), py::arg("k_res"),
+          py::arg("v_res"), py::arg("page_table"), py::arg("slots"), py::arg("seq_lens"), py::arg("starts"), py::arg("cu_read"), py::arg("max_read"),
+          py::arg("k_out"), py::arg("v_out"), py::arg("group_size"), py::arg("ring_shift") = 0);
+    m.def("sample_filtered", &sample_filtered, py::call_guard<py::gil_scoped_release>(),
+          "Next-token choice under temperature, top-k, top-p and min-p of each row (tensors of one entry per row, or None), from the given "
+          "random numbers in [0, 1); returns the ids.",
+          py::arg("logits"), py::arg("uniforms"), py::arg("temperature") = py::none(), py::arg("top_k") = py::none(), py::arg("top_p") = py::none(),
+          py::arg("min_p") = py::none(), py::arg("out") = py::none());
 }
