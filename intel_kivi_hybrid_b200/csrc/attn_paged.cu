@@ -82,7 +82,7 @@ paged_attention_kernel(PagedAttnArgs A) {
             const int row = row_first + r;
             x = load4_as(A.q, A.q_dtype, (int64_t)q.row0 + row / n_rep, h * n_rep + row % n_rep, d, vec);
         }
-        *reinterpret_cast<float4*>(q_s + r * S + d) = make_float4(x.x * A.scale_log2, x.y * A.scale_log2, x.z * A.scale_log2, x.w * A.scale_log2);
+        *reinterpret_cast<float4*>(q_s + r * S + d) = x;
     }
     float m[RPT], l[RPT], o[RPT][4 * NC];
     int last[RPT];                                       // last token that the row sees
@@ -160,14 +160,14 @@ paged_attention_kernel(PagedAttnArgs A) {
 #pragma unroll
             for (int x = 1; x < 16; x *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
             const float m_new = fmaxf(m[i], mx), base = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = exp2f(m[i] - base);      // 0 while there is no maximum
+            const float alpha = exp2f((m[i] - base) * A.scale_log2);      // 0 while there is no maximum
             m[i] = m_new;
             l[i] *= alpha;
 #pragma unroll
             for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float p = exp2f(sc[i][j] - base);
+                const float p = exp2f((sc[i][j] - base) * A.scale_log2);      // (the difference is rounded at its own size, not at the scores')
                 l[i] += p;
                 p_s[(ty * RPT + i) * (kTile + 4) + tx + 16 * j] = p;
             }
@@ -213,7 +213,7 @@ paged_attention_kernel(PagedAttnArgs A) {
                     store_quad(A.out.data, A.out_dtype, at + 4 * tx + 64 * c, make_float4(o[i][4 * c] * inv, o[i][4 * c + 1] * inv, o[i][4 * c + 2] * inv, o[i][4 * c + 3] * inv));
         } else {
             const int64_t part = (unit * A.pieces + blockIdx.z) * RT + r;
-            if (tx == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m[i], l[i]);
+            if (tx == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m[i] * A.scale_log2, l[i]);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
                 if (4 * tx + 64 * c < D)
@@ -289,14 +289,34 @@ int paged_attention_fault_clear() {
     return KIVI_OK;
 }
 
+bool paged_tc_serves(const kivi_paged_layer* L, int q_dtype);
+int run_paged_tc(const PagedAttnArgs& a, int blocks, cudaStream_t st);
+
 // ---- the cut of a call -----------------------------------------------------------
 // Rows per block, blocks (at most: what the host knows are bounds) and pieces of the
 // sequences' tokens.
-struct PagedPlan { int rows, blocks, pieces, chunk; };
+struct PagedPlan { bool tc; int rows, blocks, pieces, chunk; };
 
-static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b, int n_rep) {
+static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep) {
     PagedPlan p;
     const int64_t rows = (int64_t)b->max_new * n_rep;
+    p.tc = paged_tc_serves(L, q_dtype);
+    if (p.tc) {
+        p.rows = 256;
+        const int64_t blocks = (int64_t)b->total_new * n_rep / p.rows + b->num_seqs;
+        p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
+        // One CTA per SM: the fewest rounds of the shortest pieces, each with the start and
+        // end of a CTA on top (about four tiles).
+        const int tiles = (b->max_len + 127) / 128, most = tiles < 64 ? tiles : 64;
+        const int64_t units = (int64_t)p.blocks * L->num_kv_heads;
+        int64_t best = INT64_MAX;
+        for (int n = 1; n <= most; ++n) {
+            const int per = (tiles + n - 1) / n;
+            const int64_t cost = ((units * n + num_sms() - 1) / num_sms()) * (per + 4);
+            if (cost < best) { best = cost; p.chunk = per * 128; p.pieces = (tiles + per - 1) / per; }
+        }
+        return p;
+    }
     p.rows = rows <= 8 ? 8 : 64;
     const int64_t blocks = ((int64_t)b->total_new * n_rep) / p.rows + b->num_seqs;
     p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
@@ -328,7 +348,7 @@ static int check_attention(const kivi_paged_layer* L, const kivi_paged_batch* b,
 
 extern "C" size_t kivi_paged_attention_workspace(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep) {
     if (check_attention(L, b, q_dtype, n_rep) != KIVI_OK || b->max_new == 0) return 0;
-    const PagedPlan p = plan_paged(L, b, n_rep);
+    const PagedPlan p = plan_paged(L, b, q_dtype, n_rep);
     return p.pieces > 1 ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
 }
 
@@ -344,7 +364,7 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     }
     if (b->max_new == 0) { note_launches(0); return KIVI_OK; }
     const int D = L->head_dim;
-    const PagedPlan p = plan_paged(L, b, n_rep);
+    const PagedPlan p = plan_paged(L, b, q_dtype, n_rep);
     const size_t need = kivi_paged_attention_workspace(L, b, q_dtype, n_rep);
     KIVI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
     KIVI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
@@ -362,7 +382,11 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     cudaStream_t st = (cudaStream_t)stream;
     const size_t smem = ((size_t)(p.rows + 2 * kTile) * (D + 4) + (size_t)p.rows * (kTile + 4)) * 4;
     int rc;
-    if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
+    if (p.tc) {
+        auto grid8 = [](const kivi_rows& r) { return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.row_stride % 8 == 0 && r.head_stride % 8 == 0; };
+        a.vec = grid8(*q) && grid8(*new_k) && grid8(*new_v);
+        rc = run_paged_tc(a, p.blocks, st);
+    } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);
     if (rc) return rc;
     if (p.pieces > 1) {

@@ -72,6 +72,8 @@ int paged_cache_fault_word(int* out);
 int paged_cache_fault_clear();
 int paged_attention_fault_word(int* out);
 int paged_attention_fault_clear();
+int paged_tc_fault_word(int* out);
+int paged_tc_fault_clear();
 int run_merge(const float* part_o, const float* part_ml, void* out, const kivi_peer_gather* gather, float* lse,
               int out_dtype, int num_units, int n_rep, int n_splits, int D, cudaStream_t st);
 
@@ -89,10 +91,11 @@ extern "C" int kivi_device_fault(int* word_out) {
     if (int rc = fp32_fault_word(&copy_wait_fp32)) return rc;
     if (int rc = sample_fault_word(&copy_wait_sample)) return rc;
     if (int rc = gather_fault_word(&peer_wait)) return rc;
-    int paged_cache = 0, paged_attention = 0;
+    int paged_cache = 0, paged_attention = 0, paged_tc = 0;
     if (int rc = paged_cache_fault_word(&paged_cache)) return rc;
     if (int rc = paged_attention_fault_word(&paged_attention)) return rc;
-    *word_out = (copy_wait || copy_wait_fp32 || copy_wait_sample ? 1 : 0) | (peer_wait ? 2 : 0) | paged_cache | paged_attention;
+    if (int rc = paged_tc_fault_word(&paged_tc)) return rc;
+    *word_out = (copy_wait || copy_wait_fp32 || copy_wait_sample ? 1 : 0) | (peer_wait ? 2 : 0) | paged_cache | paged_attention | paged_tc;
     return KIVI_OK;
 }
 
@@ -102,6 +105,7 @@ extern "C" int kivi_device_fault_clear(void) {
     if (int rc = sample_fault_clear()) return rc;
     if (int rc = paged_cache_fault_clear()) return rc;
     if (int rc = paged_attention_fault_clear()) return rc;
+    if (int rc = paged_tc_fault_clear()) return rc;
     return gather_fault_clear();
 }
 
