@@ -5,13 +5,17 @@
 //
 // over tiles of 128 tokens, for two blocks of 128 rows at a time ((new token, query head)
 // pairs of one sequence and KV head: all heads of a group share the tile).  Codes become
-// numbers once per tile and serve 256 rows.  Roles of the 17 warps:
+// numbers once per tile and serve 256 rows.  Roles of the 18 warps:
 //   0-3, 4-7   one thread per row of the first / second block: running maximum and sum,
 //              weights, rescaling, output
-//   8-15       fetch codes, scales and zeros (window and new tokens: rows) and write the
-//              tile's K and V to shared memory, two stages each
+//   8-11       K of a tile: codes, scales and zeros (of the window and the new tokens: rows)
+//              become fp16 numbers in shared memory, two stages; a warp has a group of tokens
+//   12-15      V, likewise
 //   16         one thread issues the MMAs: S of a block while the other block's weights
 //              are made; P comes from tensor memory, where it takes the place of S
+//   17         one thread brings codes, scales and zeros of the tiles to come to shared
+//              memory with bulk copies, two tiles ahead (loads into registers half a tile
+//              ahead left every second tile waiting for its slowest warp)
 //
 // Operands are fp16 numbers with powers of two taken out: a row of Q and a tile of K by
 // their own largest, V by the largest that the CTA has met so far (when it grows, O is
@@ -40,8 +44,8 @@ __device__ int g_fault = 0;
 
 constexpr int kN = 128;                                  // tokens of a tile
 constexpr int kM = 128;                                  // rows of a block
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 8, kThreads = (kSoftmaxWarps + kProducerWarps + 1) * 32;
-constexpr int kProducers = kProducerWarps * 32;
+constexpr int kSoftmaxWarps = 8, kTileWarps = 4;         // (four for keys, four for values)
+constexpr int kMmaWarp = kSoftmaxWarps + 2 * kTileWarps, kCopyWarp = kMmaWarp + 1, kThreads = (kCopyWarp + 1) * 32;
 constexpr int kRing = 4;                                 // factors of so many tiles are kept
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 
@@ -74,12 +78,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : R8(r, 0), R8(r, 8) : "r"(addr) : "memory");
+}
 #undef R8
 #define R8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(addr), R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "memory");
-}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(addr), R8(r, 0), R8(r, 8) : "memory");
@@ -128,28 +132,59 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) { const uint32_t b
 template <int D> struct Shared {
     static constexpr int kBlocks = D / 64;               // blocks of 64 channels, 128 bytes a row
     static constexpr uint32_t kTileBytes = kBlocks * kN * 128;
-    static constexpr uint32_t q = 0, k = 2 * kTileBytes, v = k + 2 * kTileBytes, bars = v + 2 * kTileBytes;
+    static constexpr uint32_t q = 0, k = 2 * kTileBytes, v = k + 2 * kTileBytes, raw = v + 2 * kTileBytes;
+    // codes, scales and zeros of a tile's K or V as they lie in the pages; K of two tiles, then V
+    static constexpr uint32_t kCodes = 32 * D / 4, kFactors = D * 4;            // bytes of a group
+    static constexpr uint32_t raw_s = 4 * kCodes, raw_z = raw_s + 4 * kFactors, kRawBytes = raw_z + 4 * kFactors;
+    static constexpr uint32_t bars = raw + 4 * kRawBytes;
     static constexpr uint32_t bytes = bars + 1024 + 1024;            // (the tiles start on a boundary of 1024)
 };
 // byte of (row, 16-byte piece of a 128-byte row) of a block with the 128-byte swizzle
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return (uint32_t)row * 128u + (uint32_t)((piece ^ (row & 7)) << 4); }
 
 struct Misc {                                            // behind the tiles
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done;
+    uint64_t q_full, full[2][2], empty[2][2], s_full[2], p_half[2], p_full[2], o_done;       // full, empty: [K, V][stage]
+    uint64_t raw_full[2][2], raw_empty[2][2];
     uint32_t tmem;
     int place[2];
     int k_shift[kRing], v_shift[kRing];                  // of tile j at j % kRing
     uint32_t odd[kRing][4];                              // tokens of the tile whose values are not all finite
-    uint32_t top[2][2][kProducerWarps];                  // [tile parity][K, V][warp]
+    uint32_t top[2][2][kTileWarps];                      // [tile parity][K, V][warp]
 };
 
-// What a producer thread holds of a packed group of 32 tokens on its way to shared memory.
-// Keys: (c, m) = lane & 7, token quads 2*jq, 2*jq+1 with jq = lane >> 3; the warp has the
-// group and the block of 64 channels: channels 64*hw + 16*c + 8*m .. +7.
-// Values: r2 = lane & 3, gd & 1 = lane >> 2 & 1, c = lane >> 3; the warp has the group and gd >> 1:
-// channels 32*gd + 8*r2 .. +7 of tokens 16*kap + 4*c + n.
-struct RawK { uint32_t w[4]; float4 s[2], z[2]; };
-struct RawV { uint32_t w[2][2]; float s[2][4], z[2][4]; };
+__device__ __forceinline__ float4 lds_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 lds_float2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds_u32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    return v;
+}
+// columns from `seen` on count for nothing
+__device__ __forceinline__ void hide(uint32_t (&v)[32], int seen) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = i < seen ? v[i] : 0xff800000u;
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -194,13 +229,15 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     const bool whole = t_end == keys && blockIdx.z == 0;
 
     auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
-    if (warp == 16) {
+    if (warp == kMmaWarp) {
         if (elect_one()) {
             mbar_init(bar(misc.q_full), kM * n_sub);
             for (int i = 0; i < 2; ++i) {
-                mbar_init(bar(misc.k_full[i]), kProducerWarps); mbar_init(bar(misc.k_empty[i]), 1);
-                mbar_init(bar(misc.v_full[i]), kProducerWarps); mbar_init(bar(misc.v_empty[i]), 1);
-                mbar_init(bar(misc.s_full[i]), 1); mbar_init(bar(misc.p_full[i]), kM);
+                for (int x = 0; x < 2; ++x) {
+                    mbar_init(bar(misc.full[x][i]), kTileWarps); mbar_init(bar(misc.empty[x][i]), 1);
+                    mbar_init(bar(misc.raw_full[x][i]), 1); mbar_init(bar(misc.raw_empty[x][i]), kTileWarps);
+                }
+                mbar_init(bar(misc.s_full[i]), 1); mbar_init(bar(misc.p_half[i]), kM); mbar_init(bar(misc.p_full[i]), kM);
             }
             mbar_init(bar(misc.o_done), 1);
             mbar_init_fence();
@@ -266,7 +303,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             arrive(bar(misc.q_full));
 
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + t * kN, o_at = tmem + lanes + 2 * kN + t * D;
-            const int last = there ? q.held + token : -1;            // last token that the row sees
+            const int last = there ? q.held + token : 0x3fffffff;    // last token that the row sees (a row that is not there is in nobody's way)
             float m = -INFINITY, l = 0.0f;
             int v_shift = 0;
             const float scale = A.scale_log2;
@@ -275,23 +312,22 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 if (!wait_warp(misc.s_full[t], j)) { ok = false; break; }
                 fence_after();
                 const int t0 = t_begin + j * kN;
+                // (V of tile j stays until this block's weights are there, so its barrier cannot run ahead)
+                if (!wait_warp(misc.full[1][j & 1], j >> 1)) { ok = false; break; }
                 const int k_shift = misc.k_shift[j % kRing], v_new = misc.v_shift[j % kRing];
                 // S is 2^(q_shift + k_shift) times the score
-                const float c = scale * pow2i(-q_shift) * pow2i(-k_shift);
+                const float c = fmaxf(scale * pow2i(-q_shift) * pow2i(-k_shift), 1.0e-37f);      // (not 0: hidden columns are -inf)
                 const int seen = min(last, t_end - 1) - t0 + 1;      // columns that count
+                // (loops of one body: four roles share an instruction cache, unrolled ones cost 15 % of the call)
                 float top = -INFINITY;
 #pragma unroll 1
                 for (int x = 0; x < kN; x += 32) {
                     uint32_t v[32];
                     tmem_load32(s_at + x, v);
                     tmem_wait_load();
-                    if (__all_sync(0xffffffffu, seen >= x + 32)) {
+                    if (__any_sync(0xffffffffu, seen < x + 32)) hide(v, seen - x);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) top = fmaxf(top, x + i < seen ? __uint_as_float(v[i]) : -INFINITY);
-                    }
+                    for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
                 }
                 top *= c;
                 const bool grows = top > m + kGrowth;                // (from -inf: whenever there is a maximum)
@@ -303,13 +339,13 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     if (j > 0) {
                         const float f = (m == -INFINITY ? 1.0f : alpha) * pow2i(max(v_new - v_shift, -126));
 #pragma unroll 1
-                        for (int x = 0; x < D; x += 32) {
-                            uint32_t v[32];
-                            tmem_load32(o_at + x, v);
+                        for (int x = 0; x < D; x += 16) {
+                            uint32_t o[16];
+                            tmem_load16(o_at + x, o);
                             tmem_wait_load();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                            tmem_store32(o_at + x, v);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_store16(o_at + x, o);
                         }
                     }
                 }
@@ -323,29 +359,31 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     }
                 }
                 const float base_m = m == -INFINITY ? 0.0f : m;
+                float2 sum = make_float2(0.0f, 0.0f);
+                // Weights of the upper half, which take columns 64 .. 95 of S, then of the lower, which take
+                // 0 .. 31: the first are contracted while the second are made.
 #pragma unroll 1
-                for (int x = 0; x < kN; x += 32) {
+                for (int i4 = 2; i4 < 6; ++i4) {
+                    const int x = 32 * (i4 & 3);
                     uint32_t v[32], p[16];
                     tmem_load32(s_at + x, v);
                     tmem_wait_load();
-                    const bool all = __all_sync(0xffffffffu, seen >= x + 32);
-                    float sum0 = 0.0f, sum1 = 0.0f;
+                    if (__any_sync(0xffffffffu, seen < x + 32)) hide(v, seen - x);
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        float a = ex2(fmaf(__uint_as_float(v[i]), c, -base_m)), b = ex2(fmaf(__uint_as_float(v[i + 1]), c, -base_m));
-                        if (!all) {
-                            a = x + i < seen ? a : 0.0f;
-                            b = x + i + 1 < seen ? b : 0.0f;
-                        }
-                        sum0 += a; sum1 += b;
-                        p[i / 2] = pack_half(a, b);
+                        const float2 e = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), both(c), both(-base_m));
+                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
+                        sum = add2(sum, w);
+                        p[i / 2] = pack_half(w.x, w.y);
                     }
-                    l += sum0 + sum1;
-                    tmem_store16(s_at + x / 2, p);                   // over columns that have been read
+                    tmem_store16(s_at + (x & 64) + (x & 32) / 2, p);
+                    if (i4 & 1) {
+                        tmem_wait_store();
+                        fence_before();
+                        arrive(bar(i4 == 3 ? misc.p_half[t] : misc.p_full[t]));
+                    }
                 }
-                tmem_wait_store();
-                fence_before();
-                arrive(bar(misc.p_full[t]));
+                l += sum.x + sum.y;
             }
             if (ok && wait_warp(misc.o_done, 0)) {
                 fence_after();
@@ -370,66 +408,16 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 fence_before();
             }
         }
-    } else if (warp < kSoftmaxWarps + kProducerWarps) {
+    } else if (warp < kMmaWarp) {
         // ---------------- tiles ----------------
-        const int pw = warp - kSoftmaxWarps;
-        const int g = pw >> 1;                                       // group of the tile: two warps each
-        const int part = pw & 1;                                     // D = 128: block of 64 channels; D = 64: half of the token quads
-        const int kc = lane & 3, km = lane >> 2 & 1, jq = lane >> 3;
-        const int k_ch = (D == 128 ? 64 * part : 0) + 16 * kc + 8 * km;                      // keys: first of 8 channels
-        const int k_j0 = D == 128 ? 2 * jq : jq + 4 * part;          // token quads k_j0 .. of the group
-        const int vr = lane & 3, vg = lane >> 2 & 1, vc = lane >> 3;
-        const int v_gd = (D == 128 ? 2 * part : 0) + vg, v_ch = 32 * v_gd + 8 * vr;          // values
-        const int64_t groups_per_page = L.page_tokens / G;
-        const __nv_bfloat16* const k_ring = reinterpret_cast<const __nv_bfloat16*>(L.k_res) + ((int64_t)q.slot * H + h) * R * D;
-        const __nv_bfloat16* const v_ring = reinterpret_cast<const __nv_bfloat16*>(L.v_res) + ((int64_t)q.slot * H + h) * R * D;
-        const __nv_bfloat16* const k_new = reinterpret_cast<const __nv_bfloat16*>(A.k.data) + (int64_t)h * A.k.head_stride;
-        const __nv_bfloat16* const v_new = reinterpret_cast<const __nv_bfloat16*>(A.v.data) + (int64_t)h * A.v.head_stride;
-        auto group_at = [&](int t) { return ((int64_t)page_of(L, q, t, &g_fault) * H + h) * groups_per_page + t % L.page_tokens / G; };
-        auto packed = [&](int t0) { return t0 + G <= inside && t0 < t_end; };
-
-        RawK rk;
-        RawV rv;
-        auto fetch_k = [&](int64_t at) {
-            const uint8_t* codes = L.k_codes + at * (D * G / 4) + (D == 128 ? part * 512 : 0) + 32 * km + 4 * kc;
-#pragma unroll
-            for (int i = 0; i < (D == 128 ? 2 : 1); ++i) {
-                rk.w[2 * i] = __ldg(reinterpret_cast<const uint32_t*>(codes + (k_j0 + i) * 64));
-                rk.w[2 * i + 1] = __ldg(reinterpret_cast<const uint32_t*>(codes + (k_j0 + i) * 64 + 16));
-            }
-            const float* s = L.k_scales + at * D + k_ch;
-            const float* z = L.k_zeros + at * D + k_ch;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) { rk.s[i] = __ldg(reinterpret_cast<const float4*>(s) + i); rk.z[i] = __ldg(reinterpret_cast<const float4*>(z) + i); }
-        };
-        // values of D = 128: word (gd, kap, r, c) holds tokens 16 kap + 4 c + n in its bytes; D = 64: rows of 16 bytes a token
-        auto fetch_v = [&](int64_t at) {
-            if constexpr (D == 128) {
-                const uint32_t* codes = reinterpret_cast<const uint32_t*>(L.v_codes + at * 1024) + v_gd * 64 + 8 * vr + vc;
-#pragma unroll
-                for (int kap = 0; kap < 2; ++kap) {
-                    rv.w[kap][0] = __ldg(codes + 32 * kap); rv.w[kap][1] = __ldg(codes + 32 * kap + 4);
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int64_t f = at * 128 + (16 * kap + 4 * n + vc) * 4 + v_gd;
-                        rv.s[kap][n] = __ldg(L.v_scales + f); rv.z[kap][n] = __ldg(L.v_zeros + f);
-                    }
-                }
-            } else {                                                 // tokens 16 part + 4 vc + n, 16 bits of the row each
-                uint32_t b[4];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const int tok = 16 * part + 4 * vc + n;
-                    b[n] = __ldg(reinterpret_cast<const uint16_t*>(L.v_codes + at * 512 + tok * 16) + 4 * vg + vr);
-                    rv.s[0][n] = __ldg(L.v_scales + at * 64 + tok * 2 + v_gd); rv.z[0][n] = __ldg(L.v_zeros + at * 64 + tok * 2 + v_gd);
-                }
-                rv.w[0][0] = (b[0] & 255u) | (b[1] & 255u) << 8 | (b[2] & 255u) << 16 | b[3] << 24;
-                rv.w[0][1] = b[0] >> 8 | (b[1] >> 8) << 8 | (b[2] >> 8) << 16 | (b[3] >> 8) << 24;
-            }
-        };
-        constexpr int kKaps = D == 128 ? 2 : 1, kQuads = D == 128 ? 2 : 1;
+        const bool of_keys = warp < kSoftmaxWarps + kTileWarps;
+        const int x_ = of_keys ? 0 : 1, g = (warp - kSoftmaxWarps) & 3;          // group of the tile
+        const __nv_bfloat16* const ring = reinterpret_cast<const __nv_bfloat16*>(of_keys ? L.k_res : L.v_res) + ((int64_t)q.slot * H + h) * R * D;
+        const kivi_rows& fresh = of_keys ? A.k : A.v;
+        const __nv_bfloat16* const rows_new = reinterpret_cast<const __nv_bfloat16*>(fresh.data) + (int64_t)h * fresh.head_stride;
+        auto group_at = [&](int t) { return ((int64_t)page_of(L, q, t, &g_fault) * H + h) * (L.page_tokens / G) + t % L.page_tokens / G; };
         // rows as they are: eight channels of token t; tokens behind the piece's end are zeros
-        auto row8 = [&](bool of_keys, int t, int ch, float (&y)[8]) {
+        auto row8 = [&](int t, int ch, float (&y)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = 0.0f;
             if (t >= t_end) return;
@@ -449,8 +437,8 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 }
                 return;
             }
-            const __nv_bfloat16* from = t < q.held ? (of_keys ? k_ring : v_ring) + (int64_t)ring_slot(t, A.b.ring_shift, R) * D + ch
-                                                   : (of_keys ? k_new + ((int64_t)q.row0 + t - q.held) * A.k.row_stride : v_new + ((int64_t)q.row0 + t - q.held) * A.v.row_stride) + ch;
+            const __nv_bfloat16* from = t < q.held ? ring + (int64_t)ring_slot(t, A.b.ring_shift, R) * D + ch
+                                                   : rows_new + ((int64_t)q.row0 + t - q.held) * fresh.row_stride + ch;
             if (t < q.held || A.vec) {
                 const uint4 x = *reinterpret_cast<const uint4*>(from);
                 const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -472,156 +460,235 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         auto half8 = [&](const float (&y)[8], float f) {
             return make_uint4(pack_half(y[0] * f, y[1] * f), pack_half(y[2] * f, y[3] * f), pack_half(y[4] * f, y[5] * f), pack_half(y[6] * f, y[7] * f));
         };
-        // tokens of the thread in a group of rows as they are: keys 4 * (k_j0 + i) + n, values 16 * kap + 4 * vc + n
-        auto v_token = [&](int kap, int n) { return (D == 128 ? 16 * kap : 16 * part) + 4 * vc + n; };
-
+        // A tile's numbers: the largest magnitude first (all four warps), then its power of two.
+        // `top_of` and `convert` see the group's codes, scales and zeros in shared memory.
         int v_run = 0;                                               // biased exponent of the largest value so far
-        bool is_packed = packed(t_begin + G * g);
-        if (is_packed) { const int64_t at = group_at(t_begin + G * g); fetch_k(at); fetch_v(at); }
         bool ok = true;
-        for (int j = 0; j < n_tiles; ++j) {
-            const int t0 = t_begin + j * kN + G * g, st = j & 1;
-            // ---- largest of the tile ----
-            uint32_t k_top = 0u, v_top = 0u, odd = 0u;
-            if (is_packed) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float sv[4] = {rk.s[i].x, rk.s[i].y, rk.s[i].z, rk.s[i].w}, zv[4] = {rk.z[i].x, rk.z[i].y, rk.z[i].z, rk.z[i].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) k_top = max(k_top, max(finite_magnitude(zv[e]), finite_magnitude(fmaf(3.0f, sv[e], zv[e]))));
+        auto tiles = [&](auto&& top_of, auto&& convert, auto&& top_dense, auto&& convert_dense) {
+            for (int j = 0; j < n_tiles; ++j) {
+                const int t0 = t_begin + j * kN + G * g, st = j & 1;
+                const bool packed = t0 + G <= inside;
+                const uint32_t raw = base + S::raw + (2 * x_ + st) * S::kRawBytes;
+                uint32_t odd = 0u, top;
+                // (given up: on to the end without waiting, the other warps wait at the barrier below)
+                if (packed) {
+                    if (ok) ok = wait_warp(misc.raw_full[x_][st], j >> 1);
+                    top = top_of(raw);
+                } else {
+                    top = top_dense(t0, odd);
+                    odd = __reduce_or_sync(0xffffffffu, odd);
                 }
-#pragma unroll
-                for (int kap = 0; kap < kKaps; ++kap)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) v_top = max(v_top, max(finite_magnitude(rv.z[kap][n]), finite_magnitude(fmaf(3.0f, rv.s[kap][n], rv.z[kap][n]))));
-            } else {
-                bool none = true;
-#pragma unroll 1
-                for (int i = 0; i < 4 * kQuads; ++i) {
-                    float y[8];
-                    row8(true, t0 + 4 * k_j0 + i, k_ch, y);
-                    k_top = top8(y, k_top, none);
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (lane == 0) misc.top[st][x_][g] = top;
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + x_), "n"(32 * kTileWarps) : "memory");
+                top = __reduce_max_sync(0xffffffffu, misc.top[st][x_][lane & 3]);
+                if (!of_keys) v_run = max(v_run, exponent_of(top));
+                const int shift = shift_of(of_keys ? exponent_of(top) : v_run);
+                if (lane == 0) {
+                    if (g == 0) (of_keys ? misc.k_shift : misc.v_shift)[j % kRing] = shift;
+                    if (!of_keys) misc.odd[j % kRing][g] = odd;
                 }
-#pragma unroll 1
-                for (int i = 0; i < 4 * kKaps; ++i) {
-                    bool finite = true;
-                    const int tok = v_token(i >> 2, i & 3);
-                    float y[8];
-                    row8(false, t0 + tok, v_ch, y);
-                    v_top = top8(y, v_top, finite);
-                    if (!finite) odd |= 1u << tok;
-                }
-                odd = __reduce_or_sync(0xffffffffu, odd);
-            }
-            k_top = __reduce_max_sync(0xffffffffu, k_top);
-            v_top = __reduce_max_sync(0xffffffffu, v_top);
-            if (lane == 0) {
-                misc.top[st][0][pw] = k_top;
-                misc.top[st][1][pw] = v_top;
-                if (part == 0) misc.odd[j % kRing][g] = 0u;
-            }
-            asm volatile("bar.sync 1, %0;" ::"n"(kProducers) : "memory");
-            if (lane == 0 && odd) atomicOr(&misc.odd[j % kRing][g], odd);
-            uint32_t kt = 0u, vt = 0u;
-#pragma unroll
-            for (int w = 0; w < kProducerWarps; ++w) { kt = max(kt, misc.top[st][0][w]); vt = max(vt, misc.top[st][1][w]); }
-            const int k_shift = shift_of(exponent_of(kt));
-            v_run = max(v_run, exponent_of(vt));
-            const int v_shift = shift_of(v_run);
-            if (pw == 0 && lane == 0) { misc.k_shift[j % kRing] = k_shift; misc.v_shift[j % kRing] = v_shift; }
-
-            // ---- keys ----
-            if (ok && j >= 2) ok = wait_warp(misc.k_empty[st], (j >> 1) - 1);        // (given up: on to the end, the other warps wait at the barrier above)
-            uint8_t* const kt_s = smem + S::k + st * S::kTileBytes + (D == 128 ? part * (kN * 128) : 0);
-            const float kf = pow2i(k_shift);
-            const int k_piece = 2 * kc + km;
-            const int next = t0 + kN;
-            const bool next_packed = j + 1 < n_tiles && packed(next);
-            const int64_t next_at = next_packed ? group_at(next) : 0;
-            if (is_packed) {
-                uint32_t s2[4], z2[4];
-                s2[0] = pack_half(rk.s[0].x * kf, rk.s[0].y * kf); s2[1] = pack_half(rk.s[0].z * kf, rk.s[0].w * kf);
-                s2[2] = pack_half(rk.s[1].x * kf, rk.s[1].y * kf); s2[3] = pack_half(rk.s[1].z * kf, rk.s[1].w * kf);
-                z2[0] = pack_half(rk.z[0].x * kf, rk.z[0].y * kf); z2[1] = pack_half(rk.z[0].z * kf, rk.z[0].w * kf);
-                z2[2] = pack_half(rk.z[1].x * kf, rk.z[1].y * kf); z2[3] = pack_half(rk.z[1].z * kf, rk.z[1].w * kf);
-                uint32_t x[kQuads][4];                               // bytes of two channels, 16 bits apart
-#pragma unroll
-                for (int i = 0; i < kQuads; ++i) {
-                    x[i][0] = __byte_perm(rk.w[2 * i], 0u, 0x4140); x[i][1] = __byte_perm(rk.w[2 * i], 0u, 0x4342);
-                    x[i][2] = __byte_perm(rk.w[2 * i + 1], 0u, 0x4140); x[i][3] = __byte_perm(rk.w[2 * i + 1], 0u, 0x4342);
-                }
-                if (next_packed) fetch_k(next_at);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-#pragma unroll
-                    for (int i = 0; i < kQuads; ++i) {
-                        uint32_t y[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & (0x00030003u << (2 * n))) | k1024, kMinus1024), s2[e], z2[e]);
-                        *reinterpret_cast<uint4*>(kt_s + swizzled(G * g + 4 * (k_j0 + i) + n, k_piece)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s2[e] = hmul2(s2[e], 0x34003400u);        // a quarter
-                }
-            } else {
-                if (next_packed) fetch_k(next_at);
-#pragma unroll 1
-                for (int i = 0; i < 4 * kQuads; ++i) {
-                    const int tok = 4 * k_j0 + i;
-                    float y[8];
-                    row8(true, t0 + tok, k_ch, y);
-                    *reinterpret_cast<uint4*>(kt_s + swizzled(G * g + tok, k_piece)) = half8(y, kf);
+                const float f = pow2i(shift);
+                if (ok && j >= 2) ok = wait_warp(misc.empty[x_][st], (j >> 1) - 1);
+                const uint32_t to = base + (of_keys ? S::k : S::v) + st * S::kTileBytes + (uint32_t)(G * g) * 128u;
+                if (packed) convert(raw, to, f);
+                else convert_dense(t0, to, f);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
+                    arrive(bar(misc.raw_empty[x_][st]));
+                    arrive(bar(misc.full[x_][st]));
                 }
             }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) arrive(bar(misc.k_full[st]));
-
-            // ---- values ----
-            if (ok && j >= 2) ok = wait_warp(misc.v_empty[st], (j >> 1) - 1);
-            uint8_t* const vt_s = smem + S::v + st * S::kTileBytes + (v_ch / 64) * (kN * 128);
-            const float vf = pow2i(v_shift);
-            const int v_piece = (v_ch % 64) / 8;
-            if (is_packed) {
-                uint32_t w[kKaps][2];
-                float sv[kKaps][4], zv[kKaps][4];
+        };
+        if (of_keys) {
+            // (c, m) = lane & 7: channels 64 hw + 16 c + 8 m .. + 7, which are two words of a token
+            // quad 16 bytes apart (kblock_offset); quads jq, jq + 4 with jq = lane >> 3
+            const int c = lane & 3, m = lane >> 2 & 1, jq = lane >> 3;
+            const uint32_t piece = 2 * c + m, row0 = 4 * jq, ch = 16 * c + 8 * m;
+            tiles(
+                [&](uint32_t raw) {
+                    float top = 0.0f;
+#pragma unroll 1
+                    for (int hw = 0; hw < D / 64; ++hw)
 #pragma unroll
-                for (int kap = 0; kap < kKaps; ++kap) {
-                    w[kap][0] = rv.w[kap][0]; w[kap][1] = rv.w[kap][1];
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) { sv[kap][n] = rv.s[kap][n] * vf; zv[kap][n] = rv.z[kap][n] * vf; }
-                }
-                if (next_packed) fetch_v(next_at);
-#pragma unroll
-                for (int kap = 0; kap < kKaps; ++kap)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const uint32_t s_lo = pack_half(sv[kap][n], 0.25f * sv[kap][n]), s_hi = hmul2(s_lo, 0x2c002c00u) /* a sixteenth */, z = pack_half(zv[kap][n], zv[kap][n]);
-                        uint32_t y[4];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t b = __byte_perm(w[kap][e], 0u, 0x4040 + 0x0101 * n);      // byte n in both halves
-                            y[2 * e] = hfma2(hadd2((b & 0x000c0003u) | k1024, kMinus1024), s_lo, z);
-                            y[2 * e + 1] = hfma2(hadd2((b & 0x00c00030u) | k1024, kMinus1024), s_hi, z);
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t at = raw + g * S::kFactors + (64 * hw + ch + 4 * i) * 4;
+                            const float4 sc = lds_float4(at + S::raw_s), ze = lds_float4(at + S::raw_z);
+                            top = fmaxf(top, fmaxf(fabsf(ze.x), fabsf(fmaf(3.0f, sc.x, ze.x)))); top = fmaxf(top, fmaxf(fabsf(ze.y), fabsf(fmaf(3.0f, sc.y, ze.y))));
+                            top = fmaxf(top, fmaxf(fabsf(ze.z), fabsf(fmaf(3.0f, sc.z, ze.z)))); top = fmaxf(top, fmaxf(fabsf(ze.w), fabsf(fmaf(3.0f, sc.w, ze.w))));
                         }
-                        *reinterpret_cast<uint4*>(vt_s + swizzled(G * g + v_token(kap, n), v_piece)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
-            } else {
-                if (next_packed) fetch_v(next_at);
+                    return __float_as_uint(top);
+                },
+                [&](uint32_t raw, uint32_t to, float f) {
+                    uint32_t turn[4];                                // pieces of the rows, swizzled
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) turn[n] = to + (row0 + n) * 128 + ((piece ^ ((row0 + n) & 7)) << 4);
 #pragma unroll 1
-                for (int i = 0; i < 4 * kKaps; ++i) {
-                    const int tok = v_token(i >> 2, i & 3);
-                    float y[8];
-                    row8(false, t0 + tok, v_ch, y);
-                    bool finite = true;
-                    top8(y, 0u, finite);                             // (not finite: the rows that see it are told by `odd`)
-                    *reinterpret_cast<uint4*>(vt_s + swizzled(G * g + tok, v_piece)) = finite ? half8(y, vf) : make_uint4(0u, 0u, 0u, 0u);
+                    for (int hw = 0; hw < D / 64; ++hw) {
+                        uint32_t s2[4], z2[4], x[2][4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t af = raw + g * S::kFactors + (64 * hw + ch + 4 * i) * 4;
+                            const float4 sc = lds_float4(af + S::raw_s), ze = lds_float4(af + S::raw_z);
+                            s2[2 * i] = pack_half(sc.x * f, sc.y * f); s2[2 * i + 1] = pack_half(sc.z * f, sc.w * f);
+                            z2[2 * i] = pack_half(ze.x * f, ze.y * f); z2[2 * i + 1] = pack_half(ze.z * f, ze.w * f);
+                            // bytes of two channels, 16 bits apart
+                            const uint32_t at = raw + g * S::kCodes + hw * 512 + (jq + 4 * i) * 64 + 32 * m + 4 * c;
+                            const uint32_t a = lds_u32(at), b = lds_u32(at + 16);
+                            x[i][0] = __byte_perm(a, 0u, 0x4140); x[i][1] = __byte_perm(a, 0u, 0x4342);
+                            x[i][2] = __byte_perm(b, 0u, 0x4140); x[i][3] = __byte_perm(b, 0u, 0x4342);
+                        }
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                uint32_t y[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & (0x00030003u << (2 * n))) | k1024, kMinus1024), s2[e], z2[e]);
+                                sts128(turn[n] + hw * (kN * 128) + i * (16 * 128), y[0], y[1], y[2], y[3]);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s2[e] = hmul2(s2[e], 0x34003400u);        // a quarter
+                        }
+                    }
+                },
+                [&](int t0, uint32_t&) {
+                    uint32_t top = 0u;
+                    bool none = true;
+#pragma unroll 1
+                    for (int i = 0; i < 8 * (D / 64); ++i) {
+                        float y[8];
+                        row8(t0 + row0 + (i & 3) + 4 * (i & 4), 64 * (i >> 3) + ch, y);
+                        top = top8(y, top, none);
+                    }
+                    return top;
+                },
+                [&](int t0, uint32_t to, float f) {
+#pragma unroll 1
+                    for (int i = 0; i < 8 * (D / 64); ++i) {
+                        const uint32_t r = row0 + (i & 3) + 4 * (i & 4);
+                        float y[8];
+                        row8(t0 + r, 64 * (i >> 3) + ch, y);
+                        const uint4 x = half8(y, f);
+                        sts128(to + (i >> 3) * (kN * 128) + r * 128 + ((piece ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+                    }
+                });
+        } else {
+            // r = lane & 3, vg = lane >> 2 & 1: channels 64 p + 32 vg + 8 r .. + 7; tokens 16 kap + 4 c + n
+            // with c = lane >> 3.  D = 128: word (gd, kap, r, c) of the codes holds the four tokens n in its
+            // bytes (kivi_common.cuh); D = 64: 16 bytes a token.
+            const int r = lane & 3, vg = lane >> 2 & 1, c = lane >> 3;
+            const uint32_t piece = (4 * vg + r) ^ (4 * (c & 1)), row0 = 4 * c, ch = 32 * vg + 8 * r;
+            tiles(
+                [&](uint32_t raw) {
+                    // (every factor once: lane and quarter of the group's 32 D/32)
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i) {
+                        const uint32_t at = raw + g * S::kFactors + (i * 64 + 2 * lane) * 4;
+                        const float2 sc = lds_float2(at + S::raw_s), ze = lds_float2(at + S::raw_z);
+                        top = fmaxf(top, fmaxf(fabsf(ze.x), fabsf(fmaf(3.0f, sc.x, ze.x))));
+                        top = fmaxf(top, fmaxf(fabsf(ze.y), fabsf(fmaf(3.0f, sc.y, ze.y))));
+                    }
+                    return __float_as_uint(top);
+                },
+                [&](uint32_t raw, uint32_t to, float f) {
+#pragma unroll 1
+                    for (int pk = 0; pk < 2 * (D / 64); ++pk) {
+                        const int p = pk >> 1, kap = pk & 1;
+                        uint32_t w[2];
+                        if constexpr (D == 128) {
+                            const uint32_t at = raw + g * S::kCodes + ((2 * p + vg) * 64 + 32 * kap + 8 * r + c) * 4;
+                            w[0] = lds_u32(at); w[1] = lds_u32(at + 16);
+                        } else {
+                            w[0] = w[1] = 0u;
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) {
+                                const uint32_t b = lds_u16(raw + g * S::kCodes + (16 * kap + 4 * c + n) * 16 + 8 * vg + 2 * r);
+                                w[0] |= (b & 255u) << (8 * n); w[1] |= (b >> 8) << (8 * n);
+                            }
+                        }
+                        // factors of tokens 16 kap + 4 c + n: rows 4 n + c (kivi_common.cuh), or as they come
+                        const uint32_t at = raw + g * S::kFactors + (D == 128 ? (16 * kap + c) * 16 + (2 * p + vg) * 4 : (16 * kap + 4 * c) * 8 + vg * 4);
+                        const uint32_t out = to + p * (kN * 128) + (row0 + 16 * kap) * 128;
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const float s1 = lds_float(at + S::raw_s + n * (D == 128 ? 64 : 8)) * f, z1 = lds_float(at + S::raw_z + n * (D == 128 ? 64 : 8)) * f;
+                            const uint32_t s_lo = pack_half(s1, 0.25f * s1), s_hi = hmul2(s_lo, 0x2c002c00u) /* a sixteenth */, z = pack_half(z1, z1);
+                            uint32_t y[4];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t b = __byte_perm(w[e], 0u, 0x4040 + 0x0101 * n);      // byte n in both halves
+                                y[2 * e] = hfma2(hadd2((b & 0x000c0003u) | k1024, kMinus1024), s_lo, z);
+                                y[2 * e + 1] = hfma2(hadd2((b & 0x00c00030u) | k1024, kMinus1024), s_hi, z);
+                            }
+                            sts128(out + n * 128 + ((piece ^ n) << 4), y[0], y[1], y[2], y[3]);
+                        }
+                    }
+                },
+                [&](int t0, uint32_t& odd) {
+                    uint32_t top = 0u;
+#pragma unroll 1
+                    for (int i = 0; i < 8 * (D / 64); ++i) {
+                        const uint32_t tok = row0 + (i & 3) + 4 * (i & 4);
+                        bool finite = true;
+                        float y[8];
+                        row8(t0 + tok, 64 * (i >> 3) + ch, y);
+                        top = top8(y, top, finite);
+                        if (!finite) odd |= 1u << tok;
+                    }
+                    return top;
+                },
+                [&](int t0, uint32_t to, float f) {
+#pragma unroll 1
+                    for (int i = 0; i < 8 * (D / 64); ++i) {
+                        const uint32_t tok = row0 + (i & 3) + 4 * (i & 4);
+                        float y[8];
+                        row8(t0 + tok, 64 * (i >> 3) + ch, y);
+                        bool finite = true;
+                        top8(y, 0u, finite);                         // (not finite: the rows that see it are told by `odd`)
+                        const uint4 x = finite ? half8(y, f) : make_uint4(0u, 0u, 0u, 0u);
+                        sts128(to + (i >> 3) * (kN * 128) + tok * 128 + ((piece ^ (i & 3)) << 4), x.x, x.y, x.z, x.w);
+                    }
+                });
+        }
+    } else if (warp == kCopyWarp) {
+        // ---------------- copies ----------------
+        if (elect_one()) {
+            const uint64_t policy = l2_stream_policy();
+            const int gpp = L.page_tokens / G;
+            int page = t_begin / L.page_tokens, group = t_begin % L.page_tokens / G;
+            bool ok = true;
+            int sent = 0;
+            for (int j = 0; ok && j < n_tiles; ++j) {
+                const int t0 = t_begin + j * kN, st = j & 1;
+                const int n = min(max((inside - t0) / G, 0), kN / G);        // whole groups of the tile
+                if (n == 0) break;
+                for (int x = 0; ok && x < 2; ++x) {
+                    if (j >= 2 && !wait(misc.raw_empty[x][st], (j >> 1) - 1)) { ok = false; break; }
+                    mbar_expect_tx(bar(misc.raw_full[x][st]), n * (S::kCodes + 2 * S::kFactors));
                 }
+                for (int i = 0; ok && i < n;) {                              // runs of groups that lie in one page
+                    const int id = q.pages[page], run = min(n - i, gpp - group);
+                    const bool there = (unsigned)id < (unsigned)L.num_pages;
+                    if (!there) atomicOr(&g_fault, kPagedFault);
+                    const int64_t at = ((int64_t)(there ? id : 0) * H + h) * gpp + group;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t to = base + S::raw + (2 * x + st) * S::kRawBytes, b = bar(misc.raw_full[x][st]);
+                        bulk_g2s(to + i * S::kCodes, (x ? L.v_codes : L.k_codes) + at * S::kCodes, run * S::kCodes, b, policy);
+                        bulk_g2s(to + S::raw_s + i * S::kFactors, (x ? L.v_scales : L.k_scales) + at * D, run * S::kFactors, b, policy);
+                        bulk_g2s(to + S::raw_z + i * S::kFactors, (x ? L.v_zeros : L.k_zeros) + at * D, run * S::kFactors, b, policy);
+                    }
+                    i += run;
+                    group += run;
+                    if (group == gpp) { group = 0; ++page; }
+                }
+                if (ok) sent = j + 1;
             }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) arrive(bar(misc.v_full[st]));
-            is_packed = next_packed;
+            // no copy is under way when the block ends
+            for (int j = max(sent - 2, 0); j < sent; ++j) { wait(misc.raw_full[0][j & 1], j >> 1); wait(misc.raw_full[1][j & 1], j >> 1); }
         }
     } else if (elect_one()) {
         // ---------------- MMAs ----------------
@@ -634,26 +701,30 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             }
             mma_commit(bar(misc.s_full[t]));
         };
-        bool ok = wait(misc.q_full, 0) && wait(misc.k_full[0], 0);
+        bool ok = wait(misc.q_full, 0) && wait(misc.full[0][0], 0);
         if (ok) {
             fence_after();
             for (int t = 0; t < n_sub; ++t) scores(t, 0);
-            mma_commit(bar(misc.k_empty[0]));
+            mma_commit(bar(misc.empty[0][0]));
             for (int j = 0; ok && j < n_tiles; ++j) {
                 const int st = j & 1;
                 const bool more = j + 1 < n_tiles;
-                if (!wait(misc.v_full[st], j >> 1) || (more && !wait(misc.k_full[st ^ 1], (j + 1) >> 1))) { ok = false; break; }
+                if (!wait(misc.full[1][st], j >> 1) || (more && !wait(misc.full[0][st ^ 1], (j + 1) >> 1))) { ok = false; break; }
                 for (int t = 0; t < n_sub; ++t) {
-                    if (!wait(misc.p_full[t], j)) { ok = false; break; }
-                    fence_after();
+                    for (int half = 1; ok && half >= 0; --half) {
+                        if (!wait(half ? misc.p_half[t] : misc.p_full[t], j)) { ok = false; break; }
+                        fence_after();
 #pragma unroll
-                    for (int i = 0; i < kN / 16; ++i)
-                        mma_ts(tmem + 2 * kN + t * D, tmem + t * kN + 8 * i, smem_desc(base + S::v + st * S::kTileBytes + i * 2048, kN * 128, 1024), kPV, j > 0 || i > 0);
+                        for (int i = 0; i < kN / 32; ++i)
+                            mma_ts(tmem + 2 * kN + t * D, tmem + t * kN + 64 * half + 8 * i, smem_desc(base + S::v + st * S::kTileBytes + (4 * half + i) * 2048, kN * 128, 1024), kPV,
+                                   j > 0 || half == 0 || i > 0);
+                    }
+                    if (!ok) break;
                     if (more) scores(t, st ^ 1);
                 }
                 if (!ok) break;
-                mma_commit(bar(misc.v_empty[st]));
-                if (more) mma_commit(bar(misc.k_empty[st ^ 1]));
+                mma_commit(bar(misc.empty[1][st]));
+                if (more) mma_commit(bar(misc.empty[0][st ^ 1]));
             }
             if (ok) mma_commit(bar(misc.o_done));
         }
@@ -662,7 +733,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 }  // namespace
