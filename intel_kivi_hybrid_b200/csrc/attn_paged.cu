@@ -222,7 +222,9 @@ paged_attention_kernel(PagedAttnArgs A) {
     }
 }
 
-// Folds the pieces of a block's rows.  grid = (blocks, KV heads), 256 threads.
+// Folds the pieces of a block's rows, a thread per quad of channels of a row.
+// grid = (blocks, KV heads, slices of kFoldRows rows).
+constexpr int kFoldRows = 8;
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(PagedAttnArgs A, int RT) {
     __shared__ int place_s[2];
@@ -249,8 +251,9 @@ paged_merge_kernel(PagedAttnArgs A, int RT) {
     if (n_pieces <= 1) return;
     const int quads = D / 4;
     const int64_t part0 = ((int64_t)blockIdx.x * H + h) * A.pieces;
-    for (int i = threadIdx.x; i < n_rows * quads; i += 256) {
-        const int r = i / quads, d = 4 * (i % quads);
+    for (int i = threadIdx.x; i < kFoldRows * quads; i += 256) {
+        const int r = blockIdx.z * kFoldRows + i / quads, d = 4 * (i % quads);
+        if (r >= n_rows) break;
         float M = -INFINITY, sum = 0.0f;
         for (int p = 0; p < n_pieces; ++p) M = fmaxf(M, A.part_ml[2 * ((part0 + p) * RT + r)]);
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -390,7 +393,7 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);
     if (rc) return rc;
     if (p.pieces > 1) {
-        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads), 256, 0, st, true, a, p.rows));
+        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)((p.rows + kFoldRows - 1) / kFoldRows)), 256, 0, st, true, a, p.rows));
         note_launches(2);
     } else {
         note_launches(1);

@@ -5,15 +5,16 @@
 //
 // over tiles of 128 tokens, for two blocks of 128 rows at a time ((new token, query head)
 // pairs of one sequence and KV head: all heads of a group share the tile).  Codes become
-// numbers once per tile and serve 256 rows.  Roles of the 18 warps:
-//   0-3, 4-7   one thread per row of the first / second block: running maximum and sum,
+// numbers once per tile and serve 256 rows.  Roles of the 27 warps:
+//   0-7, 8-15  two threads per row of the first / second block: running maximum and sum,
 //              weights, rescaling, output
-//   8-11       K of a tile: codes, scales and zeros (of the window and the new tokens: rows)
+//   16-19      K of a tile: codes, scales and zeros (of the window and the new tokens: rows)
 //              become fp16 numbers in shared memory, two stages; a warp has a group of tokens
-//   12-15      V, likewise
-//   16         one thread issues the MMAs: S of a block while the other block's weights
+//   20-23      V, likewise
+//   24         one thread issues the MMAs: S of a block while the other block's weights
 //              are made; P comes from tensor memory, where it takes the place of S
-//   17         one thread brings codes, scales and zeros of the tiles to come to shared
+//   26         finds the largest factor of the tiles of codes, ahead of those who need it
+//   25         one thread brings codes, scales and zeros of the tiles to come to shared
 //              memory with bulk copies, two tiles ahead (loads into registers half a tile
 //              ahead left every second tile waiting for its slowest warp)
 //
@@ -44,9 +45,9 @@ __device__ int g_fault = 0;
 
 constexpr int kN = 128;                                  // tokens of a tile
 constexpr int kM = 128;                                  // rows of a block
-constexpr int kSoftmaxWarps = 8, kTileWarps = 4;         // (four for keys, four for values)
-constexpr int kMmaWarp = kSoftmaxWarps + 2 * kTileWarps, kCopyWarp = kMmaWarp + 1, kThreads = (kCopyWarp + 1) * 32;
-constexpr int kRing = 4;                                 // factors of so many tiles are kept
+constexpr int kSoftmaxWarps = 16, kTileWarps = 4;        // (four for keys, four for values)
+constexpr int kMmaWarp = kSoftmaxWarps + 2 * kTileWarps, kCopyWarp = kMmaWarp + 1, kTopWarp = kMmaWarp + 2, kThreads = (kTopWarp + 1) * 32;
+constexpr int kRing = 8;                                 // exponents of so many tiles are kept (they are found up to four tiles ahead of the rows)
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 
 // ---- tensor core ----------------------------------------------------------------
@@ -72,6 +73,19 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Bounded wait that sleeps in the barrier unit: 27 warps that poll take issue slots from
+// those that work.  A poll gives up after a millisecond at the latest, the wait after
+// some seconds.
+__device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < 4096; ++i) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
 
 #define R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
@@ -125,10 +139,6 @@ __device__ __forceinline__ int shift_of(int e) {         // biased exponent -> p
     return s < -110 ? -110 : s > 110 ? 110 : s;
 }
 __device__ __forceinline__ float pow2i(int s) { return __uint_as_float((uint32_t)(127 + s) << 23); }
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-// of finite numbers only
-__device__ __forceinline__ uint32_t finite_magnitude(float x) { const uint32_t b = magnitude(x); return b < 0x7f800000u ? b : 0u; }
-
 template <int D> struct Shared {
     static constexpr int kBlocks = D / 64;               // blocks of 64 channels, 128 bytes a row
     static constexpr uint32_t kTileBytes = kBlocks * kN * 128;
@@ -137,24 +147,30 @@ template <int D> struct Shared {
     static constexpr uint32_t kCodes = 32 * D / 4, kFactors = D * 4;            // bytes of a group
     static constexpr uint32_t raw_s = 4 * kCodes, raw_z = raw_s + 4 * kFactors, kRawBytes = raw_z + 4 * kFactors;
     static constexpr uint32_t bars = raw + 4 * kRawBytes;
-    static constexpr uint32_t bytes = bars + 1024 + 1024;            // (the tiles start on a boundary of 1024)
+    static constexpr uint32_t bytes = bars + 2048 + 1024;            // (the tiles start on a boundary of 1024)
 };
 // byte of (row, 16-byte piece of a 128-byte row) of a block with the 128-byte swizzle
 __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return (uint32_t)row * 128u + (uint32_t)((piece ^ (row & 7)) << 4); }
 
 struct Misc {                                            // behind the tiles
-    uint64_t q_full, full[2][2], empty[2][2], s_full[2], p_half[2], p_full[2], o_done;       // full, empty: [K, V][stage]
-    uint64_t raw_full[2][2], raw_empty[2][2];
+    uint64_t q_full, full[2][2], empty[2][2], s_full[2], p_full[2][2], o_done;       // full, empty: [K, V][stage]
+    uint64_t raw_full[2][2], raw_empty[2][2], ready[2][2];
     uint32_t tmem;
     int place[2];
-    int k_shift[kRing], v_shift[kRing];                  // of tile j at j % kRing
+    int k_top[kRing], v_top[kRing];                      // biased exponents of tile j's largest at j % kRing
     uint32_t odd[kRing][4];                              // tokens of the tile whose values are not all finite
     uint32_t top[2][2][kTileWarps];                      // [tile parity][K, V][warp]
+    __nv_bfloat16 row_top[2][2][kM];                     // [block][half of the columns][row]
 };
 
 __device__ __forceinline__ float4 lds_float4(uint32_t at) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 lds_uint4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
 __device__ __forceinline__ float2 lds_float2(uint32_t at) {
@@ -177,6 +193,19 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
     return v;
 }
+// Bits of the largest magnitude among z and z + 3 s of a group's factors (D of each): what
+// codes stand for lies between.
+template <int D>
+__device__ __forceinline__ uint32_t group_top(uint32_t factors, int lane) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        const float2 s = lds_float2(factors + Shared<D>::raw_s + (64 * i + 2 * lane) * 4), z = lds_float2(factors + Shared<D>::raw_z + (64 * i + 2 * lane) * 4);
+        top = fmaxf(top, fmaxf(fabsf(z.x), fabsf(fmaf(3.0f, s.x, z.x))));
+        top = fmaxf(top, fmaxf(fabsf(z.y), fabsf(fmaf(3.0f, s.y, z.y))));
+    }
+    return __float_as_uint(top);
+}
 // columns from `seen` on count for nothing
 __device__ __forceinline__ void hide(uint32_t (&v)[32], int seen) {
 #pragma unroll
@@ -194,7 +223,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Misc& misc = *reinterpret_cast<Misc*>(smem + S::bars);
-    static_assert(sizeof(Misc) <= 1024, "behind the tiles");
+    static_assert(sizeof(Misc) <= 2048, "behind the tiles");
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t base = smem_u32(smem);
 
@@ -231,13 +260,13 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
     if (warp == kMmaWarp) {
         if (elect_one()) {
-            mbar_init(bar(misc.q_full), kM * n_sub);
+            mbar_init(bar(misc.q_full), 2 * kM * n_sub);
             for (int i = 0; i < 2; ++i) {
                 for (int x = 0; x < 2; ++x) {
                     mbar_init(bar(misc.full[x][i]), kTileWarps); mbar_init(bar(misc.empty[x][i]), 1);
-                    mbar_init(bar(misc.raw_full[x][i]), 1); mbar_init(bar(misc.raw_empty[x][i]), kTileWarps);
+                    mbar_init(bar(misc.ready[x][i]), 1); mbar_init(bar(misc.raw_full[x][i]), 1); mbar_init(bar(misc.raw_empty[x][i]), kTileWarps);
                 }
-                mbar_init(bar(misc.s_full[i]), 1); mbar_init(bar(misc.p_half[i]), kM); mbar_init(bar(misc.p_full[i]), kM);
+                mbar_init(bar(misc.s_full[i]), 1); mbar_init(bar(misc.p_full[i][0]), kM); mbar_init(bar(misc.p_full[i][1]), kM);
             }
             mbar_init(bar(misc.o_done), 1);
             mbar_init_fence();
@@ -253,7 +282,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     // A wait that runs out is reported and ends the block's work: every role comes to the
     // barrier at the end by waits that are bounded, too.
     auto wait = [&](const uint64_t& b, int phase) {
-        if (mbar_wait(bar(b), (uint32_t)phase & 1u)) return true;
+        if (mbar_sleep(bar(b), (uint32_t)phase & 1u)) return true;
         atomicOr(&g_fault, 1);
         return false;
     };
@@ -261,7 +290,8 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
 
     if (warp < kSoftmaxWarps) {
         // ---------------- rows ----------------
-        const int t = warp >> 2, r = tid & (kM - 1);
+        // two threads to a row, 64 columns each, which hold the same maximum
+        const int t = warp >> 3, half = warp >> 2 & 1, r = tid & (kM - 1);
         if (t < n_sub) {
             const int row = row_first + t * kM + r;
             const bool there = t * kM + r < n_rows;
@@ -280,12 +310,15 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     }
                     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = max(top, max(finite_magnitude(__uint_as_float(w[i] << 16)), finite_magnitude(__uint_as_float(w[i] & 0xffff0000u))));
+                    for (int i = 0; i < 4; ++i) {                 // (the largest finite one)
+                        const uint32_t lo = (w[i] << 16) & 0x7fffffffu, hi = w[i] & 0x7fff0000u;
+                        top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+                    }
                 }
                 q_shift = shift_of(exponent_of(top));
                 const float f = pow2i(q_shift);
-#pragma unroll
-                for (int d = 0; d < D; d += 8) {
+#pragma unroll 1
+                for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 8) {
                     uint32_t w[4] = {0u, 0u, 0u, 0u};
                     if (there) {
                         const uint16_t* u = reinterpret_cast<const uint16_t*>(from + d);
@@ -309,19 +342,20 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             const float scale = A.scale_log2;
             bool ok = true;
             for (int j = 0; j < n_tiles; ++j) {
-                if (!wait_warp(misc.s_full[t], j)) { ok = false; break; }
+                // (given up: on to the end without waiting, the row's other half waits at the barrier below)
+                if (ok) ok = wait_warp(misc.s_full[t], j);
                 fence_after();
                 const int t0 = t_begin + j * kN;
                 // (V of tile j stays until this block's weights are there, so its barrier cannot run ahead)
-                if (!wait_warp(misc.full[1][j & 1], j >> 1)) { ok = false; break; }
-                const int k_shift = misc.k_shift[j % kRing], v_new = misc.v_shift[j % kRing];
+                if (ok) ok = wait_warp(misc.full[1][j & 1], j >> 1);
+                const int k_shift = shift_of(misc.k_top[j % kRing]), v_new = shift_of(misc.v_top[j % kRing]);
                 // S is 2^(q_shift + k_shift) times the score
                 const float c = fmaxf(scale * pow2i(-q_shift) * pow2i(-k_shift), 1.0e-37f);      // (not 0: hidden columns are -inf)
                 const int seen = min(last, t_end - 1) - t0 + 1;      // columns that count
-                // (loops of one body: four roles share an instruction cache, unrolled ones cost 15 % of the call)
+                // (loops of one body: the roles share an instruction cache, unrolled ones cost 15 % of the call)
                 float top = -INFINITY;
 #pragma unroll 1
-                for (int x = 0; x < kN; x += 32) {
+                for (int x = 64 * half; x < 64 * half + 64; x += 32) {
                     uint32_t v[32];
                     tmem_load32(s_at + x, v);
                     tmem_wait_load();
@@ -329,7 +363,11 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
                 }
-                top *= c;
+                // The row's other half: a maximum is a point of reference, eight bits of it do.
+                const __nv_bfloat16 mine = __float2bfloat16_rn(top * c);
+                misc.row_top[t][half][r] = mine;
+                asm volatile("bar.sync %0, %1;" ::"r"(3 + t), "n"(2 * kM) : "memory");
+                top = fmaxf(__bfloat162float(mine), __bfloat162float(misc.row_top[t][half ^ 1][r]));
                 const bool grows = top > m + kGrowth;                // (from -inf: whenever there is a maximum)
                 if (__any_sync(0xffffffffu, grows) || (j > 0 && v_new != v_shift)) {
                     const float m_new = fmaxf(m, top);
@@ -339,7 +377,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     if (j > 0) {
                         const float f = (m == -INFINITY ? 1.0f : alpha) * pow2i(max(v_new - v_shift, -126));
 #pragma unroll 1
-                        for (int x = 0; x < D; x += 16) {
+                        for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 16) {
                             uint32_t o[16];
                             tmem_load16(o_at + x, o);
                             tmem_wait_load();
@@ -360,11 +398,9 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 }
                 const float base_m = m == -INFINITY ? 0.0f : m;
                 float2 sum = make_float2(0.0f, 0.0f);
-                // Weights of the upper half, which take columns 64 .. 95 of S, then of the lower, which take
-                // 0 .. 31: the first are contracted while the second are made.
+                // Weights: columns 0 .. 63 become columns 0 .. 31, 64 .. 127 become 64 .. 95.
 #pragma unroll 1
-                for (int i4 = 2; i4 < 6; ++i4) {
-                    const int x = 32 * (i4 & 3);
+                for (int x = 64 * half; x < 64 * half + 64; x += 32) {
                     uint32_t v[32], p[16];
                     tmem_load32(s_at + x, v);
                     tmem_wait_load();
@@ -377,34 +413,38 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                         p[i / 2] = pack_half(w.x, w.y);
                     }
                     tmem_store16(s_at + (x & 64) + (x & 32) / 2, p);
-                    if (i4 & 1) {
-                        tmem_wait_store();
-                        fence_before();
-                        arrive(bar(i4 == 3 ? misc.p_half[t] : misc.p_full[t]));
-                    }
                 }
+                tmem_wait_store();
+                fence_before();
+                arrive(bar(misc.p_full[t][half]));
                 l += sum.x + sum.y;
             }
-            if (ok && wait_warp(misc.o_done, 0)) {
+            if (ok) ok = wait_warp(misc.o_done, 0);
+            {
                 fence_after();
+                // the other half's sum, through the shared memory of Q, which is not needed any more
+                float* const sums = reinterpret_cast<float*>(smem + S::q) + t * 2 * kM;
+                sums[half * kM + r] = l;
+                asm volatile("bar.sync %0, %1;" ::"r"(3 + t), "n"(2 * kM) : "memory");
+                l += sums[(half ^ 1) * kM + r];
                 const float f = pow2i(-v_shift);
                 const float by = whole ? f / l : f;
                 const int64_t at = ((int64_t)q.row0 + token) * A.out.row_stride + (int64_t)head * A.out.head_stride;
                 const int64_t part = (((int64_t)item * H + h) * A.pieces + blockIdx.z) * (2 * kM) + t * kM + r;
 #pragma unroll 1
-                for (int x = 0; x < D; x += 32) {
-                    uint32_t v[32];
-                    tmem_load32(o_at + x, v);
+                for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 16) {
+                    uint32_t o[16];
+                    tmem_load16(o_at + x, o);
                     tmem_wait_load();
                     if (!there) continue;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 o = make_float4(__uint_as_float(v[i]) * by, __uint_as_float(v[i + 1]) * by, __uint_as_float(v[i + 2]) * by, __uint_as_float(v[i + 3]) * by);
-                        if (whole) store_quad(A.out.data, A.out_dtype, at + x + i, o);
-                        else *reinterpret_cast<float4*>(A.part_o + part * D + x + i) = o;
+                    for (int i = 0; i < 16; i += 4) {
+                        const float4 y = make_float4(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by, __uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
+                        if (whole) store_quad(A.out.data, A.out_dtype, at + x + i, y);
+                        else *reinterpret_cast<float4*>(A.part_o + part * D + x + i) = y;
                     }
                 }
-                if (!whole && there) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m, l);
+                if (!whole && there && half == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m, l);
                 fence_before();
             }
         }
@@ -415,243 +455,231 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         const __nv_bfloat16* const ring = reinterpret_cast<const __nv_bfloat16*>(of_keys ? L.k_res : L.v_res) + ((int64_t)q.slot * H + h) * R * D;
         const kivi_rows& fresh = of_keys ? A.k : A.v;
         const __nv_bfloat16* const rows_new = reinterpret_cast<const __nv_bfloat16*>(fresh.data) + (int64_t)h * fresh.head_stride;
-        auto group_at = [&](int t) { return ((int64_t)page_of(L, q, t, &g_fault) * H + h) * (L.page_tokens / G) + t % L.page_tokens / G; };
-        // rows as they are: eight channels of token t; tokens behind the piece's end are zeros
-        auto row8 = [&](int t, int ch, float (&y)[8]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = 0.0f;
-            if (t >= t_end) return;
-            if (t < inside) {                                        // a token of a group that is not whole here
-                const int64_t at = group_at(t);
-                const int tt = t % G;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (of_keys) {
-                        const uint32_t b = L.k_codes[at * (D * G / 4) + kblock_offset(ch + i, tt >> 2, G / 4, 64)];
-                        y[i] = fmaf((float)((b >> (2 * (tt & 3))) & 3u), L.k_scales[at * D + ch + i], L.k_zeros[at * D + ch + i]);
-                    } else {
-                        const uint32_t b = L.v_codes[at * (D * G / 4) + vcode_offset(tt, (ch + i) / 4, D, G)];
-                        const int64_t f = at * D + vmeta_index(tt, ch / G, D, G);
-                        y[i] = fmaf((float)((b >> (2 * (i & 3))) & 3u), L.v_scales[f], L.v_zeros[f]);
-                    }
-                }
-                return;
-            }
+        // Rows as they are (window, new tokens): lane = (16-byte piece of 64 channels, token of four).
+        const int p8 = lane & 7, sub = lane >> 3;
+        auto row8 = [&](int t, int ch) {                             // eight channels of token t >= inside; behind the piece's end zeros
+            if (t >= t_end) return make_uint4(0u, 0u, 0u, 0u);
             const __nv_bfloat16* from = t < q.held ? ring + (int64_t)ring_slot(t, A.b.ring_shift, R) * D + ch
                                                    : rows_new + ((int64_t)q.row0 + t - q.held) * fresh.row_stride + ch;
-            if (t < q.held || A.vec) {
-                const uint4 x = *reinterpret_cast<const uint4*>(from);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            if (t < q.held || A.vec) return *reinterpret_cast<const uint4*>(from);
+            const uint16_t* u = reinterpret_cast<const uint16_t*>(from);
+            return make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16, u[6] | (uint32_t)u[7] << 16);
+        };
+        auto half8 = [&](const uint4& x, float f) {
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { y[2 * i] = __uint_as_float(w[i] << 16); y[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-            } else {
+            for (int i = 0; i < 4; ++i) y[i] = pack_half(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+            return make_uint4(y[0], y[1], y[2], y[3]);
+        };
+        auto top8 = [&](const uint4& x) {                            // largest magnitudes of the even and the odd channels, as bf16 bits
+            return __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+        };
+        auto any_odd = [&](uint32_t top) { return (top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u; };
+        auto place = [&](uint32_t to, int hw, int r) { return to + hw * (kN * 128) + r * 128 + ((p8 ^ (r & 7)) << 4); };
+
+        // Keys of a packed group.  (c, m) = lane & 7: channels 64 hw + 16 c + 8 m .. + 7, which are two
+        // words of a token quad 16 bytes apart (kblock_offset); quads jq, jq + 4 with jq = lane >> 3.
+        auto convert_keys = [&](uint32_t raw, uint32_t to, float f) {
+            const int c = lane & 3, m = lane >> 2 & 1, jq = lane >> 3;
+            const uint32_t ch = 16 * c + 8 * m;
+            uint32_t turn[4];                                        // pieces of the rows, swizzled
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = __bfloat162float(from[i]);
+            for (int n = 0; n < 4; ++n) turn[n] = to + (4 * jq + n) * 128 + (((2 * c + m) ^ ((4 * jq + n) & 7)) << 4);
+#pragma unroll 1
+            for (int hw = 0; hw < D / 64; ++hw) {
+                uint32_t s2[4], z2[4], x[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t af = raw + g * S::kFactors + (64 * hw + ch + 4 * i) * 4;
+                    const float4 sc = lds_float4(af + S::raw_s), ze = lds_float4(af + S::raw_z);
+                    s2[2 * i] = pack_half(sc.x * f, sc.y * f); s2[2 * i + 1] = pack_half(sc.z * f, sc.w * f);
+                    z2[2 * i] = pack_half(ze.x * f, ze.y * f); z2[2 * i + 1] = pack_half(ze.z * f, ze.w * f);
+                    // bytes of two channels, 16 bits apart
+                    const uint32_t at = raw + g * S::kCodes + hw * 512 + (jq + 4 * i) * 64 + 32 * m + 4 * c;
+                    const uint32_t a = lds_u32(at), b = lds_u32(at + 16);
+                    x[i][0] = __byte_perm(a, 0u, 0x4140); x[i][1] = __byte_perm(a, 0u, 0x4342);
+                    x[i][2] = __byte_perm(b, 0u, 0x4140); x[i][3] = __byte_perm(b, 0u, 0x4342);
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & (0x00030003u << (2 * n))) | k1024, kMinus1024), s2[e], z2[e]);
+                        sts128(turn[n] + hw * (kN * 128) + i * (16 * 128), y[0], y[1], y[2], y[3]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s2[e] = hmul2(s2[e], 0x34003400u);        // a quarter
+                }
             }
         };
-        auto top8 = [&](const float (&y)[8], uint32_t top, bool& finite) {
+        // Values of a packed group.  r = lane & 3, vg = lane >> 2 & 1: channels 64 p + 32 vg + 8 r .. + 7;
+        // tokens 16 kap + 4 c + n with c = lane >> 3.  D = 128: word (gd, kap, r, c) of the codes holds the
+        // four tokens n in its bytes (kivi_common.cuh); D = 64: 16 bytes a token.
+        auto convert_values = [&](uint32_t raw, uint32_t to, float f) {
+            const int r = lane & 3, vg = lane >> 2 & 1, c = lane >> 3;
+            const uint32_t piece = (4 * vg + r) ^ (4 * (c & 1));
+#pragma unroll 1
+            for (int pk = 0; pk < 2 * (D / 64); ++pk) {
+                const int p = pk >> 1, kap = pk & 1;
+                uint32_t w[2];
+                if constexpr (D == 128) {
+                    const uint32_t at = raw + g * S::kCodes + ((2 * p + vg) * 64 + 32 * kap + 8 * r + c) * 4;
+                    w[0] = lds_u32(at); w[1] = lds_u32(at + 16);
+                } else {
+                    w[0] = w[1] = 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                finite = finite && magnitude(y[i]) < 0x7f800000u;
-                top = max(top, finite_magnitude(y[i]));
+                    for (int n = 0; n < 4; ++n) {
+                        const uint32_t b = lds_u16(raw + g * S::kCodes + (16 * kap + 4 * c + n) * 16 + 8 * vg + 2 * r);
+                        w[0] |= (b & 255u) << (8 * n); w[1] |= (b >> 8) << (8 * n);
+                    }
+                }
+                // factors of tokens 16 kap + 4 c + n: rows 4 n + c (kivi_common.cuh), or as they come
+                const uint32_t at = raw + g * S::kFactors + (D == 128 ? (16 * kap + c) * 16 + (2 * p + vg) * 4 : (16 * kap + 4 * c) * 8 + vg * 4);
+                const uint32_t out = to + p * (kN * 128) + (4 * c + 16 * kap) * 128;
+                float sc[4], ze[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) { sc[n] = lds_float(at + S::raw_s + n * (D == 128 ? 64 : 8)); ze[n] = lds_float(at + S::raw_z + n * (D == 128 ? 64 : 8)); }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float s1 = sc[n] * f, z1 = ze[n] * f;
+                    const uint32_t s_lo = pack_half(s1, 0.25f * s1), s_hi = hmul2(s_lo, 0x2c002c00u) /* a sixteenth */, z = pack_half(z1, z1);
+                    uint32_t y[4];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t b = __byte_perm(w[e], 0u, 0x4040 + 0x0101 * n);      // byte n in both halves
+                        y[2 * e] = hfma2(hadd2((b & 0x000c0003u) | k1024, kMinus1024), s_lo, z);
+                        y[2 * e + 1] = hfma2(hadd2((b & 0x00c00030u) | k1024, kMinus1024), s_hi, z);
+                    }
+                    sts128(out + n * 128 + ((piece ^ n) << 4), y[0], y[1], y[2], y[3]);
+                }
             }
-            return top;
         };
-        auto half8 = [&](const float (&y)[8], float f) {
-            return make_uint4(pack_half(y[0] * f, y[1] * f), pack_half(y[2] * f, y[3] * f), pack_half(y[4] * f, y[5] * f), pack_half(y[6] * f, y[7] * f));
-        };
-        // A tile's numbers: the largest magnitude first (all four warps), then its power of two.
-        // `top_of` and `convert` see the group's codes, scales and zeros in shared memory.
-        int v_run = 0;                                               // biased exponent of the largest value so far
+
+        int v_top = 0;                                               // biased exponent of the largest value so far
         bool ok = true;
-        auto tiles = [&](auto&& top_of, auto&& convert, auto&& top_dense, auto&& convert_dense) {
-            for (int j = 0; j < n_tiles; ++j) {
-                const int t0 = t_begin + j * kN + G * g, st = j & 1;
-                const bool packed = t0 + G <= inside;
-                const uint32_t raw = base + S::raw + (2 * x_ + st) * S::kRawBytes;
-                uint32_t odd = 0u, top;
-                // (given up: on to the end without waiting, the other warps wait at the barrier below)
+#pragma unroll 1
+        for (int j = 0; j < n_tiles; ++j) {
+            const int tile0 = t_begin + j * kN, t0 = tile0 + G * g, st = j & 1;
+            const bool packed = t0 < inside;                         // (a group with any token in pages has all 32 there)
+            const uint32_t raw = base + S::raw + (2 * x_ + st) * S::kRawBytes;
+            const uint32_t to = base + (of_keys ? S::k : S::v) + st * S::kTileBytes + (uint32_t)(G * g) * 128u;
+            // (given up: on to the end without waiting, the other warps wait at the barrier below)
+            int e_top;
+            uint32_t odd = 0u;
+            if (tile0 + kN - G < inside) {                           // four packed groups: the power of two is known
+                if (ok) ok = wait_warp(misc.ready[x_][st], j >> 1);
+                e_top = (of_keys ? misc.k_top : misc.v_top)[j % kRing];
+                if (ok && j >= 2) ok = wait_warp(misc.empty[x_][st], (j >> 1) - 1);
+            } else {
+                // rows go to their place as they are, which finds the largest, and are converted there
+                if (ok && j >= 2) ok = wait_warp(misc.empty[x_][st], (j >> 1) - 1);
+                uint32_t top = 0u;
                 if (packed) {
                     if (ok) ok = wait_warp(misc.raw_full[x_][st], j >> 1);
-                    top = top_of(raw);
+                    top = group_top<D>(raw + g * S::kFactors, lane);
                 } else {
-                    top = top_dense(t0, odd);
-                    odd = __reduce_or_sync(0xffffffffu, odd);
+                    uint32_t pair = 0u;
+#pragma unroll 1
+                    for (int i = 0; i < 2 * (D / 64); ++i) {
+                        uint4 x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = row8(t0 + sub + 4 * (4 * (i & 1) + e), 64 * (i >> 1) + 8 * p8);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            pair = __vmaxu2(pair, top8(x[e]));
+                            sts128(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)), x[e].x, x[e].y, x[e].z, x[e].w);
+                        }
+                    }
+                    if (any_odd(pair)) {                             // the largest finite one, and whose rows are not
+                        pair = 0u;
+#pragma unroll 1
+                        for (int i = 0; i < 8 * (D / 64); ++i) {
+                            const int r = sub + 4 * (i & 7);
+                            const uint4 x = lds_uint4(place(to, i >> 3, r));
+                            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
+                                if (lo >= 0x7f80u || hi >= 0x7f80u) odd |= 1u << r;
+                                pair = __vmaxu2(pair, (lo < 0x7f80u ? lo : 0u) | (hi < 0x7f80u ? hi << 16 : 0u));
+                            }
+                        }
+                    }
+                    top = max(pair << 16, pair & 0xffff0000u);
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
                 if (lane == 0) misc.top[st][x_][g] = top;
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + x_), "n"(32 * kTileWarps) : "memory");
-                top = __reduce_max_sync(0xffffffffu, misc.top[st][x_][lane & 3]);
-                if (!of_keys) v_run = max(v_run, exponent_of(top));
-                const int shift = shift_of(of_keys ? exponent_of(top) : v_run);
-                if (lane == 0) {
-                    if (g == 0) (of_keys ? misc.k_shift : misc.v_shift)[j % kRing] = shift;
-                    if (!of_keys) misc.odd[j % kRing][g] = odd;
+                e_top = exponent_of(__reduce_max_sync(0xffffffffu, misc.top[st][x_][lane & 3]));
+                if (!of_keys) e_top = max(e_top, v_top);
+                if (g == 0 && lane == 0) (of_keys ? misc.k_top : misc.v_top)[j % kRing] = e_top;
+            }
+            v_top = e_top;
+            const float f = pow2i(shift_of(e_top));
+            if (packed) {
+                if (of_keys) convert_keys(raw, to, f);
+                else convert_values(raw, to, f);
+                if (t0 + G > inside) {
+                    // the step's own tokens of this group are served as they are, not from the page
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = 0; i < 8 * (D / 64); ++i) {
+                        const int r = sub + 4 * (i & 7);
+                        if (t0 + r < inside) continue;
+                        uint4 x = row8(t0 + r, 64 * (i >> 3) + 8 * p8);
+                        if (!of_keys && any_odd(top8(x))) { odd |= 1u << r; x = make_uint4(0u, 0u, 0u, 0u); }
+                        x = half8(x, f);
+                        sts128(place(to, i >> 3, r), x.x, x.y, x.z, x.w);
+                    }
                 }
-                const float f = pow2i(shift);
-                if (ok && j >= 2) ok = wait_warp(misc.empty[x_][st], (j >> 1) - 1);
-                const uint32_t to = base + (of_keys ? S::k : S::v) + st * S::kTileBytes + (uint32_t)(G * g) * 128u;
-                if (packed) convert(raw, to, f);
-                else convert_dense(t0, to, f);
-                fence_async();
-                __syncwarp();
-                if (lane == 0) {
-                    arrive(bar(misc.raw_empty[x_][st]));
-                    arrive(bar(misc.full[x_][st]));
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 2 * (D / 64); ++i) {
+                    uint4 x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = lds_uint4(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (!of_keys && any_odd(top8(x[e]))) x[e] = make_uint4(0u, 0u, 0u, 0u);      // (the rows that see it are told by `odd`)
+                        x[e] = half8(x[e], f);
+                        sts128(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)), x[e].x, x[e].y, x[e].z, x[e].w);
+                    }
                 }
             }
-        };
-        if (of_keys) {
-            // (c, m) = lane & 7: channels 64 hw + 16 c + 8 m .. + 7, which are two words of a token
-            // quad 16 bytes apart (kblock_offset); quads jq, jq + 4 with jq = lane >> 3
-            const int c = lane & 3, m = lane >> 2 & 1, jq = lane >> 3;
-            const uint32_t piece = 2 * c + m, row0 = 4 * jq, ch = 16 * c + 8 * m;
-            tiles(
-                [&](uint32_t raw) {
-                    float top = 0.0f;
+            if (!of_keys) {
+                odd = __reduce_or_sync(0xffffffffu, odd);
+                if (lane == 0) misc.odd[j % kRing][g] = odd;
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                arrive(bar(misc.raw_empty[x_][st]));
+                arrive(bar(misc.full[x_][st]));
+            }
+        }
+    } else if (warp == kTopWarp) {
+        // ---------------- the largest of a tile of codes ----------------
+        uint32_t v_top = 0u;
+        bool ok = true;
 #pragma unroll 1
-                    for (int hw = 0; hw < D / 64; ++hw)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t at = raw + g * S::kFactors + (64 * hw + ch + 4 * i) * 4;
-                            const float4 sc = lds_float4(at + S::raw_s), ze = lds_float4(at + S::raw_z);
-                            top = fmaxf(top, fmaxf(fabsf(ze.x), fabsf(fmaf(3.0f, sc.x, ze.x)))); top = fmaxf(top, fmaxf(fabsf(ze.y), fabsf(fmaf(3.0f, sc.y, ze.y))));
-                            top = fmaxf(top, fmaxf(fabsf(ze.z), fabsf(fmaf(3.0f, sc.z, ze.z)))); top = fmaxf(top, fmaxf(fabsf(ze.w), fabsf(fmaf(3.0f, sc.w, ze.w))));
-                        }
-                    return __float_as_uint(top);
-                },
-                [&](uint32_t raw, uint32_t to, float f) {
-                    uint32_t turn[4];                                // pieces of the rows, swizzled
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) turn[n] = to + (row0 + n) * 128 + ((piece ^ ((row0 + n) & 7)) << 4);
+        for (int j = 0; j < n_tiles && t_begin + j * kN + kN - G < inside; ++j) {
 #pragma unroll 1
-                    for (int hw = 0; hw < D / 64; ++hw) {
-                        uint32_t s2[4], z2[4], x[2][4];
+            for (int x = 0; x < 2; ++x) {
+                if (ok) ok = wait_warp(misc.raw_full[x][j & 1], j >> 1);
+                uint32_t top = 0u;
+                const uint32_t raw = base + S::raw + (2 * x + (j & 1)) * S::kRawBytes;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t af = raw + g * S::kFactors + (64 * hw + ch + 4 * i) * 4;
-                            const float4 sc = lds_float4(af + S::raw_s), ze = lds_float4(af + S::raw_z);
-                            s2[2 * i] = pack_half(sc.x * f, sc.y * f); s2[2 * i + 1] = pack_half(sc.z * f, sc.w * f);
-                            z2[2 * i] = pack_half(ze.x * f, ze.y * f); z2[2 * i + 1] = pack_half(ze.z * f, ze.w * f);
-                            // bytes of two channels, 16 bits apart
-                            const uint32_t at = raw + g * S::kCodes + hw * 512 + (jq + 4 * i) * 64 + 32 * m + 4 * c;
-                            const uint32_t a = lds_u32(at), b = lds_u32(at + 16);
-                            x[i][0] = __byte_perm(a, 0u, 0x4140); x[i][1] = __byte_perm(a, 0u, 0x4342);
-                            x[i][2] = __byte_perm(b, 0u, 0x4140); x[i][3] = __byte_perm(b, 0u, 0x4342);
-                        }
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                uint32_t y[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & (0x00030003u << (2 * n))) | k1024, kMinus1024), s2[e], z2[e]);
-                                sts128(turn[n] + hw * (kN * 128) + i * (16 * 128), y[0], y[1], y[2], y[3]);
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) s2[e] = hmul2(s2[e], 0x34003400u);        // a quarter
-                        }
-                    }
-                },
-                [&](int t0, uint32_t&) {
-                    uint32_t top = 0u;
-                    bool none = true;
-#pragma unroll 1
-                    for (int i = 0; i < 8 * (D / 64); ++i) {
-                        float y[8];
-                        row8(t0 + row0 + (i & 3) + 4 * (i & 4), 64 * (i >> 3) + ch, y);
-                        top = top8(y, top, none);
-                    }
-                    return top;
-                },
-                [&](int t0, uint32_t to, float f) {
-#pragma unroll 1
-                    for (int i = 0; i < 8 * (D / 64); ++i) {
-                        const uint32_t r = row0 + (i & 3) + 4 * (i & 4);
-                        float y[8];
-                        row8(t0 + r, 64 * (i >> 3) + ch, y);
-                        const uint4 x = half8(y, f);
-                        sts128(to + (i >> 3) * (kN * 128) + r * 128 + ((piece ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
-                    }
-                });
-        } else {
-            // r = lane & 3, vg = lane >> 2 & 1: channels 64 p + 32 vg + 8 r .. + 7; tokens 16 kap + 4 c + n
-            // with c = lane >> 3.  D = 128: word (gd, kap, r, c) of the codes holds the four tokens n in its
-            // bytes (kivi_common.cuh); D = 64: 16 bytes a token.
-            const int r = lane & 3, vg = lane >> 2 & 1, c = lane >> 3;
-            const uint32_t piece = (4 * vg + r) ^ (4 * (c & 1)), row0 = 4 * c, ch = 32 * vg + 8 * r;
-            tiles(
-                [&](uint32_t raw) {
-                    // (every factor once: lane and quarter of the group's 32 D/32)
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < D / 64; ++i) {
-                        const uint32_t at = raw + g * S::kFactors + (i * 64 + 2 * lane) * 4;
-                        const float2 sc = lds_float2(at + S::raw_s), ze = lds_float2(at + S::raw_z);
-                        top = fmaxf(top, fmaxf(fabsf(ze.x), fabsf(fmaf(3.0f, sc.x, ze.x))));
-                        top = fmaxf(top, fmaxf(fabsf(ze.y), fabsf(fmaf(3.0f, sc.y, ze.y))));
-                    }
-                    return __float_as_uint(top);
-                },
-                [&](uint32_t raw, uint32_t to, float f) {
-#pragma unroll 1
-                    for (int pk = 0; pk < 2 * (D / 64); ++pk) {
-                        const int p = pk >> 1, kap = pk & 1;
-                        uint32_t w[2];
-                        if constexpr (D == 128) {
-                            const uint32_t at = raw + g * S::kCodes + ((2 * p + vg) * 64 + 32 * kap + 8 * r + c) * 4;
-                            w[0] = lds_u32(at); w[1] = lds_u32(at + 16);
-                        } else {
-                            w[0] = w[1] = 0u;
-#pragma unroll
-                            for (int n = 0; n < 4; ++n) {
-                                const uint32_t b = lds_u16(raw + g * S::kCodes + (16 * kap + 4 * c + n) * 16 + 8 * vg + 2 * r);
-                                w[0] |= (b & 255u) << (8 * n); w[1] |= (b >> 8) << (8 * n);
-                            }
-                        }
-                        // factors of tokens 16 kap + 4 c + n: rows 4 n + c (kivi_common.cuh), or as they come
-                        const uint32_t at = raw + g * S::kFactors + (D == 128 ? (16 * kap + c) * 16 + (2 * p + vg) * 4 : (16 * kap + 4 * c) * 8 + vg * 4);
-                        const uint32_t out = to + p * (kN * 128) + (row0 + 16 * kap) * 128;
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const float s1 = lds_float(at + S::raw_s + n * (D == 128 ? 64 : 8)) * f, z1 = lds_float(at + S::raw_z + n * (D == 128 ? 64 : 8)) * f;
-                            const uint32_t s_lo = pack_half(s1, 0.25f * s1), s_hi = hmul2(s_lo, 0x2c002c00u) /* a sixteenth */, z = pack_half(z1, z1);
-                            uint32_t y[4];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t b = __byte_perm(w[e], 0u, 0x4040 + 0x0101 * n);      // byte n in both halves
-                                y[2 * e] = hfma2(hadd2((b & 0x000c0003u) | k1024, kMinus1024), s_lo, z);
-                                y[2 * e + 1] = hfma2(hadd2((b & 0x00c00030u) | k1024, kMinus1024), s_hi, z);
-                            }
-                            sts128(out + n * 128 + ((piece ^ n) << 4), y[0], y[1], y[2], y[3]);
-                        }
-                    }
-                },
-                [&](int t0, uint32_t& odd) {
-                    uint32_t top = 0u;
-#pragma unroll 1
-                    for (int i = 0; i < 8 * (D / 64); ++i) {
-                        const uint32_t tok = row0 + (i & 3) + 4 * (i & 4);
-                        bool finite = true;
-                        float y[8];
-                        row8(t0 + tok, 64 * (i >> 3) + ch, y);
-                        top = top8(y, top, finite);
-                        if (!finite) odd |= 1u << tok;
-                    }
-                    return top;
-                },
-                [&](int t0, uint32_t to, float f) {
-#pragma unroll 1
-                    for (int i = 0; i < 8 * (D / 64); ++i) {
-                        const uint32_t tok = row0 + (i & 3) + 4 * (i & 4);
-                        float y[8];
-                        row8(t0 + tok, 64 * (i >> 3) + ch, y);
-                        bool finite = true;
-                        top8(y, 0u, finite);                         // (not finite: the rows that see it are told by `odd`)
-                        const uint4 x = finite ? half8(y, f) : make_uint4(0u, 0u, 0u, 0u);
-                        sts128(to + (i >> 3) * (kN * 128) + tok * 128 + ((piece ^ (i & 3)) << 4), x.x, x.y, x.z, x.w);
-                    }
-                });
+                for (int i = 0; i < kN / G; ++i) top = max(top, group_top<D>(raw + i * S::kFactors, lane));
+                top = __reduce_max_sync(0xffffffffu, top);
+                if (x) top = v_top = max(v_top, top);
+                if (lane == 0) {
+                    (x ? misc.v_top : misc.k_top)[j % kRing] = exponent_of(top);
+                    arrive(bar(misc.ready[x][j & 1]));
+                }
+            }
         }
     } else if (warp == kCopyWarp) {
         // ---------------- copies ----------------
@@ -663,28 +691,28 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             int sent = 0;
             for (int j = 0; ok && j < n_tiles; ++j) {
                 const int t0 = t_begin + j * kN, st = j & 1;
-                const int n = min(max((inside - t0) / G, 0), kN / G);        // whole groups of the tile
+                const int n = min(max((inside - t0 + G - 1) / G, 0), kN / G);        // groups of the tile with a token in pages
                 if (n == 0) break;
-                for (int x = 0; ok && x < 2; ++x) {
+                int next_page = page, next_group = group;
+                for (int x = 0; ok && x < 2; ++x) {                          // (keys do not wait for the values' buffer)
                     if (j >= 2 && !wait(misc.raw_empty[x][st], (j >> 1) - 1)) { ok = false; break; }
-                    mbar_expect_tx(bar(misc.raw_full[x][st]), n * (S::kCodes + 2 * S::kFactors));
-                }
-                for (int i = 0; ok && i < n;) {                              // runs of groups that lie in one page
-                    const int id = q.pages[page], run = min(n - i, gpp - group);
-                    const bool there = (unsigned)id < (unsigned)L.num_pages;
-                    if (!there) atomicOr(&g_fault, kPagedFault);
-                    const int64_t at = ((int64_t)(there ? id : 0) * H + h) * gpp + group;
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t to = base + S::raw + (2 * x + st) * S::kRawBytes, b = bar(misc.raw_full[x][st]);
+                    const uint32_t to = base + S::raw + (2 * x + st) * S::kRawBytes, b = bar(misc.raw_full[x][st]);
+                    mbar_expect_tx(b, n * (S::kCodes + 2 * S::kFactors));
+                    next_page = page; next_group = group;
+                    for (int i = 0; i < n;) {                                // runs of groups that lie in one page
+                        const int id = q.pages[next_page], run = min(n - i, gpp - next_group);
+                        const bool there = (unsigned)id < (unsigned)L.num_pages;
+                        if (!there) atomicOr(&g_fault, kPagedFault);
+                        const int64_t at = ((int64_t)(there ? id : 0) * H + h) * gpp + next_group;
                         bulk_g2s(to + i * S::kCodes, (x ? L.v_codes : L.k_codes) + at * S::kCodes, run * S::kCodes, b, policy);
                         bulk_g2s(to + S::raw_s + i * S::kFactors, (x ? L.v_scales : L.k_scales) + at * D, run * S::kFactors, b, policy);
                         bulk_g2s(to + S::raw_z + i * S::kFactors, (x ? L.v_zeros : L.k_zeros) + at * D, run * S::kFactors, b, policy);
+                        i += run;
+                        next_group += run;
+                        if (next_group == gpp) { next_group = 0; ++next_page; }
                     }
-                    i += run;
-                    group += run;
-                    if (group == gpp) { group = 0; ++page; }
                 }
+                page = next_page; group = next_group;
                 if (ok) sent = j + 1;
             }
             // no copy is under way when the block ends
@@ -712,7 +740,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 if (!wait(misc.full[1][st], j >> 1) || (more && !wait(misc.full[0][st ^ 1], (j + 1) >> 1))) { ok = false; break; }
                 for (int t = 0; t < n_sub; ++t) {
                     for (int half = 1; ok && half >= 0; --half) {
-                        if (!wait(half ? misc.p_half[t] : misc.p_full[t], j)) { ok = false; break; }
+                        if (!wait(misc.p_full[t][half], j)) { ok = false; break; }
                         fence_after();
 #pragma unroll
                         for (int i = 0; i < kN / 32; ++i)
