@@ -155,6 +155,7 @@ __device__ __forceinline__ uint32_t swizzled(int row, int piece) { return (uint3
 struct Misc {                                            // behind the tiles
     uint64_t q_full, full[2][2], empty[2][2], s_full[2], p_full[2][2], o_done;       // full, empty: [K, V][stage]
     uint64_t raw_full[2][2], raw_empty[2][2], ready[2][2];
+    uint64_t v_known[4];                                 // v_top of tile j, at j % 4
     uint32_t tmem;
     int place[2];
     int k_top[kRing], v_top[kRing];                      // biased exponents of tile j's largest at j % kRing
@@ -268,6 +269,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 }
                 mbar_init(bar(misc.s_full[i]), 1); mbar_init(bar(misc.p_full[i][0]), kM); mbar_init(bar(misc.p_full[i][1]), kM);
             }
+            for (int i = 0; i < 4; ++i) mbar_init(bar(misc.v_known[i]), 1);
             mbar_init(bar(misc.o_done), 1);
             mbar_init_fence();
         }
@@ -346,9 +348,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 if (ok) ok = wait_warp(misc.s_full[t], j);
                 fence_after();
                 const int t0 = t_begin + j * kN;
-                // (V of tile j stays until this block's weights are there, so its barrier cannot run ahead)
-                if (ok) ok = wait_warp(misc.full[1][j & 1], j >> 1);
-                const int k_shift = shift_of(misc.k_top[j % kRing]), v_new = shift_of(misc.v_top[j % kRing]);
+                const int k_shift = shift_of(misc.k_top[j % kRing]);
                 // S is 2^(q_shift + k_shift) times the score
                 const float c = fmaxf(scale * pow2i(-q_shift) * pow2i(-k_shift), 1.0e-37f);      // (not 0: hidden columns are -inf)
                 const int seen = min(last, t_end - 1) - t0 + 1;      // columns that count
@@ -368,6 +368,9 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 misc.row_top[t][half][r] = mine;
                 asm volatile("bar.sync %0, %1;" ::"r"(3 + t), "n"(2 * kM) : "memory");
                 top = fmaxf(__bfloat162float(mine), __bfloat162float(misc.row_top[t][half ^ 1][r]));
+                // (V of tile j + 2 is not made before this tile's weights are contracted, so the barrier's phase is this tile's)
+                if (ok) ok = wait_warp(misc.v_known[j % 4], j >> 2);
+                const int v_new = shift_of(misc.v_top[j % kRing]);
                 const bool grows = top > m + kGrowth;                // (from -inf: whenever there is a maximum)
                 if (__any_sync(0xffffffffu, grows) || (j > 0 && v_new != v_shift)) {
                     const float m_new = fmaxf(m, top);
@@ -388,7 +391,8 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     }
                 }
                 v_shift = v_new;
-                if (t0 + kN > inside) {                              // a tile that holds rows as they are
+                if (t0 + kN > inside) {                              // a tile that holds rows as they are: whose values are not finite comes with V
+                    if (ok) ok = wait_warp(misc.full[1][j & 1], j >> 1);
                     const uint32_t* odd = misc.odd[j % kRing];
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
@@ -615,7 +619,10 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + x_), "n"(32 * kTileWarps) : "memory");
                 e_top = exponent_of(__reduce_max_sync(0xffffffffu, misc.top[st][x_][lane & 3]));
                 if (!of_keys) e_top = max(e_top, v_top);
-                if (g == 0 && lane == 0) (of_keys ? misc.k_top : misc.v_top)[j % kRing] = e_top;
+                if (g == 0 && lane == 0) {
+                    (of_keys ? misc.k_top : misc.v_top)[j % kRing] = e_top;
+                    if (!of_keys) arrive(bar(misc.v_known[j % 4]));
+                }
             }
             v_top = e_top;
             const float f = pow2i(shift_of(e_top));
@@ -678,6 +685,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 if (lane == 0) {
                     (x ? misc.v_top : misc.k_top)[j % kRing] = exponent_of(top);
                     arrive(bar(misc.ready[x][j & 1]));
+                    if (x) arrive(bar(misc.v_known[j % 4]));
                 }
             }
         }
@@ -737,7 +745,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             for (int j = 0; ok && j < n_tiles; ++j) {
                 const int st = j & 1;
                 const bool more = j + 1 < n_tiles;
-                if (!wait(misc.full[1][st], j >> 1) || (more && !wait(misc.full[0][st ^ 1], (j + 1) >> 1))) { ok = false; break; }
+                if (!wait(misc.full[1][st], j >> 1)) { ok = false; break; }
                 for (int t = 0; t < n_sub; ++t) {
                     for (int half = 1; ok && half >= 0; --half) {
                         if (!wait(misc.p_full[t][half], j)) { ok = false; break; }
@@ -747,6 +755,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                             mma_ts(tmem + 2 * kN + t * D, tmem + t * kN + 64 * half + 8 * i, smem_desc(base + S::v + st * S::kTileBytes + (4 * half + i) * 2048, kN * 128, 1024), kPV,
                                    j > 0 || half == 0 || i > 0);
                     }
+                    if (t == 0 && more && ok) ok = wait(misc.full[0][st ^ 1], (j + 1) >> 1);
                     if (!ok) break;
                     if (more) scores(t, st ^ 1);
                 }
