@@ -2,16 +2,34 @@
 // random numbers.
 //
 // m_i = exp((x_i - max) / temperature) needs no normalisation: every cut compares masses
-// with masses.  The k-th largest logit is found by bisection on the bits of an
-// order-preserving integer (counts), the nucleus likewise (fp64 sums of the masses above a
-// candidate), and the draw walks the kept masses in index order.  No sum goes through
-// atomics, so the same inputs give the same id.
+// with masses.  A CTA walks its row up to four times, each from L2:
+//   1. the largest entry and its first index;
+//   2. (top-k or top-p) entries per bin of 1/256 octave of mass, 32 octaves: the counts give
+//      the bin that the k-th largest is in, and bound the mass above any bin to 0.15 %, which
+//      leaves a few bins that the nucleus can end in;
+//   3. exact masses: all of them, those above the open bins, and a list of the entries in
+//      the open bins, on which both cuts are then found by bisection (keys of the list, so that
+//      ties stay together);
+//   4. sums of the kept masses over runs of the row, and the run, piece and entry at which
+//      the sum passes uniform * all.
+// Lists that do not fit (thousands of equal logits at a cut) are replaced by bisection over
+// the row.  Lists come in any order: what is summed over them are whole numbers (2^-50 of
+// the largest mass), so that the same inputs give the same id.
+//
+// Masses: 2^(k/256) from a table in fp64 and a correction below 2^-9 of it in fp32; the
+// exponent (x - max) log2(e) 256 / T is a product of two-term fp32 numbers, good to 1e-10.
+// fp64 takes one addition per entry.
+// Bound by latency: 4 walks of 2-3 us, 13 barriers.
 #include "kivi_common.cuh"
 
 namespace kivi {
 namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBins = 8192;                              // of 1/256 octave; the last holds what is below 2^-32
+constexpr int kPerThread = kBins / kThreads;
+constexpr int kListK = 2048, kListP = 4096;              // entries at the k-th largest, at the end of the nucleus
+constexpr float kSlack = 0.0016f;                        // 2^(0.5/256) - 1 and roundings: how far a bin's mass is off its centre's
 
 // order-preserving map float -> uint32; NaN counts as -inf
 __device__ __forceinline__ uint32_t ordered_key(float x) {
@@ -19,141 +37,404 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
     const uint32_t b = __float_as_uint(x);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-
-template <typename T> __device__ __forceinline__ float entry(const T* row, int i) { return (float)row[i]; }
-
-__device__ __forceinline__ double block_sum(double x, double* s) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    double sum = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += s[w];
-    return sum;
-}
-__device__ __forceinline__ int block_count(int x, int* s) {
-    x = __reduce_add_sync(0xffffffffu, x);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += s[w];
-    return sum;
-}
+__device__ __forceinline__ float key_to_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
 struct FilterArgs {
     const float *uniforms, *temperature, *top_p, *min_p;
     const int32_t* top_k;
 };
 
+struct Shared {
+    uint32_t bins[kBins];
+    uint32_t list_k[kListK], list_p[kListP];
+    unsigned long long mass_p[kListP];                   // in units of 2^-50
+    double exp_table[256];
+    float exp_table_f[256];
+    double sum[kWarps];
+    unsigned long long sum_u[kWarps];
+    float part[kWarps];
+    int count[kWarps];
+    uint32_t key[kWarps];
+    int first, bin_k, need, zone_lo, zone_hi, n_k, n_p, pick, last;
+    float mass_k[2], tail;
+    uint32_t cut;
+};
+
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+// sums over the block, the same bits in every thread
+__device__ __forceinline__ double block_sum(double x, double* s) {
+    x = warp_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
+    __syncthreads();
+    return warp_sum(s[threadIdx.x & 31]);
+}
+__device__ __forceinline__ unsigned long long block_sum(unsigned long long x, unsigned long long* s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = s[threadIdx.x & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+constexpr double kUnit = 1125899906842624.0;             // 2^50
+__device__ __forceinline__ unsigned long long units(double mass) { return (unsigned long long)__double2ll_rn(mass * kUnit); }
+__device__ __forceinline__ int block_count(int x, int* s) {
+    x = __reduce_add_sync(0xffffffffu, x);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, s[threadIdx.x & 31]);
+}
+
+// The entries of an aligned 16 bytes
+template <typename T> struct Granule;
+template <> struct Granule<float> {
+    static constexpr int kSize = 4;
+    __device__ static void get(const uint4& v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+    }
+};
+template <> struct Granule<__nv_bfloat16> {
+    static constexpr int kSize = 8;
+    __device__ static void get(const uint4& v, float (&x)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+};
+// f(x, index) for entries [lo, hi) of a row, by `n` threads of which this is number `me`:
+// 16 bytes at a time, four in flight, the ends one by one.
+template <typename T, typename F>
+__device__ __forceinline__ void walk(const T* row, int lo, int hi, int me, int n, const F& f) {
+    constexpr int kSize = Granule<T>::kSize;
+    const int off = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15u) / sizeof(T));
+    int body = lo + (off ? kSize - off : 0);             // first entry on a 16-byte boundary
+    if (body > hi) body = hi;
+    const int granules = (hi - body) / kSize, tail = body + granules * kSize;
+    for (int i = lo + me; i < body; i += n) f((float)row[i], i);
+    const uint4* g = reinterpret_cast<const uint4*>(row + body);
+    for (int i = me; i < granules; i += 4 * n) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * n < granules) v[j] = g[i + j * n];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * n < granules) {
+                float x[kSize];
+                Granule<T>::get(v[j], x);
+#pragma unroll
+                for (int e = 0; e < kSize; ++e) f(x[e], body + (i + j * n) * kSize + e);
+            }
+    }
+    for (int i = tail + me; i < hi; i += n) f((float)row[i], i);
+}
+
+// Masses relative to the row's largest entry.
+struct Masses {
+    float largest, c_hi, c_lo;                           // 256 log2(e) / T in two terms
+    bool only_largest;                                   // an infinite largest, or a temperature that leaves nothing else
+    const double* table;
+    const float* table_f;
+
+    // exponent in 1/256 octaves, whole and rest; false: no mass at all
+    __device__ __forceinline__ bool exponent(float x, int& k, float& rest) const {
+        const float d = __fsub_rn(x, largest);
+        const float p = __fmul_rn(d, c_hi);
+        if (!(p > -250000.0f)) return false;             // below 2^-976, -inf or NaN
+        // d = x - largest to the last bit: what the subtraction rounded away
+        const float b = __fsub_rn(x, d), lost = __fadd_rn(__fsub_rn(x, __fadd_rn(d, b)), __fsub_rn(b, largest));
+        const float whole = rintf(p);
+        k = (int)whole;
+        rest = __fsub_rn(p, whole) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi)));
+        return true;
+    }
+    // mass = hi + lo
+    __device__ __forceinline__ bool get(float x, double& hi, float& lo) const {
+        int k;
+        float r;
+        if (only_largest) {
+            hi = x == largest ? 1.0 : 0.0; lo = 0.0f;
+            return x == largest;
+        }
+        if (!exponent(x, k, r)) { hi = 0.0; lo = 0.0f; return false; }
+        const int n = k >> 8;
+        const double t = table[k & 255];
+        hi = __hiloint2double(__double2hiint(t) + (n << 20), __double2loint(t));
+        const float u = r * 0.0027076061740622863f;      // ln 2 / 256
+        const float e = u * fmaf(u, fmaf(u, 0.16666667f, 0.5f), 1.0f);       // 2^(r/256) - 1 to u^4 / 24 = 1e-13
+        // (a mass below 2^-120 needs no correction)
+        lo = n > -120 ? e * __uint_as_float(__float_as_uint(table_f[k & 255]) + (uint32_t)(n * (1 << 23))) : 0.0f;
+        return true;
+    }
+    // bin of an entry with mass
+    __device__ __forceinline__ int bin(int k) const { return -k < kBins - 1 ? (-k > 0 ? -k : 0) : kBins - 1; }
+};
+
+// sums of two terms, folded once at the end
+struct Sum {
+    double hi = 0.0;
+    float lo = 0.0f;
+    __device__ __forceinline__ void add(double h, float l) { hi += h; lo += l; }
+    __device__ __forceinline__ double value() const { return hi + (double)lo; }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1)
 sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArgs f, int64_t* __restrict__ ids) {
-    __shared__ double sum_s[kWarps];
-    __shared__ int int_s[kWarps];
-    __shared__ uint32_t key_s[kWarps];
-    __shared__ int pick_s;
-    stream_order();
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared& s = *reinterpret_cast<Shared*>(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
+    if (tid < 256) {
+        const double t = exp2((double)tid * (1.0 / 256.0));
+        s.exp_table[tid] = t;
+        s.exp_table_f[tid] = (float)t;
+    }
+    if (tid == 0) { s.first = 0x7fffffff; s.bin_k = kBins; s.need = 0; s.zone_lo = kBins; s.zone_hi = -1; s.n_k = 0; s.n_p = 0; s.pick = 0x7fffffff; s.last = -1; }
+    for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0u;
+    stream_order();
     const T* const row = settled(logits) + (int64_t)b * row_stride;
     const float u = settled(f.uniforms)[b], temperature = f.temperature ? settled(f.temperature)[b] : 1.0f;
     const float top_p = f.top_p ? settled(f.top_p)[b] : 1.0f, min_p = f.min_p ? settled(f.min_p)[b] : 0.0f;
     const int top_k = f.top_k ? settled(f.top_k)[b] : 0;
-    if (tid == 0) pick_s = 0x7fffffff;
+    const bool cut_k = top_k > 0 && top_k < vocab, cut_p = top_p < 1.0f;
 
-    // the largest and its first index
-    uint32_t best = 0u;
+    // ---- 1. the largest and its first index ----
+    float best = -INFINITY;
     int at = 0x7fffffff;
-    for (int64_t i = tid; i < vocab; i += kThreads) {
-        const uint32_t k = ordered_key(entry(row, (int)i));
-        if (k > best) { best = k; at = (int)i; }
-    }
-    const uint32_t warp_best = __reduce_max_sync(0xffffffffu, best);
-    if (lane == 0) key_s[warp] = warp_best;
+    walk(row, 0, vocab, tid, kThreads, [&](float x, int i) {
+        if (x > best || (x == best && i < at)) { best = x; at = i; }
+    });
+    const uint32_t mine = ordered_key(best), warp_best = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0) s.key[warp] = warp_best;
     __syncthreads();
-    uint32_t top = 0u;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = max(top, key_s[w]);
-    if (best == top) atomicMin(&pick_s, at);
+    const uint32_t top = __reduce_max_sync(0xffffffffu, s.key[lane]);
+    if (mine == top) atomicMin(&s.first, at);
     __syncthreads();
-    const int first = pick_s;
-    const float largest = __uint_as_float((top & 0x80000000u) ? (top & 0x7fffffffu) : ~top);
+    const float largest = key_to_float(top);
     if (!(temperature > 0.0f) || largest == -INFINITY) {
-        if (tid == 0) ids[b] = largest == -INFINITY ? 0 : first;
+        if (tid == 0) ids[b] = largest == -INFINITY ? 0 : s.first;
         return;
     }
-    auto mass = [&](float x) {
-        if (x == largest) return 1.0;
-        if (!(x > -INFINITY) || largest == INFINITY) return 0.0;
-        return exp(((double)x - (double)largest) / (double)temperature);
-    };
+    Masses m;
+    m.largest = largest;
+    const double c = 256.0 * 1.4426950408889634 / (double)temperature;
+    m.c_hi = (float)c;
+    m.c_lo = (float)(c - (double)m.c_hi);
+    m.only_largest = largest == INFINITY || temperature < 1e-30f;
+    m.table = s.exp_table;
+    m.table_f = s.exp_table_f;
 
     uint32_t cut = 0u;                                   // least key that is kept
-    if (top_k > 0 && top_k < vocab) {
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t probe = cut | (1u << bit);
-            int n = 0;
-            for (int64_t i = tid; i < vocab; i += kThreads) n += ordered_key(entry(row, (int)i)) >= probe;
-            if (block_count(n, int_s) >= top_k) cut = probe;
+    if ((cut_k || cut_p) && !m.only_largest) {
+        // ---- 2. entries per bin ----
+        walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
+            int k;
+            float r;
+            if (m.exponent(x, k, r)) atomicAdd(&s.bins[m.bin(k)], 1u);
+        });
+        __syncthreads();
+        int count[kPerThread], n = 0;
+        float mass = 0.0f;                               // of the thread's bins, by their centres
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            const int bin = tid * kPerThread + i;
+            count[i] = (int)s.bins[bin];
+            n += count[i];
+            mass += (float)count[i] * exp2f((float)-bin * (1.0f / 256.0f));
         }
-    }
-    if (top_p < 1.0f) {
-        auto above = [&](uint32_t key, bool equal) {     // mass of the entries above a key
-            double sum = 0.0;
-            for (int64_t i = tid; i < vocab; i += kThreads) {
-                const float x = entry(row, (int)i);
-                const uint32_t k = ordered_key(x);
-                if (k > key || (equal && k == key)) sum += mass(x);
+        int n_upto = n;
+        float m_upto = mass;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, n_upto, o);
+            const float y = __shfl_up_sync(0xffffffffu, m_upto, o);
+            if (lane >= o) { n_upto += x; m_upto += y; }
+        }
+        if (lane == 31) { s.count[warp] = n_upto; s.part[warp] = m_upto; }
+        if (tid == kThreads - 1) s.tail = (float)count[kPerThread - 1] * exp2f(-(kBins - 1) / 256.0f);        // (anything down to nothing)
+        __syncthreads();
+        float all = 0.0f, all_most = 0.0f;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) { n_upto += s.count[w]; m_upto += s.part[w]; }
+            all += s.part[w];
+        }
+        if (cut_k) {
+            int upto = n_upto - n;
+            float above = m_upto - mass;
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const float w = exp2f((float)-(tid * kPerThread + i) * (1.0f / 256.0f));
+                if (upto < top_k && upto + count[i] >= top_k) { s.bin_k = tid * kPerThread + i; s.need = top_k - upto; s.mass_k[0] = above + (float)(top_k - upto) * w; s.mass_k[1] = above + (float)count[i] * w; }
+                upto += count[i];
+                above += (float)count[i] * w;
             }
-            return block_sum(sum, sum_s);
-        };
-        const double most = (double)top_p * above(cut, true);
-        uint32_t c = 0u;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t probe = c + ((1u << bit) - 1u);
-            if (!(above(probe, false) < most)) c += 1u << bit;
+            __syncthreads();
         }
-        cut = max(cut, min(c, top));
+        // what the top-k cut leaves: ties with the k-th stay, up to the whole of its bin (fewer than top_k
+        // entries with a mass: no cut)
+        all_most = s.bin_k < kBins ? s.mass_k[1] : all;
+        if (s.bin_k < kBins) all = s.mass_k[0];
+        const int bin_k = s.bin_k;
+        if (cut_p) {
+            // mass above an entry of a bin: between that above the bin and that up to its end; a float's
+            // worth of doubt on sums of thousands of terms is inside the slack
+            const float lo = top_p * (all - s.tail) * (1.0f - kSlack), hi = top_p * all_most * (1.0f + kSlack);
+            float above = m_upto - mass;
+#pragma unroll
+            for (int i = 0; i < kPerThread; ++i) {
+                const int bin = tid * kPerThread + i;
+                const float upto = above + (float)count[i] * exp2f((float)-bin * (1.0f / 256.0f));
+                if (count[i] > 0 && bin <= bin_k) {
+                    const bool stays = upto * (1.0f + kSlack) < lo && bin < kBins - 1, goes = above * (1.0f - kSlack) >= hi;
+                    if (!stays && !goes) { atomicMin(&s.zone_lo, bin); atomicMax(&s.zone_hi, bin); }
+                }
+                above = upto;
+            }
+        }
+        __syncthreads();
+        const int zone_lo = s.zone_lo, zone_hi = s.zone_hi;
+        // ---- 3. exact masses ----
+        Sum in, over;                                    // bins before bin_k; of those, before the zone
+        walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
+            int k;
+            float r;
+            if (!m.exponent(x, k, r)) return;
+            const int bin = m.bin(k);
+            if (bin > bin_k) return;
+            const bool at_k = bin == bin_k, at_p = bin >= zone_lo && bin <= zone_hi;
+            if (at_k) { const int j = atomicAdd(&s.n_k, 1); if (j < kListK) s.list_k[j] = ordered_key(x); }
+            if (!cut_p) return;
+            double h;
+            float l;
+            m.get(x, h, l);
+            if (!at_k) in.add(h, l);
+            if (at_p) { const int j = atomicAdd(&s.n_p, 1); if (j < kListP) { s.list_p[j] = ordered_key(x); s.mass_p[j] = units(h + (double)l); } }
+            else if (bin < zone_lo) over.add(h, l);
+        });
+        __syncthreads();
+        const int n_k = s.n_k, n_p = s.n_p;
+        if (cut_k && bin_k < kBins) {
+            // the need-th largest of the list, or the top_k-th of the row
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t probe = cut | (1u << bit);
+                int c1 = 0;
+                if (n_k <= kListK) {
+                    for (int i = tid; i < n_k; i += kThreads) c1 += s.list_k[i] >= probe;
+                } else {
+                    walk(row, 0, vocab, tid, kThreads, [&](float x, int) { c1 += ordered_key(x) >= probe; });
+                }
+                if (block_count(c1, s.count) >= (n_k <= kListK ? s.need : top_k)) cut = probe;
+            }
+        }
+        if (cut_p) {
+            // the whole mass: bins before bin_k and what of that bin stays
+            unsigned long long rest = 0;
+            if (bin_k < kBins) {
+                if (n_k <= kListK) {
+                    for (int i = tid; i < n_k; i += kThreads)
+                        if (s.list_k[i] >= cut) { double h; float l; m.get(key_to_float(s.list_k[i]), h, l); rest += units(h + (double)l); }
+                } else {
+                    walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
+                        int k;
+                        float r;
+                        if (m.exponent(x, k, r) && m.bin(k) == bin_k && ordered_key(x) >= cut) { double h; float l; m.get(x, h, l); rest += units(h + (double)l); }
+                    });
+                }
+            }
+            const double most = (double)top_p * (block_sum(in.value(), s.sum) + (double)block_sum(rest, s.sum_u) / kUnit);
+            const double over_sum = block_sum(over.value(), s.sum);
+            // least key above which there is less than `most` (some bin is always open)
+            uint32_t key = 0u;
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t probe = key + ((1u << bit) - 1u);
+                unsigned long long x = 0;
+                if (n_p <= kListP) {
+                    for (int i = tid; i < n_p; i += kThreads) x += s.list_p[i] > probe && s.list_p[i] >= cut ? s.mass_p[i] : 0ull;
+                } else {
+                    walk(row, 0, vocab, tid, kThreads, [&](float v, int) {
+                        int k;
+                        float r;
+                        const uint32_t q = ordered_key(v);
+                        if (q > probe && q >= cut && m.exponent(v, k, r)) {
+                            const int bin = m.bin(k);
+                            if (bin >= zone_lo && bin <= zone_hi) { double h; float l; m.get(v, h, l); x += units(h + (double)l); }
+                        }
+                    });
+                }
+                if (!(over_sum + (double)block_sum(x, s.sum_u) / kUnit < most)) key += 1u << bit;
+            }
+            cut = max(cut, min(key, top));
+        }
     }
-    auto kept = [&](float x) {
-        const double m = ordered_key(x) >= cut ? mass(x) : 0.0;
-        return m >= (double)min_p || x == largest ? m : 0.0;
+    // ---- 4. the draw ----
+    auto kept = [&](float x, double& h, float& l) {
+        if (ordered_key(x) < cut || !m.get(x, h, l)) return false;
+        return x == largest || !(min_p > 0.0f) || h + (double)l >= (double)min_p;
     };
-    // the draw: a thread sums a run of neighbouring entries
-    const int64_t per = ((int64_t)vocab + kThreads - 1) / kThreads, lo = tid * per, hi = lo + per < vocab ? lo + per : vocab;
-    double mine = 0.0;
-    for (int64_t i = lo; i < hi; ++i) mine += kept(entry(row, (int)i));
-    double upto = mine;
+    // sum of the entries [lo, hi) by this warp
+    auto run_sum = [&](int lo, int hi) {
+        Sum x;
+        walk(row, lo, hi, lane, 32, [&](float v, int) {
+            double h;
+            float l;
+            if (kept(v, h, l)) x.add(h, l);
+        });
+        return warp_sum(x.value());
+    };
+    int lo = 0, hi = vocab;
+    double before = 0.0, target = 0.0;
+    for (int level = 0; level < 2; ++level) {
+        // the run of 32 that the sum passes the target in; the last with a mass where roundings leave none
+        const int per = (hi - lo + kWarps - 1) / kWarps;
+        const int a = min(lo + warp * per, hi), z = min(a + per, hi);
+        const double sum = run_sum(a, z);
+        __syncthreads();
+        if (lane == 0) s.sum[warp] = sum;
+        __syncthreads();
+        double upto = s.sum[lane];
+        const bool some = upto > 0.0;
 #pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const double x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-    }
-    __syncthreads();
-    if (lane == 31) sum_s[warp] = upto;
-    if (tid == 0) { pick_s = 0x7fffffff; int_s[0] = -1; }
-    __syncthreads();
-    double before = 0.0, all = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) { if (w < warp) before += sum_s[w]; all += sum_s[w]; }
-    const double target = (double)u * all;
-    before += upto - mine;
-    if (mine > 0.0) {
-        double sum = before;
-        int last = -1;
-        for (int64_t i = lo; i < hi; ++i) {
-            const double m = kept(entry(row, (int)i));
-            if (m > 0.0) last = (int)i;
-            sum += m;
-            if (m > 0.0 && sum > target) { atomicMin(&pick_s, (int)i); break; }
+        for (int o = 1; o < 32; o *= 2) {
+            const double x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
         }
-        atomicMax(&int_s[0], last);                      // (a number that is no less than one takes the last kept entry)
+        if (level == 0) target = (double)u * __shfl_sync(0xffffffffu, upto, 31);
+        const unsigned passes = __ballot_sync(0xffffffffu, some && before + upto > target), holds = __ballot_sync(0xffffffffu, some);
+        const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
+        const double to_w = __shfl_sync(0xffffffffu, upto, w), of_w = s.sum[w];
+        before += to_w - of_w;
+        lo = min(lo + w * per, hi);
+        hi = min(lo + per, hi);
     }
-    __syncthreads();
-    if (tid == 0) ids[b] = pick_s != 0x7fffffff ? pick_s : int_s[0];
+    if (warp == 0) {
+        int pick = -1, last = -1;
+        for (int i0 = lo; i0 < hi && pick < 0; i0 += 32) {
+            const int i = i0 + lane;
+            double h = 0.0;
+            float l = 0.0f;
+            const bool stays = i < hi && kept((float)row[i], h, l);
+            double upto = stays ? h + (double)l : 0.0;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const double x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned passes = __ballot_sync(0xffffffffu, stays && before + upto > target), holds = __ballot_sync(0xffffffffu, stays);
+            if (passes) pick = i0 + __ffs(passes) - 1;
+            if (holds) last = i0 + 31 - __clz(holds);
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) ids[b] = pick >= 0 ? pick : last;
+    }
 }
 
 }  // namespace
@@ -167,13 +448,15 @@ extern "C" int kivi_sample_filtered(const void* logits, int dtype, int batch, in
     KIVI_REQUIRE(logits != nullptr && uniforms != nullptr && ids_out != nullptr, "logits, uniforms or ids_out is null");
     KIVI_REQUIRE(dtype == KIVI_F32 || dtype == KIVI_BF16, "logits dtype must be KIVI_F32 or KIVI_BF16");
     KIVI_REQUIRE(batch > 0 && vocab > 0 && row_stride >= vocab, "batch (%d), vocab (%d) and row_stride must be positive, row_stride >= vocab", batch, vocab);
+    // (indices step past the end of a row)
+    KIVI_REQUIRE(vocab <= (1 << 30), "vocab (%d) must be at most 2^30", vocab);
     const FilterArgs f{uniforms, temperature, top_p, min_p, top_k};
-    if (dtype == KIVI_BF16)
-        KIVI_CUDA_OK(launch(sample_filtered_kernel<__nv_bfloat16>, dim3((unsigned)batch), kThreads, 0, (cudaStream_t)stream, true,
-                            reinterpret_cast<const __nv_bfloat16*>(logits), vocab, row_stride, f, ids_out));
-    else
-        KIVI_CUDA_OK(launch(sample_filtered_kernel<float>, dim3((unsigned)batch), kThreads, 0, (cudaStream_t)stream, true,
-                            reinterpret_cast<const float*>(logits), vocab, row_stride, f, ids_out));
-    note_launches(1);
-    return KIVI_OK;
+    auto go = [&](auto* kernel, auto* x) {
+        KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+        KIVI_CUDA_OK(launch(kernel, dim3((unsigned)batch), kThreads, sizeof(Shared), (cudaStream_t)stream, true, x, vocab, row_stride, f, ids_out));
+        note_launches(1);
+        return KIVI_OK;
+    };
+    return dtype == KIVI_BF16 ? go(sample_filtered_kernel<__nv_bfloat16>, reinterpret_cast<const __nv_bfloat16*>(logits))
+                              : go(sample_filtered_kernel<float>, reinterpret_cast<const float*>(logits));
 }

@@ -1,0 +1,175 @@
+"""Sampling under temperature, top-k, top-p and min-p against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from intel_kivi_hybrid_b200.extension.loader import kivi_native
+    return kivi_native
+
+
+def row_state(x, t, k, p, mp):
+    """Kept masses of one row (fp64, CPU): the definition word by word."""
+    x = x.double()
+    x = torch.where(x.isnan(), torch.full_like(x, -math.inf), x)
+    top = x.max()
+    if top == -math.inf:
+        return None
+    m = (x == top).double() if top == math.inf else torch.exp((x - top) / t)
+    stay = torch.ones_like(m, dtype=torch.bool)
+    if 0 < k < x.numel():
+        stay &= x >= x.sort(descending=True).values[k - 1]
+    in_k = torch.where(stay, m, torch.zeros_like(m))
+    if p < 1:
+        values, where = x.unique(return_inverse=True)               # ascending; ties share a value
+        per = torch.zeros(values.numel(), dtype=torch.float64).index_add_(0, where, in_k)
+        above = (per.sum() - per.cumsum(0)).clamp(min=0)
+        # sums from the top, so that what is above the largest is exactly nothing
+        above = torch.cat([per.flip(0).cumsum(0).flip(0)[1:], torch.zeros(1, dtype=torch.float64)])
+        stay &= (above < p * in_k.sum())[where] | (x == top)
+    if mp > 0:
+        stay &= (m >= mp) | (x == top)
+    return torch.where(stay, m, torch.zeros_like(m))
+
+
+def check(ops, logits, u, t=None, k=None, p=None, mp=None, cpu=None):
+    """Every id is the definition's, or the draw is within the sums' error (1e-9 of the mass, as documented) of a boundary."""
+    B, V = logits.shape
+    dev = lambda v, d: None if v is None else torch.tensor(v, dtype=d, device="cuda")  # noqa: E731
+    ids = ops.sample_filtered(logits, dev(u, torch.float32), dev(t, torch.float32), dev(k, torch.int32), dev(p, torch.float32), dev(mp, torch.float32))
+    again = ops.sample_filtered(logits, dev(u, torch.float32), dev(t, torch.float32), dev(k, torch.int32), dev(p, torch.float32), dev(mp, torch.float32))
+    assert torch.equal(ids, again)
+    x = logits.float().cpu()
+    f32 = lambda v: float(torch.tensor(v, dtype=torch.float32))  # noqa: E731
+    for b in range(B):
+        temp = f32(t[b]) if t is not None else 1.0
+        got = int(ids[b])
+        row = torch.where(x[b].isnan(), torch.full_like(x[b], -math.inf), x[b])
+        if temp <= 0 or row.max() == -math.inf:
+            assert got == (0 if row.max() == -math.inf else int((row == row.max()).nonzero()[0]))
+            continue
+        m = row_state(x[b], temp, k[b] if k is not None else 0, f32(p[b]) if p is not None else 1.0, f32(mp[b]) if mp is not None else 0.0)
+        cdf = m.cumsum(0)
+        target = f32(u[b]) * float(cdf[-1])
+        assert m[got] > 0, (b, got)
+        slack = 2e-9 * float(cdf[-1])
+        before = float(cdf[got - 1]) if got else 0.0
+        assert before <= target + slack and (float(cdf[got]) > target - slack or f32(u[b]) >= 1.0), (b, got, before, target, float(cdf[got]))
+
+
+def uniforms(B, seed):
+    return torch.rand(B, generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 2, 3, 31, 33, 1000, 4097, 50257, 131072])
+def test_filters_alone_and_together(ops, dtype, V):
+    B = 12
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = (3 * torch.randn(B, V, generator=g, device="cuda")).to(dtype)
+    u = uniforms(B, V)
+    t = [0.5 + 0.1 * i for i in range(B)]
+    k = [0, 1, 2, 5, 50, 300, 1000, V - 1, V, V + 5, 40, 7]
+    p = [1.0, 0.0, 0.1, 0.5, 0.9, 0.95, 0.99, 0.999, 1.5, 0.7, 0.3, 0.8]
+    mp = [0.0, 1.0, 0.5, 0.1, 0.05, 0.01, 0.001, -1.0, 0.2, 0.3, 0.02, 0.0]
+    check(ops, logits, u)
+    check(ops, logits, u, t)
+    check(ops, logits, u, t, k=k)
+    check(ops, logits, u, t, p=p)
+    check(ops, logits, u, t, mp=mp)
+    check(ops, logits, u, t, k, p, mp)
+    check(ops, logits, u, None, k[::-1], p, None)
+
+
+def test_strided_rows_and_odd_offsets(ops):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for dtype in (torch.float32, torch.bfloat16):
+        big = (2 * torch.randn(9, 7013, generator=g, device="cuda")).to(dtype)
+        for view in (big[:, 3:6001], big[::2, 1:], big[1:2, 5:77]):
+            B = view.shape[0]
+            check(ops, view, uniforms(B, 3), [0.9] * B, [100] * B, [0.8] * B, [0.01] * B)
+
+
+def test_ties_runs_and_equal_rows(ops):
+    """Equal logits stay together; lists at a cut that do not fit; rows of one value."""
+    B, V = 10, 30000
+    x = torch.zeros(B, V, device="cuda")
+    x[1] = 2.5
+    x[2, ::2] = 1.0
+    x[3, :5000] = 1.0
+    x[4, 100:7000] = 3.0
+    x[5, 29999] = 9.0
+    x[6] = torch.arange(V, device="cuda") % 7 - 3.0
+    x[7, 1:] = -3.0e38
+    x[8] = torch.linspace(-5, 5, V, device="cuda")
+    x[9] = (torch.arange(V, device="cuda") % 3 == 0).float() * 1e-3
+    for seed in range(3):
+        u = uniforms(B, seed)
+        check(ops, x, u, [0.7] * B, [3000] * B, [0.6] * B)
+        check(ops, x, u, [1.3] * B, None, [0.9] * B, [0.02] * B)
+        check(ops, x, u, [1.0] * B, [15000] * B)
+        check(ops, x.bfloat16(), u, [1.0] * B, [100] * B, [0.5] * B)
+
+
+def test_infinities_nan_and_the_lowest_value(ops):
+    V = 2000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(12, V, generator=g, device="cuda")
+    inf, nan = math.inf, math.nan
+    x[0] = -inf
+    x[1] = nan
+    x[2, :] = -inf
+    x[2, 1234] = -5.0
+    x[3, 50] = inf
+    x[4, [7, 900, 1500]] = inf
+    x[5, ::3] = nan
+    x[6, ::2] = -inf
+    x[7, 5:] = torch.finfo(torch.float32).min
+    x[8] = torch.finfo(torch.float32).min
+    x[9, 0] = torch.finfo(torch.float32).max
+    x[10] = torch.where(torch.arange(V, device="cuda") % 2 == 0, 3e38, -3e38)
+    x[11, :] = nan
+    x[11, 1999] = -inf
+    for args in ({}, {"t": [0.5] * 12}, {"t": [1e-35] * 12}, {"t": [0.0] * 12}, {"t": [-1.0] * 12}, {"t": [0.8] * 12, "k": [10] * 12, "p": [0.9] * 12, "mp": [0.1] * 12},
+                 {"t": [50.0] * 12, "p": [0.5] * 12}, {"t": [3e38] * 12, "k": [1500] * 12}):
+        check(ops, x, uniforms(12, 9), **args)
+
+
+def test_the_ends_of_the_unit_interval(ops):
+    x = torch.randn(6, 5000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))
+    u = [0.0, 1.0 - 2.0 ** -24, 2.0 ** -24, 0.5, 0.999, 1e-30]
+    check(ops, x, u, [0.9] * 6, None, [0.7] * 6)
+    check(ops, x, u)
+
+
+def test_ids_follow_the_distribution(ops):
+    """20000 draws of one row: counts within six standard deviations of the kept masses."""
+    V, n = 50, 20000
+    x = torch.randn(V, generator=torch.Generator().manual_seed(3))
+    m = row_state(x, 0.8, 30, 0.95, 0.02)
+    want = m / m.sum()
+    ids = ops.sample_filtered(x.cuda().expand(n, V).contiguous(), torch.rand(n, generator=torch.Generator().manual_seed(4)).cuda(), torch.full((n,), 0.8, device="cuda"),
+                              torch.full((n,), 30, dtype=torch.int32, device="cuda"), torch.full((n,), 0.95, device="cuda"), torch.full((n,), 0.02, device="cuda"))
+    got = torch.bincount(ids.cpu(), minlength=V).double()
+    assert ((got - n * want).abs() <= 6 * (n * want * (1 - want)).sqrt() + 1e-9).all()
+
+
+def test_refusals(ops):
+    x, u = torch.randn(4, 100, device="cuda"), torch.rand(4, device="cuda")
+    one = torch.ones(4, device="cuda")
+    for bad, what in ((lambda: ops.sample_filtered(x[0], u), "logits must be"), (lambda: ops.sample_filtered(x[:, ::2], u), "side by side"),
+                      (lambda: ops.sample_filtered(x.half(), u), "Float or BFloat16"), (lambda: ops.sample_filtered(x.cpu(), u), "on cuda"),
+                      (lambda: ops.sample_filtered(x, u[:3]), "uniforms must hold"), (lambda: ops.sample_filtered(x, u.double()), "uniforms must be"),
+                      (lambda: ops.sample_filtered(x, u.cpu()), "same device"), (lambda: ops.sample_filtered(x, u, one, one), "top_k must be"),
+                      (lambda: ops.sample_filtered(x, u, one[:2]), "temperature must hold"), (lambda: ops.sample_filtered(x, u, None, None, one.int()), "top_p must be"),
+                      (lambda: ops.sample_filtered(x, u, None, None, None, one.half()), "min_p must be"),
+                      (lambda: ops.sample_filtered(x, u, out=torch.zeros(4, dtype=torch.int32, device="cuda")), "out must be"),
+                      (lambda: ops.sample_filtered(x.as_strided((4, 100), (50, 1)), u), "overlap"), (lambda: ops.sample_filtered(x[:, :0], u), "vocab")):
+        with pytest.raises(RuntimeError, match=what):
+            bad()
+    assert ops.sample_filtered(x[:0], u[:0]).shape == (0,)
