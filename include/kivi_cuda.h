@@ -502,7 +502,7 @@ int kivi_paged_read(const kivi_paged_layer* layer, const kivi_paged_batch* batch
  * and the id is the first index at which the sum of the kept m_i exceeds uniform * (all of
  * it).  temperature <= 0: the argmax, lowest index first.  NaN logits count as -inf, of
  * infinite ones each has mass 1 and no other any; a row without a number above -inf gives 0.
- * Sums are in fp64, relative error of a mass below 1e-9: a draw differs from the one in
+ * Sums are in fp64, relative error of a mass below 2e-9: a draw differs from the one in
  * real arithmetic only within that of a boundary.
  * logits: device [batch][row_stride >= vocab] of dtype.  uniforms: device fp32 [batch] in
  * [0, 1).  temperature, top_p, min_p: device fp32 [batch], top_k: device int32 [batch]; NULL

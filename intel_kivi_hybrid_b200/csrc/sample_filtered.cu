@@ -8,17 +8,18 @@
 //      the bin that the k-th largest is in, and bound the mass above any bin to 0.15 %, which
 //      leaves a few bins that the nucleus can end in;
 //   3. exact masses: all of them, those above the open bins, and a list of the entries in
-//      the open bins, on which both cuts are then found by bisection (keys of the list, so that
-//      ties stay together);
+//      the open bins, on which both cuts are then found, 32 keys at a time (a warp each; keys, so
+//      that ties stay together);
 //   4. sums of the kept masses over runs of the row, and the run, piece and entry at which
 //      the sum passes uniform * all.
-// Lists that do not fit (thousands of equal logits at a cut) are replaced by bisection over
-// the row.  Lists come in any order: what is summed over them are whole numbers (2^-50 of
-// the largest mass), so that the same inputs give the same id.
+// Where a list does not fit (thousands of equal logits at a cut, as bf16 has them) the row is
+// walked again, up to four times, each of which cuts the open keys into 256 ranges.  Lists
+// come in any order and ranges add by atomics: what is summed there are whole numbers (2^-46
+// of the largest mass at 50257 entries), so that the same inputs give the same id.
 //
-// Masses: 2^(k/256) from a table in fp64 and a correction below 2^-9 of it in fp32; the
-// exponent (x - max) log2(e) 256 / T is a product of two-term fp32 numbers, good to 1e-10.
-// fp64 takes one addition per entry.
+// Masses: 2^(k/32) from a table in fp64 and a correction below 2^-6 of it in fp32 (good to
+// 2^-29 of the mass); the exponent (x - max) log2(e) 32 / T is a product of two-term fp32 numbers,
+// good to 1e-10.  fp64 takes one addition per entry.
 // Bound by latency: 4 walks of 2-3 us, 13 barriers.
 #include "kivi_common.cuh"
 
@@ -31,10 +32,10 @@ constexpr int kPerThread = kBins / kThreads;
 constexpr int kListK = 2048, kListP = 4096;              // entries at the k-th largest, at the end of the nucleus
 constexpr float kSlack = 0.0016f;                        // 2^(0.5/256) - 1 and roundings: how far a bin's mass is off its centre's
 
-// order-preserving map float -> uint32; NaN counts as -inf
+// order-preserving map float -> uint32; NaN counts as -inf, the zeros are one
 __device__ __forceinline__ uint32_t ordered_key(float x) {
     if (x != x) x = -INFINITY;
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float key_to_float(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
@@ -47,11 +48,13 @@ struct FilterArgs {
 struct Shared {
     uint32_t bins[kBins];
     uint32_t list_k[kListK], list_p[kListP];
-    unsigned long long mass_p[kListP];                   // in units of 2^-50
-    double exp_table[256];
-    float exp_table_f[256];
+    unsigned long long mass_p[kListP];                   // in whole units
+    struct { double d; float f, pad; } table[32];        // 2^(i/32)
     double sum[kWarps];
     unsigned long long sum_u[kWarps];
+    unsigned long long range[256], open_base;
+    uint32_t flag[2][kWarps];
+    uint32_t open_lo, open_hi;
     float part[kWarps];
     int count[kWarps];
     uint32_t key[kWarps];
@@ -84,16 +87,6 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long x, un
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
-constexpr double kUnit = 1125899906842624.0;             // 2^50
-__device__ __forceinline__ unsigned long long units(double mass) { return (unsigned long long)__double2ll_rn(mass * kUnit); }
-__device__ __forceinline__ int block_count(int x, int* s) {
-    x = __reduce_add_sync(0xffffffffu, x);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, s[threadIdx.x & 31]);
-}
-
 // The entries of an aligned 16 bytes
 template <typename T> struct Granule;
 template <> struct Granule<float> {
@@ -140,43 +133,38 @@ __device__ __forceinline__ void walk(const T* row, int lo, int hi, int me, int n
 
 // Masses relative to the row's largest entry.
 struct Masses {
-    float largest, c_hi, c_lo;                           // 256 log2(e) / T in two terms
+    float largest, c_hi, c_lo;                           // 32 log2(e) / T in two terms
     bool only_largest;                                   // an infinite largest, or a temperature that leaves nothing else
-    const double* table;
-    const float* table_f;
+    const Shared* s;
 
-    // exponent in 1/256 octaves, whole and rest; false: no mass at all
-    __device__ __forceinline__ bool exponent(float x, int& k, float& rest) const {
+    // mass = hi + lo; false: none
+    __device__ __forceinline__ bool get(float x, double& hi, float& lo) const {
+        hi = 0.0; lo = 0.0f;
+        if (only_largest) {
+            if (x == largest) hi = 1.0;
+            return x == largest;
+        }
         const float d = __fsub_rn(x, largest);
         const float p = __fmul_rn(d, c_hi);
-        if (!(p > -250000.0f)) return false;             // below 2^-976, -inf or NaN
+        if (!(p > -31000.0f)) return false;              // below 2^-968, -inf or NaN
         // d = x - largest to the last bit: what the subtraction rounded away
         const float b = __fsub_rn(x, d), lost = __fadd_rn(__fsub_rn(x, __fadd_rn(d, b)), __fsub_rn(b, largest));
         const float whole = rintf(p);
-        k = (int)whole;
-        rest = __fsub_rn(p, whole) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi)));
-        return true;
-    }
-    // mass = hi + lo
-    __device__ __forceinline__ bool get(float x, double& hi, float& lo) const {
-        int k;
-        float r;
-        if (only_largest) {
-            hi = x == largest ? 1.0 : 0.0; lo = 0.0f;
-            return x == largest;
-        }
-        if (!exponent(x, k, r)) { hi = 0.0; lo = 0.0f; return false; }
-        const int n = k >> 8;
-        const double t = table[k & 255];
-        hi = __hiloint2double(__double2hiint(t) + (n << 20), __double2loint(t));
-        const float u = r * 0.0027076061740622863f;      // ln 2 / 256
-        const float e = u * fmaf(u, fmaf(u, 0.16666667f, 0.5f), 1.0f);       // 2^(r/256) - 1 to u^4 / 24 = 1e-13
+        const int k = (int)whole, n = k >> 5;
+        const float r = __fsub_rn(p, whole) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi)));
+        const auto t = s->table[k & 31];
+        hi = __hiloint2double(__double2hiint(t.d) + (n << 20), __double2loint(t.d));
+        const float u = r * 0.02166084939249829f;        // ln 2 / 32
+        const float e = u * fmaf(u, fmaf(u, fmaf(u, 0.041666667f, 0.16666667f), 0.5f), 1.0f);       // 2^(r/32) - 1 to u^5 / 120 = 1e-12
         // (a mass below 2^-120 needs no correction)
-        lo = n > -120 ? e * __uint_as_float(__float_as_uint(table_f[k & 255]) + (uint32_t)(n * (1 << 23))) : 0.0f;
+        lo = n > -120 ? e * __uint_as_float(__float_as_uint(t.f) + (uint32_t)(n * (1 << 23))) : 0.0f;
         return true;
     }
-    // bin of an entry with mass
-    __device__ __forceinline__ int bin(int k) const { return -k < kBins - 1 ? (-k > 0 ? -k : 0) : kBins - 1; }
+    // bin of an entry, falling with it; -1 for one that can have no mass (-inf, NaN)
+    __device__ __forceinline__ int bin(float x) const {
+        const float p = __fmul_rn(__fmul_rn(__fsub_rn(largest, x), c_hi), 8.0f);
+        return p < (float)(kBins - 1) ? (int)rintf(p) : x > -INFINITY ? kBins - 1 : -1;
+    }
 };
 
 // sums of two terms, folded once at the end
@@ -193,10 +181,10 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
-    if (tid < 256) {
-        const double t = exp2((double)tid * (1.0 / 256.0));
-        s.exp_table[tid] = t;
-        s.exp_table_f[tid] = (float)t;
+    if (tid < 32) {
+        const double t = exp2((double)tid * (1.0 / 32.0));
+        s.table[tid].d = t;
+        s.table[tid].f = (float)t;
     }
     if (tid == 0) { s.first = 0x7fffffff; s.bin_k = kBins; s.need = 0; s.zone_lo = kBins; s.zone_hi = -1; s.n_k = 0; s.n_p = 0; s.pick = 0x7fffffff; s.last = -1; }
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0u;
@@ -205,6 +193,9 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     const float u = settled(f.uniforms)[b], temperature = f.temperature ? settled(f.temperature)[b] : 1.0f;
     const float top_p = f.top_p ? settled(f.top_p)[b] : 1.0f, min_p = f.min_p ? settled(f.min_p)[b] : 0.0f;
     const int top_k = f.top_k ? settled(f.top_k)[b] : 0;
+    // whole units of mass: a row's sum stays below 2^62
+    const double unit = (double)(1ll << (__clz(vocab) + 30 < 50 ? __clz(vocab) + 30 : 50));
+    auto units = [&](double mass) { return (unsigned long long)__double2ll_rn(mass * unit); };
     const bool cut_k = top_k > 0 && top_k < vocab, cut_p = top_p < 1.0f;
 
     // ---- 1. the largest and its first index ----
@@ -226,20 +217,18 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     }
     Masses m;
     m.largest = largest;
-    const double c = 256.0 * 1.4426950408889634 / (double)temperature;
+    const double c = 32.0 * 1.4426950408889634 / (double)temperature;
     m.c_hi = (float)c;
     m.c_lo = (float)(c - (double)m.c_hi);
     m.only_largest = largest == INFINITY || temperature < 1e-30f;
-    m.table = s.exp_table;
-    m.table_f = s.exp_table_f;
+    m.s = &s;
 
     uint32_t cut = 0u;                                   // least key that is kept
     if ((cut_k || cut_p) && !m.only_largest) {
         // ---- 2. entries per bin ----
         walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
-            int k;
-            float r;
-            if (m.exponent(x, k, r)) atomicAdd(&s.bins[m.bin(k)], 1u);
+            const int bin = m.bin(x);
+            if (bin >= 0) atomicAdd(&s.bins[bin], 1u);
         });
         __syncthreads();
         int count[kPerThread], n = 0;
@@ -305,11 +294,8 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         // ---- 3. exact masses ----
         Sum in, over;                                    // bins before bin_k; of those, before the zone
         walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
-            int k;
-            float r;
-            if (!m.exponent(x, k, r)) return;
-            const int bin = m.bin(k);
-            if (bin > bin_k) return;
+            const int bin = m.bin(x);
+            if (bin < 0 || bin > bin_k) return;
             const bool at_k = bin == bin_k, at_p = bin >= zone_lo && bin <= zone_hi;
             if (at_k) { const int j = atomicAdd(&s.n_k, 1); if (j < kListK) s.list_k[j] = ordered_key(x); }
             if (!cut_p) return;
@@ -322,62 +308,124 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         });
         __syncthreads();
         const int n_k = s.n_k, n_p = s.n_p;
-        if (cut_k && bin_k < kBins) {
-            // the need-th largest of the list, or the top_k-th of the row
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t probe = cut | (1u << bit);
-                int c1 = 0;
-                if (n_k <= kListK) {
-                    for (int i = tid; i < n_k; i += kThreads) c1 += s.list_k[i] >= probe;
-                } else {
-                    walk(row, 0, vocab, tid, kThreads, [&](float x, int) { c1 += ordered_key(x) >= probe; });
+        // The largest key for which holds(key), asked of whole warps, is true; it falls from true to
+        // false between lo and hi (0 if it is nowhere true).  32 keys at a time.
+        auto search = [&](uint32_t lo, uint32_t hi, auto&& holds) {
+            uint32_t found = 0u;
+            int buf = 0;
+            for (int shift = hi > lo ? (31 - __clz(hi - lo)) / 5 * 5 : 0; shift >= 0; shift -= 5, buf ^= 1) {
+                const uint32_t off = (uint32_t)warp << shift;
+                const bool yes = (off >> shift) == (uint32_t)warp && off <= hi - lo && holds(lo + off);
+                if (lane == 0) s.flag[buf][warp] = yes;
+                __syncthreads();
+                const unsigned all_yes = __ballot_sync(0xffffffffu, s.flag[buf][lane] != 0u);
+                if (!all_yes) return found;
+                found = lo + ((uint32_t)(31 - __clz(all_yes)) << shift);
+                lo = found;
+                hi = min(hi, lo + ((1u << shift) - 1u));
+            }
+            return found;
+        };
+        auto ends = [&](const uint32_t* list, int n, uint32_t& lo, uint32_t& hi) {
+            lo = 0xffffffffu; hi = 0u;
+            for (int i = lane; i < n; i += 32) { lo = min(lo, list[i]); hi = max(hi, list[i]); }
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_max_sync(0xffffffffu, hi);
+        };
+        // The same over the row: amount(x, key) of the keys in lo .. hi, 256 ranges of keys at a time;
+        // the largest key at which what is at or above it reaches `most` (in the amount's units).
+        auto search_row = [&](uint32_t lo, uint32_t hi, unsigned long long most, auto&& amount) {
+            if (tid == 0) { s.open_lo = lo; s.open_hi = hi; s.open_base = 0; }
+            for (;;) {
+                __syncthreads();
+                lo = s.open_lo; hi = s.open_hi;
+                if (tid < 256) s.range[tid] = 0;
+                __syncthreads();
+                const int bits = 32 - __clz(hi - lo), shift = hi > lo && bits > 8 ? bits - 8 : 0;
+                walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
+                    const uint32_t key = ordered_key(x);
+                    if (key < lo || key > hi) return;
+                    const unsigned long long a = amount(x);
+                    if (a) atomicAdd(&s.range[(key - lo) >> shift], a);
+                });
+                __syncthreads();
+                if (tid == 0) {
+                    unsigned long long upto = s.open_base;
+                    int i = 255;
+                    for (; i >= 0; --i) {
+                        if (upto + s.range[i] >= most) break;
+                        upto += s.range[i];
+                    }
+                    s.open_base = upto;
+                    if (i < 0) { s.open_lo = 1u; s.open_hi = 0u; }               // nowhere
+                    else { s.open_lo = lo + ((uint32_t)i << shift); s.open_hi = min(hi, s.open_lo + ((1u << shift) - 1u)); }
                 }
-                if (block_count(c1, s.count) >= (n_k <= kListK ? s.need : top_k)) cut = probe;
+                __syncthreads();
+                if (s.open_lo > s.open_hi) return 0u;
+                if (shift == 0) return s.open_lo;
+            }
+        };
+        if (cut_k && bin_k < kBins) {
+            if (n_k <= kListK) {
+                uint32_t lo, hi;
+                ends(s.list_k, n_k, lo, hi);
+                const int need = s.need;
+                cut = search(lo, hi, [&](uint32_t key) {
+                    int c1 = 0;
+                    for (int i = lane; i < n_k; i += 32) c1 += s.list_k[i] >= key;
+                    return __reduce_add_sync(0xffffffffu, c1) >= need;
+                });
+            } else {
+                cut = search_row(0u, 0xffffffffu, (unsigned long long)top_k, [&](float) { return 1ull; });
             }
         }
         if (cut_p) {
             // the whole mass: bins before bin_k and what of that bin stays
             unsigned long long rest = 0;
+            auto add_rest = [&](float x) { double h; float l; m.get(x, h, l); rest += units(h + (double)l); };
             if (bin_k < kBins) {
                 if (n_k <= kListK) {
                     for (int i = tid; i < n_k; i += kThreads)
-                        if (s.list_k[i] >= cut) { double h; float l; m.get(key_to_float(s.list_k[i]), h, l); rest += units(h + (double)l); }
+                        if (s.list_k[i] >= cut) add_rest(key_to_float(s.list_k[i]));
                 } else {
-                    walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
-                        int k;
-                        float r;
-                        if (m.exponent(x, k, r) && m.bin(k) == bin_k && ordered_key(x) >= cut) { double h; float l; m.get(x, h, l); rest += units(h + (double)l); }
-                    });
+                    walk(row, 0, vocab, tid, kThreads, [&](float x, int) { if (m.bin(x) == bin_k && ordered_key(x) >= cut) add_rest(x); });
                 }
             }
-            const double most = (double)top_p * (block_sum(in.value(), s.sum) + (double)block_sum(rest, s.sum_u) / kUnit);
-            const double over_sum = block_sum(over.value(), s.sum);
-            // least key above which there is less than `most` (some bin is always open)
-            uint32_t key = 0u;
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t probe = key + ((1u << bit) - 1u);
-                unsigned long long x = 0;
+            double most = (double)top_p * (block_sum(in.value(), s.sum) + (double)block_sum(rest, s.sum_u) / unit);
+            // (the least key above which there is less than top_p is the largest one at or above which there is no less)
+            most = (most - block_sum(over.value(), s.sum)) * unit;
+            uint32_t key = top;                          // (top_p <= 0: the largest alone)
+            if (most > 0.0) {
+                const unsigned long long most_u = (unsigned long long)__double2ll_ru(most);
                 if (n_p <= kListP) {
-                    for (int i = tid; i < n_p; i += kThreads) x += s.list_p[i] > probe && s.list_p[i] >= cut ? s.mass_p[i] : 0ull;
+                    uint32_t lo, hi;
+                    ends(s.list_p, n_p, lo, hi);
+                    lo = max(lo, cut);                   // (the list may hold what the top-k cut took)
+                    key = lo > hi ? 0u : search(lo, hi, [&](uint32_t probe) {
+                        unsigned long long x = 0;
+                        for (int i = lane; i < n_p; i += 32) x += s.list_p[i] >= probe ? s.mass_p[i] : 0ull;
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+                        return x >= most_u;
+                    });
                 } else {
-                    walk(row, 0, vocab, tid, kThreads, [&](float v, int) {
-                        int k;
-                        float r;
-                        const uint32_t q = ordered_key(v);
-                        if (q > probe && q >= cut && m.exponent(v, k, r)) {
-                            const int bin = m.bin(k);
-                            if (bin >= zone_lo && bin <= zone_hi) { double h; float l; m.get(v, h, l); x += units(h + (double)l); }
-                        }
+                    key = search_row(max(cut, 1u), top, most_u, [&](float x) {
+                        const int bin = m.bin(x);
+                        if (bin < zone_lo || bin > zone_hi) return 0ull;
+                        double h;
+                        float l;
+                        m.get(x, h, l);
+                        return units(h + (double)l);
                     });
                 }
-                if (!(over_sum + (double)block_sum(x, s.sum_u) / kUnit < most)) key += 1u << bit;
             }
             cut = max(cut, min(key, top));
         }
     }
     // ---- 4. the draw ----
+    const float cut_x = cut ? key_to_float(cut) : -INFINITY;
     auto kept = [&](float x, double& h, float& l) {
-        if (ordered_key(x) < cut || !m.get(x, h, l)) return false;
+        if (!(x >= cut_x) || !m.get(x, h, l)) return false;
         return x == largest || !(min_p > 0.0f) || h + (double)l >= (double)min_p;
     };
     // sum of the entries [lo, hi) by this warp
