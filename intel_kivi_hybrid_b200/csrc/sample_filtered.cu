@@ -27,6 +27,7 @@ namespace kivi {
 namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
+static_assert(kWarps == 32, "a warp looks after 32 warps' results, and fills a row of the table");
 constexpr int kBins = 8192;                              // of 1/256 octave; the last holds what is below 2^-32
 constexpr int kPerThread = kBins / kThreads;
 constexpr int kListK = 2048, kListP = 4096;              // entries at the k-th largest, at the end of the nucleus
@@ -49,12 +50,12 @@ struct Shared {
     uint32_t bins[kBins];
     uint32_t list_k[kListK], list_p[kListP];
     unsigned long long mass_p[kListP];                   // in whole units
-    struct { double d; float f, pad; } table[32];        // 2^(i/32)
+    uint32_t table_hi[32][32], table_lo[32][32];         // words of 2^(i/32), a column for each lane: no two lanes meet in a bank
     double sum[kWarps];
-    unsigned long long sum_u[kWarps];
     unsigned long long range[256], open_base;
     uint32_t flag[2][kWarps];
     uint32_t open_lo, open_hi;
+    int draw_lo, draw_hi;
     float part[kWarps];
     int count[kWarps];
     uint32_t key[kWarps];
@@ -68,25 +69,24 @@ __device__ __forceinline__ double warp_sum(double x) {
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
-// sums over the block, the same bits in every thread
-__device__ __forceinline__ double block_sum(double x, double* s) {
-    x = warp_sum(x);
+// Sums over the block of three numbers of each thread, through 24 KB of shared memory: three
+// warps add them up (32 warps that shuffle share one pipe: 2500 cycles for a sum).
+__device__ __forceinline__ void block_sums(double a, double b, double c, double* scratch, double* out) {
+    scratch[threadIdx.x] = a;
+    scratch[kThreads + threadIdx.x] = b;
+    scratch[2 * kThreads + threadIdx.x] = c;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    return warp_sum(s[threadIdx.x & 31]);
-}
-__device__ __forceinline__ unsigned long long block_sum(unsigned long long x, unsigned long long* s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < 3) {
+        double x[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        for (int i = 0; i < kThreads / 32; ++i) x[i & 3] += scratch[warp * kThreads + 32 * i + lane];
+        const double sum = warp_sum((x[0] + x[1]) + (x[2] + x[3]));
+        if (lane == 0) out[warp] = sum;
+    }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = s[threadIdx.x & 31];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
 }
+
 // The entries of an aligned 16 bytes
 template <typename T> struct Granule;
 template <> struct Granule<float> {
@@ -149,21 +149,21 @@ struct Masses {
         if (!(p > -31000.0f)) return false;              // below 2^-968, -inf or NaN
         // d = x - largest to the last bit: what the subtraction rounded away
         const float b = __fsub_rn(x, d), lost = __fadd_rn(__fsub_rn(x, __fadd_rn(d, b)), __fsub_rn(b, largest));
-        const float whole = rintf(p);
-        const int k = (int)whole, n = k >> 5;
+        const float t = __fadd_rn(p, 12582912.0f), whole = __fsub_rn(t, 12582912.0f);        // (1.5 * 2^23: rounds to a whole number)
+        const int k = __float_as_int(t) - 0x4b400000, n = k >> 5;
         const float r = __fsub_rn(p, whole) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi)));
-        const auto t = s->table[k & 31];
-        hi = __hiloint2double(__double2hiint(t.d) + (n << 20), __double2loint(t.d));
+        const uint32_t w1 = s->table_hi[k & 31][threadIdx.x & 31], w0 = s->table_lo[k & 31][threadIdx.x & 31];
+        hi = __hiloint2double((int)w1 + (n << 20), (int)w0);
         const float u = r * 0.02166084939249829f;        // ln 2 / 32
         const float e = u * fmaf(u, fmaf(u, fmaf(u, 0.041666667f, 0.16666667f), 0.5f), 1.0f);       // 2^(r/32) - 1 to u^5 / 120 = 1e-12
         // (a mass below 2^-120 needs no correction)
-        lo = n > -120 ? e * __uint_as_float(__float_as_uint(t.f) + (uint32_t)(n * (1 << 23))) : 0.0f;
+        lo = n > -120 ? e * __uint_as_float(((__funnelshift_l(w0, w1, 3) & 0x7fffffu) | 0x3f800000u) + (uint32_t)(n * (1 << 23))) : 0.0f;
         return true;
     }
     // bin of an entry, falling with it; -1 for one that can have no mass (-inf, NaN)
     __device__ __forceinline__ int bin(float x) const {
         const float p = __fmul_rn(__fmul_rn(__fsub_rn(largest, x), c_hi), 8.0f);
-        return p < (float)(kBins - 1) ? (int)rintf(p) : x > -INFINITY ? kBins - 1 : -1;
+        return p < (float)(kBins - 1) ? __float_as_int(__fadd_rn(p, 12582912.0f)) - 0x4b400000 : x > -INFINITY ? kBins - 1 : -1;
     }
 };
 
@@ -181,10 +181,10 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
-    if (tid < 32) {
-        const double t = exp2((double)tid * (1.0 / 32.0));
-        s.table[tid].d = t;
-        s.table[tid].f = (float)t;
+    {
+        const double t = exp2((double)warp * (1.0 / 32.0));
+        s.table_hi[warp][lane] = (uint32_t)__double2hiint(t);
+        s.table_lo[warp][lane] = (uint32_t)__double2loint(t);
     }
     if (tid == 0) { s.first = 0x7fffffff; s.bin_k = kBins; s.need = 0; s.zone_lo = kBins; s.zone_hi = -1; s.n_k = 0; s.n_p = 0; s.pick = 0x7fffffff; s.last = -1; }
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0u;
@@ -381,8 +381,9 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         }
         if (cut_p) {
             // the whole mass: bins before bin_k and what of that bin stays
-            unsigned long long rest = 0;
-            auto add_rest = [&](float x) { double h; float l; m.get(x, h, l); rest += units(h + (double)l); };
+            // (whole units below 2^53 of the list: exact in any order)
+            double rest = 0.0;
+            auto add_rest = [&](float x) { double h; float l; m.get(x, h, l); rest += (double)units(h + (double)l); };
             if (bin_k < kBins) {
                 if (n_k <= kListK) {
                     for (int i = tid; i < n_k; i += kThreads)
@@ -391,9 +392,11 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                     walk(row, 0, vocab, tid, kThreads, [&](float x, int) { if (m.bin(x) == bin_k && ordered_key(x) >= cut) add_rest(x); });
                 }
             }
-            double most = (double)top_p * (block_sum(in.value(), s.sum) + (double)block_sum(rest, s.sum_u) / unit);
+            __syncthreads();
+            block_sums(in.value(), over.value(), rest, reinterpret_cast<double*>(s.bins), s.sum);
+            double most = (double)top_p * (s.sum[0] + s.sum[2] / unit);
             // (the least key above which there is less than top_p is the largest one at or above which there is no less)
-            most = (most - block_sum(over.value(), s.sum)) * unit;
+            most = (most - s.sum[1]) * unit;
             uint32_t key = top;                          // (top_p <= 0: the largest alone)
             if (most > 0.0) {
                 const unsigned long long most_u = (unsigned long long)__double2ll_ru(most);
@@ -404,9 +407,10 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                     key = lo > hi ? 0u : search(lo, hi, [&](uint32_t probe) {
                         unsigned long long x = 0;
                         for (int i = lane; i < n_p; i += 32) x += s.list_p[i] >= probe ? s.mass_p[i] : 0ull;
-#pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-                        return x >= most_u;
+                        // (21 bits at a time: reductions of 32-bit numbers)
+                        const unsigned long long a = __reduce_add_sync(0xffffffffu, (uint32_t)x & 0x1fffffu), b = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 21) & 0x1fffffu),
+                                                 c = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 42));
+                        return a + (b << 21) + (c << 42) >= most_u;
                     });
                 } else {
                     key = search_row(max(cut, 1u), top, most_u, [&](float x) {
@@ -448,20 +452,23 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         __syncthreads();
         if (lane == 0) s.sum[warp] = sum;
         __syncthreads();
-        double upto = s.sum[lane];
-        const bool some = upto > 0.0;
+        if (warp == 0) {
+            double upto = s.sum[lane];
+            const bool some = upto > 0.0;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const double x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
+            for (int o = 1; o < 32; o *= 2) {
+                const double x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            if (level == 0) target = (double)u * __shfl_sync(0xffffffffu, upto, 31);
+            const unsigned passes = __ballot_sync(0xffffffffu, some && before + upto > target), holds = __ballot_sync(0xffffffffu, some);
+            const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
+            before += __shfl_sync(0xffffffffu, upto, w) - s.sum[w];
+            if (lane == 0) { s.draw_lo = min(lo + w * per, hi); s.draw_hi = min(min(lo + w * per, hi) + per, hi); }
         }
-        if (level == 0) target = (double)u * __shfl_sync(0xffffffffu, upto, 31);
-        const unsigned passes = __ballot_sync(0xffffffffu, some && before + upto > target), holds = __ballot_sync(0xffffffffu, some);
-        const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
-        const double to_w = __shfl_sync(0xffffffffu, upto, w), of_w = s.sum[w];
-        before += to_w - of_w;
-        lo = min(lo + w * per, hi);
-        hi = min(lo + per, hi);
+        __syncthreads();
+        lo = s.draw_lo;
+        hi = s.draw_hi;
     }
     if (warp == 0) {
         int pick = -1, last = -1;
