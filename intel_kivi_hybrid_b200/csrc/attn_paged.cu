@@ -14,6 +14,8 @@
 #include "paged_common.cuh"
 #include "paged_attention.cuh"
 
+#include <type_traits>
+
 namespace kivi {
 namespace {
 
@@ -173,28 +175,32 @@ paged_attention_kernel(PagedAttnArgs A) {
             }
         }
         __syncwarp();
+        // (a token that a row does not see may hold anything, infinities and NaN too: only among the step's own)
+        auto weigh = [&](auto masked) {
 #pragma unroll 2
-        for (int j = 0; j < kTile; j += 4) {
-            float4 p[RPT];
+            for (int j = 0; j < kTile; j += 4) {
+                float4 p[RPT];
 #pragma unroll
-            for (int i = 0; i < RPT; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (ty * RPT + i) * (kTile + 4) + j);
+                for (int i = 0; i < RPT; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (ty * RPT + i) * (kTile + 4) + j);
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj)
+                for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const int d = 4 * tx + 64 * c;
-                    if (DT == 256 && d >= D) break;
-                    if (DT == 64 || d < D) {
+                    for (int c = 0; c < NC; ++c) {
+                        const int d = 4 * tx + 64 * c;
+                        if (DT == 256 && d >= D) break;
                         const float4 v = *reinterpret_cast<const float4*>(v_s + (j + jj) * S + d);
 #pragma unroll
                         for (int i = 0; i < RPT; ++i) {
                             const float w = jj == 0 ? p[i].x : jj == 1 ? p[i].y : jj == 2 ? p[i].z : p[i].w;
-                            o[i][4 * c] = fmaf(w, v.x, o[i][4 * c]); o[i][4 * c + 1] = fmaf(w, v.y, o[i][4 * c + 1]);
-                            o[i][4 * c + 2] = fmaf(w, v.z, o[i][4 * c + 2]); o[i][4 * c + 3] = fmaf(w, v.w, o[i][4 * c + 3]);
+                            const bool seen = !decltype(masked)::value || t0 + j + jj <= last[i];
+                            o[i][4 * c] = fmaf(w, seen ? v.x : 0.0f, o[i][4 * c]); o[i][4 * c + 1] = fmaf(w, seen ? v.y : 0.0f, o[i][4 * c + 1]);
+                            o[i][4 * c + 2] = fmaf(w, seen ? v.z : 0.0f, o[i][4 * c + 2]); o[i][4 * c + 3] = fmaf(w, seen ? v.w : 0.0f, o[i][4 * c + 3]);
                         }
                     }
-                }
-        }
+            }
+        };
+        if (t0 + kTile > q.held) weigh(std::true_type{});
+        else weigh(std::false_type{});
         __syncwarp();
     }
     const int64_t unit = (int64_t)blockIdx.x * H + h;
@@ -295,16 +301,28 @@ int paged_attention_fault_clear() {
 bool paged_tc_serves(const kivi_paged_layer* L, int q_dtype);
 int run_paged_tc(const PagedAttnArgs& a, int blocks, cudaStream_t st);
 
+bool paged_decode_serves(const kivi_paged_layer* L, int q_dtype, int64_t max_rows);
+void paged_decode_plan(const kivi_paged_layer* L, const kivi_paged_batch* b, int n_rep, int* blocks_per_seq, int* gps, int* pieces);
+int run_paged_decode(const PagedAttnArgs& a, int blocks_per_seq, int gps, cudaStream_t st);
+
 // ---- the cut of a call -----------------------------------------------------------
 // Rows per block, blocks (at most: what the host knows are bounds) and pieces of the
 // sequences' tokens.
-struct PagedPlan { bool tc; int rows, blocks, pieces, chunk; };
+enum class PagedKernel { kDecode, kTensor, kGeneral };
+struct PagedPlan { PagedKernel kernel; int rows, blocks, pieces, chunk; };          // (decode: chunk is groups of tokens, blocks a sequence's times sequences)
 
-static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep) {
+static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, bool vec) {
     PagedPlan p;
     const int64_t rows = (int64_t)b->max_new * n_rep;
-    p.tc = paged_tc_serves(L, q_dtype);
-    if (p.tc) {
+    if (vec && paged_decode_serves(L, q_dtype, rows)) {
+        p.kernel = PagedKernel::kDecode;
+        p.rows = 4;
+        paged_decode_plan(L, b, n_rep, &p.blocks, &p.chunk, &p.pieces);
+        p.blocks *= b->num_seqs;
+        return p;
+    }
+    p.kernel = paged_tc_serves(L, q_dtype) ? PagedKernel::kTensor : PagedKernel::kGeneral;
+    if (p.kernel == PagedKernel::kTensor) {
         p.rows = 256;
         const int64_t blocks = (int64_t)b->total_new * n_rep / p.rows + b->num_seqs;
         p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
@@ -349,10 +367,15 @@ static int check_attention(const kivi_paged_layer* L, const kivi_paged_batch* b,
     return KIVI_OK;
 }
 
+static size_t plan_bytes(const kivi_paged_layer* L, const PagedPlan& p) {
+    return p.pieces > 1 || p.kernel == PagedKernel::kDecode ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
+}
+
+// (enough for rows on 16-byte boundaries, and for others, which the decode kernel does not take)
 extern "C" size_t kivi_paged_attention_workspace(const kivi_paged_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep) {
     if (check_attention(L, b, q_dtype, n_rep) != KIVI_OK || b->max_new == 0) return 0;
-    const PagedPlan p = plan_paged(L, b, q_dtype, n_rep);
-    return p.pieces > 1 ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
+    const size_t on = plan_bytes(L, plan_paged(L, b, q_dtype, n_rep, true)), off = plan_bytes(L, plan_paged(L, b, q_dtype, n_rep, false));
+    return on > off ? on : off;
 }
 
 extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_batch* b, const kivi_rows* q,
@@ -367,8 +390,14 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     }
     if (b->max_new == 0) { note_launches(0); return KIVI_OK; }
     const int D = L->head_dim;
-    const PagedPlan p = plan_paged(L, b, q_dtype, n_rep);
-    const size_t need = kivi_paged_attention_workspace(L, b, q_dtype, n_rep);
+    // rows on 16-byte boundaries
+    auto aligned = [](const kivi_rows& r, int dtype) {
+        const int n = 16 / elem_size(dtype);
+        return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
+    };
+    const bool vec16 = aligned(*q, q_dtype) && aligned(*new_k, L->res_dtype) && aligned(*new_v, L->res_dtype);
+    const PagedPlan p = plan_paged(L, b, q_dtype, n_rep, vec16);
+    const size_t need = plan_bytes(L, p);
     KIVI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
     KIVI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
     if (sm_scale <= 0.0f) sm_scale = 1.0f / sqrtf((float)D);
@@ -385,9 +414,13 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     cudaStream_t st = (cudaStream_t)stream;
     const size_t smem = ((size_t)(p.rows + 2 * kTile) * (D + 4) + (size_t)p.rows * (kTile + 4)) * 4;
     int rc;
-    if (p.tc) {
-        auto grid8 = [](const kivi_rows& r) { return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.row_stride % 8 == 0 && r.head_stride % 8 == 0; };
-        a.vec = grid8(*q) && grid8(*new_k) && grid8(*new_v);
+    if (p.kernel == PagedKernel::kDecode) {
+        if (int rc2 = run_paged_decode(a, p.blocks / b->num_seqs, p.chunk, st)) return rc2;
+        note_launches(2);
+        return KIVI_OK;
+    }
+    if (p.kernel == PagedKernel::kTensor) {
+        a.vec = vec16;
         rc = run_paged_tc(a, p.blocks, st);
     } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);

@@ -74,6 +74,8 @@ int paged_attention_fault_word(int* out);
 int paged_attention_fault_clear();
 int paged_tc_fault_word(int* out);
 int paged_tc_fault_clear();
+int paged_decode_fault_word(int* out);
+int paged_decode_fault_clear();
 int run_merge(const float* part_o, const float* part_ml, void* out, const kivi_peer_gather* gather, float* lse,
               int out_dtype, int num_units, int n_rep, int n_splits, int D, cudaStream_t st);
 
@@ -91,11 +93,12 @@ extern "C" int kivi_device_fault(int* word_out) {
     if (int rc = fp32_fault_word(&copy_wait_fp32)) return rc;
     if (int rc = sample_fault_word(&copy_wait_sample)) return rc;
     if (int rc = gather_fault_word(&peer_wait)) return rc;
-    int paged_cache = 0, paged_attention = 0, paged_tc = 0;
+    int paged_cache = 0, paged_attention = 0, paged_tc = 0, paged_decode = 0;
     if (int rc = paged_cache_fault_word(&paged_cache)) return rc;
     if (int rc = paged_attention_fault_word(&paged_attention)) return rc;
     if (int rc = paged_tc_fault_word(&paged_tc)) return rc;
-    *word_out = (copy_wait || copy_wait_fp32 || copy_wait_sample ? 1 : 0) | (peer_wait ? 2 : 0) | paged_cache | paged_attention | paged_tc;
+    if (int rc = paged_decode_fault_word(&paged_decode)) return rc;
+    *word_out = (copy_wait || copy_wait_fp32 || copy_wait_sample ? 1 : 0) | (peer_wait ? 2 : 0) | paged_cache | paged_attention | paged_tc | paged_decode;
     return KIVI_OK;
 }
 
@@ -106,6 +109,7 @@ extern "C" int kivi_device_fault_clear(void) {
     if (int rc = paged_cache_fault_clear()) return rc;
     if (int rc = paged_attention_fault_clear()) return rc;
     if (int rc = paged_tc_fault_clear()) return rc;
+    if (int rc = paged_decode_fault_clear()) return rc;
     return gather_fault_clear();
 }
 
