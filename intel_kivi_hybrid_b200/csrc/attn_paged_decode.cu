@@ -334,32 +334,44 @@ paged_decode_kernel(PagedAttnArgs A, int blocks_per_seq, int gps) {
     }
 }
 
-// grid = (row blocks of all sequences, KV heads), a thread per quad of channels of a row
-__global__ void __launch_bounds__(kRows * kD / 4)
+// grid = (row blocks of all sequences, KV heads); 128 threads have a quad of channels of a
+// row each, with many pieces several such teams share them.
+constexpr int kTeam = kRows * kD / 4;
+__global__ void __launch_bounds__(8 * kTeam)
 paged_decode_merge_kernel(PagedAttnArgs A, int blocks_per_seq, int gps) {
+    __shared__ float4 out_s[7][kTeam];
+    __shared__ float2 ml_s[7][kTeam];
     stream_order();
     settle_args(A);
     const kivi_paged_layer& L = A.L;
-    const int n_rep = A.n_rep, h = blockIdx.y;
+    const int n_rep = A.n_rep, h = blockIdx.y, team = threadIdx.x / kTeam, teams = blockDim.x / kTeam, me = threadIdx.x % kTeam;
     const int s = (int)blockIdx.x / blocks_per_seq, row_first = ((int)blockIdx.x - s * blocks_per_seq) * kRows;
     PagedSeq q;
     load_seq(L, A.b, s, q);
-    const int r = threadIdx.x >> 5, d = (threadIdx.x & 31) * 4, row = row_first + r;
-    if (row >= q.n * n_rep) return;
-    const int n_groups = min(quant_of(q.held + q.n, kG, L.residual_cap), q.held) / kG, n = 1 + (n_groups + gps - 1) / gps;
+    if (row_first >= q.n * n_rep) return;
+    const int r = me >> 5, d = (me & 31) * 4, row = row_first + r;
+    const int n_groups = min(quant_of(q.held + q.n, kG, L.residual_cap), q.held) / kG;
+    const int n = row < q.n * n_rep ? 1 + (n_groups + gps - 1) / gps : 0;
     const int64_t base = ((int64_t)blockIdx.x * L.num_kv_heads + h) * A.pieces;
-    float M = -INFINITY;
-    for (int p = 0; p < n; ++p) M = fmaxf(M, A.part_ml[2 * ((base + p) * kRows + r)]);
-    float sum = 0.0f;
+    float M = -INFINITY, sum = 0.0f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 v) {
+        if (ml.x == -INFINITY) return;
+        const float top = fmaxf(M, ml.x), w0 = ex2(M - top), w1 = ex2(ml.x - top);
+        M = top;
+        sum = fmaf(w0, sum, w1 * ml.y);
+        a.x = fmaf(w0, a.x, w1 * v.x); a.y = fmaf(w0, a.y, w1 * v.y); a.z = fmaf(w0, a.z, w1 * v.z); a.w = fmaf(w0, a.w, w1 * v.w);
+    };
 #pragma unroll 4
-    for (int p = 0; p < n; ++p) {
-        const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * ((base + p) * kRows + r));
-        const float4 v = *reinterpret_cast<const float4*>(A.part_o + ((base + p) * kRows + r) * kD + d);
-        const float w = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-        sum = fmaf(w, ml.y, sum);
-        a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y); a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
+    for (int p = team; p < n; p += teams)
+        add(*reinterpret_cast<const float2*>(A.part_ml + 2 * ((base + p) * kRows + r)), *reinterpret_cast<const float4*>(A.part_o + ((base + p) * kRows + r) * kD + d));
+    if (teams > 1) {
+        if (team) { out_s[team - 1][me] = a; ml_s[team - 1][me] = make_float2(M, sum); }
+        __syncthreads();
+        if (team) return;
+        for (int t = 0; t < teams - 1; ++t) add(ml_s[t][me], out_s[t][me]);
     }
+    if (n == 0) return;
     const float inv = 1.0f / sum;
     const int64_t at = ((int64_t)q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
     store_quad(A.out.data, A.out_dtype, at + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
@@ -371,22 +383,32 @@ static_assert(kWarps * kStages * kStageBytes >= 2 * kG * kD * 4, "the window's C
 }  // namespace
 
 bool paged_decode_serves(const kivi_paged_layer* L, int q_dtype, int64_t max_rows) {
+    // Three blocks of rows: 16 sequences x 4k, 4 query heads, 3 tokens 86 us here, 97 with 256 rows on the
+    // tensor cores; 4 tokens 106 and 98; 1 x 32k 2 tokens 64 and 59.
     // (bf16 windows with fp32 queries and the other way round go to the general kernel)
-    return L->head_dim == kD && L->group_size == kG && q_dtype == L->res_dtype && max_rows <= 16;
+    return L->head_dim == kD && L->group_size == kG && q_dtype == L->res_dtype && max_rows <= 12;
 }
 
-// Row blocks of a sequence, packed groups a piece and pieces: six rounds of CTAs on the GPU
-// (sequences shorter than the longest leave theirs unused), whole rounds of the CTA's warps.
+// Row blocks of a sequence, packed groups a piece and pieces, in whole rounds of the CTA's
+// warps (eight groups, 1.4 us).  Rounds of CTAs on the GPU times rounds of a piece, two more
+// for a CTA's start and end, and what a piece costs in the fold; but no piece above a sixth
+// of a GPU's share where that is long, since sequences shorter than the longest leave theirs
+// unused (64 ragged sequences up to 32k: 285 us with a sixth, one piece each 420).
 void paged_decode_plan(const kivi_paged_layer* L, const kivi_paged_batch* b, int n_rep, int* blocks_per_seq, int* gps, int* pieces) {
+    constexpr int kRound = kWarps * kGPS;
     *blocks_per_seq = (b->max_new * n_rep + kRows - 1) / kRows;
     const int64_t groups = quant_of(b->max_len, kG, L->residual_cap) / kG, units = (int64_t)b->num_seqs * *blocks_per_seq * L->num_kv_heads;
-    const int64_t slots = 3 * (int64_t)num_sms();
-    int64_t per = (units * groups + 6 * slots - 1) / (6 * slots);
-    const int64_t one_round = (units * groups + slots - 1) / slots;               // (few tokens: one round of CTAs)
-    if (one_round <= 2 * kWarps * kGPS) per = one_round;
-    per = (per + kWarps * kGPS - 1) / (kWarps * kGPS) * (kWarps * kGPS);
-    if (per < kWarps * kGPS) per = kWarps * kGPS;
-    while ((groups + per - 1) / per > 255) per += kWarps * kGPS;
+    const int64_t slots = 3 * (int64_t)num_sms(), share = (units * groups + slots - 1) / slots;
+    const int64_t longest = share / 6 > 96 ? share / 6 : 96;
+    double best = 1e30;
+    int64_t per = kRound;
+    for (int64_t k = 1; k * kRound < longest + kRound && k <= 4096; ++k) {
+        const int64_t n = (groups + k * kRound - 1) / (k * kRound);
+        if (n > 255 && k < 4096) continue;
+        const double cost = (double)((units * n + slots - 1) / slots) * (double)(k + 2) + 0.05 * (double)n;
+        if (cost < best) { best = cost; per = k * kRound; }
+    }
+    while ((groups + per - 1) / per > 255) per += kRound;
     *gps = (int)per;
     *pieces = 1 + (int)((groups + per - 1) / per);
 }
@@ -397,7 +419,8 @@ int run_paged_decode(const PagedAttnArgs& a, int blocks_per_seq, int gps, cudaSt
     KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes));
     const dim3 grid((unsigned)(a.b.num_seqs * blocks_per_seq), (unsigned)a.L.num_kv_heads, (unsigned)a.pieces);
     KIVI_CUDA_OK(launch(kernel, grid, kWarps * 32, kSmemBytes, st, true, a, blocks_per_seq, gps));
-    KIVI_CUDA_OK(launch(paged_decode_merge_kernel, dim3(grid.x, grid.y), kRows * kD / 4, 0, st, true, a, blocks_per_seq, gps));
+    const int teams = a.pieces > 32 ? 8 : a.pieces > 8 ? 4 : 1;
+    KIVI_CUDA_OK(launch(paged_decode_merge_kernel, dim3(grid.x, grid.y), (unsigned)(kTeam * teams), 0, st, true, a, blocks_per_seq, gps));
     return KIVI_OK;
 }
 
