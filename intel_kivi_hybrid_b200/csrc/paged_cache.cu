@@ -2,15 +2,19 @@
 //
 // One launch per append.  A sequence's new tokens are dealt out to CTAs so that nothing
 // is ordered between them:
-//   * one CTA per (sequence, KV head) takes the groups that start in the window, then
-//     writes what stays to the window -- a slot it overwrites is one of a token it has
-//     moved out before, so the order holds inside the CTA;
+//   * one CTA per KV head and group that starts in the window (one at least) quantizes it.
+//     Then it writes to the window those tokens that stay and whose slots its own tokens had,
+//     so that a slot is overwritten by the CTA that has read it; what stays and meets no token
+//     that leaves is dealt out in turn;
 //   * one CTA per whole group of new tokens and KV head quantizes that group.
-// Every CTA also turns the rows it has (keys, and the queries of its KV head), so the
-// step's tensors are read once.
+// Every CTA also turns the keys it has and, in steps of a few tokens, the queries of its KV
+// head; in longer steps the queries are a streaming kernel of their own (in the same CTAs
+// they took 160 registers: 4 x 2048 tokens 189 us, DT_SPLIT us apart).
 //
 // Bound by memory: bf16, D = 128, G = 32 moves 2.1 bytes per element of the rows in and
 // out and 0.5 per flushed element; the smallest call (one token) is launch and latency.
+// A thread takes two 16-byte vectors of a token and everything that shares their angles -- the
+// key, the value, the query heads -- so that some ten loads are in flight.
 #include "paged_common.cuh"
 
 namespace kivi {
@@ -23,90 +27,56 @@ struct Rotary {
     int dim, interleaved;
 };
 
-template <typename T> struct Quad;
-template <> struct Quad<float> {
-    __device__ static void load(const float* p, float (&x)[4], bool vec) {
-        if (vec) { const float4 v = *reinterpret_cast<const float4*>(p); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-        else { x[0] = p[0]; x[1] = p[1]; x[2] = p[2]; x[3] = p[3]; }
+// N neighbouring channels of a row; VEC: they lie on the grid of such vectors.
+template <typename T, int N, bool VEC> struct Channels;
+template <int N, bool VEC> struct Channels<float, N, VEC> {
+    __device__ static void load(const float* p, float (&x)[N]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) { const float4 v = *reinterpret_cast<const float4*>(p + i); x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w; }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = p[i];
+        }
     }
-    __device__ static void store(float* p, const float (&x)[4], bool vec) {
-        if (vec) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        else { p[0] = x[0]; p[1] = x[1]; p[2] = x[2]; p[3] = x[3]; }
+    __device__ static void store(float* p, const float (&x)[N]) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] = x[i];
+        }
     }
     __device__ static float round(float x) { return x; }
 };
-template <> struct Quad<__nv_bfloat16> {
-    __device__ static void load(const __nv_bfloat16* p, float (&x)[4], bool vec) {
-        if (vec) {
+template <int N, bool VEC> struct Channels<__nv_bfloat16, N, VEC> {
+    __device__ static void widen(uint32_t w, float& a, float& b) { a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u); }
+    __device__ static uint32_t narrow(float a, float b) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    __device__ static void load(const __nv_bfloat16* p, float (&x)[N]) {
+        if constexpr (VEC && N == 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            widen(v.x, x[0], x[1]); widen(v.y, x[2], x[3]); widen(v.z, x[4], x[5]); widen(v.w, x[6], x[7]);
+        } else if constexpr (VEC) {
             const uint2 v = *reinterpret_cast<const uint2*>(p);
-            x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-            x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+            widen(v.x, x[0], x[1]); widen(v.y, x[2], x[3]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+            for (int i = 0; i < N; ++i) x[i] = __bfloat162float(p[i]);
         }
     }
-    __device__ static void store(__nv_bfloat16* p, const float (&x)[4], bool vec) {
-        if (vec) {
-            const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-            *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-        } else {
+    __device__ static void store(__nv_bfloat16* p, const float (&x)[N]) {
+        if constexpr (VEC && N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(narrow(x[0], x[1]), narrow(x[2], x[3]), narrow(x[4], x[5]), narrow(x[6], x[7]));
+        else if constexpr (VEC) *reinterpret_cast<uint2*>(p) = make_uint2(narrow(x[0], x[1]), narrow(x[2], x[3]));
+        else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(x[i]);
+            for (int i = 0; i < N; ++i) p[i] = __float2bfloat16_rn(x[i]);
         }
     }
     __device__ static float round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
-};
-
-// Rows of one head that a CTA turns: `from` and `to` may be the same memory, so a row is
-// turned by one thread per pair of quads that exchange values.
-// A unit of work is 8 channels: quads d and e that hold each other's partners (halves), or
-// two quads of whole pairs (interleaved, or behind the rotated channels).
-template <typename T>
-struct Turn {
-    const Rotary r;
-    const int D;
-    const bool vec;                                      // rows lie on the grid of a quad
-    // unit u of D/8 (the last may hold one quad only where D % 8 == 4)
-    __device__ __forceinline__ bool halves() const { return r.table != nullptr && !r.interleaved && r.dim % 8 == 0; }
-    __device__ __forceinline__ int units() const { return (D + 7) / 8; }
-    __device__ __forceinline__ void places(int u, int& d, int& e) const {
-        const int pairs = halves() ? r.dim / 8 : 0;
-        if (u < pairs) { d = 4 * u; e = 4 * u + r.dim / 2; }
-        else { d = 8 * u; e = 8 * u + 4 < D ? 8 * u + 4 : -1; }
-    }
-    // the unit's values turned to the angles of `angle` (a row of the table) and rounded to T
-    __device__ __forceinline__ void load(const T* row, const float* angle, int d, int e, float (&x)[4], float (&y)[4]) const {
-        Quad<T>::load(row + d, x, vec);
-        if (e >= 0) Quad<T>::load(row + e, y, vec);
-        else { y[0] = y[1] = y[2] = y[3] = 0.0f; }
-        if (r.table == nullptr) return;
-        const int h = r.dim / 2;
-        if (halves()) {
-            if (d < h) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float c = angle[d + i], s = angle[h + d + i], a = x[i], b = y[i];
-                    x[i] = Quad<T>::round(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
-                    y[i] = Quad<T>::round(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)));
-                }
-            }
-            return;
-        }
-        // interleaved (halves of other sizes are refused by the host)
-        turn_pairs(angle, d, x);
-        if (e >= 0) turn_pairs(angle, e, y);
-    }
-    __device__ __forceinline__ void turn_pairs(const float* angle, int d, float (&x)[4]) const {
-        const int h = r.dim / 2;
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            if (d + i >= r.dim) break;
-            const float c = angle[(d + i) / 2], s = angle[h + (d + i) / 2], a = x[i], b = x[i + 1];
-            x[i] = Quad<T>::round(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
-            x[i + 1] = Quad<T>::round(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)));
-        }
-    }
 };
 
 struct AppendArgs {
@@ -114,66 +84,126 @@ struct AppendArgs {
     kivi_paged_batch b;
     kivi_rows k, v, q, q_out, k_out;
     Rotary rotary;
-    int n_rep, vec;
+    int n_rep, items_vary;
 };
 
-template <typename T> __device__ __forceinline__ const T* row_of(const kivi_rows& r, int64_t row, int head) {
-    return reinterpret_cast<const T*>(r.data) + row * r.row_stride + (int64_t)head * r.head_stride;
+template <typename T> __device__ __forceinline__ T* row_of(const kivi_rows& r, int64_t row, int head) {
+    return reinterpret_cast<T*>(r.data) + row * r.row_stride + (int64_t)head * r.head_stride;
 }
 
 constexpr int kThreads = 128;
+template <typename T> constexpr int kPad = 16 / sizeof(T);                // rows of a tile start 16 bytes apart in bank space
 
-// Codes of the tile in shared memory, tile[t][D + 4], to the group's place in a page.
-template <bool HALF_EVEN>
-__device__ __forceinline__ void quantize_keys_tile(const float* tile, uint8_t* block, int D, int G, uint8_t* codes, float* scales, float* zeros) {
-    const int Q = G / 4, W = D < 64 ? D : 64, S = D + 4;
+// Codes of a tile in shared memory, tile[t][D + pad], for the group's place in a page.
+template <typename T, bool HALF_EVEN>
+__device__ __forceinline__ void quantize_keys_tile(const T* tile, uint8_t* block, int D, int G, float* scales, float* zeros) {
+    const int Q = G / 4, W = D < 64 ? D : 64, S = D + kPad<T>;
     for (int d = threadIdx.x; d < D; d += kThreads) {
         float mn = 1e30f, mx = -1e30f;
-        for (int t = 0; t < G; ++t) { const float x = tile[t * S + d]; mn = fminf(mn, x); mx = fmaxf(mx, x); }
+#pragma unroll 8
+        for (int t = 0; t < G; ++t) { const float x = (float)tile[t * S + d]; mn = fminf(mn, x); mx = fmaxf(mx, x); }
         const float scale = group_scale(mn, mx), rcp = group_rcp(scale);
         scales[d] = scale;
         zeros[d] = mn;
+#pragma unroll 2
         for (int j = 0; j < Q; ++j) {
             float m[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m[i] = code_magic<HALF_EVEN>(tile[(4 * j + i) * S + d], mn, scale, rcp);
+            for (int i = 0; i < 4; ++i) m[i] = code_magic<HALF_EVEN>((float)tile[(4 * j + i) * S + d], mn, scale, rcp);
             block[kblock_offset(d, j, Q, W)] = (uint8_t)pack4_magic(m[0], m[1], m[2], m[3]);
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < D * Q / 4; i += kThreads) reinterpret_cast<uint32_t*>(codes)[i] = reinterpret_cast<const uint32_t*>(block)[i];
 }
-template <bool HALF_EVEN>
-__device__ __forceinline__ void quantize_values_tile(const float* tile, uint8_t* block, float* factors, int D, int G, uint8_t* codes, float* scales, float* zeros) {
-    const int S = D + 4, ng = D / G;
+template <typename T, bool HALF_EVEN>
+__device__ __forceinline__ void quantize_values_tile(const T* tile, uint8_t* block, float* factors, int D, int G) {
+    const int S = D + kPad<T>, ng = D / G;
     for (int i = threadIdx.x; i < G * ng; i += kThreads) {
         const int t = i % G, gd = i / G;                 // (tokens on neighbouring threads: rows are four banks apart)
-        const float* x = tile + t * S + gd * G;
+        const T* x = tile + t * S + gd * G;
         float mn = 1e30f, mx = -1e30f;
+#pragma unroll 4
         for (int c = 0; c < G; c += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(x + c);
-            mn = fminf(fminf(mn, v.x), fminf(v.y, fminf(v.z, v.w)));
-            mx = fmaxf(fmaxf(mx, v.x), fmaxf(v.y, fmaxf(v.z, v.w)));
+            float v[4];
+            Channels<T, 4, true>::load(x + c, v);
+            mn = fminf(fminf(mn, v[0]), fminf(v[1], fminf(v[2], v[3])));
+            mx = fmaxf(fmaxf(mx, v[0]), fmaxf(v[1], fmaxf(v[2], v[3])));
         }
         const float scale = group_scale(mn, mx), rcp = group_rcp(scale);
         const int at = (int)vmeta_index(t, gd, D, G);
         factors[at] = scale;
         factors[D + at] = mn;
+#pragma unroll 2
         for (int c = 0; c < G; c += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(x + c);
+            float v[4];
+            Channels<T, 4, true>::load(x + c, v);
             block[vcode_offset(t, (gd * G + c) / 4, D, G)] =
-                (uint8_t)pack4_magic(code_magic<HALF_EVEN>(v.x, mn, scale, rcp), code_magic<HALF_EVEN>(v.y, mn, scale, rcp),
-                                     code_magic<HALF_EVEN>(v.z, mn, scale, rcp), code_magic<HALF_EVEN>(v.w, mn, scale, rcp));
+                (uint8_t)pack4_magic(code_magic<HALF_EVEN>(v[0], mn, scale, rcp), code_magic<HALF_EVEN>(v[1], mn, scale, rcp),
+                                     code_magic<HALF_EVEN>(v[2], mn, scale, rcp), code_magic<HALF_EVEN>(v[3], mn, scale, rcp));
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < D * G / 16; i += kThreads) reinterpret_cast<uint32_t*>(codes)[i] = reinterpret_cast<const uint32_t*>(block)[i];
-    for (int i = threadIdx.x; i < D; i += kThreads) { scales[i] = factors[i]; zeros[i] = factors[D + i]; }
 }
 
-template <typename T, bool HALF_EVEN>
+// The turning of a row, in units of two vectors of N channels.
+template <typename T, int N, bool VEC>
+struct Turn {
+    using C = Channels<T, N, VEC>;
+    const Rotary rot;
+    const int D;
+    struct Angles { float c[N], s[N], c2[N / 2], s2[N / 2]; };
+
+    __device__ __forceinline__ bool halves() const { return rot.table != nullptr && !rot.interleaved; }
+    __device__ __forceinline__ int pairs() const { return halves() ? rot.dim / 2 / N : 0; }
+    __device__ __forceinline__ int units() const { return pairs() + (D - 2 * N * pairs() + 2 * N - 1) / (2 * N); }
+    // vectors d and e (-1: none) of unit u
+    __device__ __forceinline__ void places(int u, int& d, int& e) const {
+        if (u < pairs()) { d = N * u; e = d + rot.dim / 2; }
+        else { d = 2 * N * u; e = d + N < D ? d + N : -1; }
+    }
+    // cosines and sines for the unit's vectors: halves share theirs
+    __device__ __forceinline__ void angles(int t, int u, int d, int e, Angles& a) const {
+        if (rot.table == nullptr) return;
+        const int half = rot.dim / 2;
+        const float* row = rot.table + (int64_t)t * rot.dim;
+        if (halves()) {
+            if (u < pairs()) { Channels<float, N, VEC>::load(row + d, a.c); Channels<float, N, VEC>::load(row + half + d, a.s); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const int p = d / 2 + i, r = e / 2 + i;
+                a.c[i] = p < half ? row[p] : 1.0f; a.s[i] = p < half ? row[half + p] : 0.0f;
+                a.c2[i] = e >= 0 && r < half ? row[r] : 1.0f; a.s2[i] = e >= 0 && r < half ? row[half + r] : 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ static void pair(float c, float s, float& p, float& r) {
+        const float t = p;
+        p = C::round(__fsub_rn(__fmul_rn(t, c), __fmul_rn(r, s)));
+        r = C::round(__fadd_rn(__fmul_rn(r, c), __fmul_rn(t, s)));
+    }
+    __device__ __forceinline__ void turn(int u, int d, int e, const Angles& a, float (&x)[N], float (&y)[N]) const {
+        if (rot.table == nullptr) return;
+        if (halves()) {
+            if (u < pairs()) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) pair(a.c[i], a.s[i], x[i], y[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                if (d + 2 * i < rot.dim) pair(a.c[i], a.s[i], x[2 * i], x[2 * i + 1]);
+                if (e >= 0 && e + 2 * i < rot.dim) pair(a.c2[i], a.s2[i], y[2 * i], y[2 * i + 1]);
+            }
+        }
+    }
+};
+
+// N: channels of a vector (16 bytes, or 4 channels for shapes that those do not divide); a
+// thread has two of them of a token, which hold each other's partners where halves are
+// paired, and all heads of the token that take the same angles.
+template <typename T, int N, bool VEC, bool HALF_EVEN, bool QUERIES>
 __global__ void __launch_bounds__(kThreads)
 paged_append_kernel(AppendArgs A) {
+    using C = Channels<T, N, VEC>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int place_s[2];
     stream_order();
@@ -181,24 +211,31 @@ paged_append_kernel(AppendArgs A) {
     A.k.data = settled(A.k.data); A.v.data = settled(A.v.data); A.q.data = settled(A.q.data);
     A.rotary.table = settled(A.rotary.table);
     const kivi_paged_layer& L = A.L;
-    const int D = L.head_dim, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + 4;
-    float* const tile = reinterpret_cast<float*>(smem);                   // [G][D + 4]
-    float* const factors = tile + G * S;                                  // [2][D]
-    uint8_t* const block = reinterpret_cast<uint8_t*>(factors + 2 * D);   // [D * G / 4]
+    const int D = L.head_dim, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + kPad<T>;
+    T* const k_tile = reinterpret_cast<T*>(smem);                         // [G][D + pad]
+    T* const v_tile = k_tile + G * S;
+    float* const factors = reinterpret_cast<float*>(v_tile + G * S);      // [2][D]
+    uint8_t* const k_block = reinterpret_cast<uint8_t*>(factors + 2 * D); // [D * G / 4]
+    uint8_t* const v_block = k_block + D * G / 4;
     const int h = blockIdx.y;
 
-    // sequence s has one item for its window and one for each whole group of new tokens
+    // sequence s has an item for each group that starts in the window (one at least) and one for
+    // each whole group of new tokens
     auto fresh_groups = [&](const PagedSeq& q) {
         const int first = (q.held + G - 1) / G * G, out = quant_of(q.held + q.n, G, R);
         return out > first ? (out - first) / G : 0;
     };
+    auto window_groups = [&](const PagedSeq& q) {
+        const int first = (q.held + G - 1) / G * G, in = quant_of(q.held, G, R), out = quant_of(q.held + q.n, G, R);
+        return max(1, (min(out, first) - in) / G);
+    };
     int s = blockIdx.x, sub = 0;
-    if (A.b.max_new >= G) {
+    if (A.items_vary) {
         if (threadIdx.x < 32) {
             const ItemPlace p = find_item(blockIdx.x, A.b.num_seqs, [&](int i) {
                 PagedSeq q;
                 load_seq(L, A.b, i, q);
-                return 1 + fresh_groups(q);
+                return window_groups(q) + fresh_groups(q);
             });
             if (threadIdx.x == 0) { place_s[0] = p.s; place_s[1] = p.sub; }
         }
@@ -210,102 +247,175 @@ paged_append_kernel(AppendArgs A) {
     if (!load_seq(L, A.b, s, q)) { if (threadIdx.x == 0) atomicOr(&g_fault, kPagedFault); return; }
     if (q.n == 0) return;
 
-    const Turn<T> plain{{nullptr, 0, 0}, D, A.vec != 0}, turn{A.rotary, D, A.vec != 0};
-    const int units = turn.units();
-    auto angle_of = [&](int t) { return A.rotary.table + (int64_t)t * A.rotary.dim; };
+    const Turn<T, N, VEC> by{A.rotary, D};
+    const int units = by.units();
+    auto load2 = [&](const T* row, int d, int e, float (&x)[N], float (&y)[N]) {
+        C::load(row + d, x);
+        if (e >= 0) C::load(row + e, y);
+        else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = 0.0f;
+        }
+    };
+    auto store2 = [&](T* row, int d, int e, const float (&x)[N], const float (&y)[N]) {
+        C::store(row + d, x);
+        if (e >= 0) C::store(row + e, y);
+    };
+    auto tile2 = [&](T* row, int d, int e, const float (&x)[N], const float (&y)[N]) {
+        Channels<T, N, true>::store(row + d, x);
+        if (e >= 0) Channels<T, N, true>::store(row + e, y);
+    };
     const int64_t ring0 = ((int64_t)q.slot * H + h) * R;
     T* const k_ring = reinterpret_cast<T*>(L.k_res) + ring0 * D;
     T* const v_ring = reinterpret_cast<T*>(L.v_res) + ring0 * D;
-    auto row = [&](int t) { return (int64_t)q.row0 + (t - q.held); };
 
-    // one group of tokens t0 .. t0 + G - 1 to its page; its new tokens come from the step's rows, where `write` turned keys go out too
-    auto flush = [&](int t0, bool write) {
+    // One unit of a new token: turned keys to where `to_tile` / `to_ring` / `out` say, its values
+    // likewise, and (out) the queries of this KV head.
+    auto fresh_unit = [&](int t, int u, T* kt, T* vt, bool to_ring, bool out) {
+        const int64_t row = (int64_t)q.row0 + (t - q.held);
+        int d, e;
+        by.places(u, d, e);
+        typename Turn<T, N, VEC>::Angles a;
+        float x[N], y[N], vx[N], vy[N];
+        by.angles(t, u, d, e, a);
+        load2(row_of<const T>(A.k, row, h), d, e, x, y);
+        if (vt || to_ring) load2(row_of<const T>(A.v, row, h), d, e, vx, vy);
+        by.turn(u, d, e, a, x, y);
+        if (out && A.k_out.data) store2(row_of<T>(A.k_out, row, h), d, e, x, y);
+        if (kt) { tile2(kt, d, e, x, y); tile2(vt, d, e, vx, vy); }
+        if (to_ring) {
+            const int64_t at = (int64_t)ring_slot(t, A.b.ring_shift, R) * D;
+            Channels<T, N, VEC>::store(k_ring + at + d, x); Channels<T, N, VEC>::store(v_ring + at + d, vx);
+            if (e >= 0) { Channels<T, N, VEC>::store(k_ring + at + e, y); Channels<T, N, VEC>::store(v_ring + at + e, vy); }
+        }
+        if (QUERIES && out) {
+            for (int r0 = 0; r0 < A.n_rep; r0 += 4) {                    // four heads in flight
+                float p[4][N], z[4][N];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r0 + r < A.n_rep) load2(row_of<const T>(A.q, row, h * A.n_rep + r0 + r), d, e, p[r], z[r]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r0 + r < A.n_rep) {
+                        by.turn(u, d, e, a, p[r], z[r]);
+                        store2(row_of<T>(A.q_out, row, h * A.n_rep + r0 + r), d, e, p[r], z[r]);
+                    }
+            }
+        }
+    };
+    // the group in the tiles to its page
+    auto flush_tiles = [&](int t0) {
         const int page = q.pages[t0 / L.page_tokens];
         const bool ok = (unsigned)page < (unsigned)L.num_pages;
         if (!ok && threadIdx.x == 0) atomicOr(&g_fault, kPagedFault);
-        const int gpp = L.page_tokens / G;
-        const int64_t g = ((int64_t)(ok ? page : 0) * H + h) * gpp + t0 % L.page_tokens / G;
-        for (int pass = 0; pass < 2; ++pass) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < G * units; i += kThreads) {
-                const int t = t0 + i / units;
-                int d, e;
-                float x[4], y[4];
-                const bool fresh = t >= q.held, keys = pass == 0;
-                const Turn<T>& by = keys && fresh ? turn : plain;
-                turn.places(i % units, d, e);
-                const T* from = fresh ? row_of<T>(keys ? A.k : A.v, row(t), h) : (keys ? k_ring : v_ring) + (int64_t)ring_slot(t, A.b.ring_shift, R) * D;
-                by.load(from, by.r.table ? angle_of(t) : nullptr, d, e, x, y);
-                if (keys && fresh && write && A.k_out.data) {
-                    T* to = const_cast<T*>(row_of<T>(A.k_out, row(t), h));
-                    Quad<T>::store(to + d, x, A.vec);
-                    if (e >= 0) Quad<T>::store(to + e, y, A.vec);
-                }
-                float* const to = tile + (t - t0) * S;
-                *reinterpret_cast<float4*>(to + d) = make_float4(x[0], x[1], x[2], x[3]);
-                if (e >= 0) *reinterpret_cast<float4*>(to + e) = make_float4(y[0], y[1], y[2], y[3]);
-            }
-            __syncthreads();
-            if (!ok) continue;
-            if (pass == 0) quantize_keys_tile<HALF_EVEN>(tile, block, D, G, L.k_codes + g * (D * G / 4), L.k_scales + g * D, L.k_zeros + g * D);
-            else quantize_values_tile<HALF_EVEN>(tile, block, factors, D, G, L.v_codes + g * (D * G / 4), L.v_scales + g * D, L.v_zeros + g * D);
+        const int64_t g = ((int64_t)(ok ? page : 0) * H + h) * (L.page_tokens / G) + t0 % L.page_tokens / G;
+        __syncthreads();
+        if (!ok) return;
+        quantize_keys_tile<T, HALF_EVEN>(k_tile, k_block, D, G, L.k_scales + g * D, L.k_zeros + g * D);
+        quantize_values_tile<T, HALF_EVEN>(v_tile, v_block, factors, D, G);
+        __syncthreads();
+        const int words = D * G / 16;
+        for (int i = threadIdx.x; i < words; i += kThreads) {
+            reinterpret_cast<uint32_t*>(L.k_codes + g * (D * G / 4))[i] = reinterpret_cast<const uint32_t*>(k_block)[i];
+            reinterpret_cast<uint32_t*>(L.v_codes + g * (D * G / 4))[i] = reinterpret_cast<const uint32_t*>(v_block)[i];
         }
-    };
-    // queries of this KV head, tokens lo .. hi - 1
-    auto turn_queries = [&](int lo, int hi) {
-        if (A.q.data == nullptr) return;
-        const int per = A.n_rep * units;
-        for (int i = threadIdx.x; i < (hi - lo) * per; i += kThreads) {
-            const int t = lo + i / per, r = i % per / units;
-            int d, e;
-            float x[4], y[4];
-            turn.places(i % units, d, e);
-            turn.load(row_of<T>(A.q, row(t), h * A.n_rep + r), angle_of(t), d, e, x, y);
-            T* to = const_cast<T*>(row_of<T>(A.q_out, row(t), h * A.n_rep + r));
-            Quad<T>::store(to + d, x, A.vec);
-            if (e >= 0) Quad<T>::store(to + e, y, A.vec);
-        }
+        for (int i = threadIdx.x; i < D; i += kThreads) { L.v_scales[g * D + i] = factors[i]; L.v_zeros[g * D + i] = factors[D + i]; }
     };
 
     const int end = q.held + q.n, out = quant_of(end, G, R);
     const int first = (q.held + G - 1) / G * G, n_fresh = fresh_groups(q);
-    if (sub > 0) {
-        const int t0 = first + (sub - 1) * G;
-        flush(t0, true);
-        turn_queries(t0, t0 + G);
+    const int in = quant_of(q.held, G, R), n_window = window_groups(q);
+    if (sub >= n_window) {
+        const int t0 = first + (sub - n_window) * G;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < G * units; i += kThreads) {
+            const int j = i / units;
+            fresh_unit(t0 + j, i % units, k_tile + j * S, v_tile + j * S, false, true);
+        }
+        flush_tiles(t0);
         return;
     }
-    for (int t0 = quant_of(q.held, G, R); t0 < (out < first ? out : first); t0 += G) flush(t0, false);
-    __syncthreads();
+    const int t0 = in + sub * G;
+    if (t0 < min(out, first)) {
+        for (int i = threadIdx.x; i < G * units; i += kThreads) {
+            const int j = i / units, t = t0 + j, u = i % units;
+            if (t < q.held) {
+                int d, e;
+                float x[N], y[N], vx[N], vy[N];
+                by.places(u, d, e);
+                const int64_t at = (int64_t)ring_slot(t, A.b.ring_shift, R) * D;
+                load2(k_ring + at, d, e, x, y);
+                load2(v_ring + at, d, e, vx, vy);
+                tile2(k_tile + j * S, d, e, x, y);
+                tile2(v_tile + j * S, d, e, vx, vy);
+            } else {
+                fresh_unit(t, u, k_tile + j * S, v_tile + j * S, false, false);
+            }
+        }
+        flush_tiles(t0);
+        __syncthreads();
+    }
     // what no other CTA has: the tokens before the first whole new group and those behind the last
     const int lo = n_fresh ? first : end, hi = n_fresh ? first + n_fresh * G : end;
-    const int rest = (lo - q.held) + (end - hi);
+    const int rest = (lo - q.held) + (end - hi), leaving = min(out, q.held);
     for (int i = threadIdx.x; i < rest * units; i += kThreads) {
         const int j = i / units, t = j < lo - q.held ? q.held + j : hi + (j - (lo - q.held));
-        int d, e;
-        float x[4], y[4];
-        turn.places(i % units, d, e);
-        turn.load(row_of<T>(A.k, row(t), h), A.rotary.table ? angle_of(t) : nullptr, d, e, x, y);
-        if (A.k_out.data) {
-            T* to = const_cast<T*>(row_of<T>(A.k_out, row(t), h));
-            Quad<T>::store(to + d, x, A.vec);
-            if (e >= 0) Quad<T>::store(to + e, y, A.vec);
-        }
-        if (t < out) continue;
-        const int64_t at = (int64_t)ring_slot(t, A.b.ring_shift, R) * D;
-        Quad<T>::store(k_ring + at + d, x, A.vec);
-        if (e >= 0) Quad<T>::store(k_ring + at + e, y, A.vec);
-        plain.load(row_of<T>(A.v, row(t), h), nullptr, d, e, x, y);
-        Quad<T>::store(v_ring + at + d, x, A.vec);
-        if (e >= 0) Quad<T>::store(v_ring + at + e, y, A.vec);
+        // the token of the window that had the slot, if it leaves, says whose this is
+        const int had = in + (t - in) % R;
+        const int whose = t >= out && had < leaving ? (had - in) / G : t % n_window;
+        if (whose == sub) fresh_unit(t, i % units, nullptr, nullptr, t >= out, true);
     }
-    turn_queries(q.held, lo);
-    turn_queries(hi, end);
 }
 
-// Four channels of keys and of values of one token per thread; neighbouring threads take
-// neighbouring channels, so a row leaves in whole lines.  Bound by its writes.
-// grid = (pieces of rows, KV heads, sequences).
+// Queries of a long step, two vectors a thread and pass; the rows of a block find their
+// sequences first.  Bound by memory.
+constexpr int kTurnRows = 8;
+template <typename T, int N, bool VEC>
+__global__ void __launch_bounds__(256)
+paged_turn_kernel(AppendArgs A) {
+    using C = Channels<T, N, VEC>;
+    __shared__ int token_s[kTurnRows];
+    stream_order();
+    settle_paged(A.L, A.b);
+    A.q.data = settled(A.q.data);
+    A.rotary.table = settled(A.rotary.table);
+    const Turn<T, N, VEC> by{A.rotary, A.L.head_dim};
+    const int row0 = blockIdx.x * kTurnRows, units = by.units(), heads = A.L.num_kv_heads * A.n_rep;
+    if (threadIdx.x < kTurnRows) {
+        const int row = row0 + threadIdx.x;
+        // the last sequence that starts at or before the row (none of a sequence that is left out)
+        int lo = 0, hi = A.b.num_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (A.b.cu_new[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        PagedSeq q;
+        const bool ok = load_seq(A.L, A.b, lo, q) && row >= q.row0 && row - q.row0 < q.n;
+        token_s[threadIdx.x] = ok ? q.held + (row - q.row0) : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTurnRows * heads * units; i += 256) {
+        const int u = i % units, head = i / units % heads, r = i / units / heads, t = token_s[r];
+        if (t < 0) continue;
+        int d, e;
+        float x[N], y[N];
+        typename Turn<T, N, VEC>::Angles a;
+        by.places(u, d, e);
+        const T* from = row_of<const T>(A.q, row0 + r, head);
+        C::load(from + d, x);
+        if (e >= 0) C::load(from + e, y);
+        by.angles(t, u, d, e, a);
+        by.turn(u, d, e, a, x, y);
+        T* to = row_of<T>(A.q_out, row0 + r, head);
+        C::store(to + d, x);
+        if (e >= 0) C::store(to + e, y);
+    }
+}
+
+// Four channels of keys and values of four tokens per thread, which a word of key codes
+// holds; neighbouring threads take neighbouring channels, so a row leaves in whole lines.
+// Bound by its writes.  grid = (pieces of rows, KV heads, sequences).
 template <typename T>
 __global__ void __launch_bounds__(256)
 paged_read_kernel(kivi_paged_layer L, kivi_paged_batch b, const int32_t* starts, float* __restrict__ k_out, float* __restrict__ v_out) {
@@ -319,36 +429,53 @@ paged_read_kernel(kivi_paged_layer L, kivi_paged_batch b, const int32_t* starts,
         if (threadIdx.x == 0) atomicOr(&g_fault, kPagedFault);
         return;
     }
+    if (n == 0) return;
     PagedSeq q{held, n, r0, slot, b.page_table + (int64_t)s * b.table_width};
-    const int out = quant_of(held, G, R), Q = G / 4, W = D < 64 ? D : 64;
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < (int64_t)n * quads; i += (int64_t)gridDim.x * 256) {
-        const int t = start + (int)(i / quads), d = 4 * (int)(i % quads);
-        float4 k, v;
-        if (t < out) {
-            const int page = page_of(L, q, t, &g_fault), gpp = L.page_tokens / G;
-            const int64_t g = ((int64_t)page * H + h) * gpp + t % L.page_tokens / G;
-            const int tt = t % G;
+    const int out = quant_of(held, G, R), Q = G / 4, W = D < 64 ? D : 64, gpp = L.page_tokens / G;
+    const int first = start / 4, blocks = (start + n + 3) / 4 - first;            // quads of tokens
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < (int64_t)blocks * quads; i += (int64_t)gridDim.x * 256) {
+        const int t0 = 4 * (first + (int)(i / quads)), d = 4 * (int)(i % quads);
+        float4 k[4], v[4];
+        if (t0 < out) {                                  // (groups are whole quads)
+            const int64_t g = ((int64_t)page_of(L, q, t0, &g_fault) * H + h) * gpp + t0 % L.page_tokens / G;
+            const int tt = t0 % G;
             const uint32_t w = *reinterpret_cast<const uint32_t*>(L.k_codes + g * (D * Q) + kblock_offset(d, tt >> 2, Q, W));
             const float4 ks = *reinterpret_cast<const float4*>(L.k_scales + g * D + d), kz = *reinterpret_cast<const float4*>(L.k_zeros + g * D + d);
-            const int sh = 2 * (tt & 3);
-            k = make_float4(dequant((float)((w >> sh) & 3u), ks.x, kz.x), dequant((float)((w >> (sh + 8)) & 3u), ks.y, kz.y),
-                            dequant((float)((w >> (sh + 16)) & 3u), ks.z, kz.z), dequant((float)((w >> (sh + 24)) & 3u), ks.w, kz.w));
-            const uint32_t c = L.v_codes[g * (D * Q) + vcode_offset(tt, d / 4, D, G)];
-            const int64_t at = g * D + vmeta_index(tt, d / G, D, G);
-            const float vs = L.v_scales[at], vz = L.v_zeros[at];
-            v = make_float4(dequant((float)(c & 3u), vs, vz), dequant((float)((c >> 2) & 3u), vs, vz),
-                            dequant((float)((c >> 4) & 3u), vs, vz), dequant((float)(c >> 6), vs, vz));
+            uint32_t c[4];
+            float vs[4], vz[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                c[e] = L.v_codes[g * (D * Q) + vcode_offset(tt + e, d / 4, D, G)];
+                const int64_t at = g * D + vmeta_index(tt + e, d / G, D, G);
+                vs[e] = L.v_scales[at]; vz[e] = L.v_zeros[at];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t x = w >> (2 * e);
+                k[e] = make_float4(dequant((float)(x & 3u), ks.x, kz.x), dequant((float)((x >> 8) & 3u), ks.y, kz.y),
+                                   dequant((float)((x >> 16) & 3u), ks.z, kz.z), dequant((float)((x >> 24) & 3u), ks.w, kz.w));
+                v[e] = make_float4(dequant((float)(c[e] & 3u), vs[e], vz[e]), dequant((float)((c[e] >> 2) & 3u), vs[e], vz[e]),
+                                   dequant((float)((c[e] >> 4) & 3u), vs[e], vz[e]), dequant((float)(c[e] >> 6), vs[e], vz[e]));
+            }
         } else {
-            const int64_t at = (((int64_t)slot * H + h) * R + ring_slot(t, b.ring_shift, R)) * D + d;
-            float x[4];
-            Quad<T>::load(reinterpret_cast<const T*>(L.k_res) + at, x, false);
-            k = make_float4(x[0], x[1], x[2], x[3]);
-            Quad<T>::load(reinterpret_cast<const T*>(L.v_res) + at, x, false);
-            v = make_float4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t at = (((int64_t)slot * H + h) * R + ring_slot(min(t0 + e, held - 1), b.ring_shift, R)) * D + d;
+                float x[4];
+                Channels<T, 4, true>::load(reinterpret_cast<const T*>(L.k_res) + at, x);
+                k[e] = make_float4(x[0], x[1], x[2], x[3]);
+                Channels<T, 4, true>::load(reinterpret_cast<const T*>(L.v_res) + at, x);
+                v[e] = make_float4(x[0], x[1], x[2], x[3]);
+            }
         }
-        const int64_t to = (((int64_t)r0 + i / quads) * H + h) * D + d;
-        store_quad(k_out, KIVI_F32, to, k);
-        store_quad(v_out, KIVI_F32, to, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int t = t0 + e;
+            if (t < start || t >= start + n) continue;
+            const int64_t to = (((int64_t)r0 + (t - start)) * H + h) * D + d;
+            store_quad(k_out, KIVI_F32, to, k[e]);
+            store_quad(v_out, KIVI_F32, to, v[e]);
+        }
     }
 }
 
@@ -404,8 +531,22 @@ int check_rows(const kivi_rows* r, const char* name, int head_dim) {
     (void)head_dim;
     return KIVI_OK;
 }
-bool on_grid(const kivi_rows& r, int esz) {
-    return (reinterpret_cast<uintptr_t>(r.data) % (4 * esz)) == 0 && r.row_stride % 4 == 0 && r.head_stride % 4 == 0;
+// vectors of n channels lie on their own grid
+bool on_grid(const kivi_rows& r, int esz, int n) {
+    return (reinterpret_cast<uintptr_t>(r.data) % (n * esz)) == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
+}
+using AppendKernel = void (*)(AppendArgs);
+template <typename T>
+AppendKernel turn_kernel(bool wide, bool vec) {
+    constexpr int N = 16 / sizeof(T);
+    return wide ? paged_turn_kernel<T, N, true> : vec ? paged_turn_kernel<T, 4, true> : paged_turn_kernel<T, 4, false>;
+}
+template <typename T, bool QUERIES>
+AppendKernel append_kernel(bool wide, bool vec, bool even) {
+    constexpr int N = 16 / sizeof(T);
+    if (wide) return even ? paged_append_kernel<T, N, true, true, QUERIES> : paged_append_kernel<T, N, true, false, QUERIES>;
+    if (vec) return even ? paged_append_kernel<T, 4, true, true, QUERIES> : paged_append_kernel<T, 4, true, false, QUERIES>;
+    return even ? paged_append_kernel<T, 4, false, true, QUERIES> : paged_append_kernel<T, 4, false, false, QUERIES>;
 }
 
 }  // namespace
@@ -437,7 +578,7 @@ extern "C" int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged
         KIVI_REQUIRE(!queries, "queries are only taken together with rotary");
         KIVI_REQUIRE(k_out == nullptr || k_out->data == nullptr, "k_out is only written together with rotary");
     }
-    const size_t smem = (size_t)G * (D + 4) * 4 + 2 * D * 4 + (size_t)D * G / 4;
+    const size_t smem = 2 * (size_t)G * (D * esz + 16) + 2 * D * 4 + (size_t)D * G / 2;
     if (smem > 220 * 1024) {
         set_error("a group of %d tokens of head_dim %d does not fit shared memory", G, D);
         return KIVI_ERR_UNSUPPORTED;
@@ -448,15 +589,31 @@ extern "C" int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged
     a.rotary = {rotary, rotary ? rotary_dim : 0, interleaved ? 1 : 0};
     if (rotary) a.k_out = *k_out;
     if (queries) { a.q = *q; a.q_out = *q_out; }
-    a.vec = on_grid(a.k, esz) && on_grid(a.v, esz) && on_grid(a.k_out, esz) && on_grid(a.q, esz) && on_grid(a.q_out, esz);
-    const int64_t items = batch->max_new >= G ? (int64_t)batch->num_seqs + batch->total_new / G : batch->num_seqs;
+    auto grid = [&](int n) {
+        const bool table = rotary == nullptr || ((reinterpret_cast<uintptr_t>(rotary) & 15u) == 0 && rotary_dim % 4 == 0 && (interleaved || rotary_dim % (2 * n) == 0));
+        return D % n == 0 && table && on_grid(a.k, esz, n) && on_grid(a.v, esz, n) && on_grid(a.k_out, esz, n) && on_grid(a.q, esz, n) && on_grid(a.q_out, esz, n);
+    };
+    const bool bf16 = layer->res_dtype == KIVI_BF16, wide = bf16 ? grid(8) : grid(4), vec = grid(4);
+    cudaStream_t st = (cudaStream_t)stream;
+    int launches = 1;
+    // queries of more than a group of tokens: by themselves
+    if (queries && batch->max_new >= G) {
+        auto* const turn = bf16 ? turn_kernel<__nv_bfloat16>(wide, vec) : turn_kernel<float>(wide, vec);
+        KIVI_CUDA_OK(launch(turn, dim3((unsigned)((batch->total_new + kTurnRows - 1) / kTurnRows)), 256, 0, st, true, a));
+        a.q = a.q_out = kivi_rows{};
+        ++launches;
+    }
+    // a step of one token moves at most the group that it completes
+    a.items_vary = batch->max_new > 1;
+    const int64_t window_items = a.items_vary ? (layer->residual_cap - 1) / G + 1 : 1;
+    const int64_t items = (int64_t)batch->num_seqs * window_items + batch->total_new / G;
     KIVI_REQUIRE(items <= 0x7fffffff, "too many groups in one step");
-    auto* const kernel = layer->res_dtype == KIVI_BF16
-        ? (rounding == KIVI_ROUND_HALF_EVEN ? paged_append_kernel<__nv_bfloat16, true> : paged_append_kernel<__nv_bfloat16, false>)
-        : (rounding == KIVI_ROUND_HALF_EVEN ? paged_append_kernel<float, true> : paged_append_kernel<float, false>);
+    const bool even = rounding == KIVI_ROUND_HALF_EVEN;
+    auto* const kernel = bf16 ? (a.q.data ? append_kernel<__nv_bfloat16, true>(wide, vec, even) : append_kernel<__nv_bfloat16, false>(wide, vec, even))
+                              : (a.q.data ? append_kernel<float, true>(wide, vec, even) : append_kernel<float, false>(wide, vec, even));
     if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)items, (unsigned)layer->num_kv_heads), kThreads, smem, (cudaStream_t)stream, true, a));
-    note_launches(1);
+    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)items, (unsigned)layer->num_kv_heads), kThreads, smem, st, true, a));
+    note_launches(launches);
     return KIVI_OK;
 }
 
@@ -466,7 +623,7 @@ extern "C" int kivi_paged_read(const kivi_paged_layer* layer, const kivi_paged_b
     if (int rc = validate_batch(layer, batch)) return rc;
     KIVI_REQUIRE(starts != nullptr && k_out != nullptr && v_out != nullptr, "starts, k_out or v_out is null");
     if (batch->max_new == 0) { note_launches(0); return KIVI_OK; }
-    int64_t pieces = ((int64_t)batch->max_new * (layer->head_dim / 4) + 255) / 256;
+    int64_t pieces = (((int64_t)batch->max_new + 6) / 4 * (layer->head_dim / 4) + 255) / 256;        // (quads of tokens that the rows touch)
     if (pieces > 4096) pieces = 4096;
     auto* const kernel = layer->res_dtype == KIVI_BF16 ? paged_read_kernel<__nv_bfloat16> : paged_read_kernel<float>;
     KIVI_CUDA_OK(launch(kernel, dim3((unsigned)pieces, (unsigned)layer->num_kv_heads, (unsigned)batch->num_seqs), 256, 0, (cudaStream_t)stream, true,
