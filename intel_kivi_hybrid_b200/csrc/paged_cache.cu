@@ -9,12 +9,11 @@
 //   * one CTA per whole group of new tokens and KV head quantizes that group.
 // Every CTA also turns the keys it has and, in steps of a few tokens, the queries of its KV
 // head; in longer steps the queries are a streaming kernel of their own (in the same CTAs
-// they took 160 registers: 4 x 2048 tokens 189 us, DT_SPLIT us apart).
+// they took 160 registers: 4 x 2048 tokens 189 us, 100 apart).
 //
 // Bound by memory: bf16, D = 128, G = 32 moves 2.1 bytes per element of the rows in and
 // out and 0.5 per flushed element; the smallest call (one token) is launch and latency.
-// A thread takes two 16-byte vectors of a token and everything that shares their angles -- the
-// key, the value, the query heads -- so that some ten loads are in flight.
+// A thread takes two 16-byte vectors of a token's key and of its value at a time.
 #include "paged_common.cuh"
 
 namespace kivi {
@@ -198,8 +197,8 @@ struct Turn {
 };
 
 // N: channels of a vector (16 bytes, or 4 channels for shapes that those do not divide); a
-// thread has two of them of a token, which hold each other's partners where halves are
-// paired, and all heads of the token that take the same angles.
+// thread has two of them of a row, which hold each other's partners where halves are
+// paired.  QUERIES: a step shorter than a group, whose queries are turned here.
 template <typename T, int N, bool VEC, bool HALF_EVEN, bool QUERIES>
 __global__ void __launch_bounds__(kThreads)
 paged_append_kernel(AppendArgs A) {
@@ -269,8 +268,7 @@ paged_append_kernel(AppendArgs A) {
     T* const k_ring = reinterpret_cast<T*>(L.k_res) + ring0 * D;
     T* const v_ring = reinterpret_cast<T*>(L.v_res) + ring0 * D;
 
-    // One unit of a new token: turned keys to where `to_tile` / `to_ring` / `out` say, its values
-    // likewise, and (out) the queries of this KV head.
+    // One unit of a new token: its turned key to a tile, the window and k_out, its value likewise.
     auto fresh_unit = [&](int t, int u, T* kt, T* vt, bool to_ring, bool out) {
         const int64_t row = (int64_t)q.row0 + (t - q.held);
         int d, e;
@@ -287,20 +285,6 @@ paged_append_kernel(AppendArgs A) {
             const int64_t at = (int64_t)ring_slot(t, A.b.ring_shift, R) * D;
             Channels<T, N, VEC>::store(k_ring + at + d, x); Channels<T, N, VEC>::store(v_ring + at + d, vx);
             if (e >= 0) { Channels<T, N, VEC>::store(k_ring + at + e, y); Channels<T, N, VEC>::store(v_ring + at + e, vy); }
-        }
-        if (QUERIES && out) {
-            for (int r0 = 0; r0 < A.n_rep; r0 += 4) {                    // four heads in flight
-                float p[4][N], z[4][N];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (r0 + r < A.n_rep) load2(row_of<const T>(A.q, row, h * A.n_rep + r0 + r), d, e, p[r], z[r]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (r0 + r < A.n_rep) {
-                        by.turn(u, d, e, a, p[r], z[r]);
-                        store2(row_of<T>(A.q_out, row, h * A.n_rep + r0 + r), d, e, p[r], z[r]);
-                    }
-            }
         }
     };
     // the group in the tiles to its page
@@ -358,12 +342,27 @@ paged_append_kernel(AppendArgs A) {
     // what no other CTA has: the tokens before the first whole new group and those behind the last
     const int lo = n_fresh ? first : end, hi = n_fresh ? first + n_fresh * G : end;
     const int rest = (lo - q.held) + (end - hi), leaving = min(out, q.held);
-    for (int i = threadIdx.x; i < rest * units; i += kThreads) {
-        const int j = i / units, t = j < lo - q.held ? q.held + j : hi + (j - (lo - q.held));
+    const int slots = QUERIES ? 1 + A.n_rep : 1;         // key and value, then the query heads: a thread's work each
+    for (int i = threadIdx.x; i < rest * units * slots; i += kThreads) {
+        const int u = i % units, slot = i / units % slots, j = i / units / slots, t = j < lo - q.held ? q.held + j : hi + (j - (lo - q.held));
         // the token of the window that had the slot, if it leaves, says whose this is
         const int had = in + (t - in) % R;
         const int whose = t >= out && had < leaving ? (had - in) / G : t % n_window;
-        if (whose == sub) fresh_unit(t, i % units, nullptr, nullptr, t >= out, true);
+        if (whose != sub) continue;
+        if (!QUERIES || slot == 0) {
+            fresh_unit(t, u, nullptr, nullptr, t >= out, true);
+        } else {
+            const int64_t row = (int64_t)q.row0 + (t - q.held);
+            const int head = h * A.n_rep + slot - 1;
+            int d, e;
+            float x[N], y[N];
+            typename Turn<T, N, VEC>::Angles a;
+            by.places(u, d, e);
+            load2(row_of<const T>(A.q, row, head), d, e, x, y);
+            by.angles(t, u, d, e, a);
+            by.turn(u, d, e, a, x, y);
+            store2(row_of<T>(A.q_out, row, head), d, e, x, y);
+        }
     }
 }
 
