@@ -458,6 +458,32 @@ def sample_tokens(logits, temperature=1.0, top_k=0, do_sample=False, seed=0, ste
     return out
 
 
+def sample_filtered(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """kivi_sample_filtered: [batch, vocab] fp32 / bf16 device logits (last dim contiguous) and one fp32 number of [0, 1)
+    a row -> int64 [batch] device ids.  temperature, top_p, min_p: fp32 device tensors of one entry per row, top_k: int32;
+    None: 1, no cut."""
+    ops = _native_ops()
+    if ops is not None:
+        return ops.sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p, out)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] != 1):
+        raise RuntimeError("logits must be [batch, vocab] with entries side by side")
+    B, V = logits.shape
+    if B > 1 and logits.stride(0) < V:
+        raise RuntimeError("rows of logits overlap")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    ptr = []
+    for t, dtype in ((uniforms, torch.float32), (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32), (out, torch.int64)):
+        if t is not None:
+            _dev(t)
+            if t.dtype != dtype or t.numel() != B or t.device != logits.device:
+                raise RuntimeError(f"one {dtype} entry for each of the {B} rows is needed on {logits.device}")
+        ptr.append(None if t is None else t.data_ptr())
+    if B:
+        _check(lib.kivi_sample_filtered(logits.data_ptr(), _dt(logits), B, V, max(logits.stride(0), V), *ptr, _stream()))
+    return out
+
+
 def quantize_groups_at(store: "LayerStore", k, v, at_group: int, rounding=ROUND_HALF_AWAY):
     """Quantize whole groups of tokens k, v [num_units, n*G, D] straight into the
     packed store of ``store`` at groups at_group .. at_group + n - 1, without

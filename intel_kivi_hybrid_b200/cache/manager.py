@@ -350,6 +350,38 @@ class KiviCache:
             out = all_gather_units(out, B * self.num_kv_heads, self.shard[0], self.shard[1])
         return out.reshape(B, Hq, D)
 
+    def chunk_attention(self, layer: int, q: torch.Tensor, new_k: torch.Tensor, new_v: torch.Tensor, sm_scale: float = 0.0) -> torch.Tensor:
+        """Causal attention of several query tokens per sequence over the cache: call it after ``ingest_layer`` of the
+        same keys and values.  q [B, Hq, n, D], new_k and new_v [B, H, n, D]; returns [B, n, Hq, D].
+
+        Token i of the n attends to everything held before and to the first i + 1 of the new ones.  Those are
+        attended as they are given, also where the ingest has already moved them to the packed store; a token from
+        before the call as the store or the window has it now."""
+        from ..extension.loader import kivi_native
+        st = self._stores[layer]
+        assert st is not None, "chunk_attention() before any add_tokens()"
+        assert self.shard is None or self.shard[1] == 1, "chunk_attention() is not available on a sharded cache"
+        B, Hq, n, D = q.shape
+        H = self.num_kv_heads
+        assert B == self.batch_size and Hq % H == 0 and new_k.shape == (B, H, n, D) and new_v.shape == new_k.shape, \
+            "q must be [B, Hq, n, D], new_k and new_v [B, H, n, D]"
+        held = st.quant_len + st.res_len - n
+        assert held >= 0, f"the cache holds {held + n} tokens: ingest the {n} new ones first"
+        _, quant, _ = cabi.cache_plan(0, 0, held + n, self.G, self.R)
+        assert quant == st.quant_len, "the store was not filled by ingest_layer() / add_tokens()"
+        dev, G = st.k_codes.device, self.G
+        rows = lambda x: x.transpose(1, 2).reshape(B * n, x.shape[1], D)  # noqa: E731
+        pool = (st.k_codes.view(B, H, -1, D * G // 4), st.k_scales.view(B, H, -1, D), st.k_zeros.view(B, H, -1, D), st.v_codes.view(B, H, -1, D // 4),
+                st.v_scales.view(B, H, -1, D // G), st.v_zeros.view(B, H, -1, D // G), st.k_res.view(B, H, self.R, D), st.v_res.view(B, H, self.R, D))
+        own = torch.arange(B + 1, dtype=torch.int32, device=dev)            # every sequence is its own page and slot
+        qr, kr, vr = rows(q).to(dev), rows(new_k).to(dev, st.dtype), rows(new_v).to(dev, st.dtype)
+        if qr.dtype not in (torch.float32, torch.bfloat16):
+            qr = qr.float()
+        out = torch.empty_like(qr, memory_format=torch.contiguous_format)
+        kivi_native.paged_attention(qr, kr, vr, *pool, own[:B, None].contiguous(), own[:B], torch.full((B,), held, dtype=torch.int32, device=dev), own * n, n, held + n,
+                                    out, G, sm_scale, (st.res_start - st.quant_len) % self.R)
+        return out.view(B, n, Hq, D)
+
     def get_full_cache(self):
         """Dense past_key_values for unmodified model code (manager.py:251-290):
         dequantized history followed by the residual window, as a DynamicCache on

@@ -14,6 +14,7 @@ once every ``EOS_CHECK_EVERY`` steps over the ids produced since the last look,
 and what was generated past the first EOS is cut off, so the returned text is
 the same and at most ``EOS_CHECK_EVERY - 1`` steps are spent in vain.
 """
+from functools import partial
 from typing import Optional
 
 import torch
@@ -38,10 +39,16 @@ def _first_eos(produced, start, eos_id):
 def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_size: int = 32,
              residual_length: int = 128, device: str = "cuda", temperature: float = 1.0,
              top_k: Optional[int] = None, do_sample: bool = False, verbose: bool = False,
-             fused_attention: bool = False) -> str:
+             fused_attention: bool = False, top_p: float = 1.0, min_p: float = 0.0,
+             prefill_chunk: Optional[int] = None) -> str:
+    """The reference's arguments, and: ``fused_attention`` (below), ``top_p`` / ``min_p`` (cuts of the draw, see
+    ``sampling.sample_token``), ``prefill_chunk`` (with ``fused_attention``: the prompt goes through the model in
+    pieces of that many tokens, each attending to the packed cache, so that no forward is longer)."""
+    if prefill_chunk is not None and (not fused_attention or prefill_chunk < 1):
+        raise ValueError("prefill_chunk needs fused_attention=True and at least one token")
+    pick = partial(sample_token, temperature=temperature, top_k=top_k, do_sample=do_sample, top_p=top_p, min_p=min_p)
     if fused_attention:
-        return _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residual_length, device,
-                               temperature, top_k, do_sample, verbose)
+        return _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residual_length, device, pick, verbose, prefill_chunk)
     cache = KiviCache.from_model(model, device=device, group_size=group_size, residual_length=residual_length)
     input_ids = tokenizer(prompt, return_tensors="pt").input_ids
     model_device = next(model.parameters()).device if hasattr(model, "parameters") else input_ids.device
@@ -49,7 +56,7 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
 
     out = model(input_ids, use_cache=True)                                   # prefill
     cache.add_tokens(out.past_key_values)
-    next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample)
+    next_id = pick(out.logits[:, -1, :])
     produced = [next_id]
     eos_id = tokenizer.eos_token_id
 
@@ -64,7 +71,7 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
                 break
         out = model(next_id, past_key_values=cache.get_full_cache(), use_cache=True)
         cache.add_tokens(out.past_key_values)
-        next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample).to(model_device)
+        next_id = pick(out.logits[:, -1, :]).to(model_device)
         produced.append(next_id)
         if verbose and (step + 1) % 10 == 0:
             print(".", end="", flush=True)
@@ -77,8 +84,8 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
     return tokenizer.decode(full[0], skip_special_tokens=True)
 
 
-def _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residual_length, device,
-                    temperature, top_k, do_sample, verbose) -> str:
+def _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residual_length, device, pick, verbose,
+                    prefill_chunk) -> str:
     """Same loop with ``fused_attention=True``: the model's K/V stream straight
     into the cache and every decode step attends through
     ``KiviCache.decode_attention`` (no dense past_key_values is ever built)."""
@@ -88,9 +95,10 @@ def _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residu
     model_device = next(model.parameters()).device if hasattr(model, "parameters") else input_ids.device
     input_ids = input_ids.to(model_device)
     eos_id = tokenizer.eos_token_id
-    with attached(model, cache) as past:
-        out = model(input_ids, past_key_values=past, use_cache=True)
-        next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample)
+    with attached(model, cache, chunked=prefill_chunk is not None) as past:
+        for piece in input_ids.split(prefill_chunk or input_ids.shape[1], dim=1):
+            out = model(piece, past_key_values=past, use_cache=True)
+        next_id = pick(out.logits[:, -1, :])
         produced = [next_id]
         checked = 0
         for step in range(1, max_new_tokens):
@@ -101,7 +109,7 @@ def _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residu
                     del produced[stop + 1:]
                     break
             out = model(next_id, past_key_values=past, use_cache=True)
-            next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample).to(model_device)
+            next_id = pick(out.logits[:, -1, :]).to(model_device)
             produced.append(next_id)
             if verbose and (step + 1) % 10 == 0:
                 print(".", end="", flush=True)

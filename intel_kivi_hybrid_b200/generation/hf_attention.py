@@ -13,8 +13,10 @@ With this hook the model never sees a dense history:
   for the prefill (many query tokens, empty cache) it runs ordinary causal
   attention over the prompt's own K/V, exactly what the reference's prefill
   forward computes before the cache sees the tokens (generate.py:61-62).
-  Any other pattern (several query tokens on a non-empty cache, a padded decode
-  batch, sliding-window layers) raises instead of attending to the wrong keys.
+  Several query tokens on a cache that already holds some (a prompt in pieces, a second
+  chat turn, speculative tokens) go to ``KiviCache.chunk_attention`` where the hook was
+  attached with ``chunked=True``.  Any other pattern (such tokens without it, a padded
+  decode batch, sliding-window layers) raises instead of attending to the wrong keys.
 
 One ordering difference from the reference loop: ``update()`` appends the step's
 token and flushes *before* the step attends, so on a flush step (one in G) the
@@ -76,11 +78,12 @@ def kivi_fused_attention(module, query, key, value, attention_mask, dropout=0.0,
     """query [B, Hq, Lq, D]; key/value: the NEW tokens of this forward pass.
 
     Supported call patterns: one forward over the whole prompt on an empty cache,
-    then forwards of one token each -- the loop of generate().  Everything else
-    would silently attend to the wrong keys and is refused: several query tokens
-    on a cache that already holds a history (chunked prefill, a second chat turn,
-    speculative tokens), a decode step whose mask hides positions (left-padded
-    batches), and sliding-window layers.
+    then forwards of one token each -- the loop of generate() -- or, attached with
+    ``chunked=True``, of any number of tokens.  Everything else would silently attend
+    to the wrong keys and is refused: several query tokens on a cache that already
+    holds a history without ``chunked`` (chunked prefill, a second chat turn,
+    speculative tokens), a step whose mask hides positions (left-padded batches), and
+    sliding-window layers.
     """
     cache = getattr(module, "_kivi_cache", None)
     B, Hq, Lq, D = query.shape
@@ -105,6 +108,12 @@ def kivi_fused_attention(module, query, key, value, attention_mask, dropout=0.0,
             q = q.float()
         out = cache.decode_attention(layer, q.contiguous(), sm_scale=float(scaling or 0.0))
         return out.to(query.device, query.dtype).reshape(B, 1, Hq, D), None
+    if history > 0 and getattr(module, "_kivi_chunked", False):
+        if B > 1 and _mask_hides_something(None if attention_mask is None else attention_mask[..., -1:, :]):
+            raise RuntimeError("kivi_fused attention: the chunk's attention_mask hides key positions from its last token (padded batch); "
+                               "the fused kernel attends to every cached token. Use get_full_cache() for padded batches.")
+        out = cache.chunk_attention(layer, query, key, value, sm_scale=float(scaling or 0.0))
+        return out.to(query.device, query.dtype), None
     if history > 0:
         raise RuntimeError(f"kivi_fused attention: {Lq} query tokens on a cache that already holds {history} tokens "
                            f"(chunked prefill / multi-token step) is not supported: the packed history would be ignored. "
@@ -129,15 +138,18 @@ def _register():
 
 
 @contextlib.contextmanager
-def attached(model, kivi_cache):
+def attached(model, kivi_cache, chunked: bool = False):
     """Route ``model``'s self-attention through the KIVI cache; yields the
-    past_key_values object to pass to the model."""
+    past_key_values object to pass to the model.  ``chunked``: forwards of several
+    tokens on a cache that already holds some are served (the model may be fed its
+    prompt in pieces); without it they are refused."""
     _register()
     previous = model.config._attn_implementation
     touched = []
     for mod in model.modules():
         if hasattr(mod, "layer_idx") and hasattr(mod, "forward") and not hasattr(mod, "_kivi_cache"):
             mod._kivi_cache = kivi_cache
+            mod._kivi_chunked = chunked
             touched.append(mod)
     model.config._attn_implementation = ATTN_NAME
     try:
@@ -145,4 +157,4 @@ def attached(model, kivi_cache):
     finally:
         model.config._attn_implementation = previous
         for mod in touched:
-            del mod._kivi_cache
+            del mod._kivi_cache, mod._kivi_chunked

@@ -3,7 +3,7 @@
 import intel_kivi_hybrid_b200 as _impl
 from intel_kivi_hybrid_b200 import __version__
 
-__all__ = ["KiviCache", "generate", "__version__"]
+__all__ = ["KiviCache", "PagedKiviCache", "generate", "__version__"]
 
 
 def __getattr__(name):
