@@ -475,8 +475,13 @@ int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged_batch* bat
  * from pages and window, the step's own from new_k / new_v (turned, in full precision,
  * also those that the append has already moved to pages).
  * q, out: rows of q_dtype / out_dtype with num_kv_heads * n_rep heads.  sm_scale <= 0
- * means head_dim^-0.5.  workspace: device scratch of kivi_paged_attention_workspace()
- * bytes for the same arguments, contents need not be preserved. */
+ * means head_dim^-0.5.  out may be q itself.  workspace: device scratch of
+ * kivi_paged_attention_workspace() bytes for the same arguments, contents need not be
+ * preserved.
+ * Accuracy: fp32 operands and sums; with bf16 rows (head_dim 64 or 128, groups of 32) the
+ * dequantized numbers and the weights are rounded at 2^-12, values below 2^-27 of a tile's
+ * largest at less; sums are fp32.  A token that a row does not see does not touch it,
+ * whatever it holds. */
 size_t kivi_paged_attention_workspace(const kivi_paged_layer* layer, const kivi_paged_batch* batch, int q_dtype, int n_rep);
 int kivi_paged_attention(const kivi_paged_layer* layer, const kivi_paged_batch* batch, const kivi_rows* q,
                          int q_dtype, const kivi_rows* new_k, const kivi_rows* new_v, const kivi_rows* out,
@@ -504,8 +509,8 @@ int kivi_paged_read(const kivi_paged_layer* layer, const kivi_paged_batch* batch
  * infinite ones each has mass 1 and no other any; a row without a number above -inf gives 0.
  * Sums are in fp64, relative error of a mass below 2e-9: a draw differs from the one in
  * real arithmetic only within that of a boundary.
- * logits: device [batch][row_stride >= vocab] of dtype.  uniforms: device fp32 [batch] in
- * [0, 1).  temperature, top_p, min_p: device fp32 [batch], top_k: device int32 [batch]; NULL
+ * logits: device [batch][row_stride >= vocab, or 0: one row for all draws] of dtype.
+ * uniforms: device fp32 [batch] in [0, 1).  temperature, top_p, min_p: device fp32 [batch], top_k: device int32 [batch]; NULL
  * means 1, no cut.  ids_out: device int64 [batch]. */
 int kivi_sample_filtered(const void* logits, int dtype, int batch, int vocab, int64_t row_stride,
                          const float* uniforms, const float* temperature, const int32_t* top_k,

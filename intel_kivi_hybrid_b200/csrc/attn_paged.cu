@@ -23,20 +23,6 @@ __device__ int g_fault = 0;
 
 constexpr int kTile = 64;                                // tokens in shared memory at a time
 
-template <typename T> __device__ __forceinline__ float4 load4(const T* p, bool vec);
-template <> __device__ __forceinline__ float4 load4<float>(const float* p, bool vec) {
-    return vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
-}
-template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p, bool vec) {
-    if (!vec) return make_float4(__bfloat162float(p[0]), __bfloat162float(p[1]), __bfloat162float(p[2]), __bfloat162float(p[3]));
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
-}
-__device__ __forceinline__ float4 load4_as(const kivi_rows& r, int dtype, int64_t row, int head, int d, bool vec) {
-    const int64_t at = row * r.row_stride + (int64_t)head * r.head_stride + d;
-    return dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(r.data) + at, vec) : load4(reinterpret_cast<const float*>(r.data) + at, vec);
-}
-
 // DT: head_dim 64 or 128, or 256 for any up to that.
 template <int RPT, int TY, int DT>
 __global__ void __launch_bounds__(TY * 16)
@@ -47,7 +33,7 @@ paged_attention_kernel(PagedAttnArgs A) {
     stream_order();
     settle_args(A);
     const kivi_paged_layer& L = A.L;
-    const int D = DT == 256 ? L.head_dim : DT, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + 4, Q = G / 4, W = D < 64 ? D : 64;
+    const int D = DT == 256 ? L.head_dim : DT, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + 4;
     float* const q_s = smem_f;                           // [RT][S]
     float* const k_s = q_s + RT * S;                     // [kTile][S]
     float* const v_s = k_s + kTile * S;                  // [kTile][S]
@@ -96,37 +82,14 @@ paged_attention_kernel(PagedAttnArgs A) {
 #pragma unroll
         for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.0f;
     }
-    const int64_t ring0 = ((int64_t)q.slot * H + h) * R;
     for (int t0 = t_begin; t0 < t_end; t0 += kTile) {
         __syncthreads();                                 // the tile before has been read
         for (int i = tid; i < kTile * (D / 4); i += kThreads) {
             const int j = i / (D / 4), d = 4 * (i % (D / 4)), t = t0 + j;
             float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-            if (t < inside) {
-                const int64_t g = ((int64_t)page_of(L, q, t, &g_fault) * H + h) * (L.page_tokens / G) + t % L.page_tokens / G;
-                const int tt = t % G, sh = 2 * (tt & 3);
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(L.k_codes + g * (D * Q) + kblock_offset(d, tt >> 2, Q, W));
-                const float4 ks = *reinterpret_cast<const float4*>(L.k_scales + g * D + d), kz = *reinterpret_cast<const float4*>(L.k_zeros + g * D + d);
-                k = make_float4(fmaf((float)((w >> sh) & 3u), ks.x, kz.x), fmaf((float)((w >> (sh + 8)) & 3u), ks.y, kz.y),
-                                fmaf((float)((w >> (sh + 16)) & 3u), ks.z, kz.z), fmaf((float)((w >> (sh + 24)) & 3u), ks.w, kz.w));
-                const uint32_t c = L.v_codes[g * (D * Q) + vcode_offset(tt, d / 4, D, G)];
-                const int64_t at = g * D + vmeta_index(tt, d / G, D, G);
-                const float vs = L.v_scales[at], vz = L.v_zeros[at];
-                v = make_float4(fmaf((float)(c & 3u), vs, vz), fmaf((float)((c >> 2) & 3u), vs, vz),
-                                fmaf((float)((c >> 4) & 3u), vs, vz), fmaf((float)(c >> 6), vs, vz));
-            } else if (t < q.held) {
-                const int64_t at = (ring0 + ring_slot(t, A.b.ring_shift, R)) * D + d;
-                if (L.res_dtype == KIVI_BF16) {
-                    k = load4(reinterpret_cast<const __nv_bfloat16*>(L.k_res) + at, true);
-                    v = load4(reinterpret_cast<const __nv_bfloat16*>(L.v_res) + at, true);
-                } else {
-                    k = load4(reinterpret_cast<const float*>(L.k_res) + at, true);
-                    v = load4(reinterpret_cast<const float*>(L.v_res) + at, true);
-                }
-            } else if (t < t_end) {
-                const int64_t row = (int64_t)q.row0 + (t - q.held);
-                k = load4_as(A.k, L.res_dtype, row, h, d, vec);
-                v = load4_as(A.v, L.res_dtype, row, h, d, vec);
+            if (t < t_end) {
+                k = paged_key4(A, q, h, inside, t, d, vec, &g_fault);
+                v = paged_value4(A, q, h, inside, t, d, vec, &g_fault);
             }
             *reinterpret_cast<float4*>(k_s + j * S + d) = k;
             *reinterpret_cast<float4*>(v_s + j * S + d) = v;
@@ -228,9 +191,51 @@ paged_attention_kernel(PagedAttnArgs A) {
     }
 }
 
+// A row of the step in fp32 over all its tokens, by a warp: a lane per token of 32, then per four of
+// up to 128 channels.
+__device__ void row_in_fp32(const PagedAttnArgs& A, const PagedSeq& q, int h, int row, int inside, int lane) {
+    const int n_rep = A.n_rep, D = A.L.head_dim, d = 4 * lane, token = row / n_rep, head = h * n_rep + row % n_rep, last = q.held + token;
+    const bool vec = A.vec != 0;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int t0 = 0; t0 <= last; t0 += 32) {
+        float s = -INFINITY;
+        if (t0 + lane <= last) {
+            s = 0.0f;
+#pragma unroll 1
+            for (int e = 0; e < D; e += 4) {
+                const float4 a = load4_as(A.q, A.q_dtype, (int64_t)q.row0 + token, head, e, vec), b = paged_key4(A, q, h, inside, t0 + lane, e, vec, &g_fault);
+                s = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s))));
+            }
+        }
+        float top = s;
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = exp2f((m - base) * A.scale_log2), w = exp2f((s - base) * A.scale_log2);
+        m = m_new;
+        l = fmaf(l, alpha, w);
+        o.x *= alpha; o.y *= alpha; o.z *= alpha; o.w *= alpha;
+#pragma unroll 1
+        for (int j = 0; j < 32 && t0 + j <= last; ++j) {
+            const float wj = __shfl_sync(0xffffffffu, w, j);
+            if (d >= D) continue;
+            const float4 v = paged_value4(A, q, h, inside, t0 + j, d, vec, &g_fault);
+            o.x = fmaf(wj, v.x, o.x); o.y = fmaf(wj, v.y, o.y); o.z = fmaf(wj, v.z, o.z); o.w = fmaf(wj, v.w, o.w);
+        }
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2) l += __shfl_xor_sync(0xffffffffu, l, x);
+    const float by = 1.0f / l;
+    if (d < D)
+        store_quad(A.out.data, A.out_dtype, ((int64_t)q.row0 + token) * A.out.row_stride + (int64_t)head * A.out.head_stride + d,
+                   make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
+}
+
 // Folds the pieces of a block's rows, a thread per quad of channels of a row.
-// grid = (blocks, KV heads, slices of kFoldRows rows).
-constexpr int kFoldRows = 8;
+// grid = (blocks, KV heads, slices of kFoldRows rows, fewer where nothing is folded).
+constexpr int kFoldRows = 8;                             // (a warp each where they are computed anew)
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(PagedAttnArgs A, int RT) {
     __shared__ int place_s[2];
@@ -254,6 +259,15 @@ paged_merge_kernel(PagedAttnArgs A, int RT) {
     const int rows = q.n * n_rep, row_first = place_s[1] * RT;
     const int n_rows = rows - row_first < RT ? rows - row_first : RT;
     const int keys = q.held + (row_first + n_rows - 1) / n_rep + 1, n_pieces = (keys + A.chunk - 1) / A.chunk;
+    if (A.rough) {                                       // the tensor cores' rows that those were no good for
+        int any = 0;
+        for (int p = 0; p < n_pieces; ++p) any |= A.rough[((int64_t)blockIdx.x * H + h) * A.pieces + p];
+        if (any) {
+            const int inside = min(quant_of(q.held + q.n, L.group_size, L.residual_cap), q.held);
+            for (int r = blockIdx.z * kFoldRows + (threadIdx.x >> 5); r < n_rows; r += gridDim.z * kFoldRows) row_in_fp32(A, q, h, row_first + r, inside, threadIdx.x & 31);
+            return;
+        }
+    }
     if (n_pieces <= 1) return;
     const int quads = D / 4;
     const int64_t part0 = ((int64_t)blockIdx.x * H + h) * A.pieces;
@@ -368,7 +382,8 @@ static int check_attention(const kivi_paged_layer* L, const kivi_paged_batch* b,
 }
 
 static size_t plan_bytes(const kivi_paged_layer* L, const PagedPlan& p) {
-    return p.pieces > 1 || p.kernel == PagedKernel::kDecode ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
+    const size_t parts = (size_t)p.blocks * L->num_kv_heads * p.pieces;
+    return (p.pieces > 1 || p.kernel == PagedKernel::kDecode ? parts * p.rows * (L->head_dim + 2) * 4 : 0) + (p.kernel == PagedKernel::kTensor ? parts * 4 : 0);
 }
 
 // (enough for rows on 16-byte boundaries, and for others, which the decode kernel does not take)
@@ -421,12 +436,15 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     }
     if (p.kernel == PagedKernel::kTensor) {
         a.vec = vec16;
+        a.rough = reinterpret_cast<int*>(static_cast<char*>(workspace) + need) - (size_t)p.blocks * L->num_kv_heads * p.pieces;
         rc = run_paged_tc(a, p.blocks, st);
     } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);
     if (rc) return rc;
-    if (p.pieces > 1) {
-        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)((p.rows + kFoldRows - 1) / kFoldRows)), 256, 0, st, true, a, p.rows));
+    if (p.pieces > 1 || a.rough) {
+        // (one piece: the kernel only looks for rows to compute anew)
+        const int slices = p.pieces > 1 ? (p.rows + kFoldRows - 1) / kFoldRows : 4;
+        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)slices), 256, 0, st, true, a, p.rows));
         note_launches(2);
     } else {
         note_launches(1);

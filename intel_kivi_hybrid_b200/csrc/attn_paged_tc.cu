@@ -24,8 +24,11 @@
 // within 2^-27 of it keeps 11 bits: the dequantized numbers and the weights are rounded at
 // 2^-12, a window's bf16 numbers not at all.  bf16 operands would round at 2^-9, which is what the
 // output itself is rounded at (measured: error 1.0 of the output's own rounding, not 2).
-// Sums, maxima and O are fp32.  A row that sees a value that is not finite comes out as NaN; one
-// that does not see it is not touched by it.
+// Sums, maxima and O are fp32.  One power of two for all the tokens of a tile is no good where a row
+// does not see, or gives no weight to, a token that is far larger than the others: the rows of a CTA
+// that has met a value of 2^16 or more, an infinity or a NaN are computed on the CUDA cores in fp32
+// by the kernel that folds the pieces (a row at a time, some fifty times slower; the same code in
+// this kernel cost every call 8 %).  Below that, other tokens are exact to 2^-22.
 //
 // Codes to fp16: a 2-bit field and the exponent of 1024 make the number 1024 + c 4^n, of
 // which 1024 is taken off exactly; c 4^n (s / 4^n) + z is one fused operation for two
@@ -133,6 +136,7 @@ constexpr uint32_t k1024 = 0x64006400u, kMinus1024 = 0xe400e400u;
 // The power of two that takes a largest magnitude (its bits) to 2^13 .. 2^14, kept where
 // it and its inverse are normal numbers; nothing (or infinity) is left as it is.
 __device__ __forceinline__ int exponent_of(uint32_t bits) { return (int)(bits >> 23); }
+constexpr int kRough = 127 + 16;                         // (biased exponent)
 __device__ __forceinline__ int shift_of(int e) {         // biased exponent -> power to multiply with
     if (e == 0 || e == 255) return 0;
     const int s = 127 + 13 - e;
@@ -159,7 +163,7 @@ struct Misc {                                            // behind the tiles
     uint32_t tmem;
     int place[2];
     int k_top[kRing], v_top[kRing];                      // biased exponents of tile j's largest at j % kRing
-    uint32_t odd[kRing][4];                              // tokens of the tile whose values are not all finite
+    int rough;                                           // a value has been met that the tiles' operands are no good for
     uint32_t top[2][2][kTileWarps];                      // [tile parity][K, V][warp]
     __nv_bfloat16 row_top[2][2][kM];                     // [block][half of the columns][row]
 };
@@ -198,14 +202,15 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
 // codes stand for lies between.
 template <int D>
 __device__ __forceinline__ uint32_t group_top(uint32_t factors, int lane) {
-    float top = 0.0f;
+    uint32_t top = 0u;                                   // (as bits: a NaN is the largest)
+    auto bits = [](float x) { return __float_as_uint(fabsf(x)); };
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
         const float2 s = lds_float2(factors + Shared<D>::raw_s + (64 * i + 2 * lane) * 4), z = lds_float2(factors + Shared<D>::raw_z + (64 * i + 2 * lane) * 4);
-        top = fmaxf(top, fmaxf(fabsf(z.x), fabsf(fmaf(3.0f, s.x, z.x))));
-        top = fmaxf(top, fmaxf(fabsf(z.y), fabsf(fmaf(3.0f, s.y, z.y))));
+        top = max(top, max(bits(z.x), bits(fmaf(3.0f, s.x, z.x))));
+        top = max(top, max(bits(z.y), bits(fmaf(3.0f, s.y, z.y))));
     }
-    return __float_as_uint(top);
+    return top;
 }
 // columns from `seen` on count for nothing
 __device__ __forceinline__ void hide(uint32_t (&v)[32], int seen) {
@@ -241,7 +246,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             load_seq(L, A.b, i, q);
             return (int)(((int64_t)q.n * n_rep + 2 * kM - 1) / (2 * kM));
         });
-        if (lane == 0) { misc.place[0] = p.s; misc.place[1] = p.sub; }
+        if (lane == 0) { misc.place[0] = p.s; misc.place[1] = p.sub; misc.rough = 0; }
     }
     __syncthreads();
     const int s = misc.place[0];
@@ -391,15 +396,6 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     }
                 }
                 v_shift = v_new;
-                if (t0 + kN > inside) {                              // a tile that holds rows as they are: whose values are not finite comes with V
-                    if (ok) ok = wait_warp(misc.full[1][j & 1], j >> 1);
-                    const uint32_t* odd = misc.odd[j % kRing];
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int in_word = min(max(seen - 32 * w, 0), 32);
-                        if (odd[w] & (in_word >= 32 ? 0xffffffffu : (1u << in_word) - 1u)) l = __uint_as_float(0x7fc00000u);
-                    }
-                }
                 const float base_m = m == -INFINITY ? 0.0f : m;
                 float2 sum = make_float2(0.0f, 0.0f);
                 // Weights: columns 0 .. 63 become columns 0 .. 31, 64 .. 127 become 64 .. 95.
@@ -431,6 +427,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 sums[half * kM + r] = l;
                 asm volatile("bar.sync %0, %1;" ::"r"(3 + t), "n"(2 * kM) : "memory");
                 l += sums[(half ^ 1) * kM + r];
+                const bool rough = *const_cast<volatile int*>(&misc.rough) != 0;         // (computed elsewhere, and `out` may be `q`)
                 const float f = pow2i(-v_shift);
                 const float by = whole ? f / l : f;
                 const int64_t at = ((int64_t)q.row0 + token) * A.out.row_stride + (int64_t)head * A.out.head_stride;
@@ -440,7 +437,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     uint32_t o[16];
                     tmem_load16(o_at + x, o);
                     tmem_wait_load();
-                    if (!there) continue;
+                    if (!there || rough) continue;
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
                         const float4 y = make_float4(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by, __uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
@@ -448,7 +445,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                         else *reinterpret_cast<float4*>(A.part_o + part * D + x + i) = y;
                     }
                 }
-                if (!whole && there && half == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m, l);
+                if (!whole && there && !rough && half == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m, l);
                 fence_before();
             }
         }
@@ -479,7 +476,6 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         auto top8 = [&](const uint4& x) {                            // largest magnitudes of the even and the odd channels, as bf16 bits
             return __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
         };
-        auto any_odd = [&](uint32_t top) { return (top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u; };
         auto place = [&](uint32_t to, int hw, int r) { return to + hw * (kN * 128) + r * 128 + ((p8 ^ (r & 7)) << 4); };
 
         // Keys of a packed group.  (c, m) = lane & 7: channels 64 hw + 16 c + 8 m .. + 7, which are two
@@ -572,7 +568,6 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             const uint32_t to = base + (of_keys ? S::k : S::v) + st * S::kTileBytes + (uint32_t)(G * g) * 128u;
             // (given up: on to the end without waiting, the other warps wait at the barrier below)
             int e_top;
-            uint32_t odd = 0u;
             if (tile0 + kN - G < inside) {                           // four packed groups: the power of two is known
                 if (ok) ok = wait_warp(misc.ready[x_][st], j >> 1);
                 e_top = (of_keys ? misc.k_top : misc.v_top)[j % kRing];
@@ -597,21 +592,6 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                             sts128(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)), x[e].x, x[e].y, x[e].z, x[e].w);
                         }
                     }
-                    if (any_odd(pair)) {                             // the largest finite one, and whose rows are not
-                        pair = 0u;
-#pragma unroll 1
-                        for (int i = 0; i < 8 * (D / 64); ++i) {
-                            const int r = sub + 4 * (i & 7);
-                            const uint4 x = lds_uint4(place(to, i >> 3, r));
-                            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t lo = w[e] & 0x7fffu, hi = (w[e] >> 16) & 0x7fffu;
-                                if (lo >= 0x7f80u || hi >= 0x7f80u) odd |= 1u << r;
-                                pair = __vmaxu2(pair, (lo < 0x7f80u ? lo : 0u) | (hi < 0x7f80u ? hi << 16 : 0u));
-                            }
-                        }
-                    }
                     top = max(pair << 16, pair & 0xffff0000u);
                 }
                 top = __reduce_max_sync(0xffffffffu, top);
@@ -621,6 +601,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 if (!of_keys) e_top = max(e_top, v_top);
                 if (g == 0 && lane == 0) {
                     (of_keys ? misc.k_top : misc.v_top)[j % kRing] = e_top;
+                    if (e_top >= kRough) misc.rough = 1;
                     if (!of_keys) arrive(bar(misc.v_known[j % 4]));
                 }
             }
@@ -637,7 +618,8 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                         const int r = sub + 4 * (i & 7);
                         if (t0 + r < inside) continue;
                         uint4 x = row8(t0 + r, 64 * (i >> 3) + 8 * p8);
-                        if (!of_keys && any_odd(top8(x))) { odd |= 1u << r; x = make_uint4(0u, 0u, 0u, 0u); }
+                        const uint32_t pair = top8(x);               // (what the page stands for is as large, or the rows are not those appended)
+                        if (exponent_of(max(pair << 16, pair & 0xffff0000u)) > e_top + 1) misc.rough = 1;
                         x = half8(x, f);
                         sts128(place(to, i >> 3, r), x.x, x.y, x.z, x.w);
                     }
@@ -650,15 +632,10 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     for (int e = 0; e < 4; ++e) x[e] = lds_uint4(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if (!of_keys && any_odd(top8(x[e]))) x[e] = make_uint4(0u, 0u, 0u, 0u);      // (the rows that see it are told by `odd`)
                         x[e] = half8(x[e], f);
                         sts128(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)), x[e].x, x[e].y, x[e].z, x[e].w);
                     }
                 }
-            }
-            if (!of_keys) {
-                odd = __reduce_or_sync(0xffffffffu, odd);
-                if (lane == 0) misc.odd[j % kRing][g] = odd;
             }
             fence_async();
             __syncwarp();
@@ -684,6 +661,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 if (x) top = v_top = max(v_top, top);
                 if (lane == 0) {
                     (x ? misc.v_top : misc.k_top)[j % kRing] = exponent_of(top);
+                    if (exponent_of(top) >= kRough) misc.rough = 1;
                     arrive(bar(misc.ready[x][j & 1]));
                     if (x) arrive(bar(misc.v_known[j % 4]));
                 }
@@ -771,6 +749,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     __syncthreads();
     fence_after();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (tid == 0) A.rough[((int64_t)item * H + h) * A.pieces + blockIdx.z] = misc.rough;
 }
 
 }  // namespace

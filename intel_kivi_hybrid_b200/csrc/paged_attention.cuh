@@ -13,13 +13,58 @@ struct PagedAttnArgs {
     float scale_log2;
     int pieces, chunk;           // a block's tokens are cut into pieces of `chunk` (no block has more than `pieces`)
     float *part_o, *part_ml;     // [block][KV head][piece][row]: unnormalised output, (maximum, sum)
+    int* rough;                  // [block][KV head][piece], or null: rows to be computed in fp32 after all
 };
 
 #ifdef __CUDACC__
 __device__ __forceinline__ void settle_args(PagedAttnArgs& a) {
     settle_paged(a.L, a.b);
     a.q.data = settled(a.q.data); a.k.data = settled(a.k.data); a.v.data = settled(a.v.data);
-    a.part_o = settled(a.part_o); a.part_ml = settled(a.part_ml);
+    a.part_o = settled(a.part_o); a.part_ml = settled(a.part_ml); a.rough = settled(a.rough);
+}
+template <typename T> __device__ __forceinline__ float4 load4(const T* p, bool vec);
+template <> __device__ __forceinline__ float4 load4<float>(const float* p, bool vec) {
+    return vec ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+}
+template <> __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p, bool vec) {
+    if (!vec) return make_float4(__bfloat162float(p[0]), __bfloat162float(p[1]), __bfloat162float(p[2]), __bfloat162float(p[3]));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 load4_as(const kivi_rows& r, int dtype, int64_t row, int head, int d, bool vec) {
+    const int64_t at = row * r.row_stride + (int64_t)head * r.head_stride + d;
+    return dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(r.data) + at, vec) : load4(reinterpret_cast<const float*>(r.data) + at, vec);
+}
+
+// Four channels of token t's key (value) as it is served: from its page before `inside`, from the
+// window before `held`, else the step's own row.
+__device__ __forceinline__ float4 paged_row4(const PagedAttnArgs& A, const PagedSeq& q, const void* ring, const kivi_rows& fresh, int h, int t, int d, bool vec) {
+    const kivi_paged_layer& L = A.L;
+    if (t >= q.held) return load4_as(fresh, L.res_dtype, (int64_t)q.row0 + (t - q.held), h, d, vec);
+    const int64_t at = (((int64_t)q.slot * L.num_kv_heads + h) * L.residual_cap + ring_slot(t, A.b.ring_shift, L.residual_cap)) * L.head_dim + d;
+    return L.res_dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(ring) + at, true) : load4(reinterpret_cast<const float*>(ring) + at, true);
+}
+__device__ __forceinline__ float4 paged_key4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
+    const kivi_paged_layer& L = A.L;
+    if (t >= inside) return paged_row4(A, q, L.k_res, A.k, h, t, d, vec);
+    const int D = L.head_dim, G = L.group_size, Q = G / 4;
+    const int64_t g = ((int64_t)page_of(L, q, t, fault) * L.num_kv_heads + h) * (L.page_tokens / G) + t % L.page_tokens / G;
+    const int tt = t % G, sh = 2 * (tt & 3);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(L.k_codes + g * (D * Q) + kblock_offset(d, tt >> 2, Q, D < 64 ? D : 64));
+    const float4 s = *reinterpret_cast<const float4*>(L.k_scales + g * D + d), z = *reinterpret_cast<const float4*>(L.k_zeros + g * D + d);
+    return make_float4(fmaf((float)((w >> sh) & 3u), s.x, z.x), fmaf((float)((w >> (sh + 8)) & 3u), s.y, z.y),
+                       fmaf((float)((w >> (sh + 16)) & 3u), s.z, z.z), fmaf((float)((w >> (sh + 24)) & 3u), s.w, z.w));
+}
+__device__ __forceinline__ float4 paged_value4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
+    const kivi_paged_layer& L = A.L;
+    if (t >= inside) return paged_row4(A, q, L.v_res, A.v, h, t, d, vec);
+    const int D = L.head_dim, G = L.group_size;
+    const int64_t g = ((int64_t)page_of(L, q, t, fault) * L.num_kv_heads + h) * (L.page_tokens / G) + t % L.page_tokens / G;
+    const int tt = t % G;
+    const uint32_t c = L.v_codes[g * (D * (G / 4)) + vcode_offset(tt, d / 4, D, G)];
+    const int64_t at = g * D + vmeta_index(tt, d / G, D, G);
+    const float s = L.v_scales[at], z = L.v_zeros[at];
+    return make_float4(fmaf((float)(c & 3u), s, z), fmaf((float)((c >> 2) & 3u), s, z), fmaf((float)((c >> 4) & 3u), s, z), fmaf((float)(c >> 6), s, z));
 }
 #endif
 

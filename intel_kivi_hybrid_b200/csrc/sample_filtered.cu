@@ -502,7 +502,7 @@ extern "C" int kivi_sample_filtered(const void* logits, int dtype, int batch, in
                                     const float* top_p, const float* min_p, int64_t* ids_out, void* stream) {
     KIVI_REQUIRE(logits != nullptr && uniforms != nullptr && ids_out != nullptr, "logits, uniforms or ids_out is null");
     KIVI_REQUIRE(dtype == KIVI_F32 || dtype == KIVI_BF16, "logits dtype must be KIVI_F32 or KIVI_BF16");
-    KIVI_REQUIRE(batch > 0 && vocab > 0 && row_stride >= vocab, "batch (%d), vocab (%d) and row_stride must be positive, row_stride >= vocab", batch, vocab);
+    KIVI_REQUIRE(batch > 0 && vocab > 0 && (row_stride >= vocab || row_stride == 0), "batch (%d) and vocab (%d) must be positive, row_stride >= vocab or 0", batch, vocab);
     // (indices step past the end of a row)
     KIVI_REQUIRE(vocab <= (1 << 30), "vocab (%d) must be at most 2^30", vocab);
     const FilterArgs f{uniforms, temperature, top_p, min_p, top_k};

@@ -543,7 +543,8 @@ torch::Tensor sample_filtered(const torch::Tensor& logits, const torch::Tensor& 
     const int dtype = dtype_code(logits, "logits");
     const int64_t B = logits.size(0), V = logits.size(1);
     TORCH_CHECK(B <= kInt32Max && V > 0 && V <= kInt32Max, "batch and vocab must be below 2**31, vocab positive");
-    TORCH_CHECK(B <= 1 || logits.stride(0) >= V, "rows of logits overlap");
+    // (0: one row of logits for all draws)
+    TORCH_CHECK(B <= 1 || logits.stride(0) >= V || logits.stride(0) == 0, "rows of logits overlap");
     auto per_row = [&](const torch::Tensor& t, const char* name, torch::ScalarType type) {
         check_paged_tensor(t, name, type, logits.device());
         TORCH_CHECK(t.numel() == B, name, " must hold an entry for each of the ", B, " rows");
@@ -558,7 +559,7 @@ torch::Tensor sample_filtered(const torch::Tensor& logits, const torch::Tensor& 
     c10::cuda::CUDAGuard guard(logits.device());
     const torch::Tensor ids = out.has_value() ? *out : at::empty({B}, logits.options().dtype(torch::kLong));
     if (B == 0) return ids;
-    check(kivi_sample_filtered(logits.data_ptr(), dtype, (int)B, (int)V, std::max<int64_t>(logits.stride(0), V), (const float*)u, (const float*)t, (const int32_t*)k,
+    check(kivi_sample_filtered(logits.data_ptr(), dtype, (int)B, (int)V, B > 1 ? logits.stride(0) : V, (const float*)u, (const float*)t, (const int32_t*)k,
                                (const float*)tp, (const float*)mp, ids.data_ptr<int64_t>(), stream_of(logits)));
     return ids;
 }

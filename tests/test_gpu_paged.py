@@ -295,3 +295,242 @@ def test_attention_at_the_edges_of_windows_and_tiles(ops, dtype, held, new):
         pool.append(ops, K[0][:held], V[0][:held], [held])
         pool.lens = [held]
     check_attention(ops, pool, K, V, [new], n_rep, dtype, torch.float32, 7, scale=0.11, operand=2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -24)
+
+
+# ---- what a row must not see, arrays that lie, layouts, streams, graphs ----------------------
+
+KERNELS = [  # D, G, n_rep, new, dtype: decode, tensor cores, CUDA cores
+    (128, 32, 2, 4, torch.bfloat16), (128, 32, 4, 200, torch.bfloat16), (64, 32, 4, 200, torch.bfloat16), (128, 32, 1, 5, torch.float32), (64, 32, 3, 70, torch.float32),
+    (128, 64, 2, 33, torch.bfloat16)]
+
+
+def attend(ops, pool, q, k, v, news, arrays, out=None, max_len=None, **kw):
+    out = torch.empty_like(q) if out is None else out
+    ops.paged_attention(q, k, v, *pool.t, *arrays, max(news), max_len or max(h + n for h, n in zip(pool.lens, news)), out, pool.G, **kw)
+    return out
+
+
+@pytest.mark.parametrize("D,G,n_rep,new,dtype", KERNELS)
+def test_rows_are_not_touched_by_tokens_they_do_not_see(ops, D, G, n_rep, new, dtype):
+    """NaN, infinities and the lowest value in a later token of the step: earlier rows come out as without."""
+    H, R, held = 2, 128, 300
+    results = []
+    for poison in (None, float("nan"), float("inf"), torch.finfo(dtype).min):
+        pool = Pool(1, H, D, G, R, 2 * G, held + new, dtype)
+        k, v = rows(held + new, H, D, dtype, 1), rows(held + new, H, D, dtype, 2)
+        q = rows(new, H * n_rep, D, dtype, 3)
+        pool.append(ops, k[:held], v[:held], [held])
+        pool.lens = [held]
+        nk, nv = k[held:].clone(), v[held:].clone()
+        a = pool.append(ops, nk, nv, [new])                  # (the packed groups stay the same)
+        bad = new // 2 + 1
+        if poison is not None:
+            nk[bad, :, 3], nv[bad, :, 5], nk[-1], nv[-1] = poison, poison, poison, poison
+        results.append(attend(ops, pool, q, nk, nv, [new], a))
+        if dtype == torch.bfloat16 and G == 32 and new * n_rep > 12:
+            # tensor cores: rows that share a CTA with such a value are computed in fp32 instead, apart by both bounds (see check_attention)
+            e = float(q.float().abs().sum(-1).max()) * 12.0 * D ** -0.5 * ((D + 4) * 2.0 ** -24 + 2 * 2.0 ** -11)
+            bound = 2 * (2 * e + (held + new + 8) * 2.0 ** -24 + 2 * 2.0 ** -11) * 12.0 + results[0][:bad].float().abs() * torch.finfo(dtype).eps
+            assert ((results[-1][:bad].float() - results[0][:bad].float()).abs() <= bound).all(), poison
+        else:
+            assert torch.equal(results[0][:bad], results[-1][:bad]), poison
+        if poison is not None and not math.isfinite(poison):
+            assert not torch.isfinite(results[-1][bad:]).all(-1).any()
+
+
+@pytest.mark.parametrize("D,G,n_rep,new,dtype", KERNELS)
+def test_arrays_that_point_outside_are_reported_and_left_out(ops, D, G, n_rep, new, dtype):
+    from intel_kivi_hybrid_b200 import cabi
+    H, R, held = 2, 64, 200
+    pool = Pool(3, H, D, G, R, 2 * G, held + new, dtype)
+    k, v = rows(3 * held, H, D, dtype, 1), rows(3 * held, H, D, dtype, 2)
+    pool.append(ops, k, v, [held] * 3)
+    pool.lens = [held] * 3
+    nk, nv, q = rows(3 * new, H, D, dtype, 3), rows(3 * new, H, D, dtype, 4), rows(3 * new, H * n_rep, D, dtype, 5)
+    good = pool.append(ops, nk, nv, [new] * 3)
+    want = attend(ops, pool, q, nk, nv, [new] * 3, good)
+    assert cabi.device_fault() == 0
+    saved = [t.clone() for t in pool.t]
+    for which, value in ((1, 99), (1, -1), (2, -5), (2, 10 ** 6), (3, 10 ** 6), (3, -1)):
+        arrays = [x.clone() for x in good]
+        arrays[which][2 if which == 3 else 1] = value
+        out = torch.full_like(q, 9.0)
+        attend(ops, pool, q, nk, nv, [new] * 3, arrays, out)
+        assert cabi.device_fault() == 4
+        cabi.device_fault_clear()
+        assert torch.equal(out[:new], want[:new]) and (out[new:2 * new] == 9.0).all()
+        ops.paged_append(nk, nv, *pool.t, *arrays, new, held + new, G)
+        assert cabi.device_fault() == 4
+        cabi.device_fault_clear()
+        for i in (6, 7):                                     # what is left out writes nothing of its own
+            assert torch.equal(pool.t[i][int(good[1][1])], saved[i][int(good[1][1])])
+        for t, s in zip(pool.t, saved):
+            t.copy_(s)
+    table = good[0].clone()
+    table[1, 0] = pool.t[0].shape[0]
+    out = torch.full_like(q, 9.0)
+    attend(ops, pool, q, nk, nv, [new] * 3, [table] + good[1:], out)
+    assert cabi.device_fault() == 4
+    cabi.device_fault_clear()
+    assert torch.equal(out[:new], want[:new]) and torch.equal(out[2 * new:], want[2 * new:])
+
+
+@pytest.mark.parametrize("D,G,n_rep,new,dtype", KERNELS)
+def test_strided_and_unaligned_rows(ops, D, G, n_rep, new, dtype):
+    """Rows of one fused projection, at odd offsets, out rows with gaps: the same as from tensors of their own."""
+    H, R, held = 2, 128, 150
+    pool = Pool(2, H, D, G, R, 2 * G, held + new, dtype)
+    pool.append(ops, rows(2 * held, H, D, dtype, 1), rows(2 * held, H, D, dtype, 2), [held] * 2)
+    pool.lens = [held] * 2
+    n = 2 * new
+    k, v, q = rows(n, H, D, dtype, 3), rows(n, H, D, dtype, 4), rows(n, H * n_rep, D, dtype, 5)
+    a = pool.append(ops, k, v, [new] * 2)
+    want = attend(ops, pool, q, k, v, [new] * 2, a).float()
+    for pad, off in ((8, 0), (8, 8), (3, 1)):
+        wide = torch.zeros(n, H * (n_rep + 2) * D + pad, dtype=dtype, device=DEV)
+        heads = wide[:, off:off + H * (n_rep + 2) * D].unflatten(1, (-1, D))
+        heads[:, :H * n_rep], heads[:, H * n_rep:H * n_rep + H], heads[:, H * n_rep + H:] = q, k, v
+        out = torch.zeros(n, H * n_rep * D + pad, dtype=dtype, device=DEV)
+        view = out[:, off:off + H * n_rep * D].unflatten(1, (-1, D))
+        attend(ops, pool, heads[:, :H * n_rep], heads[:, H * n_rep:H * n_rep + H], heads[:, H * n_rep + H:], [new] * 2, a, view)
+        # rows off 16-byte boundaries may take another kernel: apart by the sum of both bounds (see check_attention;
+        # served values are at most the largest appended one and half a step, 5/6 of the range more)
+        step, top = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -24, 2 * 6.0
+        e = float(q.float().abs().sum(-1).max()) * top * D ** -0.5 * ((D + 4) * 2.0 ** -24 + 2 * step)
+        bound = 2 * (2 * e + (held + new + 8) * 2.0 ** -24 + 2 * step) * top + want.abs() * torch.finfo(dtype).eps
+        assert ((view.float() - want).abs() <= bound).all()
+        assert out.flatten().count_nonzero() <= n * H * n_rep * D
+
+
+@pytest.mark.parametrize("D,G,n_rep,new,dtype", KERNELS)
+def test_another_stream_and_a_captured_step(ops, D, G, n_rep, new, dtype):
+    """A step on a side stream, two captured steps that replay in turn, lengths that change between replays."""
+    H, R = 2, 64
+    start = [40, 130, 0]
+    total = 40 + 130 + 3 * new * 6 + 200
+    K, V = rows(total, H, D, dtype, 1), rows(total, H, D, dtype, 2)
+    def run(graph):
+        pool = Pool(3, H, D, G, R, 2 * G, 130 + new * 8, dtype, seed=7)
+        pool.append(ops, K[:170], V[:170], start)
+        pool.lens = list(start)
+        k, v, q = torch.empty(3 * new, H, D, dtype=dtype, device=DEV), torch.empty(3 * new, H, D, dtype=dtype, device=DEV), torch.empty(3 * new, H * n_rep, D, dtype=dtype, device=DEV)
+        a, out, out2 = pool.arrays([new] * 3), torch.empty_like(q), torch.empty_like(q)
+        limit = 130 + new * 8
+
+        def step(o):
+            ops.paged_append(k, v, *pool.t, *a, new, limit, G)
+            ops.paged_attention(q, k, v, *pool.t, *a, new, limit, o, G)
+        graphs = []
+        if graph:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            for t in (k, v, q):
+                t.zero_()
+            saved = [t.clone() for t in pool.t]
+            with torch.cuda.stream(side):
+                step(out)                                    # off the default stream, nothing captured
+            torch.cuda.current_stream().wait_stream(side)
+            for o in (out, out2):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    step(o)
+                graphs.append(g)
+            for t, s in zip(pool.t, saved):
+                t.copy_(s)
+        got = []
+        for i in range(6):
+            at = 170 + 3 * new * i
+            k.copy_(K[at:at + 3 * new]); v.copy_(V[at:at + 3 * new]); q.copy_(rows(3 * new, H * n_rep, D, dtype, 50 + i))
+            a[2].copy_(torch.tensor(pool.lens, dtype=torch.int32))
+            o = (out, out2)[i % 2]
+            graphs[i % 2].replay() if graph else step(o)
+            pool.lens = [n + new for n in pool.lens]
+            got.append(o.clone())
+        return got, pool.t
+    plain, pools = run(False)
+    replayed, pools2 = run(True)
+    for x, y in zip(plain, replayed):
+        assert torch.equal(x, y)
+    for x, y in zip(pools, pools2):
+        assert torch.equal(x, y)
+
+
+def test_refusals(ops):
+    D, G, R, H = 128, 32, 64, 2
+    pool = Pool(2, H, D, G, R, 64, 300, torch.bfloat16)
+    k = rows(10, H, D, torch.bfloat16, 1)
+    q = rows(10, 4, D, torch.bfloat16, 2)
+    a = pool.arrays([5, 5])
+    out, rot = torch.empty_like(q), torch.randn(300, D, device=DEV)
+    t = pool.t
+    att = lambda q=q, k=k, v=k, t=t, a=a, mn=5, ml=5, out=out, G=G, **kw: ops.paged_attention(q, k, v, *t, *a, mn, ml, out, G, **kw)  # noqa: E731
+    app = lambda k=k, v=k, t=t, a=a, mn=5, ml=5, G=G, **kw: ops.paged_append(k, v, *t, *a, mn, ml, G, **kw)  # noqa: E731
+    sub = lambda x, i, y: x[:i] + [y] + x[i + 1:]  # noqa: E731
+    for bad, what in (
+            (lambda: att(q=q.float()[:, :3]), "n_rep"), (lambda: att(q=q.half()), "Float or BFloat16"), (lambda: att(k=k.float()), "like the cache's window"),
+            (lambda: att(q=q[:9]), "must be"), (lambda: att(out=out[:, :, ::2]), "must be"), (lambda: att(out=out.as_strided(out.shape, (D, D, 1))), "overlap"),
+            (lambda: att(q=q.cpu()), "on cuda"), (lambda: att(t=sub(t, 0, t[0].cpu())), "same device"), (lambda: att(t=sub(t, 1, t[1].half())), "must be Float"),
+            (lambda: att(t=sub(t, 1, t[1][:, :1])), "must be"), (lambda: att(t=sub(t, 0, t[0][:2])), "must"), (lambda: att(G=30), "divisible by 4"), (lambda: att(G=48), "divisible by group_size"),
+            (lambda: att(a=sub(a, 0, a[0].long())), "must be Int"), (lambda: att(a=sub(a, 1, a[1][:1])), "must hold"), (lambda: att(a=sub(a, 3, a[3][:2])), "must hold"),
+            (lambda: att(mn=11), "max_new"), (lambda: att(mn=-1), "outside"), (lambda: att(ml=4), "max_len"), (lambda: att(ml=10 ** 6), "page table"), (lambda: att(ring_shift=R), "ring_shift"),
+            (lambda: app(v=k.float()), "like the cache's window"), (lambda: app(rotary=rot), "together"), (lambda: app(q=q, q_out=q), "only with rotary"),
+            (lambda: app(rotary=rot[:4], k_out=k), "positions"), (lambda: app(rotary=rot[:, :130 - 2 * 63 + 1], k_out=k), "even|contiguous"), (lambda: app(rotary=rot[:, :12].contiguous(), k_out=k), "multiple of 8"),
+            (lambda: app(rotary=rot.half(), k_out=k), "must be Float"), (lambda: app(rotary=torch.randn(300, 256, device=DEV), k_out=k), "at most head_dim"),
+            (lambda: app(rotary=rot, k_out=k, q=q, q_out=q.float()), "like the cache's window"), (lambda: app(rounding=7), "rounding"),
+            (lambda: ops.paged_read(*t, *a[:3], a[2][:1], a[3], 5, torch.empty(10, H, D, device=DEV), torch.empty(10, H, D, device=DEV), G), "starts"),
+            (lambda: ops.paged_read(*t, *a[:3], a[2], a[3], 5, torch.empty(10, H, D, device=DEV, dtype=torch.bfloat16), torch.empty(10, H, D, device=DEV), G), "must be Float")):
+        with pytest.raises(RuntimeError, match=what):
+            bad()
+
+
+@pytest.mark.parametrize("D,n_rep,held,new", [(128, 4, 300, 70), (64, 2, 0, 150), (128, 1, 5000, 40)])
+@pytest.mark.parametrize("size", [2.0 ** 15, 2.0 ** 17, 2.0 ** 60, 3.0e38])
+def test_tokens_of_any_size_among_others(ops, D, n_rep, held, new, size):
+    """Tensor cores: a value of a token with hardly any weight is huge; rows before it, and the other channels of rows
+    behind it, are as exact as without it."""
+    G, R, H = 32, 128, 2
+    pool = Pool(1, H, D, G, R, 2 * G, held + new, torch.bfloat16)
+    K, V = rows(held + new, H, D, torch.bfloat16, 1), rows(held + new, H, D, torch.bfloat16, 2)
+    q = rows(new, H * n_rep, D, torch.bfloat16, 3)
+    if held:
+        pool.append(ops, K[:held], V[:held], [held])
+        pool.lens = [held]
+    nk, nv = K[held:], V[held:]
+    a = pool.append(ops, nk, nv, [new])
+    nv[new // 2, :, 7] = size
+    got = attend(ops, pool, q, nk, nv, [new], a).double()
+    pool.lens = [held + new]
+    k, v = (x[0].double() for x in pool.read(ops, [0], [held + new]))
+    k[held:], v[held:] = nk.double(), nv.double()
+    step = 2.0 ** -11
+    for i in range(H * n_rep):
+        s = (q[:, i].double() @ k[:, i // n_rep].t()) * D ** -0.5
+        s.masked_fill_(torch.arange(held + new, device=DEV) > held + torch.arange(new, device=DEV)[:, None], -math.inf)
+        want = torch.softmax(s, 1) @ v[:, i // n_rep]
+        e = float((q[:, i].double().abs() @ k[:, i // n_rep].abs().t()).amax()) * D ** -0.5
+        # (as in check_attention; each channel by its own largest)
+        bound = (2 * e * (2 * step + (D + 4) * 2.0 ** -24) + 2 * step + (held + new + 8) * 2.0 ** -24) * v[:, i // n_rep].abs().amax(0) + want.abs() * torch.finfo(torch.bfloat16).eps / 2
+        assert ((got[:, i] - want).abs() <= bound)[torch.isfinite(want.to(torch.bfloat16))].all()
+    half = new // 2
+    clean = attend(ops, pool_before(pool, held), q[:half], nk[:half], nv[:half], [half], [a[0], a[1], a[2], torch.tensor([0, half], dtype=torch.int32, device=DEV)], max_len=held + new)
+    e = float(q.float().abs().sum(-1).max()) * 12.0 * D ** -0.5 * ((D + 4) * 2.0 ** -24 + 2 * step)
+    assert (got[:half] - clean.double()).abs().max() <= 2 * (2 * e + (held + new + 8) * 2.0 ** -24 + 2 * step) * 12.0 + 6.0 * torch.finfo(torch.bfloat16).eps
+
+
+def pool_before(pool, held):
+    pool.lens = [held]
+    return pool
+
+
+@pytest.mark.parametrize("D,G,n_rep,new,dtype", KERNELS)
+def test_out_may_be_q(ops, D, G, n_rep, new, dtype):
+    H, R, held = 2, 64, 700
+    pool = Pool(2, H, D, G, R, 2 * G, held + new, dtype)
+    pool.append(ops, rows(2 * held, H, D, dtype, 1), rows(2 * held, H, D, dtype, 2), [held] * 2)
+    pool.lens = [held] * 2
+    k, v, q = rows(2 * new, H, D, dtype, 3), rows(2 * new, H, D, dtype, 4), rows(2 * new, H * n_rep, D, dtype, 5)
+    a = pool.append(ops, k, v, [new] * 2)
+    v[new + new // 2, 1, 3] = float("inf")
+    want = attend(ops, pool, q, k, v, [new] * 2, a)
+    attend(ops, pool, q, k, v, [new] * 2, a, out=q)
+    assert torch.equal(torch.nan_to_num(q, 1.0), torch.nan_to_num(want, 1.0)) and torch.equal(torch.isfinite(q), torch.isfinite(want))

@@ -1,0 +1,118 @@
+"""Paged cache and filtered sampling without a GPU: struct layouts, refusals of the C interface, pages and lengths."""
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def cabi():
+    from intel_kivi_hybrid_b200 import cabi
+    return cabi
+
+
+def test_struct_sizes_match_the_header(cabi):
+    assert ctypes.sizeof(cabi.PagedLayer) == 8 * 4 + 8 * 8
+    assert ctypes.sizeof(cabi.PagedBatch) == 2 * 4 + 4 * 8 + 4 * 4
+    assert ctypes.sizeof(cabi.Rows) == 24
+
+
+def test_a_length_alone_says_what_is_in_pages(cabi):
+    """quantized(t) is where kivi_cache_plan leads, in whatever pieces the tokens come."""
+    from kivi_cuda import PagedKiviCache
+    for G, R in ((4, 4), (4, 9), (32, 32), (32, 100), (32, 128), (64, 200)):
+        cache = PagedKiviCache(1, 64, 1, 4, 1, page_tokens=G, group_size=G, residual_length=R, device="cpu")
+        for pieces in ((1,) * 300, (7, 100, 1, 1, 50, 3), (500,), (R - 1, 1, G, G - 1, 1)):
+            quant = res = 0
+            for n in pieces:
+                _, quant, res = cabi.cache_plan(quant, res, n, G, R)
+                assert quant == cache.quantized(quant + res)
+
+
+def test_pages_are_taken_given_back_and_run_out():
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(2, 64, 2, num_pages=6, max_sequences=2, page_tokens=64, group_size=32, residual_length=64, device="cpu")
+    a, b = cache.add_sequence(), cache.add_sequence()
+    with pytest.raises(RuntimeError, match="sequences are taken"):
+        cache.add_sequence()
+    batch = cache.begin([a, b], [200, 0])
+    assert cache.quantized(200) == 160 and cache.free_pages == 3
+    assert batch.page_table.tolist()[1] == [-1, -1, -1] and len(set(batch.page_table.tolist()[0])) == 3
+    assert batch.cu_new.tolist() == [0, 200, 200] and batch.seq_lens.tolist() == [0, 0] and (batch.max_new, batch.max_len, batch.rows) == (200, 200, 200)
+    cache.end(batch)
+    with pytest.raises(AssertionError, match="has ended"):
+        cache.end(batch)
+    assert cache.length(a) == 200 and cache.length(b) == 0
+    with pytest.raises(RuntimeError, match="pages are needed"):
+        cache.begin([b], [500])
+    assert cache.free_pages == 3                            # a refused step takes nothing
+    cache.free(a)
+    assert cache.free_pages == 6
+    c = cache.add_sequence()
+    batch = cache.begin([c], [1], max_len=300)
+    assert batch.page_table.shape == (1, 4)
+    cache.end(batch)
+    cache.refresh(batch)
+    assert batch.seq_lens.tolist() == [1] and batch.open
+    for bad, what in ((lambda: cache.begin([c, c], [1, 1]), "twice"), (lambda: cache.begin([9], [1]), "not there"), (lambda: cache.begin([c], [-1]), "negative"),
+                      (lambda: cache.begin([], []), "at least one"), (lambda: cache.begin([c], [5], max_len=3), "below"), (lambda: cache.read(0, c, 0, 99), "tokens 0")):
+        with pytest.raises(AssertionError, match=what):
+            bad()
+    for args, what in (((1, 48, 1, 1, 1), "divisible by group_size"), ((1, 64, 1, 1, 1, 48), "page_tokens"), ((1, 320, 1, 1, 1), "up to 256")):
+        with pytest.raises(AssertionError, match=what):
+            PagedKiviCache(*args)
+
+
+def test_the_c_interface_refuses_before_it_launches(cabi):
+    lib, byref = cabi.lib, ctypes.byref
+    some = 4096                                             # an address on a 16-byte boundary; nothing follows it
+
+    def layer(**kw):
+        f = dict(num_pages=4, page_tokens=64, num_kv_heads=2, head_dim=128, group_size=32, residual_cap=64, num_slots=2, res_dtype=1,
+                 **{n: some for n in ("k_codes", "k_scales", "k_zeros", "v_codes", "v_scales", "v_zeros", "k_res", "v_res")})
+        return cabi.PagedLayer(**{**f, **kw})
+
+    def batch(**kw):
+        return cabi.PagedBatch(**{**dict(num_seqs=2, table_width=4, page_table=some, slots=some, seq_lens=some, cu_new=some, total_new=8, max_new=4, max_len=100), **kw})
+
+    rows = cabi.Rows(some, 256, 128)
+
+    def call(rc):
+        return rc, lib.kivi_last_error()
+
+    def attention(L=None, b=None, q=rows, k=rows, n_rep=2, dt=1, ws=0, ws_bytes=0):
+        return call(lib.kivi_paged_attention(byref(L or layer()), byref(b or batch()), byref(q), dt, byref(k), byref(k), byref(q), dt, n_rep, 0.0, ws, ws_bytes, None))
+
+    def append(L=None, b=None, k=rows, rot=None, rot_rows=0, dim=0, q=None, rounding=0):
+        return call(lib.kivi_paged_append(byref(L or layer()), byref(b or batch()), byref(k), byref(k), rot, rot_rows, dim, 0, None if q is None else byref(q), 2,
+                                     None if q is None else byref(q), byref(k) if rot else None, rounding, None))
+
+    null = cabi.Rows(None, 0, 0)
+    for (rc, said), what in (
+            (attention(layer(num_pages=0)), b"positive"), (attention(layer(group_size=6)), b"group_size"), (attention(layer(head_dim=100)), b"divisible"), (attention(layer(head_dim=320)), b"up to 256"),
+            (attention(layer(page_tokens=40)), b"page_tokens"), (attention(layer(residual_cap=16)), b"residual_cap"), (attention(layer(res_dtype=5)), b"res_dtype"), (attention(layer(v_zeros=None)), b"null"),
+            (attention(layer(k_codes=some + 8)), b"16-byte"), (attention(b=batch(num_seqs=0)), b"num_seqs"), (attention(b=batch(num_seqs=70000)), b"num_seqs"), (attention(b=batch(page_table=None)), b"null"),
+            (attention(b=batch(max_new=9)), b"max_new"), (attention(b=batch(max_len=3)), b"max_len"), (attention(b=batch(max_len=2 ** 30 + 1)), b"max_len"), (attention(b=batch(max_len=10000)), b"page table"),
+            (attention(b=batch(ring_shift=64)), b"ring_shift"), (attention(b=batch(ring_shift=-1)), b"ring_shift"), (attention(q=null), b"null"), (attention(k=cabi.Rows(some, -1, 128)), b"negative"),
+            (attention(n_rep=0), b"n_rep"), (attention(dt=7), b"dtype"), (attention(), b"workspace too small"), (attention(ws=some + 8, ws_bytes=1 << 40), b"aligned"),
+            (append(k=null), b"null"), (append(rounding=9), b"rounding"), (append(rot=some, rot_rows=50, dim=128), b"positions"), (append(rot=some, rot_rows=500, dim=130), b"at most"),
+            (append(rot=some, rot_rows=500, dim=20), b"multiple of 8"), (append(q=rows), b"together with rotary"),
+            (call(lib.kivi_paged_read(byref(layer()), byref(batch()), None, some, some, None)), b"null"),
+            (call(lib.kivi_sample_filtered(some, 0, 1, 10, 9, some, None, None, None, None, some, None)), b"row_stride"), (call(lib.kivi_sample_filtered(some, 3, 1, 10, 10, some, None, None, None, None, some, None)), b"dtype"),
+            (call(lib.kivi_sample_filtered(some, 0, 1, 10, 10, None, None, None, None, None, some, None)), b"null"), (call(lib.kivi_sample_filtered(some, 0, 1, 2 ** 30 + 1, 2 ** 31, some, None, None, None, None, some, None)), b"2^30")):
+        assert rc == 1 and what in said, (rc, what, said)
+    assert append(layer(head_dim=256, group_size=256, page_tokens=256, residual_cap=256), batch(max_len=10))[0] == 3        # no kernel for groups that large
+    assert attention(b=batch(max_new=0))[0] == 0 and lib.kivi_last_launch_count() == 0
+
+
+def test_sample_token_on_the_host_takes_the_filters():
+    from intel_kivi_hybrid_b200.generation.sampling import sample_token
+    x = torch.tensor([[0.0, 3.0, 3.0, 1.0, -2.0]])
+    assert {int(sample_token(x, 1.0, None, True, 0.4)) for _ in range(200)} == {1, 2}       # ties at the border stay together
+    assert {int(sample_token(x, 1.0, None, True, 0.95)) for _ in range(400)} <= {0, 1, 2, 3}
+    assert {int(sample_token(x, 1.0, None, True, 1.0, 0.9)) for _ in range(200)} == {1, 2}
+    torch.manual_seed(3)
+    a = sample_token(x, 0.7, 3, True)
+    torch.manual_seed(3)
+    scaled = (x / 0.7).masked_fill(x / 0.7 < torch.topk(x / 0.7, 3).values[:, -1:], float("-inf"))
+    assert torch.equal(a, torch.multinomial(torch.softmax(scaled, -1), 1))                   # without the new filters: the reference's operations
