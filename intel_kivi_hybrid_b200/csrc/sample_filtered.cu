@@ -8,20 +8,23 @@
 //      the bin that the k-th largest is in, and bound the mass above any bin to 0.15 %, which
 //      leaves a few bins that the nucleus can end in;
 //   3. exact masses: all of them, those above the open bins, and a list of the entries in
-//      the open bins, on which both cuts are then found, 32 keys at a time (a warp each; keys, so
-//      that ties stay together);
-//   4. sums of the kept masses over runs of the row, and the run, piece and entry at which
-//      the sum passes uniform * all.
+//      the open bins, on which both cuts are then found, 256 ranges of keys at a time (keys, so
+//      that ties stay together).  A warp has a run of the row, so this walk also gives the runs'
+//      sums of what is kept for certain; the list adds its own.  What belongs where is told by
+//      thresholds on the logits, looked up once: bins, and the masses that min_p leaves, fall with them;
+//   4. the run, the piece of it and the entry at which the sum passes uniform * all.  Only where
+//      there was no third walk (no cut but min_p, or min_p above them) is the row walked for the sums.
 // Where a list does not fit (thousands of equal logits at a cut, as bf16 has them) the row is
 // walked again, up to four times, each of which cuts the open keys into 256 ranges.  Lists
 // come in any order and ranges add by atomics: what is summed there are whole numbers (2^-46
 // of the largest mass at 50257 entries), so that the same inputs give the same id.
 //
-// Masses: 2^(k/32) from a table in fp64 and a correction below 2^-6 of it in fp32 (good to
-// 2^-29 of the mass); the exponent (x - max) log2(e) 32 / T is a product of two-term fp32 numbers,
-// good to 1e-10.  fp64 takes one addition per entry.
-// Bound by latency: 4 walks of 2-3 us, 13 barriers.
+// Masses: 2^(k/32) from a table in fp64, times 1 and a correction below 2^-6 in fp32 (good to
+// 2^-29).  The exponent x c - L, c = 32 log2(e) / T, is taken with L on a grid on
+// which L and the whole number k add exactly, so one fused operation leaves its fraction.
 #include "kivi_common.cuh"
+
+#include <type_traits>
 
 namespace kivi {
 namespace {
@@ -30,7 +33,7 @@ constexpr int kThreads = 1024, kWarps = kThreads / 32;
 static_assert(kWarps == 32, "a warp looks after 32 warps' results, and fills a row of the table");
 constexpr int kBins = 8192;                              // of 1/256 octave; the last holds what is below 2^-32
 constexpr int kPerThread = kBins / kThreads;
-constexpr int kListK = 2048, kListP = 4096;              // entries at the k-th largest, at the end of the nucleus
+constexpr int kListK = 2048, kListP = 8192;              // entries at the k-th largest, at the end of the nucleus
 constexpr float kSlack = 0.0016f;                        // 2^(0.5/256) - 1 and roundings: how far a bin's mass is off its centre's
 
 // order-preserving map float -> uint32; NaN counts as -inf, the zeros are one
@@ -46,43 +49,58 @@ struct FilterArgs {
     const int32_t* top_k;
 };
 
+struct Entry { uint32_t key; int index; };
 struct Shared {
     uint32_t bins[kBins];
-    uint32_t list_k[kListK], list_p[kListP];
+    Entry list_k[kListK], list_p[kListP];
     unsigned long long mass_p[kListP];                   // in whole units
-    uint32_t table_hi[32][32], table_lo[32][32];         // words of 2^(i/32), a column for each lane: no two lanes meet in a bank
-    double sum[kWarps];
-    unsigned long long range[256], open_base;
-    uint32_t flag[2][kWarps];
+    uint2 table[32][32];                                 // 2^(i/32), less the constant of power(); a column for each lane: no two lanes meet in a bank
+    double sum[kWarps], runs[kWarps];
+    uint32_t range[256][3], run_units[kWarps][3];        // whole units in three parts of 18 bits
+    unsigned long long wide_range[256], open_base;
     uint32_t open_lo, open_hi;
     int draw_lo, draw_hi;
     float part[kWarps];
     int count[kWarps];
     uint32_t key[kWarps];
-    int first, bin_k, need, zone_lo, zone_hi, n_k, n_p, pick, last;
+    int first, bin_k, need, zone_lo, zone_hi, n_k, n_p;
     float mass_k[2], tail;
-    uint32_t cut;
+    uint32_t over_key, zone_key, in_key, k_key, min_key;
 };
+// (a list's units: 8192 times 2^18 stays in 32 bits)
+__device__ __forceinline__ void add_units(uint32_t (&to)[3], unsigned long long x) {
+    atomicAdd(&to[0], (uint32_t)x & 0x3ffffu);
+    if (x >> 18) atomicAdd(&to[1], (uint32_t)(x >> 18) & 0x3ffffu);
+    if (x >> 36) atomicAdd(&to[2], (uint32_t)(x >> 36));
+}
+__device__ __forceinline__ unsigned long long units_of(const uint32_t (&x)[3]) {
+    return x[0] + ((unsigned long long)x[1] << 18) + ((unsigned long long)x[2] << 36);
+}
 
 __device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
-// Sums over the block of three numbers of each thread, through 24 KB of shared memory: three
-// warps add them up (32 warps that shuffle share one pipe: 2500 cycles for a sum).
-__device__ __forceinline__ void block_sums(double a, double b, double c, double* scratch, double* out) {
+// Sums over the block of three numbers of each thread, and of the second over each warp, through
+// 24 KB of shared memory: four warps add them up (32 warps that shuffle share one pipe: 2500 cycles
+// for a sum).
+__device__ __forceinline__ void block_sums(double a, double b, double c, double* scratch, double* out, double* runs) {
     scratch[threadIdx.x] = a;
     scratch[kThreads + threadIdx.x] = b;
     scratch[2 * kThreads + threadIdx.x] = c;
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp < 3) {
+    if (warp < 4) {
         double x[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) x[i & 3] += scratch[warp * kThreads + 32 * i + lane];
-        const double sum = warp_sum((x[0] + x[1]) + (x[2] + x[3]));
-        if (lane == 0) out[warp] = sum;
+        for (int i = 0; i < kWarps; ++i) x[i & 3] += scratch[warp == 3 ? kThreads + 32 * lane + ((i + lane) & 31) : warp * kThreads + 32 * i + lane];
+        const double sum = (x[0] + x[1]) + (x[2] + x[3]);
+        if (warp == 3) runs[lane] = sum;
+        else {
+            const double all = warp_sum(sum);
+            if (lane == 0) out[warp] = all;
+        }
     }
     __syncthreads();
 }
@@ -104,75 +122,111 @@ template <> struct Granule<__nv_bfloat16> {
     }
 };
 // f(x, index) for entries [lo, hi) of a row, by `n` threads of which this is number `me`:
-// 16 bytes at a time, four in flight, the ends one by one.
-template <typename T, typename F>
+// 16 bytes at a time, the ends one by one.  kAtOnce: granules whose code is laid out side by side; four are in flight.
+template <typename T, int kAtOnce = 4, typename F>
 __device__ __forceinline__ void walk(const T* row, int lo, int hi, int me, int n, const F& f) {
     constexpr int kSize = Granule<T>::kSize;
     const int off = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15u) / sizeof(T));
     int body = lo + (off ? kSize - off : 0);             // first entry on a 16-byte boundary
     if (body > hi) body = hi;
     const int granules = (hi - body) / kSize, tail = body + granules * kSize;
-    for (int i = lo + me; i < body; i += n) f((float)row[i], i);
     const uint4* g = reinterpret_cast<const uint4*>(row + body);
-    for (int i = me; i < granules; i += 4 * n) {
-        uint4 v[4];
+    auto entries = [&](const uint4& v, int at) {
+        float x[kSize];
+        Granule<T>::get(v, x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j * n < granules) v[j] = g[i + j * n];
+        for (int e = 0; e < kSize; ++e) f(x[e], body + at * kSize + e);
+    };
+    if constexpr (kAtOnce == 1) {
+        // the ends, and granules of which the next two are on their way
+#pragma unroll 1
+        for (int i = me; i < (body - lo) + (hi - tail); i += n) { const int at = i < body - lo ? lo + i : tail + (i - (body - lo)); f((float)row[at], at); }
+        uint4 v = make_uint4(0u, 0u, 0u, 0u), v1 = v, v2 = v;
+        if (me < granules) v = g[me];
+        if (me + n < granules) v1 = g[me + n];
+        if (me + 2 * n < granules) v2 = g[me + 2 * n];
+#pragma unroll 1
+        for (int i = me; i < granules; i += n) {
+            uint4 v3 = v;
+            if (i + 3 * n < granules) v3 = g[i + 3 * n];
+            entries(v, i);
+            v = v1; v1 = v2; v2 = v3;
+        }
+    } else {
+        for (int i = lo + me; i < body; i += n) f((float)row[i], i);
+        for (int i = me; i < granules; i += 4 * n) {
+            uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j * n < granules) {
-                float x[kSize];
-                Granule<T>::get(v[j], x);
+            for (int j = 0; j < 4; ++j)
+                if (i + j * n < granules) v[j] = g[i + j * n];
 #pragma unroll
-                for (int e = 0; e < kSize; ++e) f(x[e], body + (i + j * n) * kSize + e);
-            }
+            for (int j = 0; j < 4; ++j)
+                if (i + j * n < granules) entries(v[j], i + j * n);
+        }
+        for (int i = tail + me; i < hi; i += n) f((float)row[i], i);
     }
-    for (int i = tail + me; i < hi; i += n) f((float)row[i], i);
 }
 
 // Masses relative to the row's largest entry.
 struct Masses {
     float largest, c_hi, c_lo;                           // 32 log2(e) / T in two terms
+    float l_hi, l_lo;                                    // the largest times that: on a grid, and the rest
+    float lowest;                                        // about 2^-940 of the largest's mass
     bool only_largest;                                   // an infinite largest, or a temperature that leaves nothing else
+    bool narrow;                                         // |l_hi| below 2^18: the grid is 2^-5 or finer
     const Shared* s;
 
-    // mass = hi + lo; false: none
-    __device__ __forceinline__ bool get(float x, double& hi, float& lo) const {
-        hi = 0.0; lo = 0.0f;
-        if (only_largest) {
-            if (x == largest) hi = 1.0;
-            return x == largest;
+    __device__ __forceinline__ void set(float top, float temperature) {
+        largest = top;
+        const double c = 32.0 * 1.4426950408889634 / (double)temperature, l = (double)top * c;
+        c_hi = (float)c;
+        c_lo = (float)(c - (double)c_hi);
+        only_largest = largest == INFINITY || temperature < 1e-30f;
+        narrow = fabs(l) < 262144.0;
+        // l + whole numbers down to -31000, in 24 bits: steps of 2^-8 up to 2^16, of 2^-5 up to 2^18 + 31000
+        const double steps = fabs(l) < 32768.0 ? 256.0 : 32.0, grid = rint(l * steps) / steps;
+        l_hi = (float)grid;
+        l_lo = (float)(l - grid);
+        lowest = top - 30000.0f / c_hi;
+    }
+    // 2^((k + r) / 32), t = k + 1.5 * 2^23.  Few instructions of the integer pipe, which bounds the third walk.
+    __device__ __forceinline__ double power(float t, float r) const {
+        const uint32_t b = __float_as_uint(t), i = b & 31u;          // (the constant's low bits are 0)
+        const uint2 w = s->table[i][threadIdx.x & 31];
+        const double at = __hiloint2double((int)((b - i) * 32768u + w.y), (int)w.x);
+        const float u = r * 0.02166084939249829f;        // ln 2 / 32
+        const float e = u * fmaf(u, fmaf(u, fmaf(u, 0.041666667f, 0.16666667f), 0.5f), 1.0f);       // 2^(r/32) - 1 to u^5 / 120 = 2e-12
+        return fma(at, (double)e, at);
+    }
+    __device__ __forceinline__ double narrow_power(float x, float p) const {
+        const float t = __fadd_rn(p, 12582912.0f), whole = __fsub_rn(t, 12582912.0f);        // (1.5 * 2^23: rounds to a whole number)
+        return power(t, __fadd_rn(__fmaf_rn(x, c_hi, -__fadd_rn(l_hi, whole)), __fmaf_rn(x, c_lo, -l_lo)));
+    }
+    // 0: none (2^-968 and less, -inf, NaN)
+    __device__ __forceinline__ double get(float x) const {
+        if (only_largest) return x == largest ? 1.0 : 0.0;
+        if (narrow) {
+            const float p = __fmaf_rn(x, c_hi, -l_hi);
+            return p > -31000.0f ? narrow_power(x, p) : 0.0;
         }
-        const float d = __fsub_rn(x, largest);
-        const float p = __fmul_rn(d, c_hi);
-        if (!(p > -31000.0f)) return false;              // below 2^-968, -inf or NaN
+        const float d = __fsub_rn(x, largest), p = __fmul_rn(d, c_hi);
+        if (!(p > -31000.0f)) return 0.0;
         // d = x - largest to the last bit: what the subtraction rounded away
         const float b = __fsub_rn(x, d), lost = __fadd_rn(__fsub_rn(x, __fadd_rn(d, b)), __fsub_rn(b, largest));
-        const float t = __fadd_rn(p, 12582912.0f), whole = __fsub_rn(t, 12582912.0f);        // (1.5 * 2^23: rounds to a whole number)
-        const int k = __float_as_int(t) - 0x4b400000, n = k >> 5;
-        const float r = __fsub_rn(p, whole) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi)));
-        const uint32_t w1 = s->table_hi[k & 31][threadIdx.x & 31], w0 = s->table_lo[k & 31][threadIdx.x & 31];
-        hi = __hiloint2double((int)w1 + (n << 20), (int)w0);
-        const float u = r * 0.02166084939249829f;        // ln 2 / 32
-        const float e = u * fmaf(u, fmaf(u, fmaf(u, 0.041666667f, 0.16666667f), 0.5f), 1.0f);       // 2^(r/32) - 1 to u^5 / 120 = 1e-12
-        // (a mass below 2^-120 needs no correction)
-        lo = n > -120 ? e * __uint_as_float(((__funnelshift_l(w0, w1, 3) & 0x7fffffu) | 0x3f800000u) + (uint32_t)(n * (1 << 23))) : 0.0f;
-        return true;
+        const float t = __fadd_rn(p, 12582912.0f);
+        return power(t, __fsub_rn(p, __fsub_rn(t, 12582912.0f)) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi))));
+    }
+    // The same for sums, where what has no mass may count as 2^-938 (kNarrow: `narrow` and not `only_largest`).
+    template <bool kNarrow>
+    __device__ __forceinline__ double get_any(float x) const {
+        if constexpr (kNarrow) { x = fmaxf(x, lowest); return narrow_power(x, __fmaf_rn(x, c_hi, -l_hi)); }
+        else return get(x);
     }
     // bin of an entry, falling with it; -1 for one that can have no mass (-inf, NaN)
     __device__ __forceinline__ int bin(float x) const {
         const float p = __fmul_rn(__fmul_rn(__fsub_rn(largest, x), c_hi), 8.0f);
         return p < (float)(kBins - 1) ? __float_as_int(__fadd_rn(p, 12582912.0f)) - 0x4b400000 : x > -INFINITY ? kBins - 1 : -1;
     }
-};
-
-// sums of two terms, folded once at the end
-struct Sum {
-    double hi = 0.0;
-    float lo = 0.0f;
-    __device__ __forceinline__ void add(double h, float l) { hi += h; lo += l; }
-    __device__ __forceinline__ double value() const { return hi + (double)lo; }
 };
 
 template <typename T>
@@ -183,10 +237,10 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
     {
         const double t = exp2((double)warp * (1.0 / 32.0));
-        s.table_hi[warp][lane] = (uint32_t)__double2hiint(t);
-        s.table_lo[warp][lane] = (uint32_t)__double2loint(t);
+        s.table[warp][lane] = make_uint2((uint32_t)__double2loint(t), (uint32_t)__double2hiint(t) - 0x4b400000u * 32768u);
     }
-    if (tid == 0) { s.first = 0x7fffffff; s.bin_k = kBins; s.need = 0; s.zone_lo = kBins; s.zone_hi = -1; s.n_k = 0; s.n_p = 0; s.pick = 0x7fffffff; s.last = -1; }
+    if (tid == 0) { s.first = 0x7fffffff; s.bin_k = kBins; s.need = 0; s.zone_lo = kBins; s.zone_hi = -1; s.n_k = 0; s.n_p = 0; s.min_key = 0u; }
+    if (tid < 3 * kWarps) s.run_units[tid / 3][tid % 3] = 0u;
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0u;
     stream_order();
     const T* const row = settled(logits) + (int64_t)b * row_stride;
@@ -216,29 +270,47 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         return;
     }
     Masses m;
-    m.largest = largest;
-    const double c = 32.0 * 1.4426950408889634 / (double)temperature;
-    m.c_hi = (float)c;
-    m.c_lo = (float)(c - (double)m.c_hi);
-    m.only_largest = largest == INFINITY || temperature < 1e-30f;
     m.s = &s;
+    m.set(largest, temperature);
+    // The least key, of those of finite logits up to the largest, for which holds(x) is true; it is true from there on
+    // (where it is not even true of the largest: one above that).  By a warp, 32 keys at a time.
+    auto least = [&](auto&& holds) {
+        uint32_t lo = 0x00800000u, hi = top;
+        if (!holds(largest)) return top + 1u;
+        while (lo < hi) {                                // (true at hi)
+            const uint32_t step = (hi - lo) / 32u + 1u, key = lo + (uint32_t)lane * step;
+            const unsigned yes = __ballot_sync(0xffffffffu, key >= hi || holds(key_to_float(key)));
+            const int f = yes ? __ffs(yes) - 1 : 32;     // (the keys of all lanes lie below hi or hold)
+            hi = f < 32 ? min(hi, lo + (uint32_t)f * step) : hi;
+            if (f > 0) lo = lo + (uint32_t)(f - 1) * step + 1u;
+            if (f == 0) hi = lo;
+        }
+        return hi;
+    };
 
     uint32_t cut = 0u;                                   // least key that is kept
-    if ((cut_k || cut_p) && !m.only_largest) {
+    bool sums_known = false;
+    if (cut_p && top_p <= 0.0f && !m.only_largest) cut = top;
+    else if ((cut_k || cut_p) && !m.only_largest) {
         // ---- 2. entries per bin ----
-        walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
+        uint32_t far = 0u;                               // (entries of the last bin would all meet in one place)
+        walk<T, 4>(row, 0, vocab, tid, kThreads, [&](float x, int) {
             const int bin = m.bin(x);
-            if (bin >= 0) atomicAdd(&s.bins[bin], 1u);
+            if (bin == kBins - 1) ++far;
+            else if (bin >= 0) atomicAdd(&s.bins[bin], 1u);
         });
+        far = __reduce_add_sync(0xffffffffu, far);
+        if (lane == 0 && far) atomicAdd(&s.bins[kBins - 1], far);
         __syncthreads();
         int count[kPerThread], n = 0;
         float mass = 0.0f;                               // of the thread's bins, by their centres
+        const float first_w = exp2f((float)-(tid * kPerThread) * (1.0f / 256.0f));
+        auto weight = [&](int i) { return first_w * (float)(1.0 - 0.0027076062 * i + 0.0000036655656 * i * i); };        // 2^(-i/256), i < 8, to 2^-19
 #pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
-            const int bin = tid * kPerThread + i;
-            count[i] = (int)s.bins[bin];
+            count[i] = (int)s.bins[tid * kPerThread + i];
             n += count[i];
-            mass += (float)count[i] * exp2f((float)-bin * (1.0f / 256.0f));
+            mass += (float)count[i] * weight(i);
         }
         int n_upto = n;
         float m_upto = mass;
@@ -249,7 +321,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             if (lane >= o) { n_upto += x; m_upto += y; }
         }
         if (lane == 31) { s.count[warp] = n_upto; s.part[warp] = m_upto; }
-        if (tid == kThreads - 1) s.tail = (float)count[kPerThread - 1] * exp2f(-(kBins - 1) / 256.0f);        // (anything down to nothing)
+        if (tid == kThreads - 1) s.tail = (float)count[kPerThread - 1] * weight(kPerThread - 1);        // (anything down to nothing)
         __syncthreads();
         float all = 0.0f, all_most = 0.0f;
         for (int w = 0; w < kWarps; ++w) {
@@ -261,7 +333,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             float above = m_upto - mass;
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
-                const float w = exp2f((float)-(tid * kPerThread + i) * (1.0f / 256.0f));
+                const float w = weight(i);
                 if (upto < top_k && upto + count[i] >= top_k) { s.bin_k = tid * kPerThread + i; s.need = top_k - upto; s.mass_k[0] = above + (float)(top_k - upto) * w; s.mass_k[1] = above + (float)count[i] * w; }
                 upto += count[i];
                 above += (float)count[i] * w;
@@ -281,7 +353,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
 #pragma unroll
             for (int i = 0; i < kPerThread; ++i) {
                 const int bin = tid * kPerThread + i;
-                const float upto = above + (float)count[i] * exp2f((float)-bin * (1.0f / 256.0f));
+                const float upto = above + (float)count[i] * weight(i);
                 if (count[i] > 0 && bin <= bin_k) {
                     const bool stays = upto * (1.0f + kSlack) < lo && bin < kBins - 1, goes = above * (1.0f - kSlack) >= hi;
                     if (!stays && !goes) { atomicMin(&s.zone_lo, bin); atomicMax(&s.zone_hi, bin); }
@@ -290,47 +362,103 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             }
         }
         __syncthreads();
-        const int zone_lo = s.zone_lo, zone_hi = s.zone_hi;
+        int zone_lo = s.zone_lo, zone_hi = s.zone_hi;
+        if (cut_p && zone_lo > zone_hi) { zone_lo = 0; zone_hi = min(bin_k, kBins - 1); }        // (never: a nucleus ends somewhere)
+        // thresholds: entries above the zone, of it, before the k-th largest's bin, of it; what min_p leaves
+        if (warp < 5) {
+            uint32_t key;
+            if (warp == 0) key = least([&](float x) { return m.bin(x) < (cut_p ? zone_lo : bin_k); });
+            else if (warp == 1) key = least([&](float x) { return m.bin(x) <= zone_hi; });
+            else if (warp == 2) key = least([&](float x) { return m.bin(x) < bin_k; });
+            else if (warp == 3) key = least([&](float x) { return m.bin(x) <= bin_k; });
+            else key = min_p > 0.0f ? min(top, least([&](float x) { return m.get(x) >= (double)min_p; })) : 0u;
+            if (lane == 0) (&s.over_key)[warp] = key;
+        }
+        __syncthreads();
+        const uint32_t over_key = s.over_key;
+        if (s.min_key < over_key) {                      // (else it lies above both cuts)
         // ---- 3. exact masses ----
-        Sum in, over;                                    // bins before bin_k; of those, before the zone
-        walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
-            const int bin = m.bin(x);
-            if (bin < 0 || bin > bin_k) return;
-            const bool at_k = bin == bin_k, at_p = bin >= zone_lo && bin <= zone_hi;
-            if (at_k) { const int j = atomicAdd(&s.n_k, 1); if (j < kListK) s.list_k[j] = ordered_key(x); }
-            if (!cut_p) return;
-            double h;
-            float l;
-            m.get(x, h, l);
-            if (!at_k) in.add(h, l);
-            if (at_p) { const int j = atomicAdd(&s.n_p, 1); if (j < kListP) { s.list_p[j] = ordered_key(x); s.mass_p[j] = units(h + (double)l); } }
-            else if (bin < zone_lo) over.add(h, l);
-        });
+        // (one above the largest finite number's key is that of +infinity)
+        const float over_x = key_to_float(over_key), zone_x = cut_p ? key_to_float(s.zone_key) : INFINITY, in_x = key_to_float(s.in_key), k_x = key_to_float(s.k_key);
+        const int run = (vocab + kWarps - 1) / kWarps;
+        double in = 0.0, over = 0.0;                     // before the k-th largest's bin; above the zone
+        auto put = [&](float x, int i) {
+            const int j = atomicAdd(&s.n_p, 1);
+            if (j < kListP) { s.list_p[j] = {ordered_key(x), i}; s.mass_p[j] = units(m.get(x)); }
+        };
+        auto third = [&](auto narrow) {
+            walk<T, 1>(row, min(warp * run, vocab), min(warp * run + run, vocab), lane, 32, [&](float x, int i) {
+                if (cut_k && !(x >= in_x)) {
+                    if (x >= k_x) {                      // of the k-th largest's bin
+                        const int j = atomicAdd(&s.n_k, 1);
+                        if (j < kListK) s.list_k[j] = {ordered_key(x), i};
+                        if (x < over_x && x >= zone_x) put(x, i);
+                    }
+                    return;
+                }
+                const double mass = m.template get_any<decltype(narrow)::value>(x);
+                in += mass;
+                if (x >= over_x) over += mass;
+                if (x < over_x && x >= zone_x) put(x, i);
+            });
+        };
+        if (m.narrow) third(std::true_type{});
+        else third(std::false_type{});
         __syncthreads();
         const int n_k = s.n_k, n_p = s.n_p;
-        // The largest key for which holds(key), asked of whole warps, is true; it falls from true to
-        // false between lo and hi (0 if it is nowhere true).  32 keys at a time.
-        auto search = [&](uint32_t lo, uint32_t hi, auto&& holds) {
-            uint32_t found = 0u;
-            int buf = 0;
-            for (int shift = hi > lo ? (31 - __clz(hi - lo)) / 5 * 5 : 0; shift >= 0; shift -= 5, buf ^= 1) {
-                const uint32_t off = (uint32_t)warp << shift;
-                const bool yes = (off >> shift) == (uint32_t)warp && off <= hi - lo && holds(lo + off);
-                if (lane == 0) s.flag[buf][warp] = yes;
-                __syncthreads();
-                const unsigned all_yes = __ballot_sync(0xffffffffu, s.flag[buf][lane] != 0u);
-                if (!all_yes) return found;
-                found = lo + ((uint32_t)(31 - __clz(all_yes)) << shift);
-                lo = found;
-                hi = min(hi, lo + ((1u << shift) - 1u));
-            }
-            return found;
-        };
-        auto ends = [&](const uint32_t* list, int n, uint32_t& lo, uint32_t& hi) {
-            lo = 0xffffffffu; hi = 0u;
-            for (int i = lane; i < n; i += 32) { lo = min(lo, list[i]); hi = max(hi, list[i]); }
+        // The largest key at which the amounts of a list's entries at or above it reach `most` (0: nowhere),
+        // among keys from `floor` on: 256 ranges of keys at a time.
+        auto search = [&](const Entry* list, int n, uint32_t floor, unsigned long long most, auto&& amount) {
+            uint32_t lo = 0xffffffffu, hi = 0u;
+            for (int i = tid; i < n; i += kThreads) { lo = min(lo, list[i].key); hi = max(hi, list[i].key); }
             lo = __reduce_min_sync(0xffffffffu, lo);
             hi = __reduce_max_sync(0xffffffffu, hi);
+            __syncthreads();
+            if (lane == 0) { s.key[warp] = lo; s.count[warp] = (int)hi; }
+            __syncthreads();
+            lo = max(floor, __reduce_min_sync(0xffffffffu, s.key[lane]));
+            hi = __reduce_max_sync(0xffffffffu, (uint32_t)s.count[lane]);
+            unsigned long long above = 0;                // at the keys behind hi
+            while (lo <= hi) {
+                if (tid < 256) { s.range[tid][0] = 0u; s.range[tid][1] = 0u; s.range[tid][2] = 0u; }
+                __syncthreads();
+                const int bits = 32 - __clz(hi - lo), shift = hi > lo && bits > 8 ? bits - 8 : 0;
+                for (int i = tid; i < n; i += kThreads)
+                    if (list[i].key >= lo && list[i].key <= hi) add_units(s.range[(list[i].key - lo) >> shift], amount(i));
+                __syncthreads();
+                if (warp == 0) {                         // lane 0 has the highest eight ranges
+                    unsigned long long x[8], sum = above;
+                    unsigned long long mine = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) { x[i] = units_of(s.range[255 - 8 * lane - i]); mine += x[i]; }
+                    unsigned long long upto = mine;
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2) {
+                        const unsigned long long y = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += y;
+                    }
+                    sum += upto - mine;
+                    int at_range = -1;
+                    unsigned long long base = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (at_range < 0 && sum + x[i] >= most) { at_range = 255 - 8 * lane - i; base = sum; }
+                        sum += x[i];
+                    }
+                    const unsigned some = __ballot_sync(0xffffffffu, at_range >= 0);
+                    if (some == 0u) { if (lane == 0) { s.open_lo = 1u; s.open_hi = 0u; } }
+                    else if (lane == __ffs(some) - 1) {
+                        s.open_lo = lo + ((uint32_t)at_range << shift);
+                        s.open_hi = min(hi, s.open_lo + ((1u << shift) - 1u));
+                        s.open_base = base;
+                    }
+                }
+                __syncthreads();
+                lo = s.open_lo; hi = s.open_hi; above = s.open_base;
+                if (shift == 0 && lo <= hi) return lo;
+                __syncthreads();
+            }
+            return 0u;
         };
         // The same over the row: amount(x, key) of the keys in lo .. hi, 256 ranges of keys at a time;
         // the largest key at which what is at or above it reaches `most` (in the amount's units).
@@ -339,22 +467,22 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             for (;;) {
                 __syncthreads();
                 lo = s.open_lo; hi = s.open_hi;
-                if (tid < 256) s.range[tid] = 0;
+                if (tid < 256) s.wide_range[tid] = 0;
                 __syncthreads();
                 const int bits = 32 - __clz(hi - lo), shift = hi > lo && bits > 8 ? bits - 8 : 0;
                 walk(row, 0, vocab, tid, kThreads, [&](float x, int) {
                     const uint32_t key = ordered_key(x);
                     if (key < lo || key > hi) return;
                     const unsigned long long a = amount(x);
-                    if (a) atomicAdd(&s.range[(key - lo) >> shift], a);
+                    if (a) atomicAdd(&s.wide_range[(key - lo) >> shift], a);
                 });
                 __syncthreads();
                 if (tid == 0) {
                     unsigned long long upto = s.open_base;
                     int i = 255;
                     for (; i >= 0; --i) {
-                        if (upto + s.range[i] >= most) break;
-                        upto += s.range[i];
+                        if (upto + s.wide_range[i] >= most) break;
+                        upto += s.wide_range[i];
                     }
                     s.open_base = upto;
                     if (i < 0) { s.open_lo = 1u; s.open_hi = 0u; }               // nowhere
@@ -367,14 +495,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         };
         if (cut_k && bin_k < kBins) {
             if (n_k <= kListK) {
-                uint32_t lo, hi;
-                ends(s.list_k, n_k, lo, hi);
-                const int need = s.need;
-                cut = search(lo, hi, [&](uint32_t key) {
-                    int c1 = 0;
-                    for (int i = lane; i < n_k; i += 32) c1 += s.list_k[i] >= key;
-                    return __reduce_add_sync(0xffffffffu, c1) >= need;
-                });
+                cut = search(s.list_k, n_k, 0u, (unsigned long long)s.need, [](int) { return 1ull; });
             } else {
                 cut = search_row(0u, 0xffffffffu, (unsigned long long)top_k, [&](float) { return 1ull; });
             }
@@ -383,64 +504,69 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             // the whole mass: bins before bin_k and what of that bin stays
             // (whole units below 2^53 of the list: exact in any order)
             double rest = 0.0;
-            auto add_rest = [&](float x) { double h; float l; m.get(x, h, l); rest += (double)units(h + (double)l); };
+            auto add_rest = [&](float x) { rest += (double)units(m.get(x)); };
             if (bin_k < kBins) {
                 if (n_k <= kListK) {
                     for (int i = tid; i < n_k; i += kThreads)
-                        if (s.list_k[i] >= cut) add_rest(key_to_float(s.list_k[i]));
+                        if (s.list_k[i].key >= cut) add_rest(key_to_float(s.list_k[i].key));
                 } else {
                     walk(row, 0, vocab, tid, kThreads, [&](float x, int) { if (m.bin(x) == bin_k && ordered_key(x) >= cut) add_rest(x); });
                 }
             }
             __syncthreads();
-            block_sums(in.value(), over.value(), rest, reinterpret_cast<double*>(s.bins), s.sum);
+            block_sums(in, over, rest, reinterpret_cast<double*>(s.bins), s.sum, s.runs);
             double most = (double)top_p * (s.sum[0] + s.sum[2] / unit);
             // (the least key above which there is less than top_p is the largest one at or above which there is no less)
             most = (most - s.sum[1]) * unit;
-            uint32_t key = top;                          // (top_p <= 0: the largest alone)
+            uint32_t key = top;                          // (never: what is above the zone is less)
             if (most > 0.0) {
                 const unsigned long long most_u = (unsigned long long)__double2ll_ru(most);
                 if (n_p <= kListP) {
-                    uint32_t lo, hi;
-                    ends(s.list_p, n_p, lo, hi);
-                    lo = max(lo, cut);                   // (the list may hold what the top-k cut took)
-                    key = lo > hi ? 0u : search(lo, hi, [&](uint32_t probe) {
-                        unsigned long long x = 0;
-                        for (int i = lane; i < n_p; i += 32) x += s.list_p[i] >= probe ? s.mass_p[i] : 0ull;
-                        // (21 bits at a time: reductions of 32-bit numbers)
-                        const unsigned long long a = __reduce_add_sync(0xffffffffu, (uint32_t)x & 0x1fffffu), b = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 21) & 0x1fffffu),
-                                                 c = __reduce_add_sync(0xffffffffu, (uint32_t)(x >> 42));
-                        return a + (b << 21) + (c << 42) >= most_u;
-                    });
+                    // (the list may hold what the top-k cut took)
+                    key = search(s.list_p, n_p, cut, most_u, [&](int i) { return s.mass_p[i]; });
+                    sums_known = key != 0u;
                 } else {
                     key = search_row(max(cut, 1u), top, most_u, [&](float x) {
                         const int bin = m.bin(x);
                         if (bin < zone_lo || bin > zone_hi) return 0ull;
-                        double h;
-                        float l;
-                        m.get(x, h, l);
-                        return units(h + (double)l);
+                        return units(m.get(x));
                     });
                 }
             }
             cut = max(cut, min(key, top));
+        } else {
+            sums_known = bin_k >= kBins || n_k <= kListK;
+            if (sums_known) block_sums(0.0, over, 0.0, reinterpret_cast<double*>(s.bins), s.sum, s.runs);
         }
+        cut = max(cut, s.min_key);
+        if (sums_known) {                                // what is kept of the list, to its runs
+            const int n = cut_p ? n_p : bin_k < kBins ? n_k : 0;
+            for (int i = tid; i < n; i += kThreads) {
+                const Entry e = cut_p ? s.list_p[i] : s.list_k[i];
+                if (e.key < cut) continue;
+                add_units(s.run_units[e.index / run], cut_p ? s.mass_p[i] : units(m.get(key_to_float(e.key))));
+            }
+            __syncthreads();
+            if (tid < kWarps) s.runs[tid] += (double)units_of(s.run_units[tid]) / unit;
+            __syncthreads();
+        }
+        }
+        cut = max(cut, s.min_key);
+    } else if (min_p > 0.0f && !m.only_largest) {
+        if (warp == 0) {
+            const uint32_t key = min(top, least([&](float x) { return m.get(x) >= (double)min_p; }));
+            if (lane == 0) s.min_key = key;
+        }
+        __syncthreads();
+        cut = s.min_key;
     }
     // ---- 4. the draw ----
     const float cut_x = cut ? key_to_float(cut) : -INFINITY;
-    auto kept = [&](float x, double& h, float& l) {
-        if (!(x >= cut_x) || !m.get(x, h, l)) return false;
-        return x == largest || !(min_p > 0.0f) || h + (double)l >= (double)min_p;
-    };
     // sum of the entries [lo, hi) by this warp
     auto run_sum = [&](int lo, int hi) {
-        Sum x;
-        walk(row, lo, hi, lane, 32, [&](float v, int) {
-            double h;
-            float l;
-            if (kept(v, h, l)) x.add(h, l);
-        });
-        return warp_sum(x.value());
+        double x = 0.0;
+        walk<T, 1>(row, lo, hi, lane, 32, [&](float v, int) { if (v >= cut_x) x += m.get(v); });
+        return warp_sum(x);
     };
     int lo = 0, hi = vocab;
     double before = 0.0, target = 0.0;
@@ -448,7 +574,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         // the run of 32 that the sum passes the target in; the last with a mass where roundings leave none
         const int per = (hi - lo + kWarps - 1) / kWarps;
         const int a = min(lo + warp * per, hi), z = min(a + per, hi);
-        const double sum = run_sum(a, z);
+        const double sum = level == 0 && sums_known ? s.runs[warp] : run_sum(a, z);
         __syncthreads();
         if (lane == 0) s.sum[warp] = sum;
         __syncthreads();
@@ -474,10 +600,9 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         int pick = -1, last = -1;
         for (int i0 = lo; i0 < hi && pick < 0; i0 += 32) {
             const int i = i0 + lane;
-            double h = 0.0;
-            float l = 0.0f;
-            const bool stays = i < hi && kept((float)row[i], h, l);
-            double upto = stays ? h + (double)l : 0.0;
+            const float x = i < hi ? (float)row[i] : -INFINITY;
+            double upto = x >= cut_x ? m.get(x) : 0.0;
+            const bool stays = upto > 0.0;
 #pragma unroll
             for (int o = 1; o < 32; o *= 2) {
                 const double x = __shfl_up_sync(0xffffffffu, upto, o);

@@ -173,3 +173,25 @@ def test_refusals(ops):
         with pytest.raises(RuntimeError, match=what):
             bad()
     assert ops.sample_filtered(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_flat_rows_low_temperatures_and_shifted_logits(ops, dtype):
+    """Thousands of entries where the nucleus ends (lists overflow), exponents beyond the fine grid, logits far from 0."""
+    B, V = 8, 70001
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(B, V, generator=g, device="cuda").to(dtype)
+    u = uniforms(B, 11)
+    p = [0.05, 0.3, 0.5, 0.7, 0.9, 0.99, 0.9999, 0.6]
+    check(ops, x, u, [20.0, 5.0, 100.0, 1e4, 2.0, 1e6, 10.0, 3e38], p=p)
+    check(ops, x, u, [20.0, 5.0, 100.0, 1e4, 2.0, 1e6, 10.0, 3e38], [60000] * B, p, [0.5, 0.9, 0.99, 0.0, 0.3, 0.0, 0.7, 1.0])
+    cold = [1e-2, 1e-3, 2e-4, 1e-4, 1e-5, 1e-8, 1e-20, 1e-29]
+    check(ops, x, u, cold)
+    check(ops, x, u, cold, [50] * B, p, [0.01] * B)
+    for shift in (1e2, -1e3, 1e4, -1e6):
+        check(ops, (x.float() + shift).to(dtype), u, [0.7] * B, [500] * B, p, [0.02] * B)
+
+
+def test_one_row_for_many_draws(ops):
+    x = torch.randn(1, 5000, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    check(ops, x.expand(64, 5000), uniforms(64, 12), [1.1] * 64, [40] * 64, [0.9] * 64)
