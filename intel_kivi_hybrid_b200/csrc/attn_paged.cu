@@ -22,6 +22,7 @@ namespace {
 __device__ int g_fault = 0;
 
 constexpr int kTile = 64;                                // tokens in shared memory at a time
+constexpr int kAtOnce = 4;
 
 // DT: head_dim 64 or 128, or 256 for any up to that.
 template <int RPT, int TY, int DT>
@@ -29,11 +30,12 @@ __global__ void __launch_bounds__(TY * 16)
 paged_attention_kernel(PagedAttnArgs A) {
     constexpr int RT = RPT * TY, kThreads = TY * 16, NC = DT / 64;       // NC: quads of channels a thread has
     extern __shared__ __align__(16) float smem_f[];
-    __shared__ int place_s[2];
+    __shared__ int place_s[2], in_group[2][kTile];
+    __shared__ int64_t at_s[2][kTile];                   // of a tile's tokens: group of the pages, or element of the window, or row
     stream_order();
     settle_args(A);
     const kivi_paged_layer& L = A.L;
-    const int D = DT == 256 ? L.head_dim : DT, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + 4;
+    const int D = DT == 256 ? L.head_dim : DT, G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, S = D + 4, Q = G / 4, W = D < 64 ? D : 64;
     float* const q_s = smem_f;                           // [RT][S]
     float* const k_s = q_s + RT * S;                     // [kTile][S]
     float* const v_s = k_s + kTile * S;                  // [kTile][S]
@@ -63,6 +65,25 @@ paged_attention_kernel(PagedAttnArgs A) {
     const bool whole = t_end == keys && blockIdx.z == 0;                 // the only piece of this block
     const bool vec = A.vec != 0;
 
+    // where a tile's tokens are, looked up a tile ahead: one division and one look at the page table a token
+    auto look_up = [&](int t0, int buf) {
+        const int t = t0 + tid;
+        if (tid >= kTile || t >= t_end) return;
+        int64_t at;
+        int tt = 0;
+        if (t < inside) {
+            const int page = t / L.page_tokens, in_page = t - page * L.page_tokens;
+            at = ((int64_t)page_of(L, q, t, &g_fault) * H + h) * (L.page_tokens / G) + in_page / G;
+            tt = in_page % G;
+        } else if (t < q.held) {
+            at = (((int64_t)q.slot * H + h) * R + ring_slot(t, A.b.ring_shift, R)) * D;
+        } else {
+            at = (int64_t)q.row0 + (t - q.held);
+        }
+        at_s[buf][tid] = at;
+        in_group[buf][tid] = tt;
+    };
+    look_up(t_begin, 0);
     for (int i = tid; i < RT * (D / 4); i += kThreads) {
         const int r = i / (D / 4), d = 4 * (i % (D / 4));
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -82,18 +103,56 @@ paged_attention_kernel(PagedAttnArgs A) {
 #pragma unroll
         for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.0f;
     }
-    for (int t0 = t_begin; t0 < t_end; t0 += kTile) {
-        __syncthreads();                                 // the tile before has been read
-        for (int i = tid; i < kTile * (D / 4); i += kThreads) {
-            const int j = i / (D / 4), d = 4 * (i % (D / 4)), t = t0 + j;
-            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-            if (t < t_end) {
-                k = paged_key4(A, q, h, inside, t, d, vec, &g_fault);
-                v = paged_value4(A, q, h, inside, t, d, vec, &g_fault);
+    int buf = 0;
+    for (int t0 = t_begin; t0 < t_end; t0 += kTile, buf ^= 1) {
+        __syncthreads();                                 // the tile before has been read, this one's places are known
+        const int64_t* const at = at_s[buf];
+        if (t0 + kTile <= inside && kTile * (DT == 256 ? 0 : DT / 4) % (kAtOnce * kThreads) == 0 && DT != 256) {
+            // all in pages: the loads of kAtOnce quads of channels are on their way together
+            for (int i0 = tid; i0 < kTile * (D / 4); i0 += kAtOnce * kThreads) {
+                uint32_t w[kAtOnce], c[kAtOnce];
+                float4 ks[kAtOnce], kz[kAtOnce];
+                float vs[kAtOnce], vz[kAtOnce];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const int i = i0 + u * kThreads, j = i / (D / 4), d = 4 * (i % (D / 4)), tt = in_group[buf][j];
+                    const int64_t g = at[j], x = g * D + vmeta_index(tt, d / G, D, G);
+                    w[u] = *reinterpret_cast<const uint32_t*>(L.k_codes + g * (D * Q) + kblock_offset(d, tt >> 2, Q, W));
+                    c[u] = L.v_codes[g * (D * Q) + vcode_offset(tt, d / 4, D, G)];
+                    ks[u] = *reinterpret_cast<const float4*>(L.k_scales + g * D + d); kz[u] = *reinterpret_cast<const float4*>(L.k_zeros + g * D + d);
+                    vs[u] = L.v_scales[x]; vz[u] = L.v_zeros[x];
+                }
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const int i = i0 + u * kThreads, j = i / (D / 4), d = 4 * (i % (D / 4)), sh = 2 * (in_group[buf][j] & 3);
+                    *reinterpret_cast<float4*>(k_s + j * S + d) =
+                        make_float4(fmaf((float)((w[u] >> sh) & 3u), ks[u].x, kz[u].x), fmaf((float)((w[u] >> (sh + 8)) & 3u), ks[u].y, kz[u].y),
+                                    fmaf((float)((w[u] >> (sh + 16)) & 3u), ks[u].z, kz[u].z), fmaf((float)((w[u] >> (sh + 24)) & 3u), ks[u].w, kz[u].w));
+                    *reinterpret_cast<float4*>(v_s + j * S + d) = make_float4(fmaf((float)(c[u] & 3u), vs[u], vz[u]), fmaf((float)((c[u] >> 2) & 3u), vs[u], vz[u]),
+                                                                              fmaf((float)((c[u] >> 4) & 3u), vs[u], vz[u]), fmaf((float)(c[u] >> 6), vs[u], vz[u]));
+                }
             }
-            *reinterpret_cast<float4*>(k_s + j * S + d) = k;
-            *reinterpret_cast<float4*>(v_s + j * S + d) = v;
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < kTile * (D / 4); i += kThreads) {
+                const int j = i / (D / 4), d = 4 * (i % (D / 4)), t = t0 + j;
+                float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+                if (t < inside) {
+                    const int tt = in_group[buf][j];
+                    k = packed_key4(L, at[j], tt, d);
+                    v = packed_value4(L, at[j], tt, d);
+                } else if (t < q.held) {
+                    k = L.res_dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(L.k_res) + at[j] + d, true) : load4(reinterpret_cast<const float*>(L.k_res) + at[j] + d, true);
+                    v = L.res_dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(L.v_res) + at[j] + d, true) : load4(reinterpret_cast<const float*>(L.v_res) + at[j] + d, true);
+                } else if (t < t_end) {
+                    k = load4_as(A.k, L.res_dtype, at[j], h, d, vec);
+                    v = load4_as(A.v, L.res_dtype, at[j], h, d, vec);
+                }
+                *reinterpret_cast<float4*>(k_s + j * S + d) = k;
+                *reinterpret_cast<float4*>(v_s + j * S + d) = v;
+            }
         }
+        look_up(t0 + kTile, buf ^ 1);
         __syncthreads();
         float sc[RPT][4];
 #pragma unroll
@@ -356,10 +415,9 @@ static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b
     const int64_t blocks = ((int64_t)b->total_new * n_rep) / p.rows + b->num_seqs;
     p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
     const int tiles = (b->max_len + kTile - 1) / kTile;
-    // as many pieces as give every SM four CTAs, no piece below two tiles
+    // as many pieces as give every SM four CTAs
     int64_t want = (4 * (int64_t)num_sms() + p.blocks * (int64_t)L->num_kv_heads - 1) / (p.blocks * (int64_t)L->num_kv_heads);
-    const int most = (tiles + 1) / 2;
-    if (want > most) want = most;
+    if (want > tiles) want = tiles;
     if (want > 256) want = 256;
     if (want < 1) want = 1;
     const int per = (int)((tiles + want - 1) / want);

@@ -44,27 +44,30 @@ __device__ __forceinline__ float4 paged_row4(const PagedAttnArgs& A, const Paged
     const int64_t at = (((int64_t)q.slot * L.num_kv_heads + h) * L.residual_cap + ring_slot(t, A.b.ring_shift, L.residual_cap)) * L.head_dim + d;
     return L.res_dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(ring) + at, true) : load4(reinterpret_cast<const float*>(ring) + at, true);
 }
-__device__ __forceinline__ float4 paged_key4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
-    const kivi_paged_layer& L = A.L;
-    if (t >= inside) return paged_row4(A, q, L.k_res, A.k, h, t, d, vec);
-    const int D = L.head_dim, G = L.group_size, Q = G / 4;
-    const int64_t g = ((int64_t)page_of(L, q, t, fault) * L.num_kv_heads + h) * (L.page_tokens / G) + t % L.page_tokens / G;
-    const int tt = t % G, sh = 2 * (tt & 3);
+// Four channels of token tt of group g of the pages.
+__device__ __forceinline__ float4 packed_key4(const kivi_paged_layer& L, int64_t g, int tt, int d) {
+    const int D = L.head_dim, Q = L.group_size / 4, sh = 2 * (tt & 3);
     const uint32_t w = *reinterpret_cast<const uint32_t*>(L.k_codes + g * (D * Q) + kblock_offset(d, tt >> 2, Q, D < 64 ? D : 64));
     const float4 s = *reinterpret_cast<const float4*>(L.k_scales + g * D + d), z = *reinterpret_cast<const float4*>(L.k_zeros + g * D + d);
     return make_float4(fmaf((float)((w >> sh) & 3u), s.x, z.x), fmaf((float)((w >> (sh + 8)) & 3u), s.y, z.y),
                        fmaf((float)((w >> (sh + 16)) & 3u), s.z, z.z), fmaf((float)((w >> (sh + 24)) & 3u), s.w, z.w));
 }
-__device__ __forceinline__ float4 paged_value4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
-    const kivi_paged_layer& L = A.L;
-    if (t >= inside) return paged_row4(A, q, L.v_res, A.v, h, t, d, vec);
+__device__ __forceinline__ float4 packed_value4(const kivi_paged_layer& L, int64_t g, int tt, int d) {
     const int D = L.head_dim, G = L.group_size;
-    const int64_t g = ((int64_t)page_of(L, q, t, fault) * L.num_kv_heads + h) * (L.page_tokens / G) + t % L.page_tokens / G;
-    const int tt = t % G;
     const uint32_t c = L.v_codes[g * (D * (G / 4)) + vcode_offset(tt, d / 4, D, G)];
     const int64_t at = g * D + vmeta_index(tt, d / G, D, G);
     const float s = L.v_scales[at], z = L.v_zeros[at];
     return make_float4(fmaf((float)(c & 3u), s, z), fmaf((float)((c >> 2) & 3u), s, z), fmaf((float)((c >> 4) & 3u), s, z), fmaf((float)(c >> 6), s, z));
+}
+__device__ __forceinline__ int64_t paged_group(const PagedAttnArgs& A, const PagedSeq& q, int h, int t, int* fault) {
+    const kivi_paged_layer& L = A.L;
+    return ((int64_t)page_of(L, q, t, fault) * L.num_kv_heads + h) * (L.page_tokens / L.group_size) + t % L.page_tokens / L.group_size;
+}
+__device__ __forceinline__ float4 paged_key4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
+    return t < inside ? packed_key4(A.L, paged_group(A, q, h, t, fault), t % A.L.group_size, d) : paged_row4(A, q, A.L.k_res, A.k, h, t, d, vec);
+}
+__device__ __forceinline__ float4 paged_value4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
+    return t < inside ? packed_value4(A.L, paged_group(A, q, h, t, fault), t % A.L.group_size, d) : paged_row4(A, q, A.L.v_res, A.v, h, t, d, vec);
 }
 #endif
 
