@@ -73,6 +73,7 @@ class PagedKiviCache:
         self._free_slots = list(range(max_sequences - 1, -1, -1))
         self._pages: dict = {}                     # sequence -> its pages
         self._lens: dict = {}                      # sequence -> tokens held
+        self._steps: dict = {}                     # sequence -> its step that has not ended
 
     @classmethod
     def from_model(cls, model, num_pages: int, max_sequences: int, **kwargs) -> "PagedKiviCache":
@@ -94,10 +95,18 @@ class PagedKiviCache:
 
     def free(self, seq: int) -> None:
         """Give a sequence's window and pages back.  Kernels queued before may still read them: later steps
-        come behind those on the same stream."""
+        come behind those on the same stream.  A step of it that has not ended is given up."""
+        self._give_up(seq)
         self._free_pages.extend(reversed(self._pages.pop(seq)))
         del self._lens[seq]
         self._free_slots.append(seq)
+
+    def _give_up(self, seq: int) -> None:
+        step = self._steps.get(seq)
+        if step is not None:
+            step.open = False
+            for s in step.seqs:
+                self._steps.pop(s, None)
 
     def length(self, seq: int) -> int:
         return self._lens[seq]
@@ -130,7 +139,8 @@ class PagedKiviCache:
 
     def begin(self, seqs: Sequence[int], new: Sequence[int], max_len: Optional[int] = None) -> PagedBatch:
         """Start a step in which sequence ``seqs[i]`` gets ``new[i]`` tokens (0 is allowed): takes the pages that the
-        step fills and lays down the arrays its kernels follow.  ``max_len``: the longest length a captured step
+        step fills and lays down the arrays its kernels follow.  A step of one of them that has not ended is given up; what it
+        has appended to some layers is not undone, so give up only what has not run.  ``max_len``: the longest length a captured step
         shall reach (default: this step's)."""
         seqs, new = [int(s) for s in seqs], [int(n) for n in new]
         assert len(seqs) == len(new) and seqs, "begin() needs at least one sequence, and new tokens for each"
@@ -148,13 +158,17 @@ class PagedKiviCache:
             cu.append(cu[-1] + n)
         width = max(1, -(-self.quantized(max_len) // self.page_tokens))
         dev = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
-        return PagedBatch(seqs, new, held, max(new), max_len, cu[-1], self._table(seqs, width).to(self.device), dev(seqs), dev(held), dev(cu))
+        batch = PagedBatch(seqs, new, held, max(new), max_len, cu[-1], self._table(seqs, width).to(self.device), dev(seqs), dev(held), dev(cu))
+        for s in seqs:
+            self._give_up(s)
+        self._steps.update((s, batch) for s in seqs)
+        return batch
 
     def append(self, layer: int, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, rotary: Optional[torch.Tensor] = None,
                q: Optional[torch.Tensor] = None, interleaved: bool = False):
         """Append the step's keys and values [rows, H, D] (of the cache's dtype).  With ``rotary`` [positions, rotary_dim]
         (fp32: cosines, then sines) keys and queries are turned to their positions first; returns (q, k) as the
-        attention wants them."""
+        attention wants them.  Once per layer and step: window slots that it has read are written again."""
         assert batch.open, "the step has ended"
         q_out = k_out = None
         if rotary is not None:
@@ -187,12 +201,15 @@ class PagedKiviCache:
         for s, h, n in zip(batch.seqs, batch.held, batch.new):
             assert self._lens.get(s) == h, f"sequence {s} has changed during the step"
             self._lens[s] = h + n
+            self._steps.pop(s, None)
         batch.open = False
 
     def refresh(self, batch: PagedBatch) -> None:
         """Open the next step of the same sequences and numbers of new tokens in the same arrays (for a captured
         step, whose kernels have their addresses)."""
         assert not batch.open, "the step has not ended"
+        for s in batch.seqs:
+            assert s in self._lens, f"sequence {s} is not there"
         held = [self._lens[s] for s in batch.seqs]
         lens = [h + n for h, n in zip(held, batch.new)]
         assert max(lens) <= batch.max_len, f"the step reaches {max(lens)} tokens, it was begun for {batch.max_len}"
@@ -200,6 +217,9 @@ class PagedKiviCache:
         batch.page_table.copy_(self._table(batch.seqs, batch.page_table.shape[1]))
         batch.seq_lens.copy_(torch.tensor(held, dtype=torch.int32))
         batch.held, batch.open = held, True
+        for s in batch.seqs:
+            self._give_up(s)
+        self._steps.update((s, batch) for s in batch.seqs)
 
     # ------------------------------------------------------------------ reading back
     def read(self, layer: int, seq: int, start: int = 0, stop: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -159,18 +159,32 @@ paged_attention_kernel(PagedAttnArgs A) {
         for (int i = 0; i < RPT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) sc[i][j] = 0.0f;
-#pragma unroll 4
-        for (int d = 0; d < D; d += 4) {
-            float4 a[RPT], b[4];
-#pragma unroll
-            for (int i = 0; i < RPT; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ty * RPT + i) * S + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * S + d);
+        // Sixteen channels by themselves and then to the sum, which is rounded a
+        // sixteenth as often: half the scores' error.
+        for (int d0 = 0; d0 < D; d0 += 16) {
+            float part[RPT][4];
 #pragma unroll
             for (int i = 0; i < RPT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    sc[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, sc[i][j]))));
+                for (int j = 0; j < 4; ++j) part[i][j] = 0.0f;
+#pragma unroll
+            for (int d = d0; d < d0 + 16; d += 4) {
+                if (DT == 256 && d >= D) break;
+                float4 a[RPT], b[4];
+#pragma unroll
+                for (int i = 0; i < RPT; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (ty * RPT + i) * S + d);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * S + d);
+#pragma unroll
+                for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        part[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, part[i][j]))));
+            }
+#pragma unroll
+            for (int i = 0; i < RPT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[i][j] += part[i][j];
         }
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {

@@ -383,8 +383,9 @@ static_assert(kWarps * kStages * kStageBytes >= 2 * kG * kD * 4, "the window's C
 }  // namespace
 
 bool paged_decode_serves(const kivi_paged_layer* L, int q_dtype, int64_t max_rows) {
-    // Three blocks of rows: 16 sequences x 4k, 4 query heads, 3 tokens 86 us here, 97 with 256 rows on the
-    // tensor cores; 4 tokens 106 and 98; 1 x 32k 2 tokens 64 and 59.
+    // Three blocks of rows (3 tokens, 4 query heads per KV head, 8 KV heads), here and with 256 rows on the
+    // 5th-generation tensor cores: 16 sequences x 4k 80 and 80 us, 64 x 2k 176 and 201, 1 x 32k 33 and 52;
+    // four blocks: 103 and 83, 229 and 203, 46 and 52.
     // (bf16 windows with fp32 queries and the other way round go to the general kernel)
     return L->head_dim == kD && L->group_size == kG && q_dtype == L->res_dtype && max_rows <= 12;
 }
@@ -393,7 +394,7 @@ bool paged_decode_serves(const kivi_paged_layer* L, int q_dtype, int64_t max_row
 // warps (eight groups, 1.4 us).  Rounds of CTAs on the GPU times rounds of a piece, two more
 // for a CTA's start and end, and what a piece costs in the fold; but no piece above a sixth
 // of a GPU's share where that is long, since sequences shorter than the longest leave theirs
-// unused (64 ragged sequences up to 32k: 285 us with a sixth, one piece each 420).
+// unused (64 ragged sequences up to 32k: 280 us).
 void paged_decode_plan(const kivi_paged_layer* L, const kivi_paged_batch* b, int n_rep, int* blocks_per_seq, int* gps, int* pieces) {
     constexpr int kRound = kWarps * kGPS;
     *blocks_per_seq = (b->max_new * n_rep + kRows - 1) / kRows;

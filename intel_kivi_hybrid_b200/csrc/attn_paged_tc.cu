@@ -5,18 +5,19 @@
 //
 // over tiles of 128 tokens, for two blocks of 128 rows at a time ((new token, query head)
 // pairs of one sequence and KV head: all heads of a group share the tile).  Codes become
-// numbers once per tile and serve 256 rows.  Roles of the 27 warps:
-//   0-7, 8-15  two threads per row of the first / second block: running maximum and sum,
+// numbers once per tile and serve 256 rows.  A CTA that has one block only gives it to both
+// groups of softmax warps, one for the even tiles and one for the odd.  Roles of the 19 warps:
+//   0-3, 4-7   a thread per row of the first / second block: running maximum and sum,
 //              weights, rescaling, output
-//   16-19      K of a tile: codes, scales and zeros (of the window and the new tokens: rows)
+//   8-11       K of a tile: codes, scales and zeros (of the window and the new tokens: rows)
 //              become fp16 numbers in shared memory, two stages; a warp has a group of tokens
-//   20-23      V, likewise
-//   24         one thread issues the MMAs: S of a block while the other block's weights
+//   12-15      V, likewise
+//   16         one thread issues the MMAs: S of a block while the other block's weights
 //              are made; P comes from tensor memory, where it takes the place of S
-//   26         finds the largest factor of the tiles of codes, ahead of those who need it
-//   25         one thread brings codes, scales and zeros of the tiles to come to shared
+//   17         one thread brings codes, scales and zeros of the tiles to come to shared
 //              memory with bulk copies, two tiles ahead (loads into registers half a tile
 //              ahead left every second tile waiting for its slowest warp)
+//   18         finds the largest factor of the tiles of codes, ahead of those who need it
 //
 // Operands are fp16 numbers with powers of two taken out: a row of Q and a tile of K by
 // their own largest, V by the largest that the CTA has met so far (when it grows, O is
@@ -34,8 +35,15 @@
 // which 1024 is taken off exactly; c 4^n (s / 4^n) + z is one fused operation for two
 // numbers.  3.3 instructions for two elements, where fp32 takes five and a conversion.
 //
-// Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle),
-// about 500 issue cycles of conversion and 800 of softmax arithmetic on each quarter.
+// Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle); measured
+// 5500.  A block's chain is what bounds it: maximum 630-1000, weights 2800 while the other block
+// makes its own, then 1400 until P V and the next scores are done.  One block: 4300, of which the
+// conversion of a tile takes 2800-3100 (bf16, 32k tokens).
+// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 398 us, 700 TFLOP/s; 4 x 2048 over
+// 16k 3262 us; 16 x 5 tokens over 4k 85 us (101 with one group of softmax warps for its one block).
+// Lost: two threads to a row that meet for its maximum (406, 3323); scores in halves of 64 tokens,
+// so that the next half's are made meanwhile (471, 3753: twice the dependent MMAs in a row);
+// maxima of the halves one after the other, without a pass for them (439, 3594: spills).
 #include "async_copy.cuh"
 #include "paged_attention.cuh"
 
@@ -48,9 +56,9 @@ __device__ int g_fault = 0;
 
 constexpr int kN = 128;                                  // tokens of a tile
 constexpr int kM = 128;                                  // rows of a block
-constexpr int kSoftmaxWarps = 16, kTileWarps = 4;        // (four for keys, four for values)
+constexpr int kSoftmaxWarps = 8, kTileWarps = 4;        // (four for keys, four for values)
 constexpr int kMmaWarp = kSoftmaxWarps + 2 * kTileWarps, kCopyWarp = kMmaWarp + 1, kTopWarp = kMmaWarp + 2, kThreads = (kTopWarp + 1) * 32;
-constexpr int kRing = 8;                                 // exponents of so many tiles are kept (they are found up to four tiles ahead of the rows)
+constexpr int kRing = 8;                                 // exponents of so many tiles are kept (they are found up to five tiles ahead of the rows)
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 
 // ---- tensor core ----------------------------------------------------------------
@@ -77,7 +85,7 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Bounded wait that sleeps in the barrier unit: 27 warps that poll take issue slots from
+// Bounded wait that sleeps in the barrier unit: 19 warps that poll take issue slots from
 // those that work.  A poll gives up after a millisecond at the latest, the wait after
 // some seconds.
 __device__ __forceinline__ bool mbar_sleep(uint32_t bar, uint32_t parity) {
@@ -165,7 +173,6 @@ struct Misc {                                            // behind the tiles
     int k_top[kRing], v_top[kRing];                      // biased exponents of tile j's largest at j % kRing
     int rough;                                           // a value has been met that the tiles' operands are no good for
     uint32_t top[2][2][kTileWarps];                      // [tile parity][K, V][warp]
-    __nv_bfloat16 row_top[2][2][kM];                     // [block][half of the columns][row]
 };
 
 __device__ __forceinline__ float4 lds_float4(uint32_t at) {
@@ -256,6 +263,9 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     const int rows = q.n * n_rep, row_first = misc.place[1] * 2 * kM;
     const int n_rows = rows - row_first < 2 * kM ? rows - row_first : 2 * kM;
     const int n_sub = n_rows > kM ? 2 : 1;
+    // One block of rows: both groups of softmax warps have it, one the even tiles and one the odd, each with
+    // scores, weights, sums and output of its own; they are joined at the end.
+    const bool turns = n_sub == 1;
     const int inside = min(quant_of(q.held + q.n, G, R), q.held);
     const int keys = q.held + (row_first + n_rows - 1) / n_rep + 1;
     const int t_begin = blockIdx.z * A.chunk;            // (a multiple of kN)
@@ -266,7 +276,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
     auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
     if (warp == kMmaWarp) {
         if (elect_one()) {
-            mbar_init(bar(misc.q_full), 2 * kM * n_sub);
+            mbar_init(bar(misc.q_full), kM * n_sub);
             for (int i = 0; i < 2; ++i) {
                 for (int x = 0; x < 2; ++x) {
                     mbar_init(bar(misc.full[x][i]), kTileWarps); mbar_init(bar(misc.empty[x][i]), 1);
@@ -297,11 +307,10 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
 
     if (warp < kSoftmaxWarps) {
         // ---------------- rows ----------------
-        // two threads to a row, 64 columns each, which hold the same maximum
-        const int t = warp >> 3, half = warp >> 2 & 1, r = tid & (kM - 1);
-        if (t < n_sub) {
-            const int row = row_first + t * kM + r;
-            const bool there = t * kM + r < n_rows;
+        const int t = warp >> 2, r = tid & (kM - 1);
+        if (t < n_sub || turns) {
+            const int in_cta = (turns ? 0 : t * kM) + r, row = row_first + in_cta;
+            const bool there = in_cta < n_rows;
             const int token = there ? row / n_rep : 0, head = h * n_rep + (there ? row % n_rep : 0);
             // the row of Q: its largest to 2^13 .. 2^14
             int q_shift = 0;
@@ -325,7 +334,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 q_shift = shift_of(exponent_of(top));
                 const float f = pow2i(q_shift);
 #pragma unroll 1
-                for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 8) {
+                for (int d = 0; d < D && t < n_sub; d += 8) {
                     uint32_t w[4] = {0u, 0u, 0u, 0u};
                     if (there) {
                         const uint16_t* u = reinterpret_cast<const uint16_t*>(from + d);
@@ -340,7 +349,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 }
             }
             fence_async();
-            arrive(bar(misc.q_full));
+            if (t < n_sub) arrive(bar(misc.q_full));
 
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + t * kN, o_at = tmem + lanes + 2 * kN + t * D;
             const int last = there ? q.held + token : 0x3fffffff;    // last token that the row sees (a row that is not there is in nobody's way)
@@ -348,9 +357,11 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             int v_shift = 0;
             const float scale = A.scale_log2;
             bool ok = true;
-            for (int j = 0; j < n_tiles; ++j) {
-                // (given up: on to the end without waiting, the row's other half waits at the barrier below)
-                if (ok) ok = wait_warp(misc.s_full[t], j);
+            const int first = turns ? t : 0, step = turns ? 2 : 1;
+            for (int j = first; j < n_tiles; j += step) {
+                const int turn = turns ? j >> 1 : j;
+                // (given up: on to the end without waiting; the groups meet at a barrier there)
+                if (ok) ok = wait_warp(misc.s_full[t], turn);
                 fence_after();
                 const int t0 = t_begin + j * kN;
                 const int k_shift = shift_of(misc.k_top[j % kRing]);
@@ -360,32 +371,29 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 // (loops of one body: the roles share an instruction cache, unrolled ones cost 15 % of the call)
                 float top = -INFINITY;
 #pragma unroll 1
-                for (int x = 64 * half; x < 64 * half + 64; x += 32) {
-                    uint32_t v[32];
-                    tmem_load32(s_at + x, v);
+                for (int x = 0; x < kN; x += 64) {
+                    uint32_t v[2][32];
+                    tmem_load32(s_at + x, v[0]);
+                    tmem_load32(s_at + x + 32, v[1]);
                     tmem_wait_load();
-                    if (__any_sync(0xffffffffu, seen < x + 32)) hide(v, seen - x);
+                    if (__any_sync(0xffffffffu, seen < x + 64)) { hide(v[0], seen - x); hide(v[1], seen - x - 32); }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
+                    for (int i = 0; i < 64; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[i / 32][i % 32]), __uint_as_float(v[i / 32][i % 32 + 1])));
                 }
-                // The row's other half: a maximum is a point of reference, eight bits of it do.
-                const __nv_bfloat16 mine = __float2bfloat16_rn(top * c);
-                misc.row_top[t][half][r] = mine;
-                asm volatile("bar.sync %0, %1;" ::"r"(3 + t), "n"(2 * kM) : "memory");
-                top = fmaxf(__bfloat162float(mine), __bfloat162float(misc.row_top[t][half ^ 1][r]));
+                top *= c;
                 // (V of tile j + 2 is not made before this tile's weights are contracted, so the barrier's phase is this tile's)
                 if (ok) ok = wait_warp(misc.v_known[j % 4], j >> 2);
                 const int v_new = shift_of(misc.v_top[j % kRing]);
                 const bool grows = top > m + kGrowth;                // (from -inf: whenever there is a maximum)
-                if (__any_sync(0xffffffffu, grows) || (j > 0 && v_new != v_shift)) {
+                if (__any_sync(0xffffffffu, grows) || (j > first && v_new != v_shift)) {
                     const float m_new = fmaxf(m, top);
                     const float alpha = m == -INFINITY ? 0.0f : ex2(m - m_new);
                     m = m_new;
                     l *= alpha;
-                    if (j > 0) {
+                    if (j > first) {
                         const float f = (m == -INFINITY ? 1.0f : alpha) * pow2i(max(v_new - v_shift, -126));
 #pragma unroll 1
-                        for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 16) {
+                        for (int x = 0; x < D; x += 16) {
                             uint32_t o[16];
                             tmem_load16(o_at + x, o);
                             tmem_wait_load();
@@ -398,54 +406,85 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 v_shift = v_new;
                 const float base_m = m == -INFINITY ? 0.0f : m;
                 float2 sum = make_float2(0.0f, 0.0f);
-                // Weights: columns 0 .. 63 become columns 0 .. 31, 64 .. 127 become 64 .. 95.
+                // Weights: columns 64 .. 127 become columns 64 .. 95 and are contracted while 0 .. 63 become columns 0 .. 31.
 #pragma unroll 1
-                for (int x = 64 * half; x < 64 * half + 64; x += 32) {
-                    uint32_t v[32], p[16];
-                    tmem_load32(s_at + x, v);
+                for (int half = 1; half >= 0; --half) {
+                    const int x = 64 * half;
+                    uint32_t v[2][32];
+                    tmem_load32(s_at + x, v[0]);
+                    tmem_load32(s_at + x + 32, v[1]);
                     tmem_wait_load();
-                    if (__any_sync(0xffffffffu, seen < x + 32)) hide(v, seen - x);
+                    if (__any_sync(0xffffffffu, seen < x + 64)) { hide(v[0], seen - x); hide(v[1], seen - x - 32); }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 e = fma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), both(c), both(-base_m));
-                        const float2 w = make_float2(ex2(e.x), ex2(e.y));
-                        sum = add2(sum, w);
-                        p[i / 2] = pack_half(w.x, w.y);
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 e = fma2(make_float2(__uint_as_float(v[k][i]), __uint_as_float(v[k][i + 1])), both(c), both(-base_m));
+                            const float2 w = make_float2(ex2(e.x), ex2(e.y));
+                            sum = add2(sum, w);
+                            p[i / 2] = pack_half(w.x, w.y);
+                        }
+                        tmem_store16(s_at + x + 16 * k, p);
                     }
-                    tmem_store16(s_at + (x & 64) + (x & 32) / 2, p);
+                    tmem_wait_store();
+                    fence_before();
+                    arrive(bar(misc.p_full[t][half]));
                 }
-                tmem_wait_store();
-                fence_before();
-                arrive(bar(misc.p_full[t][half]));
                 l += sum.x + sum.y;
             }
             if (ok) ok = wait_warp(misc.o_done, 0);
             {
                 fence_after();
-                // the other half's sum, through the shared memory of Q, which is not needed any more
-                float* const sums = reinterpret_cast<float*>(smem + S::q) + t * 2 * kM;
-                sums[half * kM + r] = l;
-                asm volatile("bar.sync %0, %1;" ::"r"(3 + t), "n"(2 * kM) : "memory");
-                l += sums[(half ^ 1) * kM + r];
                 const bool rough = *const_cast<volatile int*>(&misc.rough) != 0;         // (computed elsewhere, and `out` may be `q`)
-                const float f = pow2i(-v_shift);
-                const float by = whole ? f / l : f;
-                const int64_t at = ((int64_t)q.row0 + token) * A.out.row_stride + (int64_t)head * A.out.head_stride;
-                const int64_t part = (((int64_t)item * H + h) * A.pieces + blockIdx.z) * (2 * kM) + t * kM + r;
+                float f = pow2i(-v_shift), other = 0.0f;
+                float* const odd_o = reinterpret_cast<float*>(smem + S::k) + r;           // [channel][row]: the odd tiles' output
+                if (turns && n_tiles > 1) {
+                    float* const odd_ml = reinterpret_cast<float*>(smem + S::q) + r;
+                    if (t == 1) {
+                        odd_ml[0] = m; odd_ml[kM] = l;
 #pragma unroll 1
-                for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 16) {
+                        for (int x = 0; x < D; x += 16) {
+                            uint32_t o[16];
+                            tmem_load16(o_at + x, o);
+                            tmem_wait_load();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) odd_o[(x + i) * kM] = __uint_as_float(o[i]) * f;
+                        }
+                    }
+                    asm volatile("bar.sync 3, %0;" ::"n"(2 * kM) : "memory");
+                    if (t == 0) {
+                        const float m_odd = odd_ml[0], m_new = fmaxf(m, m_odd), b = m_new == -INFINITY ? 0.0f : m_new, mine = ex2(m - b);
+                        other = ex2(m_odd - b);
+                        l = l * mine + odd_ml[kM] * other;
+                        f *= mine;
+                        m = m_new;
+                    }
+                }
+                const bool writes = there && !rough && t < n_sub;
+                const float by = whole ? 1.0f / l : 1.0f;
+                const int64_t at = ((int64_t)q.row0 + token) * A.out.row_stride + (int64_t)head * A.out.head_stride;
+                const int64_t part = (((int64_t)item * H + h) * A.pieces + blockIdx.z) * (2 * kM) + in_cta;
+#pragma unroll 1
+                for (int x = 0; x < D; x += 16) {
                     uint32_t o[16];
                     tmem_load16(o_at + x, o);
                     tmem_wait_load();
-                    if (!there || rough) continue;
+                    if (!writes) continue;
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        const float4 y = make_float4(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by, __uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by);
+                        float y_[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            y_[e] = __uint_as_float(o[i + e]) * f;
+                            if (turns && n_tiles > 1) y_[e] = fmaf(odd_o[(x + i + e) * kM], other, y_[e]);
+                        }
+                        const float4 y = make_float4(y_[0] * by, y_[1] * by, y_[2] * by, y_[3] * by);
                         if (whole) store_quad(A.out.data, A.out_dtype, at + x + i, y);
                         else *reinterpret_cast<float4*>(A.part_o + part * D + x + i) = y;
                     }
                 }
-                if (!whole && there && !rough && half == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m, l);
+                if (!whole && writes) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m, l);
                 fence_before();
             }
         }
@@ -708,14 +747,48 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         // ---------------- MMAs ----------------
         constexpr uint32_t kQK = mma_shape(kM, kN, false), kPV = mma_shape(kM, D, true);
         auto scores = [&](int t, int st) {
+            const uint32_t rows_at = base + S::q + (turns ? 0 : t) * S::kTileBytes;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const uint32_t off = (uint32_t)(i / 4) * (kM * 128) + (i % 4) * 32;
-                mma_ss(tmem + t * kN, smem_desc(base + S::q + t * S::kTileBytes + off, 16, 1024), smem_desc(base + S::k + st * S::kTileBytes + off, 16, 1024), kQK, i > 0);
+                mma_ss(tmem + t * kN, smem_desc(rows_at + off, 16, 1024), smem_desc(base + S::k + st * S::kTileBytes + off, 16, 1024), kQK, i > 0);
             }
             mma_commit(bar(misc.s_full[t]));
         };
-        bool ok = wait(misc.q_full, 0) && wait(misc.full[0][0], 0);
+        // weights of block t in turn n times values of stage st
+        auto contract = [&](int t, int st, int n) {
+            for (int half = 1; half >= 0; --half) {
+                if (!wait(misc.p_full[t][half], n)) return false;
+                fence_after();
+#pragma unroll
+                for (int i = 0; i < kN / 32; ++i)
+                    mma_ts(tmem + 2 * kN + t * D, tmem + t * kN + 64 * half + 8 * i, smem_desc(base + S::v + st * S::kTileBytes + (4 * half + i) * 2048, kN * 128, 1024), kPV,
+                           n > 0 || half == 0 || i > 0);
+            }
+            return true;
+        };
+        bool ok = wait(misc.q_full, 0);
+        if (turns) {
+            // tile j is block j % 2's, in stage j % 2: scores of the next tile are there before this one's weights are
+            for (int j = 0; ok && j < n_tiles + 2; ++j) {
+                const int t = j & 1;
+                if (j >= 2) {
+                    ok = wait(misc.full[1][t], (j - 2) >> 1) && contract(t, t, (j - 2) >> 1);
+                    if (!ok) break;
+                    mma_commit(bar(misc.empty[1][t]));
+                }
+                if (j < n_tiles) {
+                    ok = wait(misc.full[0][t], j >> 1);
+                    if (!ok) break;
+                    fence_after();
+                    scores(t, t);
+                    mma_commit(bar(misc.empty[0][t]));
+                }
+            }
+            if (ok) mma_commit(bar(misc.o_done));
+            ok = false;                                  // (done)
+        }
+        ok = ok && wait(misc.full[0][0], 0);
         if (ok) {
             fence_after();
             for (int t = 0; t < n_sub; ++t) scores(t, 0);
@@ -725,14 +798,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 const bool more = j + 1 < n_tiles;
                 if (!wait(misc.full[1][st], j >> 1)) { ok = false; break; }
                 for (int t = 0; t < n_sub; ++t) {
-                    for (int half = 1; ok && half >= 0; --half) {
-                        if (!wait(misc.p_full[t][half], j)) { ok = false; break; }
-                        fence_after();
-#pragma unroll
-                        for (int i = 0; i < kN / 32; ++i)
-                            mma_ts(tmem + 2 * kN + t * D, tmem + t * kN + 64 * half + 8 * i, smem_desc(base + S::v + st * S::kTileBytes + (4 * half + i) * 2048, kN * 128, 1024), kPV,
-                                   j > 0 || half == 0 || i > 0);
-                    }
+                    ok = contract(t, st, j);
                     if (t == 0 && more && ok) ok = wait(misc.full[0][st ^ 1], (j + 1) >> 1);
                     if (!ok) break;
                     if (more) scores(t, st ^ 1);

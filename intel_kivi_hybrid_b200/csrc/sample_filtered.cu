@@ -22,6 +22,12 @@
 // Masses: 2^(k/32) from a table in fp64, times 1 and a correction below 2^-6 in fp32 (good to
 // 2^-29).  The exponent x c - L, c = 32 log2(e) / T, is taken with L on a grid on
 // which L and the whole number k add exactly, so one fused operation leaves its fraction.
+//
+// Bound by issue slots where rows are long, most of them the third walk's (130000 bf16 logits:
+// 140000 cycles a row, of them maximum 11000, bins 23000-31000, third walk 75000), else by
+// latency: fifteen barriers and what hangs on them.  50257 fp32 logits: one row 26 us, 128 rows
+// of all filters 33; 64 rows of 130000 bf16 73-81.  Integer instructions take two slots, so
+// masses use few of them (two-word masses by bit operations: 92 us).
 #include "kivi_common.cuh"
 
 #include <type_traits>

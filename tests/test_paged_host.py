@@ -63,6 +63,26 @@ def test_pages_are_taken_given_back_and_run_out():
             PagedKiviCache(*args)
 
 
+def test_steps_that_are_given_up_are_closed():
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(1, 64, 1, num_pages=4, max_sequences=2, page_tokens=64, group_size=32, residual_length=64, device="cpu")
+    a, b = cache.add_sequence(), cache.add_sequence()
+    first = cache.begin([a, b], [3, 4])
+    again = cache.begin([a], [5], max_len=50)
+    assert not first.open and again.open
+    cache.end(again)
+    assert cache.length(a) == 5 and cache.length(b) == 0
+    other = cache.begin([a, b], [1, 1])
+    cache.free(b)
+    with pytest.raises(AssertionError, match="has ended"):
+        cache.end(other)
+    cache.refresh(again)
+    assert again.open and again.seq_lens.tolist() == [5]
+    cache.end(again)
+    with pytest.raises(AssertionError, match="not there"):
+        cache.refresh(first)
+
+
 def test_the_c_interface_refuses_before_it_launches(cabi):
     lib, byref = cabi.lib, ctypes.byref
     some = 4096                                             # an address on a 16-byte boundary; nothing follows it
