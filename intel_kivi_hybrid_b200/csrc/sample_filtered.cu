@@ -2,7 +2,7 @@
 // random numbers.
 //
 // m_i = exp((x_i - max) / temperature) needs no normalisation: every cut compares masses
-// with masses.  A CTA walks its row up to four times, each from L2:
+// with masses.  A CTA (or a few, of a long row) walks its row up to four times, each from L2:
 //   1. the largest entry and its first index;
 //   2. (top-k or top-p) entries per bin of 1/256 octave of mass, 32 octaves: the counts give
 //      the bin that the k-th largest is in, and bound the mass above any bin to 0.15 %, which
@@ -23,20 +23,28 @@
 // 2^-29).  The exponent x c - L, c = 32 log2(e) / T, is taken with L on a grid on
 // which L and the whole number k add exactly, so one fused operation leaves its fraction.
 //
-// Bound by issue slots where rows are long, most of them the third walk's (130000 bf16 logits:
-// 140000 cycles a row, of them maximum 11000, bins 23000-31000, third walk 75000), else by
-// latency: fifteen barriers and what hangs on them.  50257 fp32 logits: one row 26 us, 128 rows
-// of all filters 33; 64 rows of 130000 bf16 73-81.  Integer instructions take two slots, so
+// Bound by issue slots where rows are long, most of them the third walk's (130000 bf16 logits in
+// one CTA: 140000 cycles a row, of them maximum 11000, bins 23000-31000, third walk 75000), else by
+// latency: fifteen barriers and what hangs on them.  50257 fp32 logits: one row 29 us, 128 rows
+// of all filters 33; 64 rows of 130000 bf16 60.  Integer instructions take two slots, so
 // masses use few of them (two-word masses by bit operations: 92 us).
 #include "kivi_common.cuh"
 
+#include <cooperative_groups.h>
 #include <type_traits>
+
+namespace cg = cooperative_groups;
 
 namespace kivi {
 namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 static_assert(kWarps == 32, "a warp looks after 32 warps' results, and fills a row of the table");
+// CTAs of a row (a cluster), and the entries that one is worth: adding up the bins of the others and
+// five barriers cost about what 20000 entries take.  us with one, two, four and eight CTAs, top-p: 16 x 130000
+// bf16 60 46 37 69 (16 clusters of eight do not all find room), 64 x 130000 81 60, 64 x 50257 fp32 42 37,
+// 16 x 50257 35 33 32 63, 1 x 50257 28 29 30 36, 8 x 16000 19 23 24.
+constexpr int kMaxCtas = 4, kLeast = 25000;
 constexpr int kBins = 8192;                              // of 1/256 octave; the last holds what is below 2^-32
 constexpr int kPerThread = kBins / kThreads;
 constexpr int kListK = 2048, kListP = 8192;              // entries at the k-th largest, at the end of the nucleus
@@ -62,10 +70,14 @@ struct Shared {
     unsigned long long mass_p[kListP];                   // in whole units
     uint2 table[32][32];                                 // 2^(i/32), less the constant of power(); a column for each lane: no two lanes meet in a bank
     double sum[kWarps], runs[kWarps];
-    uint32_t range[256][3], run_units[kWarps][3];        // whole units in three parts of 18 bits
+    uint32_t range[256][3], run_units[kMaxCtas * kWarps][3];         // whole units in three parts of 18 bits
+    // from all CTAs of the row (the last three: to the first one)
+    uint32_t peer_key[kMaxCtas];
+    int peer_first[kMaxCtas];
+    double all_runs[kMaxCtas * kWarps], sum_in[kMaxCtas], sum_over[kMaxCtas];
     unsigned long long wide_range[256], open_base;
     uint32_t open_lo, open_hi;
-    int draw_lo, draw_hi;
+    int draw_lo, draw_hi, draw_run;
     float part[kWarps];
     int count[kWarps];
     uint32_t key[kWarps];
@@ -88,21 +100,20 @@ __device__ __forceinline__ double warp_sum(double x) {
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
-// Sums over the block of three numbers of each thread, and of the second over each warp, through
-// 24 KB of shared memory: four warps add them up (32 warps that shuffle share one pipe: 2500 cycles
+// Sums over the block of two numbers of each thread, and of the second over each warp, through
+// 16 KB of shared memory: three warps add them up (32 warps that shuffle share one pipe: 2500 cycles
 // for a sum).
-__device__ __forceinline__ void block_sums(double a, double b, double c, double* scratch, double* out, double* runs) {
+__device__ __forceinline__ void block_sums(double a, double b, double* scratch, double* out, double* runs) {
     scratch[threadIdx.x] = a;
     scratch[kThreads + threadIdx.x] = b;
-    scratch[2 * kThreads + threadIdx.x] = c;
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp < 4) {
+    if (warp < 3) {
         double x[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) x[i & 3] += scratch[warp == 3 ? kThreads + 32 * lane + ((i + lane) & 31) : warp * kThreads + 32 * i + lane];
+        for (int i = 0; i < kWarps; ++i) x[i & 3] += scratch[warp == 2 ? kThreads + 32 * lane + ((i + lane) & 31) : warp * kThreads + 32 * i + lane];
         const double sum = (x[0] + x[1]) + (x[2] + x[3]);
-        if (warp == 3) runs[lane] = sum;
+        if (warp == 2) runs[lane] = sum;
         else {
             const double all = warp_sum(sum);
             if (lane == 0) out[warp] = all;
@@ -235,20 +246,27 @@ struct Masses {
     }
 };
 
-template <typename T>
+// kMany: a cluster of CTAs has a row.  Each walks its part; bins are added up by all, lists and sums go
+// to the first, which ends the draw.  What the CTAs decide on (bins, thresholds) is the same in all.
+template <typename T, bool kMany>
 __global__ void __launch_bounds__(kThreads, 1)
 sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArgs f, int64_t* __restrict__ ids) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = kMany ? (int)cluster.num_blocks() : 1, rank = kMany ? (int)cluster.block_rank() : 0, b = (int)blockIdx.x / ctas;
+    Shared& lead = kMany ? *cluster.map_shared_rank(&s, 0) : s;
+    auto sync_row = [&] { if constexpr (kMany) cluster.sync(); else __syncthreads(); };
     {
         const double t = exp2((double)warp * (1.0 / 32.0));
         s.table[warp][lane] = make_uint2((uint32_t)__double2loint(t), (uint32_t)__double2hiint(t) - 0x4b400000u * 32768u);
     }
     if (tid == 0) { s.first = 0x7fffffff; s.bin_k = kBins; s.need = 0; s.zone_lo = kBins; s.zone_hi = -1; s.n_k = 0; s.n_p = 0; s.min_key = 0u; }
-    if (tid < 3 * kWarps) s.run_units[tid / 3][tid % 3] = 0u;
+    if (tid < 3 * kMaxCtas * kWarps) s.run_units[tid / 3][tid % 3] = 0u;
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0u;
     stream_order();
+    if constexpr (kMany) cluster.sync();                 // (all are there, and their shared memory is laid out)
     const T* const row = settled(logits) + (int64_t)b * row_stride;
     const float u = settled(f.uniforms)[b], temperature = f.temperature ? settled(f.temperature)[b] : 1.0f;
     const float top_p = f.top_p ? settled(f.top_p)[b] : 1.0f, min_p = f.min_p ? settled(f.min_p)[b] : 0.0f;
@@ -261,18 +279,33 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     // ---- 1. the largest and its first index ----
     float best = -INFINITY;
     int at = 0x7fffffff;
-    walk(row, 0, vocab, tid, kThreads, [&](float x, int i) {
+    const int n_runs = ctas * kWarps, run = (vocab + n_runs - 1) / n_runs;          // a warp's part of the row
+    const int part_lo = min(rank * kWarps * run, vocab), part_hi = min(part_lo + kWarps * run, vocab);
+    walk(row, part_lo, part_hi, tid, kThreads, [&](float x, int i) {
         if (x > best || (x == best && i < at)) { best = x; at = i; }
     });
     const uint32_t mine = ordered_key(best), warp_best = __reduce_max_sync(0xffffffffu, mine);
     if (lane == 0) s.key[warp] = warp_best;
     __syncthreads();
-    const uint32_t top = __reduce_max_sync(0xffffffffu, s.key[lane]);
+    uint32_t top = __reduce_max_sync(0xffffffffu, s.key[lane]);
     if (mine == top) atomicMin(&s.first, at);
     __syncthreads();
+    int first = s.first;
+    if constexpr (kMany) {
+        if (tid < ctas) {
+            Shared& to = *cluster.map_shared_rank(&s, tid);
+            to.peer_key[rank] = top;
+            to.peer_first[rank] = first;
+        }
+        cluster.sync();
+        for (int c = 0; c < ctas; ++c) top = max(top, s.peer_key[c]);
+        first = 0x7fffffff;
+        for (int c = 0; c < ctas; ++c)
+            if (s.peer_key[c] == top) first = min(first, s.peer_first[c]);
+    }
     const float largest = key_to_float(top);
     if (!(temperature > 0.0f) || largest == -INFINITY) {
-        if (tid == 0) ids[b] = largest == -INFINITY ? 0 : s.first;
+        if (tid == 0 && rank == 0) ids[b] = largest == -INFINITY ? 0 : first;
         return;
     }
     Masses m;
@@ -295,26 +328,36 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
     };
 
     uint32_t cut = 0u;                                   // least key that is kept
-    bool sums_known = false;
+    bool sums_known = false, alone = !kMany;             // alone: the others have left
     if (cut_p && top_p <= 0.0f && !m.only_largest) cut = top;
     else if ((cut_k || cut_p) && !m.only_largest) {
         // ---- 2. entries per bin ----
         uint32_t far = 0u;                               // (entries of the last bin would all meet in one place)
-        walk<T, 4>(row, 0, vocab, tid, kThreads, [&](float x, int) {
+        walk<T, 4>(row, part_lo, part_hi, tid, kThreads, [&](float x, int) {
             const int bin = m.bin(x);
             if (bin == kBins - 1) ++far;
             else if (bin >= 0) atomicAdd(&s.bins[bin], 1u);
         });
         far = __reduce_add_sync(0xffffffffu, far);
         if (lane == 0 && far) atomicAdd(&s.bins[kBins - 1], far);
-        __syncthreads();
+        sync_row();
         int count[kPerThread], n = 0;
         float mass = 0.0f;                               // of the thread's bins, by their centres
         const float first_w = exp2f((float)-(tid * kPerThread) * (1.0f / 256.0f));
         auto weight = [&](int i) { return first_w * (float)(1.0 - 0.0027076062 * i + 0.0000036655656 * i * i); };        // 2^(-i/256), i < 8, to 2^-19
 #pragma unroll
+        for (int i = 0; i < kPerThread; ++i) count[i] = (int)s.bins[tid * kPerThread + i];
+        if constexpr (kMany) {
+            for (int c = 1; c < ctas; ++c) {
+                const uint4* other = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s, (rank + c) % ctas)->bins + tid * kPerThread);
+                const uint4 x = other[0], y = other[1];
+                count[0] += x.x; count[1] += x.y; count[2] += x.z; count[3] += x.w;
+                count[4] += y.x; count[5] += y.y; count[6] += y.z; count[7] += y.w;
+            }
+            cluster.sync();                              // (the bins become scratch)
+        }
+#pragma unroll
         for (int i = 0; i < kPerThread; ++i) {
-            count[i] = (int)s.bins[tid * kPerThread + i];
             n += count[i];
             mass += (float)count[i] * weight(i);
         }
@@ -386,18 +429,17 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         // ---- 3. exact masses ----
         // (one above the largest finite number's key is that of +infinity)
         const float over_x = key_to_float(over_key), zone_x = cut_p ? key_to_float(s.zone_key) : INFINITY, in_x = key_to_float(s.in_key), k_x = key_to_float(s.k_key);
-        const int run = (vocab + kWarps - 1) / kWarps;
         double in = 0.0, over = 0.0;                     // before the k-th largest's bin; above the zone
         auto put = [&](float x, int i) {
-            const int j = atomicAdd(&s.n_p, 1);
-            if (j < kListP) { s.list_p[j] = {ordered_key(x), i}; s.mass_p[j] = units(m.get(x)); }
+            const int j = atomicAdd(&lead.n_p, 1);
+            if (j < kListP) { lead.list_p[j] = {ordered_key(x), i}; lead.mass_p[j] = units(m.get(x)); }
         };
         auto third = [&](auto narrow) {
-            walk<T, 1>(row, min(warp * run, vocab), min(warp * run + run, vocab), lane, 32, [&](float x, int i) {
+            walk<T, 1>(row, min(part_lo + warp * run, part_hi), min(part_lo + warp * run + run, part_hi), lane, 32, [&](float x, int i) {
                 if (cut_k && !(x >= in_x)) {
                     if (x >= k_x) {                      // of the k-th largest's bin
-                        const int j = atomicAdd(&s.n_k, 1);
-                        if (j < kListK) s.list_k[j] = {ordered_key(x), i};
+                        const int j = atomicAdd(&lead.n_k, 1);
+                        if (j < kListK) lead.list_k[j] = {ordered_key(x), i};
                         if (x < over_x && x >= zone_x) put(x, i);
                     }
                     return;
@@ -411,6 +453,14 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         if (m.narrow) third(std::true_type{});
         else third(std::false_type{});
         __syncthreads();
+        block_sums(in, over, reinterpret_cast<double*>(s.bins), s.sum, s.runs);
+        if (tid < kWarps) lead.all_runs[rank * kWarps + tid] = s.runs[tid];
+        if (tid == 0) { lead.sum_in[rank] = s.sum[0]; lead.sum_over[rank] = s.sum[1]; }
+        sync_row();
+        if (rank != 0) return;
+        alone = true;
+        double all_in = 0.0, all_over = 0.0;
+        for (int c = 0; c < ctas; ++c) { all_in += s.sum_in[c]; all_over += s.sum_over[c]; }
         const int n_k = s.n_k, n_p = s.n_p;
         // The largest key at which the amounts of a list's entries at or above it reach `most` (0: nowhere),
         // among keys from `floor` on: 256 ranges of keys at a time.
@@ -519,11 +569,13 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                     walk(row, 0, vocab, tid, kThreads, [&](float x, int) { if (m.bin(x) == bin_k && ordered_key(x) >= cut) add_rest(x); });
                 }
             }
-            __syncthreads();
-            block_sums(in, over, rest, reinterpret_cast<double*>(s.bins), s.sum, s.runs);
-            double most = (double)top_p * (s.sum[0] + s.sum[2] / unit);
+            if (bin_k < kBins) {
+                __syncthreads();
+                block_sums(rest, 0.0, reinterpret_cast<double*>(s.bins), s.sum, s.runs);
+                all_in += s.sum[0] / unit;
+            }
             // (the least key above which there is less than top_p is the largest one at or above which there is no less)
-            most = (most - s.sum[1]) * unit;
+            const double most = ((double)top_p * all_in - all_over) * unit;
             uint32_t key = top;                          // (never: what is above the zone is less)
             if (most > 0.0) {
                 const unsigned long long most_u = (unsigned long long)__double2ll_ru(most);
@@ -542,7 +594,6 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             cut = max(cut, min(key, top));
         } else {
             sums_known = bin_k >= kBins || n_k <= kListK;
-            if (sums_known) block_sums(0.0, over, 0.0, reinterpret_cast<double*>(s.bins), s.sum, s.runs);
         }
         cut = max(cut, s.min_key);
         if (sums_known) {                                // what is kept of the list, to its runs
@@ -553,7 +604,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                 add_units(s.run_units[e.index / run], cut_p ? s.mass_p[i] : units(m.get(key_to_float(e.key))));
             }
             __syncthreads();
-            if (tid < kWarps) s.runs[tid] += (double)units_of(s.run_units[tid]) / unit;
+            if (tid < n_runs) s.all_runs[tid] += (double)units_of(s.run_units[tid]) / unit;
             __syncthreads();
         }
         }
@@ -574,14 +625,52 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         walk<T, 1>(row, lo, hi, lane, 32, [&](float v, int) { if (v >= cut_x) x += m.get(v); });
         return warp_sum(x);
     };
-    int lo = 0, hi = vocab;
+    if (!sums_known) {
+        // (a list that did not fit: the first CTA does the others' runs too)
+        for (int c = alone ? 0 : rank; c < (alone ? ctas : rank + 1); ++c) {
+            const int a = min((c * kWarps + warp) * run, vocab);
+            const double sum = run_sum(a, min(a + run, vocab));
+            if (lane == 0) lead.all_runs[c * kWarps + warp] = sum;
+        }
+        if (alone) __syncthreads();
+        else sync_row();
+        if (rank != 0) return;
+    }
+    // The run that the sum passes the target in, then the piece of it; the last with a mass where roundings
+    // leave none.  (before, target: the first warp's)
     double before = 0.0, target = 0.0;
-    for (int level = 0; level < 2; ++level) {
-        // the run of 32 that the sum passes the target in; the last with a mass where roundings leave none
+    int lo, hi;
+    if (warp == 0) {
+        double mine = 0.0;
+        for (int c = 0; c < ctas; ++c) mine += s.all_runs[lane * ctas + c];
+        double upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        target = (double)u * __shfl_sync(0xffffffffu, upto, 31);
+        const unsigned passes = __ballot_sync(0xffffffffu, mine > 0.0 && upto > target), holds = __ballot_sync(0xffffffffu, mine > 0.0);
+        const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
+        double at_run = __shfl_sync(0xffffffffu, upto - mine, w);
+        int pick = w * ctas;
+        for (int c = 0; c < ctas; ++c) {                 // (all lanes the same)
+            const double x = s.all_runs[w * ctas + c];
+            if (!(x > 0.0)) continue;
+            pick = w * ctas + c;
+            before = at_run;
+            if (at_run + x > target) break;
+            at_run += x;
+        }
+        if (lane == 0) s.draw_run = pick;
+    }
+    __syncthreads();
+    lo = min(s.draw_run * run, vocab);
+    hi = min(lo + run, vocab);
+    {
         const int per = (hi - lo + kWarps - 1) / kWarps;
         const int a = min(lo + warp * per, hi), z = min(a + per, hi);
-        const double sum = level == 0 && sums_known ? s.runs[warp] : run_sum(a, z);
-        __syncthreads();
+        const double sum = run_sum(a, z);
         if (lane == 0) s.sum[warp] = sum;
         __syncthreads();
         if (warp == 0) {
@@ -592,7 +681,6 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                 const double x = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += x;
             }
-            if (level == 0) target = (double)u * __shfl_sync(0xffffffffu, upto, 31);
             const unsigned passes = __ballot_sync(0xffffffffu, some && before + upto > target), holds = __ballot_sync(0xffffffffu, some);
             const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
             before += __shfl_sync(0xffffffffu, upto, w) - s.sum[w];
@@ -637,12 +725,19 @@ extern "C" int kivi_sample_filtered(const void* logits, int dtype, int batch, in
     // (indices step past the end of a row)
     KIVI_REQUIRE(vocab <= (1 << 30), "vocab (%d) must be at most 2^30", vocab);
     const FilterArgs f{uniforms, temperature, top_p, min_p, top_k};
+    // As many CTAs to a row as the GPU has to spare, each with its share of entries.
+    int ctas = 1;
+    while (ctas < kMaxCtas && (int64_t)batch * ctas * 2 <= num_sms() && vocab / (ctas * 2) >= kLeast) ctas *= 2;
     auto go = [&](auto* kernel, auto* x) {
         KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
-        KIVI_CUDA_OK(launch(kernel, dim3((unsigned)batch), kThreads, sizeof(Shared), (cudaStream_t)stream, true, x, vocab, row_stride, f, ids_out));
+        KIVI_CUDA_OK(launch_cluster(kernel, ctas > 1 ? ctas : 0, dim3((unsigned)batch * (unsigned)ctas), kThreads, sizeof(Shared), (cudaStream_t)stream, true, x, vocab, row_stride, f, ids_out));
         note_launches(1);
         return KIVI_OK;
     };
-    return dtype == KIVI_BF16 ? go(sample_filtered_kernel<__nv_bfloat16>, reinterpret_cast<const __nv_bfloat16*>(logits))
-                              : go(sample_filtered_kernel<float>, reinterpret_cast<const float*>(logits));
+    auto of = [&](auto many) {
+        constexpr bool kMany = decltype(many)::value;
+        return dtype == KIVI_BF16 ? go(sample_filtered_kernel<__nv_bfloat16, kMany>, reinterpret_cast<const __nv_bfloat16*>(logits))
+                                  : go(sample_filtered_kernel<float, kMany>, reinterpret_cast<const float*>(logits));
+    };
+    return ctas > 1 ? of(std::true_type{}) : of(std::false_type{});
 }

@@ -66,7 +66,7 @@ class KiviPastKeyValues(DynamicCache):
 
 def _mask_hides_something(attention_mask) -> bool:
     """True if an attention mask excludes any key position (costs a device sync:
-    only evaluated for batched decode steps, where padding can occur)."""
+    only evaluated for batched decode steps, where padding can occur, and for chunks)."""
     if attention_mask is None:
         return False
     if attention_mask.dtype == torch.bool:
@@ -109,7 +109,7 @@ def kivi_fused_attention(module, query, key, value, attention_mask, dropout=0.0,
         out = cache.decode_attention(layer, q.contiguous(), sm_scale=float(scaling or 0.0))
         return out.to(query.device, query.dtype).reshape(B, 1, Hq, D), None
     if history > 0 and getattr(module, "_kivi_chunked", False):
-        if B > 1 and _mask_hides_something(None if attention_mask is None else attention_mask[..., -1:, :]):
+        if _mask_hides_something(None if attention_mask is None else attention_mask[..., -1:, :]):
             raise RuntimeError("kivi_fused attention: the chunk's attention_mask hides key positions from its last token (padded batch); "
                                "the fused kernel attends to every cached token. Use get_full_cache() for padded batches.")
         out = cache.chunk_attention(layer, query, key, value, sm_scale=float(scaling or 0.0))

@@ -195,3 +195,22 @@ def test_flat_rows_low_temperatures_and_shifted_logits(ops, dtype):
 def test_one_row_for_many_draws(ops):
     x = torch.randn(1, 5000, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
     check(ops, x.expand(64, 5000), uniforms(64, 12), [1.1] * 64, [40] * 64, [0.9] * 64)
+
+
+@pytest.mark.parametrize("B", [1, 37, 74, 75])
+@pytest.mark.parametrize("V", [50000, 100003, 131071])
+def test_rows_of_several_ctas(ops, B, V):
+    """Long rows of small batches are cut between CTAs: ties across their borders, the largest in the last part, nothing kept in
+    some parts, cuts whose lists do not fit, rows without a cut."""
+    g = torch.Generator(device="cuda").manual_seed(V + B)
+    x = 2 * torch.randn(B, V, generator=g, device="cuda")
+    x[0, V - 1] = 30.0
+    x[B // 2, ::2] = 1.25
+    x[B - 1, :V // 3] = -math.inf
+    x[B - 1, V // 2] = math.inf if B > 1 else 5.0
+    u = uniforms(B, V)
+    pick = lambda *a: [a[i % len(a)] for i in range(B)]  # noqa: E731
+    check(ops, x, u, pick(1.0, 0.0, 0.7, 30.0), pick(0, 40, 20000), pick(0.9, 1.0, 0.5, 0.0, 0.99), pick(0.0, 0.05, 0.0, 0.5, 0.0))
+    check(ops, x.bfloat16(), u, pick(1.0, 0.6), None, pick(0.95, 0.3, 1.0), None)
+    check(ops, x, u)
+    check(ops, x, u, None, None, None, pick(0.2, 0.001))
