@@ -39,9 +39,13 @@
 // 5500.  A block's chain is what bounds it: maximum 630-1000, weights 2800 while the other block
 // makes its own, then 1400 until P V and the next scores are done.  One block: 4300, of which the
 // conversion of a tile takes 2800-3100 (bf16, 32k tokens).
-// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 398 us, 700 TFLOP/s; 4 x 2048 over
-// 16k 3262 us; 16 x 5 tokens over 4k 85 us (101 with one group of softmax warps for its one block).
-// Lost: two threads to a row that meet for its maximum (406, 3323); scores in halves of 64 tokens,
+// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 391 us, 710 TFLOP/s; 4 x 2048 over
+// 16k 3246 us; 16 x 5 tokens over 4k 78 us.  The roles share an instruction cache, so bodies are
+// small: with the MMAs of a tile and four tokens of a key quad side by side 403, 3280, 90, with the
+// conversions' channels unrolled too 423, 3393, 99; but weights by 32 columns 426, 3440 (81) and
+// values a token at a time 394, 3271, 88.
+// Lost: two threads to a row that meet for its maximum (406, 3323, 101 with one group of softmax
+// warps for one block); scores in halves of 64 tokens,
 // so that the next half's are made meanwhile (471, 3753: twice the dependent MMAs in a row);
 // maxima of the halves one after the other, without a pass for them (439, 3594: spills).
 #include "async_copy.cuh"
@@ -371,14 +375,13 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 // (loops of one body: the roles share an instruction cache, unrolled ones cost 15 % of the call)
                 float top = -INFINITY;
 #pragma unroll 1
-                for (int x = 0; x < kN; x += 64) {
-                    uint32_t v[2][32];
-                    tmem_load32(s_at + x, v[0]);
-                    tmem_load32(s_at + x + 32, v[1]);
+                for (int x = 0; x < kN; x += 32) {
+                    uint32_t v[32];
+                    tmem_load32(s_at + x, v);
                     tmem_wait_load();
-                    if (__any_sync(0xffffffffu, seen < x + 64)) { hide(v[0], seen - x); hide(v[1], seen - x - 32); }
+                    if (__any_sync(0xffffffffu, seen < x + 32)) hide(v, seen - x);
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[i / 32][i % 32]), __uint_as_float(v[i / 32][i % 32 + 1])));
+                    for (int i = 0; i < 32; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
                 }
                 top *= c;
                 // (V of tile j + 2 is not made before this tile's weights are contracted, so the barrier's phase is this tile's)
@@ -522,9 +525,6 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         auto convert_keys = [&](uint32_t raw, uint32_t to, float f) {
             const int c = lane & 3, m = lane >> 2 & 1, jq = lane >> 3;
             const uint32_t ch = 16 * c + 8 * m;
-            uint32_t turn[4];                                        // pieces of the rows, swizzled
-#pragma unroll
-            for (int n = 0; n < 4; ++n) turn[n] = to + (4 * jq + n) * 128 + (((2 * c + m) ^ ((4 * jq + n) & 7)) << 4);
 #pragma unroll 1
             for (int hw = 0; hw < D / 64; ++hw) {
                 uint32_t s2[4], z2[4], x[2][4];
@@ -540,14 +540,15 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     x[i][0] = __byte_perm(a, 0u, 0x4140); x[i][1] = __byte_perm(a, 0u, 0x4342);
                     x[i][2] = __byte_perm(b, 0u, 0x4140); x[i][3] = __byte_perm(b, 0u, 0x4342);
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int n = 0; n < 4; ++n) {
+                    const uint32_t turn = to + (4 * jq + n) * 128 + (((2 * c + m) ^ ((4 * jq + n) & 7)) << 4);      // piece of the row, swizzled
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint32_t y[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & (0x00030003u << (2 * n))) | k1024, kMinus1024), s2[e], z2[e]);
-                        sts128(turn[n] + hw * (kN * 128) + i * (16 * 128), y[0], y[1], y[2], y[3]);
+                        sts128(turn + hw * (kN * 128) + i * (16 * 128), y[0], y[1], y[2], y[3]);
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s2[e] = hmul2(s2[e], 0x34003400u);        // a quarter
@@ -748,7 +749,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         constexpr uint32_t kQK = mma_shape(kM, kN, false), kPV = mma_shape(kM, D, true);
         auto scores = [&](int t, int st) {
             const uint32_t rows_at = base + S::q + (turns ? 0 : t) * S::kTileBytes;
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < D / 16; ++i) {
                 const uint32_t off = (uint32_t)(i / 4) * (kM * 128) + (i % 4) * 32;
                 mma_ss(tmem + t * kN, smem_desc(rows_at + off, 16, 1024), smem_desc(base + S::k + st * S::kTileBytes + off, 16, 1024), kQK, i > 0);
@@ -760,7 +761,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             for (int half = 1; half >= 0; --half) {
                 if (!wait(misc.p_full[t][half], n)) return false;
                 fence_after();
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < kN / 32; ++i)
                     mma_ts(tmem + 2 * kN + t * D, tmem + t * kN + 64 * half + 8 * i, smem_desc(base + S::v + st * S::kTileBytes + (4 * half + i) * 2048, kN * 128, 1024), kPV,
                            n > 0 || half == 0 || i > 0);
