@@ -25,9 +25,12 @@ __device__ int g_fault = 0;
 
 constexpr int kTile = 64;                                // tokens in shared memory at a time
 constexpr int kAtOnce = 4;
+constexpr int kTensorRows = 256;                         // of a CTA on the tensor cores
 
 // DT: head_dim 64 or 128, or 256 for any up to that.
-template <int RPT, int TY, int DT>
+// AGAIN: the same for the pieces of the tensor-core kernel's blocks (256 rows) that it has flagged, in place
+// of what it would have written; four CTAs to such a piece.
+template <int RPT, int TY, int DT, bool AGAIN = false>
 __global__ void __launch_bounds__(TY * 16)
 paged_attention_kernel(PagedAttnArgs A) {
     constexpr int RT = RPT * TY, kThreads = TY * 16, NC = DT / 64;       // NC: quads of channels a thread has
@@ -43,12 +46,17 @@ paged_attention_kernel(PagedAttnArgs A) {
     float* const v_s = k_s + kTile * S;                  // [kTile][S]
     float* const p_s = v_s + kTile * S;                  // [RT][kTile + 4]
     const int h = blockIdx.y, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) report_left_out(L, A.b, &g_fault);
+    constexpr int BT = AGAIN ? kTensorRows : RT;         // rows of a block
+    const int block = AGAIN ? blockIdx.x / (BT / RT) : blockIdx.x, row_in_block = AGAIN ? blockIdx.x % (BT / RT) * RT : 0;
+    const int64_t unit = (int64_t)block * H + h;
+    // (a block that no sequence has may hold any flag, and is not found below)
+    if (AGAIN && A.rough[unit * A.pieces + blockIdx.z] == 0) return;
+    if (!AGAIN && blockIdx.x + blockIdx.y + blockIdx.z == 0) report_left_out(L, A.b, &g_fault);
     if (tid < 32) {
-        const ItemPlace p = find_item(blockIdx.x, A.b.num_seqs, [&](int i) {
+        const ItemPlace p = find_item(block, A.b.num_seqs, [&](int i) {
             PagedSeq q;
             load_seq(L, A.b, i, q);
-            return (int)(((int64_t)q.n * A.n_rep + RT - 1) / RT);
+            return (int)(((int64_t)q.n * A.n_rep + BT - 1) / BT);
         });
         if (tid == 0) { place_s[0] = p.s; place_s[1] = p.sub; }
     }
@@ -57,10 +65,12 @@ paged_attention_kernel(PagedAttnArgs A) {
     if (s >= A.b.num_seqs) return;
     PagedSeq q;
     load_seq(L, A.b, s, q);                              // (sequences left out have no items)
-    const int n_rep = A.n_rep, rows = q.n * n_rep, row_first = place_s[1] * RT;
+    const int n_rep = A.n_rep, rows = q.n * n_rep, row_first = place_s[1] * BT + row_in_block;
     const int n_rows = rows - row_first < RT ? rows - row_first : RT;
+    if (AGAIN && n_rows <= 0) return;
     const int inside = min(quant_of(q.held + q.n, G, R), q.held);        // tokens read from pages
-    const int keys = q.held + (row_first + n_rows - 1) / n_rep + 1;      // tokens the block's last row sees
+    const int last_row = min(place_s[1] * BT + BT, rows) - 1;
+    const int keys = q.held + last_row / n_rep + 1;      // tokens the block's last row sees
     const int t_begin = blockIdx.z * A.chunk;
     if (t_begin >= keys) return;
     const int t_end = min(t_begin + A.chunk, keys);
@@ -241,7 +251,6 @@ paged_attention_kernel(PagedAttnArgs A) {
         else weigh(std::false_type{});
         __syncwarp();
     }
-    const int64_t unit = (int64_t)blockIdx.x * H + h;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
 #pragma unroll
@@ -256,7 +265,7 @@ paged_attention_kernel(PagedAttnArgs A) {
                 if (4 * tx + 64 * c < D)
                     store_quad(A.out.data, A.out_dtype, at + 4 * tx + 64 * c, make_float4(o[i][4 * c] * inv, o[i][4 * c + 1] * inv, o[i][4 * c + 2] * inv, o[i][4 * c + 3] * inv));
         } else {
-            const int64_t part = (unit * A.pieces + blockIdx.z) * RT + r;
+            const int64_t part = (unit * A.pieces + blockIdx.z) * BT + row_in_block + r;
             if (tx == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m[i] * A.scale_log2, l[i]);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
@@ -266,51 +275,9 @@ paged_attention_kernel(PagedAttnArgs A) {
     }
 }
 
-// A row of the step in fp32 over all its tokens, by a warp: a lane per token of 32, then per four of
-// up to 128 channels.
-__device__ void row_in_fp32(const PagedAttnArgs& A, const PagedSeq& q, int h, int row, int inside, int lane) {
-    const int n_rep = A.n_rep, D = A.L.head_dim, d = 4 * lane, token = row / n_rep, head = h * n_rep + row % n_rep, last = q.held + token;
-    const bool vec = A.vec != 0;
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int t0 = 0; t0 <= last; t0 += 32) {
-        float s = -INFINITY;
-        if (t0 + lane <= last) {
-            s = 0.0f;
-#pragma unroll 1
-            for (int e = 0; e < D; e += 4) {
-                const float4 a = load4_as(A.q, A.q_dtype, (int64_t)q.row0 + token, head, e, vec), b = paged_key4(A, q, h, inside, t0 + lane, e, vec, &g_fault);
-                s = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s))));
-            }
-        }
-        float top = s;
-#pragma unroll
-        for (int x = 1; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = exp2f((m - base) * A.scale_log2), w = exp2f((s - base) * A.scale_log2);
-        m = m_new;
-        l = fmaf(l, alpha, w);
-        o.x *= alpha; o.y *= alpha; o.z *= alpha; o.w *= alpha;
-#pragma unroll 1
-        for (int j = 0; j < 32 && t0 + j <= last; ++j) {
-            const float wj = __shfl_sync(0xffffffffu, w, j);
-            if (d >= D) continue;
-            const float4 v = paged_value4(A, q, h, inside, t0 + j, d, vec, &g_fault);
-            o.x = fmaf(wj, v.x, o.x); o.y = fmaf(wj, v.y, o.y); o.z = fmaf(wj, v.z, o.z); o.w = fmaf(wj, v.w, o.w);
-        }
-    }
-#pragma unroll
-    for (int x = 1; x < 32; x *= 2) l += __shfl_xor_sync(0xffffffffu, l, x);
-    const float by = 1.0f / l;
-    if (d < D)
-        store_quad(A.out.data, A.out_dtype, ((int64_t)q.row0 + token) * A.out.row_stride + (int64_t)head * A.out.head_stride + d,
-                   make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
-}
-
 // Folds the pieces of a block's rows, a thread per quad of channels of a row.
-// grid = (blocks, KV heads, slices of kFoldRows rows, fewer where nothing is folded).
-constexpr int kFoldRows = 8;                             // (a warp each where they are computed anew)
+// grid = (blocks, KV heads, slices of kFoldRows rows).
+constexpr int kFoldRows = 8;
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(PagedAttnArgs A, int RT) {
     __shared__ int place_s[2];
@@ -334,15 +301,6 @@ paged_merge_kernel(PagedAttnArgs A, int RT) {
     const int rows = q.n * n_rep, row_first = place_s[1] * RT;
     const int n_rows = rows - row_first < RT ? rows - row_first : RT;
     const int keys = q.held + (row_first + n_rows - 1) / n_rep + 1, n_pieces = (keys + A.chunk - 1) / A.chunk;
-    if (A.rough) {                                       // the tensor cores' rows that those were no good for
-        int any = 0;
-        for (int p = 0; p < n_pieces; ++p) any |= A.rough[((int64_t)blockIdx.x * H + h) * A.pieces + p];
-        if (any) {
-            const int inside = min(quant_of(q.held + q.n, L.group_size, L.residual_cap), q.held);
-            for (int r = blockIdx.z * kFoldRows + (threadIdx.x >> 5); r < n_rows; r += gridDim.z * kFoldRows) row_in_fp32(A, q, h, row_first + r, inside, threadIdx.x & 31);
-            return;
-        }
-    }
     if (n_pieces <= 1) return;
     const int quads = D / 4;
     const int64_t part0 = ((int64_t)blockIdx.x * H + h) * A.pieces;
@@ -372,6 +330,16 @@ int run_general(const PagedAttnArgs& a, int blocks, size_t smem, cudaStream_t st
     auto* const kernel = paged_attention_kernel<RPT, TY, DT>;
     if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     KIVI_CUDA_OK(launch(kernel, dim3((unsigned)blocks, (unsigned)a.L.num_kv_heads, (unsigned)a.pieces), TY * 16, smem, st, true, a));
+    return KIVI_OK;
+}
+
+// what the tensor cores have flagged (rows of 64 by CTAs that see in one load that there is nothing to do)
+template <int DT>
+int run_again(const PagedAttnArgs& a, int blocks, cudaStream_t st) {
+    auto* const kernel = paged_attention_kernel<4, 16, DT, true>;
+    const size_t smem = ((size_t)(64 + 2 * kTile) * (DT + 4) + (size_t)64 * (kTile + 4)) * 4;
+    KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)blocks * (kTensorRows / 64), (unsigned)a.L.num_kv_heads, (unsigned)a.pieces), 256, smem, st, true, a));
     return KIVI_OK;
 }
 
@@ -412,7 +380,7 @@ static PagedPlan plan_paged(const kivi_paged_layer* L, const kivi_paged_batch* b
     }
     p.kernel = paged_tc_serves(L, q_dtype) ? PagedKernel::kTensor : PagedKernel::kGeneral;
     if (p.kernel == PagedKernel::kTensor) {
-        p.rows = 256;
+        p.rows = kTensorRows;
         const int64_t blocks = (int64_t)b->total_new * n_rep / p.rows + b->num_seqs;
         p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
         // One CTA per SM: the fewest rounds of the shortest pieces, each with the start and
@@ -512,16 +480,15 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
         a.vec = vec16;
         a.rough = reinterpret_cast<int*>(static_cast<char*>(workspace) + need) - (size_t)p.blocks * L->num_kv_heads * p.pieces;
         rc = run_paged_tc(a, p.blocks, st);
+        if (!rc) rc = D == 64 ? run_again<64>(a, p.blocks, st) : run_again<128>(a, p.blocks, st);
     } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);
     if (rc) return rc;
-    if (p.pieces > 1 || a.rough) {
-        // (one piece: the kernel only looks for rows to compute anew)
-        const int slices = p.pieces > 1 ? (p.rows + kFoldRows - 1) / kFoldRows : 4;
-        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)slices), 256, 0, st, true, a, p.rows));
-        note_launches(2);
-    } else {
-        note_launches(1);
+    int launches = p.kernel == PagedKernel::kTensor ? 2 : 1;
+    if (p.pieces > 1) {
+        KIVI_CUDA_OK(launch(paged_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)((p.rows + kFoldRows - 1) / kFoldRows)), 256, 0, st, true, a, p.rows));
+        ++launches;
     }
+    note_launches(launches);
     return KIVI_OK;
 }

@@ -28,8 +28,8 @@
 // Sums, maxima and O are fp32.  One power of two for all the tokens of a tile is no good where a row
 // does not see, or gives no weight to, a token that is far larger than the others: the rows of a CTA
 // that has met a value of 2^16 or more, an infinity or a NaN are computed on the CUDA cores in fp32
-// by the kernel that folds the pieces (a row at a time, some fifty times slower; the same code in
-// this kernel cost every call 8 %).  Below that, other tokens are exact to 2^-22.
+// by a launch behind this one (attn_paged.cu; the 512 rows below take 5.7 ms if all are; a fallback
+// within this kernel cost every call 8 %).  Below that, other tokens are exact to 2^-22.
 //
 // Codes to fp16: a 2-bit field and the exponent of 1024 make the number 1024 + c 4^n, of
 // which 1024 is taken off exactly; c 4^n (s / 4^n) + z is one fused operation for two
@@ -40,7 +40,7 @@
 // makes its own, then 1400 until P V and the next scores are done.  One block: 4300, of which the
 // conversion of a tile takes 2800-3100 (bf16, 32k tokens).
 // 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 391 us, 710 TFLOP/s; 4 x 2048 over
-// 16k 3246 us; 16 x 5 tokens over 4k 78 us.  The roles share an instruction cache, so bodies are
+// 16k 3217 us; 16 x 5 tokens over 4k 74 us.  The roles share an instruction cache, so bodies are
 // small: with the MMAs of a tile and four tokens of a key quad side by side 403, 3280, 90, with the
 // conversions' channels unrolled too 423, 3393, 99; but weights by 32 columns 426, 3440 (81) and
 // values a token at a time 394, 3271, 88.
@@ -439,7 +439,7 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
             if (ok) ok = wait_warp(misc.o_done, 0);
             {
                 fence_after();
-                const bool rough = *const_cast<volatile int*>(&misc.rough) != 0;         // (computed elsewhere, and `out` may be `q`)
+                const bool rough = *const_cast<volatile int*>(&misc.rough) != 0;         // (computed by another launch, and `out` may be `q`)
                 float f = pow2i(-v_shift), other = 0.0f;
                 float* const odd_o = reinterpret_cast<float*>(smem + S::k) + r;           // [channel][row]: the odd tiles' output
                 if (turns && n_tiles > 1) {

@@ -36,14 +36,6 @@ __device__ __forceinline__ float4 load4_as(const kivi_rows& r, int dtype, int64_
     return dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(r.data) + at, vec) : load4(reinterpret_cast<const float*>(r.data) + at, vec);
 }
 
-// Four channels of token t's key (value) as it is served: from its page before `inside`, from the
-// window before `held`, else the step's own row.
-__device__ __forceinline__ float4 paged_row4(const PagedAttnArgs& A, const PagedSeq& q, const void* ring, const kivi_rows& fresh, int h, int t, int d, bool vec) {
-    const kivi_paged_layer& L = A.L;
-    if (t >= q.held) return load4_as(fresh, L.res_dtype, (int64_t)q.row0 + (t - q.held), h, d, vec);
-    const int64_t at = (((int64_t)q.slot * L.num_kv_heads + h) * L.residual_cap + ring_slot(t, A.b.ring_shift, L.residual_cap)) * L.head_dim + d;
-    return L.res_dtype == KIVI_BF16 ? load4(reinterpret_cast<const __nv_bfloat16*>(ring) + at, true) : load4(reinterpret_cast<const float*>(ring) + at, true);
-}
 // Four channels of token tt of group g of the pages.
 __device__ __forceinline__ float4 packed_key4(const kivi_paged_layer& L, int64_t g, int tt, int d) {
     const int D = L.head_dim, Q = L.group_size / 4, sh = 2 * (tt & 3);
@@ -58,16 +50,6 @@ __device__ __forceinline__ float4 packed_value4(const kivi_paged_layer& L, int64
     const int64_t at = g * D + vmeta_index(tt, d / G, D, G);
     const float s = L.v_scales[at], z = L.v_zeros[at];
     return make_float4(fmaf((float)(c & 3u), s, z), fmaf((float)((c >> 2) & 3u), s, z), fmaf((float)((c >> 4) & 3u), s, z), fmaf((float)(c >> 6), s, z));
-}
-__device__ __forceinline__ int64_t paged_group(const PagedAttnArgs& A, const PagedSeq& q, int h, int t, int* fault) {
-    const kivi_paged_layer& L = A.L;
-    return ((int64_t)page_of(L, q, t, fault) * L.num_kv_heads + h) * (L.page_tokens / L.group_size) + t % L.page_tokens / L.group_size;
-}
-__device__ __forceinline__ float4 paged_key4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
-    return t < inside ? packed_key4(A.L, paged_group(A, q, h, t, fault), t % A.L.group_size, d) : paged_row4(A, q, A.L.k_res, A.k, h, t, d, vec);
-}
-__device__ __forceinline__ float4 paged_value4(const PagedAttnArgs& A, const PagedSeq& q, int h, int inside, int t, int d, bool vec, int* fault) {
-    return t < inside ? packed_value4(A.L, paged_group(A, q, h, t, fault), t % A.L.group_size, d) : paged_row4(A, q, A.L.v_res, A.v, h, t, d, vec);
 }
 #endif
 
