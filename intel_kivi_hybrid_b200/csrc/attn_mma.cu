@@ -157,7 +157,7 @@ attn_mma_kernel(kivi_layer L, int64_t quant_len, int res_start, int res_len,
             bulk_g2s(dst + kGPS * 1024, L.k_scales + g * 128, ng * 512, bar, policy);
             bulk_g2s(dst + kGPS * 1536, L.k_zeros + g * 128, ng * 512, bar, policy);
             bulk_g2s(dst + kGPS * 2048, L.v_codes + g * 1024, ng * 1024, bar, policy);
-            bulk_g2s(dst + kGPS * 3072, L.v_scales + g * 128, ng * 512, bar, policy);
+            bulk_g2s(dst + kGPS * 3 * 1024, L.v_scales + g * 128, ng * 512, bar, policy);
             bulk_g2s(dst + kGPS * 3584, L.v_zeros + g * 128, ng * 512, bar, policy);
         }
         __syncwarp();

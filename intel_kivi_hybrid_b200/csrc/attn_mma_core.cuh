@@ -606,7 +606,7 @@ __device__ __forceinline__ void process_groups(const uint8_t* __restrict__ sb, c
     const uint32_t spare = WIDE ? smem_u32(sb + kGPS * 1024) : 0u;
     qk_phase<NG, WIDE>(sb, reinterpret_cast<const float*>(sb + kGPS * 1024), reinterpret_cast<const float*>(sb + kGPS * 1536), v, scratch, spare, s, fine);
     softmax_phase<NG, WIDE>(s, fine, st);
-    pv_phase<NG, WIDE>(sb + kGPS * 2048, reinterpret_cast<const float*>(sb + kGPS * 3072), reinterpret_cast<const float*>(sb + kGPS * 3584), s, v, scratch, spare, st);
+    pv_phase<NG, WIDE>(sb + kGPS * 2048, reinterpret_cast<const float*>(sb + kGPS * 3 * 1024), reinterpret_cast<const float*>(sb + kGPS * 3584), s, v, scratch, spare, st);
     // what was written over the stage comes before the copy that fills it again
     if constexpr (WIDE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -817,7 +817,7 @@ __device__ __forceinline__ void process_groups(const uint8_t* __restrict__ sb, c
     float s[4];
     qk_one<NG>(sb, reinterpret_cast<const float*>(sb + kGPS * 1024), reinterpret_cast<const float*>(sb + kGPS * 1536), v, scratch, s);
     softmax_one(s, st);
-    pv_one<NG>(sb + kGPS * 2048, reinterpret_cast<const float*>(sb + kGPS * 3072), reinterpret_cast<const float*>(sb + kGPS * 3584), s, v, scratch, st);
+    pv_one<NG>(sb + kGPS * 2048, reinterpret_cast<const float*>(sb + kGPS * 3 * 1024), reinterpret_cast<const float*>(sb + kGPS * 3584), s, v, scratch, st);
 }
 
 __device__ __forceinline__ void clear(WarpState& st) {

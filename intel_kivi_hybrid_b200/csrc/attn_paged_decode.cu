@@ -174,7 +174,7 @@ paged_decode_kernel(PagedAttnArgs A, int blocks_per_seq, int gps) {
                 bulk_g2s(dst + kGPS * 1024 + at * 512, L.k_scales + g * 128, n * 512, bar, policy);
                 bulk_g2s(dst + kGPS * 1536 + at * 512, L.k_zeros + g * 128, n * 512, bar, policy);
                 bulk_g2s(dst + kGPS * 2048 + at * 1024, L.v_codes + g * 1024, n * 1024, bar, policy);
-                bulk_g2s(dst + kGPS * 3072 + at * 512, L.v_scales + g * 128, n * 512, bar, policy);
+                bulk_g2s(dst + kGPS * 3 * 1024 + at * 512, L.v_scales + g * 128, n * 512, bar, policy);
                 bulk_g2s(dst + kGPS * 3584 + at * 512, L.v_zeros + g * 128, n * 512, bar, policy);
             };
             if (b == a + 1) copy(0, a, ng);
