@@ -39,11 +39,11 @@
 // 5500.  A block's chain is what bounds it: maximum 630-1000, weights 2800 while the other block
 // makes its own, then 1400 until P V and the next scores are done.  One block: 4300, of which the
 // conversion of a tile takes 2800-3100 (bf16, 32k tokens).
-// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 391 us, 710 TFLOP/s; 4 x 2048 over
-// 16k 3217 us; 16 x 5 tokens over 4k 74 us.  The roles share an instruction cache, so bodies are
-// small: with the MMAs of a tile and four tokens of a key quad side by side 403, 3280, 90, with the
-// conversions' channels unrolled too 423, 3393, 99; but weights by 32 columns 426, 3440 (81) and
-// values a token at a time 394, 3271, 88.
+// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 385 us, 720 TFLOP/s; 4 x 2048 over
+// 16k 3114 us; 16 x 5 tokens over 4k 76 us; a prompt of 4 x 2048 440 us.  The roles share an
+// instruction cache, so bodies are small: with the MMAs of a tile and four tokens of a key quad side
+// by side 403 us where this form had 391, 3280 (3246), 90 (78), with the conversions' channels unrolled
+// too 423, 3393, 99; but weights by 32 columns 426, 3440 (81) and values a token at a time 394, 3271, 88.
 // Lost: two threads to a row that meet for its maximum (406, 3323, 101 with one group of softmax
 // warps for one block); scores in halves of 64 tokens,
 // so that the next half's are made meanwhile (471, 3753: twice the dependent MMAs in a row);
@@ -209,6 +209,11 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
     return v;
 }
+// 16 bytes to shared memory, or zeros
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Bits of the largest magnitude among z and z + 3 s of a group's factors (D of each): what
 // codes stand for lies between.
 template <int D>
@@ -500,10 +505,12 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
         const __nv_bfloat16* const rows_new = reinterpret_cast<const __nv_bfloat16*>(fresh.data) + (int64_t)h * fresh.head_stride;
         // Rows as they are (window, new tokens): lane = (16-byte piece of 64 channels, token of four).
         const int p8 = lane & 7, sub = lane >> 3;
-        auto row8 = [&](int t, int ch) {                             // eight channels of token t >= inside; behind the piece's end zeros
+        auto row_at = [&](int t) {                                   // token t >= inside
+            return t < q.held ? ring + (int64_t)ring_slot(t, A.b.ring_shift, R) * D : rows_new + ((int64_t)q.row0 + t - q.held) * fresh.row_stride;
+        };
+        auto row8 = [&](int t, int ch) {                             // its eight channels; behind the piece's end zeros
             if (t >= t_end) return make_uint4(0u, 0u, 0u, 0u);
-            const __nv_bfloat16* from = t < q.held ? ring + (int64_t)ring_slot(t, A.b.ring_shift, R) * D + ch
-                                                   : rows_new + ((int64_t)q.row0 + t - q.held) * fresh.row_stride + ch;
+            const __nv_bfloat16* from = row_at(t) + ch;
             if (t < q.held || A.vec) return *reinterpret_cast<const uint4*>(from);
             const uint16_t* u = reinterpret_cast<const uint16_t*>(from);
             return make_uint4(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16, u[4] | (uint32_t)u[5] << 16, u[6] | (uint32_t)u[7] << 16);
@@ -621,16 +628,27 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                     top = group_top<D>(raw + g * S::kFactors, lane);
                 } else {
                     uint32_t pair = 0u;
+                    // All of a lane's copies are on their way at once, and it reads them back itself (loads of four
+                    // through registers: 4 x 2048 tokens of a prompt 521 us, of eight 463, so 440).
 #pragma unroll 1
-                    for (int i = 0; i < 2 * (D / 64); ++i) {
+                    for (int i = 0; i < 8 * (D / 64); ++i) {
+                        const int r = sub + 4 * (i & 7), t = t0 + r, ch = 64 * (i >> 3) + 8 * p8;
+                        const uint32_t at = place(to, i >> 3, r);
+                        if (t >= q.held && !A.vec) {
+                            const uint4 x = row8(t, ch);
+                            sts128(at, x.x, x.y, x.z, x.w);
+                        } else {
+                            copy16(at, row_at(min(t, t_end - 1)) + ch, t < t_end);
+                        }
+                    }
+                    copies_wait();
+#pragma unroll 1
+                    for (int i = 0; i < 8 * (D / 64); i += 4) {
                         uint4 x[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = row8(t0 + sub + 4 * (4 * (i & 1) + e), 64 * (i >> 1) + 8 * p8);
+                        for (int e = 0; e < 4; ++e) x[e] = lds_uint4(place(to, i >> 3, sub + 4 * ((i + e) & 7)));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            pair = __vmaxu2(pair, top8(x[e]));
-                            sts128(place(to, i >> 1, sub + 4 * (4 * (i & 1) + e)), x[e].x, x[e].y, x[e].z, x[e].w);
-                        }
+                        for (int e = 0; e < 4; ++e) pair = __vmaxu2(pair, top8(x[e]));
                     }
                     top = max(pair << 16, pair & 0xffff0000u);
                 }
