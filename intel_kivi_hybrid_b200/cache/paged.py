@@ -95,7 +95,8 @@ class PagedKiviCache:
 
     def free(self, seq: int) -> None:
         """Give a sequence's window and pages back.  Kernels queued before may still read them: later steps
-        come behind those on the same stream.  A step of it that has not ended is given up."""
+        come behind those on the same stream.  A step of it that has not ended is given up, for its other
+        sequences too (``begin``)."""
         self._give_up(seq)
         self._free_pages.extend(reversed(self._pages.pop(seq)))
         del self._lens[seq]
@@ -107,6 +108,16 @@ class PagedKiviCache:
             step.open = False
             for s in step.seqs:
                 self._steps.pop(s, None)
+                self._trim(s)
+
+    def _pages_for(self, tokens: int) -> int:
+        return -(-self.quantized(tokens) // self.page_tokens)
+
+    def _trim(self, seq: int) -> None:
+        """Give back the pages that a step took and did not come to fill."""
+        pages, keep = self._pages[seq], self._pages_for(self._lens[seq])
+        self._free_pages.extend(reversed(pages[keep:]))
+        del pages[keep:]
 
     def length(self, seq: int) -> int:
         return self._lens[seq]
@@ -125,22 +136,27 @@ class PagedKiviCache:
         return self._layers[i]
 
     # ------------------------------------------------------------------ steps
-    def _take_pages(self, seqs, lens) -> None:
-        need = {s: -(-self.quantized(n) // self.page_tokens) - len(self._pages[s]) for s, n in zip(seqs, lens)}
-        total = sum(max(0, n) for n in need.values())
-        if total > len(self._free_pages):
-            raise RuntimeError(f"{total} pages are needed, {len(self._free_pages)} of {self.num_pages} are free")
+    def _start(self, seqs, lens) -> None:
+        """Give up the steps of ``seqs`` that have not ended and take the pages for ``lens`` tokens; raises before
+        anything has changed."""
+        touched = set(seqs).union(*(self._steps[s].seqs for s in seqs if s in self._steps))
+        free = len(self._free_pages) + sum(len(self._pages[s]) - self._pages_for(self._lens[s]) for s in touched)
+        need = {s: self._pages_for(n) - self._pages_for(self._lens[s]) for s, n in zip(seqs, lens)}
+        if sum(need.values()) > free:
+            raise RuntimeError(f"{sum(need.values())} pages are needed, {free} of {self.num_pages} are free")
         for s, n in need.items():
-            for _ in range(n):
-                self._pages[s].append(self._free_pages.pop())
+            self._give_up(s)
+            self._trim(s)
+        for s, n in need.items():
+            self._pages[s].extend(self._free_pages.pop() for _ in range(n))
 
     def _table(self, seqs, width) -> torch.Tensor:
         return torch.tensor([self._pages[s] + [-1] * (width - len(self._pages[s])) for s in seqs], dtype=torch.int32).reshape(len(seqs), width)
 
     def begin(self, seqs: Sequence[int], new: Sequence[int], max_len: Optional[int] = None) -> PagedBatch:
         """Start a step in which sequence ``seqs[i]`` gets ``new[i]`` tokens (0 is allowed): takes the pages that the
-        step fills and lays down the arrays its kernels follow.  A step of one of them that has not ended is given up; what it
-        has appended to some layers is not undone, so give up only what has not run.  ``max_len``: the longest length a captured step
+        step fills and lays down the arrays its kernels follow.  A step of one of them that has not ended is given up and its pages
+        are given back; what it has appended to some layers is not undone, so give up only what has not run.  ``max_len``: the longest length a captured step
         shall reach (default: this step's)."""
         seqs, new = [int(s) for s in seqs], [int(n) for n in new]
         assert len(seqs) == len(new) and seqs, "begin() needs at least one sequence, and new tokens for each"
@@ -151,7 +167,7 @@ class PagedKiviCache:
         held = [self._lens[s] for s in seqs]
         longest = max(h + n for h, n in zip(held, new))
         assert max_len is None or max_len >= longest, f"max_len ({max_len}) is below this step's longest length ({longest})"
-        self._take_pages(seqs, [h + n for h, n in zip(held, new)])
+        self._start(seqs, [h + n for h, n in zip(held, new)])
         max_len = max_len or longest
         cu = [0]
         for n in new:
@@ -159,8 +175,6 @@ class PagedKiviCache:
         width = max(1, -(-self.quantized(max_len) // self.page_tokens))
         dev = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
         batch = PagedBatch(seqs, new, held, max(new), max_len, cu[-1], self._table(seqs, width).to(self.device), dev(seqs), dev(held), dev(cu))
-        for s in seqs:
-            self._give_up(s)
         self._steps.update((s, batch) for s in seqs)
         return batch
 
@@ -213,12 +227,10 @@ class PagedKiviCache:
         held = [self._lens[s] for s in batch.seqs]
         lens = [h + n for h, n in zip(held, batch.new)]
         assert max(lens) <= batch.max_len, f"the step reaches {max(lens)} tokens, it was begun for {batch.max_len}"
-        self._take_pages(batch.seqs, lens)
+        self._start(batch.seqs, lens)
         batch.page_table.copy_(self._table(batch.seqs, batch.page_table.shape[1]))
         batch.seq_lens.copy_(torch.tensor(held, dtype=torch.int32))
         batch.held, batch.open = held, True
-        for s in batch.seqs:
-            self._give_up(s)
         self._steps.update((s, batch) for s in batch.seqs)
 
     # ------------------------------------------------------------------ reading back

@@ -136,3 +136,34 @@ def test_sample_token_on_the_host_takes_the_filters():
     torch.manual_seed(3)
     scaled = (x / 0.7).masked_fill(x / 0.7 < torch.topk(x / 0.7, 3).values[:, -1:], float("-inf"))
     assert torch.equal(a, torch.multinomial(torch.softmax(scaled, -1), 1))                   # without the new filters: the reference's operations
+
+
+def test_a_step_that_is_given_up_gives_its_pages_back():
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(1, 64, 1, num_pages=8, max_sequences=3, page_tokens=64, group_size=32, residual_length=64, device="cpu")
+    a, b, c = (cache.add_sequence() for _ in range(3))
+    cache.end(cache.begin([a], [200]))                      # three pages
+    assert cache.free_pages == 5
+    kept = list(cache._pages[a])
+    long = cache.begin([a, b], [200, 130])                  # three more, and two
+    assert cache.free_pages == 0
+    with pytest.raises(RuntimeError, match="6 pages are needed, 5 of 8 are free"):
+        cache.begin([b, c], [300, 190])                     # (what the open step of a and b has taken counts as free)
+    assert long.open and cache.free_pages == 0
+    short = cache.begin([b], [1])                           # a table of one page
+    assert not long.open and short.page_table.tolist() == [[-1]] and cache.free_pages == 5 and cache._pages[a] == kept
+    cache.end(short)
+    again = cache.begin([a, b], [1, 1], max_len=300)
+    cache.end(again)
+    longer = cache.begin([b, a], [350, 1])
+    assert cache.free_pages == 0 and longer.page_table.shape == (2, 5)
+    cache.refresh(again)                                    # its arrays are those of shorter steps
+    assert not longer.open and cache.free_pages == 5
+    assert again.page_table.tolist() == [kept + [-1], [-1] * 4]
+    cache.end(again)
+    assert (cache.length(a), cache.length(b)) == (202, 3)
+    cache.begin([a, b], [1, 300])
+    cache.free(b)                                           # gives up the step for both
+    assert cache.free_pages == 5 and cache._pages[a] == kept
+    cache.free(a)
+    assert sorted(cache._free_pages) == list(range(8))
