@@ -212,8 +212,9 @@ class PagedKiviCache:
     def end(self, batch: PagedBatch) -> None:
         """The step is done in all layers: its tokens are the sequences' own."""
         assert batch.open, "the step has ended"
-        for s, h, n in zip(batch.seqs, batch.held, batch.new):
+        for s, h in zip(batch.seqs, batch.held):
             assert self._lens.get(s) == h, f"sequence {s} has changed during the step"
+        for s, h, n in zip(batch.seqs, batch.held, batch.new):
             self._lens[s] = h + n
             self._steps.pop(s, None)
         batch.open = False

@@ -167,3 +167,17 @@ def test_a_step_that_is_given_up_gives_its_pages_back():
     assert cache.free_pages == 5 and cache._pages[a] == kept
     cache.free(a)
     assert sorted(cache._free_pages) == list(range(8))
+
+
+def test_a_step_ends_for_all_its_sequences_or_for_none():
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(1, 64, 1, num_pages=4, max_sequences=2, page_tokens=64, group_size=32, residual_length=64, device="cpu")
+    a, b = cache.add_sequence(), cache.add_sequence()
+    batch = cache.begin([a, b], [3, 4])
+    cache._lens[b] = 1
+    with pytest.raises(AssertionError, match=f"sequence {b} has changed"):
+        cache.end(batch)
+    assert (cache.length(a), batch.open) == (0, True)
+    cache._lens[b] = 0
+    cache.end(batch)
+    assert (cache.length(a), cache.length(b)) == (3, 4)
