@@ -236,10 +236,12 @@ class PagedKiviCache:
 
     # ------------------------------------------------------------------ reading back
     def read(self, layer: int, seq: int, start: int = 0, stop: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Tokens start .. stop-1 of a sequence as they are served: fp32 keys and values [tokens, H, D]."""
+        """Tokens start .. stop-1 of a sequence as they are served: fp32 keys and values [tokens, H, D].  Not while a
+        step of the sequence is open: the step's append has moved tokens to pages and taken their slots in the window."""
         held = self._lens[seq]
         stop = held if stop is None else stop
         assert 0 <= start <= stop <= held, f"tokens {start} .. {stop} of a sequence of {held}"
+        assert seq not in self._steps, f"a step of sequence {seq} has not ended"
         k = torch.empty(stop - start, self.num_kv_heads, self.head_dim, device=self.device)
         v = torch.empty_like(k)
         if stop > start:

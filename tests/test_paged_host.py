@@ -181,3 +181,17 @@ def test_a_step_ends_for_all_its_sequences_or_for_none():
     cache._lens[b] = 0
     cache.end(batch)
     assert (cache.length(a), cache.length(b)) == (3, 4)
+
+
+def test_a_sequence_is_not_read_within_a_step():
+    """Between append and end the window's slots hold the step's tokens already, and the length is the one before."""
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(1, 64, 1, num_pages=4, max_sequences=2, page_tokens=64, group_size=32, residual_length=64, device="cpu")
+    a, b = cache.add_sequence(), cache.add_sequence()
+    cache.end(cache.begin([a, b], [60, 5]))
+    batch = cache.begin([a], [10])
+    with pytest.raises(AssertionError, match="has not ended"):
+        cache.read(0, a)
+    assert cache.read(0, b, 5, 5)[0].shape == (0, 1, 64)    # (the other one has no open step)
+    cache.end(batch)
+    assert cache.read(0, a, 70)[0].shape == (0, 1, 64)
