@@ -20,7 +20,8 @@ A step of the model, over any set of its sequences::
 are while they are in the window or new, as their codes stand for once they are in pages.
 
 All kernels follow arrays in device memory, so a step can be captured: ``begin(..., max_len=...)`` with the longest
-length it shall reach, and before each replay ``end(batch)`` and ``refresh(batch)``.
+length it shall reach, and before each replay ``end(batch)`` and ``refresh(batch)``.  A layer's arrays are laid
+out by its first step, which therefore is not a captured one.
 """
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
@@ -128,6 +129,9 @@ class PagedKiviCache:
 
     def _layer(self, i: int) -> Tuple[torch.Tensor, ...]:
         if self._layers[i] is None:
+            # (the arrays would belong to the graph, and every replay would empty them)
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"layer {i} is used for the first time in a captured step: run a step outside first")
             P, H, D, G, R, T = max(1, self.num_pages), self.num_kv_heads, self.head_dim, self.G, self.R, self.page_tokens
             z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=self.device)  # noqa: E731
             self._layers[i] = (z(P, H, T // G, D * G // 4, dtype=torch.uint8), z(P, H, T // G, D), z(P, H, T // G, D),

@@ -195,3 +195,14 @@ def test_a_sequence_is_not_read_within_a_step():
     assert cache.read(0, b, 5, 5)[0].shape == (0, 1, 64)    # (the other one has no open step)
     cache.end(batch)
     assert cache.read(0, a, 70)[0].shape == (0, 1, 64)
+
+
+def test_a_layer_s_arrays_are_not_laid_out_within_a_capture(monkeypatch):
+    """Memory that is allocated and cleared while a step is captured would be cleared again by every replay."""
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(2, 64, 1, num_pages=4, max_sequences=2, page_tokens=64, group_size=32, residual_length=64)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="first time in a captured step"):
+        cache._layer(1)
+    cache._layers[1] = ()                                   # (laid out by a step before)
+    assert cache._layer(1) == ()
