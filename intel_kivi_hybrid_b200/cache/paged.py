@@ -256,10 +256,13 @@ class PagedKiviCache:
         return k, v
 
     def check_device_fault(self) -> None:
-        """Raise if a kernel has met arrays that point outside the cache, or a wait has run out (synchronises)."""
-        word = cabi.device_fault()
+        """Raise if a kernel has met arrays that point outside the cache, or a wait has run out (synchronises).  The
+        word is that of the cache's device, whichever is the current one."""
+        with torch.cuda.device(self.device):
+            word = cabi.device_fault()
+            if word:
+                cabi.device_fault_clear()
         if word:
-            cabi.device_fault_clear()
             raise RuntimeError(f"kivi_cuda device fault word = {word}; outputs since the last check may be wrong")
 
     def __repr__(self):

@@ -206,3 +206,27 @@ def test_a_layer_s_arrays_are_not_laid_out_within_a_capture(monkeypatch):
         cache._layer(1)
     cache._layers[1] = ()                                   # (laid out by a step before)
     assert cache._layer(1) == ()
+
+
+def test_the_fault_word_is_that_of_the_cache_s_device(monkeypatch):
+    from kivi_cuda import PagedKiviCache
+    from intel_kivi_hybrid_b200.cache import paged
+    current, words = [0], {0: 0, 1: 4}
+
+    class On:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(paged.cabi, "device_fault", lambda: words[current[0]])
+    monkeypatch.setattr(paged.cabi, "device_fault_clear", lambda: words.update({current[0]: 0}))
+    make = lambda i: PagedKiviCache(1, 64, 1, num_pages=4, max_sequences=2, page_tokens=64, group_size=32, residual_length=64, device=f"cuda:{i}")  # noqa: E731
+    make(0).check_device_fault()
+    with pytest.raises(RuntimeError, match="word = 4"):
+        make(1).check_device_fault()
+    assert words == {0: 0, 1: 0}
