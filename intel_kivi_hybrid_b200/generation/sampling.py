@@ -68,12 +68,15 @@ def sample_token(logits: torch.Tensor, temperature: float, top_k: Optional[int],
         return _default(logits, temperature, top_k, do_sample, top_p, min_p)
     if not do_sample:
         return torch.argmax(logits, dim=-1, keepdim=True)
+    filtered = top_p < 1.0 or min_p > 0.0
+    if filtered and logits.dtype in (torch.float16, torch.bfloat16):
+        logits = logits.float()              # (in 8 or 11 bits different probabilities become ties, and their sums stand still)
     scaled = logits / max(temperature, 1e-8)
     if top_k is not None:
         kth = torch.topk(scaled, top_k, dim=-1).values[:, -1:]
         scaled = scaled.masked_fill(scaled < kth, float("-inf"))
     probs = torch.softmax(scaled, dim=-1)
-    if top_p < 1.0 or min_p > 0.0:
+    if filtered:
         # what lies above an entry: the mass of the strictly larger ones, the same for ties
         largest = probs.amax(-1, keepdim=True)
         ordered, order = probs.sort(dim=-1, descending=True)

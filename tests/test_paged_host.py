@@ -230,3 +230,20 @@ def test_the_fault_word_is_that_of_the_cache_s_device(monkeypatch):
     with pytest.raises(RuntimeError, match="word = 4"):
         make(1).check_device_fault()
     assert words == {0: 0, 1: 0}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("top_p,min_p", [(0.5, 0.0), (0.9, 0.0), (0.99, 0.02), (1.0, 0.3)])
+def test_the_filters_on_the_host_cut_where_the_definition_does(monkeypatch, dtype, top_p, min_p):
+    """What is kept of 1000 logits of either type, against the definition in 64 bits."""
+    from intel_kivi_hybrid_b200.generation import sampling
+    kept = []
+    monkeypatch.setattr(torch, "multinomial", lambda p, num_samples: kept.append(p > 0) or torch.zeros(p.shape[0], 1, dtype=torch.int64))
+    x = torch.stack([torch.linspace(0.0, -3.0, 1000), torch.linspace(-1.0, 7.0, 1000)]).to(dtype)
+    sampling.sample_token(x, 0.8, None, True, top_p, min_p)
+    for row, got in zip(x.double(), kept[0]):
+        p = torch.softmax(row / 0.8, 0)
+        above = torch.tensor([float(p[row > r].sum()) for r in row])
+        margin = (above - top_p).abs().min() if top_p < 1.0 else (p / p.max() - min_p).abs().min()
+        assert margin > 1e-5                                # (no entry is at the border: the answer is one set)
+        assert torch.equal(got, (above < top_p if top_p < 1.0 else torch.ones_like(got)) & (p >= min_p * p.max()))
