@@ -4,8 +4,9 @@
 // is ordered between them:
 //   * one CTA per KV head and group that starts in the window (one at least) quantizes it.
 //     Then it writes to the window those tokens that stay and whose slots its own tokens had,
-//     so that a slot is overwritten by the CTA that has read it; what stays and meets no token
-//     that leaves is dealt out in turn;
+//     so that a slot is overwritten by the CTA that has read it, and the turned keys of its own
+//     new tokens, whose rows may be overwritten by them; what stays and meets no token that
+//     leaves is dealt out in turn;
 //   * one CTA per whole group of new tokens and KV head quantizes that group.
 // Every CTA also turns the keys it has and, in steps of a few tokens, the queries of its KV
 // head; in longer steps the queries are a streaming kernel of their own (in the same CTAs
@@ -348,9 +349,10 @@ paged_append_kernel(AppendArgs A) {
     const int slots = QUERIES ? 1 + A.n_rep : 1;         // key and value, then the query heads: a thread's work each
     for (int i = threadIdx.x; i < rest * units * slots; i += kThreads) {
         const int u = i % units, slot = i / units % slots, j = i / units / slots, t = j < lo - q.held ? q.held + j : hi + (j - (lo - q.held));
-        // the token of the window that had the slot, if it leaves, says whose this is
+        // A token that stays: the token of the window that had the slot, if it leaves, says whose it is.  One that
+        // leaves with a group of the window is that group's CTA's, which has read its row (k_out may be new_k).
         const int had = in + (t - in) % R;
-        const int whose = t >= out && had < leaving ? (had - in) / G : t % n_window;
+        const int whose = t < min(out, first) ? (t - in) / G : t >= out && had < leaving ? (had - in) / G : t % n_window;
         if (whose != sub) continue;
         if (!QUERIES || slot == 0) {
             fresh_unit(t, u, nullptr, nullptr, t >= out, true);

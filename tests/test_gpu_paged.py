@@ -534,3 +534,31 @@ def test_out_may_be_q(ops, D, G, n_rep, new, dtype):
     want = attend(ops, pool, q, k, v, [new] * 2, a)
     attend(ops, pool, q, k, v, [new] * 2, a, out=q)
     assert torch.equal(torch.nan_to_num(q, 1.0), torch.nan_to_num(want, 1.0)) and torch.equal(torch.isfinite(q), torch.isfinite(want))
+
+
+@pytest.mark.parametrize("D,G,R,page,dtype,held,new", [
+    (128, 32, 128, 64, torch.bfloat16, 100, 200), (128, 32, 128, 64, torch.float32, 120, 150), (128, 32, 64, 64, torch.bfloat16, 50, 100), (64, 16, 100, 48, torch.float32, 93, 130),
+    (12, 4, 9, 8, torch.bfloat16, 7, 30), (128, 32, 128, 64, torch.bfloat16, 125, 101)])
+def test_rows_turned_in_place_while_groups_of_the_window_leave(ops, D, G, R, page, dtype, held, new):
+    """New tokens that complete a group of the window are read by the CTA that packs the group; where k_out is new_k no other
+    may write their turned rows. Many sequences, several groups of the window each: pages, windows and rows as out of place."""
+    seqs, H, n_rep = 96, 4, 2
+    assert (held + G - 1) // G * G - quant(held, G, R) >= 2 * G and held % G and quant(held + new, G, R) >= (held + G - 1) // G * G
+    angle = torch.rand(held + new, D // 2, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV) * 6.3
+    rotary = torch.cat([angle.cos(), angle.sin()], 1)
+    k0, v0 = rows(seqs * held, H, D, dtype, 1), rows(seqs * held, H, D, dtype, 2)
+    k, v, q = rows(seqs * new, H, D, dtype, 3), rows(seqs * new, H, D, dtype, 4), rows(seqs * new, H * n_rep, D, dtype, 5)
+
+    def run(in_place):
+        pool = Pool(seqs, H, D, G, R, page, held + new, dtype)
+        pool.append(ops, k0, v0, [held] * seqs)
+        pool.lens = [held] * seqs
+        nk, nq = k.clone(), q.clone()
+        k_out, q_out = (nk, nq) if in_place else (torch.empty_like(nk), torch.empty_like(nq))
+        pool.append(ops, nk, v, [new] * seqs, rotary=rotary, q=nq, q_out=q_out, k_out=k_out, interleaved=D == 12)
+        return pool.t + [k_out, q_out]
+    want = run(False)
+    assert torch.equal(want[8], turned(k, rotary, torch.arange(held, held + new).repeat(seqs).cuda(), D, D == 12))
+    for _ in range(5):
+        for x, y in zip(run(True), want):
+            assert torch.equal(x, y)
