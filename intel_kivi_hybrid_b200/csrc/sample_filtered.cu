@@ -427,8 +427,9 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         const uint32_t over_key = s.over_key;
         if (s.min_key < over_key) {                      // (else it lies above both cuts)
         // ---- 3. exact masses ----
-        // (one above the largest finite number's key is that of +infinity)
-        const float over_x = key_to_float(over_key), zone_x = cut_p ? key_to_float(s.zone_key) : INFINITY, in_x = key_to_float(s.in_key), k_x = key_to_float(s.k_key);
+        // (one above the largest finite number's key is that of +infinity; what counts as 2^-938 for want of a
+        // mass is in no run's sum, or a draw of 0 would end in a run of such entries)
+        const float over_x = fmaxf(key_to_float(over_key), m.lowest), zone_x = cut_p ? key_to_float(s.zone_key) : INFINITY, in_x = key_to_float(s.in_key), k_x = key_to_float(s.k_key);
         double in = 0.0, over = 0.0;                     // before the k-th largest's bin; above the zone
         auto put = [&](float x, int i) {
             const int j = atomicAdd(&lead.n_p, 1);
@@ -651,7 +652,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
         }
         target = (double)u * __shfl_sync(0xffffffffu, upto, 31);
         const unsigned passes = __ballot_sync(0xffffffffu, mine > 0.0 && upto > target), holds = __ballot_sync(0xffffffffu, mine > 0.0);
-        const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
+        const int w = passes ? __ffs(passes) - 1 : max(31 - __clz(holds), 0);        // (never nothing: the largest is kept)
         double at_run = __shfl_sync(0xffffffffu, upto - mine, w);
         int pick = w * ctas;
         for (int c = 0; c < ctas; ++c) {                 // (all lanes the same)
@@ -682,7 +683,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                 if (lane >= o) upto += x;
             }
             const unsigned passes = __ballot_sync(0xffffffffu, some && before + upto > target), holds = __ballot_sync(0xffffffffu, some);
-            const int w = passes ? __ffs(passes) - 1 : 31 - __clz(holds);
+            const int w = passes ? __ffs(passes) - 1 : max(31 - __clz(holds), 0);
             before += __shfl_sync(0xffffffffu, upto, w) - s.sum[w];
             if (lane == 0) { s.draw_lo = min(lo + w * per, hi); s.draw_hi = min(min(lo + w * per, hi) + per, hi); }
         }
@@ -707,7 +708,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             if (holds) last = i0 + 31 - __clz(holds);
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (lane == 0) ids[b] = pick >= 0 ? pick : last;
+        if (lane == 0) ids[b] = pick >= 0 ? pick : max(last, 0);
     }
 }
 

@@ -214,3 +214,27 @@ def test_rows_of_several_ctas(ops, B, V):
     check(ops, x.bfloat16(), u, pick(1.0, 0.6), None, pick(0.95, 0.3, 1.0), None)
     check(ops, x, u)
     check(ops, x, u, None, None, None, pick(0.2, 0.001))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [3200, 60000, 130000])
+def test_a_draw_of_nothing_where_most_entries_have_no_mass(ops, dtype, V):
+    """uniform 0 is the first entry that is kept with a mass: finite logits far below the largest come before it, in the row's
+    first entries, in its first run and in others, with more of them asked for than there are."""
+    B = 10
+    x = torch.full((B, V), -math.inf, device="cuda")
+    x[:, V - 200] = 100.0
+    x[0, 5] = 0.0
+    x[1, 0] = 0.0
+    x[2, [0, 40, V // 2, V - 1]] = torch.tensor([0.0, -3.0, 1.0, 2.0], device="cuda")
+    x[3, :V // 3] = 0.0
+    x[4, ::2] = torch.where(x[4, ::2] > 0, x[4, ::2], torch.zeros((), device="cuda"))
+    x[5] = torch.where(x[5] > 0, x[5], torch.full((), torch.finfo(dtype).min, device="cuda"))
+    x[6, V - 201] = 99.9
+    x[7, 3] = 99.0
+    x[8, V // 2:V // 2 + 50] = 50.0
+    x = x.to(dtype)
+    t = [0.05] * 9 + [1e-3]
+    for u in (0.0, 1e-45, 2.0 ** -24, 1.0 - 2.0 ** -24):
+        for args in ({"k": [1000] * B}, {"k": [V - 1] * B}, {"k": [2] * B}, {"k": [1000] * B, "mp": [1e-30] * B}, {"p": [0.999999] * B}, {"k": [V - 1] * B, "p": [0.5] * B}, {"mp": [0.3] * B}, {}):
+            check(ops, x, [u] * B, t, **args)
