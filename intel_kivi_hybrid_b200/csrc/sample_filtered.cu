@@ -186,15 +186,17 @@ __device__ __forceinline__ void walk(const T* row, int lo, int hi, int me, int n
 
 // Masses relative to the row's largest entry.
 struct Masses {
-    float largest, c_hi, c_lo;                           // 32 log2(e) / T in two terms
+    float largest, half_largest, c_hi, c_lo;             // 32 log2(e) / T in two terms
     float l_hi, l_lo;                                    // the largest times that: on a grid, and the rest
     float lowest;                                        // about 2^-940 of the largest's mass
     bool only_largest;                                   // an infinite largest, or a temperature that leaves nothing else
     bool narrow;                                         // |l_hi| below 2^18: the grid is 2^-5 or finer
+    bool bounded;                                        // narrow, and `lowest` is a number (not at temperatures of 2^115 and more)
     const Shared* s;
 
     __device__ __forceinline__ void set(float top, float temperature) {
         largest = top;
+        half_largest = 0.5f * top;
         const double c = 32.0 * 1.4426950408889634 / (double)temperature, l = (double)top * c;
         c_hi = (float)c;
         c_lo = (float)(c - (double)c_hi);
@@ -205,6 +207,7 @@ struct Masses {
         l_hi = (float)grid;
         l_lo = (float)(l - grid);
         lowest = top - 30000.0f / c_hi;
+        bounded = narrow && lowest > -INFINITY;
     }
     // 2^((k + r) / 32), t = k + 1.5 * 2^23.  Few instructions of the integer pipe, which bounds the third walk.
     __device__ __forceinline__ double power(float t, float r) const {
@@ -233,15 +236,16 @@ struct Masses {
         const float t = __fadd_rn(p, 12582912.0f);
         return power(t, __fsub_rn(p, __fsub_rn(t, 12582912.0f)) + (__fmaf_rn(d, c_hi, -p) + __fmaf_rn(d, c_lo, __fmul_rn(lost, c_hi))));
     }
-    // The same for sums, where what has no mass may count as 2^-938 (kNarrow: `narrow` and not `only_largest`).
-    template <bool kNarrow>
+    // The same for sums, where what has no mass may count as 2^-938 (kBounded: `bounded` and not `only_largest`).
+    template <bool kBounded>
     __device__ __forceinline__ double get_any(float x) const {
-        if constexpr (kNarrow) { x = fmaxf(x, lowest); return narrow_power(x, __fmaf_rn(x, c_hi, -l_hi)); }
+        if constexpr (kBounded) { x = fmaxf(x, lowest); return narrow_power(x, __fmaf_rn(x, c_hi, -l_hi)); }
         else return get(x);
     }
-    // bin of an entry, falling with it; -1 for one that can have no mass (-inf, NaN)
+    // bin of an entry, falling with it; -1 for one that can have no mass (-inf, NaN).  (Half the difference: the
+    // whole may be above fp32's largest number.)
     __device__ __forceinline__ int bin(float x) const {
-        const float p = __fmul_rn(__fmul_rn(__fsub_rn(largest, x), c_hi), 8.0f);
+        const float p = __fmul_rn(__fmul_rn(__fmaf_rn(-0.5f, x, half_largest), c_hi), 16.0f);
         return p < (float)(kBins - 1) ? __float_as_int(__fadd_rn(p, 12582912.0f)) - 0x4b400000 : x > -INFINITY ? kBins - 1 : -1;
     }
 };
@@ -435,7 +439,7 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
             const int j = atomicAdd(&lead.n_p, 1);
             if (j < kListP) { lead.list_p[j] = {ordered_key(x), i}; lead.mass_p[j] = units(m.get(x)); }
         };
-        auto third = [&](auto narrow) {
+        auto third = [&](auto bounded) {
             walk<T, 1>(row, min(part_lo + warp * run, part_hi), min(part_lo + warp * run + run, part_hi), lane, 32, [&](float x, int i) {
                 if (cut_k && !(x >= in_x)) {
                     if (x >= k_x) {                      // of the k-th largest's bin
@@ -445,13 +449,13 @@ sample_filtered_kernel(const T* logits, int vocab, int64_t row_stride, FilterArg
                     }
                     return;
                 }
-                const double mass = m.template get_any<decltype(narrow)::value>(x);
+                const double mass = m.template get_any<decltype(bounded)::value>(x);
                 in += mass;
                 if (x >= over_x) over += mass;
                 if (x < over_x && x >= zone_x) put(x, i);
             });
         };
-        if (m.narrow) third(std::true_type{});
+        if (m.bounded) third(std::true_type{});
         else third(std::false_type{});
         __syncthreads();
         block_sums(in, over, reinterpret_cast<double*>(s.bins), s.sum, s.runs);

@@ -238,3 +238,31 @@ def test_a_draw_of_nothing_where_most_entries_have_no_mass(ops, dtype, V):
     for u in (0.0, 1e-45, 2.0 ** -24, 1.0 - 2.0 ** -24):
         for args in ({"k": [1000] * B}, {"k": [V - 1] * B}, {"k": [2] * B}, {"k": [1000] * B, "mp": [1e-30] * B}, {"p": [0.999999] * B}, {"k": [V - 1] * B, "p": [0.5] * B}, {"mp": [0.3] * B}, {}):
             check(ops, x, [u] * B, t, **args)
+
+
+@pytest.mark.parametrize("V", [2000, 60000])
+def test_temperatures_near_the_largest_number_and_infinite_ones(ops, V):
+    """Every finite logit has a mass then, -inf and NaN have none; logits apart by more than the largest number."""
+    B = 8
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(B, V, generator=g, device="cuda")
+    x[0, ::2] = -math.inf
+    x[1, ::3] = math.nan
+    x[2] = torch.where(torch.arange(V, device="cuda") % 5 == 0, 3e38, -3e38)
+    x[3] *= 1e38
+    x[4, :V - 1] = -math.inf
+    x[5, 1:] = torch.finfo(torch.float32).min
+    x[6] = -3.3e38 - 1e37 * torch.rand(V, generator=g, device="cuda")
+    k, p, mp = [V - 1] * B, [0.7, 0.3, 0.9, 0.5, 0.5, 0.9, 0.6, 0.99], [0.1] * B
+    for args in ({}, {"k": k}, {"p": p}, {"mp": mp}, {"k": [V // 3] * B, "p": p}, {"k": k, "p": p, "mp": mp}):
+        for seed, t in ((1, 3e38), (2, 1e38), (3, 1e37), (4, 6e35), (5, 1e35)):
+            check(ops, x, uniforms(B, seed), [t] * B, **args)
+        # an infinite temperature: all masses 1, so that 10^300 in the definition's 64 bits is the same to its last bit
+        dev = lambda v, d=torch.float32: None if v is None else torch.tensor(v, dtype=d, device="cuda")  # noqa: E731
+        u = uniforms(B, 6)
+        ids = ops.sample_filtered(x, dev(u), dev([math.inf] * B), dev(args.get("k"), torch.int32), dev(args.get("p")), dev(args.get("mp"))).tolist()
+        for b in range(B):
+            m = row_state(x[b].cpu(), 1e300, args["k"][b] if "k" in args else 0, float(torch.tensor(p[b])) if "p" in args else 1.0, mp[b] if "mp" in args else 0.0)
+            cdf = m.cumsum(0)
+            target = float(torch.tensor(u[b])) * float(cdf[-1])
+            assert m[ids[b]] > 0 and float(cdf[ids[b]]) - 1.0 <= target + 2e-9 * float(cdf[-1]) and float(cdf[ids[b]]) > target - 2e-9 * float(cdf[-1]), (b, ids[b])
