@@ -28,14 +28,16 @@ struct PagedSeq {
     const int32_t* pages;   // its row of the page table
 };
 
-// Sequence s of the batch; false (and n = 0) for one whose numbers do not fit the arrays:
-// no kernel follows them.  Every number that is used as an index below comes from here.
+// Sequence s of the batch; false (and held = n = 0, so that it is counted as an empty one where work
+// is dealt out) for one whose numbers do not fit the arrays: no kernel follows them.  Every number
+// that is used as an index below comes from here.
 __device__ __forceinline__ bool load_seq(const kivi_paged_layer& L, const kivi_paged_batch& b, int s, PagedSeq& q) {
     const int r0 = b.cu_new[s], r1 = b.cu_new[s + 1], held = b.seq_lens[s], slot = b.slots[s];
     q.pages = b.page_table + (int64_t)s * b.table_width;
-    q.row0 = r0; q.held = held; q.slot = slot; q.n = 0;
+    q.row0 = r0; q.held = 0; q.slot = slot; q.n = 0;
     if (r0 < 0 || r1 < r0 || r1 > b.total_new || r1 - r0 > b.max_new) return false;
     if (held < 0 || held > b.max_len - (r1 - r0) || slot < 0 || slot >= L.num_slots) return false;
+    q.held = held;
     q.n = r1 - r0;
     return true;
 }

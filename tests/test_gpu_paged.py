@@ -562,3 +562,32 @@ def test_rows_turned_in_place_while_groups_of_the_window_leave(ops, D, G, R, pag
     for _ in range(5):
         for x, y in zip(run(True), want):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 64, 10 ** 6])
+def test_a_sequence_that_is_left_out_takes_no_other_s_place(ops, length):
+    """A length that lies, beside sequences whose groups use every CTA of the launch: theirs are appended as without it."""
+    from intel_kivi_hybrid_b200 import cabi
+    D, G, R, H = 128, 32, 32, 2
+    news, start = [1] + [33] * 7, [0] + [31] * 7
+    pool = Pool(8, H, D, G, R, 64, 96, torch.bfloat16)
+    pool.append(ops, rows(sum(start), H, D, torch.bfloat16, 1), rows(sum(start), H, D, torch.bfloat16, 2), start)
+    before = [t.clone() for t in pool.t]
+    pool.lens = list(start)
+    k, v, rotary = rows(sum(news), H, D, torch.bfloat16, 3), rows(sum(news), H, D, torch.bfloat16, 4), torch.randn(96, D, device=DEV)
+    got = []
+    for lie in (False, True):
+        for t, b in zip(pool.t, before):
+            t.copy_(b)
+        a, k_out = pool.arrays(news), torch.zeros_like(k)
+        if lie:
+            a[2][0] = length
+        ops.paged_append(k, v, *pool.t, *a, 33, 96, G, rotary=rotary, k_out=k_out)
+        got.append([t.clone() for t in pool.t] + [k_out[1:]])
+    assert cabi.device_fault() == 4
+    cabi.device_fault_clear()
+    slot = int(pool.slots[0])
+    for x, y in zip(*got):
+        if x.shape[0] == before[6].shape[0]:
+            x[slot] = y[slot]                               # (the window of the one that is left out)
+        assert torch.equal(x, y)
