@@ -325,10 +325,15 @@ paged_merge_kernel(PagedAttnArgs A, int RT) {
     }
 }
 
+constexpr size_t general_bytes(int rows, int D) { return ((size_t)(rows + 2 * kTile) * (D + 4) + (size_t)rows * (kTile + 4)) * 4; }
+
 template <int RPT, int TY, int DT>
-int run_general(const PagedAttnArgs& a, int blocks, size_t smem, cudaStream_t st) {
+int run_general(const PagedAttnArgs& a, int blocks, cudaStream_t st) {
     auto* const kernel = paged_attention_kernel<RPT, TY, DT>;
-    if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (the limit is the kernel's, not the call's: what every call sets is the most that one needs)
+    constexpr size_t most = general_bytes(RPT * TY, DT);
+    if (most > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    const size_t smem = general_bytes(RPT * TY, a.L.head_dim);
     KIVI_CUDA_OK(launch(kernel, dim3((unsigned)blocks, (unsigned)a.L.num_kv_heads, (unsigned)a.pieces), TY * 16, smem, st, true, a));
     return KIVI_OK;
 }
@@ -337,7 +342,7 @@ int run_general(const PagedAttnArgs& a, int blocks, size_t smem, cudaStream_t st
 template <int DT>
 int run_again(const PagedAttnArgs& a, int blocks, cudaStream_t st) {
     auto* const kernel = paged_attention_kernel<4, 16, DT, true>;
-    const size_t smem = ((size_t)(64 + 2 * kTile) * (DT + 4) + (size_t)64 * (kTile + 4)) * 4;
+    constexpr size_t smem = general_bytes(64, DT);
     KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     KIVI_CUDA_OK(launch(kernel, dim3((unsigned)blocks * (kTensorRows / 64), (unsigned)a.L.num_kv_heads, (unsigned)a.pieces), 256, smem, st, true, a));
     return KIVI_OK;
@@ -469,7 +474,6 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
     a.part_ml = a.part_o + (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * D;
     a.vec = grid4(*q, q_dtype) && grid4(*new_k, L->res_dtype) && grid4(*new_v, L->res_dtype);
     cudaStream_t st = (cudaStream_t)stream;
-    const size_t smem = ((size_t)(p.rows + 2 * kTile) * (D + 4) + (size_t)p.rows * (kTile + 4)) * 4;
     int rc;
     if (p.kernel == PagedKernel::kDecode) {
         if (int rc2 = run_paged_decode(a, p.blocks / b->num_seqs, p.chunk, st)) return rc2;
@@ -481,8 +485,8 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
         a.rough = reinterpret_cast<int*>(static_cast<char*>(workspace) + need) - (size_t)p.blocks * L->num_kv_heads * p.pieces;
         rc = run_paged_tc(a, p.blocks, st);
         if (!rc) rc = D == 64 ? run_again<64>(a, p.blocks, st) : run_again<128>(a, p.blocks, st);
-    } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, smem, st) : run_general<1, 8, 256>(a, p.blocks, smem, st);
-    else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, smem, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, smem, st) : run_general<4, 16, 256>(a, p.blocks, smem, st);
+    } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, st) : run_general<1, 8, 256>(a, p.blocks, st);
+    else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, st) : run_general<4, 16, 256>(a, p.blocks, st);
     if (rc) return rc;
     int launches = p.kernel == PagedKernel::kTensor ? 2 : 1;
     if (p.pieces > 1) {

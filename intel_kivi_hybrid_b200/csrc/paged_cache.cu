@@ -585,7 +585,8 @@ extern "C" int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged
         KIVI_REQUIRE(k_out == nullptr || k_out->data == nullptr, "k_out is only written together with rotary");
     }
     const size_t smem = 2 * (size_t)G * (D * esz + 16) + 2 * D * 4 + (size_t)D * G / 2;
-    if (smem > 220 * 1024) {
+    constexpr size_t kMostSmem = 220 * 1024;
+    if (smem > kMostSmem) {
         set_error("a group of %d tokens of head_dim %d does not fit shared memory", G, D);
         return KIVI_ERR_UNSUPPORTED;
     }
@@ -617,7 +618,8 @@ extern "C" int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged
     const bool even = rounding == KIVI_ROUND_HALF_EVEN, fixed = D == 128 && G == 32;
     auto* const kernel = bf16 ? (a.q.data ? append_kernel<__nv_bfloat16, true>(wide, vec, even, fixed) : append_kernel<__nv_bfloat16, false>(wide, vec, even, fixed))
                               : (a.q.data ? append_kernel<float, true>(wide, vec, even, fixed) : append_kernel<float, false>(wide, vec, even, fixed));
-    if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (the limit is the kernel's, not the call's: two calls at once set the same)
+    if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem));
     KIVI_CUDA_OK(launch(kernel, dim3((unsigned)items, (unsigned)layer->num_kv_heads), kThreads, smem, st, true, a));
     note_launches(launches);
     return KIVI_OK;

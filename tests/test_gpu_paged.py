@@ -591,3 +591,32 @@ def test_a_sequence_that_is_left_out_takes_no_other_s_place(ops, length):
         if x.shape[0] == before[6].shape[0]:
             x[slot] = y[slot]                               # (the window of the one that is left out)
         assert torch.equal(x, y)
+
+
+def test_calls_of_two_threads_with_other_shapes(ops):
+    """Two caches whose kernels are the same and whose shared memory is not: neither thread's call is refused for the other's."""
+    import threading
+    failed = []
+
+    def work(D, seed):
+        try:
+            G, R, H, n = 32, 64, 2, 70
+            with torch.cuda.stream(torch.cuda.Stream()):
+                pool = Pool(1, H, D, G, R, 64, 200, torch.float32, seed)
+                k, q = rows(n, H, D, torch.float32, seed), rows(n, H, D, torch.float32, seed + 1)
+                a, want = pool.append(ops, k, k, [n]), None
+                for _ in range(400):
+                    pool.append(ops, k, k, [n])
+                    out = attend(ops, pool, q, k, k, [n], a)
+                    want = out if want is None else want
+                    if not torch.equal(out, want):
+                        failed.append(f"head_dim {D}: another result")
+                        return
+        except Exception as e:  # noqa: BLE001
+            failed.append(f"head_dim {D}: {e}")
+    threads = [threading.Thread(target=work, args=(D, i)) for i, D in enumerate((192, 256, 192, 256))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
