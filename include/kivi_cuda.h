@@ -464,7 +464,8 @@ typedef struct kivi_rows {
  * first rotary_dim channels of a head take part, in pairs (i, i + rotary_dim/2) or, with
  * interleaved != 0, (2i, 2i+1): a' = a cos - b sin, b' = b cos + a sin, two products and
  * one sum in fp32, each rounded, the result rounded to res_dtype.  k_out and q_out receive
- * the turned rows; they may be the inputs themselves. */
+ * the turned rows; they may be the inputs themselves (the same rows: other overlaps are not
+ * for it, and rows that start where the input does but lie differently are refused). */
 int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged_batch* batch,
                       const kivi_rows* new_k, const kivi_rows* new_v, const float* rotary, int rotary_rows,
                       int rotary_dim, int interleaved, const kivi_rows* q, int n_rep, const kivi_rows* q_out,
@@ -475,7 +476,7 @@ int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged_batch* bat
  * from pages and window, the step's own from new_k / new_v (turned, in full precision,
  * also those that the append has already moved to pages).
  * q, out: rows of q_dtype / out_dtype with num_kv_heads * n_rep heads.  sm_scale <= 0
- * means head_dim^-0.5.  out may be q itself.  workspace: device scratch of
+ * means head_dim^-0.5.  out may be q itself (of the same type, laid out the same).  workspace: device scratch of
  * kivi_paged_attention_workspace() bytes for the same arguments, contents need not be
  * preserved.
  * Accuracy: fp32 operands and sums; with bf16 rows (head_dim 64 or 128, groups of 32) the

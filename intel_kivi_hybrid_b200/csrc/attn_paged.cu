@@ -450,6 +450,7 @@ extern "C" int kivi_paged_attention(const kivi_paged_layer* L, const kivi_paged_
         KIVI_REQUIRE(r != nullptr && r->data != nullptr, "q, new_k, new_v or out is null");
         KIVI_REQUIRE(r->row_stride >= 0 && r->head_stride >= 0, "q, new_k, new_v or out has a negative stride");
     }
+    if (int rc = validate_in_place(out, "out", q, "q", b->total_new, L->num_kv_heads * n_rep, out_dtype == q_dtype)) return rc;
     if (b->max_new == 0) { note_launches(0); return KIVI_OK; }
     const int D = L->head_dim;
     // rows on 16-byte boundaries

@@ -518,6 +518,12 @@ int validate_batch(const kivi_paged_layer* L, const kivi_paged_batch* b) {
     return KIVI_OK;
 }
 
+int validate_in_place(const kivi_rows* to, const char* to_name, const kivi_rows* from, const char* from_name, int rows, int heads, bool same_type) {
+    KIVI_REQUIRE(to->data != from->data || (same_type && (rows <= 1 || to->row_stride == from->row_stride) && (heads <= 1 || to->head_stride == from->head_stride)),
+                 "%s starts where %s does but is laid out differently", to_name, from_name);
+    return KIVI_OK;
+}
+
 int paged_cache_fault_word(int* out) {
     KIVI_CUDA_OK(cudaMemcpyFromSymbol(out, g_fault, sizeof(int)));
     return KIVI_OK;
@@ -530,10 +536,9 @@ int paged_cache_fault_clear() {
 
 namespace {
 
-int check_rows(const kivi_rows* r, const char* name, int head_dim) {
+int check_rows(const kivi_rows* r, const char* name) {
     KIVI_REQUIRE(r != nullptr && r->data != nullptr, "%s is null", name);
     KIVI_REQUIRE(r->row_stride >= 0 && r->head_stride >= 0, "%s has a negative stride", name);
-    (void)head_dim;
     return KIVI_OK;
 }
 // vectors of n channels lie on their own grid
@@ -567,18 +572,20 @@ extern "C" int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged
     if (int rc = validate_paged(layer)) return rc;
     if (int rc = validate_batch(layer, batch)) return rc;
     const int D = layer->head_dim, G = layer->group_size, esz = elem_size(layer->res_dtype);
-    if (int rc = check_rows(new_k, "new_k", D)) return rc;
-    if (int rc = check_rows(new_v, "new_v", D)) return rc;
+    if (int rc = check_rows(new_k, "new_k")) return rc;
+    if (int rc = check_rows(new_v, "new_v")) return rc;
     KIVI_REQUIRE(rounding == KIVI_ROUND_HALF_AWAY || rounding == KIVI_ROUND_HALF_EVEN, "rounding must be KIVI_ROUND_HALF_AWAY or KIVI_ROUND_HALF_EVEN");
     const bool queries = q != nullptr && q->data != nullptr;
     if (rotary != nullptr) {
         KIVI_REQUIRE(rotary_dim > 0 && rotary_dim <= D && rotary_dim % 2 == 0, "rotary_dim (%d) must be even and at most head_dim (%d)", rotary_dim, D);
         KIVI_REQUIRE(interleaved || rotary_dim % 8 == 0, "rotary_dim (%d) must be a multiple of 8 where channels half of it apart are paired", rotary_dim);
         KIVI_REQUIRE(rotary_rows >= batch->max_len, "rotary holds %d positions, max_len is %d", rotary_rows, batch->max_len);
-        if (int rc = check_rows(k_out, "k_out", D)) return rc;
+        if (int rc = check_rows(k_out, "k_out")) return rc;
+        if (int rc = validate_in_place(k_out, "k_out", new_k, "new_k", batch->total_new, layer->num_kv_heads, true)) return rc;
         if (queries) {
             KIVI_REQUIRE(n_rep >= 1, "n_rep (%d) must be positive", n_rep);
-            if (int rc = check_rows(q_out, "q_out", D)) return rc;
+            if (int rc = check_rows(q_out, "q_out")) return rc;
+            if (int rc = validate_in_place(q_out, "q_out", q, "q", batch->total_new, layer->num_kv_heads * n_rep, true)) return rc;
         }
     } else {
         KIVI_REQUIRE(!queries, "queries are only taken together with rotary");

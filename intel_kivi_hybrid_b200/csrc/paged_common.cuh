@@ -101,5 +101,8 @@ __device__ __forceinline__ void settle_paged(kivi_paged_layer& L, kivi_paged_bat
 // ---- host side -------------------------------------------------------------------
 int validate_paged(const kivi_paged_layer* L);
 int validate_batch(const kivi_paged_layer* L, const kivi_paged_batch* b);
+// Rows that are written where rows are read: the same ones, or none of them (an element must not be
+// written while another row's reader still wants it).
+int validate_in_place(const kivi_rows* to, const char* to_name, const kivi_rows* from, const char* from_name, int rows, int heads, bool same_type);
 
 }  // namespace kivi

@@ -474,7 +474,6 @@ void paged_append(const torch::Tensor& new_k, const torch::Tensor& new_v, const 
         check_activation(*k_out, "k_out", p);
         ko = rows_of(*k_out, "k_out", rows, H, p);
         check_written(*k_out, "k_out");
-        TORCH_CHECK(ko.data != k.data || (ko.row_stride == k.row_stride && ko.head_stride == k.head_stride), "k_out starts where new_k does but is laid out differently");
     }
     if (q.has_value()) {
         TORCH_CHECK(q->dim() == 3 && q->size(1) % H == 0 && q->size(1) > 0, "q must be [rows, n_rep * kv_heads, head_dim]");
@@ -484,7 +483,6 @@ void paged_append(const torch::Tensor& new_k, const torch::Tensor& new_v, const 
         qr = rows_of(*q, "q", rows, q->size(1), p);
         qo = rows_of(*q_out, "q_out", rows, q->size(1), p);
         check_written(*q_out, "q_out");
-        TORCH_CHECK(qo.data != qr.data || (qo.row_stride == qr.row_stride && qo.head_stride == qr.head_stride), "q_out starts where q does but is laid out differently");
     }
     c10::cuda::CUDAGuard guard(p.device);
     if (rows == 0) return;

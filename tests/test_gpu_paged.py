@@ -620,3 +620,25 @@ def test_calls_of_two_threads_with_other_shapes(ops):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_rows_laid_out_otherwise_over_their_input_are_refused(ops):
+    D, G, R, H = 128, 32, 64, 2
+    pool = Pool(2, H, D, G, R, 64, 300, torch.bfloat16)
+    k, q = rows(10, H, D, torch.bfloat16, 1), rows(10, 2 * H, D, torch.bfloat16, 2)
+    a, rot = pool.arrays([5, 5]), torch.randn(300, D, device=DEV)
+    turn = lambda x: x.as_strided(x.shape, (D, x.shape[0] * D, 1))  # noqa: E731
+    wide = torch.zeros(10, 2 * H, D, device=DEV)
+    for bad, what in ((lambda: attend(ops, pool, q, k, k, [5, 5], a, out=turn(q)), "out starts where q does"),
+                      (lambda: attend(ops, pool, wide.view(torch.bfloat16).flatten()[:q.numel()].view(q.shape), k, k, [5, 5], a, out=wide), "out starts where q does"),
+                      (lambda: ops.paged_append(k, k.clone(), *pool.t, *a, 5, 5, G, rot, q, turn(q), k), "q_out starts where q does"),
+                      (lambda: ops.paged_append(k, k.clone(), *pool.t, *a, 5, 5, G, rot, q, q, turn(k)), "k_out starts where new_k does")):
+        with pytest.raises(RuntimeError, match=what):
+            bad()
+    # one row has no other to be in the way of
+    one, b = rows(1, 2 * H, D, torch.bfloat16, 3), pool.arrays([1, 0])
+    k1 = rows(1, H, D, torch.bfloat16, 4)
+    ops.paged_append(k1, k1, *pool.t, *b, 1, 1, G)
+    want = attend(ops, pool, one, k1, k1, [1, 0], b)
+    attend(ops, pool, one, k1, k1, [1, 0], b, out=one.as_strided(one.shape, (7 * H * D, D, 1)))
+    assert torch.equal(one, want)

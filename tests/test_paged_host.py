@@ -247,3 +247,27 @@ def test_the_filters_on_the_host_cut_where_the_definition_does(monkeypatch, dtyp
         margin = (above - top_p).abs().min() if top_p < 1.0 else (p / p.max() - min_p).abs().min()
         assert margin > 1e-5                                # (no entry is at the border: the answer is one set)
         assert torch.equal(got, (above < top_p if top_p < 1.0 else torch.ones_like(got)) & (p >= min_p * p.max()))
+
+
+def test_rows_written_in_place_lie_where_they_were_read(cabi):
+    """The C interface, before it launches: rows that start where the input does and lie otherwise are refused."""
+    lib, byref, some = cabi.lib, ctypes.byref, 4096
+    layer = cabi.PagedLayer(num_pages=4, page_tokens=64, num_kv_heads=2, head_dim=128, group_size=32, residual_cap=64, num_slots=2, res_dtype=1,
+                            **{n: some for n in ("k_codes", "k_scales", "k_zeros", "v_codes", "v_scales", "v_zeros", "k_res", "v_res")})
+    batch = lambda total: cabi.PagedBatch(num_seqs=1, table_width=4, page_table=some, slots=some, seq_lens=some, cu_new=some, total_new=total, max_new=1, max_len=100)  # noqa: E731
+    at = lambda row, head, p=some: cabi.Rows(p, row, head)  # noqa: E731
+
+    def attention(q, out, out_dtype=1, total=8):
+        other = at(256, 128, some * 5)
+        rc = lib.kivi_paged_attention(byref(layer), byref(batch(total)), byref(q), 1, byref(other), byref(other), byref(out), out_dtype, 2, 0.0, None, 0, None)
+        return rc, lib.kivi_last_error()
+
+    def append(k, k_out, q, q_out):
+        rc = lib.kivi_paged_append(byref(layer), byref(batch(8)), byref(k), byref(at(256, 128, some * 5)), some * 7, 100, 128, 0, byref(q), 2, byref(q_out), byref(k_out), 0, None)
+        return rc, lib.kivi_last_error()
+    kv, q = at(256, 128, some * 3), at(512, 128)
+    for (rc, said), what in ((attention(q, at(512, 512)), b"out starts where q does"), (attention(q, at(1024, 128)), b"out starts where q does"), (attention(q, q, 0), b"out starts where q does"),
+                             (append(kv, at(128, 1024, some * 3), q, q), b"k_out starts where new_k does"), (append(kv, kv, q, at(128, 1024)), b"q_out starts where q does")):
+        assert rc == 1 and what in said, (rc, what, said)
+    for rc, said in (attention(q, q), attention(q, at(1024, 128), total=1), attention(q, at(1024, 128, some * 9), 0)):
+        assert rc == 1 and b"workspace too small" in said               # (the check behind it)
