@@ -459,16 +459,16 @@ def sample_tokens(logits, temperature=1.0, top_k=0, do_sample=False, seed=0, ste
 
 
 def sample_filtered(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
-    """kivi_sample_filtered: [batch, vocab] fp32 / bf16 device logits (last dim contiguous) and one fp32 number of [0, 1)
-    a row -> int64 [batch] device ids.  temperature, top_p, min_p: fp32 device tensors of one entry per row, top_k: int32;
-    None: 1, no cut."""
+    """kivi_sample_filtered: [batch, vocab] fp32 / bf16 device logits (last dim contiguous; one row, expanded, may serve
+    all) and one fp32 number of [0, 1) a row -> int64 [batch] device ids.  temperature, top_p, min_p: fp32 device tensors
+    of one entry per row, top_k: int32; None: 1, no cut."""
     ops = _native_ops()
     if ops is not None:
         return ops.sample_filtered(logits, uniforms, temperature, top_k, top_p, min_p, out)
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] != 1):
         raise RuntimeError("logits must be [batch, vocab] with entries side by side")
     B, V = logits.shape
-    if B > 1 and logits.stride(0) < V:
+    if B > 1 and 0 != logits.stride(0) < V:
         raise RuntimeError("rows of logits overlap")
     if out is None:
         out = torch.empty(B, dtype=torch.int64, device=logits.device)
@@ -480,7 +480,7 @@ def sample_filtered(logits, uniforms, temperature=None, top_k=None, top_p=None, 
                 raise RuntimeError(f"one {dtype} entry for each of the {B} rows is needed on {logits.device}")
         ptr.append(None if t is None else t.data_ptr())
     if B:
-        _check(lib.kivi_sample_filtered(logits.data_ptr(), _dt(logits), B, V, max(logits.stride(0), V), *ptr, _stream()))
+        _check(lib.kivi_sample_filtered(logits.data_ptr(), _dt(logits), B, V, logits.stride(0) if B > 1 else V, *ptr, _stream()))
     return out
 
 

@@ -266,3 +266,19 @@ def test_temperatures_near_the_largest_number_and_infinite_ones(ops, V):
             cdf = m.cumsum(0)
             target = float(torch.tensor(u[b])) * float(cdf[-1])
             assert m[ids[b]] > 0 and float(cdf[ids[b]]) - 1.0 <= target + 2e-9 * float(cdf[-1]) and float(cdf[ids[b]]) > target - 2e-9 * float(cdf[-1]), (b, ids[b])
+
+
+def test_the_call_without_the_extension_takes_what_the_extension_takes(ops, monkeypatch):
+    from intel_kivi_hybrid_b200 import cabi
+    monkeypatch.setattr(cabi, "_native_ops", lambda: None)
+    x = 2 * torch.randn(8, 3001, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    row = lambda v, d=torch.float32: torch.full((8,), v, dtype=d, device="cuda")  # noqa: E731
+    u = torch.rand(8, generator=torch.Generator().manual_seed(8)).cuda()
+    for logits in (x, x.bfloat16(), x[:1].expand(8, 3001), x[:, 1:], x[:, :1]):
+        args = (logits, u, row(0.9), row(40, torch.int32), row(0.9), row(0.01))
+        assert torch.equal(cabi.sample_filtered(*args), ops.sample_filtered(*args))
+    assert torch.equal(cabi.sample_filtered(x[3:4, 7:], u[:1]), ops.sample_filtered(x[3:4, 7:], u[:1]))
+    for bad, what in ((lambda: cabi.sample_filtered(x.as_strided((8, 100), (50, 1)), u), "overlap"), (lambda: cabi.sample_filtered(x, u[:3]), "one torch.float32 entry"),
+                      (lambda: cabi.sample_filtered(x[:, ::2], u), "side by side")):
+        with pytest.raises(RuntimeError, match=what):
+            bad()
