@@ -479,9 +479,15 @@ int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged_batch* bat
  * means head_dim^-0.5.  out may be q itself (of the same type, laid out the same).  workspace: device scratch of
  * kivi_paged_attention_workspace() bytes for the same arguments, contents need not be
  * preserved.
- * Accuracy: fp32 operands and sums; with bf16 rows (head_dim 64 or 128, groups of 32) the
- * dequantized numbers and the weights are rounded at 2^-12, values below 2^-27 of a tile's
- * largest at less; sums are fp32.  A token that a row does not see does not touch it,
+ * Accuracy: sums are fp32, operands too but for two kinds of call, both with groups of 32.
+ * Steps of up to 12 rows a sequence (max_new * n_rep) with head_dim 128 and q of the window's
+ * type: fixed-point numbers for what is packed, as in kivi_decode_attention.  Other bf16 rows
+ * with head_dim 64 or 128: fp16 numbers for all, less a power of two for a row of q and for 128
+ * tokens; q and the window's and the step's tokens are not rounded by that, weights are at
+ * 2^-11, a packed token's scale and zero at 2^-11 each and what its code stands for once more,
+ * so that it is off by up to 2^-11 (code * scale + |zero| + |itself|), and numbers below 2^-27 of
+ * the largest of 128 tokens by more.  Where keys or values reach 2^16, infinity or NaN, the rows
+ * beside them are computed in fp32.  A token that a row does not see does not touch it,
  * whatever it holds. */
 size_t kivi_paged_attention_workspace(const kivi_paged_layer* layer, const kivi_paged_batch* batch, int q_dtype, int n_rep);
 int kivi_paged_attention(const kivi_paged_layer* layer, const kivi_paged_batch* batch, const kivi_rows* q,

@@ -17,7 +17,8 @@ A step of the model, over any set of its sequences::
 
 ``step`` is ``append`` (keys and queries turned to their positions on the way, whole groups quantized into pages) and
 ``attention`` (causal, over pages, window and the step's own tokens).  A sequence's tokens are attended as they
-are while they are in the window or new, as their codes stand for once they are in pages.
+are while they are in the window or new, as their codes stand for once they are in pages.  What a step has
+appended stays until its sequence is freed: tokens that a speculative decoder rejects cannot be taken back.
 
 All kernels follow arrays in device memory, so a step can be captured: ``begin(..., max_len=...)`` with the longest
 length it shall reach, and before each replay ``end(batch)`` and ``refresh(batch)``.  A layer's arrays are laid

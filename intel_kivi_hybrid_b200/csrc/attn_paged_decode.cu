@@ -14,7 +14,7 @@
 // a second kernel folds them.
 //
 // Bound as the contiguous kernel is: HBM and issue slots at length, latency with few tokens.
-// 16 rows at most: a block of four rows costs what it costs there (510 instructions of a warp
+// 12 rows at most: a block of four rows costs what it costs there (510 instructions of a warp
 // per group), the tensor-core kernel with 256 rows (attn_paged_tc.cu) the same for all.
 #include "attn_mma_core.cuh"
 #include "paged_attention.cuh"

@@ -25,7 +25,8 @@
 //
 // Bound by issue slots where rows are long, most of them the third walk's (130000 bf16 logits in
 // one CTA: 140000 cycles a row, of them maximum 11000, bins 23000-31000, third walk 75000), else by
-// latency: fifteen barriers and what hangs on them.  50257 fp32 logits: one row 29 us, 128 rows
+// latency: fourteen barriers up to the exact masses, seven to nine for each list that is searched, five
+// for the draw, and what hangs on them.  50257 fp32 logits: one row 29 us, 128 rows
 // of all filters 33; 64 rows of 130000 bf16 60.  Integer instructions take two slots, so
 // masses use few of them (two-word masses by bit operations: 92 us).
 #include "kivi_common.cuh"

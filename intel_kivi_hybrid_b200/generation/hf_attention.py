@@ -14,8 +14,8 @@ With this hook the model never sees a dense history:
   attention over the prompt's own K/V, exactly what the reference's prefill
   forward computes before the cache sees the tokens (generate.py:61-62).
   Several query tokens on a cache that already holds some (a prompt in pieces, a second
-  chat turn, speculative tokens) go to ``KiviCache.chunk_attention`` where the hook was
-  attached with ``chunked=True``.  Any other pattern (such tokens without it, a padded
+  chat turn; the cache keeps them all, so not tokens that may be rejected) go to
+  ``KiviCache.chunk_attention`` where the hook was attached with ``chunked=True``.  Any other pattern (such tokens without it, a padded
   decode batch, sliding-window layers) raises instead of attending to the wrong keys.
 
 One ordering difference from the reference loop: ``update()`` appends the step's
