@@ -642,3 +642,33 @@ def test_rows_laid_out_otherwise_over_their_input_are_refused(ops):
     want = attend(ops, pool, one, k1, k1, [1, 0], b)
     attend(ops, pool, one, k1, k1, [1, 0], b, out=one.as_strided(one.shape, (7 * H * D, D, 1)))
     assert torch.equal(one, want)
+
+
+@pytest.mark.parametrize("D,G,n_rep,new,dtype", KERNELS)
+def test_pages_and_slots_behind_two_to_the_31(ops, D, G, n_rep, new, dtype):
+    """The same sequences in a small pool and at the end of one whose arrays pass 2^31 bytes of codes and elements of the window."""
+    H, R, held, page = 2, 64, 200, 64
+    small = Pool(2, H, D, G, R, page, held + new, dtype)
+    n_pages, n_slots = small.t[0].shape[0], small.t[6].shape[0]
+    far_pages, far_slots = 2 ** 31 // (H * page * D // 4) + 10, 2 ** 31 // (H * R * D) + 10
+    if dtype == torch.float32:
+        far_slots = n_slots                                 # (8 GB and more a window: offsets in elements are those of bf16)
+    big = Pool.__new__(Pool)
+    big.__dict__.update(small.__dict__)
+    big.t = [torch.empty((far_pages if i < 6 else far_slots,) + t.shape[1:], dtype=t.dtype, device=DEV) for i, t in enumerate(small.t)]
+    big.table, big.slots = small.table + (far_pages - n_pages), small.slots + (far_slots - n_slots)
+    k0, v0 = rows(2 * held, H, D, dtype, 1), rows(2 * held, H, D, dtype, 2)
+    k, v, q = rows(2 * new, H, D, dtype, 3), rows(2 * new, H, D, dtype, 4), rows(2 * new, H * n_rep, D, dtype, 5)
+    got = []
+    for pool in (small, big):
+        pool.lens = [0, 0]
+        pool.append(ops, k0, v0, [held] * 2)
+        pool.lens = [held] * 2
+        a = pool.append(ops, k, v, [new] * 2)
+        out = attend(ops, pool, q, k, v, [new] * 2, a)
+        pool.lens = [held + new] * 2
+        got.append([out, *(torch.cat(x) for x in pool.read(ops, [0, 0], [held + new] * 2))])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    del pool, big, got
+    torch.cuda.empty_cache()
