@@ -484,9 +484,9 @@ int kivi_paged_append(const kivi_paged_layer* layer, const kivi_paged_batch* bat
  * type: fixed-point numbers for what is packed, as in kivi_decode_attention.  Other bf16 rows
  * with head_dim 64 or 128: fp16 numbers for all, less a power of two for a row of q and for 128
  * tokens; q and the window's and the step's tokens are not rounded by that, weights are at
- * 2^-11, a packed token's scale and zero at 2^-11 each and what its code stands for once more,
- * so that it is off by up to 2^-11 (code * scale + |zero| + |itself|), and numbers below 2^-27 of
- * the largest of 128 tokens by more.  Where keys or values reach 2^16, infinity or NaN, the rows
+ * 2^-11, a packed token's scale and the sum of zero and scale at 2^-11 each and what its code stands
+ * for once more, so that it is off by up to 2^-11 (|code - 1| scale + |zero + scale| + |itself|), and
+ * numbers below 2^-27 of the largest of 128 tokens by more.  Where keys or values reach 2^16, infinity or NaN, the rows
  * beside them are computed in fp32.  A token that a row does not see does not touch it,
  * whatever it holds. */
 size_t kivi_paged_attention_workspace(const kivi_paged_layer* layer, const kivi_paged_batch* batch, int q_dtype, int n_rep);

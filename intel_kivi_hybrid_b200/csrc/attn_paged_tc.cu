@@ -24,8 +24,10 @@
 // rescaled as for a new maximum).  The largest is between 2^13 and 2^14, so whatever is
 // within 2^-27 of it keeps 11 bits: a window's bf16 numbers are not rounded, weights at 2^-11, a
 // group's scales and zeros at 2^-11 too (the same way for its 32 tokens) and what a code stands for
-// once more.  bf16 operands would round at 2^-8, which is what the output itself is rounded at
-// (measured: 0.0020 of the output's 2-norm off 64 bits where its own rounding is 0.0017).
+// once more.  Codes count from 1, and z + s stands where z would, since those are smaller than c s and
+// z where numbers lie on both sides of 0 (from 0: a step of 385 us took 383, and the error below was
+// 0.0020).  bf16 operands would round at 2^-8, which is what the output itself is rounded at
+// (measured: 0.0018 of the output's 2-norm off 64 bits where its own rounding is 0.0017).
 // Sums, maxima and O are fp32.  One power of two for all the tokens of a tile is no good where a row
 // does not see, or gives no weight to, a token that is far larger than the others: the rows of a CTA
 // that has met a value of 2^16 or more, an infinity or a NaN are computed on the CUDA cores in fp32
@@ -33,8 +35,8 @@
 // within this kernel cost every call 8 %).  Below that, other tokens are exact to 2^-22.
 //
 // Codes to fp16: a 2-bit field and the exponent of 1024 make the number 1024 + c 4^n, of
-// which 1024 is taken off exactly; c 4^n (s / 4^n) + z is one fused operation for two
-// numbers.  3.3 instructions for two elements, where fp32 takes five and a conversion.
+// which 1024 + 4^n is taken off exactly; (c - 1) 4^n (s / 4^n) + (z + s) is one fused operation
+// for two numbers.  3.3 instructions for two elements, where fp32 takes five and a conversion.
 //
 // Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle); measured
 // 5500.  A block's chain is what bounds it: maximum 630-1000, weights 2800 while the other block
@@ -146,7 +148,7 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-constexpr uint32_t k1024 = 0x64006400u, kMinus1024 = 0xe400e400u;
+constexpr uint32_t k1024 = 0x64006400u, kMinus1024 = 0xe400e400u;        // (neighbours are 1 apart: bits of 1024 + n are 0x6400 + n)
 
 // The power of two that takes a largest magnitude (its bits) to 2^13 .. 2^14, kept where
 // it and its inverse are normal numbers; nothing (or infinity) is left as it is.
@@ -542,22 +544,24 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t af = raw + g * S::kFactors + (64 * hw + ch + 4 * i) * 4;
                     const float4 sc = lds_float4(af + S::raw_s), ze = lds_float4(af + S::raw_z);
-                    s2[2 * i] = pack_half(sc.x * f, sc.y * f); s2[2 * i + 1] = pack_half(sc.z * f, sc.w * f);
-                    z2[2 * i] = pack_half(ze.x * f, ze.y * f); z2[2 * i + 1] = pack_half(ze.z * f, ze.w * f);
+                    const float4 sf = make_float4(sc.x * f, sc.y * f, sc.z * f, sc.w * f);
+                    s2[2 * i] = pack_half(sf.x, sf.y); s2[2 * i + 1] = pack_half(sf.z, sf.w);
+                    z2[2 * i] = pack_half(fmaf(ze.x, f, sf.x), fmaf(ze.y, f, sf.y)); z2[2 * i + 1] = pack_half(fmaf(ze.z, f, sf.z), fmaf(ze.w, f, sf.w));
                     // bytes of two channels, 16 bits apart
                     const uint32_t at = raw + g * S::kCodes + hw * 512 + (jq + 4 * i) * 64 + 32 * m + 4 * c;
                     const uint32_t a = lds_u32(at), b = lds_u32(at + 16);
                     x[i][0] = __byte_perm(a, 0u, 0x4140); x[i][1] = __byte_perm(a, 0u, 0x4342);
                     x[i][2] = __byte_perm(b, 0u, 0x4140); x[i][3] = __byte_perm(b, 0u, 0x4342);
                 }
+                uint32_t one = kMinus1024 + 0x00010001u, mask = 0x00030003u;        // -(1024 + 4^n), and the codes' places
 #pragma unroll 1
-                for (int n = 0; n < 4; ++n) {
+                for (int n = 0; n < 4; ++n, one = 4u * one - 3u * kMinus1024, mask <<= 2) {
                     const uint32_t turn = to + (4 * jq + n) * 128 + (((2 * c + m) ^ ((4 * jq + n) & 7)) << 4);      // piece of the row, swizzled
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         uint32_t y[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & (0x00030003u << (2 * n))) | k1024, kMinus1024), s2[e], z2[e]);
+                        for (int e = 0; e < 4; ++e) y[e] = hfma2(hadd2((x[i][e] & mask) | k1024, one), s2[e], z2[e]);
                         sts128(turn + hw * (kN * 128) + i * (16 * 128), y[0], y[1], y[2], y[3]);
                     }
 #pragma unroll
@@ -594,14 +598,14 @@ paged_attention_tc_kernel(PagedAttnArgs A) {
                 for (int n = 0; n < 4; ++n) { sc[n] = lds_float(at + S::raw_s + n * (D == 128 ? 64 : 8)); ze[n] = lds_float(at + S::raw_z + n * (D == 128 ? 64 : 8)); }
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    const float s1 = sc[n] * f, z1 = ze[n] * f;
+                    const float s1 = sc[n] * f, z1 = fmaf(ze[n], f, s1);
                     const uint32_t s_lo = pack_half(s1, 0.25f * s1), s_hi = hmul2(s_lo, 0x2c002c00u) /* a sixteenth */, z = pack_half(z1, z1);
                     uint32_t y[4];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const uint32_t b = __byte_perm(w[e], 0u, 0x4040 + 0x0101 * n);      // byte n in both halves
-                        y[2 * e] = hfma2(hadd2((b & 0x000c0003u) | k1024, kMinus1024), s_lo, z);
-                        y[2 * e + 1] = hfma2(hadd2((b & 0x00c00030u) | k1024, kMinus1024), s_hi, z);
+                        y[2 * e] = hfma2(hadd2((b & 0x000c0003u) | k1024, kMinus1024 + 0x00040001u), s_lo, z);
+                        y[2 * e + 1] = hfma2(hadd2((b & 0x00c00030u) | k1024, kMinus1024 + 0x00400010u), s_hi, z);
                     }
                     sts128(out + n * 128 + ((piece ^ n) << 4), y[0], y[1], y[2], y[3]);
                 }
