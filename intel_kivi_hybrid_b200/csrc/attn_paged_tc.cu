@@ -25,8 +25,8 @@
 // within 2^-27 of it keeps 11 bits: a window's bf16 numbers are not rounded, weights at 2^-11, a
 // group's scales and zeros at 2^-11 too (the same way for its 32 tokens) and what a code stands for
 // once more.  Codes count from 1, and z + s stands where z would, since those are smaller than c s and
-// z where numbers lie on both sides of 0 (from 0: a step of 385 us took 383, and the error below was
-// 0.0020).  bf16 operands would round at 2^-8, which is what the output itself is rounded at
+// z where numbers lie on both sides of 0 (from 0: 389 us where the 512 rows below take 391, and the error
+// after this 0.0020).  bf16 operands would round at 2^-8, which is what the output itself is rounded at
 // (measured: 0.0018 of the output's 2-norm off 64 bits where its own rounding is 0.0017).
 // Sums, maxima and O are fp32.  One power of two for all the tokens of a tile is no good where a row
 // does not see, or gives no weight to, a token that is far larger than the others: the rows of a CTA
@@ -42,8 +42,8 @@
 // 5500.  A block's chain is what bounds it: maximum 630-1000, weights 2800 while the other block
 // makes its own, then 1400 until P V and the next scores are done.  One block: 4300, of which the
 // conversion of a tile takes 2800-3100 (bf16, 32k tokens).
-// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 385 us, 720 TFLOP/s; 4 x 2048 over
-// 16k 3114 us; 16 x 5 tokens over 4k 76 us; a prompt of 4 x 2048 440 us.  The roles share an
+// 512 rows of 4 heads per KV head over 32k tokens, 8 KV heads: 391 us, 708 TFLOP/s; 4 x 2048 over
+// 16k 3142 us; 16 x 5 tokens over 4k 76 us; a prompt of 4 x 2048 440 us.  The roles share an
 // instruction cache, so bodies are small: with the MMAs of a tile and four tokens of a key quad side
 // by side 403 us where this form had 391, 3280 (3246), 90 (78), with the conversions' channels unrolled
 // too 423, 3393, 99; but weights by 32 columns 426, 3440 (81) and values a token at a time 394, 3271, 88.
