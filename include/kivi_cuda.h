@@ -523,6 +523,108 @@ int kivi_sample_filtered(const void* logits, int dtype, int batch, int vocab, in
                          const float* uniforms, const float* temperature, const int32_t* top_k,
                          const float* top_p, const float* min_p, int64_t* ids_out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The paged cache in 8 bits: the same batches, windows and lengths, with whole blocks of
+ * G tokens held as e4m3 numbers and one scale for each block and head.
+ *
+ * No counterpart in the reference.  For models that 2 bits are too coarse for.
+ *   k_codes  [num_pages][num_kv_heads][page_tokens][D]: byte (t, d) at t*D + (p ^ w)*16 + d%16 with p = d/16 and
+ *            w = t & 7 where D is a multiple of 128, (t >> 1) & 3 where D is 64, else 0
+ *   v_codes  [num_pages][num_kv_heads][page_tokens*D]: byte (t, d) at (t/N*D + d)*N + i, N = 32, or 16 where G is no
+ *            multiple of 32; u = t % N stands at i = (u >> 1 & 3)*N/4 + (u >> 4)*4 + (u >> 3 & 1)*2 + (u & 1)
+ *   k_scales, v_scales [num_pages][num_kv_heads][page_tokens/G]
+ *   k_res, v_res as in kivi_paged_layer
+ * A block's scale is max(a / 448, 1e-30) in fp32, a its largest finite magnitude; x is held as the e4m3 number next
+ * to x * (1 / scale) (ties to even), infinities as the largest one, NaN as 0: whatever is in pages is finite.
+ * A code stands for its number times the scale, rounded to fp32.
+ * ---------------------------------------------------------------------- */
+typedef struct kivi_paged8_layer {
+    int32_t num_pages, page_tokens; /* page_tokens: multiple of group_size */
+    int32_t num_kv_heads, head_dim; /* head_dim: multiple of 16, <= 256 */
+    int32_t group_size, residual_cap; /* group_size: multiple of 16, <= 256 and <= residual_cap */
+    int32_t num_slots, res_dtype;
+    uint8_t* k_codes;
+    float* k_scales;
+    uint8_t* v_codes;
+    float* v_scales;
+    void* k_res;
+    void* v_res;
+} kivi_paged8_layer;
+
+/* How keys and queries are turned: as in kivi_paged_append, with these differences.  Pairs half of dim apart want a
+ * multiple of 16.  positions != NULL, device int32 [num_axes][total_new]: pair i of a token in row r is turned by row
+ * positions[pair_axis[i]][r] of the table in place of the token's place in its sequence; pair_axis: device int32
+ * [dim / 2].  A position outside the table or an axis outside 0 .. num_axes-1 is read as 0 and bit 2 of the fault
+ * word is set. */
+typedef struct kivi_rotary {
+    const float* table; /* device fp32 [rows][dim]; NULL: rows are taken as they are */
+    int32_t rows, dim, interleaved;
+    int32_t num_axes; /* with positions */
+    const int32_t* positions;
+    const int32_t* pair_axis;
+} kivi_rotary;
+
+/* kivi_paged_append for the cache in 8 bits (batch->ring_shift must be 0). */
+int kivi_paged8_append(const kivi_paged8_layer* layer, const kivi_paged_batch* batch,
+                       const kivi_rows* new_k, const kivi_rows* new_v, const kivi_rotary* rotary,
+                       const kivi_rows* q, int n_rep, const kivi_rows* q_out, const kivi_rows* k_out, void* stream);
+
+/* What is done to scores before the softmax.  With x = q k sm_scale, p the row's place in its sequence and j the
+ * token's: softcap > 0: x = softcap * tanh(x / softcap); then slopes != NULL, device fp32 [num_kv_heads * n_rep]:
+ * x += slopes[head] * (j - p).  Token j is seen by the row when p - window < j <= p (window <= 0: when j <= p), or when
+ * j < prefix[s] and the sequence holds it after the step (prefix: device int32 [num_seqs], NULL: 0; negative counts
+ * as 0): a prefix is seen by all rows, those before its end too. */
+typedef struct kivi_score_rules {
+    float softcap;
+    int32_t window;
+    const float* slopes;
+    const int32_t* prefix;
+} kivi_score_rules;
+
+/* Attention of a step's rows after kivi_paged8_append of the same batch, as kivi_paged_attention; rules may be NULL.
+ * A token that a row does not see does not touch it, whatever it holds. */
+size_t kivi_paged8_attention_workspace(const kivi_paged8_layer* layer, const kivi_paged_batch* batch, int q_dtype, int n_rep,
+                                       const kivi_score_rules* rules);
+int kivi_paged8_attention(const kivi_paged8_layer* layer, const kivi_paged_batch* batch, const kivi_rows* q,
+                          int q_dtype, const kivi_rows* new_k, const kivi_rows* new_v, const kivi_rows* out,
+                          int out_dtype, int n_rep, float sm_scale, const kivi_score_rules* rules, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* kivi_paged_read for the cache in 8 bits. */
+int kivi_paged8_read(const kivi_paged8_layer* layer, const kivi_paged_batch* batch, const int32_t* starts,
+                     float* k_out, float* v_out, void* stream);
+
+/* Penalties, biases and masks on a step's logits.
+ *
+ * No counterpart in the reference, whose sample_token (src/kivi_sycl/generation/sampling.py:10-25) takes logits as they are.
+ * Row b has had the tokens tokens[cu_tokens[b]] .. tokens[cu_tokens[b+1]-1], of which the first prompt_lens[b] were
+ * given and the others said.  In fp32, for token i: x = logits[b][i]; where the row has had it, x = x > 0 ? x /
+ * repetition[b] : x * repetition[b]; x -= frequency[b] * (times said); where it was said, x -= presence[b]; then
+ * x += bias of i, when one of bias_ids[cu_bias[b]] .. is i (the last of them stands); then -inf where bit i % 32 of word
+ * i / 32 of the row's mask is 0.  The mask is row allowed_rows[b] of allowed (-1: the row has none; NULL: row b).
+ * Ids outside 0 .. vocab-1 count for nothing.  Bounds that contradict num_tokens or num_bias are read as an empty
+ * list, a mask row from num_masks on as -1, and bit 2 of the fault word is set.
+ * tokens, bias_ids: device int64.  cu_tokens, cu_bias: device int32 [batch + 1]; prompt_lens: device int32 [batch]; any
+ * of prompt_lens (0), repetition (1), frequency (0), presence (0) may be NULL; tokens, bias_ids and allowed too.
+ * out: rows of the same type, logits itself or apart from it. */
+typedef struct kivi_logit_rules {
+    const int64_t* tokens;
+    const int32_t* cu_tokens;
+    const int32_t* prompt_lens;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int64_t* bias_ids;
+    const float* bias;
+    const int32_t* cu_bias;
+    const int32_t* allowed; /* [num_masks][mask_stride] words, mask_stride >= (vocab + 31) / 32 */
+    const int32_t* allowed_rows;
+    int32_t num_tokens, num_bias, num_masks;
+    int64_t mask_stride;
+} kivi_logit_rules;
+int kivi_adjust_logits(const void* logits, int dtype, int batch, int vocab, int64_t row_stride, const kivi_logit_rules* rules,
+                       void* out, int64_t out_stride, void* stream);
+
 /* Self-test (allocates 4 bytes, synchronises): the largest k for which the
  * tensor core, adding the products 1 and 2^-k to the addend -1 in one m16n8k16
  * fp16 MMA, still returns exactly 2^-k -- i.e. how many bits below the largest

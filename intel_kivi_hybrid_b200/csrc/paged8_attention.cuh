@@ -1,0 +1,54 @@
+// Arguments that the attention kernels over a paged cache in 8 bits share, and what a row sees.
+#pragma once
+
+#include "paged8.cuh"
+#include "paged_attention.cuh"
+
+namespace kivi {
+
+struct Paged8Attn {
+    kivi_paged8_layer L;
+    kivi_paged_batch b;
+    kivi_rows q, k, v, out;
+    kivi_score_rules rules;
+    int q_dtype, out_dtype, n_rep, vec;
+    float scale;                 // of q k
+    int pieces, chunk;           // a block's tiles of tokens are cut into pieces of `chunk` (no block has more than `pieces`)
+    float *part_o, *part_ml;     // [block][KV head][piece][row]: unnormalised output, (maximum, sum) in powers of two
+};
+
+// The tiles of T tokens that rows at places p_lo .. p_hi of a sequence of `total` tokens see something of: those of
+// the prefix and those from the first row's window on, without what lies between.
+struct Span {
+    int n, n1, gap;              // tiles; tile v is token tile v for v < n1, else v + gap
+    __host__ __device__ __forceinline__ int tile(int v) const { return v < n1 ? v : v + gap; }
+};
+__host__ __device__ __forceinline__ Span span_of(int T, int total, int p_lo, int p_hi, int window, int prefix) {
+    const int P = prefix < 0 ? 0 : prefix < total ? prefix : total, end = p_hi + 1 > P ? p_hi + 1 : P;
+    const int from = window > 0 && p_lo >= window ? p_lo - window + 1 : 0;
+    Span s{(end + T - 1) / T, 0, 0};
+    if (from > P) {
+        s.n1 = (P + T - 1) / T;
+        const int second = from / T > s.n1 ? from / T : s.n1;
+        s.gap = second - s.n1;
+        s.n -= s.gap;
+    }
+    return s;
+}
+// first token of a row's window (the row is at place p)
+__host__ __device__ __forceinline__ int window_from(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int prefix_of(const kivi_score_rules& r, int s, int total) {
+    const int p = r.prefix ? r.prefix[s] : 0;
+    return p < 0 ? 0 : p < total ? p : total;
+}
+__device__ __forceinline__ void settle_args(Paged8Attn& a) {
+    settle_paged8(a.L, a.b);
+    a.q.data = settled(a.q.data); a.k.data = settled(a.k.data); a.v.data = settled(a.v.data);
+    a.rules.slopes = settled(a.rules.slopes); a.rules.prefix = settled(a.rules.prefix);
+    a.part_o = settled(a.part_o); a.part_ml = settled(a.part_ml);
+}
+#endif
+
+}  // namespace kivi

@@ -31,7 +31,9 @@ struct PagedSeq {
 // Sequence s of the batch; false (and held = n = 0, so that it is counted as an empty one where work
 // is dealt out) for one whose numbers do not fit the arrays: no kernel follows them.  Every number
 // that is used as an index below comes from here.
-__device__ __forceinline__ bool load_seq(const kivi_paged_layer& L, const kivi_paged_batch& b, int s, PagedSeq& q) {
+// (Layer: kivi_paged_layer or kivi_paged8_layer)
+template <typename Layer>
+__device__ __forceinline__ bool load_seq(const Layer& L, const kivi_paged_batch& b, int s, PagedSeq& q) {
     const int r0 = b.cu_new[s], r1 = b.cu_new[s + 1], held = b.seq_lens[s], slot = b.slots[s];
     q.pages = b.page_table + (int64_t)s * b.table_width;
     q.row0 = r0; q.held = 0; q.slot = slot; q.n = 0;
@@ -43,7 +45,8 @@ __device__ __forceinline__ bool load_seq(const kivi_paged_layer& L, const kivi_p
 }
 
 // One block of a launch tells of the sequences that are left out.
-__device__ __forceinline__ void report_left_out(const kivi_paged_layer& L, const kivi_paged_batch& b, int* fault) {
+template <typename Layer>
+__device__ __forceinline__ void report_left_out(const Layer& L, const kivi_paged_batch& b, int* fault) {
     for (int s = threadIdx.x; s < b.num_seqs; s += blockDim.x) {
         PagedSeq q;
         if (!load_seq(L, b, s, q)) atomicOr(fault, kPagedFault);
@@ -52,7 +55,8 @@ __device__ __forceinline__ void report_left_out(const kivi_paged_layer& L, const
 
 // page of group position t (t a token index below quant_of); a bad entry counts as page 0
 // and is reported
-__device__ __forceinline__ int page_of(const kivi_paged_layer& L, const PagedSeq& q, int t, int* fault) {
+template <typename Layer>
+__device__ __forceinline__ int page_of(const Layer& L, const PagedSeq& q, int t, int* fault) {
     const int p = q.pages[t / L.page_tokens];
     if ((unsigned)p < (unsigned)L.num_pages) return p;
     atomicOr(fault, kPagedFault);

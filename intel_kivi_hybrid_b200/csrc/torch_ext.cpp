@@ -533,6 +533,232 @@ void paged_read(const torch::Tensor& k_packed, const torch::Tensor& k_scales, co
     check(kivi_paged_read(&p.L, &p.b, starts.data_ptr<int32_t>(), k_out.data_ptr<float>(), v_out.data_ptr<float>(), stream_of(k_res)));
 }
 
+// ---- paged cache in 8 bits ---------------------------------------------------------
+struct Paged8Operands {
+    kivi_paged8_layer L;
+    kivi_paged_batch b;
+    torch::Device device;
+};
+
+Paged8Operands paged8_operands(const torch::Tensor& k_codes, const torch::Tensor& k_scales, const torch::Tensor& v_codes, const torch::Tensor& v_scales,
+                               const torch::Tensor& k_res, const torch::Tensor& v_res, const torch::Tensor& page_table, const torch::Tensor& slots,
+                               const torch::Tensor& seq_lens, const torch::Tensor& cu_new, int64_t total_new, int64_t max_new, int64_t max_len, int64_t G) {
+    Paged8Operands p{{}, {}, k_res.device()};
+    TORCH_CHECK(k_res.is_cuda(), "k_res must be on cuda but got ", k_res.device().str());
+    TORCH_CHECK(k_res.scalar_type() == torch::kFloat32 || k_res.scalar_type() == torch::kBFloat16, "k_res must be Float or BFloat16 but got ", torch::toString(k_res.scalar_type()));
+    TORCH_CHECK(k_res.dim() == 4 && v_res.sizes() == k_res.sizes(), "k_res and v_res must both be [slots, kv_heads, R, D]");
+    const auto type = k_res.scalar_type();
+    check_paged_tensor(k_res, "k_res", type, p.device);
+    check_paged_tensor(v_res, "v_res", type, p.device);
+    check_paged_tensor(k_codes, "k_codes", torch::kUInt8, p.device);
+    check_paged_tensor(v_codes, "v_codes", torch::kUInt8, p.device);
+    check_paged_tensor(k_scales, "k_scales", torch::kFloat32, p.device);
+    check_paged_tensor(v_scales, "v_scales", torch::kFloat32, p.device);
+    check_paged_tensor(page_table, "page_table", torch::kInt, p.device);
+    check_paged_tensor(slots, "slots", torch::kInt, p.device);
+    check_paged_tensor(seq_lens, "seq_lens", torch::kInt, p.device);
+    check_paged_tensor(cu_new, "cu_new", torch::kInt, p.device);
+    const int64_t n_slots = k_res.size(0), H = k_res.size(1), R = k_res.size(2), D = k_res.size(3);
+    TORCH_CHECK(G > 0 && G % 16 == 0, "group_size must be a positive multiple of 16, got ", G);
+    TORCH_CHECK(D > 0 && D % 16 == 0, "head_dim (", D, ") must be a multiple of 16");
+    TORCH_CHECK(k_codes.dim() == 4 && k_codes.size(1) == H && k_codes.size(3) == D && k_codes.numel() > 0 && k_codes.size(2) % G == 0,
+                "k_codes must be [pages, kv_heads, page_tokens, head_dim] with page_tokens a multiple of group_size (", G, ")");
+    const int64_t pages = k_codes.size(0), T = k_codes.size(2);
+    TORCH_CHECK(v_codes.numel() == k_codes.numel(), "v_codes size must match k_codes size");
+    TORCH_CHECK(k_scales.numel() == pages * H * (T / G) && v_scales.numel() == k_scales.numel(), "k_scales / v_scales size must equal pages * kv_heads * page_tokens / group_size = ", pages * H * (T / G));
+    TORCH_CHECK(page_table.dim() == 2, "page_table must be [sequences, pages of a sequence]");
+    const int64_t n = page_table.size(0), width = page_table.size(1);
+    TORCH_CHECK(slots.numel() == n && seq_lens.numel() == n && cu_new.numel() == n + 1,
+                "slots, seq_lens and cu_new must hold ", n, ", ", n, " and ", n + 1, " entries for a page table of ", n, " sequences");
+    for (int64_t x : {n, width, pages, T, G, H, R, n_slots, total_new, max_new, max_len})
+        TORCH_CHECK(x >= 0 && x <= kInt32Max, "a size (", x, ") is outside 0 .. 2**31 - 1");
+    p.L = {(int32_t)pages, (int32_t)T, (int32_t)H, (int32_t)D, (int32_t)G, (int32_t)R, (int32_t)n_slots, type == torch::kFloat32 ? KIVI_F32 : KIVI_BF16,
+           k_codes.data_ptr<uint8_t>(), k_scales.data_ptr<float>(), v_codes.data_ptr<uint8_t>(), v_scales.data_ptr<float>(), k_res.data_ptr(), v_res.data_ptr()};
+    p.b = {(int32_t)n, (int32_t)width, page_table.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), cu_new.data_ptr<int32_t>(),
+           (int32_t)total_new, (int32_t)max_new, (int32_t)max_len, 0};
+    return p;
+}
+// (what rows_of and check_activation look at)
+PagedOperands rows_like(const Paged8Operands& p) {
+    PagedOperands r{{}, p.b, p.device};
+    r.L.head_dim = p.L.head_dim;
+    r.L.res_dtype = p.L.res_dtype;
+    return r;
+}
+
+void paged8_append(const torch::Tensor& new_k, const torch::Tensor& new_v, const torch::Tensor& k_codes, const torch::Tensor& k_scales, const torch::Tensor& v_codes,
+                   const torch::Tensor& v_scales, const torch::Tensor& k_res, const torch::Tensor& v_res, const torch::Tensor& page_table, const torch::Tensor& slots,
+                   const torch::Tensor& seq_lens, const torch::Tensor& cu_new, int64_t max_new, int64_t max_len, int64_t group_size,
+                   const c10::optional<torch::Tensor>& rotary, const c10::optional<torch::Tensor>& q, const c10::optional<torch::Tensor>& q_out,
+                   const c10::optional<torch::Tensor>& k_out, bool interleaved, const c10::optional<torch::Tensor>& positions,
+                   const c10::optional<torch::Tensor>& pair_axis) {
+    TORCH_CHECK(new_k.dim() == 3, "new_k must be [rows, kv_heads, head_dim]");
+    const Paged8Operands p = paged8_operands(k_codes, k_scales, v_codes, v_scales, k_res, v_res, page_table, slots, seq_lens, cu_new, new_k.size(0), max_new, max_len, group_size);
+    const PagedOperands like = rows_like(p);
+    const int64_t rows = new_k.size(0), H = p.L.num_kv_heads;
+    check_activation(new_k, "new_k", like);
+    check_activation(new_v, "new_v", like);
+    const kivi_rows k = rows_of(new_k, "new_k", rows, H, like), v = rows_of(new_v, "new_v", rows, H, like);
+    TORCH_CHECK(rotary.has_value() == k_out.has_value(), "rotary and k_out are given together or not at all");
+    TORCH_CHECK(q.has_value() == q_out.has_value() && (!q.has_value() || rotary.has_value()), "q and q_out are given together, and only with rotary");
+    TORCH_CHECK(positions.has_value() == pair_axis.has_value() && (!positions.has_value() || rotary.has_value()), "positions and pair_axis are given together, and only with rotary");
+    kivi_rows qr{}, qo{}, ko{};
+    kivi_rotary rot{};
+    int64_t n_rep = 1;
+    if (rotary.has_value()) {
+        check_paged_tensor(*rotary, "rotary", torch::kFloat32, p.device);
+        TORCH_CHECK(rotary->dim() == 2 && rotary->size(1) <= kInt32Max, "rotary must be [positions, rotary_dim]: cosines, then sines");
+        check_activation(*k_out, "k_out", like);
+        ko = rows_of(*k_out, "k_out", rows, H, like);
+        check_written(*k_out, "k_out");
+        rot = {rotary->data_ptr<float>(), (int32_t)std::min<int64_t>(rotary->size(0), kInt32Max), (int32_t)rotary->size(1), interleaved ? 1 : 0, 0, nullptr, nullptr};
+    }
+    if (positions.has_value()) {
+        check_paged_tensor(*positions, "positions", torch::kInt, p.device);
+        check_paged_tensor(*pair_axis, "pair_axis", torch::kInt, p.device);
+        TORCH_CHECK(positions->dim() == 2 && positions->size(1) == rows && positions->size(0) >= 1 && positions->size(0) <= kInt32Max, "positions must be [axes, ", rows, "]");
+        TORCH_CHECK(pair_axis->numel() == rotary->size(1) / 2, "pair_axis must hold an axis for each of the ", rotary->size(1) / 2, " pairs");
+        rot.num_axes = (int32_t)positions->size(0);
+        rot.positions = positions->data_ptr<int32_t>();
+        rot.pair_axis = pair_axis->data_ptr<int32_t>();
+    }
+    if (q.has_value()) {
+        TORCH_CHECK(q->dim() == 3 && q->size(1) % H == 0 && q->size(1) > 0, "q must be [rows, n_rep * kv_heads, head_dim]");
+        n_rep = q->size(1) / H;
+        check_activation(*q, "q", like);
+        check_activation(*q_out, "q_out", like);
+        qr = rows_of(*q, "q", rows, q->size(1), like);
+        qo = rows_of(*q_out, "q_out", rows, q->size(1), like);
+        check_written(*q_out, "q_out");
+    }
+    c10::cuda::CUDAGuard guard(p.device);
+    if (rows == 0) return;
+    check(kivi_paged8_append(&p.L, &p.b, &k, &v, &rot, &qr, (int)std::min<int64_t>(n_rep, kInt32Max), &qo, &ko, stream_of(k_res)));
+}
+
+void paged8_attention(const torch::Tensor& q, const torch::Tensor& new_k, const torch::Tensor& new_v, const torch::Tensor& k_codes, const torch::Tensor& k_scales,
+                      const torch::Tensor& v_codes, const torch::Tensor& v_scales, const torch::Tensor& k_res, const torch::Tensor& v_res, const torch::Tensor& page_table,
+                      const torch::Tensor& slots, const torch::Tensor& seq_lens, const torch::Tensor& cu_new, int64_t max_new, int64_t max_len, const torch::Tensor& out,
+                      int64_t group_size, double sm_scale, double softcap, const c10::optional<torch::Tensor>& slopes, int64_t window,
+                      const c10::optional<torch::Tensor>& prefix) {
+    TORCH_CHECK(q.dim() == 3, "q must be [rows, n_rep * kv_heads, head_dim]");
+    const Paged8Operands p = paged8_operands(k_codes, k_scales, v_codes, v_scales, k_res, v_res, page_table, slots, seq_lens, cu_new, q.size(0), max_new, max_len, group_size);
+    const PagedOperands like = rows_like(p);
+    const int64_t rows = q.size(0), H = p.L.num_kv_heads;
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % H == 0, "q must be [rows, n_rep * kv_heads, head_dim]");
+    const int64_t n_rep = q.size(1) / H;
+    check_activation(new_k, "new_k", like);
+    check_activation(new_v, "new_v", like);
+    const int q_dtype = dtype_code(q, "q"), out_dtype = dtype_code(out, "out");
+    const kivi_rows qr = rows_of(q, "q", rows, q.size(1), like), k = rows_of(new_k, "new_k", rows, H, like), v = rows_of(new_v, "new_v", rows, H, like),
+                    o = rows_of(out, "out", rows, q.size(1), like);
+    check_written(out, "out");
+    TORCH_CHECK(softcap >= 0.0, "softcap must be 0 (none) or positive");
+    TORCH_CHECK(window >= 0, "window must be 0 (none) or positive");
+    kivi_score_rules rules{(float)softcap, (int32_t)std::min<int64_t>(window, kInt32Max), nullptr, nullptr};
+    TORCH_CHECK(softcap == 0.0 || rules.softcap > 0.0f, "softcap is too small");
+    if (slopes.has_value()) {
+        check_paged_tensor(*slopes, "slopes", torch::kFloat32, p.device);
+        TORCH_CHECK(slopes->numel() == q.size(1), "slopes must hold an entry for each of the ", q.size(1), " query heads");
+        rules.slopes = slopes->data_ptr<float>();
+    }
+    if (prefix.has_value()) {
+        check_paged_tensor(*prefix, "prefix", torch::kInt, p.device);
+        TORCH_CHECK(prefix->numel() == p.b.num_seqs, "prefix must hold an entry for each of the ", p.b.num_seqs, " sequences");
+        rules.prefix = prefix->data_ptr<int32_t>();
+    }
+    c10::cuda::CUDAGuard guard(p.device);
+    if (rows == 0) return;
+    const size_t need = kivi_paged8_attention_workspace(&p.L, &p.b, q_dtype, (int)std::min<int64_t>(n_rep, kInt32Max), &rules);
+    const torch::Tensor ws = need ? at::empty({(int64_t)need}, q.options().dtype(torch::kUInt8)) : torch::Tensor();
+    check(kivi_paged8_attention(&p.L, &p.b, &qr, q_dtype, &k, &v, &o, out_dtype, (int)std::min<int64_t>(n_rep, kInt32Max), (float)sm_scale, &rules,
+                                need ? ws.data_ptr() : nullptr, need, stream_of(k_res)));
+}
+
+void paged8_read(const torch::Tensor& k_codes, const torch::Tensor& k_scales, const torch::Tensor& v_codes, const torch::Tensor& v_scales, const torch::Tensor& k_res,
+                 const torch::Tensor& v_res, const torch::Tensor& page_table, const torch::Tensor& slots, const torch::Tensor& seq_lens, const torch::Tensor& starts,
+                 const torch::Tensor& cu_read, int64_t max_read, const torch::Tensor& k_out, const torch::Tensor& v_out, int64_t group_size) {
+    TORCH_CHECK(k_out.dim() == 3, "k_out must be [rows, kv_heads, head_dim]");
+    Paged8Operands p = paged8_operands(k_codes, k_scales, v_codes, v_scales, k_res, v_res, page_table, slots, seq_lens, cu_read, k_out.size(0), max_read, 0, group_size);
+    // the longest sequence that the page table describes
+    p.b.max_len = (int32_t)std::min<int64_t>((int64_t)p.b.table_width * p.L.page_tokens + p.L.residual_cap - 1, 1 << 30);
+    check_paged_tensor(starts, "starts", torch::kInt, p.device);
+    TORCH_CHECK(starts.numel() == p.b.num_seqs, "starts must hold an entry for every sequence");
+    check_paged_tensor(k_out, "k_out", torch::kFloat32, p.device);
+    check_paged_tensor(v_out, "v_out", torch::kFloat32, p.device);
+    TORCH_CHECK(k_out.size(1) == p.L.num_kv_heads && k_out.size(2) == p.L.head_dim && v_out.sizes() == k_out.sizes(), "k_out and v_out must both be [rows, kv_heads, head_dim]");
+    c10::cuda::CUDAGuard guard(p.device);
+    if (k_out.size(0) == 0) return;
+    check(kivi_paged8_read(&p.L, &p.b, starts.data_ptr<int32_t>(), k_out.data_ptr<float>(), v_out.data_ptr<float>(), stream_of(k_res)));
+}
+
+torch::Tensor adjust_logits(const torch::Tensor& logits, const c10::optional<torch::Tensor>& out, const c10::optional<torch::Tensor>& tokens,
+                            const c10::optional<torch::Tensor>& cu_tokens, const c10::optional<torch::Tensor>& prompt_lens, const c10::optional<torch::Tensor>& repetition,
+                            const c10::optional<torch::Tensor>& frequency, const c10::optional<torch::Tensor>& presence, const c10::optional<torch::Tensor>& bias_ids,
+                            const c10::optional<torch::Tensor>& bias, const c10::optional<torch::Tensor>& cu_bias, const c10::optional<torch::Tensor>& allowed,
+                            const c10::optional<torch::Tensor>& allowed_rows) {
+    TORCH_CHECK(logits.is_cuda(), "logits must be on cuda but got ", logits.device().str());
+    TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [batch, vocab] with entries side by side");
+    const int dtype = dtype_code(logits, "logits");
+    const int64_t B = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(B <= 65535 && V > 0 && V <= 0x7fff0000, "batch must be at most 65535, vocab between 1 and 2**31 - 2**16");
+    TORCH_CHECK(B <= 1 || logits.stride(0) >= V || logits.stride(0) == 0, "rows of logits overlap");
+    if (out.has_value()) {
+        TORCH_CHECK(out->device() == logits.device(), "out is on ", out->device().str(), " but logits is on ", logits.device().str(), ": all tensors of one call must be on the same device");
+        TORCH_CHECK(out->scalar_type() == logits.scalar_type() && out->sizes() == logits.sizes(), "out must be like logits");
+        TORCH_CHECK((out->stride(1) == 1 || V == 1) && (B <= 1 || out->stride(0) >= V), "out must have entries side by side and rows apart");
+        const auto lo = (uintptr_t)logits.data_ptr(), olo = (uintptr_t)out->data_ptr();
+        const uintptr_t size = logits.element_size();
+        const uintptr_t hi = lo + ((B ? B - 1 : 0) * logits.stride(0) + V) * size, ohi = olo + ((B ? B - 1 : 0) * out->stride(0) + V) * size;
+        TORCH_CHECK(B == 0 || lo >= ohi || olo >= hi || (lo == olo && (B == 1 || logits.stride(0) == out->stride(0))), "out lies over logits but is laid out differently");
+    }
+    auto given = [&](const c10::optional<torch::Tensor>& t, const char* name, torch::ScalarType type, int64_t n) -> void* {
+        if (!t.has_value()) return nullptr;
+        check_paged_tensor(*t, name, type, logits.device());
+        TORCH_CHECK(n < 0 || t->numel() == n, name, " must hold ", n, " entries for ", B, " rows");
+        TORCH_CHECK(t->numel() <= kInt32Max, name, " has too many entries");
+        return t->data_ptr();
+    };
+    kivi_logit_rules r{};
+    TORCH_CHECK(tokens.has_value() == cu_tokens.has_value(), "tokens and cu_tokens are given together or not at all");
+    TORCH_CHECK(tokens.has_value() || (!prompt_lens.has_value() && !repetition.has_value() && !frequency.has_value() && !presence.has_value()), "penalties need tokens");
+    TORCH_CHECK(bias_ids.has_value() == bias.has_value() && bias.has_value() == cu_bias.has_value(), "bias_ids, bias and cu_bias are given together or not at all");
+    TORCH_CHECK(allowed.has_value() || !allowed_rows.has_value(), "allowed_rows need allowed");
+    if (tokens.has_value()) {
+        r.tokens = (const int64_t*)given(tokens, "tokens", torch::kLong, -1);
+        r.num_tokens = (int32_t)tokens->numel();
+        if (r.num_tokens == 0) r.tokens = nullptr;
+    }
+    r.cu_tokens = (const int32_t*)given(cu_tokens, "cu_tokens", torch::kInt, B + 1);
+    r.prompt_lens = (const int32_t*)given(prompt_lens, "prompt_lens", torch::kInt, B);
+    r.repetition = (const float*)given(repetition, "repetition", torch::kFloat32, B);
+    r.frequency = (const float*)given(frequency, "frequency", torch::kFloat32, B);
+    r.presence = (const float*)given(presence, "presence", torch::kFloat32, B);
+    if (r.tokens == nullptr) r.prompt_lens = nullptr, r.repetition = r.frequency = r.presence = nullptr;        // (an empty list: nothing to penalise)
+    if (bias_ids.has_value()) {
+        r.bias_ids = (const int64_t*)given(bias_ids, "bias_ids", torch::kLong, -1);
+        r.num_bias = (int32_t)bias_ids->numel();
+        r.bias = (const float*)given(bias, "bias", torch::kFloat32, bias_ids->numel());
+        if (r.num_bias == 0) r.bias_ids = nullptr;
+    }
+    r.cu_bias = (const int32_t*)given(cu_bias, "cu_bias", torch::kInt, B + 1);
+    if (allowed.has_value()) {
+        check_paged_tensor(*allowed, "allowed", torch::kInt, logits.device());
+        TORCH_CHECK(allowed->dim() == 2 && allowed->size(1) >= (V + 31) / 32, "allowed must be [masks, ", (V + 31) / 32, " words of 32 bits]");
+        TORCH_CHECK(allowed->size(0) >= 1 && allowed->size(0) <= kInt32Max, "allowed holds no mask");
+        TORCH_CHECK(allowed_rows.has_value() || allowed->size(0) == B, "allowed must hold a mask for each of the ", B, " rows where allowed_rows is not given");
+        r.allowed = allowed->data_ptr<int32_t>();
+        r.num_masks = (int32_t)allowed->size(0);
+        r.mask_stride = allowed->size(1);
+    }
+    r.allowed_rows = (const int32_t*)given(allowed_rows, "allowed_rows", torch::kInt, B);
+    c10::cuda::CUDAGuard guard(logits.device());
+    const torch::Tensor to = out.has_value() ? *out : at::empty({B, V}, logits.options());
+    if (B == 0) return to;
+    check(kivi_adjust_logits(logits.data_ptr(), dtype, (int)B, (int)V, B > 1 ? logits.stride(0) : V, &r, to.data_ptr(), B > 1 ? to.stride(0) : V, stream_of(logits)));
+    return to;
+}
+
 torch::Tensor sample_filtered(const torch::Tensor& logits, const torch::Tensor& uniforms, const c10::optional<torch::Tensor>& temperature,
                               const c10::optional<torch::Tensor>& top_k, const c10::optional<torch::Tensor>& top_p, const c10::optional<torch::Tensor>& min_p,
                               const c10::optional<torch::Tensor>& out) {
@@ -714,6 +940,30 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("k_packed"), py::arg("k_scales"), py::arg("k_zeros"), py::arg("v_packed"), py::arg("v_scales"), py::arg("v_zeros"), py::arg("k_res"),
           py::arg("v_res"), py::arg("page_table"), py::arg("slots"), py::arg("seq_lens"), py::arg("starts"), py::arg("cu_read"), py::arg("max_read"),
           py::arg("k_out"), py::arg("v_out"), py::arg("group_size"), py::arg("ring_shift") = 0);
+    // ---- paged cache in 8 bits, logits ------------------------------------------------
+    m.def("paged8_append", &paged8_append, py::call_guard<py::gil_scoped_release>(),
+          "paged_append for a cache in 8 bits: whole blocks of group_size tokens become e4m3 numbers with a scale for each block and head. With "
+          "positions [axes, rows] and pair_axis [rotary_dim / 2] pair i of a token is turned by its position on axis pair_axis[i]. Stream-ordered.",
+          py::arg("new_k"), py::arg("new_v"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("k_res"), py::arg("v_res"),
+          py::arg("page_table"), py::arg("slots"), py::arg("seq_lens"), py::arg("cu_new"), py::arg("max_new"), py::arg("max_len"), py::arg("group_size"),
+          py::arg("rotary") = py::none(), py::arg("q") = py::none(), py::arg("q_out") = py::none(), py::arg("k_out") = py::none(), py::arg("interleaved") = false,
+          py::arg("positions") = py::none(), py::arg("pair_axis") = py::none());
+    m.def("paged8_attention", &paged8_attention, py::call_guard<py::gil_scoped_release>(),
+          "paged_attention over a cache in 8 bits, after paged8_append of the same batch. softcap: x becomes softcap * tanh(x / softcap); slopes (one per "
+          "query head): x gets slope * (place of the token - place of the row); window: a row sees the last `window` tokens up to its own; prefix (one per "
+          "sequence): and the first `prefix` tokens, whatever its own place.",
+          py::arg("q"), py::arg("new_k"), py::arg("new_v"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("k_res"),
+          py::arg("v_res"), py::arg("page_table"), py::arg("slots"), py::arg("seq_lens"), py::arg("cu_new"), py::arg("max_new"), py::arg("max_len"), py::arg("out"),
+          py::arg("group_size"), py::arg("sm_scale") = 0.0, py::arg("softcap") = 0.0, py::arg("slopes") = py::none(), py::arg("window") = 0, py::arg("prefix") = py::none());
+    m.def("paged8_read", &paged8_read, py::call_guard<py::gil_scoped_release>(), "paged_read for a cache in 8 bits.",
+          py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("k_res"), py::arg("v_res"), py::arg("page_table"), py::arg("slots"),
+          py::arg("seq_lens"), py::arg("starts"), py::arg("cu_read"), py::arg("max_read"), py::arg("k_out"), py::arg("v_out"), py::arg("group_size"));
+    m.def("adjust_logits", &adjust_logits, py::call_guard<py::gil_scoped_release>(),
+          "Penalties for tokens [cu_tokens] that a row has had (the first prompt_lens of them were given, the others said), biases [cu_bias] and masks "
+          "(bits of allowed [masks, words], row allowed_rows of it or -1) on logits [batch, vocab]; returns out (new rows, or logits itself).",
+          py::arg("logits"), py::arg("out") = py::none(), py::arg("tokens") = py::none(), py::arg("cu_tokens") = py::none(), py::arg("prompt_lens") = py::none(),
+          py::arg("repetition") = py::none(), py::arg("frequency") = py::none(), py::arg("presence") = py::none(), py::arg("bias_ids") = py::none(),
+          py::arg("bias") = py::none(), py::arg("cu_bias") = py::none(), py::arg("allowed") = py::none(), py::arg("allowed_rows") = py::none());
     m.def("sample_filtered", &sample_filtered, py::call_guard<py::gil_scoped_release>(),
           "Next-token choice under temperature, top-k, top-p and min-p of each row (tensors of one entry per row, or None), from the given "
           "random numbers in [0, 1); returns the ids.",
