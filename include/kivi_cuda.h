@@ -534,8 +534,8 @@ int kivi_sample_filtered(const void* logits, int dtype, int batch, int vocab, in
  *            multiple of 32; u = t % N stands at i = (u >> 1 & 3)*N/4 + (u >> 4)*4 + (u >> 3 & 1)*2 + (u & 1)
  *   k_scales, v_scales [num_pages][num_kv_heads][page_tokens/G]
  *   k_res, v_res as in kivi_paged_layer
- * A block's scale is max(a / 448, 1e-30) in fp32, a its largest finite magnitude; x is held as the e4m3 number next
- * to x * (1 / scale) (ties to even), infinities as the largest one, NaN as 0: whatever is in pages is finite.
+ * A block's scale is max(a * fl(1 / 448), 1e-30) in fp32, a its largest finite magnitude; x is held as the e4m3 number
+ * next to x * fl(1 / scale) (ties to even), infinities as the largest one, NaN as 0: whatever is in pages is finite.
  * A code stands for its number times the scale, rounded to fp32.
  * ---------------------------------------------------------------------- */
 typedef struct kivi_paged8_layer {

@@ -345,13 +345,23 @@ int paged8_attention_fault_clear() {
     return KIVI_OK;
 }
 
+bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows);
+size_t paged8_decode_parts();
+int run_paged8_decode(const Paged8Attn& a, cudaStream_t st);
+
 // ---- the cut of a call -----------------------------------------------------------
 // Rows per block, blocks (at most: what the host knows are bounds) and pieces of the tiles that a block sees.
-struct Paged8Plan { int rows, blocks, pieces, chunk; };
+enum class Paged8Kernel { kDecode, kGeneral };
+struct Paged8Plan { Paged8Kernel kernel; int rows, blocks, pieces, chunk; };
 
-static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch* b, int n_rep, const kivi_score_rules& rules) {
-    Paged8Plan p;
+static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, const kivi_score_rules& rules) {
+    Paged8Plan p{};
     const int64_t rows = (int64_t)b->max_new * n_rep;
+    if (paged8_decode_serves(L, q_dtype, rows)) {
+        p.kernel = Paged8Kernel::kDecode;
+        return p;
+    }
+    p.kernel = Paged8Kernel::kGeneral;
     p.rows = rows <= 8 ? 8 : 64;
     const int64_t blocks = ((int64_t)b->total_new * n_rep) / p.rows + b->num_seqs;
     p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
@@ -385,12 +395,13 @@ static int check_attention8(const kivi_paged8_layer* L, const kivi_paged_batch* 
 }
 
 static size_t plan_bytes(const kivi_paged8_layer* L, const Paged8Plan& p) {
+    if (p.kernel == Paged8Kernel::kDecode) return paged8_decode_parts() * (L->head_dim + 2) * 4;
     return p.pieces > 1 ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
 }
 
 extern "C" size_t kivi_paged8_attention_workspace(const kivi_paged8_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, const kivi_score_rules* rules) {
     if (check_attention8(L, b, q_dtype, n_rep, rules) != KIVI_OK || b->max_new == 0) return 0;
-    return plan_bytes(L, plan_paged8(L, b, n_rep, rules ? *rules : kivi_score_rules{}));
+    return plan_bytes(L, plan_paged8(L, b, q_dtype, n_rep, rules ? *rules : kivi_score_rules{}));
 }
 
 extern "C" int kivi_paged8_attention(const kivi_paged8_layer* L, const kivi_paged_batch* b, const kivi_rows* q,
@@ -409,7 +420,7 @@ extern "C" int kivi_paged8_attention(const kivi_paged8_layer* L, const kivi_page
     const int D = L->head_dim;
     Paged8Attn a{};
     a.rules = rules ? *rules : kivi_score_rules{};
-    const Paged8Plan p = plan_paged8(L, b, n_rep, a.rules);
+    const Paged8Plan p = plan_paged8(L, b, q_dtype, n_rep, a.rules);
     const size_t need = plan_bytes(L, p);
     KIVI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small: %zu bytes given, %zu needed", workspace_bytes, need);
     KIVI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "workspace must be 16-byte aligned");
@@ -421,9 +432,14 @@ extern "C" int kivi_paged8_attention(const kivi_paged8_layer* L, const kivi_page
     a.scale = sm_scale > 0.0f ? sm_scale : 1.0f / sqrtf((float)D);
     a.pieces = p.pieces; a.chunk = p.chunk;
     a.part_o = reinterpret_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * D;
+    a.part_ml = a.part_o + (p.kernel == Paged8Kernel::kDecode ? paged8_decode_parts() : (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows) * D;
     a.vec = grid4(*q, q_dtype) && grid4(*new_k, L->res_dtype) && grid4(*new_v, L->res_dtype);
     cudaStream_t st = (cudaStream_t)stream;
+    if (p.kernel == Paged8Kernel::kDecode) {
+        if (int rc = run_paged8_decode(a, st)) return rc;
+        note_launches(2);
+        return KIVI_OK;
+    }
     int rc;
     if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, st) : run_general<1, 8, 256>(a, p.blocks, st);
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, st) : run_general<4, 16, 256>(a, p.blocks, st);

@@ -26,7 +26,7 @@ __host__ __device__ __forceinline__ int value8_place(int u, int run) {          
 }
 __host__ __device__ __forceinline__ int value8_offset(int t, int d, int D, int run) { return (t / run * D + d) * run + value8_place(t % run, run); }
 
-constexpr float kE4m3Largest = 448.0f, kLeastScale = 1e-30f;
+constexpr float kPerLargest = 1.0f / 448.0f, kLeastScale = 1e-30f;          // (448: the largest e4m3 number)
 
 #ifdef __CUDACC__
 

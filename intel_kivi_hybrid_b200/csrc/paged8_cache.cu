@@ -314,7 +314,7 @@ paged8_append_kernel(Append8Args A) {
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kThreads / 32; ++w) { k_top = fmaxf(k_top, top_s[0][w]); v_top = fmaxf(v_top, top_s[1][w]); }
-        const float k_scale = fmaxf(__fdiv_rn(k_top, kE4m3Largest), kLeastScale), v_scale = fmaxf(__fdiv_rn(v_top, kE4m3Largest), kLeastScale);
+        const float k_scale = fmaxf(__fmul_rn(k_top, kPerLargest), kLeastScale), v_scale = fmaxf(__fmul_rn(v_top, kPerLargest), kLeastScale);
         const float k_inv = __frcp_rn(k_scale), v_inv = __frcp_rn(v_scale);
 
         const int page = q.pages[t0 / L.page_tokens], in_page = t0 % L.page_tokens;
