@@ -348,10 +348,13 @@ int paged8_attention_fault_clear() {
 bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows);
 size_t paged8_decode_parts();
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st);
+bool paged8_tc_serves(const kivi_paged8_layer* L, int q_dtype);
+int run_paged8_tc(const Paged8Attn& a, int blocks, cudaStream_t st);
 
 // ---- the cut of a call -----------------------------------------------------------
 // Rows per block, blocks (at most: what the host knows are bounds) and pieces of the tiles that a block sees.
-enum class Paged8Kernel { kDecode, kGeneral };
+enum class Paged8Kernel { kDecode, kTensor, kGeneral };
+constexpr int kTensorRows = 256, kTensorTile = 128;      // of a CTA on the tensor cores
 struct Paged8Plan { Paged8Kernel kernel; int rows, blocks, pieces, chunk; };
 
 static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, const kivi_score_rules& rules) {
@@ -361,14 +364,35 @@ static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch
         p.kernel = Paged8Kernel::kDecode;
         return p;
     }
+    auto blocks_of = [&](int block_rows) {
+        const int64_t blocks = (int64_t)b->total_new * n_rep / block_rows + b->num_seqs;
+        return (int)(blocks < (1 << 30) ? blocks : (1 << 30));
+    };
+    // tiles of T tokens that a block sees (how long prefixes are the host does not know)
+    auto tiles_of = [&](int T, int block_rows) {
+        const int64_t all = ((int64_t)b->max_len + T - 1) / T, near = ((int64_t)rules.window + block_rows / n_rep + 1 + 2 * T) / T;
+        return rules.window > 0 && rules.prefix == nullptr && near < all ? near : all;
+    };
+    if (paged8_tc_serves(L, q_dtype)) {
+        p.kernel = Paged8Kernel::kTensor;
+        p.rows = kTensorRows;
+        p.blocks = blocks_of(p.rows);
+        // One CTA per SM: the fewest rounds of the shortest pieces, each with the start and
+        // end of a CTA on top (about four tiles).
+        const int tiles = (int)tiles_of(kTensorTile, p.rows), most = tiles < 64 ? tiles : 64;
+        const int64_t units = (int64_t)p.blocks * L->num_kv_heads;
+        int64_t best = INT64_MAX;
+        for (int n = 1; n <= most; ++n) {
+            const int per = (tiles + n - 1) / n;
+            const int64_t cost = ((units * n + num_sms() - 1) / num_sms()) * (per + 4);
+            if (cost < best) { best = cost; p.chunk = per; p.pieces = (tiles + per - 1) / per; }
+        }
+        return p;
+    }
     p.kernel = Paged8Kernel::kGeneral;
     p.rows = rows <= 8 ? 8 : 64;
-    const int64_t blocks = ((int64_t)b->total_new * n_rep) / p.rows + b->num_seqs;
-    p.blocks = (int)(blocks < (1 << 30) ? blocks : (1 << 30));
-    int64_t tiles = ((int64_t)b->max_len + kTile - 1) / kTile;
-    // (how long prefixes are the host does not know)
-    const int64_t near = ((int64_t)rules.window + p.rows / n_rep + 2 * kTile) / kTile + 1;
-    if (rules.window > 0 && rules.prefix == nullptr && near < tiles) tiles = near;
+    p.blocks = blocks_of(p.rows);
+    const int64_t tiles = tiles_of(kTile, p.rows);
     // as many pieces as give every SM four CTAs
     int64_t want = (4 * (int64_t)num_sms() + p.blocks * (int64_t)L->num_kv_heads - 1) / (p.blocks * (int64_t)L->num_kv_heads);
     if (want > tiles) want = tiles;
@@ -440,13 +464,18 @@ extern "C" int kivi_paged8_attention(const kivi_paged8_layer* L, const kivi_page
         note_launches(2);
         return KIVI_OK;
     }
-    int rc;
-    if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, st) : run_general<1, 8, 256>(a, p.blocks, st);
+    int rc, tile = kTile;
+    if (p.kernel == Paged8Kernel::kTensor) {
+        auto aligned = [](const kivi_rows& r) { return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.row_stride % 8 == 0 && r.head_stride % 8 == 0; };
+        a.vec = aligned(*q) && aligned(*new_k) && aligned(*new_v);
+        tile = kTensorTile;
+        rc = run_paged8_tc(a, p.blocks, st);
+    } else if (p.rows == 8) rc = D == 64 ? run_general<1, 8, 64>(a, p.blocks, st) : D == 128 ? run_general<1, 8, 128>(a, p.blocks, st) : run_general<1, 8, 256>(a, p.blocks, st);
     else rc = D == 64 ? run_general<4, 16, 64>(a, p.blocks, st) : D == 128 ? run_general<4, 16, 128>(a, p.blocks, st) : run_general<4, 16, 256>(a, p.blocks, st);
     if (rc) return rc;
     int launches = 1;
     if (p.pieces > 1) {
-        KIVI_CUDA_OK(launch(paged8_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)((p.rows + kFoldRows - 1) / kFoldRows)), 256, 0, st, true, a, p.rows, kTile));
+        KIVI_CUDA_OK(launch(paged8_merge_kernel, dim3((unsigned)p.blocks, (unsigned)L->num_kv_heads, (unsigned)((p.rows + kFoldRows - 1) / kFoldRows)), 256, 0, st, true, a, p.rows, tile));
         ++launches;
     }
     note_launches(launches);

@@ -82,6 +82,8 @@ int paged8_attention_fault_word(int* out);
 int paged8_attention_fault_clear();
 int paged8_decode_fault_word(int* out);
 int paged8_decode_fault_clear();
+int paged8_tc_fault_word(int* out);
+int paged8_tc_fault_clear();
 int logit_rules_fault_word(int* out);
 int logit_rules_fault_clear();
 int run_merge(const float* part_o, const float* part_ml, void* out, const kivi_peer_gather* gather, float* lse,
@@ -106,13 +108,14 @@ extern "C" int kivi_device_fault(int* word_out) {
     if (int rc = paged_attention_fault_word(&paged_attention)) return rc;
     if (int rc = paged_tc_fault_word(&paged_tc)) return rc;
     if (int rc = paged_decode_fault_word(&paged_decode)) return rc;
-    int paged8_cache = 0, paged8_attention = 0, paged8_decode = 0, logit_rules = 0;
+    int paged8_cache = 0, paged8_attention = 0, paged8_decode = 0, paged8_tc = 0, logit_rules = 0;
     if (int rc = paged8_cache_fault_word(&paged8_cache)) return rc;
     if (int rc = paged8_attention_fault_word(&paged8_attention)) return rc;
     if (int rc = paged8_decode_fault_word(&paged8_decode)) return rc;
+    if (int rc = paged8_tc_fault_word(&paged8_tc)) return rc;
     if (int rc = logit_rules_fault_word(&logit_rules)) return rc;
     *word_out = (copy_wait || copy_wait_fp32 || copy_wait_sample ? 1 : 0) | (peer_wait ? 2 : 0) | paged_cache | paged_attention | paged_tc | paged_decode |
-                paged8_cache | paged8_attention | paged8_decode | logit_rules;
+                paged8_cache | paged8_attention | paged8_decode | paged8_tc | logit_rules;
     return KIVI_OK;
 }
 
@@ -127,6 +130,7 @@ extern "C" int kivi_device_fault_clear(void) {
     if (int rc = paged8_cache_fault_clear()) return rc;
     if (int rc = paged8_attention_fault_clear()) return rc;
     if (int rc = paged8_decode_fault_clear()) return rc;
+    if (int rc = paged8_tc_fault_clear()) return rc;
     if (int rc = logit_rules_fault_clear()) return rc;
     return gather_fault_clear();
 }
