@@ -346,7 +346,7 @@ int paged8_attention_fault_clear() {
 }
 
 bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows);
-size_t paged8_decode_parts();
+size_t paged8_decode_parts(int64_t max_rows);
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st);
 bool paged8_tc_serves(const kivi_paged8_layer* L, int q_dtype);
 int run_paged8_tc(const Paged8Attn& a, int blocks, cudaStream_t st);
@@ -362,6 +362,9 @@ static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch
     const int64_t rows = (int64_t)b->max_new * n_rep;
     if (paged8_decode_serves(L, q_dtype, rows)) {
         p.kernel = Paged8Kernel::kDecode;
+        p.rows = 1;
+        p.blocks = (int)paged8_decode_parts(rows);
+        p.pieces = 1;
         return p;
     }
     auto blocks_of = [&](int block_rows) {
@@ -419,7 +422,7 @@ static int check_attention8(const kivi_paged8_layer* L, const kivi_paged_batch* 
 }
 
 static size_t plan_bytes(const kivi_paged8_layer* L, const Paged8Plan& p) {
-    if (p.kernel == Paged8Kernel::kDecode) return paged8_decode_parts() * (L->head_dim + 2) * 4;
+    if (p.kernel == Paged8Kernel::kDecode) return (size_t)p.blocks * (L->head_dim + 2) * 4;
     return p.pieces > 1 ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
 }
 
@@ -456,7 +459,7 @@ extern "C" int kivi_paged8_attention(const kivi_paged8_layer* L, const kivi_page
     a.scale = sm_scale > 0.0f ? sm_scale : 1.0f / sqrtf((float)D);
     a.pieces = p.pieces; a.chunk = p.chunk;
     a.part_o = reinterpret_cast<float*>(workspace);
-    a.part_ml = a.part_o + (p.kernel == Paged8Kernel::kDecode ? paged8_decode_parts() : (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows) * D;
+    a.part_ml = a.part_o + (p.kernel == Paged8Kernel::kDecode ? (size_t)p.blocks : (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows) * D;
     a.vec = grid4(*q, q_dtype) && grid4(*new_k, L->res_dtype) && grid4(*new_v, L->res_dtype);
     cudaStream_t st = (cudaStream_t)stream;
     if (p.kernel == Paged8Kernel::kDecode) {

@@ -3,10 +3,12 @@
 //
 //   S = Q K^T,  P = 2^(rules(S) - m),  O = O + P V,  out = O / sum P
 //
-// by mma.sync m16n8k16 for sixteen rows ((new token, query head) pairs of one sequence and
-// KV head), 32 tokens of a page to a warp at a time.  What bounds it is the page's bytes:
-// a 32-token tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions
-// and 64 MMAs of a warp (twice the MMAs for fp32 rows), a quarter of the time its bytes take.
+// by mma.sync m16n8k16, 32 tokens of a page to a warp at a time.  Tokens (and channels of V)
+// are the sixteen rows of an MMA, the (new token, query head) pairs of one sequence and KV head
+// its eight columns, up to three times eight to a unit: with the pairs as rows a single token of four heads took twice
+// the MMAs and the registers (64 ragged sequences up to 32k 555 us).  Weights change places with movmatrix in between.
+// What bounds it is the page's bytes: a tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions
+// and 32 MMAs of a warp (fp32 rows: 64).
 //
 // Work is dealt out evenly whatever the sequences' lengths: the tiles of all (sequence, KV
 // head, block of rows) units lie one after the other, the window and the step's own tokens
@@ -22,24 +24,22 @@
 // of two, but for what is below 2^-27 of its largest; fp32 rows are two fp16 numbers (22 bits).  A block's key scale
 // multiplies the scores, its value scale the weights, which are fp16 (bf16 rows: rounded at
 // 2^-12 of themselves, where the output is rounded at 2^-9) or two of them, less the power of
-// two of the largest value scale so far.  Window and own tokens are contracted as bf16 numbers, exact for
+// two of the largest such product that the row has met.  Window and own tokens are contracted as bf16 numbers, exact for
 // bf16 rows (weights at 2^-9 there: bf16 reaches as far as the values do); fp32 ones as three, the six products that matter.  Sums are fp32.
 #include "async_copy.cuh"
 #include "paged8_attention.cuh"
-
-#include <type_traits>
 
 namespace kivi {
 namespace {
 
 __device__ int g_fault = 0;
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kStages = 2;
-constexpr int kRows = 16, kTile = 32;                    // rows of a unit, tokens of a tile
+constexpr int kStages = 2;
+constexpr int kTile = 32;                                // tokens of a tile
 constexpr int kPerSm = 2;                                // CTAs
 constexpr int kLeast = 8;                                // tiles of a CTA
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
-constexpr int kHeadroom = 5;                             // value scales are brought to 2^5 .. 2^6: weights stay below 2^14
+constexpr float kHeadroom = 8.0f, kSlack = 6.0f;         // products of weight and scale: up to 2^8, or 2^14 before their reference moves
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -64,17 +64,17 @@ __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
     return y;
 }
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// what is left of two numbers after their first term
-__device__ __forceinline__ uint32_t half2_rest(float lo, float hi, uint32_t first) { return half2_of(lo - half_lo(first), hi - half_hi(first)); }
-// two numbers as N bf16 terms
-template <int N> __device__ __forceinline__ void bf16_terms(float lo, float hi, uint32_t (&w)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        w[i] = bf16x2_of(lo, hi);
-        lo -= bf_lo(w[i]); hi -= bf_hi(w[i]);
-    }
+// four neighbouring numbers as they lie
+__device__ __forceinline__ uint2 quad_of(const __nv_bfloat16* p, bool vec) {
+    if (vec) return *reinterpret_cast<const uint2*>(p);
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+    return make_uint2(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16);
+}
+// bf16 numbers that are not finite become 0
+__device__ __forceinline__ uint32_t finite_pair(uint32_t w, bool& odd) {
+    if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; odd = true; }
+    if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; odd = true; }
+    return w;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
     uint4 v;
@@ -89,43 +89,49 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
 __device__ __forceinline__ void ldmatrix_trans(uint32_t at, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
+// an 8 x 8 matrix of 16-bit numbers, a row to four lanes, with rows and columns in each other's place
+__device__ __forceinline__ uint32_t turned(uint32_t w) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(w));
+    return y;
+}
 __device__ __forceinline__ float pow2i(int s) { return __uint_as_float((uint32_t)(127 + max(-126, min(127, s))) << 23); }
 
 // ---- the line of work ---------------------------------------------------------------
 struct SeqWork {
     PagedSeq q;
-    int total, inside, prefix, rows, blocks;             // rows of the step, blocks of kRows of them
+    int total, inside, prefix, rows, blocks;             // rows of the step, units' blocks of them
     int tiles, tail;                                     // of a unit: packed tiles, and positions that the other tokens count for
     Span span;
     __device__ __forceinline__ int cost() const { return tiles + tail; }
 };
-template <bool F32>
-__device__ __forceinline__ bool seq_work(const Paged8Attn& A, int s, SeqWork& w) {
+__device__ __forceinline__ bool seq_work(const Paged8Attn& A, int unit_rows, int s, SeqWork& w) {
     const kivi_paged8_layer& L = A.L;
     if (!load_seq(L, A.b, s, w.q) || w.q.n == 0) { w.blocks = w.tiles = w.tail = 0; return false; }
     w.rows = w.q.n * A.n_rep;
-    w.blocks = (w.rows + kRows - 1) / kRows;
+    w.blocks = (w.rows + unit_rows - 1) / unit_rows;
     w.total = w.q.held + w.q.n;
     w.inside = min(quant_of(w.total, L.group_size, L.residual_cap), w.q.held);
     w.prefix = prefix_of(A.rules, s, w.total);
     w.span = span_of(kTile, w.total, w.q.held, w.total - 1, A.rules.window, w.prefix);
     const int packed = (w.inside + kTile - 1) / kTile;
     w.tiles = min(w.span.n1, packed) + max(0, packed - (w.span.n1 + w.span.gap));
-    w.tail = 1 + (w.total - w.inside) * (F32 ? 4 : 2) / kTile;
+    w.tail = 1 + (w.total - w.inside) * elem_size(L.res_dtype) / kTile;
     return true;
 }
 
 struct Line { int64_t cost; int64_t before; int first; };         // all positions; those before sequence `first`, which has position `at`
 
 // Called by the whole CTA: the line's length, and which sequence has position at(length).
-template <bool F32, typename At>
-__device__ __forceinline__ Line find_line(const Paged8Attn& A, int64_t* scratch /* [kWarps + 2] shared */, const At& at) {
+template <int kWarps, typename At>
+__device__ __forceinline__ Line find_line(const Paged8Attn& A, int unit_rows, int64_t* scratch /* [kWarps + 2] shared */, const At& at) {
+    constexpr int kThreads = 32 * kWarps;
     const int n = A.b.num_seqs, H = A.L.num_kv_heads, per = (n + kThreads - 1) / kThreads;
     int64_t mine = 0;
     for (int i = 0; i < per; ++i) {
         const int s = threadIdx.x * per + i;
         SeqWork w;
-        if (s < n && seq_work<F32>(A, s, w)) mine += (int64_t)H * w.blocks * w.cost();
+        if (s < n && seq_work(A, unit_rows, s, w)) mine += (int64_t)H * w.blocks * w.cost();
     }
     // sums of what comes before each thread's sequences
     int64_t sum = mine;
@@ -148,7 +154,7 @@ __device__ __forceinline__ Line find_line(const Paged8Attn& A, int64_t* scratch 
         for (int i = 0; i < per; ++i) {
             const int s = threadIdx.x * per + i;
             SeqWork w;
-            const int64_t c = s < n && seq_work<F32>(A, s, w) ? (int64_t)H * w.blocks * w.cost() : 0;
+            const int64_t c = s < n && seq_work(A, unit_rows, s, w) ? (int64_t)H * w.blocks * w.cost() : 0;
             if (want < before + c) { scratch[kWarps] = s; scratch[kWarps + 1] = before; break; }
             before += c;
         }
@@ -161,8 +167,7 @@ __host__ __device__ __forceinline__ int64_t per_cta(int64_t cost, int ctas) {
     return per < kLeast ? kLeast : per;
 }
 
-// The CTA's segments, one after the other.
-template <bool F32>
+// The CTA's segments, one after the other.  (In shared memory: as registers two of them were 60 of a thread's.)
 struct Walk {
     SeqWork w;
     int64_t at, end, off;                                // next position, the CTA's end, the sequence's first position
@@ -170,13 +175,13 @@ struct Walk {
     int64_t unit;                                        // its unit's first position
     int a, b;                                            // its positions within the unit
 
-    __device__ __forceinline__ bool next(const Paged8Attn& A) {
+    __device__ __forceinline__ bool next(const Paged8Attn& A, int unit_rows) {
         while (at < end) {
             const int64_t size = (int64_t)A.L.num_kv_heads * w.blocks * w.cost();
             if (at >= off + size) {
                 off += size;
                 if (++s >= A.b.num_seqs) return false;
-                seq_work<F32>(A, s, w);
+                seq_work(A, unit_rows, s, w);
                 continue;
             }
             const int c = w.cost();
@@ -194,392 +199,435 @@ struct Walk {
     __device__ __forceinline__ bool has_tail() const { return a <= w.tiles && w.tiles < b; }
 };
 
-template <int D> struct Layout {
+// Warps of a CTA, two CTAs to an SM: what registers and shared memory hold (64 ragged sequences up to 32k with
+// four: 488 us).
+constexpr int warps_of(int nb) { return nb == 1 ? 6 : 4; }
+template <int D, int NB> struct Layout {
+    static constexpr int kRows = 8 * NB, kWarps = warps_of(NB), kHalf = kWarps / 2;
     static constexpr int kPart = kTile * D;              // bytes of a tile's keys, or values
-    static constexpr int kQ = D + 4, kO = D + 8;         // floats of a row
-    static constexpr int kVStage = 16 * D * 2;           // bytes: values of sixteen tokens as bf16
+    static constexpr int kQ = D + 8, kO = D + 4;         // bf16 numbers, floats of a row
+    static constexpr int kVStage = 8 * D * 2;            // bytes: values of eight tokens as bf16
     static constexpr int ring = 0, fold = ring + kWarps * kStages * 2 * kPart;
-    static constexpr int kFold = 2 * kRows * kO * 4 > kWarps * kVStage ? 2 * kRows * kO * 4 : kWarps * kVStage;
-    static constexpr int q = fold + kFold, ml = q + kRows * kQ * 4, scratch = ml + 2 * kRows * 8, bars = scratch + (kWarps + 2) * 8;
-    static constexpr int bytes = bars + kWarps * kStages * 8;
+    static constexpr int kFold = kHalf * kRows * kO * 4 > kWarps * kVStage ? kHalf * kRows * kO * 4 : kWarps * kVStage;
+    static constexpr int q = fold + kFold, ml = q + kRows * kQ * 2, scratch = ml + kHalf * kRows * 8, walks = scratch + (kWarps + 2) * 8;
+    static constexpr int bars = walks + (kWarps + 1) * (int)sizeof(Walk);
+    static constexpr int bytes = bars + kWarps * kStages * 16;
 };
 
-template <int D, bool F32, bool RULES>
-__global__ void __launch_bounds__(kThreads, kPerSm)
+template <int D, int NB, bool RULES>
+__global__ void __launch_bounds__(32 * warps_of(NB), kPerSm)
 paged8_decode_kernel(Paged8Attn A) {
-    using S = Layout<D>;
-    constexpr int kSteps = D / 16, kChan = D / 4;        // MMAs along the channels; channels of a lane's keys
-    constexpr int kTerms = F32 ? 2 : 1, kBf = F32 ? 3 : 1;
+    using S = Layout<D, NB>;
+    constexpr int kWarps = S::kWarps, kThreads = 32 * kWarps, kRows = S::kRows, kSteps = D / 16, kChan = D / 4;        // MMAs along the channels; channels of a lane's keys
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t = lane & 3;
     stream_order();
     settle_args(A);
     cudaTriggerProgrammaticLaunchCompletion();           // (the fold's few blocks wait for this kernel's end)
     const kivi_paged8_layer& L = A.L;
-    const int G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, n_rep = A.n_rep, window = A.rules.window;
+    const int R = L.residual_cap, H = L.num_kv_heads, n_rep = A.n_rep, window = A.rules.window;
     if (blockIdx.x == 0) report_left_out(L, A.b, &g_fault);
-    float* const q_s = reinterpret_cast<float*>(smem + S::q);
+    __nv_bfloat16* const q_s = reinterpret_cast<__nv_bfloat16*>(smem + S::q);
     float* const fold_s = reinterpret_cast<float*>(smem + S::fold);
     float* const ml_s = reinterpret_cast<float*>(smem + S::ml);
     const uint32_t ring = smem_u32(smem + S::ring) + warp * (kStages * 2 * S::kPart), v_stage = smem_u32(smem + S::fold) + warp * S::kVStage;
-    const uint32_t bars = smem_u32(smem + S::bars) + warp * (kStages * 8);
+    const uint32_t bars = smem_u32(smem + S::bars) + warp * (kStages * 16);          // of a stage: keys, values
     if (lane == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+        for (int i = 0; i < 2 * kStages; ++i) mbar_init(bars + 8 * i, 1);
         mbar_init_fence();
     }
-    const Line line = find_line<F32>(A, reinterpret_cast<int64_t*>(smem + S::scratch), [&](int64_t cost) { return per_cta(cost, gridDim.x) * blockIdx.x; });
+    const Line line = find_line<kWarps>(A, kRows, reinterpret_cast<int64_t*>(smem + S::scratch), [&](int64_t cost) { return per_cta(cost, gridDim.x) * blockIdx.x; });
     if (line.first < 0) return;
     const int64_t per = per_cta(line.cost, gridDim.x);
-    Walk<F32> walk, ahead;                               // what is computed, and what is copied
-    walk.s = line.first; walk.off = line.before;
-    walk.at = per * blockIdx.x; walk.end = min(walk.at + per, line.cost);
-    seq_work<F32>(A, walk.s, walk.w);
-    ahead = walk;
+    Walk& walk = *reinterpret_cast<Walk*>(smem + S::walks);                 // what is computed
+    Walk& ahead = (&walk)[1 + warp];                                         // what the warp copies: its first lane's
+    auto start = [&](Walk& w) {
+        w.s = line.first; w.off = line.before;
+        w.at = per * blockIdx.x; w.end = min(w.at + per, line.cost);
+        seq_work(A, kRows, w.s, w.w);
+    };
+    if (tid == 0) start(walk);
     const uint64_t policy = l2_stream_policy();
 
-    // ---- copies: the warp's next tile into a stage; its scales come along in registers
-    bool more = ahead.next(A);
-    int av = more ? ahead.a + warp : 0, issued = 0;
+    // ---- copies, all of them the first lane's: the warp's next tile into a stage
+    const int per_page = L.page_tokens / kTile, per_block = L.group_size / kTile;            // tiles
+    const uint32_t block_of = (1u << 20) / per_block + 1;                                    // tile of a page / per_block, for up to 2^15 tiles
+    int av = 0, a_end = 0, n1 = 0, a_head = 0, page = 0, in_page = 0, next_page = 0, issued = 0;         // the tile; its place among the sequence's pages
+    const int32_t* a_pages = nullptr;
+    bool more = true;
     float2 scales[kStages];
+    int64_t v_from[kStages];
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) scales[i] = make_float2(0.f, 0.f);
+    for (int i = 0; i < kStages; ++i) { scales[i] = make_float2(0.f, 0.f); v_from[i] = -1; }
     auto settle_next = [&] {                             // on to the warp's next tile
-        while (more && av >= ahead.tiles_end()) {
-            more = ahead.next(A);
-            if (more) av = ahead.a + warp;
+        if (av < a_end && !(av >= n1 && av - kWarps < n1)) {
+            in_page += kWarps;
+            while (in_page >= per_page) { in_page -= per_page; ++page; }
+        } else {
+            while (av >= a_end) {
+                more = ahead.next(A, kRows);
+                if (!more) return;
+                av = ahead.a + warp;
+                a_end = ahead.tiles_end();
+                n1 = ahead.w.span.n1; a_head = ahead.h; a_pages = ahead.w.q.pages;
+            }
+            const int tile = ahead.w.span.tile(av);
+            page = tile / per_page;
+            in_page = tile - page * per_page;
         }
+        next_page = a_pages[page];
     };
-    settle_next();
-    int next_page = 0;
-    auto look_up = [&] { if (more) next_page = ahead.w.q.pages[ahead.w.span.tile(av) * kTile / L.page_tokens]; };
-    look_up();
-    auto issue = [&](int stage, float2& sc) {
+    // Keys of the next tile, when the ones before them have been contracted; its values follow when theirs have.
+    auto issue_keys = [&](int stage, float2& sc, int64_t& values) {
+        values = -1;
         if (!more) return;
-        const int t0 = ahead.w.span.tile(av) * kTile, in_page = t0 % L.page_tokens;
         const bool there = (unsigned)next_page < (unsigned)L.num_pages;
         if (!there) atomicOr(&g_fault, kPagedFault);
-        const int64_t unit = (int64_t)(there ? next_page : 0) * H + ahead.h;
-        const int64_t at = (unit * L.page_tokens + in_page) * D, f = unit * (L.page_tokens / G) + in_page / G;
-        if (lane == 0) {
-            const uint32_t to = ring + stage * (2 * S::kPart), b = bars + 8 * stage;
-            mbar_expect_tx(b, 2 * S::kPart);
-            bulk_g2s(to, L.k_codes + at, S::kPart, b, policy);
-            bulk_g2s(to + S::kPart, L.v_codes + at, S::kPart, b, policy);
-        }
+        const int64_t unit = (there ? next_page : 0) * (int64_t)H + a_head;
+        const int64_t f = unit * (uint32_t)(L.page_tokens / L.group_size) + (uint32_t)(((uint64_t)(uint32_t)in_page * block_of) >> 20);
+        values = (unit * per_page + in_page) * S::kPart;
+        mbar_expect_tx(bars + 16 * stage, S::kPart);
+        bulk_g2s(ring + stage * (2 * S::kPart), L.k_codes + values, S::kPart, bars + 16 * stage, policy);
         sc = make_float2(L.k_scales[f], L.v_scales[f]);
         ++issued;
         av += kWarps;
         settle_next();
-        look_up();
     };
+    auto issue_values = [&](int stage, int64_t from) {
+        if (from < 0) return;
+        mbar_expect_tx(bars + 16 * stage + 8, S::kPart);
+        bulk_g2s(ring + stage * (2 * S::kPart) + S::kPart, L.v_codes + from, S::kPart, bars + 16 * stage + 8, policy);
+    };
+    if (lane == 0) {
+        start(ahead);
+        settle_next();
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) issue(i, scales[i]);
+        for (int i = 0; i < kStages; ++i) { issue_keys(i, scales[i], v_from[i]); issue_values(i, v_from[i]); }
+    }
     int taken = 0;
     bool ok = true;
 
-    while (walk.next(A)) {
+    for (;;) {
+        __syncthreads();                                 // (the unit before is folded)
+        if (tid == 0 && !walk.next(A, kRows)) walk.h = -1;
+        __syncthreads();
+        if (walk.h < 0) break;
         const PagedSeq& q = walk.w.q;
         const int h = walk.h, row_first = walk.rb * kRows, n_rows = min(kRows, walk.w.rows - row_first), inside = walk.w.inside, prefix = walk.w.prefix;
         // ---- the unit's queries
-        __syncthreads();                                 // (the unit before is folded)
         for (int i = tid; i < kRows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row_first + r;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < n_rows) x = load4_as(A.q, F32 ? KIVI_F32 : KIVI_BF16, (int64_t)q.row0 + row / n_rep, h * n_rep + row % n_rep, d, A.vec != 0);
-            *reinterpret_cast<float4*>(q_s + r * S::kQ + d) = x;
+            uint2 x = make_uint2(0u, 0u);
+            if (r < n_rows) x = quad_of(reinterpret_cast<const __nv_bfloat16*>(A.q.data) + ((int64_t)q.row0 + row / n_rep) * A.q.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.q.head_stride + d, A.vec != 0);
+            *reinterpret_cast<uint2*>(q_s + r * S::kQ + d) = x;
         }
         __syncthreads();
-        // A lane has channels kChan t .. of rows g and g + 8, four to an MMA; keys lie the same way.
-        uint32_t qa[kTerms][kSteps][4];
-        float unscale[2];                                // of a contracted score, and to powers of two where nothing else is done to it
-        {
-            int shift[2];
+        // As an operand a lane has channels kChan t .. of row 8 b + g, four to an MMA; keys lie the same way.
+        uint32_t qb[NB][kSteps][2];
+        float unscale[NB][2];                            // of a contracted score of rows 8 b + 2 t and the next, and to powers of two where nothing else is done to it
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                float top = 0.0f;
-                for (int c = 0; c < kChan; c += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(q_s + (g + 8 * hf) * S::kQ + kChan * t + c);
-                    top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = (int)(__float_as_uint(top) >> 23);
-                shift[hf] = e == 0 || e == 255 ? 0 : max(-110, min(110, 127 + 13 - e));       // largest to 2^13 .. 2^14
-                unscale[hf] = A.scale * pow2i(-shift[hf]) * (RULES ? 1.0f : 1.4426950408889634f);
+        for (int b = 0; b < NB; ++b) {
+            float top = 0.0f;
+            for (int c = 0; c < kChan; c += 4) {
+                const float4 x = load4(q_s + (8 * b + g) * S::kQ + kChan * t + c, true);
+                const float y[4] = {fabsf(x.x), fabsf(x.y), fabsf(x.z), fabsf(x.w)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, y[i] <= 3.4e38f ? y[i] : 0.0f);         // (the largest finite one)
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = (int)(__float_as_uint(top) >> 23), shift = e == 0 ? 0 : max(-110, min(110, 127 + 13 - e));       // largest to 2^13 .. 2^14
+            const float f = pow2i(shift);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                float4 x = load4(q_s + (8 * b + g) * S::kQ + kChan * t + 4 * i, true);
+                x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+                qb[b][i][0] = half2_of(x.x, x.y);
+                qb[b][i][1] = half2_of(x.z, x.w);
             }
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float f = pow2i(shift[hf]);
-                    float4 x = *reinterpret_cast<const float4*>(q_s + (g + 8 * hf) * S::kQ + kChan * t + 4 * i);
-                    x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-                    qa[0][i][hf] = half2_of(x.x, x.y);
-                    qa[0][i][2 + hf] = half2_of(x.z, x.w);
-                    if constexpr (F32) {
-                        qa[kTerms - 1][i][hf] = half2_rest(x.x, x.y, qa[0][i][hf]);
-                        qa[kTerms - 1][i][2 + hf] = half2_rest(x.z, x.w, qa[0][i][2 + hf]);
-                    }
-                }
+            for (int e2 = 0; e2 < 2; ++e2)
+                unscale[b][e2] = A.scale * pow2i(-__shfl_sync(0xffffffffu, shift, 4 * (2 * t + e2))) * (RULES ? 1.0f : 1.4426950408889634f);
         }
-        int place[2], from[2];
-        float slope[2];
+        int place[NB][2], from[NB][2];
+        float slope[NB][2];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            const int r = g + 8 * hf, row = row_first + r;
-            // (a row that is not there sees what the first one sees, and is not written)
-            place[hf] = q.held + (r < n_rows ? row : row_first) / n_rep;
-            from[hf] = window_from(place[hf], window);
-            slope[hf] = RULES && A.rules.slopes && r < n_rows ? A.rules.slopes[h * n_rep + row % n_rep] : 0.0f;
-        }
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * b + 2 * t + e, row = row_first + r;
+                // (a row that is not there sees what the first one sees, and is not written)
+                place[b][e] = q.held + (r < n_rows ? row : row_first) / n_rep;
+                from[b][e] = window_from(place[b][e], window);
+                slope[b][e] = RULES && A.rules.slopes && r < n_rows ? A.rules.slopes[h * n_rep + row % n_rep] : 0.0f;
+            }
         const int from_most = window_from(q.held + (row_first + n_rows - 1) / n_rep, window);
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[D / 8][4];
-        int v_exp = -1000;                               // O is 2^(kHeadroom - v_exp) times what it stands for
+        // o[c][b]: channels 16 c + g and + 8 of rows 8 b + 2 t and the next
+        float m[NB][2], l[NB][2], ref[NB][2], o[D / 16][NB][4];           // ref: the largest score plus value scale so far; O is 2^(kHeadroom - ref) times what it stands for
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[c][e] = 0.0f;
-        auto rescale = [&](float f0, float f1) {
+            for (int e = 0; e < 2; ++e) { m[b][e] = -INFINITY; l[b][e] = 0.0f; ref[b][e] = -1.0e30f; }
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) { o[c][0] *= f0; o[c][1] *= f0; o[c][2] *= f1; o[c][3] *= f1; }
+        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][b][e] = 0.0f;
+        auto rescale = [&](int b, float f0, float f1) {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) { o[c][b][0] *= f0; o[c][b][1] *= f1; o[c][b][2] *= f0; o[c][b][3] *= f1; }
         };
-        auto reach = [&](int e) {                        // value scales up to 2^(e + 1)
-            if (e > v_exp) {
-                if (v_exp != -1000) { const float f = pow2i(v_exp - e); rescale(f, f); }
-                v_exp = e;
-            }
-        };
-        // Scores x[n] (tokens t0 + 8 n + 2 t and the next, rows g and g + 8), in powers of two or (RULES) as contracted
-        // and scaled, to weights.  hidden(token, hf): the row does not see it.
-        auto weights = [&](auto& x, int t0, bool some_hidden, auto&& hidden) {
+        // Scores x[n][b] (tokens t0 + 16 n + g and + 8, rows 8 b + 2 t and the next) to weights; u: what makes powers of two
+        // of them (RULES: scores).  hidden(token, b, e): the row does not see it.  lift: their value scale's power of two, rounded
+        // up.  up: what weights times the value scale are multiplied with to be on O's scale.
+        auto weights = [&](auto& x, const float (&u)[NB][2], int t0, bool some_hidden, auto&& hidden, float lift, float (&up)[NB][2]) {
             constexpr int N = sizeof(x) / sizeof(x[0]);
-            if constexpr (RULES) {
-                const bool capped = A.rules.softcap > 0.0f;
-                const float cap = A.rules.softcap, inv_cap = capped ? 2.0f * 1.4426950408889634f / cap : 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if constexpr (RULES) {
+                    const bool capped = A.rules.softcap > 0.0f;
+                    const float cap = A.rules.softcap, inv_cap = capped ? 2.0f * 1.4426950408889634f / cap : 0.0f;
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float y = x[n][b][e] * u[b][e & 1];
+                            // tanh(z) = 1 - 2 / (1 + e^(2z))
+                            if (capped) y = cap - __fdividef(2.0f * cap, 1.0f + ex2(y * inv_cap > 120.0f ? 120.0f : y * inv_cap));
+                            y = fmaf(slope[b][e & 1], (float)(t0 + 16 * n + g + 8 * (e >> 1) - place[b][e & 1]), y);
+                            x[n][b][e] = y * 1.4426950408889634f;
+                        }
+                }
+                if (some_hidden) {
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (hidden(t0 + 16 * n + g + 8 * (e >> 1), b, e & 1)) x[n][b][e] = -INFINITY;
+                }
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    top[0] = fmaxf(top[0], fmaxf(x[n][b][0], x[n][b][2]));
+                    top[1] = fmaxf(top[1], fmaxf(x[n][b][1], x[n][b][3]));
+                }
+                float base[2], by[2];
+                bool grows = false;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+                    top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+                    by[e] = RULES ? 1.0f : u[b][e];
+                    top[e] *= by[e];
+                    if (top[e] > m[b][e] + kGrowth) {    // (from -inf: whenever there is a maximum)
+                        l[b][e] *= m[b][e] == -INFINITY ? 0.0f : ex2(m[b][e] - top[e]);
+                        m[b][e] = top[e];
+                    }
+                    base[e] = m[b][e] == -INFINITY ? 0.0f : m[b][e];
+                    top[e] += lift;
+                    grows |= top[e] > ref[b][e] + kSlack;
+                }
+                if (__any_sync(0xffffffffu, grows)) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool grow = top[e] > ref[b][e];
+                        f[e] = grow ? ex2(ref[b][e] - top[e]) : 1.0f;
+                        if (grow) ref[b][e] = top[e];
+                    }
+                    rescale(b, f[0], f[1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) up[b][e] = ex2(fminf(base[e] - ref[b][e] + kHeadroom, 126.0f));
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float y = x[n][e];
-                        // tanh(z) = 1 - 2 / (1 + e^(2z))
-                        if (capped) y = F32 ? cap * tanhf(y / cap) : cap - __fdividef(2.0f * cap, 1.0f + ex2(y * inv_cap > 120.0f ? 120.0f : y * inv_cap));
-                        y = fmaf(slope[e >> 1], (float)(t0 + 8 * n + 2 * t + (e & 1) - place[e >> 1]), y);
-                        x[n][e] = y * 1.4426950408889634f;
+                        x[n][b][e] = ex2(fmaf(x[n][b][e], by[e & 1], -base[e & 1]));
+                        l[b][e & 1] += x[n][b][e];
                     }
             }
-            if (some_hidden) {
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (hidden(t0 + 8 * n + 2 * t + (e & 1), e >> 1)) x[n][e] = -INFINITY;
-            }
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                top[0] = fmaxf(top[0], fmaxf(x[n][0], x[n][1]));
-                top[1] = fmaxf(top[1], fmaxf(x[n][2], x[n][3]));
-            }
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
-                top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
-            }
-            if (__any_sync(0xffffffffu, top[0] > m[0] + kGrowth || top[1] > m[1] + kGrowth)) {
-                float f[2];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const float m_new = fmaxf(m[hf], top[hf]);
-                    f[hf] = m[hf] == -INFINITY ? 0.0f : ex2(m[hf] - m_new);
-                    m[hf] = m_new;
-                    l[hf] *= f[hf];
-                }
-                rescale(f[0], f[1]);
-            }
-            const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-#pragma unroll
-            for (int n = 0; n < N; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[n][e] = F32 ? exp2f(x[n][e] - base[e >> 1]) : ex2(x[n][e] - base[e >> 1]);
-#pragma unroll
-            for (int n = 0; n < N; ++n) { l[0] += x[n][0] + x[n][1]; l[1] += x[n][2] + x[n][3]; }
         };
 
         // ---- tiles of pages
-        for (int v = walk.a + warp; v < walk.tiles_end(); v += kWarps) {
-            const int stage = taken % kStages, t0 = walk.w.span.tile(v) * kTile;
-            const float2 sc = stage ? scales[kStages - 1] : scales[0];
+        const Span span = walk.w.span;
+        const int v_end = walk.tiles_end();
+        for (int v = walk.a + warp; v < v_end; v += kWarps) {
+            const int stage = taken % kStages, t0 = span.tile(v) * kTile;
+            float2 sc = stage ? scales[kStages - 1] : scales[0];
+            sc.x = __shfl_sync(0xffffffffu, sc.x, 0); sc.y = __shfl_sync(0xffffffffu, sc.y, 0);
             static_assert(kStages == 2, "scales of a stage are picked by hand");
-            if (ok && !mbar_wait(bars + 8 * stage, (uint32_t)(taken / kStages) & 1u)) { atomicOr(&g_fault, 1); ok = false; }
+            const uint32_t phase = (uint32_t)(taken / kStages) & 1u;
+            if (ok && !mbar_wait(bars + 16 * stage, phase)) { atomicOr(&g_fault, 1); ok = false; }
             ok = __all_sync(0xffffffffu, ok);
             const uint32_t keys = ring + stage * (2 * S::kPart), values = keys + S::kPart;
-            float x[4][4];
+            float x[2][NB][4], x2[2][NB][4];             // (two sums each: an MMA waits for the one before it)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int p = 0; p < kChan / 16; ++p) {
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][b][e] = x2[n][b][e] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < kChan / 16; ++p)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
                     const int piece = D == 128 ? (2 * t + p) ^ g : t ^ (g >> 1 & 3);
-                    const uint4 k = lds128(keys + (8 * n + g) * D + 16 * piece);
-                    const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+                    const uint4 k0 = lds128(keys + (16 * n + g) * D + 16 * piece), k1 = lds128(keys + (16 * n + 8 + g) * D + 16 * piece);
+                    const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t b0 = e4m3x2_to_half2(w[i] & 0xffffu), b1 = e4m3x2_to_half2(w[i] >> 16);
+                        uint32_t a[4];
+                        e4m3x4_to_half2(w0[i], a[0], a[2]);
+                        e4m3x4_to_half2(w1[i], a[1], a[3]);
 #pragma unroll
-                        for (int term = kTerms - 1; term >= 0; --term) mma_f16(x[n], qa[term][4 * p + i], b0, b1);
+                        for (int b = 0; b < NB; ++b)
+                            mma_f16(i & 1 ? x2[n][b] : x[n][b], a, qb[b][4 * p + i][0], qb[b][4 * p + i][1]);
                     }
                 }
-            }
-            const float u0 = unscale[0] * sc.x, u1 = unscale[1] * sc.x;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) { x[n][0] *= u0; x[n][1] *= u0; x[n][2] *= u1; x[n][3] *= u1; }
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[n][b][e] += x2[n][b][e];
+            __syncwarp();                                // (the keys have been read)
+            if (lane == 0) {
+                if (stage) issue_keys(kStages - 1, scales[kStages - 1], v_from[kStages - 1]);
+                else issue_keys(0, scales[0], v_from[0]);
+            }
+            __syncwarp();
+            float u[NB][2], f[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) { u[b][0] = fmaxf(unscale[b][0] * sc.x, 1.0e-37f); u[b][1] = fmaxf(unscale[b][1] * sc.x, 1.0e-37f); }      // (not 0: hidden scores are -inf)
             // (a page's tokens come before every row)
             const bool edge = t0 + kTile > inside || (t0 < from_most && t0 + kTile > prefix);
-            weights(x, t0, edge, [&](int tok, int hf) { return tok >= inside || (tok < from[hf] && tok >= prefix); });
-            const int e = (int)(__float_as_uint(sc.y) >> 23) - 127;
-            reach(e);
-            const float f = sc.y * pow2i(kHeadroom - v_exp);
+            weights(x, u, t0, edge, [&](int tok, int b, int e) { return tok >= inside || (tok < from[b][e] && tok >= prefix); },
+                    (float)((int)(__float_as_uint(sc.y) >> 23) - 126), f);
+            // weights as the other operand: rows and tokens change places eight by eight
+            uint32_t pb[NB][2][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t pa[kTerms][4];
+            for (int b = 0; b < NB; ++b) {
+                f[b][0] = fminf(f[b][0] * sc.y, 1.0e37f);
+                f[b][1] = fminf(f[b][1] * sc.y, 1.0e37f);
 #pragma unroll
-                for (int e2 = 0; e2 < 4; ++e2) {         // (row g, g + 8, then the next eight tokens)
-                    const float lo = x[2 * i + (e2 >> 1)][2 * (e2 & 1)] * f, hi = x[2 * i + (e2 >> 1)][2 * (e2 & 1) + 1] * f;
-                    pa[0][e2] = half2_of(lo, hi);
-                    if constexpr (F32) pa[kTerms - 1][e2] = half2_rest(lo, hi, pa[0][e2]);
-                }
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int e2 = 0; e2 < 2; ++e2) {
-                    // (kept as they were rounded)
-                    x[2 * i + e2][0] = __uint_as_float(pa[0][2 * e2]); x[2 * i + e2][1] = __uint_as_float(pa[0][2 * e2 + 1]);
-                    if constexpr (F32) { x[2 * i + e2][2] = __uint_as_float(pa[kTerms - 1][2 * e2]); x[2 * i + e2][3] = __uint_as_float(pa[kTerms - 1][2 * e2 + 1]); }
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                const uint2 w = lds64(values + (8 * c + g) * kTile + 8 * t);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t y = i ? w.y : w.x, b0 = e4m3x2_to_half2(y & 0xffffu), b1 = e4m3x2_to_half2(y >> 16);
-#pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term) {
-                        const uint32_t pa[4] = {__float_as_uint(x[2 * i][2 * term]), __float_as_uint(x[2 * i][2 * term + 1]),
-                                                __float_as_uint(x[2 * i + 1][2 * term]), __float_as_uint(x[2 * i + 1][2 * term + 1])};
-                        mma_f16(o[c], pa, b0, b1);
+                    for (int e = 0; e < 2; ++e) {
+                        const float lo = x[n][b][2 * e] * f[b][0], hi = x[n][b][2 * e + 1] * f[b][1];
+                        pb[b][n][e] = turned(half2_of(lo, hi));
                     }
+            }
+            if (ok && !mbar_wait(bars + 16 * stage + 8, phase)) { atomicOr(&g_fault, 1); ok = false; }
+            ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                const uint2 w0 = lds64(values + (16 * c + g) * kTile + 8 * t), w1 = lds64(values + (16 * c + 8 + g) * kTile + 8 * t);
+                uint32_t a[2][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    e4m3x4_to_half2(n ? w0.y : w0.x, a[n][0], a[n][2]);
+                    e4m3x4_to_half2(n ? w1.y : w1.x, a[n][1], a[n][3]);
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) mma_f16(o[c][b], a[n], pb[b][n][0], pb[b][n][1]);
                 }
             }
-            __syncwarp();                                // (the stage has been read)
+            __syncwarp();                                // (the values have been read)
             ++taken;
-            if (stage) issue(kStages - 1, scales[kStages - 1]);
-            else issue(0, scales[0]);
+            if (lane == 0) issue_values(stage, stage ? v_from[kStages - 1] : v_from[0]);
+            __syncwarp();
         }
 
         // ---- the window and the step's own tokens, sixteen at a time
         if (walk.has_tail()) {
-            using T = typename std::conditional<F32, float, __nv_bfloat16>::type;
+            using T = __nv_bfloat16;
             const T* const k_ring = reinterpret_cast<const T*>(L.k_res) + ((int64_t)q.slot * H + h) * R * D;
             const T* const v_ring = reinterpret_cast<const T*>(L.v_res) + ((int64_t)q.slot * H + h) * R * D;
+            const int total = walk.w.total;
             auto row_at = [&](int tok, bool of_keys) -> const T* {
                 if (tok < q.held) return (of_keys ? k_ring : v_ring) + (int64_t)ring_slot(tok, 0, R) * D;
                 const kivi_rows& r = of_keys ? A.k : A.v;
-                return reinterpret_cast<const T*>(r.data) + ((int64_t)q.row0 + min(tok, walk.w.total - 1) - q.held) * r.row_stride + (int64_t)h * r.head_stride;
+                return reinterpret_cast<const T*>(r.data) + ((int64_t)q.row0 + min(tok, total - 1) - q.held) * r.row_stride + (int64_t)h * r.head_stride;
             };
-            for (int t0 = inside + 16 * warp; t0 < walk.w.total; t0 += 16 * kWarps) {
-                float x[2][4];
+            float one[NB][2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.0f;
-                    const int tok = t0 + 8 * n + g;
-                    const T* const from_row = row_at(tok, true) + kChan * t;
-                    const bool vec = tok < q.held || A.vec;
-                    float4 kx[kChan / 4];
+            for (int b = 0; b < NB; ++b) one[b][0] = one[b][1] = A.scale * (RULES ? 1.0f : 1.4426950408889634f);
+            for (int t0 = inside + 16 * warp; t0 < total; t0 += 16 * kWarps) {
+                float x[1][NB][4];
 #pragma unroll
-                    for (int i = 0; i < kChan / 4; ++i) kx[i] = load4(from_row + 4 * i, vec);
+                for (int b = 0; b < NB; ++b) x[0][b][0] = x[0][b][1] = x[0][b][2] = x[0][b][3] = 0.0f;
+                const T* const row0 = row_at(t0 + g, true) + kChan * t;
+                const T* const row1 = row_at(t0 + 8 + g, true) + kChan * t;
+                const bool vec0 = t0 + g < q.held || A.vec, vec1 = t0 + 8 + g < q.held || A.vec;
+                uint2 k0[kSteps], k1[kSteps];
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        uint32_t qb[kBf][4], b0[kBf], b1[kBf];
-                        bf16_terms(kx[i].x, kx[i].y, b0);
-                        bf16_terms(kx[i].z, kx[i].w, b1);
+                for (int i = 0; i < kSteps; ++i) { k0[i] = quad_of(row0 + 4 * i, vec0); k1[i] = quad_of(row1 + 4 * i, vec1); }
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            const float4 y = *reinterpret_cast<const float4*>(q_s + (g + 8 * hf) * S::kQ + kChan * t + 4 * i);
-                            uint32_t lo[kBf], hi[kBf];
-                            bf16_terms(y.x, y.y, lo);
-                            bf16_terms(y.z, y.w, hi);
+                for (int i = 0; i < kSteps; ++i) {
+                    const uint32_t a[4] = {k0[i].x, k1[i].x, k0[i].y, k1[i].y};
 #pragma unroll
-                            for (int term = 0; term < kBf; ++term) { qb[term][hf] = lo[term]; qb[term][2 + hf] = hi[term]; }
-                        }
-#pragma unroll
-                        for (int sum = kBf - 1; sum >= 0; --sum)                 // products of like size together, the small ones first
-#pragma unroll
-                            for (int a = 0; a <= sum; ++a) mma_bf16(x[n], qb[a], b0[sum - a], b1[sum - a]);
+                    for (int b = 0; b < NB; ++b) {
+                        const uint2 y = *reinterpret_cast<const uint2*>(q_s + (8 * b + g) * S::kQ + kChan * t + 4 * i);
+                        mma_bf16(x[0][b], a, y.x, y.y);
                     }
                 }
-                const float u = A.scale * (RULES ? 1.0f : 1.4426950408889634f);
+                auto hidden = [&](int tok, int b, int e) { return tok >= total || ((tok > place[b][e] || tok < from[b][e]) && tok >= prefix); };
+                float f[NB][2];
+                weights(x, one, t0, true, hidden, 1.0f, f);
+                uint32_t pb[NB][2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[n][e] *= u;
-                auto hidden = [&](int tok, int hf) { return tok >= walk.w.total || ((tok > place[hf] || tok < from[hf]) && tok >= prefix); };
-                weights(x, t0, true, hidden);
-                reach(0);
-                const float f = pow2i(kHeadroom - v_exp);
-                uint32_t pb[kBf][4];
-#pragma unroll
-                for (int e2 = 0; e2 < 4; ++e2) {
-                    uint32_t terms[kBf];
-                    bf16_terms(x[e2 >> 1][2 * (e2 & 1)] * f, x[e2 >> 1][2 * (e2 & 1) + 1] * f, terms);
-#pragma unroll
-                    for (int term = 0; term < kBf; ++term) pb[term][e2] = terms[term];
-                }
-                // Values go through shared memory, a term at a time.  One that is not finite would reach rows that do not
+                    for (int e = 0; e < 2; ++e) pb[b][e] = turned(bf16x2_of(x[0][b][2 * e] * f[b][0], x[0][b][2 * e + 1] * f[b][1]));
+                // Values go through shared memory, eight tokens at a time.  One that is not finite would reach rows that do not
                 // see it through weights of 0: it is left out there, and added to the rows that do.
                 bool odd = false;
+                uint32_t a[D / 16][4];
 #pragma unroll
-                for (int term = 0; term < kBf; ++term) {
+                for (int half = 0; half < 2; ++half) {
                     __syncwarp();
-                    for (int i = lane; i < 16 * (D / 8); i += 32) {
-                        const int j = i / (D / 8), p = i % (D / 8), tok = t0 + j;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const int j = (32 * i + lane) / (D / 8), p = lane % (D / 8), tok = t0 + 8 * half + j;
                         const T* const from_row = row_at(tok, false) + 8 * p;
                         const bool vec = tok < q.held || A.vec;
-                        float4 y[2] = {load4(from_row, vec), load4(from_row + 4, vec)};
-                        uint32_t w[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float a = k & 1 ? y[k >> 1].z : y[k >> 1].x, b = k & 1 ? y[k >> 1].w : y[k >> 1].y;
-                            if (!(fabsf(a) <= 3.4028234e38f)) { odd = true; a = 0.0f; }
-                            if (!(fabsf(b) <= 3.4028234e38f)) { odd = true; b = 0.0f; }
-                            uint32_t terms[kBf];
-                            bf16_terms(a, b, terms);
-                            w[k] = tok < walk.w.total ? terms[term] : 0u;
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(v_stage + j * (2 * D) + ((p ^ (j & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        const uint2 lo = quad_of(from_row, vec), hi = quad_of(from_row + 4, vec);
+                        const bool there = tok < total;
+                        const uint32_t w[4] = {there ? finite_pair(lo.x, odd) : 0u, there ? finite_pair(lo.y, odd) : 0u, there ? finite_pair(hi.x, odd) : 0u, there ? finite_pair(hi.y, odd) : 0u};
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(v_stage + j * (2 * D) + ((p ^ j) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                     }
                     __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < D / 8; c += 2) {
+                    for (int c = 0; c < D / 16; c += 2) {
                         uint32_t r[4];
-                        const int j = (lane & 7) + (lane & 8), p = c + (lane >> 4);
-                        ldmatrix_trans(v_stage + j * (2 * D) + ((p ^ (j & 7)) << 4), r);
-#pragma unroll
-                        for (int a = kBf - 1 - term; a >= 0; --a) {
-                            mma_bf16(o[c], pb[a], r[0], r[1]);
-                            mma_bf16(o[c + 1], pb[a], r[2], r[3]);
-                        }
+                        const int j = lane & 7, p = 2 * c + (lane >> 3);
+                        ldmatrix_trans(v_stage + j * (2 * D) + ((p ^ j) << 4), r);
+                        a[c][2 * half] = r[0]; a[c][2 * half + 1] = r[1];
+                        a[c + 1][2 * half] = r[2]; a[c + 1][2 * half + 1] = r[3];
                     }
                 }
-                if (__any_sync(0xffffffffu, odd)) {
-                    for (int j = 0; j < 16; ++j) {
-                        const int tok = t0 + j;
-                        if (tok >= walk.w.total) break;
-                        const T* const from_row = row_at(tok, false);
 #pragma unroll
-                        for (int c = 0; c < D / 8; ++c)
+                for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) mma_bf16(o[c][b], a[c], pb[b][0], pb[b][1]);
+                if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+                    for (int j = 0; j < 16 && t0 + j < total; ++j) {
+                        const T* const from_row = row_at(t0 + j, false);
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float y = (float)from_row[8 * c + 2 * t + (e & 1)];
-                                if (!(fabsf(y) <= 3.4028234e38f) && !hidden(tok, e >> 1)) o[c][e] += y;
+                                const float y = __bfloat162float(from_row[16 * c + 8 * (e >> 1) + g]);
+                                if (fabsf(y) <= 3.4028234e38f) continue;
+#pragma unroll
+                                for (int b = 0; b < NB; ++b)
+                                    if (!hidden(t0 + j, b, e & 1)) o[c][b][e] += y;
                             }
                     }
                 }
@@ -588,108 +636,110 @@ paged8_decode_kernel(Paged8Attn A) {
 
         // ---- the warps meet
         {
-            const float f = pow2i(v_exp == -1000 ? 0 : v_exp - kHeadroom);
-            rescale(f, f);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-                l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+            for (int b = 0; b < NB; ++b) {
+                // (weights in powers of two from the maximum; nothing seen: 0)
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    f[e] = m[b][e] == -INFINITY ? 0.0f : ex2(fmaxf(ref[b][e] - m[b][e] - kHeadroom, -126.0f));
+                    l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], 4);
+                    l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], 8);
+                    l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], 16);
+                }
+                rescale(b, f[0], f[1]);
             }
             auto leave = [&](int buf) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int r = g + 8 * hf;
-                    if (r >= n_rows) continue;
-                    if (t == 0) *reinterpret_cast<float2*>(ml_s + (buf * kRows + r) * 2) = make_float2(m[hf], l[hf]);
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c)
-                        *reinterpret_cast<float2*>(fold_s + (buf * kRows + r) * S::kO + 8 * c + 2 * t) = make_float2(o[c][2 * hf], o[c][2 * hf + 1]);
-                }
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 8 * b + 2 * t + e;
+                        if (r >= n_rows) continue;
+                        if (g == 0) *reinterpret_cast<float2*>(ml_s + (buf * kRows + r) * 2) = make_float2(m[b][e], l[b][e]);
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            fold_s[(buf * kRows + r) * S::kO + 16 * c + g] = o[c][b][e];
+                            fold_s[(buf * kRows + r) * S::kO + 16 * c + 8 + g] = o[c][b][2 + e];
+                        }
+                    }
             };
             auto take = [&](int buf) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int r = g + 8 * hf;
-                    if (r >= n_rows) continue;
-                    const float2 ml = *reinterpret_cast<const float2*>(ml_s + (buf * kRows + r) * 2);
-                    const float M = fmaxf(m[hf], ml.x), b = M == -INFINITY ? 0.0f : M;
-                    const float mine = F32 ? exp2f(m[hf] - b) : ex2(m[hf] - b), other = F32 ? exp2f(ml.x - b) : ex2(ml.x - b);
-                    m[hf] = M;
-                    l[hf] = l[hf] * mine + ml.y * other;
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        const float2 y = *reinterpret_cast<const float2*>(fold_s + (buf * kRows + r) * S::kO + 8 * c + 2 * t);
-                        o[c][2 * hf] = fmaf(y.x, other, o[c][2 * hf] * mine);
-                        o[c][2 * hf + 1] = fmaf(y.y, other, o[c][2 * hf + 1] * mine);
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 8 * b + 2 * t + e;
+                        if (r >= n_rows) continue;
+                        const float2 ml = *reinterpret_cast<const float2*>(ml_s + (buf * kRows + r) * 2);
+                        const float M = fmaxf(m[b][e], ml.x), from_0 = M == -INFINITY ? 0.0f : M, mine = ex2(m[b][e] - from_0), other = ex2(ml.x - from_0);
+                        m[b][e] = M;
+                        l[b][e] = l[b][e] * mine + ml.y * other;
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c) {
+                            o[c][b][e] = fmaf(fold_s[(buf * kRows + r) * S::kO + 16 * c + g], other, o[c][b][e] * mine);
+                            o[c][b][2 + e] = fmaf(fold_s[(buf * kRows + r) * S::kO + 16 * c + 8 + g], other, o[c][b][2 + e] * mine);
+                        }
                     }
-                }
             };
             __syncthreads();                             // (values of the tail have been read)
-            if (warp >= 2) leave(warp - 2);
+            if (warp >= S::kHalf) leave(warp - S::kHalf);
             __syncthreads();
-            if (warp < 2) take(warp);
+            if (warp < S::kHalf) take(warp);
             __syncthreads();
-            if (warp == 1) leave(0);
+            if (warp > 0 && warp < S::kHalf) leave(warp);
             __syncthreads();
             if (warp == 0) {
-                take(0);
-                // the CTAs that have something of the unit
-                const int64_t c0 = walk.unit / per, c1 = (walk.unit + walk.w.tiles) / per;
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int r = g + 8 * hf, row = row_first + r;
-                    if (r >= n_rows) continue;
-                    if (c0 == c1) {
-                        const float inv = 1.0f / l[hf];  // (a row sees itself: l > 0)
-                        const int64_t at = ((int64_t)q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
-#pragma unroll
-                        for (int c = 0; c < D / 8; ++c) {
-                            const int64_t i = at + 8 * c + 2 * t;
-                            const float a = o[c][2 * hf] * inv, b = o[c][2 * hf + 1] * inv;
-                            if (A.out_dtype == KIVI_BF16) {
-                                __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(A.out.data) + i;
-                                if ((reinterpret_cast<uintptr_t>(to) & 3u) == 0) *reinterpret_cast<uint32_t*>(to) = bf16x2_of(a, b);
-                                else { to[0] = __float2bfloat16_rn(a); to[1] = __float2bfloat16_rn(b); }
-                            } else {
-                                float* to = reinterpret_cast<float*>(A.out.data) + i;
-                                to[0] = a; to[1] = b;
-                            }
-                        }
-                    } else {
-                        const int64_t slot = 2 * (int64_t)blockIdx.x + (c0 == (int64_t)blockIdx.x ? 1 : 0), part = slot * kRows + r;
-                        if (t == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = make_float2(m[hf], l[hf]);
-#pragma unroll
-                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<float2*>(A.part_o + part * D + 8 * c + 2 * t) = make_float2(o[c][2 * hf], o[c][2 * hf + 1]);
-                    }
+#pragma unroll 1
+                for (int i = 1; i < S::kHalf; ++i) take(i);
+                leave(0);
+            }
+            __syncthreads();
+            // the CTAs that have something of the unit
+            const int64_t c0 = walk.unit / per, c1 = (walk.unit + walk.w.tiles) / per;
+            const int64_t slot = 2 * (int64_t)blockIdx.x + (c0 == (int64_t)blockIdx.x ? 1 : 0);
+            for (int i = tid; i < n_rows * (D / 4); i += kThreads) {
+                const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row_first + r;
+                const float4 y = *reinterpret_cast<const float4*>(fold_s + r * S::kO + d);
+                const float2 ml = *reinterpret_cast<const float2*>(ml_s + r * 2);
+                if (c0 == c1) {
+                    const float inv = 1.0f / ml.y;       // (a row sees itself: the sum is above 0)
+                    const int64_t at = ((int64_t)q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
+                    store_quad(A.out.data, A.out_dtype, at + d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+                } else {
+                    const int64_t part = slot * kRows + r;
+                    if (d == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * part) = ml;
+                    *reinterpret_cast<float4*>(A.part_o + part * D + d) = y;
                 }
             }
         }
     }
     // (a stage that a wait has given up on is not left to the next block's shared memory)
-    for (; taken < issued; ++taken) mbar_wait(bars + 8 * (taken % kStages), (uint32_t)(taken / kStages) & 1u);
+    for (; lane == 0 && taken < issued; ++taken)
+        for (int i = 0; i < 2; ++i) mbar_wait(bars + 16 * (taken % kStages) + 8 * i, (uint32_t)(taken / kStages) & 1u);
 }
 
 // Folds the units that lie across a CTA's end.  Block c has the unit that position c per lies in, if it is the first
 // such end there; a thread a quad of channels of a row.
-template <bool F32>
-__global__ void __launch_bounds__(kThreads)
-paged8_fold_kernel(Paged8Attn A, int ctas) {
+__global__ void __launch_bounds__(128)
+paged8_fold_kernel(Paged8Attn A, int unit_rows, int ctas) {
+    constexpr int kWarps = 4, kThreads = 32 * kWarps;
     __shared__ int64_t scratch[kWarps + 2];
     stream_order();
     settle_args(A);
     const int c = blockIdx.x + 1, D = A.L.head_dim, n_rep = A.n_rep;
-    const Line line = find_line<F32>(A, scratch, [&](int64_t cost) { return per_cta(cost, ctas) * c; });
+    const Line line = find_line<kWarps>(A, unit_rows, scratch, [&](int64_t cost) { return per_cta(cost, ctas) * c; });
     if (line.first < 0) return;
     const int64_t per = per_cta(line.cost, ctas), at = per * c;
     SeqWork w;
-    seq_work<F32>(A, line.first, w);
+    seq_work(A, unit_rows, line.first, w);
     const int64_t u = (at - line.before) / w.cost(), unit = line.before + u * w.cost();
     const int64_t c0 = unit / per, c1 = (unit + w.tiles) / per;
     if (unit == at || c0 != c - 1 || c1 == c0) return;
-    const int h = (int)(u / w.blocks), row_first = (int)(u % w.blocks) * kRows, n_rows = min(kRows, w.rows - row_first), quads = D / 4;
+    const int h = (int)(u / w.blocks), row_first = (int)(u % w.blocks) * unit_rows, n_rows = min(unit_rows, w.rows - row_first), quads = D / 4;
     for (int i = threadIdx.x; i < n_rows * quads; i += kThreads) {
         const int r = i / quads, d = 4 * (i % quads);
-        auto part = [&](int64_t k) { return (2 * k + (k == c0 ? 1 : 0)) * kRows + r; };
+        auto part = [&](int64_t k) { return (2 * k + (k == c0 ? 1 : 0)) * unit_rows + r; };
         float M = -INFINITY, sum = 0.0f;
 #pragma unroll 4
         for (int64_t k = c0; k <= c1; ++k) M = fmaxf(M, A.part_ml[2 * part(k)]);
@@ -709,28 +759,42 @@ paged8_fold_kernel(Paged8Attn A, int ctas) {
     }
 }
 
-template <int D, bool F32, bool RULES>
-int go(const Paged8Attn& a, int ctas, cudaStream_t st) {
-    auto* const kernel = paged8_decode_kernel<D, F32, RULES>;
-    KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::bytes));
-    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)ctas), kThreads, Layout<D>::bytes, st, true, a));
-    KIVI_CUDA_OK(launch(paged8_fold_kernel<F32>, dim3((unsigned)(ctas - 1)), kThreads, 0, st, true, a, ctas));
+constexpr int kMostBlocks = 3, kMostRows = 64;
+
+// Blocks of eight rows of a unit: all of a sequence's rows in one unit where registers hold them, so that its bytes are
+// read once.
+int unit_blocks(int64_t max_rows) {
+    const int64_t need = (max_rows + 7) / 8;
+    return need <= kMostBlocks ? (int)need : kMostBlocks;
+}
+
+template <int D, int NB, bool RULES>
+int go(const Paged8Attn& a, cudaStream_t st) {
+    constexpr int kSmem = Layout<D, NB>::bytes;
+    auto* const kernel = paged8_decode_kernel<D, NB, RULES>;
+    const int ctas = kPerSm * num_sms();
+    KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)ctas), 32 * warps_of(NB), kSmem, st, true, a));
+    KIVI_CUDA_OK(launch(paged8_fold_kernel, dim3((unsigned)(ctas - 1)), 128, 0, st, true, a, 8 * NB, ctas));
     return KIVI_OK;
+}
+template <int D, int NB>
+int go(const Paged8Attn& a, cudaStream_t st) {
+    const bool rules = a.rules.softcap > 0.0f || a.rules.slopes != nullptr;
+    return rules ? go<D, NB, true>(a, st) : go<D, NB, false>(a, st);
 }
 
 }  // namespace
 
 bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows) {
-    return (L->head_dim == 64 || L->head_dim == 128) && L->group_size % 32 == 0 && q_dtype == L->res_dtype && max_rows <= 64;
+    return (L->head_dim == 64 || L->head_dim == 128) && L->group_size % kTile == 0 && q_dtype == KIVI_BF16 && L->res_dtype == KIVI_BF16 && max_rows <= kMostRows;
 }
-int paged8_decode_ctas() { return kPerSm * num_sms(); }
-size_t paged8_decode_parts() { return (size_t)paged8_decode_ctas() * 2 * kRows; }          // rows of partials
+size_t paged8_decode_parts(int64_t max_rows) { return (size_t)kPerSm * num_sms() * 2 * 8 * unit_blocks(max_rows); }          // rows of partials
 
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st) {
-    const bool f32 = a.q_dtype == KIVI_F32, rules = a.rules.softcap > 0.0f || a.rules.slopes != nullptr;
-    const int n = paged8_decode_ctas();
-    if (a.L.head_dim == 64) return f32 ? (rules ? go<64, true, true>(a, n, st) : go<64, true, false>(a, n, st)) : (rules ? go<64, false, true>(a, n, st) : go<64, false, false>(a, n, st));
-    return f32 ? (rules ? go<128, true, true>(a, n, st) : go<128, true, false>(a, n, st)) : (rules ? go<128, false, true>(a, n, st) : go<128, false, false>(a, n, st));
+    const int nb = unit_blocks((int64_t)a.b.max_new * a.n_rep);
+    if (a.L.head_dim == 64) return nb == 1 ? go<64, 1>(a, st) : nb == 2 ? go<64, 2>(a, st) : go<64, 3>(a, st);
+    return nb == 1 ? go<128, 1>(a, st) : nb == 2 ? go<128, 2>(a, st) : go<128, 3>(a, st);
 }
 
 int paged8_decode_fault_word(int* out) {

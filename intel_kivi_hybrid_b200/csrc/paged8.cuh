@@ -42,6 +42,10 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
     asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(y) : "r"(two));
     return y;
 }
+// a word's four numbers, two and two
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
 __device__ __forceinline__ float half_lo(uint32_t h) {
     float y;
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.f32.f16 %0, a;\n\t}" : "=f"(y) : "r"(h));
@@ -54,7 +58,8 @@ __device__ __forceinline__ float half_hi(uint32_t h) {
 }
 // a word's four numbers
 __device__ __forceinline__ float4 e4m3x4(uint32_t w) {
-    const uint32_t a = e4m3x2_to_half2(w & 0xffffu), b = e4m3x2_to_half2(w >> 16);
+    uint32_t a, b;
+    e4m3x4_to_half2(w, a, b);
     return make_float4(half_lo(a), half_hi(a), half_lo(b), half_hi(b));
 }
 
