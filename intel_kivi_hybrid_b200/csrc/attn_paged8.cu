@@ -347,6 +347,7 @@ int paged8_attention_fault_clear() {
 
 bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows);
 size_t paged8_decode_parts(int64_t max_rows);
+int paged8_decode_notes();
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st);
 bool paged8_tc_serves(const kivi_paged8_layer* L, int q_dtype);
 int run_paged8_tc(const Paged8Attn& a, int blocks, cudaStream_t st);
@@ -422,7 +423,7 @@ static int check_attention8(const kivi_paged8_layer* L, const kivi_paged_batch* 
 }
 
 static size_t plan_bytes(const kivi_paged8_layer* L, const Paged8Plan& p) {
-    if (p.kernel == Paged8Kernel::kDecode) return (size_t)p.blocks * (L->head_dim + 2) * 4;
+    if (p.kernel == Paged8Kernel::kDecode) return ((size_t)p.blocks * (L->head_dim + 2) + paged8_decode_notes()) * 4;
     return p.pieces > 1 ? (size_t)p.blocks * L->num_kv_heads * p.pieces * p.rows * (L->head_dim + 2) * 4 : 0;
 }
 
@@ -463,6 +464,7 @@ extern "C" int kivi_paged8_attention(const kivi_paged8_layer* L, const kivi_page
     a.vec = grid4(*q, q_dtype) && grid4(*new_k, L->res_dtype) && grid4(*new_v, L->res_dtype);
     cudaStream_t st = (cudaStream_t)stream;
     if (p.kernel == Paged8Kernel::kDecode) {
+        a.notes = reinterpret_cast<int*>(a.part_ml + (size_t)p.blocks * 2);
         if (int rc = run_paged8_decode(a, st)) return rc;
         note_launches(2);
         return KIVI_OK;

@@ -5,7 +5,7 @@
 //
 // by mma.sync m16n8k16, 32 tokens of a page to a warp at a time.  Tokens (and channels of V)
 // are the sixteen rows of an MMA, the (new token, query head) pairs of one sequence and KV head
-// its eight columns, up to three times eight to a unit: with the pairs as rows a single token of four heads took twice
+// its eight columns, up to twice eight to a unit: with the pairs as rows a single token of four heads took twice
 // the MMAs and the registers (64 ragged sequences up to 32k 555 us).  Weights change places with movmatrix in between.
 // What bounds it is the page's bytes: a tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions
 // and 32 MMAs of a warp (fp32 rows: 64).
@@ -37,6 +37,7 @@ __device__ int g_fault = 0;
 constexpr int kStages = 2;
 constexpr int kTile = 32;                                // tokens of a tile
 constexpr int kPerSm = 2;                                // CTAs
+constexpr int kNote = 8;                                 // numbers of a CTA's note to the fold: CTAs behind it that have some of the unit, row0, head, first row, rows
 constexpr int kLeast = 8;                                // tiles of a CTA
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 constexpr float kHeadroom = 8.0f, kSlack = 6.0f;         // products of weight and scale: up to 2^8, or 2^14 before their reference moves
@@ -75,6 +76,9 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w, bool& odd) {
     if ((w & 0x7f80u) == 0x7f80u) { w &= 0xffff0000u; odd = true; }
     if ((w & 0x7f800000u) == 0x7f800000u) { w &= 0xffffu; odd = true; }
     return w;
+}
+__device__ __forceinline__ void copy8(uint32_t to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
     uint4 v;
@@ -120,17 +124,17 @@ __device__ __forceinline__ bool seq_work(const Paged8Attn& A, int unit_rows, int
     return true;
 }
 
-struct Line { int64_t cost; int64_t before; int first; };         // all positions; those before sequence `first`, which has position `at`
+struct Line { int64_t cost, before; int first; };        // all positions; those before sequence `first`
 
-// Called by the whole CTA: the line's length, and which sequence has position at(length).
+// Called by the whole CTA: the line's length, and which sequence has position at(length) (-1: none), which comes to `found`.
 template <int kWarps, typename At>
-__device__ __forceinline__ Line find_line(const Paged8Attn& A, int unit_rows, int64_t* scratch /* [kWarps + 2] shared */, const At& at) {
+__device__ __forceinline__ Line find_line(const Paged8Attn& A, int unit_rows, int64_t* scratch /* [kWarps + 2] shared */, SeqWork& found /* shared */, const At& at) {
     constexpr int kThreads = 32 * kWarps;
     const int n = A.b.num_seqs, H = A.L.num_kv_heads, per = (n + kThreads - 1) / kThreads;
+    SeqWork w;
     int64_t mine = 0;
     for (int i = 0; i < per; ++i) {
         const int s = threadIdx.x * per + i;
-        SeqWork w;
         if (s < n && seq_work(A, unit_rows, s, w)) mine += (int64_t)H * w.blocks * w.cost();
     }
     // sums of what comes before each thread's sequences
@@ -153,9 +157,9 @@ __device__ __forceinline__ Line find_line(const Paged8Attn& A, int unit_rows, in
     if (want >= before && want < before + mine) {
         for (int i = 0; i < per; ++i) {
             const int s = threadIdx.x * per + i;
-            SeqWork w;
-            const int64_t c = s < n && seq_work(A, unit_rows, s, w) ? (int64_t)H * w.blocks * w.cost() : 0;
-            if (want < before + c) { scratch[kWarps] = s; scratch[kWarps + 1] = before; break; }
+            if (per > 1 && (s >= n || !seq_work(A, unit_rows, s, w))) continue;
+            const int64_t c = (int64_t)H * w.blocks * w.cost();
+            if (want < before + c) { scratch[kWarps] = s; scratch[kWarps + 1] = before; found = w; break; }
             before += c;
         }
     }
@@ -185,9 +189,10 @@ struct Walk {
                 continue;
             }
             const int c = w.cost();
-            const int64_t u = (at - off) / c;
-            h = (int)(u / w.blocks); rb = (int)(u % w.blocks);
-            unit = off + u * c;
+            const uint64_t x = (uint64_t)(at - off);
+            const uint32_t u = x >> 32 ? (uint32_t)(x / (uint32_t)c) : (uint32_t)x / (uint32_t)c;        // (a sequence's units are fewer than 2^32)
+            h = (int)(u / (uint32_t)w.blocks); rb = (int)(u % (uint32_t)w.blocks);
+            unit = off + (int64_t)u * c;
             a = (int)(at - unit);
             b = (int)min((int64_t)c, end - unit);
             at = unit + b;
@@ -236,17 +241,19 @@ paged8_decode_kernel(Paged8Attn A) {
         for (int i = 0; i < 2 * kStages; ++i) mbar_init(bars + 8 * i, 1);
         mbar_init_fence();
     }
-    const Line line = find_line<kWarps>(A, kRows, reinterpret_cast<int64_t*>(smem + S::scratch), [&](int64_t cost) { return per_cta(cost, gridDim.x) * blockIdx.x; });
-    if (line.first < 0) return;
-    const int64_t per = per_cta(line.cost, gridDim.x);
     Walk& walk = *reinterpret_cast<Walk*>(smem + S::walks);                 // what is computed
     Walk& ahead = (&walk)[1 + warp];                                         // what the warp copies: its first lane's
-    auto start = [&](Walk& w) {
-        w.s = line.first; w.off = line.before;
-        w.at = per * blockIdx.x; w.end = min(w.at + per, line.cost);
-        seq_work(A, kRows, w.s, w.w);
-    };
-    if (tid == 0) start(walk);
+    int* const note = A.notes + kNote * (int)blockIdx.x;
+    const Line line = find_line<kWarps>(A, kRows, reinterpret_cast<int64_t*>(smem + S::scratch), walk.w, [&](int64_t cost) { return per_cta(cost, gridDim.x) * blockIdx.x; });
+    if (tid == 0) note[0] = 0;                           // (nothing of this CTA's is to be folded, so far)
+    if (line.first < 0) return;
+    const int64_t per = per_cta(line.cost, gridDim.x);
+    if (tid == 0) {
+        walk.s = line.first; walk.off = line.before;
+        walk.at = per * blockIdx.x; walk.end = min(walk.at + per, line.cost);
+    }
+    __syncthreads();
+    if (lane == 0) ahead = walk;
     const uint64_t policy = l2_stream_policy();
 
     // ---- copies, all of them the first lane's: the warp's next tile into a stage
@@ -298,14 +305,8 @@ paged8_decode_kernel(Paged8Attn A) {
         mbar_expect_tx(bars + 16 * stage + 8, S::kPart);
         bulk_g2s(ring + stage * (2 * S::kPart) + S::kPart, L.v_codes + from, S::kPart, bars + 16 * stage + 8, policy);
     };
-    if (lane == 0) {
-        start(ahead);
-        settle_next();
-#pragma unroll
-        for (int i = 0; i < kStages; ++i) { issue_keys(i, scales[i], v_from[i]); issue_values(i, v_from[i]); }
-    }
     int taken = 0;
-    bool ok = true;
+    bool ok = true, started = false;
 
     for (;;) {
         __syncthreads();                                 // (the unit before is folded)
@@ -317,10 +318,33 @@ paged8_decode_kernel(Paged8Attn A) {
         // ---- the unit's queries
         for (int i = tid; i < kRows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row_first + r;
-            uint2 x = make_uint2(0u, 0u);
-            if (r < n_rows) x = quad_of(reinterpret_cast<const __nv_bfloat16*>(A.q.data) + ((int64_t)q.row0 + row / n_rep) * A.q.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.q.head_stride + d, A.vec != 0);
-            *reinterpret_cast<uint2*>(q_s + r * S::kQ + d) = x;
+            const __nv_bfloat16* const from_row = reinterpret_cast<const __nv_bfloat16*>(A.q.data) + ((int64_t)q.row0 + row / n_rep) * A.q.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.q.head_stride + d;
+            if (r >= n_rows || !A.vec) *reinterpret_cast<uint2*>(q_s + r * S::kQ + d) = r < n_rows ? quad_of(from_row, false) : make_uint2(0u, 0u);
+            else copy8(smem_u32(q_s + r * S::kQ + d), from_row);
         }
+        if (!started && lane == 0) {
+            settle_next();
+#pragma unroll
+            for (int i = 0; i < kStages; ++i) { issue_keys(i, scales[i], v_from[i]); issue_values(i, v_from[i]); }
+        }
+        started = true;
+        __syncwarp();
+        const int total = walk.w.total;
+        const __nv_bfloat16* const k_ring = reinterpret_cast<const __nv_bfloat16*>(L.k_res) + ((int64_t)q.slot * H + h) * R * D;
+        const __nv_bfloat16* const v_ring = reinterpret_cast<const __nv_bfloat16*>(L.v_res) + ((int64_t)q.slot * H + h) * R * D;
+        auto row_at = [&](int tok, bool of_keys) -> const __nv_bfloat16* {
+            if (tok < q.held) return (of_keys ? k_ring : v_ring) + (int64_t)ring_slot(tok, 0, R) * D;
+            const kivi_rows& r = of_keys ? A.k : A.v;
+            return reinterpret_cast<const __nv_bfloat16*>(r.data) + ((int64_t)q.row0 + min(tok, total - 1) - q.held) * r.row_stride + (int64_t)h * r.head_stride;
+        };
+        if (walk.has_tail())                             // the rows that come last are on their way to L2 meanwhile
+            for (int t0 = inside + 16 * warp; t0 < total; t0 += 16 * kWarps)
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    const char* const at = reinterpret_cast<const char*>(row_at(t0 + (lane & 15), lane < 16)) + 128 * i;
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+                }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
         // As an operand a lane has channels kChan t .. of row 8 b + g, four to an MMA; keys lie the same way.
         uint32_t qb[NB][kSteps][2];
@@ -545,15 +569,6 @@ paged8_decode_kernel(Paged8Attn A) {
 
         // ---- the window and the step's own tokens, sixteen at a time
         if (walk.has_tail()) {
-            using T = __nv_bfloat16;
-            const T* const k_ring = reinterpret_cast<const T*>(L.k_res) + ((int64_t)q.slot * H + h) * R * D;
-            const T* const v_ring = reinterpret_cast<const T*>(L.v_res) + ((int64_t)q.slot * H + h) * R * D;
-            const int total = walk.w.total;
-            auto row_at = [&](int tok, bool of_keys) -> const T* {
-                if (tok < q.held) return (of_keys ? k_ring : v_ring) + (int64_t)ring_slot(tok, 0, R) * D;
-                const kivi_rows& r = of_keys ? A.k : A.v;
-                return reinterpret_cast<const T*>(r.data) + ((int64_t)q.row0 + min(tok, total - 1) - q.held) * r.row_stride + (int64_t)h * r.head_stride;
-            };
             float one[NB][2];
 #pragma unroll
             for (int b = 0; b < NB; ++b) one[b][0] = one[b][1] = A.scale * (RULES ? 1.0f : 1.4426950408889634f);
@@ -561,12 +576,21 @@ paged8_decode_kernel(Paged8Attn A) {
                 float x[1][NB][4];
 #pragma unroll
                 for (int b = 0; b < NB; ++b) x[0][b][0] = x[0][b][1] = x[0][b][2] = x[0][b][3] = 0.0f;
-                const T* const row0 = row_at(t0 + g, true) + kChan * t;
-                const T* const row1 = row_at(t0 + 8 + g, true) + kChan * t;
+                const __nv_bfloat16* const row0 = row_at(t0 + g, true) + kChan * t;
+                const __nv_bfloat16* const row1 = row_at(t0 + 8 + g, true) + kChan * t;
                 const bool vec0 = t0 + g < q.held || A.vec, vec1 = t0 + 8 + g < q.held || A.vec;
-                uint2 k0[kSteps], k1[kSteps];
+                uint2 k0[kSteps], k1[kSteps], vw[2][D / 32][2];          // (all on their way together)
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) { k0[i] = quad_of(row0 + 4 * i, vec0); k1[i] = quad_of(row1 + 4 * i, vec1); }
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const int tok = t0 + 8 * half + (32 * i + lane) / (D / 8);
+                        const __nv_bfloat16* const from_row = row_at(tok, false) + 8 * (lane % (D / 8));
+                        const bool vec = tok < q.held || A.vec;
+                        vw[half][i][0] = quad_of(from_row, vec); vw[half][i][1] = quad_of(from_row + 4, vec);
+                    }
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     const uint32_t a[4] = {k0[i].x, k1[i].x, k0[i].y, k1[i].y};
@@ -594,9 +618,7 @@ paged8_decode_kernel(Paged8Attn A) {
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i) {
                         const int j = (32 * i + lane) / (D / 8), p = lane % (D / 8), tok = t0 + 8 * half + j;
-                        const T* const from_row = row_at(tok, false) + 8 * p;
-                        const bool vec = tok < q.held || A.vec;
-                        const uint2 lo = quad_of(from_row, vec), hi = quad_of(from_row + 4, vec);
+                        const uint2 lo = vw[half][i][0], hi = vw[half][i][1];
                         const bool there = tok < total;
                         const uint32_t w[4] = {there ? finite_pair(lo.x, odd) : 0u, there ? finite_pair(lo.y, odd) : 0u, there ? finite_pair(hi.x, odd) : 0u, there ? finite_pair(hi.y, odd) : 0u};
                         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(v_stage + j * (2 * D) + ((p ^ j) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
@@ -618,7 +640,7 @@ paged8_decode_kernel(Paged8Attn A) {
                 if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll 1
                     for (int j = 0; j < 16 && t0 + j < total; ++j) {
-                        const T* const from_row = row_at(t0 + j, false);
+                        const __nv_bfloat16* const from_row = row_at(t0 + j, false);
 #pragma unroll
                         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
@@ -698,6 +720,10 @@ paged8_decode_kernel(Paged8Attn A) {
             // the CTAs that have something of the unit
             const int64_t c0 = walk.unit / per, c1 = (walk.unit + walk.w.tiles) / per;
             const int64_t slot = 2 * (int64_t)blockIdx.x + (c0 == (int64_t)blockIdx.x ? 1 : 0);
+            if (tid == 0 && c0 != c1 && c0 == (int64_t)blockIdx.x) {
+                note[1] = q.row0; note[2] = h; note[3] = row_first; note[4] = n_rows;
+                note[0] = (int)(c1 - c0);
+            }
             for (int i = tid; i < n_rows * (D / 4); i += kThreads) {
                 const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row_first + r;
                 const float4 y = *reinterpret_cast<const float4*>(fold_s + r * S::kO + d);
@@ -719,33 +745,26 @@ paged8_decode_kernel(Paged8Attn A) {
         for (int i = 0; i < 2; ++i) mbar_wait(bars + 16 * (taken % kStages) + 8 * i, (uint32_t)(taken / kStages) & 1u);
 }
 
-// Folds the units that lie across a CTA's end.  Block c has the unit that position c per lies in, if it is the first
-// such end there; a thread a quad of channels of a row.
+// Folds the units that lie across a CTA's end: block c the one that CTA c has left a note of.  A thread has a quad
+// of channels of a row.
 __global__ void __launch_bounds__(128)
-paged8_fold_kernel(Paged8Attn A, int unit_rows, int ctas) {
-    constexpr int kWarps = 4, kThreads = 32 * kWarps;
-    __shared__ int64_t scratch[kWarps + 2];
+paged8_fold_kernel(Paged8Attn A, int unit_rows) {
     stream_order();
     settle_args(A);
-    const int c = blockIdx.x + 1, D = A.L.head_dim, n_rep = A.n_rep;
-    const Line line = find_line<kWarps>(A, unit_rows, scratch, [&](int64_t cost) { return per_cta(cost, ctas) * c; });
-    if (line.first < 0) return;
-    const int64_t per = per_cta(line.cost, ctas), at = per * c;
-    SeqWork w;
-    seq_work(A, unit_rows, line.first, w);
-    const int64_t u = (at - line.before) / w.cost(), unit = line.before + u * w.cost();
-    const int64_t c0 = unit / per, c1 = (unit + w.tiles) / per;
-    if (unit == at || c0 != c - 1 || c1 == c0) return;
-    const int h = (int)(u / w.blocks), row_first = (int)(u % w.blocks) * unit_rows, n_rows = min(unit_rows, w.rows - row_first), quads = D / 4;
-    for (int i = threadIdx.x; i < n_rows * quads; i += kThreads) {
+    const int c = blockIdx.x, D = A.L.head_dim, n_rep = A.n_rep, quads = D / 4;
+    const int* const note = A.notes + kNote * c;
+    const int more = note[0];
+    if (more <= 0) return;
+    const int row0 = note[1], h = note[2], row_first = note[3], n_rows = note[4];
+    for (int i = threadIdx.x; i < n_rows * quads; i += 128) {
         const int r = i / quads, d = 4 * (i % quads);
-        auto part = [&](int64_t k) { return (2 * k + (k == c0 ? 1 : 0)) * unit_rows + r; };
+        auto part = [&](int k) { return (int64_t)(2 * (c + k) + (k == 0 ? 1 : 0)) * unit_rows + r; };
         float M = -INFINITY, sum = 0.0f;
 #pragma unroll 4
-        for (int64_t k = c0; k <= c1; ++k) M = fmaxf(M, A.part_ml[2 * part(k)]);
+        for (int k = 0; k <= more; ++k) M = fmaxf(M, A.part_ml[2 * part(k)]);
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int64_t k = c0; k <= c1; ++k) {
+        for (int k = 0; k <= more; ++k) {
             const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * part(k));
             const float4 v = *reinterpret_cast<const float4*>(A.part_o + part(k) * D + d);
             const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);         // (nothing of it is seen: O is 0)
@@ -754,7 +773,7 @@ paged8_fold_kernel(Paged8Attn A, int unit_rows, int ctas) {
         }
         const float inv = 1.0f / sum;
         const int row = row_first + r;
-        const int64_t to = ((int64_t)w.q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
+        const int64_t to = ((int64_t)row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
         store_quad(A.out.data, A.out_dtype, to + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
     }
 }
@@ -775,7 +794,7 @@ int go(const Paged8Attn& a, cudaStream_t st) {
     const int ctas = kPerSm * num_sms();
     KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     KIVI_CUDA_OK(launch(kernel, dim3((unsigned)ctas), 32 * warps_of(NB), kSmem, st, true, a));
-    KIVI_CUDA_OK(launch(paged8_fold_kernel, dim3((unsigned)(ctas - 1)), 128, 0, st, true, a, 8 * NB, ctas));
+    KIVI_CUDA_OK(launch(paged8_fold_kernel, dim3((unsigned)(ctas - 1)), 128, 0, st, true, a, 8 * NB));
     return KIVI_OK;
 }
 template <int D, int NB>
@@ -789,6 +808,7 @@ int go(const Paged8Attn& a, cudaStream_t st) {
 bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows) {
     return (L->head_dim == 64 || L->head_dim == 128) && L->group_size % kTile == 0 && q_dtype == KIVI_BF16 && L->res_dtype == KIVI_BF16 && max_rows <= kMostRows;
 }
+int paged8_decode_notes() { return kPerSm * num_sms() * kNote; }           // whole numbers behind the partials
 size_t paged8_decode_parts(int64_t max_rows) { return (size_t)kPerSm * num_sms() * 2 * 8 * unit_blocks(max_rows); }          // rows of partials
 
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st) {

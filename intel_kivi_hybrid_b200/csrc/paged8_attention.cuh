@@ -15,6 +15,7 @@ struct Paged8Attn {
     float scale;                 // of q k
     int pieces, chunk;           // a block's tiles of tokens are cut into pieces of `chunk` (no block has more than `pieces`)
     float *part_o, *part_ml;     // [block][KV head][piece][row]: unnormalised output, (maximum, sum) in powers of two
+    int* notes;                  // of CTAs to the fold (attn_paged8_decode.cu)
 };
 
 // The tiles of T tokens that rows at places p_lo .. p_hi of a sequence of `total` tokens see something of: those of
@@ -47,7 +48,7 @@ __device__ __forceinline__ void settle_args(Paged8Attn& a) {
     settle_paged8(a.L, a.b);
     a.q.data = settled(a.q.data); a.k.data = settled(a.k.data); a.v.data = settled(a.v.data);
     a.rules.slopes = settled(a.rules.slopes); a.rules.prefix = settled(a.rules.prefix);
-    a.part_o = settled(a.part_o); a.part_ml = settled(a.part_ml);
+    a.part_o = settled(a.part_o); a.part_ml = settled(a.part_ml); a.notes = settled(a.notes);
 }
 #endif
 
