@@ -3,15 +3,18 @@
 //   x = had ? (x > 0 ? x / r : x r) : x,   x -= f * times said,   x -= p if said,
 //   x += bias,   x = -inf where the mask has no bit
 //
-// A CTA takes a stretch of a row that its threads hold in registers, 16-byte vectors on the
-// row's own grid (rows of 50257 numbers start anywhere).  What the row has had is counted
-// in shared memory, a word for each entry of the stretch: every CTA of a row reads all of
-// the row's list and keeps what falls into its stretch.  Counts are whole numbers and the
-// last bias is found by its place, so the order in which threads come changes nothing.
+// A CTA takes a stretch of a row, 16-byte vectors on the row's own grid (rows of 50257 numbers
+// start anywhere): copies it to `out`, with -inf where the mask says so, and then writes the
+// entries that a list speaks of once more.  What the row has had is counted in shared memory, 16 bits
+// for each entry of the stretch, and 16 for the last bias's place in its list: every CTA of a row reads all of
+// the row's lists and keeps what falls into its stretch.  Rows with longer lists have 32 bits, for
+// half of the stretch at a time.  Of an entry's several mentions the first that comes writes it, all the same number,
+// and of several biases the last: counts are whole numbers, so the order in which threads come changes nothing.
 //
-// Bound by memory for many rows, by latency for one: bounds of the lists, tokens, counts,
-// one after the other, with the logits on their way meanwhile.  Long stretches read the lists
-// less often, short ones give one row to more SMs (stretch_threads).
+// Bound by memory without lists, by latency with them: bounds of the lists, ids, counts, ids again, logits, one
+// after the other, so that what counts is how many CTAs an SM holds.  128 x 130000 bf16 with lists of 2100 and of 150:
+// 66 us with the stretch in registers and every word looked over, 55 with words of 32 bits, 64 with the lists shared
+// out over a cluster that counts in each other's shared memory.
 #include "kivi_common.cuh"
 
 namespace kivi {
@@ -29,34 +32,25 @@ struct LogitArgs {
     kivi_logit_rules r;
 };
 
-template <typename T> struct Pack;
-template <> struct Pack<float> {
-    static constexpr int N = 4;
-    __device__ static void load(const float* p, float (&x)[4]) { const float4 v = *reinterpret_cast<const float4*>(p); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-    __device__ static void store(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
-};
-template <> struct Pack<__nv_bfloat16> {
-    static constexpr int N = 8;
-    __device__ static void load(const __nv_bfloat16* p, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    }
-    __device__ static void store(__nv_bfloat16* p, const float (&x)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&t);
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
+template <typename T> constexpr int kPack = 16 / sizeof(T);              // numbers of a vector
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+// a vector's numbers without a bit become -inf
+template <typename T> __device__ __forceinline__ uint4 masked(uint4 v, uint32_t bits) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            if (!(bits >> i & 1u)) w[i] = 0xff800000u;
+        } else {
+            if (!(bits >> (2 * i) & 1u)) w[i] = (w[i] & 0xffff0000u) | 0xff80u;
+            if (!(bits >> (2 * i + 1) & 1u)) w[i] = (w[i] & 0xffffu) | 0xff800000u;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // the part of a list that is a row's; bounds that the array does not have: nothing
 __device__ __forceinline__ int2 list_of(const int32_t* cu, int row, int total) {
@@ -68,11 +62,37 @@ __device__ __forceinline__ int2 list_of(const int32_t* cu, int row, int total) {
     return make_int2(lo, hi);
 }
 
+// Counters of 16 or 32 bits.
+struct Counters {
+    uint8_t* at;
+    bool wide;
+    __device__ uint32_t given() const { return wide ? 0x80000000u : 0x8000u; }   // had in the prompt
+    __device__ uint32_t taken() const { return wide ? 0x40000000u : 0x4000u; }   // written; below: times said
+    __device__ uint32_t get(int i) const { return wide ? reinterpret_cast<const uint32_t*>(at)[i] : reinterpret_cast<const uint16_t*>(at)[i]; }
+    __device__ uint32_t put(int i, uint32_t bits, bool add) const {              // what was there before
+        uint32_t* const word = reinterpret_cast<uint32_t*>(at) + (wide ? i : i >> 1);
+        const int shift = wide ? 0 : 16 * (i & 1);
+        const uint32_t was = (add ? atomicAdd(word, bits << shift) : atomicOr(word, bits << shift)) >> shift;
+        return wide ? was : was & 0xffffu;
+    }
+    __device__ void most(int i, uint32_t place) const {
+        if (wide) { atomicMax(reinterpret_cast<uint32_t*>(at) + i, place); return; }
+        unsigned short* const half = reinterpret_cast<unsigned short*>(at) + i;
+        unsigned short was = *half;
+        while (was < place) {
+            const unsigned short now = atomicCAS(half, was, (unsigned short)place);
+            if (now == was) break;
+            was = now;
+        }
+    }
+};
+constexpr int kNarrowTokens = 0x3fff, kNarrowBiases = 0xfffe;
+
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS)
 adjust_logits_kernel(LogitArgs A) {
-    constexpr int N = Pack<T>::N, kEntries = THREADS * kVectors * N;
-    extern __shared__ __align__(16) uint32_t word_s[];   // [kEntries]
+    constexpr int N = kPack<T>, kEntries = THREADS * kVectors * N;
+    extern __shared__ __align__(16) uint8_t counters[];  // 2 * kEntries bytes where there are tokens, then as many where there are biases
     stream_order();
     const kivi_logit_rules& r = A.r;
     const int row = blockIdx.y, tid = threadIdx.x;
@@ -83,123 +103,121 @@ adjust_logits_kernel(LogitArgs A) {
     const int64_t first = (int64_t)blockIdx.x * kEntries - before;
     if (first >= A.vocab) return;
     const bool apart = ((reinterpret_cast<uintptr_t>(out) / sizeof(T)) & (N - 1)) != (unsigned)before;        // (out's vectors lie elsewhere)
-    float x[kVectors][N];
+    const bool tokens = r.tokens != nullptr, biases = r.bias_ids != nullptr, copies = out != in || r.allowed != nullptr;
+    uint4 x[kVectors];
+    if (copies)
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int64_t i = first + (v * THREADS + tid) * N;
-        if (i >= 0 && i + N <= A.vocab) Pack<T>::load(in + i, x[v]);
-        else {
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[v][e] = i + e >= 0 && i + e < A.vocab ? as_float(in[i + e]) : 0.0f;
+        for (int v = 0; v < kVectors; ++v) {
+            const int64_t i = first + (v * THREADS + tid) * N;
+            x[v] = i >= 0 && i + N <= A.vocab ? *reinterpret_cast<const uint4*>(in + i) : make_uint4(0u, 0u, 0u, 0u);
         }
-    }
-    auto clear = [&] {
-#pragma unroll
-        for (int i = 0; i < kEntries; i += 4 * THREADS) *reinterpret_cast<uint4*>(word_s + i + 4 * tid) = make_uint4(0u, 0u, 0u, 0u);
-        __syncthreads();
-    };
-    // a list's ids that lie in the stretch
-    auto scan = [&](const int64_t* ids, int2 list, auto&& take) {
-        for (int i0 = list.x; i0 < list.y; i0 += 4 * THREADS) {
-            int64_t id[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) { const int i = i0 + u * THREADS + tid; id[u] = i < list.y && i >= i0 ? ids[i] : -1; }
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (id[u] >= 0 && id[u] < A.vocab && id[u] >= first && id[u] < first + kEntries) take((int)(id[u] - first), i0 + u * THREADS + tid);
-        }
-        __syncthreads();
-    };
-    auto each = [&](auto&& f) {
-#pragma unroll
-        for (int v = 0; v < kVectors; ++v)
-#pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const uint4 w = *reinterpret_cast<const uint4*>(word_s + (v * THREADS + tid) * N + e);
-                if ((w.x | w.y | w.z | w.w) == 0u) continue;
-                if (w.x) f(x[v][e], w.x);
-                if (w.y) f(x[v][e + 1], w.y);
-                if (w.z) f(x[v][e + 2], w.z);
-                if (w.w) f(x[v][e + 3], w.w);
-            }
-    };
-    if (r.tokens != nullptr) {
-        const int2 list = list_of(settled(r.cu_tokens), row, r.num_tokens);
-        const int given = r.prompt_lens ? max(0, settled(r.prompt_lens)[row]) : 0;
-        const float rep = r.repetition ? settled(r.repetition)[row] : 1.0f, freq = r.frequency ? settled(r.frequency)[row] : 0.0f, pres = r.presence ? settled(r.presence)[row] : 0.0f;
-        clear();
-        scan(settled(r.tokens), list, [&](int at, int i) {
-            if (i - list.x < given) atomicOr(word_s + at, 0x80000000u);
-            else atomicAdd(word_s + at, 1u);
-        });
-        each([&](float& y, uint32_t w) {
-            if (rep != 1.0f) y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-            const uint32_t said = w & 0x7fffffffu;
-            if (said) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)said)), pres);
-        });
-    }
-    if (r.bias_ids != nullptr) {
-        const int2 list = list_of(settled(r.cu_bias), row, r.num_bias);
-        const float* const bias = settled(r.bias);
-        __syncthreads();                                 // (the counts have been read)
-        clear();
-        scan(settled(r.bias_ids), list, [&](int at, int i) { atomicMax(word_s + at, (uint32_t)i + 1u); });
-        each([&](float& y, uint32_t w) { y = __fadd_rn(y, bias[w - 1u]); });
-    }
+    const int2 said = tokens ? list_of(settled(r.cu_tokens), row, r.num_tokens) : make_int2(0, 0), given = biases ? list_of(settled(r.cu_bias), row, r.num_bias) : make_int2(0, 0);
+    int m = -1;
     if (r.allowed != nullptr) {
-        int m = r.allowed_rows ? settled(r.allowed_rows)[row] : row;
+        m = r.allowed_rows ? settled(r.allowed_rows)[row] : row;
         if (m >= r.num_masks) {
             if (tid == 0 && blockIdx.x == 0) atomicOr(&g_fault, kListFault);
             m = -1;
         }
-        if (m >= 0) {
-            const uint32_t* const mask = reinterpret_cast<const uint32_t*>(settled(r.allowed)) + m * r.mask_stride;
-            const int last_word = (A.vocab - 1) >> 5;
+    }
+    const uint32_t* const mask = m >= 0 ? reinterpret_cast<const uint32_t*>(settled(r.allowed)) + m * r.mask_stride : nullptr;
+    const int prompt = tokens && r.prompt_lens ? max(0, settled(r.prompt_lens)[row]) : 0;
+    const float rep = tokens && r.repetition ? settled(r.repetition)[row] : 1.0f, freq = tokens && r.frequency ? settled(r.frequency)[row] : 0.0f,
+                pres = tokens && r.presence ? settled(r.presence)[row] : 0.0f;
+    const float* const bias = settled(r.bias);
+    auto copy = [&] {
 #pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                const int64_t i = first + (v * THREADS + tid) * N;
-                if (i + N <= 0 || i >= A.vocab) continue;
+        for (int v = 0; v < kVectors; ++v) {
+            const int64_t i = first + (v * THREADS + tid) * N;
+            if (i + N <= 0 || i >= A.vocab) continue;
+            uint32_t bits = 0xffffffffu;
+            if (mask != nullptr) {
                 const int w = (int)(i >> 5);             // (a vector that begins before the row: word -1, which is not read)
-                const uint32_t lo = w >= 0 ? mask[w] : 0u, hi = ((i + N - 1) >> 5) > w && w < last_word ? mask[w + 1] : 0u;
-                const uint32_t bits = __funnelshift_r(lo, hi, (uint32_t)(i & 31));
+                const uint32_t lo = w >= 0 ? mask[w] : 0u, hi = ((i + N - 1) >> 5) > w && w < (A.vocab - 1) >> 5 ? mask[w + 1] : 0u;
+                bits = __funnelshift_r(lo, hi, (uint32_t)(i & 31));
+            }
+            if (i >= 0 && i + N <= A.vocab) {
+                const uint4 y = masked<T>(x[v], bits);
+                if (!apart) *reinterpret_cast<uint4*>(out + i) = y;
+                else {
 #pragma unroll
+                    for (int e = 0; e < N; ++e) out[i + e] = reinterpret_cast<const T*>(&y)[e];
+                }
+            } else {
                 for (int e = 0; e < N; ++e)
-                    if (!((bits >> e) & 1u)) x[v][e] = -INFINITY;
+                    if (i + e >= 0 && i + e < A.vocab) {
+                        if (bits >> e & 1u) out[i + e] = in[i + e];
+                        else put(out + i + e, -INFINITY);
+                    }
             }
         }
-    }
+    };
+    if (!tokens && !biases) { copy(); return; }
+    const bool wide = said.y - said.x > kNarrowTokens || given.y - given.x > kNarrowBiases;
+    const int part = wide ? kEntries / 2 : kEntries;
+    const Counters had{counters, wide}, last{counters + (tokens ? 2 * kEntries : 0), wide};
+    {
+#pragma unroll 1
+        for (int64_t from = first; from < first + kEntries && from < A.vocab; from += part) {
+            // a list's ids that lie in the part
+            auto scan = [&](const int64_t* ids, int2 list, auto&& take) {
+                for (int64_t i0 = list.x; i0 < list.y; i0 += 4 * THREADS) {
+                    int64_t id[4];
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        const int64_t i = first + (v * THREADS + tid) * N;
-        if (!apart && i >= 0 && i + N <= A.vocab) Pack<T>::store(out + i, x[v]);
-        else {
+                    for (int u = 0; u < 4; ++u) { const int64_t i = i0 + u * THREADS + tid; id[u] = i < list.y ? ids[i] : -1; }
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (i + e >= 0 && i + e < A.vocab) put(out + i + e, x[v][e]);
+                    for (int u = 0; u < 4; ++u)
+                        if (id[u] >= 0 && id[u] < A.vocab && id[u] >= from && id[u] < from + part) take(id[u], (int)(i0 + u * THREADS) + tid);
+                }
+            };
+            if (from != first) __syncthreads();
+            for (int i = 16 * tid; i < (tokens + biases) * 2 * kEntries; i += 16 * THREADS) *reinterpret_cast<uint4*>(counters + i) = make_uint4(0u, 0u, 0u, 0u);
+            __syncthreads();
+            scan(settled(r.tokens), said, [&](int64_t id, int i) {
+                const bool was_given = i - said.x < prompt;
+                had.put((int)(id - from), was_given ? had.given() : 1u, !was_given);
+            });
+            scan(settled(r.bias_ids), given, [&](int64_t id, int i) { last.most((int)(id - from), (uint32_t)(i - given.x) + 1u); });
+            if (copies && from == first) copy();
+            __syncthreads();
+            auto write = [&](int64_t id, uint32_t word, uint32_t place) {
+                if (mask != nullptr && !(mask[id >> 5] >> (id & 31) & 1u)) return;
+                float y = as_float(in[id]);
+                if (word) {
+                    if (rep != 1.0f) y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                    const uint32_t n = word & (had.taken() - 1u);
+                    if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)n)), pres);
+                }
+                if (place) y = __fadd_rn(y, bias[given.x + (int)place - 1]);
+                put(out + id, y);
+            };
+            scan(settled(r.tokens), said, [&](int64_t id, int) {
+                const uint32_t word = had.put((int)(id - from), had.taken(), false);
+                if (!(word & had.taken())) write(id, word, biases ? last.get((int)(id - from)) : 0u);
+            });
+            scan(settled(r.bias_ids), given, [&](int64_t id, int i) {
+                const uint32_t place = (uint32_t)(i - given.x) + 1u;
+                if (last.get((int)(id - from)) == place && (!tokens || had.get((int)(id - from)) == 0u)) write(id, 0u, place);
+            });
         }
     }
 }
 
 template <typename T, int THREADS>
 int run_adjust(const LogitArgs& a, cudaStream_t st) {
-    constexpr int kEntries = THREADS * kVectors * Pack<T>::N, kSmem = kEntries * 4;
+    constexpr int kEntries = THREADS * kVectors * kPack<T>, kMostSmem = kEntries * 4;
     auto* const kernel = adjust_logits_kernel<T, THREADS>;
-    if (kSmem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    const int64_t stretches = ((int64_t)a.vocab + Pack<T>::N - 1 + kEntries - 1) / kEntries;          // (a row may begin N - 1 entries into its first vector)
-    const bool lists = a.r.tokens != nullptr || a.r.bias_ids != nullptr;
-    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)stretches, (unsigned)a.batch), THREADS, lists ? kSmem : 0, st, true, a));
+    if (kMostSmem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
+    const int64_t stretches = ((int64_t)a.vocab + kPack<T> - 1 + kEntries - 1) / kEntries;          // (a row may begin N - 1 entries into its first vector)
+    const int lists = (a.r.tokens != nullptr) + (a.r.bias_ids != nullptr);
+    KIVI_CUDA_OK(launch(kernel, dim3((unsigned)stretches, (unsigned)a.batch), THREADS, (size_t)lists * 2 * kEntries, st, true, a));
     return KIVI_OK;
 }
 
-// Threads of a CTA: as many as still leave two CTAs to an SM.
-template <typename T> int stretch_threads(const LogitArgs& a) {
-    int threads = 512;
-    while (threads > 128 && (int64_t)a.batch * ((a.vocab + threads * kVectors * Pack<T>::N - 1) / (threads * kVectors * Pack<T>::N)) < 2 * num_sms()) threads /= 2;
-    return threads;
-}
+// Threads of a CTA: 256 where that leaves two CTAs to an SM, else 128.
 template <typename T> int adjust(const LogitArgs& a, cudaStream_t st) {
-    const int threads = stretch_threads<T>(a);
-    return threads == 512 ? run_adjust<T, 512>(a, st) : threads == 256 ? run_adjust<T, 256>(a, st) : run_adjust<T, 128>(a, st);
+    constexpr int kEntries = 512 * kVectors * kPack<T>;
+    return (int64_t)a.batch * ((a.vocab + kEntries - 1) / kEntries) >= 2 * num_sms() ? run_adjust<T, 512>(a, st) : run_adjust<T, 128>(a, st);
 }
 
 }  // namespace
@@ -233,6 +251,7 @@ extern "C" int kivi_adjust_logits(const void* logits, int dtype, int batch, int 
     KIVI_REQUIRE(rules->tokens == nullptr || (rules->cu_tokens != nullptr && rules->num_tokens >= 0), "tokens need cu_tokens");
     KIVI_REQUIRE(rules->tokens != nullptr || (!rules->prompt_lens && !rules->repetition && !rules->frequency && !rules->presence), "penalties need tokens");
     KIVI_REQUIRE(rules->bias_ids == nullptr || (rules->bias != nullptr && rules->cu_bias != nullptr && rules->num_bias >= 0), "bias_ids need bias and cu_bias");
+    KIVI_REQUIRE(rules->num_tokens < (1 << 30), "tokens holds %d ids, 2^30 or more", rules->num_tokens);
     KIVI_REQUIRE(rules->allowed != nullptr || rules->allowed_rows == nullptr, "allowed_rows need allowed");
     if (rules->allowed != nullptr) {
         KIVI_REQUIRE(rules->mask_stride >= ((int64_t)vocab + 31) / 32, "a mask of %lld words does not hold %d bits", (long long)rules->mask_stride, vocab);
