@@ -48,6 +48,30 @@ class Rows(_c.Structure):
     _fields_ = [("data", _vp), ("row_stride", _i64), ("head_stride", _i64)]
 
 
+class Paged8Layer(_c.Structure):
+    """struct kivi_paged8_layer of include/kivi_cuda.h."""
+    _fields_ = [(n, _c.c_int32) for n in ("num_pages", "page_tokens", "num_kv_heads", "head_dim", "group_size", "residual_cap",
+                                          "num_slots", "res_dtype")] + \
+               [(n, _vp) for n in ("k_codes", "k_scales", "v_codes", "v_scales", "k_res", "v_res")]
+
+
+class Rotary(_c.Structure):
+    """struct kivi_rotary of include/kivi_cuda.h."""
+    _fields_ = [("table", _vp), ("rows", _c.c_int32), ("dim", _c.c_int32), ("interleaved", _c.c_int32), ("num_axes", _c.c_int32), ("positions", _vp),
+                ("pair_axis", _vp)]
+
+
+class ScoreRules(_c.Structure):
+    """struct kivi_score_rules of include/kivi_cuda.h."""
+    _fields_ = [("softcap", _f), ("window", _c.c_int32), ("slopes", _vp), ("prefix", _vp)]
+
+
+class LogitRules(_c.Structure):
+    """struct kivi_logit_rules of include/kivi_cuda.h."""
+    _fields_ = [(n, _vp) for n in ("tokens", "cu_tokens", "prompt_lens", "repetition", "frequency", "presence", "bias_ids", "bias", "cu_bias", "allowed",
+                                   "allowed_rows")] + [(n, _c.c_int32) for n in ("num_tokens", "num_bias", "num_masks")] + [("mask_stride", _i64)]
+
+
 PEER_MAX_WORLD = 8
 
 
@@ -102,6 +126,13 @@ SIGNATURES = {
     "kivi_paged_attention": (_int, [_c.POINTER(PagedLayer), _c.POINTER(PagedBatch), _c.POINTER(Rows), _int, _c.POINTER(Rows), _c.POINTER(Rows),
                                     _c.POINTER(Rows), _int, _int, _f, _vp, _c.c_size_t, _vp]),
     "kivi_paged_read": (_int, [_c.POINTER(PagedLayer), _c.POINTER(PagedBatch), _vp, _vp, _vp, _vp]),
+    "kivi_paged8_append": (_int, [_c.POINTER(Paged8Layer), _c.POINTER(PagedBatch), _c.POINTER(Rows), _c.POINTER(Rows), _c.POINTER(Rotary),
+                                  _c.POINTER(Rows), _int, _c.POINTER(Rows), _c.POINTER(Rows), _vp]),
+    "kivi_paged8_attention_workspace": (_c.c_size_t, [_c.POINTER(Paged8Layer), _c.POINTER(PagedBatch), _int, _int, _c.POINTER(ScoreRules)]),
+    "kivi_paged8_attention": (_int, [_c.POINTER(Paged8Layer), _c.POINTER(PagedBatch), _c.POINTER(Rows), _int, _c.POINTER(Rows), _c.POINTER(Rows),
+                                     _c.POINTER(Rows), _int, _int, _f, _c.POINTER(ScoreRules), _vp, _c.c_size_t, _vp]),
+    "kivi_paged8_read": (_int, [_c.POINTER(Paged8Layer), _c.POINTER(PagedBatch), _vp, _vp, _vp, _vp]),
+    "kivi_adjust_logits": (_int, [_vp, _int, _int, _int, _i64, _c.POINTER(LogitRules), _vp, _i64, _vp]),
     "kivi_peer_alloc": (_int, [_c.c_size_t, _c.POINTER(_vp), _c.c_char_p]),
     "kivi_peer_open": (_int, [_c.c_char_p, _c.POINTER(_vp)]),
     "kivi_peer_close": (_int, [_vp]),

@@ -23,6 +23,11 @@ appended stays until its sequence is freed: tokens that a speculative decoder re
 All kernels follow arrays in device memory, so a step can be captured: ``begin(..., max_len=...)`` with the longest
 length it shall reach, and before each replay ``end(batch)`` and ``refresh(batch)``.  A layer's arrays are laid
 out by its first step, which therefore is not a captured one.
+
+``codes="e4m3"`` holds pages in 8 bits, for models that 2 bits are too coarse for: e4m3 numbers with one scale for
+each block of ``group_size`` tokens and head, keys and values apart, four times the bytes.  Windows, lengths and steps are the
+same.  Such a cache also takes positions on several axes (``append``) and what models do to scores
+(``attention``): a cap by tanh, a bias that falls with distance, a sliding window, a prefix that all rows see.
 """
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence, Tuple
@@ -55,17 +60,23 @@ class PagedBatch:
 class PagedKiviCache:
     def __init__(self, num_layers: int, head_dim: int, num_kv_heads: int, num_pages: int, max_sequences: int,
                  page_tokens: int = 256, group_size: int = 32, residual_length: int = 128, dtype=torch.bfloat16,
-                 device: str = "cuda", rounding: str = "half_away"):
+                 device: str = "cuda", rounding: str = "half_away", codes: str = "2bit"):
         G, R, D = group_size, residual_length, head_dim
-        assert D % G == 0, f"head_dim ({D}) must be divisible by group_size ({G})"
-        assert G >= 4 and G % 4 == 0, f"group_size ({G}) must be >= 4 and divisible by 4"
-        assert D <= 256 and (D <= 64 or D % 64 == 0), f"head_dim ({D}) must be <= 64 or a multiple of 64 up to 256"
+        assert codes in ("2bit", "e4m3"), f"codes ({codes!r}) must be '2bit' or 'e4m3'"
+        if codes == "2bit":
+            assert D % G == 0, f"head_dim ({D}) must be divisible by group_size ({G})"
+            assert G >= 4 and G % 4 == 0, f"group_size ({G}) must be >= 4 and divisible by 4"
+            assert D <= 256 and (D <= 64 or D % 64 == 0), f"head_dim ({D}) must be <= 64 or a multiple of 64 up to 256"
+        else:
+            assert 16 <= G <= 256 and G % 16 == 0, f"group_size ({G}) must be a multiple of 16 up to 256"
+            assert 16 <= D <= 256 and D % 16 == 0, f"head_dim ({D}) must be a multiple of 16 up to 256"
+            assert rounding == "half_away", "rounding is of 2-bit codes: e4m3 numbers round to even"
         assert G <= R, f"group_size ({G}) must not exceed residual_length ({R})"
         assert page_tokens > 0 and page_tokens % G == 0, f"page_tokens ({page_tokens}) must be a multiple of group_size ({G})"
         assert num_pages >= 0 and max_sequences > 0 and num_kv_heads > 0
         assert dtype in (torch.bfloat16, torch.float32)
         assert rounding in ("half_away", "half_even")
-        self.num_layers, self.head_dim, self.num_kv_heads = num_layers, D, num_kv_heads
+        self.num_layers, self.head_dim, self.num_kv_heads, self.codes = num_layers, D, num_kv_heads, codes
         self.G, self.R, self.page_tokens, self.dtype = G, R, page_tokens, dtype
         self.num_pages, self.max_sequences = num_pages, max_sequences
         self.device = torch.device(device)
@@ -135,6 +146,10 @@ class PagedKiviCache:
                 raise RuntimeError(f"layer {i} is used for the first time in a captured step: run a step outside first")
             P, H, D, G, R, T = max(1, self.num_pages), self.num_kv_heads, self.head_dim, self.G, self.R, self.page_tokens
             z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype, device=self.device)  # noqa: E731
+            if self.codes == "e4m3":
+                self._layers[i] = (z(P, H, T, D, dtype=torch.uint8), z(P, H, T // G), z(P, H, T, D, dtype=torch.uint8), z(P, H, T // G),
+                                   z(self.max_sequences, H, R, D, dtype=self.dtype), z(self.max_sequences, H, R, D, dtype=self.dtype))
+                return self._layers[i]
             self._layers[i] = (z(P, H, T // G, D * G // 4, dtype=torch.uint8), z(P, H, T // G, D), z(P, H, T // G, D),
                                z(P, H, T, D // 4, dtype=torch.uint8), z(P, H, T, D // G), z(P, H, T, D // G),
                                z(self.max_sequences, H, R, D, dtype=self.dtype), z(self.max_sequences, H, R, D, dtype=self.dtype))
@@ -184,35 +199,57 @@ class PagedKiviCache:
         return batch
 
     def append(self, layer: int, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, rotary: Optional[torch.Tensor] = None,
-               q: Optional[torch.Tensor] = None, interleaved: bool = False):
+               q: Optional[torch.Tensor] = None, interleaved: bool = False, positions: Optional[torch.Tensor] = None,
+               pair_axis: Optional[torch.Tensor] = None):
         """Append the step's keys and values [rows, H, D] (of the cache's dtype).  With ``rotary`` [positions, rotary_dim]
         (fp32: cosines, then sines) keys and queries are turned to their positions first; returns (q, k) as the
-        attention wants them.  Once per layer and step: window slots that it has read are written again."""
+        attention wants them.  Once per layer and step: window slots that it has read are written again.
+
+        ``positions`` int32 [axes, rows] and ``pair_axis`` int32 [rotary_dim / 2] (``codes="e4m3"``): pair i of a token is
+        turned by its position on axis ``pair_axis[i]`` in place of its place in the sequence (images and video: time, height,
+        width)."""
         assert batch.open, "the step has ended"
         q_out = k_out = None
         if rotary is not None:
             k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
             q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        kivi_native.paged_append(k, v, *self._layer(layer), batch.page_table, batch.slots, batch.seq_lens, batch.cu_new, batch.max_new, batch.max_len,
-                                 self.G, rotary, q if rotary is not None else None, q_out, k_out, interleaved, self.rounding)
+        where = (batch.page_table, batch.slots, batch.seq_lens, batch.cu_new, batch.max_new, batch.max_len, self.G)
+        turned = q if rotary is not None else None
+        if self.codes == "e4m3":
+            kivi_native.paged8_append(k, v, *self._layer(layer), *where, rotary, turned, q_out, k_out, interleaved, positions, pair_axis)
+        else:
+            if positions is not None or pair_axis is not None:
+                raise ValueError("positions on several axes need codes='e4m3'")
+            kivi_native.paged_append(k, v, *self._layer(layer), *where, rotary, turned, q_out, k_out, interleaved, self.rounding)
         return (q, k) if rotary is None else (q_out, k_out)
 
     def attention(self, layer: int, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float = 0.0,
-                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  out: Optional[torch.Tensor] = None, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, window: int = 0,
+                  prefix: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of the step's rows, after ``append`` of the same step: [rows, Hq, D].  q, k: as ``append``
-        returned them."""
+        returned them.
+
+        With ``codes="e4m3"``, x a score: ``softcap`` > 0: x becomes softcap * tanh(x / softcap); ``slopes`` fp32 [Hq]: then x gets
+        slopes[head] * (place of the token - place of the row); ``window`` > 0: a row sees the last ``window`` tokens up to its
+        own; ``prefix`` int32 [sequences of the batch]: and the sequence's first ``prefix`` tokens, those behind it too."""
         assert batch.open, "the step has ended"
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        kivi_native.paged_attention(q, k, v, *self._layer(layer), batch.page_table, batch.slots, batch.seq_lens, batch.cu_new, batch.max_new, batch.max_len,
-                                    out, self.G, sm_scale)
+        where = (batch.page_table, batch.slots, batch.seq_lens, batch.cu_new, batch.max_new, batch.max_len)
+        if self.codes == "e4m3":
+            kivi_native.paged8_attention(q, k, v, *self._layer(layer), *where, out, self.G, sm_scale, softcap, slopes, window, prefix)
+        else:
+            if softcap or slopes is not None or window or prefix is not None:
+                raise ValueError("softcap, slopes, window and prefix need codes='e4m3'")
+            kivi_native.paged_attention(q, k, v, *self._layer(layer), *where, out, self.G, sm_scale)
         return out
 
     def step(self, layer: int, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rotary: Optional[torch.Tensor] = None,
-             sm_scale: float = 0.0, interleaved: bool = False) -> torch.Tensor:
-        """``append`` and ``attention`` of one layer."""
-        q, k = self.append(layer, batch, k, v, rotary, q, interleaved)
-        return self.attention(layer, batch, q, k, v, sm_scale)
+             sm_scale: float = 0.0, interleaved: bool = False, positions: Optional[torch.Tensor] = None, pair_axis: Optional[torch.Tensor] = None,
+             **rules) -> torch.Tensor:
+        """``append`` and ``attention`` of one layer (``rules``: softcap, slopes, window, prefix)."""
+        q, k = self.append(layer, batch, k, v, rotary, q, interleaved, positions, pair_axis)
+        return self.attention(layer, batch, q, k, v, sm_scale, **rules)
 
     def end(self, batch: PagedBatch) -> None:
         """The step is done in all layers: its tokens are the sequences' own."""
@@ -252,8 +289,9 @@ class PagedKiviCache:
         if stop > start:
             dev = lambda x: torch.tensor(x, dtype=torch.int32).to(self.device)  # noqa: E731
             width = max(1, len(self._pages[seq]))
-            kivi_native.paged_read(*self._layer(layer), self._table([seq], width).to(self.device), dev([seq]), dev([held]), dev([start]), dev([0, stop - start]),
-                                   stop - start, k, v, self.G)
+            read = kivi_native.paged8_read if self.codes == "e4m3" else kivi_native.paged_read
+            read(*self._layer(layer), self._table([seq], width).to(self.device), dev([seq]), dev([held]), dev([start]), dev([0, stop - start]),
+                 stop - start, k, v, self.G)
         return k, v
 
     def check_device_fault(self) -> None:
@@ -267,5 +305,5 @@ class PagedKiviCache:
             raise RuntimeError(f"kivi_cuda device fault word = {word}; outputs since the last check may be wrong")
 
     def __repr__(self):
-        return (f"PagedKiviCache(layers={self.num_layers}, head_dim={self.head_dim}, G={self.G}, R={self.R}, "
+        return (f"PagedKiviCache(layers={self.num_layers}, head_dim={self.head_dim}, codes={self.codes}, G={self.G}, R={self.R}, "
                 f"pages={self.num_pages - len(self._free_pages)}/{self.num_pages} of {self.page_tokens}, sequences={len(self._lens)})")

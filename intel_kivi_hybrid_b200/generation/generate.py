@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from ..cache.manager import KiviCache
+from .logits import LogitRules
 from .sampling import sample_token
 
 __all__ = ["generate"]
@@ -40,13 +41,29 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
              residual_length: int = 128, device: str = "cuda", temperature: float = 1.0,
              top_k: Optional[int] = None, do_sample: bool = False, verbose: bool = False,
              fused_attention: bool = False, top_p: float = 1.0, min_p: float = 0.0,
-             prefill_chunk: Optional[int] = None) -> str:
+             prefill_chunk: Optional[int] = None, repetition_penalty: float = 1.0, frequency_penalty: float = 0.0,
+             presence_penalty: float = 0.0, logit_bias=None, allowed=None) -> str:
     """The reference's arguments, and: ``fused_attention`` (below), ``top_p`` / ``min_p`` (cuts of the draw, see
     ``sampling.sample_token``), ``prefill_chunk`` (with ``fused_attention``: the prompt goes through the model in
-    pieces of that many tokens, each attending to the packed cache, so that no forward is longer)."""
+    pieces of that many tokens, each attending to the packed cache, so that no forward is longer), and penalties, biases
+    and masks on the logits before the choice (``repetition_penalty``, ``frequency_penalty``, ``presence_penalty``,
+    ``logit_bias``, ``allowed``: see ``logits.LogitRules``)."""
     if prefill_chunk is not None and (not fused_attention or prefill_chunk < 1):
         raise ValueError("prefill_chunk needs fused_attention=True and at least one token")
-    pick = partial(sample_token, temperature=temperature, top_k=top_k, do_sample=do_sample, top_p=top_p, min_p=min_p)
+    choose = partial(sample_token, temperature=temperature, top_k=top_k, do_sample=do_sample, top_p=top_p, min_p=min_p)
+    ruled = (repetition_penalty, frequency_penalty, presence_penalty) != (1.0, 0.0, 0.0) or logit_bias or allowed is not None
+    rules = None
+
+    def pick(logits, input_ids):
+        nonlocal rules
+        if not ruled:
+            return choose(logits)
+        if rules is None:
+            rules = LogitRules(input_ids, max_new_tokens, logits.device, repetition_penalty, frequency_penalty, presence_penalty, logit_bias, allowed)
+        ids = choose(rules(logits))
+        rules.said(ids)
+        return ids
+
     if fused_attention:
         return _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residual_length, device, pick, verbose, prefill_chunk)
     cache = KiviCache.from_model(model, device=device, group_size=group_size, residual_length=residual_length)
@@ -56,7 +73,7 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
 
     out = model(input_ids, use_cache=True)                                   # prefill
     cache.add_tokens(out.past_key_values)
-    next_id = pick(out.logits[:, -1, :])
+    next_id = pick(out.logits[:, -1, :], input_ids)
     produced = [next_id]
     eos_id = tokenizer.eos_token_id
 
@@ -71,7 +88,7 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
                 break
         out = model(next_id, past_key_values=cache.get_full_cache(), use_cache=True)
         cache.add_tokens(out.past_key_values)
-        next_id = pick(out.logits[:, -1, :]).to(model_device)
+        next_id = pick(out.logits[:, -1, :], input_ids).to(model_device)
         produced.append(next_id)
         if verbose and (step + 1) % 10 == 0:
             print(".", end="", flush=True)
@@ -98,7 +115,7 @@ def _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residu
     with attached(model, cache, chunked=prefill_chunk is not None) as past:
         for piece in input_ids.split(prefill_chunk or input_ids.shape[1], dim=1):
             out = model(piece, past_key_values=past, use_cache=True)
-        next_id = pick(out.logits[:, -1, :])
+        next_id = pick(out.logits[:, -1, :], input_ids)
         produced = [next_id]
         checked = 0
         for step in range(1, max_new_tokens):
@@ -109,7 +126,7 @@ def _generate_fused(model, tokenizer, prompt, max_new_tokens, group_size, residu
                     del produced[stop + 1:]
                     break
             out = model(next_id, past_key_values=past, use_cache=True)
-            next_id = pick(out.logits[:, -1, :]).to(model_device)
+            next_id = pick(out.logits[:, -1, :], input_ids).to(model_device)
             produced.append(next_id)
             if verbose and (step + 1) % 10 == 0:
                 print(".", end="", flush=True)
