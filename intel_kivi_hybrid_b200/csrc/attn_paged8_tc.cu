@@ -9,11 +9,12 @@
 //   0-3, 4-7   a thread per row of the first / second block, which holds the 128 scores of a
 //              tile in registers (184, taken from the other warps: setmaxnreg): maximum, weights,
 //              running sum, rescaling, output
-//   8-11       values of a tile of pages become fp16 numbers in shared memory; tiles of the
+//   8-11       values of a tile of pages become fp16 numbers in shared memory; those of the
 //              window and the new tokens are brought as they are
 //   12         one thread issues the MMAs: S of a block while the other block's weights are
 //              made; P comes from tensor memory, where it takes the place of S
 //   13         one thread brings the bytes of the pages to shared memory with bulk copies
+//   14, 15     keys of the window and the new tokens, as they are
 //
 // Keys of a page are operands as they lie: S is two MMAs of kind f8f6f4, a row of Q less a
 // power of two being the sum of two e4m3 numbers (a bf16 number is, as far as 2^-9 of the
@@ -38,7 +39,7 @@ __device__ int g_fault = 0;
 constexpr int kN = 128;                                  // tokens of a tile
 constexpr int kM = 128;                                  // rows of a block
 constexpr int kG = 32;                                   // tokens that share their scales
-constexpr int kThreads = 512, kStageWarp = 8, kMmaWarp = 12, kCopyWarp = 13;
+constexpr int kThreads = 512, kStageWarp = 8, kMmaWarp = 12, kCopyWarp = 13, kKeyWarp = 14;
 constexpr int kRing = 8;                                 // scales of so many tiles are kept
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 constexpr float kHeadroom = 8.0f, kSlack = 6.0f;         // products of weight and scale: up to 2^8, or 2^14 before their reference moves
@@ -235,7 +236,7 @@ paged8_tc_kernel(Paged8Attn A) {
             const bool capped = RULES && A.rules.softcap > 0.0f;
             const float cap = A.rules.softcap * kLog2e, slope = RULES && A.rules.slopes && there ? A.rules.slopes[head] * kLog2e : 0.0f;
             const float to_x = capped ? A.scale / A.rules.softcap : A.scale * kLog2e;
-            float m = -INFINITY, ref = -1.0e30f, l = 0.0f;   // ref: the largest maximum plus value scale, so far
+            float m = -INFINITY, ref = -1.0e30f, l = 0.0f, base_m = 0.0f, up = 0.0f;         // ref: the largest maximum plus value scale, so far; up: from weights times scales to O's
             bool ok = true;
             for (int j = 0; j < n_tiles; ++j) {
                 // (given up: on to the end without waiting)
@@ -280,14 +281,17 @@ paged8_tc_kernel(Paged8Attn A) {
                         }
                     }
                     if (A.rules.slopes != nullptr) {
-                        const float start = slope * (float)(t0 - place);
 #pragma unroll
-                        for (int g = 0; g < 4; ++g)
+                        for (int g = 0; g < 4; ++g) {
+                            const float start = slope * (float)(t0 + kG * g - place);
+                            float2 b = make_float2(start, start + slope);
+                            const float2 on = both(2.0f * slope);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const float2 b = fma2(both(slope), make_float2((float)(kG * g + i), (float)(kG * g + i + 1)), both(start));
                                 put2(g, i, capped ? add2(at2(g, i), b) : fma2(at2(g, i), both(c[g]), b));
+                                b = add2(b, on);
                             }
+                        }
                     }
                     if (capped || A.rules.slopes != nullptr) c[0] = c[1] = c[2] = c[3] = 1.0f;
                 }
@@ -314,31 +318,33 @@ paged8_tc_kernel(Paged8Attn A) {
                     top[g] = fmaxf(a, b) * c[g];
                 }
                 const float top_all = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                if (top_all > m + kGrowth) {             // (from -inf: whenever there is a maximum)
-                    l *= m == -INFINITY ? 0.0f : ex2(m - top_all);
-                    m = top_all;
-                }
-                // a value scale's power of two, rounded up
-                float most = -INFINITY;
+                float most = -INFINITY;                  // with the value scales' powers of two, rounded up
 #pragma unroll
                 for (int g = 0; g < 4; ++g) most = fmaxf(most, top[g] + (float)((int)(__float_as_uint(lift[g]) >> 23) - 126));
-                const bool grows = most > ref + kSlack;
-                if (__any_sync(0xffffffffu, grows)) {
-                    const float f = grows ? ex2(ref - most) : 1.0f;
-                    if (grows) ref = most;
-                    if (j > 0) {
+                if (__any_sync(0xffffffffu, top_all > m + kGrowth || most > ref + kSlack)) {
+                    if (top_all > m + kGrowth) {         // (from -inf: whenever there is a maximum)
+                        l *= m == -INFINITY ? 0.0f : ex2(m - top_all);
+                        m = top_all;
+                        base_m = m;
+                    }
+                    const bool grows = most > ref + kSlack;
+                    if (__any_sync(0xffffffffu, grows)) {
+                        const float f = grows ? ex2(ref - most) : 1.0f;
+                        if (grows) ref = most;
+                        if (j > 0) {
 #pragma unroll 1
-                        for (int x = 0; x < D; x += 16) {
-                            uint32_t o[16];
-                            tmem_load16(o_at + x, o);
-                            tmem_wait_load();
+                            for (int x = 0; x < D; x += 16) {
+                                uint32_t o[16];
+                                tmem_load16(o_at + x, o);
+                                tmem_wait_load();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_store16(o_at + x, o);
+                                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_store16(o_at + x, o);
+                            }
                         }
                     }
+                    up = ex2(fminf(base_m - ref + kHeadroom, 126.0f));
                 }
-                const float base_m = m == -INFINITY ? 0.0f : m, up = ex2(fminf(base_m - ref + kHeadroom, 126.0f));
                 float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
@@ -410,12 +416,84 @@ paged8_tc_kernel(Paged8Attn A) {
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        auto scale_at = [&](int tok) {                   // of a token in pages
+            const int64_t unit = (int64_t)page_of(L, q, tok, &g_fault) * H + h;
+            return unit * (L.page_tokens / L.group_size) + tok % L.page_tokens / L.group_size;
+        };
+        // Keys or values of tokens first .. first + 31 to rows at .. of a tile of 64-channel halves, by a warp.
+        auto group_of_rows = [&](bool of_keys, int first, int at, uint32_t to) {
+            constexpr int kPieces = D / 8, kStep = 32 / kPieces;             // 16-byte pieces of a row; rows that a warp takes at a time
+            const int p = lane % kPieces, r0 = lane / kPieces;
+            auto place_of = [&](int r) { return to + (uint32_t)(p >> 3) * (kN * 128) + swizzled(at + r, p & 7); };
+            const kivi_rows& fresh = of_keys ? A.k : A.v;
+            const __nv_bfloat16* const fresh0 = reinterpret_cast<const __nv_bfloat16*>(fresh.data) + (int64_t)q.row0 * fresh.row_stride + (int64_t)h * fresh.head_stride + 8 * p;
+            if (first < inside) {
+                const int64_t unit = (int64_t)page_of(L, q, first, &g_fault) * H + h;
+                const int in_page = first % L.page_tokens;
+                const uint8_t* const codes = (of_keys ? L.k_codes : L.v_codes) + unit * L.page_tokens * D;
+                // (a group that is not all there is rounded, its scale is 1)
+                const float f = first + kG <= inside ? 1.0f : (of_keys ? L.k_scales : L.v_scales)[scale_at(first)];
+#pragma unroll 1
+                for (int r = r0; r < kG && first + r < inside; r += kStep) {
+                    uint32_t b[2] = {0u, 0u}, w[4];
+                    if (of_keys) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(codes + key8_offset(in_page + r, 8 * p, D));
+                        b[0] = x.x; b[1] = x.y;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) b[e >> 2] |= (uint32_t)codes[value8_offset(in_page + r, 8 * p + e, D, 32)] << (8 * (e & 3));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float4 x = e4m3x4(b[e]);
+                        w[2 * e] = pack_bf16(x.x * f, x.y * f); w[2 * e + 1] = pack_bf16(x.z * f, x.w * f);
+                    }
+                    sts128(place_of(r), w[0], w[1], w[2], w[3]);
+                }
+                if (first + kG <= inside) return;
+            }
+            // all of a lane's copies are on their way at once
+            if (first >= q.held && first + kG <= total && A.vec) {
+                const __nv_bfloat16* from = fresh0 + (int64_t)(first - q.held + r0) * fresh.row_stride;
+                const int64_t step = kStep * fresh.row_stride;
+#pragma unroll 4
+                for (int r = r0; r < kG; r += kStep, from += step) copy16(place_of(r), from, true);
+            } else {
+                const __nv_bfloat16* const ring = reinterpret_cast<const __nv_bfloat16*>(of_keys ? L.k_res : L.v_res) + ((int64_t)q.slot * H + h) * R * D + 8 * p;
+#pragma unroll 1
+                for (int r = r0; r < kG; r += kStep) {
+                    const int tok = first + r;
+                    if (tok < inside) continue;
+                    const bool held = tok < q.held, in = tok < total;
+                    const __nv_bfloat16* const from = held ? ring + (int64_t)ring_slot(tok, 0, R) * D : fresh0 + (int64_t)(in ? tok - q.held : 0) * fresh.row_stride;
+                    if (held || A.vec) { copy16(place_of(r), from, in); continue; }
+                    const uint16_t* u = reinterpret_cast<const uint16_t*>(from);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = in ? u[2 * e] | (uint32_t)u[2 * e + 1] << 16 : 0u;
+                    sts128(place_of(r), w[0], w[1], w[2], w[3]);
+                }
+            }
+            copies_wait();
+            if (of_keys) return;
+            // a lane looks its values over
+#pragma unroll 4
+            for (int r = r0; r < kG; r += kStep) {
+                const uint4 x = lds_uint4(place_of(r));
+                uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if ((w[e] & 0x7f80u) == 0x7f80u) { w[e] &= 0xffff0000u; bad = true; }
+                    if ((w[e] & 0x7f800000u) == 0x7f800000u) { w[e] &= 0xffffu; bad = true; }
+                }
+                if (bad) { misc.odd = 1; sts128(place_of(r), w[0], w[1], w[2], w[3]); }
+            }
+        };
         if (warp < kMmaWarp) {
             // ---------------- values; tiles of rows ----------------
             const int i128 = tid & 127, g = warp - kStageWarp;
             auto meet = [&] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-            const __nv_bfloat16* const k_ring = reinterpret_cast<const __nv_bfloat16*>(L.k_res) + ((int64_t)q.slot * H + h) * R * D;
-            const __nv_bfloat16* const v_ring = reinterpret_cast<const __nv_bfloat16*>(L.v_res) + ((int64_t)q.slot * H + h) * R * D;
             bool ok = true;
 #pragma unroll 1
             for (int j = 0; j < n_tiles; ++j) {
@@ -444,92 +522,40 @@ paged8_tc_kernel(Paged8Attn A) {
                     meet();
                     if (i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.v_full[st])); }
                 } else {
-                    if (ok && j >= 2) ok = wait_warp(misc.a_empty[st], (j >> 1) - 1) && wait_warp(misc.v_empty[st], (j >> 1) - 1);
-                    // a warp has a group of 32 tokens: rows of keys to 64-channel halves, values likewise
+                    if (ok && j >= 2) ok = wait_warp(misc.v_empty[st], (j >> 1) - 1);
+                    group_of_rows(false, t0 + kG * g, kG * g, v_at);
+                    fence_async();
+                    meet();
+                    // (its keys' stage is free: the tile before the last has been contracted)
+                    if (i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.v_full[st])); }
+                }
+            }
+        } else if (warp >= kKeyWarp) {
+            // ---------------- keys of tiles of rows, and all their scales ----------------
+            bool ok = true;
+#pragma unroll 1
+            for (int j = 0; j < n_tiles; ++j) {
+                const int st = j & 1, t0 = tile_start(j);
+                // (every phase is waited for in its turn, the pages' tiles' too: a barrier tells a phase from the next one only)
+                if (ok && j >= 2) ok = wait_warp(misc.a_empty[st], (j >> 1) - 1);
+                if (j < n_packed) continue;
+#pragma unroll 1
+                for (int g = 2 * (warp - kKeyWarp); g < 2 * (warp - kKeyWarp) + 2; ++g) {
                     const int first = t0 + kG * g;
-                    float ks = 1.0f, vs = 1.0f;
-                    auto to_at = [&](int r, int p) { return (uint32_t)(p >> 3) * (kN * 128) + swizzled(r, p & 7); };
-                    if (first < inside) {
-                        const int64_t unit = (int64_t)page_of(L, q, first, &g_fault) * H + h;
-                        const int in_page = first % L.page_tokens;
-                        const int64_t f = unit * (L.page_tokens / L.group_size) + in_page / L.group_size;
-                        const bool all = first + kG <= inside;       // (else what is in pages is rounded)
-                        const float kf = all ? 1.0f : L.k_scales[f], vf = all ? 1.0f : L.v_scales[f];
-                        if (all) { ks = L.k_scales[f]; vs = L.v_scales[f]; }
-                        const uint8_t* const kc = L.k_codes + unit * L.page_tokens * D;
-                        const uint8_t* const vc = L.v_codes + unit * L.page_tokens * D;
-#pragma unroll 1
-                        for (int i = lane; i < kG * (D / 8); i += 32) {
-                            const int r = i / (D / 8), p = i % (D / 8);
-                            if (first + r >= inside) continue;
-                            const uint2 kb = *reinterpret_cast<const uint2*>(kc + key8_offset(in_page + r, 8 * p, D));
-                            uint32_t vb[2] = {0u, 0u};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) vb[e >> 2] |= (uint32_t)vc[value8_offset(in_page + r, 8 * p + e, D, 32)] << (8 * (e & 3));
-                            const uint32_t kw[2] = {kb.x, kb.y};
-                            uint32_t k[4], x[4];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float4 a = e4m3x4(kw[e]), b = e4m3x4(vb[e]);
-                                k[2 * e] = pack_bf16(a.x * kf, a.y * kf); k[2 * e + 1] = pack_bf16(a.z * kf, a.w * kf);
-                                x[2 * e] = pack_bf16(b.x * vf, b.y * vf); x[2 * e + 1] = pack_bf16(b.z * vf, b.w * vf);
-                            }
-                            sts128(a_at + to_at(kG * g + r, p), k[0], k[1], k[2], k[3]);
-                            sts128(v_at + to_at(kG * g + r, p), x[0], x[1], x[2], x[3]);
-                        }
-                    }
-                    if (first + kG > inside) {
-                        // all of a lane's copies are on their way at once, and it looks the values over itself
-#pragma unroll 1
-                        for (int i = lane; i < kG * (D / 8); i += 32) {
-                            const int r = i / (D / 8), p = i % (D / 8), tok = first + r;
-                            if (tok < inside) continue;
-                            const bool held = tok < q.held, in = tok < total;
-                            const int64_t slot = held ? (int64_t)ring_slot(tok, 0, R) * D : 0, row = (int64_t)q.row0 + (in ? tok - q.held : 0);
-                            const __nv_bfloat16* const kr = held ? k_ring + slot : reinterpret_cast<const __nv_bfloat16*>(A.k.data) + row * A.k.row_stride + (int64_t)h * A.k.head_stride;
-                            const __nv_bfloat16* const vr = held ? v_ring + slot : reinterpret_cast<const __nv_bfloat16*>(A.v.data) + row * A.v.row_stride + (int64_t)h * A.v.head_stride;
-                            const uint32_t at = to_at(kG * g + r, p);
-                            if (held || A.vec) {
-                                copy16(a_at + at, kr + 8 * p, in);
-                                copy16(v_at + at, vr + 8 * p, in);
-                            } else {
-                                const uint16_t* ku = reinterpret_cast<const uint16_t*>(kr + 8 * p);
-                                const uint16_t* vu = reinterpret_cast<const uint16_t*>(vr + 8 * p);
-                                uint32_t k[4], x[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    k[e] = in ? ku[2 * e] | (uint32_t)ku[2 * e + 1] << 16 : 0u;
-                                    x[e] = in ? vu[2 * e] | (uint32_t)vu[2 * e + 1] << 16 : 0u;
-                                }
-                                sts128(a_at + at, k[0], k[1], k[2], k[3]);
-                                sts128(v_at + at, x[0], x[1], x[2], x[3]);
-                            }
-                        }
-                        copies_wait();
-#pragma unroll 1
-                        for (int i = lane; i < kG * (D / 8); i += 32) {
-                            const int r = i / (D / 8), p = i % (D / 8);
-                            if (first + r < inside) continue;
-                            const uint32_t at = v_at + to_at(kG * g + r, p);
-                            uint4 x = lds_uint4(at);
-                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                            bool bad = false;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                if ((w[e] & 0x7f80u) == 0x7f80u) { w[e] &= 0xffff0000u; bad = true; }
-                                if ((w[e] & 0x7f800000u) == 0x7f800000u) { w[e] &= 0xffffu; bad = true; }
-                            }
-                            if (bad) { misc.odd = 1; sts128(at, w[0], w[1], w[2], w[3]); }
-                        }
-                    }
+                    group_of_rows(true, first, kG * g, base + S::a + st * S::kTile);
                     if (lane == 0) {
+                        float ks = 1.0f, vs = 1.0f;
+                        if (first + kG <= inside) {
+                            const int64_t f = scale_at(first);
+                            ks = L.k_scales[f]; vs = L.v_scales[f];
+                        }
                         reinterpret_cast<float*>(&misc.k_scale[j % kRing])[g] = ks;
                         reinterpret_cast<float*>(&misc.v_scale[j % kRing])[g] = vs;
                     }
-                    fence_async();
-                    meet();
-                    if (i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.k_full[st])); arrive(bar(misc.v_full[st])); }
                 }
+                fence_async();
+                asm volatile("bar.sync 2, 64;" ::: "memory");
+                if (tid == 32 * kKeyWarp) arrive(bar(misc.k_full[st]));
             }
         } else if (warp == kCopyWarp) {
             // ---------------- copies ----------------
