@@ -6,9 +6,8 @@
 // over tiles of 128 tokens, for two blocks of 128 rows at a time ((new token, query head)
 // pairs of one sequence and KV head: all heads of a group share the tile).  Roles of the 16
 // warps:
-//   0-3, 4-7   a thread per row of the first / second block, which holds the 128 scores of a
-//              tile in registers (184, taken from the other warps: setmaxnreg): maximum, weights,
-//              running sum, rescaling, output
+//   0-3, 4-7   a thread per row of the first / second block: maximum, weights, running sum,
+//              rescaling, output
 //   8-11       values of a tile of pages become fp16 numbers in shared memory; those of the
 //              window and the new tokens are brought as they are
 //   12         one thread issues the MMAs: S of a block while the other block's weights are
@@ -31,6 +30,8 @@
 #include "paged8_attention.cuh"
 #include "tcgen05.cuh"
 
+#include <type_traits>
+
 namespace kivi {
 namespace {
 
@@ -43,7 +44,6 @@ constexpr int kThreads = 512, kStageWarp = 8, kMmaWarp = 12, kCopyWarp = 13, kKe
 constexpr int kRing = 8;                                 // scales of so many tiles are kept
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 constexpr float kHeadroom = 8.0f, kSlack = 6.0f;         // products of weight and scale: up to 2^8, or 2^14 before their reference moves
-constexpr int kRowRegs = 184, kOtherRegs = 72;           // 2 x 128 x (184 + 72) = 512 x 128
 
 template <int D> struct Shared {
     static constexpr uint32_t kRow = D == 128 ? 128 : 64;            // bytes of a row of e4m3 operands
@@ -166,7 +166,6 @@ paged8_tc_kernel(Paged8Attn A) {
     auto wait_warp = [&](const uint64_t& b, int phase) { return __all_sync(0xffffffffu, wait(b, phase)) != 0; };
 
     if (warp < kStageWarp) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
         // ---------------- rows ----------------
         const int t = warp >> 2, r = tid & (kM - 1);
         if (t < n_sub) {
@@ -233,6 +232,7 @@ paged8_tc_kernel(Paged8Attn A) {
 
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + t * kN, o_at = tmem + lanes + 2 * kN + t * D;
             constexpr float kLog2e = 1.4426950408889634f;
+            auto factor = [](float scale, float to) { return fmaxf(scale * to, 1.0e-37f); };         // (not 0: hidden columns are -inf)
             const bool capped = RULES && A.rules.softcap > 0.0f;
             const float cap = A.rules.softcap * kLog2e, slope = RULES && A.rules.slopes && there ? A.rules.slopes[head] * kLog2e : 0.0f;
             const float to_x = capped ? A.scale / A.rules.softcap : A.scale * kLog2e;
@@ -244,83 +244,84 @@ paged8_tc_kernel(Paged8Attn A) {
                 fence_after();
                 const int t0 = tile_start(j);
                 const bool packed = j < n_packed;
-                float c[4], lift[4];
-                {
-                    const float4 ks = misc.k_scale[j % kRing], vs = misc.v_scale[j % kRing];
-                    const float f = to_x * (packed ? pow2i(-q_shift) : 1.0f);
-                    c[0] = fmaxf(ks.x * f, 1.0e-37f); c[1] = fmaxf(ks.y * f, 1.0e-37f); c[2] = fmaxf(ks.z * f, 1.0e-37f); c[3] = fmaxf(ks.w * f, 1.0e-37f);      // (not 0: hidden columns are -inf)
-                    lift[0] = vs.x; lift[1] = vs.y; lift[2] = vs.z; lift[3] = vs.w;
-                }
-                uint32_t v[4][32];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) tmem_load32(s_at + kG * g, v[g]);
-                tmem_wait_load();
-                auto at2 = [&](int g, int i) { return make_float2(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])); };
-                auto put2 = [&](int g, int i, float2 x) { v[g][i] = __float_as_uint(x.x); v[g][i + 1] = __float_as_uint(x.y); };
-                if constexpr (RULES) {
-                    if (capped) {
-                        float far = 0.0f;
-#pragma unroll
-                        for (int g = 0; g < 4; ++g)
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                const float2 z = mul2(at2(g, i), both(c[g]));
-                                far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
-                                put2(g, i, z);
-                            }
-                        if (__any_sync(0xffffffffu, far > 0.8f)) {
-#pragma unroll
-                            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[g][i] = __float_as_uint(capped_far(__uint_as_float(v[g][i]), cap));
-                        } else {
-#pragma unroll
-                            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                                for (int i = 0; i < 32; i += 2) put2(g, i, capped_near(at2(g, i), cap));
-                        }
-                    }
-                    if (A.rules.slopes != nullptr) {
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const float start = slope * (float)(t0 + kG * g - place);
-                            float2 b = make_float2(start, start + slope);
-                            const float2 on = both(2.0f * slope);
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                put2(g, i, capped ? add2(at2(g, i), b) : fma2(at2(g, i), both(c[g]), b));
-                                b = add2(b, on);
-                            }
-                        }
-                    }
-                    if (capped || A.rules.slopes != nullptr) c[0] = c[1] = c[2] = c[3] = 1.0f;
-                }
+                const float* const k_scales = reinterpret_cast<const float*>(&misc.k_scale[j % kRing]);
+                const float* const v_scales = reinterpret_cast<const float*>(&misc.v_scale[j % kRing]);
+                const float to_c = to_x * (packed ? pow2i(-q_shift) : 1.0f);
                 // columns that the row sees: below `near`, and lo .. hi
                 const int near = prefix - t0, lo = from - t0, hi = place - t0;
-                if (__any_sync(0xffffffffu, near < kN && (lo > 0 || hi < kN - 1))) {
+                const bool edge = __any_sync(0xffffffffu, near < kN && (lo > 0 || hi < kN - 1));
+                float top_all = -INFINITY, most = -INFINITY;         // most: with the value scales' powers of two, rounded up
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t v[2][32];
+                    tmem_load32(s_at + 64 * half, v[0]);
+                    tmem_load32(s_at + 64 * half + 32, v[1]);
+                    const float c[2] = {factor(k_scales[2 * half], to_c), factor(k_scales[2 * half + 1], to_c)};
+                    tmem_wait_load();
+                    auto at2 = [&](int g, int i) { return make_float2(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])); };
+                    auto put2 = [&](int g, int i, float2 x) { v[g][i] = __float_as_uint(x.x); v[g][i + 1] = __float_as_uint(x.y); };
+                    if constexpr (RULES) {
+                        if (capped) {
+                            float far = 0.0f;
 #pragma unroll
-                    for (int g = 0; g < 4; ++g)
+                            for (int g = 0; g < 2; ++g)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int col = kG * g + i;
-                            if (!(col < near || (col >= lo && col <= hi))) v[g][i] = 0xff800000u;
+                                for (int i = 0; i < 32; i += 2) {
+                                    const float2 z = mul2(at2(g, i), both(c[g]));
+                                    far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
+                                    put2(g, i, z);
+                                }
+                            if (__any_sync(0xffffffffu, far > 0.8f)) {
+#pragma unroll
+                                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) v[g][i] = __float_as_uint(capped_far(__uint_as_float(v[g][i]), cap));
+                            } else {
+#pragma unroll
+                                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                    for (int i = 0; i < 32; i += 2) put2(g, i, capped_near(at2(g, i), cap));
+                            }
                         }
-                }
-                float top[4];
+                        if (A.rules.slopes != nullptr) {
+                            const float2 on = both(2.0f * slope);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    float a = -INFINITY, b = -INFINITY;
+                            for (int g = 0; g < 2; ++g) {
+                                const float start = slope * (float)(t0 + 64 * half + kG * g - place);
+                                float2 b = make_float2(start, start + slope);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        a = fmaxf(a, fmaxf(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])));
-                        b = fmaxf(b, fmaxf(__uint_as_float(v[g][i + 2]), __uint_as_float(v[g][i + 3])));
+                                for (int i = 0; i < 32; i += 2) {
+                                    put2(g, i, capped ? add2(at2(g, i), b) : fma2(at2(g, i), both(c[g]), b));
+                                    b = add2(b, on);
+                                }
+                            }
+                        }
                     }
-                    top[g] = fmaxf(a, b) * c[g];
-                }
-                const float top_all = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                float most = -INFINITY;                  // with the value scales' powers of two, rounded up
+                    if (edge) {
+                        const int a = near - 64 * half, b = lo - 64 * half, e = hi - 64 * half;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) most = fmaxf(most, top[g] + (float)((int)(__float_as_uint(lift[g]) >> 23) - 126));
+                        for (int i = 0; i < 64; ++i)
+                            if (!(i < a || (i >= b && i <= e))) v[i / 32][i % 32] = 0xff800000u;
+                    }
+                    if (RULES || edge)                   // (read again below)
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+#pragma unroll
+                            for (int i = 0; i < 32; i += 16) tmem_store16(s_at + 64 * half + kG * g + i, reinterpret_cast<const uint32_t(&)[16]>(v[g][i]));
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        float x = -INFINITY, y = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            x = fmaxf(x, fmaxf(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])));
+                            y = fmaxf(y, fmaxf(__uint_as_float(v[g][i + 2]), __uint_as_float(v[g][i + 3])));
+                        }
+                        x = fmaxf(x, y) * (RULES ? 1.0f : c[g]);
+                        top_all = fmaxf(top_all, x);
+                        most = fmaxf(most, x + (float)((int)(__float_as_uint(v_scales[2 * half + g]) >> 23) - 126));
+                    }
+                }
+                if (RULES || edge) tmem_wait_store();
                 if (__any_sync(0xffffffffu, top_all > m + kGrowth || most > ref + kSlack)) {
                     if (top_all > m + kGrowth) {         // (from -inf: whenever there is a maximum)
                         l *= m == -INFINITY ? 0.0f : ex2(m - top_all);
@@ -346,24 +347,34 @@ paged8_tc_kernel(Paged8Attn A) {
                     up = ex2(fminf(base_m - ref + kHeadroom, 126.0f));
                 }
                 float2 sum = make_float2(0.0f, 0.0f);
+                auto weights = [&](auto as_half) {
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t v[2][32];
+                        tmem_load32(s_at + 64 * half, v[0]);
+                        tmem_load32(s_at + 64 * half + 32, v[1]);
+                        const float c[2] = {RULES ? 1.0f : factor(k_scales[2 * half], to_c), RULES ? 1.0f : factor(k_scales[2 * half + 1], to_c)};
+                        const float raise[2] = {fminf(v_scales[2 * half] * up, 1.0e37f), fminf(v_scales[2 * half + 1] * up, 1.0e37f)};
+                        tmem_wait_load();
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float raise = fminf(lift[g] * up, 1.0e37f);
-                    uint32_t p[16];
+                        for (int g = 0; g < 2; ++g) {
+                            uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 w = ex2x2(fma2(at2(g, i), both(c[g]), both(-base_m)));
-                        sum = add2(sum, w);
-                        const float2 y = mul2(w, both(raise));
-                        p[i / 2] = packed ? pack_half(y.x, y.y) : pack_bf16(y.x, y.y);
-                    }
-                    tmem_store16(s_at + 16 * g, p);
-                    if (g & 1) {
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 w = ex2x2(fma2(make_float2(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])), both(c[g]), both(-base_m)));
+                                sum = add2(sum, w);
+                                const float2 y = mul2(w, both(raise[g]));
+                                p[i / 2] = decltype(as_half)::value ? pack_half(y.x, y.y) : pack_bf16(y.x, y.y);
+                            }
+                            tmem_store16(s_at + 32 * half + 16 * g, p);
+                        }
                         tmem_wait_store();
                         fence_before();
-                        arrive(bar(misc.p_full[t][g >> 1]));
+                        arrive(bar(misc.p_full[t][half]));
                     }
-                }
+                };
+                if (packed) weights(std::true_type{});
+                else weights(std::false_type{});
                 l += sum.x + sum.y;
                 if (j + 1 == n_packed && j + 1 < n_tiles) {
                     // (S of this tile is there, so Q has been read)
@@ -415,7 +426,6 @@ paged8_tc_kernel(Paged8Attn A) {
             fence_before();
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         auto scale_at = [&](int tok) {                   // of a token in pages
             const int64_t unit = (int64_t)page_of(L, q, tok, &g_fault) * H + h;
             return unit * (L.page_tokens / L.group_size) + tok % L.page_tokens / L.group_size;
@@ -591,65 +601,85 @@ paged8_tc_kernel(Paged8Attn A) {
                 // no copy is under way when the block ends
                 for (int j = max(sent - 2, 0); j < sent; ++j) wait(misc.k_full[j & 1], j >> 1);
             }
-        } else if (warp == kMmaWarp && elect_one()) {
+        } else if (warp == kMmaWarp) {
             // ---------------- MMAs ----------------
+            // The whole warp goes through the steps and one lane issues, with operands that are the same in all lanes and
+            // offsets that are constants: an MMA takes 10 cycles to issue that way, and 130 from a branch of one
+            // lane with descriptors made in a loop (a tile 4300 cycles, 4100 of them for issuing 32 MMAs).
             constexpr uint32_t kF8 = mma_shape(kM, kN, false), kPages = mma_shape(kM, D, false), kBf16 = mma_shape(kM, kN, false, 1u), kRowsV = mma_shape(kM, D, true, 1u);
             constexpr uint32_t kSwizzle = D == 128 ? 2u : 4u;
+            const uint32_t base_u = __shfl_sync(0xffffffffu, base, 0), tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
             auto scores = [&](int t, int j) {
-                const uint32_t q_at = base + S::q + t * S::kTile, k_at = base + S::a + (j & 1) * S::kTile, to = tmem + t * kN;
+                const uint32_t q_at = base_u + S::q + t * S::kTile, k_at = base_u + S::a + (j & 1) * S::kTile, to = tmem_u + t * kN;
                 if (j < n_packed) {
-#pragma unroll 1
-                    for (int i = 0; i < 2 * (D / 32); ++i) {
-                        const uint32_t off = (uint32_t)(i % (D / 32)) * 32u;
-                        mma_f8_ss(to, smem_desc(q_at + (i / (D / 32)) * S::kF8 + off, 16, 8 * S::kRow, kSwizzle), smem_desc(k_at + off, 16, 8 * S::kRow, kSwizzle), kF8, i > 0);
+                    const uint64_t qd = smem_desc(q_at, 16, 8 * S::kRow, kSwizzle), kd = smem_desc(k_at, 16, 8 * S::kRow, kSwizzle);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < 2 * (D / 32); ++i)
+                            mma_f8_ss(to, qd + ((i / (D / 32)) * S::kF8 + (i % (D / 32)) * 32u) / 16u, kd + (i % (D / 32)) * 2u, kF8, i > 0);
+                        mma_commit(bar(misc.s_full[t]));
                     }
                 } else {
-#pragma unroll 1
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t off = (uint32_t)(i / 4) * (kM * 128) + (i % 4) * 32;
-                        mma_ss(to, smem_desc(q_at + off, 16, 1024), smem_desc(k_at + off, 16, 1024), kBf16, i > 0);
+                    const uint64_t qd = smem_desc(q_at, 16, 1024), kd = smem_desc(k_at, 16, 1024);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            const uint32_t off = ((uint32_t)(i / 4) * (kM * 128) + (i % 4) * 32) / 16;
+                            mma_ss(to, qd + off, kd + off, kBf16, i > 0);
+                        }
+                        mma_commit(bar(misc.s_full[t]));
                     }
                 }
-                mma_commit(bar(misc.s_full[t]));
+                __syncwarp();
             };
             // weights of block t of tile j times its values
             auto contract = [&](int t, int j) {
-                const uint32_t v_at = base + S::v + (j & 1) * S::kTile;
+                const uint32_t v_at = base_u + S::v + (j & 1) * S::kTile, to = tmem_u + 2 * kN + t * D, p_at = tmem_u + t * kN;
+                const bool packed = j < n_packed;
+                const uint64_t vd = packed ? smem_desc(v_at, 16, 1024) : smem_desc(v_at, kN * 128, 1024);
+#pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (!wait(misc.p_full[t][half], j)) return false;
+                    if (!wait_warp(misc.p_full[t][half], j)) return false;
                     fence_after();
-#pragma unroll 1
-                    for (int i = 0; i < kN / 32; ++i) {
-                        const uint32_t p_at = tmem + t * kN + 32 * half + 8 * i, to = tmem + 2 * kN + t * D;
-                        const bool add = j > 0 || half > 0 || i > 0;
-                        if (j < n_packed) mma_ts(to, p_at, smem_desc(v_at + half * (D * 128) + i * 32, 16, 1024), kPages, add);
-                        else mma_ts(to, p_at, smem_desc(v_at + (4 * half + i) * 2048, kN * 128, 1024), kRowsV, add);
+                    if (packed) {
+                        if (elect_one()) {
+#pragma unroll
+                            for (int i = 0; i < kN / 32; ++i) mma_ts(to, p_at + 32 * half + 8 * i, vd + (half * (D * 128) + i * 32) / 16, kPages, j > 0 || half > 0 || i > 0);
+                        }
+                    } else if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < kN / 32; ++i) mma_ts(to, p_at + 32 * half + 8 * i, vd + (4 * half + i) * 128, kRowsV, j > 0 || half > 0 || i > 0);
                     }
+                    __syncwarp();
                 }
                 return true;
             };
-            bool ok = wait(misc.q_full, 0) && wait(misc.k_full[0], 0);
+            auto commit = [&](const uint64_t& b) {
+                if (elect_one()) mma_commit(bar(b));
+                __syncwarp();
+            };
+            bool ok = wait_warp(misc.q_full, 0) && wait_warp(misc.k_full[0], 0);
             if (ok) {
                 fence_after();
                 for (int t = 0; t < n_sub; ++t) scores(t, 0);
-                mma_commit(bar(misc.a_empty[0]));
+                commit(misc.a_empty[0]);
                 for (int j = 0; ok && j < n_tiles; ++j) {
                     const int st = j & 1;
                     const bool more = j + 1 < n_tiles, turns = more && j + 1 == n_packed;
-                    if (!wait(misc.v_full[st], j >> 1)) { ok = false; break; }
+                    if (!wait_warp(misc.v_full[st], j >> 1)) { ok = false; break; }
                     for (int t = 0; t < n_sub; ++t) {
                         ok = contract(t, j);
-                        if (t == 0 && more && ok) ok = wait(misc.k_full[st ^ 1], (j + 1) >> 1);
-                        if (turns && ok) ok = wait(misc.q_again[t], 0);
+                        if (t == 0 && more && ok) ok = wait_warp(misc.k_full[st ^ 1], (j + 1) >> 1);
+                        if (turns && ok) ok = wait_warp(misc.q_again[t], 0);
                         if (!ok) break;
                         fence_after();
                         if (more) scores(t, j + 1);
                     }
                     if (!ok) break;
-                    mma_commit(bar(misc.v_empty[st]));
-                    if (more) mma_commit(bar(misc.a_empty[st ^ 1]));
+                    commit(misc.v_empty[st]);
+                    if (more) commit(misc.a_empty[st ^ 1]);
                 }
-                if (ok) mma_commit(bar(misc.o_done));
+                if (ok) commit(misc.o_done);
             }
         }
     }
