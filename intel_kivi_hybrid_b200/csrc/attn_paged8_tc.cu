@@ -60,13 +60,18 @@ struct Misc {                                            // behind the tiles
     uint32_t tmem;
     int place[2];
     int odd;                                             // a value that is not finite has been met
-    float4 k_scale[kRing], v_scale[kRing];               // of tile j's four groups at j % kRing
+    float4 k_scale[kRing], v_scale[kRing];               // of tile j's four groups at j % kRing; values': their log2
 };
 
 __device__ __forceinline__ float2 ex2x2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t y;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+__device__ __forceinline__ float log2_of(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float pow2i(int s) { return __uint_as_float((uint32_t)(127 + max(-126, min(127, s))) << 23); }
@@ -236,7 +241,7 @@ paged8_tc_kernel(Paged8Attn A) {
             const bool capped = RULES && A.rules.softcap > 0.0f;
             const float cap = A.rules.softcap * kLog2e, slope = RULES && A.rules.slopes && there ? A.rules.slopes[head] * kLog2e : 0.0f;
             const float to_x = capped ? A.scale / A.rules.softcap : A.scale * kLog2e;
-            float m = -INFINITY, ref = -1.0e30f, l = 0.0f, base_m = 0.0f, up = 0.0f;         // ref: the largest maximum plus value scale, so far; up: from weights times scales to O's
+            float m = -INFINITY, ref = -1.0e30f, l = 0.0f, base_m = 0.0f, up = 0.0f;         // ref: the largest maximum plus value scale, so far; up: log2 of what brings weights times scales to O's scale
             bool ok = true;
             for (int j = 0; j < n_tiles; ++j) {
                 // (given up: on to the end without waiting)
@@ -250,7 +255,7 @@ paged8_tc_kernel(Paged8Attn A) {
                 // columns that the row sees: below `near`, and lo .. hi
                 const int near = prefix - t0, lo = from - t0, hi = place - t0;
                 const bool edge = __any_sync(0xffffffffu, near < kN && (lo > 0 || hi < kN - 1));
-                float top_all = -INFINITY, most = -INFINITY;         // most: with the value scales' powers of two, rounded up
+                float top_all = -INFINITY, most = -INFINITY;         // most: with the value scales
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     uint32_t v[2][32];
@@ -318,7 +323,7 @@ paged8_tc_kernel(Paged8Attn A) {
                         }
                         x = fmaxf(x, y) * (RULES ? 1.0f : c[g]);
                         top_all = fmaxf(top_all, x);
-                        most = fmaxf(most, x + (float)((int)(__float_as_uint(v_scales[2 * half + g]) >> 23) - 126));
+                        most = fmaxf(most, x + v_scales[2 * half + g]);
                     }
                 }
                 if (RULES || edge) tmem_wait_store();
@@ -344,9 +349,8 @@ paged8_tc_kernel(Paged8Attn A) {
                             }
                         }
                     }
-                    up = ex2(fminf(base_m - ref + kHeadroom, 126.0f));
+                    up = fminf(base_m - ref + kHeadroom, 126.0f);
                 }
-                float2 sum = make_float2(0.0f, 0.0f);
                 auto weights = [&](auto as_half) {
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
@@ -354,18 +358,21 @@ paged8_tc_kernel(Paged8Attn A) {
                         tmem_load32(s_at + 64 * half, v[0]);
                         tmem_load32(s_at + 64 * half + 32, v[1]);
                         const float c[2] = {RULES ? 1.0f : factor(k_scales[2 * half], to_c), RULES ? 1.0f : factor(k_scales[2 * half + 1], to_c)};
-                        const float raise[2] = {fminf(v_scales[2 * half] * up, 1.0e37f), fminf(v_scales[2 * half + 1] * up, 1.0e37f)};
+                        // weights times value scales, on O's scale: 2^(lift) p.  (Below 2^-60 they are 0 as fp16 whatever they are.)
+                        const float lift[2] = {fmaxf(v_scales[2 * half] + up, -60.0f), fmaxf(v_scales[2 * half + 1] + up, -60.0f)};
                         tmem_wait_load();
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             uint32_t p[16];
+                            const float2 off = both(lift[g] - base_m);
+                            float2 part = make_float2(0.0f, 0.0f);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
-                                const float2 w = ex2x2(fma2(make_float2(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])), both(c[g]), both(-base_m)));
-                                sum = add2(sum, w);
-                                const float2 y = mul2(w, both(raise[g]));
-                                p[i / 2] = decltype(as_half)::value ? pack_half(y.x, y.y) : pack_bf16(y.x, y.y);
+                                const float2 w = ex2x2(fma2(make_float2(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])), both(c[g]), off));
+                                part = add2(part, w);
+                                p[i / 2] = decltype(as_half)::value ? pack_half(w.x, w.y) : pack_bf16(w.x, w.y);
                             }
+                            l = fmaf(part.x + part.y, ex2(-lift[g]), l);
                             tmem_store16(s_at + 32 * half + 16 * g, p);
                         }
                         tmem_wait_store();
@@ -375,7 +382,6 @@ paged8_tc_kernel(Paged8Attn A) {
                 };
                 if (packed) weights(std::true_type{});
                 else weights(std::false_type{});
-                l += sum.x + sum.y;
                 if (j + 1 == n_packed && j + 1 < n_tiles) {
                     // (S of this tile is there, so Q has been read)
                     q_as_bf16();
@@ -560,7 +566,7 @@ paged8_tc_kernel(Paged8Attn A) {
                             ks = L.k_scales[f]; vs = L.v_scales[f];
                         }
                         reinterpret_cast<float*>(&misc.k_scale[j % kRing])[g] = ks;
-                        reinterpret_cast<float*>(&misc.v_scale[j % kRing])[g] = vs;
+                        reinterpret_cast<float*>(&misc.v_scale[j % kRing])[g] = log2_of(vs);
                     }
                 }
                 fence_async();
@@ -589,7 +595,7 @@ paged8_tc_kernel(Paged8Attn A) {
                         ks[i] = L.k_scales[f]; vs[i] = L.v_scales[f];
                     }
                     misc.k_scale[j % kRing] = make_float4(ks[0], ks[1], ks[2], ks[3]);
-                    misc.v_scale[j % kRing] = make_float4(vs[0], vs[1], vs[2], vs[3]);
+                    misc.v_scale[j % kRing] = make_float4(log2_of(vs[0]), log2_of(vs[1]), log2_of(vs[2]), log2_of(vs[3]));
                     mbar_expect_tx(b, 2 * kN * D);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
