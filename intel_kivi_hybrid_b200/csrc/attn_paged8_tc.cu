@@ -682,8 +682,11 @@ paged8_tc_kernel(Paged8Attn A) {
                         if (more) scores(t, j + 1);
                     }
                     if (!ok) break;
-                    commit(misc.v_empty[st]);
-                    if (more) commit(misc.a_empty[st ^ 1]);
+                    if (elect_one()) {
+                        mma_commit(bar(misc.v_empty[st]));
+                        if (more) mma_commit(bar(misc.a_empty[st ^ 1]));
+                    }
+                    __syncwarp();
                 }
                 if (ok) commit(misc.o_done);
             }
