@@ -17,7 +17,10 @@
 // runs of tokens (rows of 36 bytes: of 32, eight lanes meet in a bank).
 //
 // Bound by memory: bf16, D = 128, G = 32 moves 2 bytes per element of the rows in and out
-// and 1 per element that leaves.
+// and 1 per element that leaves.  What it takes beyond that is latency, so CTAs an SM count: 4 x 2048 tokens
+// of 8 and 32 heads, three axes, 123 us with the 100 registers that a thread would like, 74 with the 64 that leave room
+// for four CTAs and with a row's angles in shared memory for all of its heads (2 x 5003 fp32: 180, 135 with three).
+// One token of 64 sequences: launch and latency.
 #include <float.h>
 
 #include "paged8.cuh"
@@ -29,6 +32,7 @@ __device__ int g_fault = 0;
 
 constexpr int kThreads = 256;
 constexpr int kTurnUnits = 8;                            // pairs of vectors of queries that a thread turns, about
+constexpr int kMostTurnRows = 8;                         // rows of a CTA, whose angles are in shared memory
 
 struct Append8Args {
     kivi_paged8_layer L;
@@ -185,7 +189,7 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
 
 // ONE: a unit for a thread, whose numbers stay in registers.
 template <typename T, bool VEC, bool ONE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
 paged8_append_kernel(Append8Args A) {
     extern __shared__ __align__(16) uint8_t v_block[];   // [G / run][D][run + 4]
     __shared__ int place_s[2];
@@ -201,7 +205,8 @@ paged8_append_kernel(Append8Args A) {
     if ((int64_t)blockIdx.x >= (int64_t)A.items * H) {
         // ---------------- queries ----------------
         const int row0 = (int)(blockIdx.x - (int64_t)A.items * H) * A.turn_rows, heads = H * A.n_rep;
-        int* const token_s = reinterpret_cast<int*>(v_block);
+        float* const turn_s = reinterpret_cast<float*>(v_block);             // [turn_rows][dim]: a row's cosines and sines, for all its heads
+        __shared__ int token_s[kMostTurnRows];
         if (tid < A.turn_rows) {
             const int row = row0 + tid;
             // the last sequence that starts at or before the row (none of a sequence that is left out)
@@ -216,15 +221,28 @@ paged8_append_kernel(Append8Args A) {
             token_s[tid] = ok ? q.held + (row - q.row0) : -1;
         }
         __syncthreads();
-        for (int i = tid; i < A.turn_rows * heads * units; i += kThreads) {
-            const int u = i % units, head = i / units % heads, r = i / units / heads, t = token_s[r];
+        const int dim = A.rot.dim, half = dim / 2;
+        for (int i = tid; i < A.turn_rows * half; i += kThreads) {
+            const int r = i / half, pair = i % half, t = token_s[r];
             if (t < 0) continue;
+            const float* const at = A.rot.table + (int64_t)(A.rot.positions ? axis_row(A.rot, pair, row0 + r, rows_all) : t) * dim + pair;
+            turn_s[r * dim + pair] = at[0];
+            turn_s[r * dim + half + pair] = at[half];
+        }
+        __syncthreads();
+        kivi_rotary staged = A.rot;                      // (row r of the block's own table)
+        staged.table = turn_s;
+        staged.positions = nullptr;
+#pragma unroll 2
+        for (int i = tid; i < A.turn_rows * heads * units; i += kThreads) {
+            const int u = i % units, head = i / units % heads, r = i / units / heads;
+            if (token_s[r] < 0) continue;
             int d, e;
             float x[8], y[8];
             places(A.rot, u, d, e);
             const T* from = row_of<const T>(A.q, row0 + r, head);
             load8<VEC>(from + d, x); load8<VEC>(from + e, y);
-            turn_unit<T>(A.rot, u, t, row0 + r, rows_all, x, y);
+            turn_unit<T>(staged, u, r, 0, 0, x, y);
             T* to = row_of<T>(A.q_out, row0 + r, head);
             store8<VEC>(to + d, x); store8<VEC>(to + e, y);
         }
@@ -549,13 +567,14 @@ extern "C" int kivi_paged8_append(const kivi_paged8_layer* layer, const kivi_pag
     a.turn_rows = 1;
     if (queries) {
         const int64_t per_row = (int64_t)H * n_rep * units;
-        while (a.turn_rows < 32 && (a.turn_rows + 1) * per_row <= kThreads * kTurnUnits && (int64_t)batch->total_new > (int64_t)a.turn_rows * num_sms()) ++a.turn_rows;
+        while (a.turn_rows < kMostTurnRows && (a.turn_rows + 1) * per_row <= kThreads * kTurnUnits && (int64_t)batch->total_new > (int64_t)a.turn_rows * num_sms()) ++a.turn_rows;
         turn_blocks = ((int64_t)batch->total_new + a.turn_rows - 1) / a.turn_rows;
     }
     KIVI_REQUIRE(items * H + turn_blocks <= 0x7fffffff, "too many blocks in one step");
     a.items = (int)items;
     const int run = value8_run(G);
-    const size_t smem = (size_t)G / run * D * (run + 4);         // (80 KB at the most)
+    size_t smem = (size_t)G / run * D * (run + 4);               // (80 KB at the most)
+    if (queries && smem < (size_t)a.turn_rows * rotary->dim * 4) smem = (size_t)a.turn_rows * rotary->dim * 4;
     auto* const kernel = layer->res_dtype == KIVI_BF16 ? append_kernel<__nv_bfloat16>(vec, G * units <= kThreads) : append_kernel<float>(vec, G * units <= kThreads);
     constexpr int kMostSmem = 256 / 16 * 256 * 20;               // (the limit is the kernel's, not the call's: two calls at once set the same)
     if (smem > 48 * 1024) KIVI_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem));
