@@ -23,8 +23,9 @@
 // scale less the power of two of the largest such product that the row has met, so that neither
 // a row's own range nor what other rows see takes its bits.  Two terms of e4m3 would do for P's bits, not for its range.
 // Window and new tokens are bf16 operands as they are, Q and P then too: Q is written again
-// when the pages are done.  A group of 32 tokens of which some are in pages only is rounded to bf16.  A value that is
-// not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
+// when the pages are done.  Where only some of a group's tokens come from its page, the others' scores are divided by
+// its scale (keys rounded to bf16 instead: 0.0027 off 64 bits where the output's rounding is 0.0017), and its values are rounded
+// to bf16.  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
 //
 // Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle).
 #include "paged8_attention.cuh"
@@ -255,6 +256,22 @@ paged8_tc_kernel(Paged8Attn A) {
                 // columns that the row sees: below `near`, and lo .. hi
                 const int near = prefix - t0, lo = from - t0, hi = place - t0;
                 const bool edge = __any_sync(0xffffffffu, near < kN && (lo > 0 || hi < kN - 1));
+                // a group of which the first columns alone come from its page: the others' scores are divided by its scale
+                const int cut = inside - t0;
+                if (cut > 0 && cut < kN && cut % kG != 0) {
+                    const float inv = 1.0f / k_scales[cut / kG];
+#pragma unroll 1
+                    for (int x = cut / kG * kG; x < cut / kG * kG + kG; x += 16) {
+                        uint32_t o[16];
+                        tmem_load16(s_at + x, o);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (x + i >= cut) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+                        tmem_store16(s_at + x, o);
+                    }
+                    tmem_wait_store();
+                }
                 float top_all = -INFINITY, most = -INFINITY;         // most: with the value scales
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
@@ -447,8 +464,7 @@ paged8_tc_kernel(Paged8Attn A) {
                 const int64_t unit = (int64_t)page_of(L, q, first, &g_fault) * H + h;
                 const int in_page = first % L.page_tokens;
                 const uint8_t* const codes = (of_keys ? L.k_codes : L.v_codes) + unit * L.page_tokens * D;
-                // (a group that is not all there is rounded, its scale is 1)
-                const float f = first + kG <= inside ? 1.0f : (of_keys ? L.k_scales : L.v_scales)[scale_at(first)];
+                const float f = of_keys || first + kG <= inside ? 1.0f : L.v_scales[scale_at(first)];
 #pragma unroll 1
                 for (int r = r0; r < kG && first + r < inside; r += kStep) {
                     uint32_t b[2] = {0u, 0u}, w[4];
@@ -561,9 +577,10 @@ paged8_tc_kernel(Paged8Attn A) {
                     group_of_rows(true, first, kG * g, base + S::a + st * S::kTile);
                     if (lane == 0) {
                         float ks = 1.0f, vs = 1.0f;
-                        if (first + kG <= inside) {
+                        if (first < inside) {
                             const int64_t f = scale_at(first);
-                            ks = L.k_scales[f]; vs = L.v_scales[f];
+                            ks = L.k_scales[f];
+                            if (first + kG <= inside) vs = L.v_scales[f];
                         }
                         reinterpret_cast<float*>(&misc.k_scale[j % kRing])[g] = ks;
                         reinterpret_cast<float*>(&misc.v_scale[j % kRing])[g] = log2_of(vs);
