@@ -1,31 +1,27 @@
-// Attention of a few rows over a paged cache in 8 bits: head_dim 64 and 128, blocks of whole
-// 32 tokens, queries of the window's type.
+// Attention of a few bf16 rows over a paged cache in 8 bits: head_dim 64 and 128, blocks of whole 32 tokens.
 //
 //   S = Q K^T,  P = 2^(rules(S) - m),  O = O + P V,  out = O / sum P
 //
-// by mma.sync m16n8k16, 32 tokens of a page to a warp at a time.  Tokens (and channels of V)
-// are the sixteen rows of an MMA, the (new token, query head) pairs of one sequence and KV head
-// its eight columns, up to twice eight to a unit: with the pairs as rows a single token of four heads took twice
-// the MMAs and the registers (64 ragged sequences up to 32k 555 us).  Weights change places with movmatrix in between.
-// What bounds it is the page's bytes: a tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions
-// and 32 MMAs of a warp (fp32 rows: 64).
-//
-// Work is dealt out evenly whatever the sequences' lengths: the tiles of all (sequence, KV
+// Work is dealt out evenly whatever the sequences' lengths: the 32-token tiles of all (sequence, KV
 // head, block of rows) units lie one after the other, the window and the step's own tokens
 // as a few tiles more, and CTA c has positions c per .. (c + 1) per - 1 of that line,
 // with `per` from the lengths in device memory.  A unit in one CTA is finished there; of the others
 // a CTA has two at most, its first and its last, whose partials it leaves in slots 2c and
 // 2c + 1 for a second kernel.  Nothing depends on the order in which CTAs run.
 //
-// A warp has a ring of stages that bulk copies fill, its lane issues them; the four warps
-// take tiles in turn and meet at a unit's end.
+// By mma.sync m16n8k16, 32 tokens of a page to a warp at a time; tokens (and channels of V) are the sixteen
+// rows of an MMA, the (new token, query head) pairs of one
+// sequence and KV head its eight columns, up to three times eight to a unit: with the pairs as rows a single token of
+// four heads took twice the MMAs and the registers (64 ragged sequences up to 32k 555 us, 384 now).  Weights change places with
+// movmatrix in between.  A tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions and 32 MMAs of a warp,
+// less than its bytes take.  A warp has a ring of stages that bulk copies fill, its first lane issues them; the warps take
+// tiles in turn and meet at a unit's end.
 //
 // Numbers: e4m3 codes are exact as fp16.  A row of bf16 queries is exact as fp16 after a power
-// of two, but for what is below 2^-27 of its largest; fp32 rows are two fp16 numbers (22 bits).  A block's key scale
-// multiplies the scores, its value scale the weights, which are fp16 (bf16 rows: rounded at
-// 2^-12 of themselves, where the output is rounded at 2^-9) or two of them, less the power of
-// two of the largest such product that the row has met.  Window and own tokens are contracted as bf16 numbers, exact for
-// bf16 rows (weights at 2^-9 there: bf16 reaches as far as the values do); fp32 ones as three, the six products that matter.  Sums are fp32.
+// of two, but for what is below 2^-27 of its largest.  A block's key scale multiplies the scores, its value scale the weights,
+// which are fp16 (rounded at 2^-12 of themselves, where the output is rounded at 2^-9), less the power of
+// two of the largest such product that the row has met.  Window and own tokens are contracted as the bf16 numbers they are
+// (weights at 2^-9 there: bf16 reaches as far as the values do).  Sums are fp32.
 #include "async_copy.cuh"
 #include "paged8_attention.cuh"
 
