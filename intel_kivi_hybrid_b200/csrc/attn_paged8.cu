@@ -13,7 +13,7 @@
 //
 // Bound by the FMA pipe with 64 rows (4 x 160 tokens of GPT-2-small over 512 53 us; weights of tokens beside values that are not
 // finite are selected token by token, in all tiles of rows that cost 59), by shared memory with few: bytes loaded a tile ahead into
-// registers changed nothing (16 x 8192 tokens, 4 heads, fp32: 753 us, 792).
+// registers changed nothing (16 x 8192 tokens, 8 x 4 heads, fp32: 753 us, 792; up to four rows of long sequences go elsewhere).
 #include "paged8_attention.cuh"
 
 #include <type_traits>
@@ -353,7 +353,7 @@ int paged8_attention_fault_clear() {
     return KIVI_OK;
 }
 
-bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows);
+bool paged8_decode_serves(const kivi_paged8_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, int window);
 size_t paged8_decode_parts(int64_t max_rows);
 int paged8_decode_notes();
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st);
@@ -369,7 +369,7 @@ struct Paged8Plan { Paged8Kernel kernel; int rows, blocks, pieces, chunk; };
 static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, const kivi_score_rules& rules) {
     Paged8Plan p{};
     const int64_t rows = (int64_t)b->max_new * n_rep;
-    if (paged8_decode_serves(L, q_dtype, rows)) {
+    if (paged8_decode_serves(L, b, q_dtype, n_rep, rules.window)) {
         p.kernel = Paged8Kernel::kDecode;
         p.rows = 1;
         p.blocks = (int)paged8_decode_parts(rows);

@@ -1,4 +1,4 @@
-// Attention of a few bf16 rows over a paged cache in 8 bits: head_dim 64 and 128, blocks of whole 32 tokens.
+// Attention of a few rows over a paged cache in 8 bits, head_dim 64 and 128.
 //
 //   S = Q K^T,  P = 2^(rules(S) - m),  O = O + P V,  out = O / sum P
 //
@@ -9,8 +9,8 @@
 // a CTA has two at most, its first and its last, whose partials it leaves in slots 2c and
 // 2c + 1 for a second kernel.  Nothing depends on the order in which CTAs run.
 //
-// By mma.sync m16n8k16, 32 tokens of a page to a warp at a time; tokens (and channels of V) are the sixteen
-// rows of an MMA, the (new token, query head) pairs of one
+// paged8_decode_kernel: bf16, blocks of whole 32 tokens.  mma.sync m16n8k16, 32 tokens of a page to a warp
+// at a time; tokens (and channels of V) are the sixteen rows of an MMA, the (new token, query head) pairs of one
 // sequence and KV head its eight columns, up to three times eight to a unit: with the pairs as rows a single token of
 // four heads took twice the MMAs and the registers (64 ragged sequences up to 32k 555 us, 384 now).  Weights change places with
 // movmatrix in between.  A tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions and 32 MMAs of a warp,
@@ -22,6 +22,8 @@
 // which are fp16 (rounded at 2^-12 of themselves, where the output is rounded at 2^-9), less the power of
 // two of the largest such product that the row has met.  Window and own tokens are contracted as the bf16 numbers they are
 // (weights at 2^-9 there: bf16 reaches as far as the values do).  Sums are fp32.
+//
+// paged8_lanes_kernel: fp32 and mixed types, and blocks of 16: CUDA cores, fp32 throughout (below).
 #include "async_copy.cuh"
 #include "paged8_attention.cuh"
 
@@ -162,9 +164,9 @@ __device__ __forceinline__ Line find_line(const Paged8Attn& A, int unit_rows, in
     __syncthreads();
     return {total, scratch[kWarps + 1], (int)scratch[kWarps]};
 }
-__host__ __device__ __forceinline__ int64_t per_cta(int64_t cost, int ctas) {
+__host__ __device__ __forceinline__ int64_t per_cta(int64_t cost, int ctas, int least) {
     const int64_t per = (cost + ctas - 1) / ctas;
-    return per < kLeast ? kLeast : per;
+    return per < least ? least : per;
 }
 
 // The CTA's segments, one after the other.  (In shared memory: as registers two of them were 60 of a thread's.)
@@ -240,10 +242,10 @@ paged8_decode_kernel(Paged8Attn A) {
     Walk& walk = *reinterpret_cast<Walk*>(smem + S::walks);                 // what is computed
     Walk& ahead = (&walk)[1 + warp];                                         // what the warp copies: its first lane's
     int* const note = A.notes + kNote * (int)blockIdx.x;
-    const Line line = find_line<kWarps>(A, kRows, reinterpret_cast<int64_t*>(smem + S::scratch), walk.w, [&](int64_t cost) { return per_cta(cost, gridDim.x) * blockIdx.x; });
+    const Line line = find_line<kWarps>(A, kRows, reinterpret_cast<int64_t*>(smem + S::scratch), walk.w, [&](int64_t cost) { return per_cta(cost, gridDim.x, kLeast) * blockIdx.x; });
     if (tid == 0) note[0] = 0;                           // (nothing of this CTA's is to be folded, so far)
     if (line.first < 0) return;
-    const int64_t per = per_cta(line.cost, gridDim.x);
+    const int64_t per = per_cta(line.cost, gridDim.x, kLeast);
     if (tid == 0) {
         walk.s = line.first; walk.off = line.before;
         walk.at = per * blockIdx.x; walk.end = min(walk.at + per, line.cost);
@@ -741,6 +743,321 @@ paged8_decode_kernel(Paged8Attn A) {
         for (int i = 0; i < 2; ++i) mbar_wait(bars + 16 * (taken % kStages) + 8 * i, (uint32_t)(taken / kStages) & 1u);
 }
 
+// ---- up to four rows on the CUDA cores ---------------------------------------------------------
+// The same line of work for long sequences that the tensor cores do not take: fp32 rows (an MMA truncates what it adds: 1.1e-6 off
+// 64 bits where fp32 sums are 3e-7), mixed types, blocks of 16 tokens.  A lane has sixteen channels of a
+// token's key, a warp reads 512 bytes in a row, a token's lanes add up their parts.  Of the values a lane has sixteen tokens
+// of a channel; the two lanes of a channel add up at a unit's end.  Keys of the next tile are on their way while values are weighed,
+// and the other way round, 4 KB of each a warp.  A row or two to a unit: with four, queries, sums and bytes do not
+// fit into 255 registers (16 x 8192 tokens, 8 x 4 heads of 128, fp32: 489 us, 450 as two units of two that find the bytes in L2).
+// Bound by issue: 16 bytes are 16 FMAs a row and 12 conversions (28 x 14650 tokens, 4 heads, fp32: 278 us for 431 MB, 1.55 TB/s; the general
+// kernel 1090).
+constexpr int kLaneWarps = 4;
+template <int D, int NR> struct LaneLayout {
+    static constexpr int kO = D + 4;                     // floats of a row
+    static constexpr int p = 0, q = p + kLaneWarps * NR * 32 * 4, fold = q + NR * kO * 4, ml = fold + kLaneWarps * NR * kO * 4, scratch = ml + kLaneWarps * NR * 8;
+    static constexpr int walks = scratch + (kLaneWarps + 2) * 8, bytes = walks + (int)sizeof(Walk);
+};
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(32 * kLaneWarps, 2)
+paged8_lanes_kernel(Paged8Attn A) {
+    using S = LaneLayout<D, NR>;
+    constexpr int kWarps = kLaneWarps, kThreads = 32 * kWarps, kPieces = D / 16, kSteps = D / 16, kTokens = 32 / kPieces;      // tokens of a step's keys
+    __shared__ __align__(16) uint8_t smem[S::bytes];
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    stream_order();
+    settle_args(A);
+    cudaTriggerProgrammaticLaunchCompletion();           // (the fold's few blocks wait for this kernel's end)
+    const kivi_paged8_layer& L = A.L;
+    const int G = L.group_size, R = L.residual_cap, H = L.num_kv_heads, n_rep = A.n_rep, window = A.rules.window, run = value8_run(G);
+    if (blockIdx.x == 0) report_left_out(L, A.b, &g_fault);
+    float* const p_s = reinterpret_cast<float*>(smem + S::p) + warp * NR * 32;           // [row][place of a token among the value bytes]
+    float* const q_s = reinterpret_cast<float*>(smem + S::q);
+    float* const fold_s = reinterpret_cast<float*>(smem + S::fold);
+    float2* const ml_s = reinterpret_cast<float2*>(smem + S::ml);
+    Walk& walk = *reinterpret_cast<Walk*>(smem + S::walks);
+    int* const note = A.notes + kNote * (int)blockIdx.x;
+    const Line line = find_line<kWarps>(A, NR, reinterpret_cast<int64_t*>(smem + S::scratch), walk.w, [&](int64_t cost) { return per_cta(cost, gridDim.x, kWarps) * blockIdx.x; });
+    if (tid == 0) note[0] = 0;                           // (nothing of this CTA's is to be folded, so far)
+    if (line.first < 0) return;
+    const int64_t per = per_cta(line.cost, gridDim.x, kWarps);
+    if (tid == 0) {
+        walk.s = line.first; walk.off = line.before;
+        walk.at = per * blockIdx.x; walk.end = min(walk.at + per, line.cost);
+    }
+    // a lane's part of a tile: channels 16 piece .. of tokens kTokens i + first_token; sixteen tokens of channels 16 i + channel
+    const int piece = lane % kPieces, first_token = lane / kPieces;
+    const int part = run == 32 ? lane & 1 : lane >> 4, channel = run == 32 ? lane >> 1 : lane & 15;
+    const bool capped = A.rules.softcap > 0.0f;
+    constexpr float kLog2e = 1.4426950408889634f;
+
+    for (;;) {
+        __syncthreads();                                 // (the unit before is folded)
+        if (tid == 0 && !walk.next(A, NR)) walk.h = -1;
+        __syncthreads();
+        if (walk.h < 0) break;
+        const PagedSeq q = walk.w.q;
+        const int h = walk.h, row_first = walk.rb * NR, n_rows = min(NR, walk.w.rows - row_first), inside = walk.w.inside, prefix = walk.w.prefix, total = walk.w.total;
+        const Span span = walk.w.span;
+        const int v_end = walk.tiles_end(), v_begin = walk.a;
+        const bool has_tail = walk.has_tail();
+        for (int i = tid; i < NR * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row_first + r;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < n_rows) x = load4_as(A.q, A.q_dtype, (int64_t)q.row0 + row / n_rep, h * n_rep + row % n_rep, d, A.vec != 0);
+            *reinterpret_cast<float4*>(q_s + r * S::kO + d) = x;
+        }
+        __syncthreads();
+        int place[NR], from[NR];
+        float slope[NR], m[NR], l[NR], o[NR][kSteps];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const int row = row_first + r;
+            // (a row that is not there sees what the first one sees, and is not written)
+            place[r] = q.held + (r < n_rows ? row : row_first) / n_rep;
+            from[r] = window_from(place[r], window);
+            slope[r] = A.rules.slopes && r < n_rows ? A.rules.slopes[h * n_rep + row % n_rep] : 0.0f;
+            m[r] = -INFINITY; l[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) o[r][i] = 0.0f;
+        }
+        // a contracted score as the rules leave it
+        auto ruled = [&](float x, int r, int tok) {
+            x *= A.scale;
+            if (capped) x = A.rules.softcap * tanhf(x / A.rules.softcap);
+            return fmaf(slope[r], (float)(tok - place[r]), x);
+        };
+        auto hidden = [&](int tok, int r) { return tok >= total || ((tok > place[r] || tok < from[r]) && tok >= prefix); };
+        auto move = [&](int r, float top) {              // to a larger maximum; what that leaves of the sums so far
+            if (top <= m[r]) return 1.0f;
+            const float f = m[r] == -INFINITY ? 0.0f : exp2f((m[r] - top) * kLog2e);
+            m[r] = top;
+            l[r] *= f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) o[r][i] *= f;
+            return f;
+        };
+
+        // ---- tiles of pages
+        float2 scale_next[2];
+        auto look_up = [&](int v) {                      // the scales of a tile's sixteens (pages and blocks are whole sixteens)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = span.tile(v) * kTile + 16 * i;
+                scale_next[i] = make_float2(0.0f, 0.0f);
+                if (t >= inside) continue;
+                const int64_t f = ((int64_t)page_of(L, q, t, &g_fault) * H + h) * (L.page_tokens / G) + t % L.page_tokens / G;
+                scale_next[i] = make_float2(L.k_scales[f], L.v_scales[f]);
+            }
+        };
+        uint4 kx[kSteps], vx[kSteps];
+        float2 scale[2];
+        auto load_tile = [&](int v, bool of_keys) {
+            const int t0 = span.tile(v) * kTile;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                // keys: token kTokens i + first_token; values: the run that has the lane's part
+                const int t = of_keys ? t0 + kTokens * i + first_token : t0 + (run == 32 ? 0 : 16 * part);
+                const int sixteen = t & ~15;
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (sixteen < inside) {
+                    const int64_t base = ((int64_t)page_of(L, q, sixteen, &g_fault) * H + h) * L.page_tokens * D;
+                    const int in_page = t % L.page_tokens;
+                    x = of_keys ? *reinterpret_cast<const uint4*>(L.k_codes + base + key8_offset(in_page, 16 * piece, D))
+                                : *reinterpret_cast<const uint4*>(L.v_codes + base + (int64_t)in_page * D + (16 * i + channel) * run + (run == 32 ? 16 * part : 0));
+                }
+                (of_keys ? kx : vx)[i] = x;
+            }
+        };
+        int v = v_begin + warp;
+        if (v < v_end) { load_tile(v, true); load_tile(v, false); look_up(v); }
+        for (; v < v_end; v += kWarps) {
+            const int t0 = span.tile(v) * kTile;
+            scale[0] = scale_next[0]; scale[1] = scale_next[1];
+            float x[NR][kSteps];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const uint32_t w[4] = {kx[i].x, kx[i].y, kx[i].z, kx[i].w};
+                float k[16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 y = e4m3x4(w[e]);
+                    k[4 * e] = y.x; k[4 * e + 1] = y.y; k[4 * e + 2] = y.z; k[4 * e + 3] = y.w;
+                }
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 y = *reinterpret_cast<const float4*>(q_s + r * S::kO + 16 * piece + e);
+                        sum = fmaf(k[e], y.x, fmaf(k[e + 1], y.y, fmaf(k[e + 2], y.z, fmaf(k[e + 3], y.w, sum))));
+                    }
+                    x[r][i] = sum;
+                }
+            }
+            if (v + kWarps < v_end) { load_tile(v + kWarps, true); look_up(v + kWarps); }
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+                    for (int b = 1; b < kPieces; b *= 2) x[r][i] += __shfl_xor_sync(0xffffffffu, x[r][i], b);
+                    const int u = kTokens * i + first_token, tok = t0 + u;
+                    x[r][i] = ruled(x[r][i] * (u < 16 ? scale[0].x : scale[1].x), r, tok);
+                    if (tok >= inside || (tok < from[r] && tok >= prefix)) x[r][i] = -INFINITY;      // (a page's tokens come before every row)
+                    top = fmaxf(top, x[r][i]);
+                }
+#pragma unroll
+                for (int b = kPieces; b < 32; b *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+                move(r, top);
+                const float base = m[r] == -INFINITY ? 0.0f : m[r];
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const int u = kTokens * i + first_token;
+                    const float p = exp2f((x[r][i] - base) * kLog2e);
+                    if (piece == 0) {
+                        l[r] += p;
+                        p_s[r * 32 + (run == 32 ? value8_place(u, 32) : (u & 16) + value8_place(u & 15, 16))] = p;
+                    }
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                float w[16];
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(p_s + r * 32 + 16 * part + e);
+                    w[e] = y.x; w[e + 1] = y.y; w[e + 2] = y.z; w[e + 3] = y.w;
+                }
+                const float by = run == 32 ? scale[0].y : part ? scale[1].y : scale[0].y;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    const uint32_t c[4] = {vx[i].x, vx[i].y, vx[i].z, vx[i].w};
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 y = e4m3x4(c[e]);
+                        sum = fmaf(w[4 * e], y.x, fmaf(w[4 * e + 1], y.y, fmaf(w[4 * e + 2], y.z, fmaf(w[4 * e + 3], y.w, sum))));
+                    }
+                    o[r][i] = fmaf(sum, by, o[r][i]);
+                }
+            }
+            if (v + kWarps < v_end) load_tile(v + kWarps, false);
+            __syncwarp();                                // (weights have been read)
+        }
+
+        // ---- the window and the step's own tokens, eight at a time: a lane has D / 32 channels of each
+        float l_tail[NR], o_tail[NR][D / 32];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            l_tail[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) o_tail[r][c] = 0.0f;
+        }
+        if (has_tail) {
+            constexpr int kC = D / 32, kAt = 8;
+            const T* const k_ring = reinterpret_cast<const T*>(L.k_res) + ((int64_t)q.slot * H + h) * R * D;
+            const T* const v_ring = reinterpret_cast<const T*>(L.v_res) + ((int64_t)q.slot * H + h) * R * D;
+            auto row_at = [&](int tok, bool of_keys) -> const T* {
+                if (tok < q.held) return (of_keys ? k_ring : v_ring) + (int64_t)ring_slot(tok, 0, R) * D;
+                const kivi_rows& r = of_keys ? A.k : A.v;
+                return reinterpret_cast<const T*>(r.data) + ((int64_t)q.row0 + min(tok, total - 1) - q.held) * r.row_stride + (int64_t)h * r.head_stride;
+            };
+            for (int t0 = inside + kAt * warp; t0 < total; t0 += kAt * kWarps) {
+                float k[kAt][kC], y[kAt][kC];
+#pragma unroll
+                for (int j = 0; j < kAt; ++j) {
+                    const T* const kr = row_at(t0 + j, true) + lane;
+                    const T* const vr = row_at(t0 + j, false) + lane;
+#pragma unroll
+                    for (int c = 0; c < kC; ++c) { k[j][c] = (float)kr[32 * c]; y[j][c] = (float)vr[32 * c]; }
+                }
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float x[kAt], top = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < kAt; ++j) {
+                        x[j] = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < kC; ++c) x[j] = fmaf(k[j][c], q_s[r * S::kO + 32 * c + lane], x[j]);
+#pragma unroll
+                        for (int b = 1; b < 32; b *= 2) x[j] += __shfl_xor_sync(0xffffffffu, x[j], b);
+                        x[j] = hidden(t0 + j, r) ? -INFINITY : ruled(x[j], r, t0 + j);
+                        top = fmaxf(top, x[j]);
+                    }
+                    const float f = move(r, top), base = m[r] == -INFINITY ? 0.0f : m[r];
+                    l_tail[r] *= f;
+#pragma unroll
+                    for (int c = 0; c < kC; ++c) o_tail[r][c] *= f;
+#pragma unroll
+                    for (int j = 0; j < kAt; ++j) {
+                        const float p = exp2f((x[j] - base) * kLog2e);
+                        l_tail[r] += p;
+                        // (a token that the row does not see may hold anything, infinities and NaN too)
+                        const bool seen = !hidden(t0 + j, r);
+#pragma unroll
+                        for (int c = 0; c < kC; ++c) o_tail[r][c] = fmaf(p, seen ? y[j][c] : 0.0f, o_tail[r][c]);
+                    }
+                }
+            }
+        }
+
+        // ---- the warps meet: each leaves its rows, all of them add up
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int b = kPieces; b < 32; b *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], b);
+            l[r] = __shfl_sync(0xffffffffu, l[r], 0) + l_tail[r];
+            float* const mine = fold_s + (warp * NR + r) * S::kO;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], run == 32 ? 1 : 16);
+                if (part == 0) mine[16 * i + channel] = o[r][i];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) mine[32 * c + lane] += o_tail[r][c];
+            if (lane == 0) ml_s[warp * NR + r] = make_float2(m[r] * kLog2e, l[r]);          // (partials: in powers of two)
+        }
+        __syncthreads();
+        // the CTAs that have something of the unit
+        const int64_t c0 = walk.unit / per, c1 = (walk.unit + walk.w.tiles) / per;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (c0 == (int64_t)blockIdx.x ? 1 : 0);
+        if (tid == 0 && c0 != c1 && c0 == (int64_t)blockIdx.x) {
+            note[1] = q.row0; note[2] = h; note[3] = row_first; note[4] = n_rows;
+            note[0] = (int)(c1 - c0);
+        }
+        for (int i = tid; i < n_rows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = 4 * (i % (D / 4)), row = row_first + r;
+            float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_s[w * NR + r].x);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 ml = ml_s[w * NR + r];
+                const float4 y = *reinterpret_cast<const float4*>(fold_s + (w * NR + r) * S::kO + d);
+                const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+                if (ml.x == -INFINITY && ml.y == 0.0f) continue;      // (nothing of it is seen)
+                sum = fmaf(f, ml.y, sum);
+                a.x = fmaf(f, y.x, a.x); a.y = fmaf(f, y.y, a.y); a.z = fmaf(f, y.z, a.z); a.w = fmaf(f, y.w, a.w);
+            }
+            if (c0 == c1) {
+                const float inv = 1.0f / sum;            // (a row sees itself: the sum is above 0)
+                const int64_t at = ((int64_t)q.row0 + row / n_rep) * A.out.row_stride + (int64_t)(h * n_rep + row % n_rep) * A.out.head_stride;
+                store_quad(A.out.data, A.out_dtype, at + d, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+            } else {
+                const int64_t partial = slot * NR + r;
+                if (d == 0) *reinterpret_cast<float2*>(A.part_ml + 2 * partial) = make_float2(M, sum);
+                *reinterpret_cast<float4*>(A.part_o + partial * D + d) = a;
+            }
+        }
+    }
+}
+
 // Folds the units that lie across a CTA's end: block c the one that CTA c has left a note of.  A thread has a quad
 // of channels of a row.
 __global__ void __launch_bounds__(128)
@@ -774,7 +1091,7 @@ paged8_fold_kernel(Paged8Attn A, int unit_rows) {
     }
 }
 
-constexpr int kMostBlocks = 3, kMostRows = 64;
+constexpr int kMostBlocks = 3, kMostRows = 64, kLaneRows = 2, kMostLaneRows = 4;
 
 // Blocks of eight rows of a unit: all of a sequence's rows in one unit where registers hold them, so that its bytes are
 // read once.
@@ -801,13 +1118,37 @@ int go(const Paged8Attn& a, cudaStream_t st) {
 
 }  // namespace
 
-bool paged8_decode_serves(const kivi_paged8_layer* L, int q_dtype, int64_t max_rows) {
-    return (L->head_dim == 64 || L->head_dim == 128) && L->group_size % kTile == 0 && q_dtype == KIVI_BF16 && L->res_dtype == KIVI_BF16 && max_rows <= kMostRows;
+static bool on_tensor_cores(const kivi_paged8_layer* L, int q_dtype) { return L->group_size % kTile == 0 && q_dtype == KIVI_BF16 && L->res_dtype == KIVI_BF16; }
+bool paged8_decode_serves(const kivi_paged8_layer* L, const kivi_paged_batch* b, int q_dtype, int n_rep, int window) {
+    if (L->head_dim != 64 && L->head_dim != 128) return false;
+    const int64_t rows = (int64_t)b->max_new * n_rep;
+    if (on_tensor_cores(L, q_dtype)) return rows <= kMostRows;
+    // Lanes: fp32, 16 sequences of 8192 tokens, 8 heads of 128: 241 us against 790 of the general kernel for two rows, 450 against 790 for four (4
+    // heads, eight rows: 452 against 347); one sequence of 2048, 12 heads of 64: 31 against 34; four of 712 29 against 26 (a second
+    // launch); four of 2048 with four rows 66 against 60.
+    const int len = window > 0 && window < b->max_len ? window : b->max_len;
+    return rows <= kMostLaneRows && len >= (rows <= kLaneRows ? 2048 : 4096);
 }
 int paged8_decode_notes() { return kPerSm * num_sms() * kNote; }           // whole numbers behind the partials
 size_t paged8_decode_parts(int64_t max_rows) { return (size_t)kPerSm * num_sms() * 2 * 8 * unit_blocks(max_rows); }          // rows of partials
 
+namespace {
+template <typename T, int D, int NR> int go_lanes(const Paged8Attn& a, cudaStream_t st) {
+    const int ctas = kPerSm * num_sms();
+    KIVI_CUDA_OK(launch(paged8_lanes_kernel<T, D, NR>, dim3((unsigned)ctas), 32 * kLaneWarps, 0, st, true, a));
+    KIVI_CUDA_OK(launch(paged8_fold_kernel, dim3((unsigned)(ctas - 1)), 128, 0, st, true, a, NR));
+    return KIVI_OK;
+}
+template <typename T, int D> int go_lanes(const Paged8Attn& a, cudaStream_t st) {
+    return (int64_t)a.b.max_new * a.n_rep == 1 ? go_lanes<T, D, 1>(a, st) : go_lanes<T, D, kLaneRows>(a, st);
+}
+}  // namespace
+
 int run_paged8_decode(const Paged8Attn& a, cudaStream_t st) {
+    if (!on_tensor_cores(&a.L, a.q_dtype)) {
+        if (a.L.res_dtype == KIVI_F32) return a.L.head_dim == 64 ? go_lanes<float, 64>(a, st) : go_lanes<float, 128>(a, st);
+        return a.L.head_dim == 64 ? go_lanes<__nv_bfloat16, 64>(a, st) : go_lanes<__nv_bfloat16, 128>(a, st);
+    }
     const int nb = unit_blocks((int64_t)a.b.max_new * a.n_rep);
     if (a.L.head_dim == 64) return nb == 1 ? go<64, 1>(a, st) : nb == 2 ? go<64, 2>(a, st) : go<64, 3>(a, st);
     return nb == 1 ? go<128, 1>(a, st) : nb == 2 ? go<128, 2>(a, st) : go<128, 3>(a, st);

@@ -642,3 +642,101 @@ def test_the_2_bit_cache_refuses_what_it_does_not_have():
         cache.step(0, batch, q, k, k, rotary=torch.ones(4, 64, device=DEV), positions=ones, pair_axis=ones)
     with pytest.raises(ValueError, match="e4m3"):
         cache.attention(0, batch, q, k, k, window=3)
+
+
+# ---- up to four rows over long sequences, fp32 and mixed types: a kernel of their own from 2048 tokens on -----------
+LONG = [  # D, G, R, page, H, n_rep, q type, cache type, held, new
+    (64, 32, 128, 128, 3, 1, F32, F32, [2500, 0, 1, 712], [1, 1, 1, 0]),
+    (128, 32, 128, 64, 2, 2, F32, F32, [4200, 33, 2047, 160], [1, 1, 1, 1]),
+    (128, 96, 96, 96, 1, 2, F32, F32, [4333, 95, 0], [2, 1, 2]),
+    (64, 16, 16, 48, 2, 2, BF, BF, [2100, 15, 47], [1, 1, 0]),
+    (128, 16, 40, 16, 1, 4, BF, BF, [4111, 100], [1, 1]),
+    (128, 32, 128, 256, 2, 1, F32, BF, [4100, 31], [3, 4]),
+    (64, 64, 64, 64, 1, 3, BF, F32, [4500, 62, 63], [1, 1, 1]),
+]
+
+
+@pytest.mark.parametrize("rules", RULES + [{"window": 2600, "prefix": 40}], ids=lambda r: "-".join(f"{k}{v}" for k, v in r.items()) or "plain")
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(str(x).replace("torch.", "").replace(" ", "") for x in c))
+def test_attention_of_few_rows_over_long_sequences(ops, case, rules):
+    D, G, R, page, H, n_rep, q_dtype, dtype, before, news = case
+    pool = Pool(len(news), H, D, G, R, page, max(b + n for b, n in zip(before, news)), dtype)
+    k, v = rows(sum(before), H, D, dtype, 1), rows(sum(before), H, D, dtype, 2)
+    k[..., 7] *= 5
+    pool.append(ops, k, v, before)
+    n = sum(news)
+
+    def off(x):                                             # heads first, an element off the 16-byte grid
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape[1], x.shape[0], D).transpose(0, 1)
+        return y.copy_(x)
+    k, v, q = (rows(n, heads, D, t, s) for heads, t, s in ((H, dtype, 3), (H, dtype, 4), (H * n_rep, q_dtype, 5)))
+    if D == 64:
+        k, v, q = off(k), off(v), off(q)
+    a = pool.append(ops, k, v, news)
+    slopes = torch.tensor([2.0 ** -(i % 8 + 1) for i in range(H * n_rep)], device=DEV) if rules.get("slopes") else None
+    prefix = [max(0, rules["prefix"] - 3 * s) for s in range(len(news))] if "prefix" in rules else None
+    got = attend(ops, pool, q, k, v, a, softcap=rules.get("cap", 0.0), slopes=slopes, window=rules.get("window", 0),
+                 prefix=None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device=DEV))
+    want, size, S = reference(pool, q, news, rules.get("cap", 0.0), slopes, rules.get("window", 0), prefix)
+    close(got, want, size, tolerance(q_dtype, S))
+
+
+@pytest.mark.parametrize("n_rep", [1, 2])
+def test_few_rows_may_hide_anything_and_their_faults_are_reported(ops, n_rep):
+    """A NaN and an infinity in the window that rows of a shorter window do not see, a page that is not there, a sequence whose window is not there."""
+    D, w = 128, 2048
+    pool = Pool(2, 1, D, 32, 2400, 64, 5000, F32)
+    pool.append(ops, rows(5000 - 2, 1, D, F32, 1), rows(5000 - 2, 1, D, F32, 2), [4000, 998])
+    k, v, q = rows(2, 1, D, F32, 3), rows(2, 1, D, F32, 4), rows(2, n_rep, D, F32, 5)
+    a = pool.append(ops, k, v, [1, 1])
+    want, size, S = reference(pool, q, [1, 1], window=w)
+    slot, bad = int(pool.slots[0]), 4000 - 2100             # held in the window of 2400, outside the 2048 that the row sees
+    pool.t[4][slot, 0, bad % 2400, 5] = float("nan")
+    pool.t[5][slot, 0, bad % 2400, 9] = float("inf")
+    close(attend(ops, pool, q, k, v, a, window=w), want, size, tolerance(F32, S))
+    assert fault_word() == 0
+    b = list(a)
+    b[0] = a[0].clone()
+    b[0][0, 1] = 10 ** 6
+    attend(ops, pool, q, k, v, b)
+    assert fault_word() == 4
+    b = list(a)
+    b[1] = a[1].clone()
+    b[1][0] = 99
+    out = attend(ops, pool, q, k, v, b, window=w)
+    assert fault_word() == 4
+    assert out[0].isnan().all() and out[1].isfinite().all()
+
+
+@pytest.mark.parametrize("n_rep", [1, 3])
+def test_captured_few_rows_follow_the_lengths(ops, n_rep):
+    H, D = 2, 64
+    pool = Pool(2, H, D, 32, 64, 64, 4500, F32)
+    pool.append(ops, rows(4400, H, D, F32, 1), rows(4400, H, D, F32, 2), [4200, 200])
+    k, v, q = rows(2, H, D, F32, 3), rows(2, H, D, F32, 4), rows(2, H * n_rep, D, F32, 5)
+    arrays = pool.arrays([1, 1])
+    arrays[5] = 4500
+    out = torch.zeros_like(q)
+
+    def step():
+        ops.paged8_append(k, v, *pool.t, *arrays, 32)
+        ops.paged8_attention(q, k, v, *pool.t, *arrays, out, 32)
+    saved = [x.clone() for x in pool.t]
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    other = Pool(2, H, D, 32, 64, 64, 4500, F32)
+    for x, y in zip(pool.t, saved):
+        x.copy_(y)
+    other.append(ops, rows(4400, H, D, F32, 1), rows(4400, H, D, F32, 2), [4200, 200])
+    for i in range(2):
+        k.copy_(rows(2, H, D, F32, 10 + i)); v.copy_(rows(2, H, D, F32, 20 + i)); q.copy_(rows(2, H * n_rep, D, F32, 30 + i))
+        arrays[2].copy_(torch.tensor(other.lens, dtype=torch.int32))
+        graph.replay()
+        other.append(ops, k.clone(), v.clone(), [1, 1])
+        want, size, S = reference(other, q, [1, 1])
+        close(out, want, size, tolerance(F32, S))
