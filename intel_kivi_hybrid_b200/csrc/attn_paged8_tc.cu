@@ -43,6 +43,10 @@ constexpr int kM = 128;                                  // rows of a block
 constexpr int kG = 32;                                   // tokens that share their scales
 constexpr int kThreads = 512, kStageWarp = 8, kMmaWarp = 12, kCopyWarp = 13, kKeyWarp = 14;
 constexpr int kRing = 8;                                 // scales of so many tiles are kept
+// Who says of each tile that its keys' stage may be filled again: the MMAs, the values' warps, each of the two keys' warps,
+// and the copies (in tiles of rows the first keys' warp for them).  A barrier tells a phase from the next one only, so whoever
+// waits for it has a part in each of its phases and cannot be overtaken by two.
+constexpr int kStageUsers = 5;
 constexpr float kGrowth = 8.0f;                          // weights up to 2^8 are let stand before the maximum moves
 constexpr float kHeadroom = 8.0f, kSlack = 6.0f;         // products of weight and scale: up to 2^8, or 2^14 before their reference moves
 
@@ -147,7 +151,7 @@ paged8_tc_kernel(Paged8Attn A) {
             mbar_init(bar(misc.q_full), kM * n_sub);
             for (int i = 0; i < 2; ++i) {
                 mbar_init(bar(misc.q_again[i]), kM);
-                mbar_init(bar(misc.k_full[i]), 1); mbar_init(bar(misc.a_empty[i]), 2);
+                mbar_init(bar(misc.k_full[i]), 1); mbar_init(bar(misc.a_empty[i]), kStageUsers);
                 mbar_init(bar(misc.v_full[i]), 1); mbar_init(bar(misc.v_empty[i]), 1);
                 mbar_init(bar(misc.s_full[i]), 1); mbar_init(bar(misc.p_full[i][0]), kM); mbar_init(bar(misc.p_full[i][1]), kM);
             }
@@ -524,6 +528,7 @@ paged8_tc_kernel(Paged8Attn A) {
         };
         if (warp < kMmaWarp) {
             // ---------------- values; tiles of rows ----------------
+            // (whoever has given up a wait says no more that anything is done: the others give up in their turn)
             const int i128 = tid & 127, g = warp - kStageWarp;
             auto meet = [&] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
             bool ok = true;
@@ -552,14 +557,14 @@ paged8_tc_kernel(Paged8Attn A) {
                     }
                     fence_async();
                     meet();
-                    if (i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.v_full[st])); }
+                    if (ok && i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.v_full[st])); }
                 } else {
-                    if (ok && j >= 2) ok = wait_warp(misc.v_empty[st], (j >> 1) - 1);
+                    if (ok && j >= 2) ok = wait_warp(misc.a_empty[st], (j >> 1) - 1) && wait_warp(misc.v_empty[st], (j >> 1) - 1);
                     group_of_rows(false, t0 + kG * g, kG * g, v_at);
                     fence_async();
                     meet();
-                    // (its keys' stage is free: the tile before the last has been contracted)
-                    if (i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.v_full[st])); }
+                    // (nothing of these values lies in the keys' stage)
+                    if (ok && i128 == 0) { arrive(bar(misc.a_empty[st])); arrive(bar(misc.v_full[st])); }
                 }
             }
         } else if (warp >= kKeyWarp) {
@@ -568,9 +573,12 @@ paged8_tc_kernel(Paged8Attn A) {
 #pragma unroll 1
             for (int j = 0; j < n_tiles; ++j) {
                 const int st = j & 1, t0 = tile_start(j);
-                // (every phase is waited for in its turn, the pages' tiles' too: a barrier tells a phase from the next one only)
+                // (every phase is waited for in its turn, the pages' tiles' too)
                 if (ok && j >= 2) ok = wait_warp(misc.a_empty[st], (j >> 1) - 1);
-                if (j < n_packed) continue;
+                if (j < n_packed) {
+                    if (ok && lane == 0) arrive(bar(misc.a_empty[st]));
+                    continue;
+                }
 #pragma unroll 1
                 for (int g = 2 * (warp - kKeyWarp); g < 2 * (warp - kKeyWarp) + 2; ++g) {
                     const int first = t0 + kG * g;
@@ -588,7 +596,11 @@ paged8_tc_kernel(Paged8Attn A) {
                 }
                 fence_async();
                 asm volatile("bar.sync 2, 64;" ::: "memory");
-                if (tid == 32 * kKeyWarp) arrive(bar(misc.k_full[st]));
+                if (ok && lane == 0) arrive(bar(misc.a_empty[st]));
+                if (ok && tid == 32 * kKeyWarp) {
+                    arrive(bar(misc.a_empty[st]));       // (in place of the copies)
+                    arrive(bar(misc.k_full[st]));
+                }
             }
         } else if (warp == kCopyWarp) {
             // ---------------- copies ----------------
@@ -619,10 +631,12 @@ paged8_tc_kernel(Paged8Attn A) {
                         bulk_g2s(to + i * (kG * D), L.k_codes + at[i], kG * D, b, policy);
                         bulk_g2s(to + S::raw_v + i * (kG * D), L.v_codes + at[i], kG * D, b, policy);
                     }
+                    if (j < n_packed - 2) arrive(bar(misc.a_empty[st]));
                     sent = j + 1;
                 }
-                // no copy is under way when the block ends
-                for (int j = max(sent - 2, 0); j < sent; ++j) wait(misc.k_full[j & 1], j >> 1);
+                // no copy is under way when the block ends (and nobody fills the last two stages again before this has been seen)
+                for (int j = max(sent - 2, 0); j < sent; ++j)
+                    if (wait(misc.k_full[j & 1], j >> 1) && ok) arrive(bar(misc.a_empty[j & 1]));
             }
         } else if (warp == kMmaWarp) {
             // ---------------- MMAs ----------------

@@ -740,3 +740,20 @@ def test_captured_few_rows_follow_the_lengths(ops, n_rep):
         other.append(ops, k.clone(), v.clone(), [1, 1])
         want, size, S = reference(other, q, [1, 1])
         close(out, want, size, tolerance(F32, S))
+
+
+# ---- many tiles to a CTA of the tensor-core kernel ---------------------------------------------
+@pytest.mark.parametrize("D,held,window", [(128, [0, 200, 300, 450, 600, 5000], 0), (64, [130, 255, 384, 513, 2000, 3], 0), (128, [1000, 1100, 1250, 1400, 5000, 4000], 700)])
+def test_tiles_of_pages_and_of_rows_by_turns(ops, D, held, window):
+    """144 blocks of rows, so that each goes through all of its tiles: none, odd and even numbers of tiles of pages before those of
+    rows.  Every call returns the same, and no wait runs out."""
+    H, n_rep, new = 8, 2, [256] * len(held)
+    pool = Pool(len(held), H, D, 32, 128, 256, max(held) + 256, BF)
+    pool.append(ops, rows(sum(held), H, D, BF, 1), rows(sum(held), H, D, BF, 2), held)
+    n = sum(new)
+    k, v, q = rows(n, H, D, BF, 3), rows(n, H, D, BF, 4), rows(n, H * n_rep, D, BF, 5)
+    a = pool.append(ops, k, v, new)
+    got = attend(ops, pool, q, k, v, a, window=window)
+    want, size, S = reference(pool, q, new, window=window)
+    close(got, want, size, tolerance(BF, S))
+    assert all(torch.equal(attend(ops, pool, q, k, v, a, window=window), got) for _ in range(20))
