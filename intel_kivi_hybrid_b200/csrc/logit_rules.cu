@@ -152,7 +152,10 @@ adjust_logits_kernel(LogitArgs A) {
             }
         }
     };
-    if (!tokens && !biases) { copy(); return; }
+    if (!tokens && !biases) {                            // (in place and without a mask there is nothing to do, and nothing has been loaded)
+        if (copies) copy();
+        return;
+    }
     const bool wide = said.y - said.x > kNarrowTokens || given.y - given.x > kNarrowBiases;
     const int part = wide ? kEntries / 2 : kEntries;
     const Counters had{counters, wide}, last{counters + (tokens ? 2 * kEntries : 0), wide};

@@ -222,6 +222,23 @@ def test_refusals(ops):
     assert torch.equal(ops.adjust_logits(x, tokens=t[:0], cu_tokens=ints([0, 0, 0]), frequency=f), x)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("B,V,start", [(1, 50257, 0), (3, 1003, 5), (300, 2051, 0)])
+def test_nothing_to_do_in_place_changes_nothing(ops, dtype, B, V, start):
+    """A first step without history: no rules, or lists of nothing."""
+    space = torch.randn(start + B * V, device=DEV).to(dtype)
+    x = space[start:].view(B, V)
+    space[start] = float("nan")
+    kept = space.clone()
+    none, bounds = ints([], torch.int64), ints([0] * (B + 1))
+    for args in ({}, {"tokens": none, "cu_tokens": bounds, "frequency": torch.ones(B, device=DEV), "repetition": torch.full((B,), 2.0, device=DEV)},
+                 {"bias_ids": none, "bias": torch.empty(0, device=DEV), "cu_bias": bounds},
+                 {"tokens": ints([3], torch.int64), "cu_tokens": bounds, "presence": torch.ones(B, device=DEV)}):
+        assert ops.adjust_logits(x, x, **args).data_ptr() == x.data_ptr()
+        assert torch.equal(space.view(torch.uint8), kept.view(torch.uint8))
+        assert torch.equal(ops.adjust_logits(x, **args).view(torch.uint8), x.contiguous().view(torch.uint8))
+
+
 # ---- as it is used ---------------------------------------------------------------------
 def test_rules_of_a_run_on_the_device_and_on_the_host():
     """LogitRules over several steps: the device's kernel and the host's torch form agree, and both with the formula."""
