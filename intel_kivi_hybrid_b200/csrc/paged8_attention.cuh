@@ -39,6 +39,12 @@ __host__ __device__ __forceinline__ Span span_of(int T, int total, int p_lo, int
 // first token of a row's window (the row is at place p)
 __host__ __device__ __forceinline__ int window_from(int p, int window) { return window > 0 && p >= window ? p - window + 1 : 0; }
 
+// cap * tanh(z) where exponentials are cheaper than tanhf.  Up to |z| = kTanhNear z times an even polynomial, fitted (tanh z to
+// 1.2e-6 of itself, in fp32); beyond by tanh z = 1 - 2 / (1 + e^(2z)), which near 0 would be off by 2^-23 of the cap, whatever
+// the score.
+constexpr float kTanhNear = 0.8f;
+constexpr float kTanh1 = 0.9999990463256836f, kTanh3 = -0.33325737714767456f, kTanh5 = 0.13233496248722076f, kTanh7 = -0.04925421252846718f, kTanh9 = 0.012158339843153954f;
+
 #ifdef __CUDACC__
 __device__ __forceinline__ int prefix_of(const kivi_score_rules& r, int s, int total) {
     const int p = r.prefix ? r.prefix[s] : 0;

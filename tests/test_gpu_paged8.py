@@ -757,3 +757,48 @@ def test_tiles_of_pages_and_of_rows_by_turns(ops, D, held, window):
     want, size, S = reference(pool, q, new, window=window)
     close(got, want, size, tolerance(BF, S))
     assert all(torch.equal(attend(ops, pool, q, k, v, a, window=window), got) for _ in range(20))
+
+
+# ---- caps that hardly cap ---------------------------------------------------------------------
+def stepped(ops, new, n_rep, D, H=1, held=400, seed=0):
+    pool = Pool(1, H, D, 32, 64, 64, held + new, BF)
+    pool.append(ops, rows(held, H, D, BF, seed + 1), rows(held, H, D, BF, seed + 2), [held])
+    return pool, rows(new, H, D, BF, seed + 3), rows(new, H, D, BF, seed + 4), rows(new, H * n_rep, D, BF, seed + 5)
+
+
+@pytest.mark.parametrize("cap", [1e4, 1e5, 1e6, 1e8, 1e10])
+@pytest.mark.parametrize("new,n_rep,D", [(1, 4, 128), (5, 3, 64), (5, 4, 128), (130, 1, 128), (100, 2, 64)])
+def test_caps_far_above_the_scores(ops, new, n_rep, D, cap):
+    """The cap is there in form alone: the rows are those without it, at the ordinary tolerance (tanh z is off by 1.2e-6 of itself at
+    the most, which for scores up to 8 is below 2^-16)."""
+    pool, k, v, q = stepped(ops, new, n_rep, D)
+    a = pool.append(ops, k, v, [new])
+    got = attend(ops, pool, q, k, v, a, softcap=cap)
+    want, size, S = reference(pool, q, [new], cap=cap)
+    close(got, want, size, tolerance(BF, S))
+    free, _, _ = reference(pool, q, [new])
+    close(got, free, size, tolerance(BF, S))
+
+
+@pytest.mark.parametrize("new,n_rep", [(1, 4), (7, 3)])
+@pytest.mark.parametrize("hidden", [False, True])
+def test_a_cap_that_one_row_reaches(ops, new, n_rep, hidden):
+    """A row whose scores are far above the cap, or an infinite key that the others do not see, costs its neighbours nothing."""
+    pool, k, v, q = stepped(ops, new, n_rep, 128)
+    loud = torch.zeros(new, n_rep, dtype=torch.bool, device=DEV)
+    want_k = k
+    if hidden and new > 1:
+        want_k = k.clone()
+        k[new - 1, 0, 3] = float("inf")
+        loud[new - 1] = True
+    else:
+        q[0, 0] *= 2.0 ** 30
+        loud[0, 0] = True
+    a = pool.arrays([new])
+    ops.paged8_append(k, v, *pool.t, *a, 32)
+    pool.K[0], pool.V[0] = torch.cat([pool.K[0], want_k]), torch.cat([pool.V[0], v])
+    pool.before, pool.lens = [400], [400 + new]
+    got = attend(ops, pool, q, k, v, a, softcap=1e7)
+    want, size, S = reference(pool, q, [new], cap=1e7)
+    close(got[~loud], want[~loud], size[~loud], tolerance(BF, S))
+    assert got[loud].isfinite().all()
