@@ -81,14 +81,13 @@ __device__ __forceinline__ float log2_of(float x) {
 }
 __device__ __forceinline__ float pow2i(int s) { return __uint_as_float((uint32_t)(127 + max(-126, min(127, s))) << 23); }
 
-// cap * tanh(z) of two numbers.  Up to |z| = 0.8 an odd polynomial, fitted (relative error below 1e-6); beyond by
-// tanh z = 1 - 2 / (1 + e^(2z)).
+// cap * tanh(z)
 __device__ __forceinline__ float2 capped_near(float2 z, float cap) {
     const float2 s = mul2(z, z);
-    float2 p = fma2(s, both(0.012158339843153954f), both(-0.04925421252846718f));
-    p = fma2(p, s, both(0.13233496248722076f));
-    p = fma2(p, s, both(-0.33325737714767456f));
-    p = fma2(p, s, both(0.9999990463256836f));
+    float2 p = fma2(s, both(kTanh9), both(kTanh7));
+    p = fma2(p, s, both(kTanh5));
+    p = fma2(p, s, both(kTanh3));
+    p = fma2(p, s, both(kTanh1));
     return mul2(mul2(p, z), both(cap));
 }
 __device__ __forceinline__ float capped_far(float z, float cap) {
@@ -297,11 +296,21 @@ paged8_tc_kernel(Paged8Attn A) {
                                     far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
                                     put2(g, i, z);
                                 }
-                            if (__any_sync(0xffffffffu, far > 0.8f)) {
+                            if (__any_sync(0xffffffffu, far > kTanhNear)) {
+                                if (A.rules.softcap <= kSmallCap) {
 #pragma unroll
-                                for (int g = 0; g < 2; ++g)
+                                    for (int g = 0; g < 2; ++g)
 #pragma unroll
-                                    for (int i = 0; i < 32; ++i) v[g][i] = __float_as_uint(capped_far(__uint_as_float(v[g][i]), cap));
+                                        for (int i = 0; i < 32; ++i) v[g][i] = __float_as_uint(capped_far(__uint_as_float(v[g][i]), cap));
+                                } else {                 // (what is near 0 is not to pay for what is far)
+#pragma unroll
+                                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                                        for (int i = 0; i < 32; i += 2) {
+                                            const float2 z = at2(g, i), y = capped_near(z, cap);
+                                            put2(g, i, make_float2(fabsf(z.x) <= kTanhNear ? y.x : capped_far(z.x, cap), fabsf(z.y) <= kTanhNear ? y.y : capped_far(z.y, cap)));
+                                        }
+                                }
                             } else {
 #pragma unroll
                                 for (int g = 0; g < 2; ++g)

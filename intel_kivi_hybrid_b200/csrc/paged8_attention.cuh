@@ -43,6 +43,7 @@ __host__ __device__ __forceinline__ int window_from(int p, int window) { return 
 // 1.2e-6 of itself, in fp32); beyond by tanh z = 1 - 2 / (1 + e^(2z)), which near 0 would be off by 2^-23 of the cap, whatever
 // the score.
 constexpr float kTanhNear = 0.8f;
+constexpr float kSmallCap = 256.0f;                      // up to it the latter does for all scores: off by 2^-13 at the most
 constexpr float kTanh1 = 0.9999990463256836f, kTanh3 = -0.33325737714767456f, kTanh5 = 0.13233496248722076f, kTanh7 = -0.04925421252846718f, kTanh9 = 0.012158339843153954f;
 
 #ifdef __CUDACC__

@@ -780,7 +780,7 @@ def test_caps_far_above_the_scores(ops, new, n_rep, D, cap):
     close(got, free, size, tolerance(BF, S))
 
 
-@pytest.mark.parametrize("new,n_rep", [(1, 4), (7, 3)])
+@pytest.mark.parametrize("new,n_rep", [(1, 4), (7, 3), (130, 1), (100, 2)])
 @pytest.mark.parametrize("hidden", [False, True])
 def test_a_cap_that_one_row_reaches(ops, new, n_rep, hidden):
     """A row whose scores are far above the cap, or an infinite key that the others do not see, costs its neighbours nothing."""
