@@ -802,3 +802,18 @@ def test_a_cap_that_one_row_reaches(ops, new, n_rep, hidden):
     want, size, S = reference(pool, q, [new], cap=1e7)
     close(got[~loud], want[~loud], size[~loud], tolerance(BF, S))
     assert got[loud].isfinite().all()
+
+
+# ---- pieces of which a row sees one token ------------------------------------------------------
+@pytest.mark.parametrize("dtype,D,held,new", [(F32, 64, 316, 5), (F32, 128, 300, 21), (F32, 96, 300, 85), (BF, 128, 300, 85), (BF, 64, 300, 85), (BF, 128, 5000, 1), (BF, 128, 380, 5), (F32, 128, 4096, 1)])
+def test_a_nan_that_a_piece_holds_alone_is_kept(ops, dtype, D, held, new):
+    """The last row's own key is NaN and the first token of a tile: no other row is touched, and this one is NaN."""
+    pool = Pool(1, 1, D, 32, 64, 64, held + new, dtype)
+    pool.append(ops, rows(held, 1, D, dtype, 1), rows(held, 1, D, dtype, 2), [held])
+    k, v, q = rows(new, 1, D, dtype, 3), rows(new, 1, D, dtype, 4), rows(new, 1, D, dtype, 5)
+    k[new - 1, 0, 3] = float("nan")
+    a = pool.append(ops, k, v, [new])
+    got = attend(ops, pool, q, k, v, a)
+    assert got[new - 1].isnan().all()
+    want, size, S = reference(pool, q, [new])
+    close(got[:new - 1], want[:new - 1], size[:new - 1], tolerance(dtype, S)) if new > 1 else None
