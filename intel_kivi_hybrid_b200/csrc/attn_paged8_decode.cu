@@ -370,7 +370,7 @@ paged8_decode_kernel(Paged8Attn A) {
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = (int)(__float_as_uint(top) >> 23), shift = e == 0 ? 0 : max(-110, min(110, 127 + 13 - e));       // largest to 2^13 .. 2^14
+            const int e = (int)(__float_as_uint(top) >> 23), shift = min(126, 127 + 13 - e);             // largest to 2^13 .. 2^14 (what is below 2^-113 as far as a power of two goes)
             const float f = pow2i(shift);
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {

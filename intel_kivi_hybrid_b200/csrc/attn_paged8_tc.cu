@@ -23,9 +23,9 @@
 // scale less the power of two of the largest such product that the row has met, so that neither
 // a row's own range nor what other rows see takes its bits.  Two terms of e4m3 would do for P's bits, not for its range.
 // Window and new tokens are bf16 operands as they are, Q and P then too: Q is written again
-// when the pages are done.  Where only some of a group's tokens come from its page, the others' scores are divided by
-// its scale (keys rounded to bf16 instead: 0.0027 off 64 bits where the output's rounding is 0.0017), and its values are rounded
-// to bf16.  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
+// when the pages are done.  Keys of a page are there codes times their scale's power of two, and its rest multiplies S; where only
+// some of a group's tokens come from the page, the others' scores are divided by that rest (keys rounded to bf16 instead: 0.0027 off
+// 64 bits where the output's rounding is 0.0017), and the page's values are rounded to bf16.  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
 //
 // Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle).
 #include "paged8_attention.cuh"
@@ -80,6 +80,8 @@ __device__ __forceinline__ float log2_of(float x) {
     return y;
 }
 __device__ __forceinline__ float pow2i(int s) { return __uint_as_float((uint32_t)(127 + max(-126, min(127, s))) << 23); }
+
+__device__ __forceinline__ float power_of(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }         // the power of two below it
 
 // cap * tanh(z)
 __device__ __forceinline__ float2 capped_near(float2 z, float cap) {
@@ -207,7 +209,7 @@ paged8_tc_kernel(Paged8Attn A) {
                     }
                 }
                 const int e = (int)(top >> 23);
-                q_shift = e == 0 ? 0 : max(-110, min(110, 127 + 7 - e));              // to 2^7 .. 2^8
+                q_shift = min(126, 127 + 7 - e);          // to 2^7 .. 2^8 (what is below 2^-119 as far as a power of two goes)
                 const float f = pow2i(q_shift);
 #pragma unroll 1
                 for (int d = 0; d < D; d += 16) {
@@ -259,7 +261,7 @@ paged8_tc_kernel(Paged8Attn A) {
                 // columns that the row sees: below `near`, and lo .. hi
                 const int near = prefix - t0, lo = from - t0, hi = place - t0;
                 const bool edge = __any_sync(0xffffffffu, near < kN && (lo > 0 || hi < kN - 1));
-                // a group of which the first columns alone come from its page: the others' scores are divided by its scale
+                // a group of which the first columns alone come from its page: the others' scores are divided by what multiplies it
                 const int cut = inside - t0;
                 if (cut > 0 && cut < kN && cut % kG != 0) {
                     const float inv = 1.0f / k_scales[cut / kG];
@@ -477,7 +479,8 @@ paged8_tc_kernel(Paged8Attn A) {
                 const int64_t unit = (int64_t)page_of(L, q, first, &g_fault) * H + h;
                 const int in_page = first % L.page_tokens;
                 const uint8_t* const codes = (of_keys ? L.k_codes : L.v_codes) + unit * L.page_tokens * D;
-                const float f = of_keys || first + kG <= inside ? 1.0f : L.v_scales[scale_at(first)];
+                // keys are codes times their scale's power of two, which bf16 holds exactly: q k then fits where the formula's does
+                const float f = of_keys ? power_of(L.k_scales[scale_at(first)]) : first + kG <= inside ? 1.0f : L.v_scales[scale_at(first)];
 #pragma unroll 1
                 for (int r = r0; r < kG && first + r < inside; r += kStep) {
                     uint32_t b[2] = {0u, 0u}, w[4];
@@ -596,7 +599,7 @@ paged8_tc_kernel(Paged8Attn A) {
                         float ks = 1.0f, vs = 1.0f;
                         if (first < inside) {
                             const int64_t f = scale_at(first);
-                            ks = L.k_scales[f];
+                            ks = L.k_scales[f] / power_of(L.k_scales[f]);
                             if (first + kG <= inside) vs = L.v_scales[f];
                         }
                         reinterpret_cast<float*>(&misc.k_scale[j % kRing])[g] = ks;

@@ -817,3 +817,19 @@ def test_a_nan_that_a_piece_holds_alone_is_kept(ops, dtype, D, held, new):
     assert got[new - 1].isnan().all()
     want, size, S = reference(pool, q, [new])
     close(got[:new - 1], want[:new - 1], size[:new - 1], tolerance(dtype, S)) if new > 1 else None
+
+
+# ---- queries at the ends of bf16's range ------------------------------------------------------
+@pytest.mark.parametrize("new,n_rep,D", [(1, 4, 128), (5, 3, 64), (130, 1, 128), (100, 2, 64)])
+@pytest.mark.parametrize("size_q,size_k,scale", [(126, -30, -98), (120, -20, -102), (-100, 60, 33), (-118, 80, 33)])
+def test_queries_of_any_size(ops, new, n_rep, D, size_q, size_k, scale):
+    """Queries, keys and sm_scale as powers of two whose product is ordinary."""
+    held = 400
+    pool = Pool(1, 1, D, 32, 64, 64, held + new, BF)
+    pool.append(ops, rows(held, 1, D, BF, 1) * 2.0 ** size_k, rows(held, 1, D, BF, 2), [held])
+    k, v, q = rows(new, 1, D, BF, 3) * 2.0 ** size_k, rows(new, 1, D, BF, 4), rows(new, n_rep, D, BF, 5).clamp(-1.9, 1.9)
+    a = pool.append(ops, k, v, [new])
+    sm_scale = 2.0 ** scale
+    got = attend(ops, pool, (q.float() * 2.0 ** size_q).to(BF), k, v, a, sm_scale=sm_scale)
+    want, size, S = reference(pool, q.double() * (2.0 ** (size_q + scale) * math.sqrt(D)), [new])
+    close(got, want, size, tolerance(BF, S))
