@@ -84,8 +84,9 @@ class LogitRules:
         for b in range(self.batch):
             if "cu_tokens" in self._args:
                 had = self.tokens[b, :self.held]
-                said = torch.bincount(had[self.given:].clamp(max=V), minlength=V + 1)[:V].float()
-                seen = torch.bincount(had.clamp(max=V), minlength=V + 1)[:V] > 0
+                had = torch.where((had < 0) | (had > V), V, had)             # (ids outside count for nothing)
+                said = torch.bincount(had[self.given:], minlength=V + 1)[:V].float()
+                seen = torch.bincount(had, minlength=V + 1)[:V] > 0
                 x[b] = torch.where(seen, torch.where(x[b] > 0, x[b] / repetition, x[b] * repetition), x[b]) - frequency * said - presence * (said > 0)
             for i, number in self.bias.items():
                 if 0 <= i < V:

@@ -274,6 +274,17 @@ def test_rules_of_a_run_on_the_device_and_on_the_host():
         LogitRules(prompt, 1, repetition=0.0)
 
 
+def test_ids_below_zero_count_for_nothing_on_the_device():
+    from kivi_cuda import LogitRules
+    V = 12
+    prompt = torch.tensor([[-1, -100, 3, 4], [5, 2 ** 40, V, -2 ** 50]])
+    dev, host = (LogitRules(p, 2, repetition=2.0, frequency=0.5, presence=0.25) for p in (prompt.cuda(), prompt))
+    for said in ([-7, 5], [3, -1]):
+        x = torch.randn(2, V)
+        assert torch.equal(dev(x.cuda()).cpu(), host(x))
+        dev.said(torch.tensor(said).cuda()); host.said(torch.tensor(said))
+
+
 @pytest.mark.parametrize("fused", [False, True])
 def test_generate_with_rules(fused):
     """Greedy decoding of a small model: a presence penalty no logit reaches forbids what was said, a bias and a mask decide."""

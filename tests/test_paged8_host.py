@@ -105,3 +105,18 @@ def test_logit_rules_on_the_host():
         LogitRules(prompt, 1, allowed=lambda ids: torch.zeros(1, 1))(x)
     with pytest.raises(ValueError, match="vocab"):
         rules(x[0])
+
+
+def test_ids_below_zero_count_for_nothing_on_the_host():
+    """A prompt padded with ids that are none, as the device has it."""
+    from intel_kivi_hybrid_b200.generation.logits import LogitRules
+    V = 12
+    prompt = torch.tensor([[-1, -100, 3, 4], [5, 2 ** 40, V, -2 ** 50]])
+    rules = LogitRules(prompt, 2, repetition=2.0, frequency=0.5, presence=0.25)
+    x = torch.ones(2, V)
+    want = torch.ones(2, V)
+    want[0, 3] = want[0, 4] = want[1, 5] = 0.5
+    assert torch.equal(rules(x), want)
+    rules.said(torch.tensor([-7, 5]))
+    want[1, 5] -= 0.75
+    assert torch.equal(rules(x), want)
