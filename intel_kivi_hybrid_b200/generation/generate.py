@@ -59,7 +59,8 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
         if not ruled:
             return choose(logits)
         if rules is None:
-            rules = LogitRules(input_ids, max_new_tokens, logits.device, repetition_penalty, frequency_penalty, presence_penalty, logit_bias, allowed)
+            # (the prompt gives a token whatever max_new_tokens is)
+            rules = LogitRules(input_ids, max(1, max_new_tokens), logits.device, repetition_penalty, frequency_penalty, presence_penalty, logit_bias, allowed)
         ids = choose(rules(logits))
         rules.said(ids)
         return ids

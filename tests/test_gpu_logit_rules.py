@@ -311,3 +311,25 @@ def test_generate_with_rules(fused):
     words[0, 0] = 0b110000                                  # tokens 4 and 5 alone
     assert set(run(allowed=lambda ids: words)) <= {4, 5}
     assert run(repetition_penalty=1.0, frequency_penalty=0.0) == plain
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("n", [0, 1])
+def test_generate_of_hardly_any_tokens_with_rules(fused, n):
+    """The first token comes of the prompt whatever max_new_tokens is, with rules as without."""
+    transformers = pytest.importorskip("transformers")
+    from kivi_cuda import generate
+    torch.manual_seed(0)
+    model = transformers.GPT2LMHeadModel(transformers.GPT2Config(n_layer=1, n_head=2, n_embd=64, vocab_size=64, n_positions=64)).cuda().eval()
+
+    class Tokenizer:
+        eos_token_id = None
+
+        def __call__(self, text, return_tensors):
+            return type("E", (), {"input_ids": torch.tensor([[int(c) for c in text.split()]])})
+
+        def decode(self, ids, skip_special_tokens):
+            return " ".join(str(int(i)) for i in ids)
+    run = lambda **kw: generate(model, Tokenizer(), "1 2 3", max_new_tokens=n, fused_attention=fused, residual_length=32, **kw).split()  # noqa: E731
+    assert len(run()) == 4
+    assert run(logit_bias={9: 1000.0}) == ["1", "2", "3", "9"]
