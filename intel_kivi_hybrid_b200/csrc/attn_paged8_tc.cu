@@ -25,7 +25,7 @@
 // Window and new tokens are bf16 operands as they are, Q and P then too: Q is written again
 // when the pages are done.  Keys of a page are there codes times their scale's power of two, and its rest multiplies S; where only
 // some of a group's tokens come from the page, the others' scores are divided by that rest (keys rounded to bf16 instead: 0.0027 off
-// 64 bits where the output's rounding is 0.0017), and the page's values are rounded to bf16.  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
+// 64 bits where the output's rounding is 0.0017), and the page's values are held the same way, their rest in the weights.  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
 //
 // Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle).
 #include "paged8_attention.cuh"
@@ -66,6 +66,7 @@ struct Misc {                                            // behind the tiles
     int place[2];
     int odd;                                             // a value that is not finite has been met
     float4 k_scale[kRing], v_scale[kRing];               // of tile j's four groups at j % kRing; values': their log2
+    float v_rest;                                        // of the group that is partly in its page: its values' scale over their power of two
 };
 
 __device__ __forceinline__ float2 ex2x2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
@@ -81,7 +82,9 @@ __device__ __forceinline__ float log2_of(float x) {
 }
 __device__ __forceinline__ float pow2i(int s) { return __uint_as_float((uint32_t)(127 + max(-126, min(127, s))) << 23); }
 
-__device__ __forceinline__ float power_of(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }         // the power of two below it
+// a scale as a power of two and the rest, 1 to 2
+__device__ __forceinline__ float power_of(float x) { return __uint_as_float(__float_as_uint(x) & 0x7f800000u); }
+__device__ __forceinline__ float rest_of(float x) { return __uint_as_float((__float_as_uint(x) & 0x7fffffu) | 0x3f800000u); }
 
 // cap * tanh(z)
 __device__ __forceinline__ float2 capped_near(float2 z, float cap) {
@@ -263,8 +266,9 @@ paged8_tc_kernel(Paged8Attn A) {
                 const bool edge = __any_sync(0xffffffffu, near < kN && (lo > 0 || hi < kN - 1));
                 // a group of which the first columns alone come from its page: the others' scores are divided by what multiplies it
                 const int cut = inside - t0;
-                if (cut > 0 && cut < kN && cut % kG != 0) {
-                    const float inv = 1.0f / k_scales[cut / kG];
+                const bool cuts = cut > 0 && cut < kN && cut % kG != 0;
+                if (cuts) {
+                    const float inv = __fdividef(1.0f, k_scales[cut / kG]);
 #pragma unroll 1
                     for (int x = cut / kG * kG; x < cut / kG * kG + kG; x += 16) {
                         uint32_t o[16];
@@ -412,8 +416,34 @@ paged8_tc_kernel(Paged8Attn A) {
                         arrive(bar(misc.p_full[t][half]));
                     }
                 };
+                // the same in the tile with a group that is partly in its page, whose values want the rest of their scale
+                auto weights_cut = [&] {
+#pragma unroll 1
+                    for (int x = 0; x < kN; x += 16) {
+                        const int g = x / kG, edge = g == cut / kG ? cut - x : 0;            // columns before it have the rest
+                        uint32_t v[16], p[8];
+                        tmem_load16(s_at + x, v);
+                        const float c = RULES ? 1.0f : factor(k_scales[g], to_c), lift = fmaxf(v_scales[g] + up, -60.0f), off = lift - base_m, rest = misc.v_rest;
+                        tmem_wait_load();
+                        float part = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const float w0 = ex2(fmaf(__uint_as_float(v[i]), c, off)), w1 = ex2(fmaf(__uint_as_float(v[i + 1]), c, off));
+                            part += w0 + w1;
+                            p[i / 2] = pack_bf16(i < edge ? w0 * rest : w0, i + 1 < edge ? w1 * rest : w1);
+                        }
+                        l = fmaf(part, ex2(-lift), l);
+                        tmem_store8(s_at + x / 2, p);
+                        if (x % 64 == 48) {
+                            tmem_wait_store();
+                            fence_before();
+                            arrive(bar(misc.p_full[t][x / 64]));
+                        }
+                    }
+                };
                 if (packed) weights(std::true_type{});
-                else weights(std::false_type{});
+                else if (!cuts) weights(std::false_type{});
+                else weights_cut();
                 if (j + 1 == n_packed && j + 1 < n_tiles) {
                     // (S of this tile is there, so Q has been read)
                     q_as_bf16();
@@ -479,8 +509,8 @@ paged8_tc_kernel(Paged8Attn A) {
                 const int64_t unit = (int64_t)page_of(L, q, first, &g_fault) * H + h;
                 const int in_page = first % L.page_tokens;
                 const uint8_t* const codes = (of_keys ? L.k_codes : L.v_codes) + unit * L.page_tokens * D;
-                // keys are codes times their scale's power of two, which bf16 holds exactly: q k then fits where the formula's does
-                const float f = of_keys ? power_of(L.k_scales[scale_at(first)]) : first + kG <= inside ? 1.0f : L.v_scales[scale_at(first)];
+                // codes times their scale's power of two, which bf16 holds exactly: q k then fits where the formula's does
+                const float f = of_keys ? power_of(L.k_scales[scale_at(first)]) : first + kG <= inside ? 1.0f : power_of(L.v_scales[scale_at(first)]);
 #pragma unroll 1
                 for (int r = r0; r < kG && first + r < inside; r += kStep) {
                     uint32_t b[2] = {0u, 0u}, w[4];
@@ -599,8 +629,9 @@ paged8_tc_kernel(Paged8Attn A) {
                         float ks = 1.0f, vs = 1.0f;
                         if (first < inside) {
                             const int64_t f = scale_at(first);
-                            ks = L.k_scales[f] / power_of(L.k_scales[f]);
+                            ks = rest_of(L.k_scales[f]);
                             if (first + kG <= inside) vs = L.v_scales[f];
+                            else misc.v_rest = rest_of(L.v_scales[f]);
                         }
                         reinterpret_cast<float*>(&misc.k_scale[j % kRing])[g] = ks;
                         reinterpret_cast<float*>(&misc.v_scale[j % kRing])[g] = log2_of(vs);

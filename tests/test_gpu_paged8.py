@@ -833,3 +833,19 @@ def test_queries_of_any_size(ops, new, n_rep, D, size_q, size_k, scale):
     got = attend(ops, pool, (q.float() * 2.0 ** size_q).to(BF), k, v, a, sm_scale=sm_scale)
     want, size, S = reference(pool, q.double() * (2.0 ** (size_q + scale) * math.sqrt(D)), [new])
     close(got, want, size, tolerance(BF, S))
+
+
+# ---- blocks that are partly in their pages -------------------------------------------------------
+@pytest.mark.parametrize("D,G,R,held,new,n_rep", [(128, 32, 100, 300, 80, 1), (64, 32, 32, 1, 31, 8), (128, 256, 256, 255, 70, 3), (64, 96, 97, 98, 200, 2), (128, 32, 32, 47, 5, 3)])
+@pytest.mark.parametrize("rules", [{}, {"softcap": 30.0}])
+def test_loud_values_of_a_block_that_this_step_fills(ops, D, G, R, held, new, n_rep, rules):
+    """Tokens held before the step are in their page behind it, the others of their block are read as rows: an output that comes of the
+    former alone, 2^20 times as large, is off by its weights' rounding and no more."""
+    pool = Pool(1, 2, D, G, R, G, held + new, BF)
+    k0, v0 = rows(held, 2, D, BF, 1), rows(held, 2, D, BF, 2)
+    v0[-3:] *= 2.0 ** 20
+    pool.append(ops, k0, v0, [held])
+    k, v, q = rows(new, 2, D, BF, 3), rows(new, 2, D, BF, 4), rows(new, 2 * n_rep, D, BF, 5)
+    a = pool.append(ops, k, v, [new])
+    want, size, S = reference(pool, q, [new], cap=rules.get("softcap", 0.0))
+    close(attend(ops, pool, q, k, v, a, F32, **rules), want, size, tolerance(BF, S))
