@@ -312,7 +312,7 @@ paged_merge_kernel(PagedAttnArgs A, int RT) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int p = 0; p < n_pieces; ++p) {
             const float2 ml = *reinterpret_cast<const float2*>(A.part_ml + 2 * ((part0 + p) * RT + r));
-            if (ml.x == -INFINITY) continue;             // a piece behind the row's own token
+            if (ml.x == -INFINITY && ml.y == 0.0f) continue;         // a piece behind the row's own token (of what it sees, NaN may be all)
             const float w = exp2f(ml.x - M);
             const float4 v = *reinterpret_cast<const float4*>(A.part_o + ((part0 + p) * RT + r) * D + d);
             sum = fmaf(w, ml.y, sum);

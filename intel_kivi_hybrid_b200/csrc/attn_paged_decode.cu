@@ -328,7 +328,7 @@ paged_decode_kernel(PagedAttnArgs A, int blocks_per_seq, int gps) {
         for (int w2 = 0; w2 < kWarps; ++w2) M = fmaxf(M, ml_s[(w2 * 4 + r) * 2]);
         for (int w2 = 0; w2 < kWarps; ++w2) {
             const float mw = ml_s[(w2 * 4 + r) * 2];
-            if (mw != -INFINITY) ls += ml_s[(w2 * 4 + r) * 2 + 1] * ex2(mw - M);
+            ls += ml_s[(w2 * 4 + r) * 2 + 1] * (mw == -INFINITY ? 0.0f : ex2(mw - M));       // (no maximum: 0, or NaN where NaN is all that was seen)
         }
         *reinterpret_cast<float2*>(A.part_ml + 2 * (base + r)) = make_float2(M, ls);
     }
@@ -356,7 +356,7 @@ paged_decode_merge_kernel(PagedAttnArgs A, int blocks_per_seq, int gps) {
     float M = -INFINITY, sum = 0.0f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](float2 ml, float4 v) {
-        if (ml.x == -INFINITY) return;
+        if (ml.x == -INFINITY && ml.y == 0.0f) return;
         const float top = fmaxf(M, ml.x), w0 = ex2(M - top), w1 = ex2(ml.x - top);
         M = top;
         sum = fmaf(w0, sum, w1 * ml.y);

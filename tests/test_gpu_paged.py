@@ -695,3 +695,19 @@ def test_packed_numbers_on_the_tensor_cores_are_rounded_from_the_middle_of_their
     k[held:], v[held:] = K[held:].double(), V[held:].double()
     want, _ = attended(q.double(), k, v, held, n_rep, D ** -0.5)
     assert float((got - want).norm() / want.norm()) < 5.5e-4
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32), (128, torch.float32)])
+@pytest.mark.parametrize("R,total,new,n_rep", [(128, 385, 1, 1), (128, 385, 5, 4), (128, 321, 21, 1), (128, 513, 140, 4), (32, 65, 1, 4), (32, 97, 1, 1)])
+def test_a_nan_that_a_piece_holds_alone_is_kept(D, dtype, R, total, new, n_rep):
+    """The last row's own key is NaN and the first token of a tile or all of the window: this row is NaN and no other."""
+    from kivi_cuda import PagedKiviCache
+    cache = PagedKiviCache(1, D, 1, num_pages=20, max_sequences=1, page_tokens=64, group_size=32, residual_length=R, dtype=dtype)
+    seq, held = cache.add_sequence(), total - new
+    step = cache.begin([seq], [held])
+    cache.append(0, step, rows(held, 1, D, dtype, 1), rows(held, 1, D, dtype, 2))
+    cache.end(step)
+    q, k, v = rows(new, n_rep, D, dtype, 3), rows(new, 1, D, dtype, 4), rows(new, 1, D, dtype, 5)
+    k[new - 1, 0, 3] = float("nan")
+    out = cache.step(0, cache.begin([seq], [new]), q, k, v)
+    assert out[new - 1].isnan().all() and out[:new - 1].isfinite().all()
