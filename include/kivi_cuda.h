@@ -582,7 +582,8 @@ typedef struct kivi_score_rules {
 } kivi_score_rules;
 
 /* Attention of a step's rows after kivi_paged8_append of the same batch, as kivi_paged_attention; rules may be NULL.
- * A token that a row does not see does not touch it, whatever it holds.  Sums and softmax statistics are fp32.  bf16 rows of
+ * A token that a row does not see does not touch it, whatever it holds.  Sums and softmax statistics are fp32, and divided by the
+ * weights' sum at the end: values up to 2^100 in magnitude are in reach for rows of a million tokens.  bf16 rows of
  * 64 or 128 channels over blocks of whole 32 tokens go through the tensor cores, their weights as fp16 (beside the
  * window's and the new rows' values bf16) numbers; all others are fp32 throughout. */
 size_t kivi_paged8_attention_workspace(const kivi_paged8_layer* layer, const kivi_paged_batch* batch, int q_dtype, int n_rep,

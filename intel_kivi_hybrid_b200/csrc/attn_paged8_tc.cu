@@ -100,7 +100,10 @@ __device__ __forceinline__ float capped_far(float z, float cap) {
     return cap - __fdividef(2.0f * cap, 1.0f + ex2(e > 120.0f ? 120.0f : e));
 }
 
-template <int D, bool RULES>
+// What is done to scores: nothing, slopes alone, a cap up to kSmallCap, any cap (both of them with slopes or without).
+enum { kNoRules, kSlopes, kSmallCaps, kAnyCaps };
+
+template <int D, int RULES>
 __global__ void __launch_bounds__(kThreads, 1)
 paged8_tc_kernel(Paged8Attn A) {
     using S = Shared<D>;
@@ -247,11 +250,11 @@ paged8_tc_kernel(Paged8Attn A) {
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + t * kN, o_at = tmem + lanes + 2 * kN + t * D;
             constexpr float kLog2e = 1.4426950408889634f;
             auto factor = [](float scale, float to) { return fmaxf(scale * to, 1.0e-37f); };         // (not 0: hidden columns are -inf)
-            const bool capped = RULES && A.rules.softcap > 0.0f;
-            const float cap = A.rules.softcap * kLog2e, slope = RULES && A.rules.slopes && there ? A.rules.slopes[head] * kLog2e : 0.0f;
+            const bool capped = RULES >= kSmallCaps && A.rules.softcap > 0.0f, biased = RULES != kNoRules && A.rules.slopes != nullptr;
+            const float cap = A.rules.softcap * kLog2e, slope = biased && there ? A.rules.slopes[head] * kLog2e : 0.0f;
             const float to_x = capped ? A.scale / A.rules.softcap : A.scale * kLog2e;
             float m = -INFINITY, ref = -1.0e30f, l = 0.0f, base_m = 0.0f, up = 0.0f;         // ref: the largest maximum plus value scale, so far; up: log2 of what brings weights times scales to O's scale
-            bool ok = true;
+            bool ok = true, low = false;                 // low: a row of the warp has `up` below -60
             for (int j = 0; j < n_tiles; ++j) {
                 // (given up: on to the end without waiting)
                 if (ok) ok = wait_warp(misc.s_full[t], j);
@@ -291,7 +294,7 @@ paged8_tc_kernel(Paged8Attn A) {
                     tmem_wait_load();
                     auto at2 = [&](int g, int i) { return make_float2(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])); };
                     auto put2 = [&](int g, int i, float2 x) { v[g][i] = __float_as_uint(x.x); v[g][i + 1] = __float_as_uint(x.y); };
-                    if constexpr (RULES) {
+                    if constexpr (RULES != kNoRules) {
                         if (capped) {
                             float far = 0.0f;
 #pragma unroll
@@ -303,7 +306,7 @@ paged8_tc_kernel(Paged8Attn A) {
                                     put2(g, i, z);
                                 }
                             if (__any_sync(0xffffffffu, far > kTanhNear)) {
-                                if (A.rules.softcap <= kSmallCap) {
+                                if constexpr (RULES != kAnyCaps) {
 #pragma unroll
                                     for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -324,7 +327,7 @@ paged8_tc_kernel(Paged8Attn A) {
                                     for (int i = 0; i < 32; i += 2) put2(g, i, capped_near(at2(g, i), cap));
                             }
                         }
-                        if (A.rules.slopes != nullptr) {
+                        if (biased) {
                             const float2 on = both(2.0f * slope);
 #pragma unroll
                             for (int g = 0; g < 2; ++g) {
@@ -344,7 +347,7 @@ paged8_tc_kernel(Paged8Attn A) {
                         for (int i = 0; i < 64; ++i)
                             if (!(i < a || (i >= b && i <= e))) v[i / 32][i % 32] = 0xff800000u;
                     }
-                    if (RULES || edge)                   // (read again below)
+                    if (RULES != kNoRules || edge)              // (read again below)
 #pragma unroll
                         for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -357,12 +360,12 @@ paged8_tc_kernel(Paged8Attn A) {
                             x = fmaxf(x, fmaxf(__uint_as_float(v[g][i]), __uint_as_float(v[g][i + 1])));
                             y = fmaxf(y, fmaxf(__uint_as_float(v[g][i + 2]), __uint_as_float(v[g][i + 3])));
                         }
-                        x = fmaxf(x, y) * (RULES ? 1.0f : c[g]);
+                        x = fmaxf(x, y) * (RULES != kNoRules ? 1.0f : c[g]);
                         top_all = fmaxf(top_all, x);
                         most = fmaxf(most, x + v_scales[2 * half + g]);
                     }
                 }
-                if (RULES || edge) tmem_wait_store();
+                if (RULES != kNoRules || edge) tmem_wait_store();
                 if (__any_sync(0xffffffffu, top_all > m + kGrowth || most > ref + kSlack)) {
                     if (top_all > m + kGrowth) {         // (from -inf: whenever there is a maximum)
                         l *= m == -INFINITY ? 0.0f : ex2(m - top_all);
@@ -386,6 +389,7 @@ paged8_tc_kernel(Paged8Attn A) {
                         }
                     }
                     up = fminf(base_m - ref + kHeadroom, 126.0f);
+                    low = __any_sync(0xffffffffu, up < -60.0f);
                 }
                 auto weights = [&](auto as_half) {
 #pragma unroll 1
@@ -393,9 +397,12 @@ paged8_tc_kernel(Paged8Attn A) {
                         uint32_t v[2][32];
                         tmem_load32(s_at + 64 * half, v[0]);
                         tmem_load32(s_at + 64 * half + 32, v[1]);
-                        const float c[2] = {RULES ? 1.0f : factor(k_scales[2 * half], to_c), RULES ? 1.0f : factor(k_scales[2 * half + 1], to_c)};
-                        // weights times value scales, on O's scale: 2^(lift) p.  (Below 2^-60 they are 0 as fp16 whatever they are.)
-                        const float lift[2] = {fmaxf(v_scales[2 * half] + up, -60.0f), fmaxf(v_scales[2 * half + 1] + up, -60.0f)};
+                        const float c[2] = {RULES != kNoRules ? 1.0f : factor(k_scales[2 * half], to_c), RULES != kNoRules ? 1.0f : factor(k_scales[2 * half + 1], to_c)};
+                        // weights times value scales, on O's scale: 2^(lift) p.  (Below 2^-60 they are 0 as fp16 whatever they are, and bf16 ones are not made here.)
+                        // (Tiles of rows have scales of 1 here.  Read all the same where there are no rules: 380 us, 390 without, for 512 rows over
+                        // 32k; prompts of 2 x 4001 with a cap 642, 653 with.)
+                        constexpr bool kScaled = decltype(as_half)::value || RULES == kNoRules;
+                        const float lift[2] = {fmaxf(kScaled ? v_scales[2 * half] + up : up, -60.0f), fmaxf(kScaled ? v_scales[2 * half + 1] + up : up, -60.0f)};
                         tmem_wait_load();
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
@@ -416,23 +423,24 @@ paged8_tc_kernel(Paged8Attn A) {
                         arrive(bar(misc.p_full[t][half]));
                     }
                 };
-                // the same in the tile with a group that is partly in its page, whose values want the rest of their scale
-                auto weights_cut = [&] {
+                // The same for tiles of rows that are rare: with tokens of pages, of which a group that is partly there wants the rest of its
+                // values' scale; and beside values so much larger that weights on O's scale are below 2^-60, which bf16 holds as well as 1.
+                auto weights_rare = [&] {
 #pragma unroll 1
                     for (int x = 0; x < kN; x += 16) {
-                        const int g = x / kG, edge = g == cut / kG ? cut - x : 0;            // columns before it have the rest
+                        const int g = x / kG, edge = cuts && g == cut / kG ? cut - x : 0;            // columns before it have the rest
                         uint32_t v[16], p[8];
                         tmem_load16(s_at + x, v);
-                        const float c = RULES ? 1.0f : factor(k_scales[g], to_c), lift = fmaxf(v_scales[g] + up, -60.0f), off = lift - base_m, rest = misc.v_rest;
+                        const float c = RULES != kNoRules ? 1.0f : factor(k_scales[g], to_c), f = ex2(fminf(fmaxf(v_scales[g] + up, -126.0f), 126.0f)), f_cut = f * misc.v_rest;
                         tmem_wait_load();
                         float part = 0.0f;
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            const float w0 = ex2(fmaf(__uint_as_float(v[i]), c, off)), w1 = ex2(fmaf(__uint_as_float(v[i + 1]), c, off));
+                            const float w0 = ex2(fmaf(__uint_as_float(v[i]), c, -base_m)), w1 = ex2(fmaf(__uint_as_float(v[i + 1]), c, -base_m));
                             part += w0 + w1;
-                            p[i / 2] = pack_bf16(i < edge ? w0 * rest : w0, i + 1 < edge ? w1 * rest : w1);
+                            p[i / 2] = pack_bf16(w0 * (i < edge ? f_cut : f), w1 * (i + 1 < edge ? f_cut : f));
                         }
-                        l = fmaf(part, ex2(-lift), l);
+                        l += part;
                         tmem_store8(s_at + x / 2, p);
                         if (x % 64 == 48) {
                             tmem_wait_store();
@@ -441,9 +449,12 @@ paged8_tc_kernel(Paged8Attn A) {
                         }
                     }
                 };
-                if (packed) weights(std::true_type{});
-                else if (!cuts) weights(std::false_type{});
-                else weights_cut();
+                if (packed) {
+                    weights(std::true_type{});
+                } else {
+                    if (t0 < inside || low) weights_rare();
+                    else weights(std::false_type{});
+                }
                 if (j + 1 == n_packed && j + 1 < n_tiles) {
                     // (S of this tile is there, so Q has been read)
                     q_as_bf16();
@@ -785,9 +796,13 @@ int run_paged8_tc(const Paged8Attn& a, int blocks, cudaStream_t st) {
         KIVI_CUDA_OK(launch(kernel, dim3((unsigned)blocks, (unsigned)a.L.num_kv_heads, (unsigned)a.pieces), kThreads, smem, st, true, a));
         return KIVI_OK;
     };
-    const bool rules = a.rules.softcap > 0.0f || a.rules.slopes != nullptr;
-    if (a.L.head_dim == 128) return rules ? go(paged8_tc_kernel<128, true>, Shared<128>::bytes) : go(paged8_tc_kernel<128, false>, Shared<128>::bytes);
-    return rules ? go(paged8_tc_kernel<64, true>, Shared<64>::bytes) : go(paged8_tc_kernel<64, false>, Shared<64>::bytes);
+    auto go_rules = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        if (a.rules.softcap > kSmallCap) return go(paged8_tc_kernel<D, kAnyCaps>, Shared<D>::bytes);
+        if (a.rules.softcap > 0.0f) return go(paged8_tc_kernel<D, kSmallCaps>, Shared<D>::bytes);
+        return a.rules.slopes != nullptr ? go(paged8_tc_kernel<D, kSlopes>, Shared<D>::bytes) : go(paged8_tc_kernel<D, kNoRules>, Shared<D>::bytes);
+    };
+    return a.L.head_dim == 128 ? go_rules(std::integral_constant<int, 128>{}) : go_rules(std::integral_constant<int, 64>{});
 }
 
 int paged8_tc_fault_word(int* out) {

@@ -849,3 +849,18 @@ def test_loud_values_of_a_block_that_this_step_fills(ops, D, G, R, held, new, n_
     a = pool.append(ops, k, v, [new])
     want, size, S = reference(pool, q, [new], cap=rules.get("softcap", 0.0))
     close(attend(ops, pool, q, k, v, a, F32, **rules), want, size, tolerance(BF, S))
+
+
+# ---- values of any size ---------------------------------------------------------------------------
+@pytest.mark.parametrize("old,fresh", [(60, 60), (90, 90), (100, 100), (100, 0), (0, 100), (100, 60), (-90, -90), (-90, 0)])
+@pytest.mark.parametrize("new,n_rep,D,R", [(1, 4, 128, 128), (5, 3, 64, 64), (130, 1, 128, 128), (100, 2, 64, 64), (90, 1, 128, 300)])
+def test_values_of_any_size(ops, new, n_rep, D, R, old, fresh):
+    """Values held before the step and values of the step, as powers of two: in pages, in the window and new they share a row's sum."""
+    held = 500
+    pool = Pool(1, 1, D, 32, R, 64, held + new, BF)
+    pool.append(ops, rows(held, 1, D, BF, 1), rows(held, 1, D, BF, 2) * 2.0 ** old, [held])
+    k, v, q = rows(new, 1, D, BF, 3), rows(new, 1, D, BF, 4) * 2.0 ** fresh, rows(new, n_rep, D, BF, 5)
+    a = pool.append(ops, k, v, [new])
+    for rules in ({}, {"softcap": 5.0, "window": 200}):
+        want, size, S = reference(pool, q, [new], cap=rules.get("softcap", 0.0), window=rules.get("window", 0))
+        close(attend(ops, pool, q, k, v, a, **rules), want, size, tolerance(BF, S))
