@@ -402,7 +402,9 @@ static Paged8Plan plan_paged8(const kivi_paged8_layer* L, const kivi_paged_batch
         return p;
     }
     p.kernel = Paged8Kernel::kGeneral;
-    p.rows = rows <= 8 ? 8 : 64;
+    // Blocks of 8 rows against blocks of 64, fp32: 16 x 1000, 8 heads of 128, 93 us against 218 for 8 rows, 206 against 220 for 16, 222 against 222
+    // for 24, 371 against 228 for 32; 4 x 1000, 12 heads of 64, 36 against 67, 48 against 67, 52 against 69, 62 against 69.
+    p.rows = rows <= 24 ? 8 : 64;
     p.blocks = blocks_of(p.rows);
     const int64_t tiles = tiles_of(kTile, p.rows);
     // as many pieces as give every SM four CTAs

@@ -1111,7 +1111,10 @@ paged8_fold_kernel(Paged8Attn A, int unit_rows) {
     }
 }
 
-constexpr int kMostBlocks = 3, kMostRows = 64, kLaneRows = 2, kMostLaneRows = 4;
+// kMostRows: all of a sequence's rows in one unit.  Beyond it its bytes are read again for every 24 rows: 16 x 8192, 8 x 4 heads, bf16, 130 us
+// for 24 rows where the tensor-core kernel takes 190, 194 against 188 for 32, 286 against 249 for 64; 64 x 2048 204 against 264, then 362 against
+// 266.  (One sequence of 32768: 60 against 69 for 8 rows, 89 and 124 against 69 for 16 and 24.)
+constexpr int kMostBlocks = 3, kMostRows = 8 * kMostBlocks, kLaneRows = 2, kMostLaneRows = 4;
 
 // Blocks of eight rows of a unit: all of a sequence's rows in one unit where registers hold them, so that its bytes are
 // read once.
