@@ -12,16 +12,16 @@
 // paged8_decode_kernel: bf16, blocks of whole 32 tokens.  mma.sync m16n8k16, 32 tokens of a page to a warp
 // at a time; tokens (and channels of V) are the sixteen rows of an MMA, the (new token, query head) pairs of one
 // sequence and KV head its eight columns, up to three times eight to a unit: with the pairs as rows a single token of
-// four heads took twice the MMAs and the registers (64 ragged sequences up to 32k 555 us, 384 now).  Weights change places with
+// four heads took twice the MMAs and the registers (64 ragged sequences up to 32k 555 us, 385 to 406 now).  Weights change places with
 // movmatrix in between.  A tile is 4 KB of keys and 4 KB of values (head_dim 128), 128 conversions and 32 MMAs of a warp,
 // less than its bytes take.  A warp has a ring of stages that bulk copies fill, its first lane issues them; the warps take
 // tiles in turn and meet at a unit's end.
 //
 // Numbers: e4m3 codes are exact as fp16.  A row of bf16 queries is exact as fp16 after a power
 // of two, but for what is below 2^-27 of its largest.  A block's key scale multiplies the scores, its value scale the weights,
-// which are fp16 (rounded at 2^-12 of themselves, where the output is rounded at 2^-9), less the power of
+// which are fp16 (rounded at 2^-11 of themselves, where a bf16 output is rounded at 2^-8), less the power of
 // two of the largest such product that the row has met.  Window and own tokens are contracted as the bf16 numbers they are
-// (weights at 2^-9 there: bf16 reaches as far as the values do).  Sums are fp32.
+// (weights at 2^-8 there: bf16 reaches as far as the values do).  Sums are fp32.
 //
 // paged8_lanes_kernel: fp32 and mixed types, and blocks of 16: CUDA cores, fp32 throughout (below).
 #include "async_copy.cuh"

@@ -17,7 +17,7 @@
 //
 // Keys of a page are operands as they lie: S is two MMAs of kind f8f6f4, a row of Q less a
 // power of two being the sum of two e4m3 numbers (a bf16 number is, as far as 2^-9 of the
-// row's largest; what is smaller is off by 2^-19 of it).  They take as long as one of fp16 operands
+// row's largest; what is smaller is off by 2^-17 of it).  They take as long as one of fp16 operands
 // would, without a conversion of K, the shared memory it takes and its traffic there.  A block's key scale multiplies S.
 // Values are fp16, which e4m3 numbers are exactly, with P in fp16: a weight times its value
 // scale less the power of two of the largest such product that the row has met, so that neither
@@ -25,7 +25,10 @@
 // Window and new tokens are bf16 operands as they are, Q and P then too: Q is written again
 // when the pages are done.  Keys of a page are there codes times their scale's power of two, and its rest multiplies S; where only
 // some of a group's tokens come from the page, the others' scores are divided by that rest (keys rounded to bf16 instead: 0.0027 off
-// 64 bits where the output's rounding is 0.0017), and the page's values are held the same way, their rest in the weights.  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the outputs of the rows that see it.
+// 64 bits where the output's rounding is 0.0017), and the page's values are held the same way, their rest in the weights.  P is rounded
+// at 2^-8 there, at 2^-11 over pages: bf16 for the values' range (0.0019 to 0.0022 off 64 bits where most of the weight lies on such
+// rows).  A value that is not finite would reach all rows of a tile through weights of 0: it is left out there, and added to the
+// outputs of the rows that see it.
 //
 // Per tile and SM: 2048 cycles of MMA for 256 rows, 2048 of exponentials (16 a cycle).
 #include "paged8_attention.cuh"

@@ -217,7 +217,7 @@ int run_adjust(const LogitArgs& a, cudaStream_t st) {
     return KIVI_OK;
 }
 
-// Threads of a CTA: 256 where that leaves two CTAs to an SM, else 128.
+// Threads of a CTA: 512 where that leaves two CTAs to an SM, else 128.
 template <typename T> int adjust(const LogitArgs& a, cudaStream_t st) {
     constexpr int kEntries = 512 * kVectors * kPack<T>;
     return (int64_t)a.batch * ((a.vocab + kEntries - 1) / kEntries) >= 2 * num_sms() ? run_adjust<T, 512>(a, st) : run_adjust<T, 128>(a, st);
