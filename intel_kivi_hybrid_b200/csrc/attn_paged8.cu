@@ -96,7 +96,7 @@ paged8_attention_kernel(Paged8Attn A) {
     // the maximum are then rounded at their own size.
     const bool capped = A.rules.softcap > 0.0f, plain = !capped && A.rules.slopes == nullptr;
     const float to_log2 = (plain ? A.scale : 1.0f) * 1.4426950408889634f;
-    const float inv_cap = capped ? A.scale / A.rules.softcap : 0.0f;
+    const float inv_cap = capped ? 1.0f / A.rules.softcap : 0.0f;
     float m[RPT], l[RPT], o[RPT][4 * NC], slope[RPT];
     int place[RPT], from[RPT];                           // of the row, and of its window's first token
 #pragma unroll
@@ -202,7 +202,7 @@ paged8_attention_kernel(Paged8Attn A) {
             for (int j = 0; j < 4; ++j) {
                 const int t = t0 + tx + 16 * j;
                 if (!plain) {
-                    sc[i][j] = capped ? A.rules.softcap * tanhf(sc[i][j] * inv_cap) : sc[i][j] * A.scale;
+                    sc[i][j] = capped ? A.rules.softcap * tanhf(sc[i][j] * A.scale * inv_cap) : sc[i][j] * A.scale;
                     sc[i][j] = fmaf(slope[i], (float)(t - place[i]), sc[i][j]);
                 }
                 if (!sees(i, t)) sc[i][j] = -INFINITY;

@@ -103,7 +103,8 @@ __device__ __forceinline__ float capped_far(float z, float cap) {
     return cap - __fdividef(2.0f * cap, 1.0f + ex2(e > 120.0f ? 120.0f : e));
 }
 
-// What is done to scores: nothing, slopes alone, a cap up to kSmallCap, any cap (both of them with slopes or without).
+// What is done to scores: nothing, slopes alone, a cap up to kSmallCap and not far above sm_scale, any cap (both of them with
+// slopes or without).
 enum { kNoRules, kSlopes, kSmallCaps, kAnyCaps };
 
 template <int D, int RULES>
@@ -252,10 +253,11 @@ paged8_tc_kernel(Paged8Attn A) {
 
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, s_at = tmem + lanes + t * kN, o_at = tmem + lanes + 2 * kN + t * D;
             constexpr float kLog2e = 1.4426950408889634f;
-            auto factor = [](float scale, float to) { return fmaxf(scale * to, 1.0e-37f); };         // (not 0: hidden columns are -inf)
+            auto factor = [](float scale, float to) { return fmaxf(scale * to, 1.2e-38f); };         // (not 0: hidden columns are -inf)
             const bool capped = RULES >= kSmallCaps && A.rules.softcap > 0.0f, biased = RULES != kNoRules && A.rules.slopes != nullptr;
             const float cap = A.rules.softcap * kLog2e, slope = biased && there ? A.rules.slopes[head] * kLog2e : 0.0f;
-            const float to_x = capped ? A.scale / A.rules.softcap : A.scale * kLog2e;
+            // (Any cap: to scores first, then over the cap: the two at once may be below what fp32 holds.)
+            const float to_x = RULES == kAnyCaps ? A.scale : capped ? A.scale / A.rules.softcap : A.scale * kLog2e, inv_cap = RULES == kAnyCaps ? 1.0f / A.rules.softcap : 1.0f;
             float m = -INFINITY, ref = -1.0e30f, l = 0.0f, base_m = 0.0f, up = 0.0f;         // ref: the largest maximum plus value scale, so far; up: log2 of what brings weights times scales to O's scale
             bool ok = true, low = false;                 // low: a row of the warp has `up` below -60
             for (int j = 0; j < n_tiles; ++j) {
@@ -304,7 +306,8 @@ paged8_tc_kernel(Paged8Attn A) {
                             for (int g = 0; g < 2; ++g)
 #pragma unroll
                                 for (int i = 0; i < 32; i += 2) {
-                                    const float2 z = mul2(at2(g, i), both(c[g]));
+                                    float2 z = mul2(at2(g, i), both(c[g]));
+                                    if constexpr (RULES == kAnyCaps) z = mul2(z, both(inv_cap));
                                     far = fmaxf(far, fmaxf(fabsf(z.x), fabsf(z.y)));
                                     put2(g, i, z);
                                 }
@@ -801,7 +804,7 @@ int run_paged8_tc(const Paged8Attn& a, int blocks, cudaStream_t st) {
     };
     auto go_rules = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        if (a.rules.softcap > kSmallCap) return go(paged8_tc_kernel<D, kAnyCaps>, Shared<D>::bytes);
+        if (a.rules.softcap > kSmallCap || a.scale < 1e-28f * a.rules.softcap) return go(paged8_tc_kernel<D, kAnyCaps>, Shared<D>::bytes);
         if (a.rules.softcap > 0.0f) return go(paged8_tc_kernel<D, kSmallCaps>, Shared<D>::bytes);
         return a.rules.slopes != nullptr ? go(paged8_tc_kernel<D, kSlopes>, Shared<D>::bytes) : go(paged8_tc_kernel<D, kNoRules>, Shared<D>::bytes);
     };

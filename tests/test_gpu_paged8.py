@@ -864,3 +864,19 @@ def test_values_of_any_size(ops, new, n_rep, D, R, old, fresh):
     for rules in ({}, {"softcap": 5.0, "window": 200}):
         want, size, S = reference(pool, q, [new], cap=rules.get("softcap", 0.0), window=rules.get("window", 0))
         close(attend(ops, pool, q, k, v, a, **rules), want, size, tolerance(BF, S))
+
+
+@pytest.mark.parametrize("dtype,new,n_rep,D", [(BF, 1, 4, 128), (BF, 5, 3, 64), (BF, 130, 1, 128), (BF, 100, 2, 64), (F32, 30, 1, 96)])
+@pytest.mark.parametrize("size_q,cap", [(100, 1e9), (118, 1e10), (118, 4.0), (-100, 1e9), (-60, 4.0)])
+def test_caps_of_queries_of_any_size(ops, dtype, new, n_rep, D, size_q, cap):
+    """sm_scale over the cap is below what fp32 holds; neither is."""
+    held = 400
+    pool = Pool(1, 1, D, 32, 64, 64, held + new, dtype)
+    size_k = (0 if dtype == F32 else -30) if size_q > 0 else 70
+    pool.append(ops, rows(held, 1, D, dtype, 1) * 2.0 ** size_k, rows(held, 1, D, dtype, 2), [held])
+    k, v, q = rows(new, 1, D, dtype, 3) * 2.0 ** size_k, rows(new, 1, D, dtype, 4), rows(new, n_rep, D, dtype, 5).clamp(-1.9, 1.9)
+    a = pool.append(ops, k, v, [new])
+    scale = min(-3 - size_q - size_k, 33)
+    got = attend(ops, pool, (q.float() * 2.0 ** size_q).to(dtype), k, v, a, sm_scale=2.0 ** scale, softcap=cap)
+    want, size, S = reference(pool, q.double() * (2.0 ** (size_q + scale) * math.sqrt(D)), [new], cap=cap)
+    close(got, want, size, tolerance(dtype, S))
