@@ -880,3 +880,17 @@ def test_caps_of_queries_of_any_size(ops, dtype, new, n_rep, D, size_q, cap):
     got = attend(ops, pool, (q.float() * 2.0 ** size_q).to(dtype), k, v, a, sm_scale=2.0 ** scale, softcap=cap)
     want, size, S = reference(pool, q.double() * (2.0 ** (size_q + scale) * math.sqrt(D)), [new], cap=cap)
     close(got, want, size, tolerance(dtype, S))
+
+
+@pytest.mark.parametrize("D,G", [(256, 64), (256, 32), (240, 48), (144, 16), (80, 32), (16, 32)])
+@pytest.mark.parametrize("held,news", [([300, 0], [1, 1]), ([130, 517], [6, 3]), ([200, 64], [70, 1])])
+def test_bf16_heads_of_other_sizes(ops, D, G, held, news):
+    pool = Pool(2, 2, D, G, 64, 2 * G, max(held) + max(news), BF)
+    pool.append(ops, rows(sum(held), 2, D, BF, 1), rows(sum(held), 2, D, BF, 2), held)
+    n = sum(news)
+    k, v, q = rows(n, 2, D, BF, 3), rows(n, 2, D, BF, 4), rows(n, 6, D, BF, 5)
+    a = pool.append(ops, k, v, news)
+    slopes = torch.tensor([2.0 ** -(i + 1) for i in range(6)], device=DEV)
+    for rules in ({}, {"softcap": 30.0, "window": 100}, {"slopes": slopes}):
+        want, size, S = reference(pool, q, news, rules.get("softcap", 0.0), rules.get("slopes"), rules.get("window", 0))
+        close(attend(ops, pool, q, k, v, a, **rules), want, size, tolerance(BF, S))
